@@ -239,6 +239,94 @@ RAVEN_API int raven_merge_topk_gathered_device(const void* d_gathered, uint32_t 
                                                uint32_t* d_out_ids, float* d_out_dists, uint32_t* d_out_counts,
                                                void* stream);
 
+/* ---- scoring (no reference counterpart) -----------------------------------
+ * Exhaustive scores beside the graph search: FP8 rows, products of a query
+ * batch with rows (all of them, or those of each query's group) and the best k
+ * of each row of scores. Device buffers on the current device; asynchronous on
+ * `stream` (NULL = the CUDA default stream). Scratch comes from the
+ * stream-ordered pool, per call: calls on several streams, and captured graphs,
+ * share nothing. */
+
+#define RAVEN_TYPE_F32 0
+#define RAVEN_TYPE_F16 1
+#define RAVEN_TYPE_BF16 2
+#define RAVEN_TYPE_FP8 3 /* e4m3 codes, one power-of-two scale per 128 values */
+
+/* bits of *d_status, which calls only ever set (the caller clears it) */
+#define RAVEN_S_OFFSETS 1  /* a group's offsets fall or leave the rows: it counted as empty */
+#define RAVEN_S_CAPACITY 2 /* scores past the output's capacity were not written */
+#define RAVEN_S_WAIT 4     /* a wait inside the kernel ran out: the scores are not valid */
+
+/* Rows of `dim` values, row i at data + i * ld values (codes). FP8 rows also
+ * have exponent bytes, row i at exps + i * ld_exps, one per 128 values: a value
+ * is its code times 2^(byte - 127). Layout of FP8 rows: codes start on 16 bytes
+ * and ld is a multiple of 16; exps start on 4 bytes and ld_exps is a multiple
+ * of 4, at least ceil(dim / 128). f16 and bf16 rows start on 16 bytes and ld is
+ * a multiple of 8; queries that a call encodes may have any ld >= dim. */
+typedef struct {
+  const void* data;
+  const uint8_t* exps; /* FP8 only */
+  uint64_t rows;       /* < 2^31 */
+  uint64_t ld;
+  uint64_t ld_exps; /* FP8 only */
+  int32_t type;     /* RAVEN_TYPE_* */
+} raven_rows;
+
+/* Encodes f32, f16 or bf16 rows (any ld >= dim, values in 1..65536 per row) as
+ * FP8. The scale of a block is the least power of two 2^e, e >= -127, with
+ * max|x| <= 448 * 2^e (1 for a block of zeros); codes are rounded to nearest
+ * even. Infinities and NaN become the NaN code and do not count for the scale.
+ * Code bytes up to a multiple of 16 values are 0, exponent bytes up to a
+ * multiple of 4 are 127; bytes past those are left as they were. */
+RAVEN_API int raven_fp8_encode_device(const void* d_rows, int32_t type, uint64_t n, uint32_t dim, uint64_t ld,
+                                      uint8_t* d_codes, uint64_t ld_codes, uint8_t* d_exps, uint64_t ld_exps,
+                                      void* stream);
+/* The f32 values FP8 rows stand for (exact; infinite from 2^128). */
+RAVEN_API int raven_fp8_decode_device(const uint8_t* d_codes, uint64_t ld_codes, const uint8_t* d_exps,
+                                      uint64_t ld_exps, uint64_t n, uint32_t dim, float* d_out, uint64_t ld,
+                                      void* stream);
+/* FP8 rows of an index's uploaded vectors (n x dim, in the caller's order of
+ * values), on the index's device. */
+RAVEN_API int raven_index_fp8_device(raven_index* ix, uint8_t* d_codes, uint64_t ld_codes, uint8_t* d_exps,
+                                     uint64_t ld_exps, void* stream);
+
+/* out[i * ld_out + j] = alpha * <q_i, v_j> + (d_bias ? d_bias[j] : 0), summed
+ * in f32 on the tensor cores and rounded once to out_type (f32, f16, bf16).
+ * alpha = -2 with d_bias[j] = |v_j|^2 gives squared distances less |q_i|^2.
+ * Vectors are FP8, f16 or bf16; queries have the same type, or, with FP8
+ * vectors, any type (they are encoded first). d_status may be NULL. */
+RAVEN_API int raven_scores_device(const raven_rows* q, const raven_rows* v, uint32_t dim, float alpha,
+                                  const float* d_bias, void* d_out, int32_t out_type, uint64_t ld_out,
+                                  int32_t* d_status, void* stream);
+
+/* Scores by group: queries [d_q_offsets[g], d_q_offsets[g + 1]) against vectors
+ * [d_v_offsets[g], d_v_offsets[g + 1]), for g < groups; both offset arrays
+ * (groups + 1 each, on the device) rise, and groups may be empty on either
+ * side. Output packed: groups in order, in a group its queries in order, for
+ * each the scores of the group's vectors. At most `capacity` elements are
+ * written: a query's scores in a tile of 128 vectors are written when they fit
+ * whole. Queries outside every group have no scores. */
+RAVEN_API int raven_group_scores_device(const raven_rows* q, const int64_t* d_q_offsets, const raven_rows* v,
+                                        const int64_t* d_v_offsets, uint32_t groups, uint32_t dim, float alpha,
+                                        const float* d_bias, void* d_out, int32_t out_type, uint64_t capacity,
+                                        int32_t* d_status, void* stream);
+
+/* d_row_starts[i] (nq + 1 values) = where query i's scores start in the packed
+ * output; the last one is its size. Queries before the first group start at 0,
+ * those behind the last group at the size. */
+RAVEN_API int raven_group_rows_device(const int64_t* d_q_offsets, const int64_t* d_v_offsets, uint32_t groups,
+                                      uint64_t nq, uint64_t n, int64_t* d_row_starts, int32_t* d_status, void* stream);
+
+/* The best k (1..256) scores of each of nq rows, best first (largest, or
+ * smallest with largest = 0), equal scores by the lower index, NaN after every
+ * number, -0 equal to 0. Rows are n scores at pitch ld, or with d_row_starts
+ * (nq + 1 values on the device) the scores [d_row_starts[i], d_row_starts[i + 1])
+ * of n in all. d_ids: indexes within the row; d_counts (may be NULL): min(k, row
+ * length); slots past the count are 0. Values have the scores' type. */
+RAVEN_API int raven_topk_rows_device(const void* d_scores, int32_t type, uint64_t nq, uint64_t n, uint64_t ld,
+                                     const int64_t* d_row_starts, uint32_t k, int32_t largest, void* d_vals,
+                                     uint32_t* d_ids, uint32_t* d_counts, void* stream);
+
 typedef struct {
   uint32_t max_ef;      /* largest pool capacity (fixed ef or adaptive max) */
   uint32_t max_dim;     /* largest vector dimension */

@@ -27,6 +27,15 @@ RAVEN_QUANT_SQ4 = 0
 RAVEN_QUANT_SQ8 = 1
 RAVEN_QUANT_F32 = 2
 
+RAVEN_TYPE_F32 = 0
+RAVEN_TYPE_F16 = 1
+RAVEN_TYPE_BF16 = 2
+RAVEN_TYPE_FP8 = 3
+
+RAVEN_S_OFFSETS = 1
+RAVEN_S_CAPACITY = 2
+RAVEN_S_WAIT = 4
+
 u32p = C.POINTER(C.c_uint32)
 f32p = C.POINTER(C.c_float)
 i32p = C.POINTER(C.c_int32)
@@ -108,6 +117,17 @@ class Limits(C.Structure):
     _fields_ = [("max_ef", C.c_uint32), ("max_dim", C.c_uint32), ("max_r", C.c_uint32), ("max_nav_k", C.c_uint32)]
 
 
+class Rows(C.Structure):
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("exps", C.c_void_p),
+        ("rows", C.c_uint64),
+        ("ld", C.c_uint64),
+        ("ld_exps", C.c_uint64),
+        ("type", C.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/raven_gpu.h
 SIGNATURES = {
     "raven_graph_build": (C.c_int, [f32p, C.c_uint64, C.c_uint32, C.POINTER(BuildConfig), C.POINTER(C.c_void_p)]),
@@ -138,6 +158,20 @@ SIGNATURES = {
     "raven_merge_topk_gathered_device": (C.c_int, [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint64,
                                                    C.c_uint32, C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p,
                                                    C.c_void_p]),
+    "raven_fp8_encode_device": (C.c_int, [C.c_void_p, C.c_int32, C.c_uint64, C.c_uint32, C.c_uint64, C.c_void_p,
+                                          C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "raven_fp8_decode_device": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint32,
+                                          C.c_void_p, C.c_uint64, C.c_void_p]),
+    "raven_index_fp8_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "raven_scores_device": (C.c_int, [C.POINTER(Rows), C.POINTER(Rows), C.c_uint32, C.c_float, C.c_void_p, C.c_void_p,
+                                      C.c_int32, C.c_uint64, C.c_void_p, C.c_void_p]),
+    "raven_group_scores_device": (C.c_int, [C.POINTER(Rows), C.c_void_p, C.POINTER(Rows), C.c_void_p, C.c_uint32,
+                                            C.c_uint32, C.c_float, C.c_void_p, C.c_void_p, C.c_int32, C.c_uint64,
+                                            C.c_void_p, C.c_void_p]),
+    "raven_group_rows_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint64, C.c_uint64, C.c_void_p,
+                                          C.c_void_p, C.c_void_p]),
+    "raven_topk_rows_device": (C.c_int, [C.c_void_p, C.c_int32, C.c_uint64, C.c_uint64, C.c_uint64, C.c_void_p,
+                                         C.c_uint32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "raven_limits": (None, [C.POINTER(Limits)]),
     "raven_index_set_tuning": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32]),
     "raven_index_set_small_batch": (C.c_int, [C.c_void_p, C.c_uint64]),

@@ -17,8 +17,9 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libraven_gpu.so")
 
-SOURCES = ["raven_gpu.cu", "host_index.cpp"]
-DEPS = SOURCES + ["search_kernel.cuh", "search_cta.cuh", "knn_tc.cuh", "host_index.h"]
+SOURCES = ["raven_gpu.cu", "scoring.cu", "host_index.cpp"]
+DEPS = SOURCES + ["search_kernel.cuh", "search_cta.cuh", "knn_tc.cuh", "score_tc.cuh", "topk.cuh", "internal.h",
+                  "host_index.h"]
 
 
 def nvcc_path() -> str:
@@ -48,6 +49,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         "-gencode", "arch=compute_100a,code=sm_100a",
         "-lineinfo",
         "-shared",
+        "-t", "0",  # translation units side by side
         "-Xcompiler", "-fPIC,-fopenmp,-O3,-mavx2,-mfma,-fvisibility=hidden",
         "-Xptxas", "-v" if verbose else "-O3",
         "-I", os.path.join(ROOT, "include"),

@@ -25,6 +25,7 @@
 
 #include "../../include/raven_gpu.h"
 #include "host_index.h"
+#include "internal.h"
 #include "knn_tc.cuh"
 #include "search_cta.cuh"
 #include "search_kernel.cuh"
@@ -1493,6 +1494,15 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
   return fn;
 }
 
+}  // namespace
+
+namespace raven_internal {
+int fail(int code, const std::string& msg) { return ::fail(code, msg); }
+PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() { return ::encode_tiled(); }
+}  // namespace raven_internal
+
+namespace {
+
 // f32 matrix of `rows` rows, `cols` used columns, row stride `ld` floats
 // (ld * 4 a multiple of 16 bytes); box 32 columns x 128 rows, 128-byte
 // swizzle (the K-major SW128 operand layout), out-of-range elements read 0.
@@ -1704,6 +1714,16 @@ int raven_merge_topk_gathered_device(const void* d_gathered, uint32_t n_shards, 
       d_out_counts);
   CU(cudaGetLastError());
   return RAVEN_OK;
+}
+
+int raven_index_fp8_device(raven_index* ix, uint8_t* d_codes, uint64_t ld_codes, uint8_t* d_exps, uint64_t ld_exps,
+                           void* stream) {
+  NvtxRange nvtx_range("raven.index_fp8");
+  if (!ix) return fail(RAVEN_EINVAL, "null index");
+  CU(cudaSetDevice(ix->device));
+  if (ix->n == 0) return RAVEN_OK;
+  return raven_internal::fp8_encode_lane_major(ix->d_vec, ix->n, ix->dim, d_codes, ld_codes, d_exps, ld_exps,
+                                               (cudaStream_t)stream);
 }
 
 int raven_index_set_small_batch(raven_index* ix, uint64_t max_nq) {

@@ -1,0 +1,558 @@
+// Scoring operators of the C ABI (include/raven_gpu.h): FP8 rows with a scale
+// for each block of 128 values, scores of queries against rows (dense and
+// grouped, score_tc.cuh) and the best k of each row of scores (topk.cuh).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <nvtx3/nvToolsExt.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "../../include/raven_gpu.h"
+#include "internal.h"
+#include "score_tc.cuh"
+#include "topk.cuh"
+
+using raven_internal::encode_tiled;
+using raven_internal::fail;
+
+namespace {
+
+struct NvtxRange {
+  explicit NvtxRange(const char* name) { nvtxRangePushA(name); }
+  ~NvtxRange() { nvtxRangePop(); }
+  NvtxRange(const NvtxRange&) = delete;
+  NvtxRange& operator=(const NvtxRange&) = delete;
+};
+
+#define CU(call)                                                                        \
+  do {                                                                                  \
+    cudaError_t e_ = (call);                                                            \
+    if (e_ != cudaSuccess) return fail(RAVEN_ECUDA, std::string(#call ": ") + cudaGetErrorString(e_)); \
+  } while (0)
+
+constexpr uint64_t kMaxRows = 0x7fffffffull;  // rows are TMA coordinates (int32)
+constexpr uint32_t kMaxDim = 65536;
+constexpr uint32_t kBlock = 128;              // values under one scale
+
+uint64_t type_size(int32_t t) {
+  return t == RAVEN_TYPE_F32 ? 4 : t == RAVEN_TYPE_F16 || t == RAVEN_TYPE_BF16 ? 2 : t == RAVEN_TYPE_FP8 ? 1 : 0;
+}
+bool aligned(const void* p, uint64_t a) { return (uintptr_t)p % a == 0; }
+
+// SMs of the current device.
+int sm_count(int* out) {
+  static std::mutex mu;
+  static int count[256] = {};
+  int dev = 0;
+  CU(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lk(mu);
+  if (dev < 0 || dev >= 256) return fail(RAVEN_EINVAL, "device ordinal out of range");
+  if (!count[dev]) CU(cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev));
+  *out = count[dev];
+  return RAVEN_OK;
+}
+
+// ---------------------------------------------------------------------------
+// FP8 rows. Block b of a row: e = the least exponent with max|x| <= 448 * 2^e
+// over its finite values (0 when they are all zero, at least -127), code =
+// e4m3(x * 2^-e) to nearest even, exponent byte = e + 127. A power of two
+// scales exactly, so the only rounding is e4m3's own (half a step, 2^-4 of the
+// value; 2^-10 * 2^e below the type's normal range).
+// One warp per block: lane l holds values 4l..4l+3, so a block is read in one
+// piece of 512 or 256 bytes and written in one of 128.
+// ---------------------------------------------------------------------------
+__device__ inline float load_value(const float* p) { return *p; }
+__device__ inline float load_value(const __half* p) { return __half2float(*p); }
+__device__ inline float load_value(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+
+template <typename T>
+__device__ inline void load4(const T* p, float (&x)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 v = *(const float4*)p;
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+    const uint2 v = *(const uint2*)p;
+    const T* h = (const T*)&v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = load_value(h + i);
+  }
+}
+
+// VEC: pitch and address let four values be read at once. LANE: lane-major
+// rows (element e of the first 16C at (e % 16) * C + e / 16).
+template <typename T, bool VEC, bool LANE>
+__global__ void __launch_bounds__(256) fp8_encode_kernel(const T* __restrict__ in, uint64_t n, uint32_t dim, uint64_t ld,
+                                                         uint8_t* __restrict__ codes, uint64_t ld_codes,
+                                                         uint8_t* __restrict__ exps, uint64_t ld_exps) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t nb = (dim + kBlock - 1) / kBlock, nb4 = (nb + 3) / 4 * 4, dim16 = (dim + 15) / 16 * 16;
+  const uint64_t units = n * nb;
+  const uint64_t warps = (uint64_t)gridDim.x * (blockDim.x >> 5);
+  for (uint64_t u = (uint64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += warps) {
+    const uint64_t row = u / nb;
+    const uint32_t b = (uint32_t)(u - row * nb);
+    const uint32_t d = b * kBlock + 4 * lane;
+    const T* r = in + row * ld;
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (VEC && d + 4 <= dim) {
+      load4(r + d, x);
+    } else {
+      const uint32_t C = dim / 16;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t e = d + i;
+        if (e < dim) x[i] = load_value(r + (LANE && e < 16 * C ? (e % 16) * C + e / 16 : e));
+      }
+    }
+    uint32_t top = 0;  // largest finite magnitude, as bits
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = __float_as_uint(x[i]) & 0x7fffffffu;
+      if (a < 0x7f800000u) top = max(top, a);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    // 448 = 1.75 * 2^8: one exponent more when the mantissa is above 1.75
+    int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+    e = top == 0 ? 0 : max(e, -127);
+    const float inv = e == -127 ? 1.7014118346046923e38f : __uint_as_float((uint32_t)(127 - e) << 23);  // 2^-e
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool finite = (__float_as_uint(x[i]) & 0x7fffffffu) < 0x7f800000u;
+      const uint32_t c = finite ? (uint32_t)__nv_cvt_float_to_fp8(x[i] * inv, __NV_SATFINITE, __NV_E4M3) : 0x7fu;
+      word |= c << (8 * i);
+    }
+    if (d < dim16) *(uint32_t*)(codes + row * ld_codes + d) = word;
+    if (lane == 0) exps[row * ld_exps + b] = (uint8_t)(e + 127);
+    if (b + 1 == nb && lane < (int)(nb4 - nb)) exps[row * ld_exps + nb + lane] = 127;
+  }
+}
+
+__global__ void __launch_bounds__(256) fp8_decode_kernel(const uint8_t* __restrict__ codes, uint64_t ld_codes,
+                                                         const uint8_t* __restrict__ exps, uint64_t ld_exps, uint64_t n,
+                                                         uint32_t dim, float* __restrict__ out, uint64_t ld) {
+  const uint64_t total = n * dim;
+  for (uint64_t t = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; t < total; t += (uint64_t)gridDim.x * blockDim.x) {
+    const uint64_t row = t / dim;
+    const uint32_t d = (uint32_t)(t - row * dim);
+    const __half_raw h = __nv_cvt_fp8_to_halfraw(codes[row * ld_codes + d], __NV_E4M3);
+    out[row * ld + d] = ldexpf(__half2float(*(const __half*)&h), (int)exps[row * ld_exps + d / kBlock] - 127);
+  }
+}
+
+template <typename T, bool LANE>
+cudaError_t launch_encode(const void* x, uint64_t n, uint32_t dim, uint64_t ld, uint8_t* codes, uint64_t ld_codes,
+                          uint8_t* exps, uint64_t ld_exps, int sms, cudaStream_t st) {
+  const uint64_t units = n * ((dim + kBlock - 1) / kBlock);
+  const unsigned grid = (unsigned)std::min<uint64_t>((units + 7) / 8, (uint64_t)sms * 16);
+  const bool vec = !LANE && ld % 4 == 0 && aligned(x, 4 * sizeof(T));
+  if (vec)
+    fp8_encode_kernel<T, true, LANE><<<grid, 256, 0, st>>>((const T*)x, n, dim, ld, codes, ld_codes, exps, ld_exps);
+  else
+    fp8_encode_kernel<T, false, LANE><<<grid, 256, 0, st>>>((const T*)x, n, dim, ld, codes, ld_codes, exps, ld_exps);
+  return cudaGetLastError();
+}
+
+int encode_rows(const void* x, int32_t type, uint64_t n, uint32_t dim, uint64_t ld, uint8_t* codes, uint64_t ld_codes,
+                uint8_t* exps, uint64_t ld_exps, cudaStream_t st) {
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  if (type == RAVEN_TYPE_F32)
+    CU((launch_encode<float, false>(x, n, dim, ld, codes, ld_codes, exps, ld_exps, sms, st)));
+  else if (type == RAVEN_TYPE_F16)
+    CU((launch_encode<__half, false>(x, n, dim, ld, codes, ld_codes, exps, ld_exps, sms, st)));
+  else
+    CU((launch_encode<__nv_bfloat16, false>(x, n, dim, ld, codes, ld_codes, exps, ld_exps, sms, st)));
+  return RAVEN_OK;
+}
+
+uint64_t exps_pitch(uint32_t dim) { return ((dim + kBlock - 1) / kBlock + 3) / 4 * 4; }
+uint64_t codes_pitch(uint32_t dim) { return (dim + 15) / 16 * 16; }
+
+int check_dim(uint32_t dim) {
+  if (dim == 0 || dim > kMaxDim) return fail(RAVEN_ELIMIT, "dim must be in 1..65536");
+  return RAVEN_OK;
+}
+int check_fp8(const uint8_t* codes, uint64_t ld_codes, const uint8_t* exps, uint64_t ld_exps, uint32_t dim) {
+  if (!codes || !exps) return fail(RAVEN_EINVAL, "FP8 rows need codes and exponents");
+  if (!aligned(codes, 16) || ld_codes % 16 || ld_codes < codes_pitch(dim))
+    return fail(RAVEN_EINVAL, "FP8 codes must start on 16 bytes, their pitch a multiple of 16 of at least dim");
+  if (!aligned(exps, 4) || ld_exps % 4 || ld_exps < exps_pitch(dim))
+    return fail(RAVEN_EINVAL, "FP8 exponents must start on 4 bytes, their pitch a multiple of 4 of at least dim / 128");
+  return RAVEN_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Scores.
+// ---------------------------------------------------------------------------
+// K-major rows as boxes of 128 bytes x `box` rows with the 128-byte swizzle;
+// elements past dim, and rows past the last, read 0.
+bool rows_map(CUtensorMap* m, const void* base, int32_t type, uint32_t dim, uint64_t rows, uint64_t ld, uint32_t box) {
+  PFN_cuTensorMapEncodeTiled_v12000 f = encode_tiled();
+  if (!f) return false;
+  const uint64_t size = type_size(type);
+  cuuint64_t gdim[2] = {dim, rows};
+  cuuint64_t gstride[1] = {ld * size};
+  cuuint32_t b[2] = {(cuuint32_t)(128 / size), box};
+  cuuint32_t es[2] = {1, 1};
+  return f(m, size == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, (void*)base, gdim, gstride,
+           b, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool FP8, int BN>
+cudaError_t launch_score(const CUtensorMap& q, const CUtensorMap& v, const raven_score::Params& p, unsigned grid,
+                         cudaStream_t st) {
+  using L = raven_score::Layout<FP8, BN>;
+  auto kern = raven_score::score_kernel<FP8, BN>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes);
+  if (e != cudaSuccess) return e;
+  kern<<<grid, L::kThreads, L::kBytes, st>>>(q, v, p);
+  return cudaGetLastError();
+}
+
+template <bool FP8>
+cudaError_t dispatch_score(uint32_t bn, const CUtensorMap& q, const CUtensorMap& v, const raven_score::Params& p,
+                           unsigned grid, cudaStream_t st) {
+  if (bn <= 32) return launch_score<FP8, 32>(q, v, p, grid, st);
+  if (bn <= 64) return launch_score<FP8, 64>(q, v, p, grid, st);
+  if (bn <= 128) return launch_score<FP8, 128>(q, v, p, grid, st);
+  return launch_score<FP8, FP8 ? 192 : 256>(q, v, p, grid, st);
+}
+
+int check_rows(const raven_rows* r, uint32_t dim, const char* what) {
+  const std::string w(what);
+  if (!r) return fail(RAVEN_EINVAL, w + ": null");
+  const uint64_t size = type_size(r->type);
+  if (!size) return fail(RAVEN_EINVAL, w + ": unknown type");
+  if (r->rows > kMaxRows) return fail(RAVEN_ELIMIT, w + ": more than 2^31 - 1 rows");
+  if (r->rows == 0) return RAVEN_OK;
+  if (!r->data) return fail(RAVEN_EINVAL, w + ": null data");
+  if (r->ld < dim) return fail(RAVEN_EINVAL, w + ": pitch below dim");
+  if (!aligned(r->data, size)) return fail(RAVEN_EINVAL, w + ": data is not aligned to its type");
+  if (r->type == RAVEN_TYPE_FP8)
+    return check_fp8((const uint8_t*)r->data, r->ld, r->exps, r->ld_exps, dim);
+  return RAVEN_OK;
+}
+
+// Dense (qo null) and grouped scores.
+int run_scores(const raven_rows* q, const int64_t* qo, const raven_rows* v, const int64_t* vo, uint32_t groups,
+               uint32_t dim, float alpha, const float* bias, void* out, int32_t out_type, uint64_t ld, uint64_t capacity,
+               int32_t* status, void* stream) {
+  if (int rc = check_dim(dim)) return rc;
+  if (int rc = check_rows(q, dim, "queries")) return rc;
+  if (int rc = check_rows(v, dim, "vectors")) return rc;
+  if (v->type == RAVEN_TYPE_F32) return fail(RAVEN_EINVAL, "vectors: type must be f16, bf16 or FP8");
+  const bool fp8 = v->type == RAVEN_TYPE_FP8;
+  if (!fp8 && q->type != v->type) return fail(RAVEN_EINVAL, "queries must have the vectors' type");
+  if (out_type != RAVEN_TYPE_F32 && out_type != RAVEN_TYPE_F16 && out_type != RAVEN_TYPE_BF16)
+    return fail(RAVEN_EINVAL, "scores: type must be f32, f16 or bf16");
+  if (q->rows == 0 || v->rows == 0 || groups == 0) return RAVEN_OK;
+  if (!out) return fail(RAVEN_EINVAL, "scores: null output");
+  if (!aligned(out, type_size(out_type))) return fail(RAVEN_EINVAL, "scores: output is not aligned to its type");
+  if (!qo && ld < v->rows) return fail(RAVEN_EINVAL, "scores: output pitch below the number of vectors");
+  const bool encode = fp8 && q->type != RAVEN_TYPE_FP8;
+  if (!fp8)
+    for (const raven_rows* r : {q, v})
+      if (!aligned(r->data, 16) || r->ld % 8)
+        return fail(RAVEN_EINVAL, "16-bit rows must start on 16 bytes, their pitch a multiple of 8 values");
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  cudaStream_t st = (cudaStream_t)stream;  // NULL: the CUDA default stream
+
+  raven_score::Params p{};
+  p.nq = q->rows;
+  p.n = v->rows;
+  const uint64_t bytes = (uint64_t)dim * type_size(v->type);
+  p.nkb = (uint32_t)((bytes + 127) / 128);
+  p.last_k = (uint32_t)((bytes - (p.nkb - 1) * 128ull + 31) / 32);
+  p.groups = groups;
+  p.qo = qo;
+  p.vo = vo;
+  p.alpha = alpha;
+  p.bias = bias;
+  p.out = out;
+  p.out_type = out_type == RAVEN_TYPE_F32 ? raven_score::kOutF32
+               : out_type == RAVEN_TYPE_F16 ? raven_score::kOutF16 : raven_score::kOutBf16;
+  p.ld = ld;
+  p.capacity = capacity;
+  p.status = status;
+  // instruction descriptor, M = 128. FP8: types e4m3 (0), exponent scales (bit 23);
+  // 16-bit: f32 accumulator (bit 4), types f16 (0) or bf16 (1)
+  const uint32_t ty = v->type == RAVEN_TYPE_BF16 ? 1u : 0u;
+  p.idesc = fp8 ? (1u << 23) | (1u << 27) : (1u << 4) | (ty << 7) | (ty << 10) | (8u << 24);
+
+  raven_rows qq = *q;
+  uint8_t* tmp = nullptr;
+  if (encode) {  // the queries' codes live until the product is done, in stream order
+    qq.type = RAVEN_TYPE_FP8;
+    qq.ld = codes_pitch(dim);
+    qq.ld_exps = exps_pitch(dim);
+    const uint64_t cb = (qq.rows * qq.ld + 255) / 256 * 256;
+    CU(cudaMallocAsync((void**)&tmp, cb + qq.rows * qq.ld_exps, st));
+    qq.data = tmp;
+    qq.exps = tmp + cb;
+    const int rc = encode_rows(q->data, q->type, q->rows, dim, q->ld, tmp, qq.ld, tmp + cb, qq.ld_exps, st);
+    if (rc) {
+      cudaFreeAsync(tmp, st);
+      return rc;
+    }
+  }
+  p.qe = qq.exps;
+  p.ve = v->exps;
+  p.ld_qe = qq.ld_exps;
+  p.ld_ve = v->ld_exps;
+
+  // Queries per tile: enough for a group (twice the mean where groups differ),
+  // and not so many that SMs are left without a tile.
+  uint64_t want = qo ? 2 * ((p.nq + groups - 1) / groups) : p.nq;
+  const uint64_t vt = (p.n + raven_score::kBM - 1) / raven_score::kBM;
+  uint32_t bn = want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 ? 128 : fp8 ? 192 : 256;
+  if (!qo)
+    while (bn > 32 && vt * ((p.nq + bn - 1) / bn) < (uint64_t)sms) bn = bn > 128 ? 128 : bn / 2;
+  const uint64_t most = qo ? (uint64_t)sms : vt * ((p.nq + bn - 1) / bn);
+  const unsigned grid = (unsigned)std::min<uint64_t>(most, (uint64_t)sms);
+
+  CUtensorMap mq, mv;
+  cudaError_t e = cudaErrorInvalidValue;
+  if (rows_map(&mq, qq.data, qq.type, dim, qq.rows, qq.ld, raven_score::kQBox) &&
+      rows_map(&mv, v->data, v->type, dim, v->rows, v->ld, raven_score::kBM))
+    e = fp8 ? dispatch_score<true>(bn, mq, mv, p, grid, st) : dispatch_score<false>(bn, mq, mv, p, grid, st);
+  if (tmp) cudaFreeAsync(tmp, st);
+  if (e != cudaSuccess) return fail(RAVEN_ECUDA, std::string("scores: ") + cudaGetErrorString(e));
+  return RAVEN_OK;
+}
+
+// Where each query's scores start in grouped scores: starts[i] for query i of
+// group g is sum over earlier groups of m h_n plus its place times n_g. Blocks
+// take runs of 256 groups; each sums the groups before its run by itself.
+__global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* __restrict__ qo, const int64_t* __restrict__ vo,
+                                                         uint32_t groups, uint64_t nq, uint64_t n,
+                                                         int64_t* __restrict__ starts, int* status) {
+  __shared__ int64_t part[256];
+  __shared__ int64_t gq[256], gm[256], gn[256];
+  const uint32_t g0 = blockIdx.x * 256u, tid = threadIdx.x;
+  bool bad = false;
+  auto read = [&](uint32_t g, int64_t& a, int64_t& m, int64_t& c) {
+    const int64_t q0 = qo[g], q1 = qo[g + 1], v0 = vo[g], v1 = vo[g + 1];
+    const bool ok = q0 >= 0 && q1 >= q0 && (uint64_t)q1 <= nq && v0 >= 0 && v1 >= v0 && (uint64_t)v1 <= n;
+    bad |= !ok;
+    a = ok ? q0 : 0;
+    m = ok ? q1 - q0 : 0;
+    c = ok ? v1 - v0 : 0;
+  };
+  int64_t sum = 0, a, m, c;
+  for (uint32_t g = tid; g < g0; g += 256) {
+    read(g, a, m, c);
+    sum += m * c;
+  }
+  part[tid] = sum;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if ((int)tid < o) part[tid] += part[tid + o];
+    __syncthreads();
+  }
+  const int64_t before = part[0];
+  __syncthreads();
+  a = m = c = 0;
+  if (g0 + tid < groups) read(g0 + tid, a, m, c);
+  gq[tid] = a;
+  gm[tid] = m;
+  gn[tid] = c;
+  part[tid] = m * c;
+  __syncthreads();
+  for (int o = 1; o < 256; o <<= 1) {
+    const int64_t x = (int)tid >= o ? part[tid - o] : 0;
+    __syncthreads();
+    part[tid] += x;
+    __syncthreads();
+  }
+  for (uint32_t j = tid >> 5; j < 256; j += 8) {  // a warp per group
+    const int64_t base = before + part[j] - gm[j] * gn[j];
+    for (int64_t i = tid & 31; i < gm[j]; i += 32) starts[gq[j] + i] = base + i * gn[j];
+  }
+  // queries before the first group start at 0, those behind the last one at the end
+  if (g0 + 256 >= groups) {
+    const int64_t total = before + part[255];
+    int64_t last = qo[groups];
+    last = last < 0 ? 0 : last > (int64_t)nq ? (int64_t)nq : last;
+    for (int64_t i = last + tid; i <= (int64_t)nq; i += 256) starts[i] = total;
+  }
+  if (blockIdx.x == 0) {
+    int64_t first = qo[0];
+    first = first < 0 ? 0 : first > (int64_t)nq ? (int64_t)nq : first;
+    for (int64_t i = tid; i < first; i += 256) starts[i] = 0;
+  }
+  if (bad && status) atomicOr(status, raven_score::kStatusOffsets);
+}
+
+// ---------------------------------------------------------------------------
+// Top-k of rows.
+// ---------------------------------------------------------------------------
+template <typename T, int TEAM>
+cudaError_t launch_topk(const raven_topk::Params& p, cudaStream_t st) {
+  using TM = raven_topk::Team<TEAM>;
+  auto kern = raven_topk::topk_kernel<T, TEAM>;
+  const int smem = TM::kTeams * (int)sizeof(raven_topk::Shared<TEAM>);
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const uint64_t units = p.nq * p.parts;
+  kern<<<(unsigned)((units + TM::kTeams - 1) / TM::kTeams), raven_topk::kCtaThreads, smem, st>>>(p);
+  return cudaGetLastError();
+}
+template <int TEAM>
+cudaError_t dispatch_topk(int32_t type, const raven_topk::Params& p, cudaStream_t st) {
+  return type == RAVEN_TYPE_F32   ? launch_topk<float, TEAM>(p, st)
+         : type == RAVEN_TYPE_F16 ? launch_topk<__half, TEAM>(p, st)
+                                  : launch_topk<__nv_bfloat16, TEAM>(p, st);
+}
+
+}  // namespace
+
+namespace raven_internal {
+
+int fp8_encode_lane_major(const float* d_rows, uint64_t n, uint32_t dim, uint8_t* d_codes, uint64_t ld_codes,
+                          uint8_t* d_exps, uint64_t ld_exps, cudaStream_t st) {
+  if (int rc = check_fp8(d_codes, ld_codes, d_exps, ld_exps, dim)) return rc;
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  CU((launch_encode<float, true>(d_rows, n, dim, dim, d_codes, ld_codes, d_exps, ld_exps, sms, st)));
+  return RAVEN_OK;
+}
+
+}  // namespace raven_internal
+
+extern "C" {
+
+int raven_fp8_encode_device(const void* d_rows, int32_t type, uint64_t n, uint32_t dim, uint64_t ld, uint8_t* d_codes,
+                            uint64_t ld_codes, uint8_t* d_exps, uint64_t ld_exps, void* stream) {
+  NvtxRange nvtx_range("raven.fp8_encode");
+  if (int rc = check_dim(dim)) return rc;
+  if (type != RAVEN_TYPE_F32 && type != RAVEN_TYPE_F16 && type != RAVEN_TYPE_BF16)
+    return fail(RAVEN_EINVAL, "rows: type must be f32, f16 or bf16");
+  if (n == 0) return RAVEN_OK;
+  if (n > kMaxRows) return fail(RAVEN_ELIMIT, "rows: more than 2^31 - 1");
+  if (!d_rows) return fail(RAVEN_EINVAL, "rows: null");
+  if (ld < dim) return fail(RAVEN_EINVAL, "rows: pitch below dim");
+  if (!aligned(d_rows, type_size(type))) return fail(RAVEN_EINVAL, "rows: not aligned to their type");
+  if (int rc = check_fp8(d_codes, ld_codes, d_exps, ld_exps, dim)) return rc;
+  return encode_rows(d_rows, type, n, dim, ld, d_codes, ld_codes, d_exps, ld_exps, (cudaStream_t)stream);
+}
+
+int raven_fp8_decode_device(const uint8_t* d_codes, uint64_t ld_codes, const uint8_t* d_exps, uint64_t ld_exps,
+                            uint64_t n, uint32_t dim, float* d_out, uint64_t ld, void* stream) {
+  NvtxRange nvtx_range("raven.fp8_decode");
+  if (int rc = check_dim(dim)) return rc;
+  if (n == 0) return RAVEN_OK;
+  if (n > kMaxRows) return fail(RAVEN_ELIMIT, "rows: more than 2^31 - 1");
+  if (int rc = check_fp8(d_codes, ld_codes, d_exps, ld_exps, dim)) return rc;
+  if (!d_out || !aligned(d_out, 4)) return fail(RAVEN_EINVAL, "output: null or not aligned to f32");
+  if (ld < dim) return fail(RAVEN_EINVAL, "output: pitch below dim");
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  const unsigned grid = (unsigned)std::min<uint64_t>((n * dim + 255) / 256, (uint64_t)sms * 16);
+  fp8_decode_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(d_codes, ld_codes, d_exps, ld_exps, n, dim, d_out, ld);
+  CU(cudaGetLastError());
+  return RAVEN_OK;
+}
+
+int raven_scores_device(const raven_rows* q, const raven_rows* v, uint32_t dim, float alpha, const float* d_bias,
+                        void* d_out, int32_t out_type, uint64_t ld_out, int32_t* d_status, void* stream) {
+  NvtxRange nvtx_range("raven.scores");
+  return run_scores(q, nullptr, v, nullptr, 1, dim, alpha, d_bias, d_out, out_type, ld_out, 0, d_status, stream);
+}
+
+int raven_group_scores_device(const raven_rows* q, const int64_t* d_q_offsets, const raven_rows* v,
+                              const int64_t* d_v_offsets, uint32_t groups, uint32_t dim, float alpha,
+                              const float* d_bias, void* d_out, int32_t out_type, uint64_t capacity, int32_t* d_status,
+                              void* stream) {
+  NvtxRange nvtx_range("raven.group_scores");
+  if (groups && (!d_q_offsets || !d_v_offsets)) return fail(RAVEN_EINVAL, "offsets: null");
+  if (groups && (!aligned(d_q_offsets, 8) || !aligned(d_v_offsets, 8)))
+    return fail(RAVEN_EINVAL, "offsets: not aligned to 64 bits");
+  if (capacity == 0) groups = 0;
+  return run_scores(q, d_q_offsets, v, d_v_offsets, groups, dim, alpha, d_bias, d_out, out_type, 0, capacity, d_status,
+                    stream);
+}
+
+int raven_group_rows_device(const int64_t* d_q_offsets, const int64_t* d_v_offsets, uint32_t groups, uint64_t nq,
+                            uint64_t n, int64_t* d_row_starts, int32_t* d_status, void* stream) {
+  NvtxRange nvtx_range("raven.group_rows");
+  if (groups == 0) return fail(RAVEN_EINVAL, "groups must be >= 1");
+  if (nq > kMaxRows || n > kMaxRows) return fail(RAVEN_ELIMIT, "more than 2^31 - 1 queries or vectors");
+  if (!d_q_offsets || !d_v_offsets || !d_row_starts) return fail(RAVEN_EINVAL, "null argument");
+  if (!aligned(d_q_offsets, 8) || !aligned(d_v_offsets, 8) || !aligned(d_row_starts, 8))
+    return fail(RAVEN_EINVAL, "offsets and row starts: not aligned to 64 bits");
+  group_rows_kernel<<<(groups + 255) / 256, 256, 0, (cudaStream_t)stream>>>(d_q_offsets, d_v_offsets, groups, nq, n,
+                                                                            d_row_starts, d_status);
+  CU(cudaGetLastError());
+  return RAVEN_OK;
+}
+
+int raven_topk_rows_device(const void* d_scores, int32_t type, uint64_t nq, uint64_t n, uint64_t ld,
+                           const int64_t* d_row_starts, uint32_t k, int32_t largest, void* d_vals, uint32_t* d_ids,
+                           uint32_t* d_counts, void* stream) {
+  NvtxRange nvtx_range("raven.topk_rows");
+  if (type != RAVEN_TYPE_F32 && type != RAVEN_TYPE_F16 && type != RAVEN_TYPE_BF16)
+    return fail(RAVEN_EINVAL, "scores: type must be f32, f16 or bf16");
+  if (k == 0 || k > raven_topk::kMaxK) return fail(RAVEN_ELIMIT, "k must be in 1..256");
+  if (nq > kMaxRows) return fail(RAVEN_ELIMIT, "more than 2^31 - 1 rows");
+  if (!d_row_starts && n > kMaxRows) return fail(RAVEN_ELIMIT, "rows of more than 2^31 - 1 scores");
+  if (nq == 0) return RAVEN_OK;
+  if (!d_vals || !d_ids) return fail(RAVEN_EINVAL, "null output");
+  if (!d_scores && n) return fail(RAVEN_EINVAL, "scores: null");
+  if (!d_row_starts && ld < n) return fail(RAVEN_EINVAL, "scores: pitch below the row length");
+  const uint64_t size = type_size(type);
+  if (!aligned(d_scores, size) || !aligned(d_vals, size) || !aligned(d_ids, 4) || !aligned(d_counts, 4) ||
+      !aligned(d_row_starts, 8))
+    return fail(RAVEN_EINVAL, "an argument is not aligned to its type");
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  raven_topk::Params p{};
+  p.x = d_scores;
+  p.nq = nq;
+  p.n = n;
+  p.ld = ld;
+  p.starts = d_row_starts;
+  p.total = n;
+  p.k = k;
+  p.largest = largest != 0;
+  p.type = type == RAVEN_TYPE_F32 ? 0 : type == RAVEN_TYPE_F16 ? 1 : 2;
+  p.vals = d_vals;
+  p.ids = d_ids;
+  p.counts = d_counts;
+  // A warp takes rows of up to 1024 scores (1024 rows of one wave's teams fill
+  // the GPU), a CTA longer ones; where rows are too few to fill the GPU twice
+  // over, each is split into parts of at least two tiles. Ragged rows go by
+  // their mean.
+  const uint64_t len = d_row_starts ? (n + nq - 1) / nq : n;
+  const bool warp = len <= 1024;
+  uint64_t parts = 1;
+  const uint64_t tile = raven_topk::kCtaThreads * 16ull;
+  if (!warp && nq < 4ull * sms) parts = std::max<uint64_t>(1, std::min<uint64_t>(8ull * sms / nq, len / (2 * tile)));
+  parts = std::min<uint64_t>(parts, 2ull * sms);
+  p.parts = (uint32_t)parts;
+  uint64_t* tmp = nullptr;
+  if (parts > 1) {
+    CU(cudaMallocAsync((void**)&tmp, nq * parts * k * 8, st));
+    p.lists = tmp;
+  }
+  cudaError_t e = warp ? dispatch_topk<32>(type, p, st) : dispatch_topk<raven_topk::kCtaThreads>(type, p, st);
+  if (e == cudaSuccess && parts > 1) {
+    raven_topk::Params j = p;
+    j.x = tmp;
+    j.n = parts * k;
+    j.parts = 1;
+    raven_topk::topk_join_kernel<<<(unsigned)nq, raven_topk::kCtaThreads,
+                                   sizeof(raven_topk::Shared<raven_topk::kCtaThreads>), st>>>(j);
+    e = cudaGetLastError();
+  }
+  if (tmp) cudaFreeAsync(tmp, st);
+  if (e != cudaSuccess) return fail(RAVEN_ECUDA, std::string("topk: ") + cudaGetErrorString(e));
+  return RAVEN_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,305 @@
+"""Exhaustive scores beside the graph search, on torch tensors of one GPU.
+
+* `Fp8Rows`      — embedding rows as e4m3 codes with one power-of-two scale per
+                   128 values (a quarter of f32, like the SQ8 codes, but with a
+                   scale for each block of each row): encode / decode / of_index.
+* `scores`       — every query against every row (FP8, f16 or bf16 rows).
+* `group_scores` — the queries of each group against the rows of that group,
+                   groups of any size: partitions (tenants, lists) of a
+                   collection, or one projection per group.
+* `group_rows`   — where each query's scores start in grouped scores.
+* `top_k`        — the best k of each row of scores, dense or packed.
+
+Everything runs in libraven_gpu.so on the current stream of the tensors'
+device and returns without waiting. The reference has no counterpart: it
+scores every vector only in its tests (test_pybinding.py:16-18), by numpy.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import _lib as L
+
+BLOCK = 128  # values under one scale
+
+_TYPES = {torch.float32: L.RAVEN_TYPE_F32, torch.float16: L.RAVEN_TYPE_F16, torch.bfloat16: L.RAVEN_TYPE_BF16}
+
+
+def _up(x: int, m: int) -> int:
+    return -(-x // m) * m
+
+
+def _matrix(x, name: str) -> torch.Tensor:
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError(f"{name} must be a 2-D tensor")
+    if not x.is_cuda:
+        raise ValueError(f"{name} must be on a GPU")
+    if x.dtype not in _TYPES:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16, not {x.dtype}")
+    if x.shape[1] == 0:
+        raise ValueError(f"{name} has rows of no values")
+    # one row, or rows of one value, may come with any strides
+    if (x.stride(1) != 1 and x.shape[1] > 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        raise ValueError(f"{name} must hold each row's values side by side and its rows one after another")
+    return x
+
+
+def _pitch(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
+
+
+def _on(device: torch.device, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"all tensors must be on {device}, got one on {t.device}")
+
+
+def _call(device: torch.device, fn, *args) -> None:
+    """The library call with `device` current, on its current stream."""
+    if torch.cuda.current_device() == device.index:
+        L.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            L.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+
+
+def aligned_rows(x: torch.Tensor) -> torch.Tensor:
+    """The rows of `x` as `scores` takes 16-bit rows: starting on 16 bytes, 16
+    bytes times a whole number apart. A copy where `x` is not laid out so."""
+    _matrix(x, "rows")
+    step = 16 // x.element_size()
+    if x.data_ptr() % 16 == 0 and _pitch(x) % step == 0:
+        return x
+    out = x.new_empty(x.shape[0], _up(x.shape[1], step))[:, : x.shape[1]]
+    out.copy_(x)
+    return out
+
+
+class Fp8Rows:
+    """Rows held as FP8: `codes` uint8 [n, roundup(dim, 16)] (e4m3) and `exps`
+    uint8 [n, roundup(ceil(dim / 128), 4)]; a value is its code times
+    2^(exps - 127) of its block of 128."""
+
+    def __init__(self, codes: torch.Tensor, exps: torch.Tensor, dim: int):
+        for name, t, most in (("codes", codes, _up(dim, 16)), ("exps", exps, _up(-(-dim // BLOCK), 4))):
+            if t.dtype != torch.uint8 or t.dim() != 2 or not t.is_cuda or t.stride(1) != 1:
+                raise ValueError(f"{name} must be a 2-D uint8 tensor on a GPU, each row's bytes side by side")
+            if t.shape[1] < most:
+                raise ValueError(f"{name} must have at least {most} columns for dim {dim}, got {t.shape[1]}")
+        if dim < 1:
+            raise ValueError("dim must be at least 1")
+        if codes.shape[0] != exps.shape[0] or codes.device != exps.device:
+            raise ValueError("codes and exps must have the same rows and device")
+        self.codes, self.exps, self.dim = codes, exps, int(dim)
+        self.device = codes.device
+        self._rows = L.Rows(codes.data_ptr(), exps.data_ptr(), codes.shape[0], _pitch(codes), _pitch(exps),
+                            L.RAVEN_TYPE_FP8)
+
+    def __len__(self) -> int:
+        return self.codes.shape[0]
+
+    @staticmethod
+    def empty(n: int, dim: int, device) -> "Fp8Rows":
+        """Room for n rows, uninitialised."""
+        if dim < 1 or n < 0:
+            raise ValueError("n must not be negative and dim at least 1")
+        return Fp8Rows(torch.empty(n, _up(dim, 16), dtype=torch.uint8, device=device),
+                       torch.empty(n, _up(-(-dim // BLOCK), 4), dtype=torch.uint8, device=device), dim)
+
+    @staticmethod
+    def encode(x: torch.Tensor, out: Optional["Fp8Rows"] = None) -> "Fp8Rows":
+        """The rows of a float32, float16 or bfloat16 matrix, rounded to nearest
+        even. The scale of a block is the least power of two that brings its
+        values to at most 448; infinities and NaN become NaN. `out`: rows to
+        write instead of new ones (len(x) of them)."""
+        _matrix(x, "x")
+        n, dim = x.shape
+        if out is None:
+            out = Fp8Rows.empty(n, dim, x.device)
+        elif len(out) != n or out.dim != dim:
+            raise ValueError(f"out holds {len(out)} rows of {out.dim}, expected {n} of {dim}")
+        _on(x.device, out.codes)
+        r = out._rows
+        _call(x.device, L.load().raven_fp8_encode_device, x.data_ptr(), _TYPES[x.dtype], n, dim, _pitch(x), r.data, r.ld,
+              r.exps, r.ld_exps)
+        return out
+
+    @staticmethod
+    def of_index(index) -> "Fp8Rows":
+        """FP8 rows of the vectors of a `DeviceIndex`, on its GPU."""
+        device = torch.device("cuda", index.device)
+        out = Fp8Rows.empty(index.n, index.dim, device)
+        r = out._rows
+        _call(device, L.load().raven_index_fp8_device, index._h, r.data, r.ld, r.exps, r.ld_exps)
+        return out
+
+    def decode(self) -> torch.Tensor:
+        """The values, float32 [n, dim] (exact)."""
+        out = torch.empty(len(self), self.dim, dtype=torch.float32, device=self.device)
+        r = self._rows
+        _call(self.device, L.load().raven_fp8_decode_device, r.data, r.ld, r.exps, r.ld_exps, len(self), self.dim,
+              out.data_ptr(), self.dim)
+        return out
+
+    def rows(self, first: int, count: int) -> "Fp8Rows":
+        """Rows [first, first + count), without a copy."""
+        if first < 0 or count < 0 or first + count > len(self):
+            raise ValueError(f"rows [{first}, {first + count}) of {len(self)}")
+        return Fp8Rows(self.codes[first:first + count], self.exps[first:first + count], self.dim)
+
+
+Rows = Union[torch.Tensor, Fp8Rows]
+
+
+def _operands(queries: Rows, vectors: Rows, dtype: torch.dtype, bias: Optional[torch.Tensor]):
+    """(device, dim, queries, vectors) as the library takes them, with what must stay alive."""
+    keep = None
+    if isinstance(vectors, Fp8Rows):
+        device, dim, v, n = vectors.device, vectors.dim, vectors._rows, len(vectors)
+    else:
+        _matrix(vectors, "vectors")
+        if vectors.dtype == torch.float32:
+            raise ValueError("vectors must be Fp8Rows, float16 or bfloat16 (Fp8Rows.encode holds float32 rows as FP8)")
+        device, (n, dim) = vectors.device, vectors.shape
+        if vectors.data_ptr() % 16 or _pitch(vectors) % 8:
+            raise ValueError("16-bit vectors must start on 16 bytes, a multiple of 8 values apart "
+                             "(aligned_rows makes them so)")
+        v = L.Rows(vectors.data_ptr(), None, n, _pitch(vectors), 0, _TYPES[vectors.dtype])
+    if isinstance(queries, Fp8Rows):
+        if not isinstance(vectors, Fp8Rows):
+            raise ValueError("FP8 queries need FP8 vectors")
+        qdim, nq, q, qdev = queries.dim, len(queries), queries._rows, queries.device
+    else:
+        _matrix(queries, "queries")
+        if not isinstance(vectors, Fp8Rows):
+            if queries.dtype != vectors.dtype:
+                raise ValueError(f"queries must have the vectors' type {vectors.dtype}, got {queries.dtype}")
+            queries = aligned_rows(queries)
+        nq, qdim = queries.shape
+        q, qdev, keep = L.Rows(queries.data_ptr(), None, nq, _pitch(queries), 0, _TYPES[queries.dtype]), queries.device, queries
+    if qdim != dim:
+        raise ValueError(f"dim mismatch: expected {dim}, got {qdim}")
+    if qdev != device:
+        raise ValueError(f"all tensors must be on {device}, got one on {qdev}")
+    if dtype not in _TYPES:
+        raise ValueError(f"scores must be float32, float16 or bfloat16, not {dtype}")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()):
+        raise ValueError(f"bias must be a contiguous float32 tensor of {n} values")
+    _on(device, bias)
+    return device, dim, nq, n, q, v, keep
+
+
+def _status(status: Optional[torch.Tensor], device) -> Optional[int]:
+    if status is None:
+        return None
+    if status.dtype != torch.int32 or status.numel() != 1:
+        raise ValueError("status must be an int32 tensor of one value")
+    _on(device, status)
+    return status.data_ptr()
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def scores(queries: Rows, vectors: Rows, *, alpha: float = 1.0, bias: Optional[torch.Tensor] = None,
+           dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None,
+           status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """alpha * <query, vector> + bias[vector] for every pair, [nq, n] of `dtype`:
+    summed in float32 on the tensor cores, rounded once. Float queries against
+    FP8 rows are encoded first. alpha = -2 with the vectors' squared norms as
+    bias ranks like squared distances. `out`: a matrix of `dtype` to write (any
+    row pitch). `status`: an int32 that gets RAVEN_S_* bits."""
+    device, dim, nq, n, q, v, keep = _operands(queries, vectors, dtype, bias)
+    if out is None:
+        out = torch.empty(nq, n, dtype=dtype, device=device)
+    elif out.shape != (nq, n) or out.dtype != dtype or (n > 1 and out.stride(1) != 1) or (nq > 1 and out.stride(0) < n):
+        raise ValueError(f"out must be a {dtype} matrix of {nq} x {n}, each row's values side by side")
+    _on(device, out)
+    _call(device, L.load().raven_scores_device, q, v, dim, alpha, _ptr(bias), out.data_ptr(), _TYPES[dtype],
+          max(_pitch(out), 1), _status(status, device))
+    return out
+
+
+def _offsets(name: str, t: torch.Tensor, device) -> int:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int64 or t.dim() != 1 or t.numel() < 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous 1-D int64 tensor")
+    _on(device, t)
+    return t.numel() - 1
+
+
+def group_scores(queries: Rows, query_offsets: torch.Tensor, vectors: Rows, vector_offsets: torch.Tensor, *,
+                 total: Optional[int] = None, alpha: float = 1.0, bias: Optional[torch.Tensor] = None,
+                 dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None,
+                 status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Scores of the queries [query_offsets[g], query_offsets[g + 1]) against the
+    vectors [vector_offsets[g], vector_offsets[g + 1]) for each group g, packed:
+    groups in order, their queries in order, for each the scores of its group's
+    vectors. Offsets are int64 tensors on the GPU, rising; either side of a group
+    may be empty.
+
+    `total` is the number of scores (the program that made the groups knows it:
+    the sum of queries times vectors; the last of `group_rows`), or `out` a 1-D
+    tensor with room for them. No more than that is written."""
+    device, dim, nq, n, q, v, keep = _operands(queries, vectors, dtype, bias)
+    groups = _offsets("query_offsets", query_offsets, device)
+    if _offsets("vector_offsets", vector_offsets, device) != groups:
+        raise ValueError("query_offsets and vector_offsets must have the same length")
+    if out is None:
+        if total is None:
+            raise ValueError("total or out is needed: the number of scores is known on the GPU only")
+        out = torch.empty(total, dtype=dtype, device=device)
+    elif out.dim() != 1 or out.dtype != dtype or not out.is_contiguous() or (total is not None and out.numel() < total):
+        raise ValueError(f"out must be a contiguous 1-D {dtype} tensor with room for the scores")
+    _on(device, out)
+    _call(device, L.load().raven_group_scores_device, q, query_offsets.data_ptr(), v, vector_offsets.data_ptr(), groups,
+          dim, alpha, _ptr(bias), out.data_ptr(), _TYPES[dtype], out.numel(), _status(status, device))
+    return out
+
+
+def group_rows(query_offsets: torch.Tensor, vector_offsets: torch.Tensor, nq: int, n: int,
+               status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """int64 [nq + 1]: where each query's scores start in the output of
+    `group_scores`, and its size; the row_starts of `top_k`."""
+    device = query_offsets.device
+    groups = _offsets("query_offsets", query_offsets, device)
+    if _offsets("vector_offsets", vector_offsets, device) != groups:
+        raise ValueError("query_offsets and vector_offsets must have the same length")
+    if not query_offsets.is_cuda:
+        raise ValueError("query_offsets must be on a GPU")
+    if groups == 0 or nq < 0 or n < 0:
+        raise ValueError("there must be at least one group, and nq and n must not be negative")
+    out = torch.empty(nq + 1, dtype=torch.int64, device=device)
+    _call(device, L.load().raven_group_rows_device, query_offsets.data_ptr(), vector_offsets.data_ptr(), groups, nq, n,
+          out.data_ptr(), _status(status, device))
+    return out
+
+
+def top_k(scores: torch.Tensor, k: int, *, largest: bool = True,
+          row_starts: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(values [nq, k], ids [nq, k] int32, counts [nq] int32) of the best k
+    (1..256) of each row, best first, equal scores by the lower index, NaN after
+    every number. Rows are those of a matrix, or with `row_starts` (int64, nq + 1
+    values) pieces of a packed 1-D tensor; ids count within the row. Slots past a
+    row's count (rows of fewer than k) are 0."""
+    if not isinstance(scores, torch.Tensor) or not scores.is_cuda or scores.dtype not in _TYPES:
+        raise ValueError("scores must be a float32, float16 or bfloat16 tensor on a GPU")
+    if row_starts is None:
+        if scores.dim() != 2 or (scores.shape[1] > 1 and scores.stride(1) != 1) or \
+                (scores.shape[0] > 1 and scores.stride(0) < scores.shape[1]):
+            raise ValueError("scores must be a matrix with each row's values side by side")
+        (nq, n), ld, starts = scores.shape, _pitch(scores), None
+    else:
+        if scores.dim() != 1 or not scores.is_contiguous():
+            raise ValueError("packed scores must be a contiguous 1-D tensor")
+        nq, n, ld, starts = _offsets("row_starts", row_starts, scores.device), scores.numel(), 0, row_starts.data_ptr()
+    device = scores.device
+    vals = torch.empty(nq, max(k, 0), dtype=scores.dtype, device=device)
+    ids = torch.empty(nq, max(k, 0), dtype=torch.int32, device=device)
+    counts = torch.empty(nq, dtype=torch.int32, device=device)
+    _call(device, L.load().raven_topk_rows_device, scores.data_ptr(), _TYPES[scores.dtype], nq, n, ld, starts, k,
+          int(largest), vals.data_ptr(), ids.data_ptr(), counts.data_ptr())
+    return vals, ids, counts

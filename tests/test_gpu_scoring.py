@@ -1,0 +1,505 @@
+"""Scoring operators on the GPU against 64-bit definitions (scoring_util.py):
+FP8 rows, dense and grouped scores, top-k of rows, and a run of them together."""
+import numpy as np
+import pytest
+
+import scoring_util as U
+
+pytestmark = pytest.mark.gpu
+
+TYPES = ("f32", "f16", "bf16")
+
+
+def _torch():
+    import torch
+
+    return torch
+
+
+def _dt(name):
+    torch = _torch()
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+@pytest.fixture(scope="module")
+def S(raven_lib):
+    from raven_b200 import scoring
+
+    return scoring
+
+
+def _data(n, dim, seed, spread=6.0):
+    """Rows whose blocks differ in size by up to 2^spread either way."""
+    r = np.random.default_rng(seed)
+    x = r.normal(size=(n, dim))
+    nb = -(-dim // U.BLOCK)
+    return x * np.repeat(2.0 ** r.uniform(-spread, spread, (n, nb)), U.BLOCK, axis=1)[:, :dim]
+
+
+def _gpu(x, t="f32"):
+    torch = _torch()
+    return torch.from_numpy(np.ascontiguousarray(x)).cuda().to(_dt(t))
+
+
+def _np(t):
+    return t.double().cpu().numpy()
+
+
+# ---- FP8 rows -----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("n,dim", [(1, 1), (3, 16), (7, 100), (33, 128), (5, 129), (20, 515), (300, 96), (2, 1500)])
+def test_fp8_encode_decode(S, t, n, dim):
+    x = _gpu(_data(n, dim, n * 1000 + dim), t)
+    rows = S.Fp8Rows.encode(x)
+    want, e = U.fp8_values(_np(x))
+    nb = e.shape[1]
+    exps = rows.exps.cpu().numpy().astype(np.int64)
+    np.testing.assert_array_equal(exps[:, :nb] - 127, e)
+    assert np.all(exps[:, nb:] == 127)
+    assert np.all(rows.codes.cpu().numpy()[:, dim:] == 0)
+    np.testing.assert_array_equal(_np(rows.decode()), want)
+
+
+def test_fp8_encode_special_values(S):
+    x = np.zeros((8, 260))
+    x[1, 3] = 1e-42                       # an f32 subnormal: the least exponent
+    x[2, 130] = np.finfo(np.float32).max  # the largest exponent
+    x[3, :5] = [448.0, -448.0, 464.0, 1.0, 2.0 ** -9]
+    x[4, 0], x[4, 1], x[4, 2] = np.inf, 3.0, -np.inf
+    x[5, 200], x[5, 201] = np.nan, -7.0
+    x[6, :] = np.nan
+    x[7, :] = 17.0 * 2.0 ** -np.arange(260.0)  # ties and values below e4m3's normal range
+    rows = S.Fp8Rows.encode(_gpu(x))
+    want, e = U.fp8_values(x.astype(np.float32))
+    np.testing.assert_array_equal(rows.exps.cpu().numpy()[:, :3].astype(np.int64) - 127, e)
+    with np.errstate(over="ignore"):  # f32's largest value rounds to 2^128, which f32 cannot hold
+        np.testing.assert_array_equal(rows.decode().cpu().numpy(), want.astype(np.float32))
+
+
+def test_fp8_encode_ties_to_even(S):
+    # 448 fixes the scale at 1; halves between neighbours go to the even code
+    x = np.zeros((1, 128))
+    x[0, :6] = [448.0, 17.0, 19.0, 25.0, 27.0, -17.0]
+    got = _np(S.Fp8Rows.encode(_gpu(x)).decode())[0, :6]
+    np.testing.assert_array_equal(got, [448.0, 16.0, 20.0, 24.0, 28.0, -16.0])
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_fp8_encode_strided_rows_and_reuse(S, t):
+    torch = _torch()
+    big = _gpu(_data(40, 333, 5), t)
+    x = big[3:33:2, 5:205]  # pitch 666, rows that do not start on 16 bytes
+    want, _ = U.fp8_values(_np(x))
+    out = S.Fp8Rows(torch.full((15, 256), 9, dtype=torch.uint8, device="cuda"),
+                    torch.full((15, 8), 9, dtype=torch.uint8, device="cuda"), 200)
+    assert S.Fp8Rows.encode(x, out=out) is out
+    np.testing.assert_array_equal(_np(out.decode()), want)
+    assert bool((out.codes[:, 208:] == 9).all()) and bool((out.exps[:, 4:] == 9).all())
+
+
+def test_fp8_of_index(S, small_case):
+    from raven_b200.index import DeviceIndex
+
+    base, _, g = small_case
+    rows = S.Fp8Rows.of_index(DeviceIndex(g, base, sq4=True))
+    want = S.Fp8Rows.encode(_gpu(base))
+    assert bool((rows.codes == want.codes).all()) and bool((rows.exps == want.exps).all())
+
+
+# ---- dense scores ---------------------------------------------------------------
+
+
+def _check(got, q, v, t, alpha=1.0, bias=None):
+    exact = alpha * (q @ v.T) + (0.0 if bias is None else bias[None, :])
+    eps = _torch().finfo(_dt(t)).eps
+    off = np.abs(_np(got) - exact)
+    lim = U.score_bound(q, v, alpha, bias, eps, exact)
+    assert off.shape == lim.shape
+    assert np.all(off <= lim), (off / lim).max()
+
+
+SHAPES = [(1, 1, 1), (1, 1000, 128), (3, 77, 100), (16, 128, 96), (17, 129, 130), (33, 1000, 512), (64, 300, 640),
+          (100, 257, 33), (130, 500, 1000), (200, 640, 129), (257, 20000, 64), (500, 311, 2050), (1, 64, 8192)]
+
+
+@pytest.mark.parametrize("nq,n,dim", SHAPES)
+@pytest.mark.parametrize("qt,out", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16")])
+def test_scores_fp8(S, nq, n, dim, qt, out):
+    # bounded spread: f16 scores stay finite
+    q, v = _gpu(_data(nq, dim, 1, 2.0), qt), _gpu(_data(n, dim, 2, 2.0) / dim)
+    rows = S.Fp8Rows.encode(v)
+    got = S.scores(q, rows, dtype=_dt(out))
+    qv, _ = U.fp8_values(_np(q))
+    _check(got, qv, _np(rows.decode()), out)
+    assert bool((S.scores(S.Fp8Rows.encode(q), rows, dtype=_dt(out)) == got).all())
+
+
+def test_scores_fp8_far_scales(S):
+    """Blocks of very different size: every exponent reaches its own block, row and query."""
+    q, v = _gpu(_data(140, 1400, 3, 20.0)), _gpu(_data(270, 1400, 4, 20.0))
+    rows = S.Fp8Rows.encode(v)
+    qv, _ = U.fp8_values(_np(q))
+    _check(S.scores(q, rows), qv, _np(rows.decode()), "f32")
+
+
+@pytest.mark.parametrize("nq,n,dim", SHAPES)
+@pytest.mark.parametrize("t,out", [("f16", "f32"), ("bf16", "bf16")])
+def test_scores_16bit(S, nq, n, dim, t, out):
+    q, v = S.aligned_rows(_gpu(_data(nq, dim, 5, 1.0), t)), S.aligned_rows(_gpu(_data(n, dim, 6, 1.0), t))
+    _check(S.scores(q, v, dtype=_dt(out)), _np(q), _np(v), out)
+
+
+def test_scores_alpha_bias_pitch(S):
+    torch = _torch()
+    q, v = _data(70, 200, 7, 1.0), _data(333, 200, 8, 1.0)
+    rows = S.Fp8Rows.encode(_gpu(v))
+    vv, (qv, _) = _np(rows.decode()), U.fp8_values(_gpu(q).cpu().numpy())
+    norms = (rows.decode() ** 2).sum(1)
+    room = torch.full((70, 400), 7.0, device="cuda")
+    got = S.scores(_gpu(q), rows, alpha=-2.0, bias=norms, out=room[:, 11:344])
+    _check(got, qv, vv, "f32", -2.0, _np(norms))
+    assert bool((room[:, :11] == 7.0).all()) and bool((room[:, 344:] == 7.0).all())
+
+
+def test_scores_not_finite_rows_stay_apart(S):
+    """A row or query with NaN or infinities only spoils its own scores."""
+    q, v = _data(40, 150, 9, 1.0), _data(200, 150, 10, 1.0)
+    clean = S.scores(_gpu(q), S.Fp8Rows.encode(_gpu(v)))
+    q[7, 3], v[131, 140], v[5, 0] = np.nan, np.inf, np.nan
+    got = S.scores(_gpu(q), S.Fp8Rows.encode(_gpu(v)))
+    bad = np.zeros((40, 200), bool)
+    bad[7], bad[:, 131], bad[:, 5] = True, True, True
+    got, clean = _np(got), _np(clean)
+    assert np.all(np.isnan(got[bad]))
+    # the blocks that hold what is not finite have another scale; no other score moves
+    np.testing.assert_array_equal(got[~bad], clean[~bad])
+
+
+def test_scores_empty(S):
+    torch = _torch()
+    rows = S.Fp8Rows.encode(_gpu(_data(5, 64, 1)))
+    assert S.scores(torch.empty(0, 64, device="cuda"), rows).shape == (0, 5)
+    assert S.scores(torch.zeros(3, 64, device="cuda"), rows.rows(2, 0)).shape == (3, 0)
+    assert S.Fp8Rows.encode(torch.empty(0, 64, device="cuda")).decode().shape == (0, 64)
+
+
+def test_scores_large_offsets(S):
+    """Scores past 2^31 elements."""
+    torch = _torch()
+    nq, n = 70_000, 33_000
+    q = torch.randint(-3, 4, (nq, 16), device="cuda").half()
+    v = torch.randint(-3, 4, (n, 16), device="cuda").half()
+    out = S.scores(q, v, dtype=torch.float16)
+    want = q[-300:].float() @ v.float().T  # whole numbers: exact
+    assert bool((out[-300:].float() == want).all())
+    assert bool((out[:200].float() == q[:200].float() @ v.float().T).all())
+
+
+# ---- grouped scores ---------------------------------------------------------------
+
+
+def _groups(seed, groups, nq, n, even=False):
+    r = np.random.default_rng(seed)
+
+    def cut(total):
+        w = r.random(groups) ** 3 * (r.random(groups) > 0.2)
+        w[0] += 1e-3
+        c = np.rint(np.cumsum(w) / w.sum() * total).astype(np.int64)
+        c[-1] = total
+        return np.concatenate([[0], c])
+
+    return cut(nq), np.arange(groups + 1) * (n // groups) if even else cut(n)
+
+
+def _grouped(S, t, out, groups, nq, n, dim, seed, even=False, alpha=1.0, with_bias=False):
+    torch = _torch()
+    qo, vo = _groups(seed, groups, nq, n, even)
+    q, v = _data(nq, dim, seed + 1, 1.0), _data(n, dim, seed + 2, 1.0)
+    bias = np.random.default_rng(seed).normal(size=n).astype(np.float32) if with_bias else None
+    if t == "fp8":
+        qd, rows = _gpu(q, "bf16"), S.Fp8Rows.encode(_gpu(v))
+        qv, vv = U.fp8_values(_np(qd))[0], _np(rows.decode())
+    else:
+        qd, rows = S.aligned_rows(_gpu(q, t)), S.aligned_rows(_gpu(v, t))
+        qv, vv = _np(qd), _np(rows)
+    total = int(((qo[1:] - qo[:-1]) * (vo[1:] - vo[:-1])).sum())
+    room = torch.full((total + 100,), 5.0, dtype=_dt(out), device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = S.group_scores(qd, torch.from_numpy(qo).cuda(), rows, torch.from_numpy(vo).cuda(), total=total, out=room,
+                         dtype=_dt(out), alpha=alpha, bias=None if bias is None else _gpu(bias), status=status)
+    assert int(status) == 0
+    assert bool((room[total:] == 5.0).all())
+    at = 0
+    for g in range(groups):
+        m, c = int(qo[g + 1] - qo[g]), int(vo[g + 1] - vo[g])
+        if m * c:
+            _check(got[at:at + m * c].view(m, c), qv[qo[g]:qo[g + 1]], vv[vo[g]:vo[g + 1]], out, alpha,
+                   None if bias is None else bias[vo[g]:vo[g + 1]].astype(np.float64))
+        at += m * c
+    assert at == total
+    starts = S.group_rows(torch.from_numpy(qo).cuda(), torch.from_numpy(vo).cuda(), nq, n).cpu().numpy()
+    width = np.zeros(nq, np.int64)
+    for g in range(groups):
+        width[qo[g]:qo[g + 1]] = vo[g + 1] - vo[g]
+    np.testing.assert_array_equal(starts, np.concatenate([[0], np.cumsum(width)]))
+
+
+@pytest.mark.parametrize("t,out", [("f16", "f32"), ("bf16", "bf16"), ("fp8", "f32"), ("fp8", "f16")])
+@pytest.mark.parametrize("groups,nq,n,dim,even", [(1, 5, 7, 8, False), (3, 40, 700, 128, False),
+                                                  (40, 300, 3000, 72, False), (70, 200, 7000, 520, True),
+                                                  (300, 1000, 2000, 40, False), (5, 900, 1500, 136, False),
+                                                  (2, 3, 4, 1000, False)])
+def test_group_scores(S, t, out, groups, nq, n, dim, even):
+    _grouped(S, t, out, groups, nq, n, dim, groups + nq, even)
+
+
+def test_group_scores_alpha_bias(S):
+    _grouped(S, "fp8", "f32", 9, 80, 900, 200, 3, alpha=-2.0, with_bias=True)
+    _grouped(S, "bf16", "f32", 9, 80, 900, 200, 4, alpha=0.5, with_bias=True)
+
+
+def test_group_scores_rows_outside_groups(S):
+    """Offsets need not cover the rows: what lies outside has no scores, and an
+    unreached NaN row spoils none."""
+    torch = _torch()
+    q, v = _gpu(_data(50, 64, 1, 1.0), "f16"), _gpu(_data(90, 64, 2, 1.0), "f16")
+    q[:4], q[30:], v[:10], v[60:] = float("nan"), float("nan"), float("nan"), float("nan")
+    qo, vo = torch.tensor([4, 4, 30], device="cuda"), torch.tensor([10, 20, 60], device="cuda")
+    got = S.group_scores(q, qo, v, vo, total=26 * 40)
+    _check(got.view(26, 40), _np(q)[4:30], _np(v)[20:60], "f32")
+    starts = S.group_rows(qo, vo, 50, 90).cpu().numpy()
+    np.testing.assert_array_equal(starts, [0] * 4 + list(range(0, 26 * 40, 40)) + [26 * 40] * 21)
+
+
+def test_group_scores_bad_offsets_and_small_outputs(S):
+    """Offsets that fall or leave the rows count as empty groups; scores past the
+    output are not written; both set the status."""
+    torch = _torch()
+    q, v = _gpu(_data(20, 64, 1, 1.0), "bf16"), _gpu(_data(30, 64, 2, 1.0), "bf16")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for qo, vo in (([0, 10, 5], [0, 10, 20]), ([0, 10, 20], [0, 10, 31]), ([-1, 10, 20], [0, 0, 30]),
+                   ([0, 10, 20], [0, 1 << 62, 30])):
+        status.zero_()
+        room = torch.full((700,), 5.0, device="cuda")
+        S.group_scores(q, torch.tensor(qo, device="cuda"), v, torch.tensor(vo, device="cuda"), out=room, status=status)
+        assert int(status) & 1
+        status.zero_()
+        S.group_rows(torch.tensor(qo, device="cuda"), torch.tensor(vo, device="cuda"), 20, 30, status=status)
+        assert int(status) & 1
+    status.zero_()
+    room = torch.full((700,), 5.0, device="cuda")
+    qo, vo = torch.tensor([0, 20], device="cuda"), torch.tensor([0, 30], device="cuda")
+    S.group_scores(q, qo, v, vo, out=room[:100], status=status)  # three queries' scores fit
+    assert int(status) == 2
+    _check(room[:90].view(3, 30), _np(q)[:3], _np(v), "f32")
+    assert bool((room[90:] == 5.0).all())
+
+
+# ---- top-k --------------------------------------------------------------------------
+
+
+def _top(S, rows, k, largest, t, ragged):
+    torch = _torch()
+    if ragged:
+        flat = np.concatenate([np.asarray(r, np.float64) for r in rows]) if rows else np.zeros(0)
+        x = _gpu(flat, t)
+        starts = np.concatenate([[0], np.cumsum([len(r) for r in rows])]).astype(np.int64)
+        vals, ids, counts = S.top_k(x, k, largest=largest, row_starts=torch.from_numpy(starts).cuda())
+        held = _np(x)
+        rows = [held[a:b] for a, b in zip(starts[:-1], starts[1:])]
+    else:
+        x = _gpu(np.asarray(rows), t)
+        vals, ids, counts = S.top_k(x, k, largest=largest)
+        rows = list(_np(x))
+    wv, wi, wc = U.top_k(rows, k, largest)
+    np.testing.assert_array_equal(counts.cpu().numpy(), wc)
+    np.testing.assert_array_equal(_np(vals), wv)
+    np.testing.assert_array_equal(ids.cpu().numpy(), wi)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("largest", [True, False])
+@pytest.mark.parametrize("nq,n,k", [(1, 1, 1), (3, 5, 8), (9, 100, 10), (40, 1000, 33), (5, 1025, 256), (2, 5000, 1),
+                                    (7, 9001, 100), (700, 3000, 10), (1, 300_001, 10), (2, 100_003, 256),
+                                    (600, 5003, 256)])
+def test_top_k(S, t, largest, nq, n, k):
+    r = np.random.default_rng(nq + n + k)
+    _top(S, r.normal(size=(nq, n)), k, largest, t, False)
+
+
+@pytest.mark.parametrize("kind", ["equal", "rising", "falling", "few", "special", "nan"])
+@pytest.mark.parametrize("n,k", [(40, 50), (700, 20), (9000, 64), (40_000, 256)])
+def test_top_k_hard_rows(S, kind, n, k):
+    r = np.random.default_rng(n)
+    x = {"equal": np.full((3, n), 2.5), "rising": np.tile(np.arange(n) / 1000.0, (3, 1)),
+         "falling": np.tile(-np.arange(n) / 1000.0, (3, 1)), "few": r.integers(0, 3, (3, n)).astype(float),
+         "special": r.choice([0.0, -0.0, np.inf, -np.inf, np.nan, 1.0, -1.0], (3, n)),
+         "nan": np.full((3, n), np.nan)}[kind]
+    for largest in (True, False):
+        _top(S, x, k, largest, "f32", False)
+        _top(S, x, k, largest, "bf16", False)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_top_k_ragged(S, t):
+    r = np.random.default_rng(4)
+    for lens in ([0], [0, 3, 0, 1, 17], list(r.integers(0, 60, 300)), [50_000, 0, 1, 20_011], list(r.integers(0, 9000, 40))):
+        _top(S, [r.normal(size=n) for n in lens], 16, True, t, True)
+        _top(S, [r.integers(0, 9, n).astype(float) for n in lens], 100, False, t, True)
+
+
+def test_top_k_pitch_and_bad_starts(S):
+    torch = _torch()
+    x = torch.randn(9, 3000, device="cuda")
+    for part in (x[:, 1:2001], x[1::3, 7:1500], x[:, :1]):
+        got = S.top_k(part, 5)
+        want = U.top_k(list(_np(part)), 5, True)
+        np.testing.assert_array_equal(got[1].cpu().numpy(), want[1])
+    # starts that fall or leave the scores: those rows are cut to what is there
+    flat = torch.arange(100.0, device="cuda")
+    vals, ids, counts = S.top_k(flat, 3, row_starts=torch.tensor([-5, 10, 5, 90, 1 << 60], device="cuda"))
+    assert counts.tolist() == [0, 0, 3, 3] and vals[2].tolist() == [89.0, 88.0, 87.0] and vals[3].tolist() == [99.0, 98.0, 97.0]
+
+
+# ---- together ------------------------------------------------------------------------
+
+
+def test_partitioned_search(S):
+    """Queries go to their best partition by the centroids' scores, are scored
+    against its rows, and keep the best ten: the run a program makes."""
+    torch = _torch()
+    parts, n, nq, dim, k = 30, 6000, 200, 128, 10
+    x, q = _data(n, dim, 1, 0.5), _gpu(_data(nq, dim, 2, 0.5))
+    vo = _groups(5, parts, 0, n)[1]
+    cent = _gpu(np.stack([x[a:b].mean(0) if b > a else np.full(dim, -1e3) for a, b in zip(vo[:-1], vo[1:])]))
+    rows = S.Fp8Rows.encode(_gpu(x))
+    _, best, _ = S.top_k(S.scores(q, S.Fp8Rows.encode(cent)), 1)
+    order = torch.argsort(best[:, 0].long(), stable=True)
+    qo = torch.searchsorted(best[order, 0].long(), torch.arange(parts + 1, device="cuda"))
+    vod = torch.from_numpy(vo).cuda()
+    starts = S.group_rows(qo, vod, nq, n)
+    packed = S.group_scores(q[order], qo, rows, vod, total=int(starts[-1]))
+    vals, ids, counts = S.top_k(packed, k, row_starts=starts)
+    # the same from the whole matrix of scores
+    full = S.scores(q[order], rows)
+    b = best[order, 0].long().tolist()
+    for i in range(nq):
+        lo, hi = int(vo[b[i]]), int(vo[b[i] + 1])
+        assert bool((packed[int(starts[i]):int(starts[i + 1])] == full[i, lo:hi]).all())
+    wv, wi, wc = U.top_k([_np(full[i, int(vo[b[i]]):int(vo[b[i] + 1])]) for i in range(nq)], k, True)
+    np.testing.assert_array_equal(counts.cpu().numpy(), wc)
+    np.testing.assert_array_equal(ids.cpu().numpy(), wi)
+    np.testing.assert_array_equal(_np(vals), wv)
+
+
+def test_nearest_by_scores_matches_exact_knn(S, small_case):
+    """alpha = -2 with squared norms as bias, then the smallest ten, finds the
+    exact kNN of the rows that the FP8 codes stand for."""
+    torch = _torch()
+    from raven_b200.index import DeviceIndex
+
+    base, q, g = small_case
+    rows = S.Fp8Rows.of_index(DeviceIndex(g, base, sq4=True))
+    v = rows.decode().double()
+    qv = S.Fp8Rows.encode(_gpu(q)).decode().double()
+    sc = S.scores(_gpu(q), rows, alpha=-2.0, bias=(v ** 2).sum(1).float())
+    vals, ids, _ = S.top_k(sc, 10, largest=False)
+    d = torch.cdist(qv, v) ** 2 - (qv ** 2).sum(1, keepdim=True)
+    want = torch.sort(d, dim=1).values[:, :10]
+    # scores of at most 2^22 in f32: 128 additions and the bias are off by at most 130 * 2^-23 * 2^22
+    assert float((vals.double() - want).abs().max()) <= 65.0 + 1e-3
+    exact_at = d.gather(1, ids.long())
+    assert float((vals.double() - exact_at).abs().max()) <= 65.0 + 1e-3
+
+
+def test_streams_and_graphs(S):
+    """Two streams at once, and two captured graphs replayed on new inputs, give
+    what eager calls give."""
+    torch = _torch()
+    rows = S.Fp8Rows.encode(_gpu(_data(5000, 256, 1, 1.0)))
+    qs = [_gpu(_data(300, 256, 10 + i, 1.0)) for i in range(4)]
+    want = [S.top_k(S.scores(q, rows), 20) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for _ in range(5):
+        got = []
+        for s, q in zip(streams, qs):
+            with torch.cuda.stream(s):
+                got.append(S.top_k(S.scores(q, rows), 20))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(bool((x == y).all()) for x, y in zip(a, b))
+    long = _gpu(np.random.default_rng(0).normal(size=(2, 200_000)))
+    want_long = S.top_k(long, 50)
+    graphs = []
+    for q in qs[:2]:
+        buf = torch.empty_like(q)
+        graph = torch.cuda.CUDAGraph()
+        side = torch.cuda.Stream()
+        with torch.cuda.graph(graph, stream=side):
+            r = S.top_k(S.scores(buf, rows), 20)
+            r_long = S.top_k(long, 50)
+        graphs.append((graph, buf, r, r_long))
+    for turn in range(3):
+        for (graph, buf, _, _), s, i in zip(graphs, streams, (turn % 4, (turn + 1) % 4)):
+            with torch.cuda.stream(s):
+                buf.copy_(qs[i])
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, r, r_long), i in zip(graphs, (turn % 4, (turn + 1) % 4)):
+            assert all(bool((x == y).all()) for x, y in zip(r, want[i]))
+            assert all(bool((x == y).all()) for x, y in zip(r_long, want_long))
+
+
+def test_same_results_every_time(S):
+    torch = _torch()
+    q, rows = _gpu(_data(90, 700, 1, 1.0)), S.Fp8Rows.encode(_gpu(_data(3000, 700, 2, 1.0)))
+    a = [S.scores(q, rows) for _ in range(5)]
+    x = torch.randint(0, 50, (300, 20_000), device="cuda").float()
+    b = [S.top_k(x, 40) for _ in range(5)]
+    for y in a[1:]:
+        assert bool((y == a[0]).all())
+    for y in b[1:]:
+        assert all(bool((u == w).all()) for u, w in zip(y, b[0]))
+
+
+def test_refusals(S):
+    torch = _torch()
+    f = lambda *s, t="f32": torch.zeros(*s, device="cuda", dtype=_dt(t))  # noqa: E731
+    rows = S.Fp8Rows.encode(f(10, 64))
+    off = torch.tensor([0, 5], device="cuda")
+    for call in (
+        lambda: S.scores(f(3, 32), rows),                                  # dim
+        lambda: S.scores(f(3, 64), f(4, 64)),                              # float32 vectors
+        lambda: S.scores(f(3, 64, t="f16"), f(4, 64, t="bf16")),           # two types
+        lambda: S.scores(rows, f(4, 64, t="bf16")),                        # FP8 queries, 16-bit vectors
+        lambda: S.scores(f(3, 60, t="f16"), f(4, 60, t="f16")),            # pitch of 120 bytes
+        lambda: S.scores(f(3, 64, t="f16"), f(4, 72, t="f16")[:, 1:65]),   # not on 16 bytes
+        lambda: S.scores(f(3, 64), rows, bias=f(9)),
+        lambda: S.scores(f(3, 64), rows, out=f(3, 9)),
+        lambda: S.scores(f(3, 64), rows, dtype=torch.float64),
+        lambda: S.scores(f(3, 64).cpu(), rows),
+        lambda: S.scores(f(3, 64), rows, status=torch.zeros(1, dtype=torch.int64, device="cuda")),
+        lambda: S.scores(f(64, 3).T, rows),
+        lambda: S.group_scores(f(3, 64), off, rows, off),                  # no size
+        lambda: S.group_scores(f(3, 64), off.int(), rows, off, total=1),
+        lambda: S.group_scores(f(3, 64), off, rows, torch.tensor([0, 1, 2], device="cuda"), total=1),
+        lambda: S.group_scores(f(3, 64), off, rows, off, total=20, out=f(10)),
+        lambda: S.Fp8Rows.encode(f(10, 64), out=rows.rows(0, 9)),
+        lambda: S.Fp8Rows(rows.codes[:, :48], rows.exps, 64),
+        lambda: rows.rows(5, 6),
+        lambda: S.top_k(f(4, 4).T, 2),
+        lambda: S.top_k(f(16), 2),
+        lambda: S.top_k(f(4, 4).int(), 2),
+    ):
+        with pytest.raises(ValueError):
+            call()
+    from raven_b200 import RavenError
+
+    for call in (lambda: S.top_k(f(4, 4), 0), lambda: S.top_k(f(4, 4), 257),
+                 lambda: S.Fp8Rows.encode(f(2, 65537))):
+        with pytest.raises(RavenError):
+            call()
