@@ -21,8 +21,8 @@
 //   warp 0      TMA: per K block 128 rows of v and the tile's queries
 //   warp 1      issues the MMAs
 //   warp 2      owns the tensor memory; finds the CTA's tiles
-//   warps 4-7   epilogue: one accumulator is stored while the next is filled
-//   warps 8-11  (FP8) bring the tile's exponents to tensor memory, each warp
+//   warps 4-11  epilogue: one accumulator is stored while the next is filled
+//   warps 12-15 (FP8) bring the tile's exponents to tensor memory, each warp
 //               its 32 lanes (every lane quadrant holds a copy)
 // A tile's size is known on the device only (group sizes are device data): the
 // N of its instructions and the queries it loads follow the group.
@@ -51,7 +51,6 @@ using raven_tc::sw128_desc;
 using raven_tc::tc_fence_after;
 using raven_tc::tc_fence_before;
 using raven_tc::tma_load_2d;
-using raven_tc::tmem_ld32;
 
 constexpr int kBM = 128;               // rows of v per tile
 constexpr int kQBox = 32;              // queries per TMA box
@@ -60,7 +59,7 @@ constexpr uint32_t kQBoxBytes = kQBox * 128;
 constexpr int kInfo = 4;               // tiles found ahead
 constexpr int kSf = 4;                 // exponent buffers in tensor memory
 constexpr int kSfCols = 16;            // columns of one: 4 for the rows, 8 for the queries
-constexpr uint64_t kBand = 8;          // query tiles walked together (they share a tile of v in L2)
+constexpr uint32_t kBand = 8;          // query tiles walked together (they share a tile of v in L2)
 
 enum : int { kOutF32 = 0, kOutF16 = 1, kOutBf16 = 2 };
 enum : int { kStatusOffsets = 1, kStatusCapacity = 2, kStatusWait = 4 };
@@ -96,8 +95,8 @@ template <bool FP8, int BN>
 struct Layout {
   static constexpr uint32_t kStage = kABytes + BN * 128;
   static constexpr int kStages = (int)((204u * 1024) / kStage) < 10 ? (int)((204u * 1024) / kStage) : 10;
-  static constexpr int kThreads = FP8 ? 384 : 256;
-  static constexpr int kConsumers = FP8 ? 10 : 6;  // arrivals that free a tile slot
+  static constexpr int kThreads = FP8 ? 512 : 384;
+  static constexpr int kConsumers = FP8 ? 14 : 10;  // arrivals that free a tile slot
   static constexpr uint32_t kBars = kStages * kStage;
   // full[S], empty[S], acc_full[2], acc_empty[2], info_full[I], info_empty[I], sf_full[F], sf_empty[F], drain
   static constexpr uint32_t kNumBars = 2 * kStages + 4 + 2 * kInfo + 2 * kSf + 1;
@@ -129,7 +128,8 @@ __device__ inline void mma_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t ide
 
 // Finds the tiles of one CTA, in order, by one warp: groups are read 32 at a
 // time (one per lane) and their tiles counted by a warp scan; a CTA's tiles
-// rise, so the groups are walked once.
+// rise, so the groups are walked once. The lane that holds a tile's group works
+// out the tile. Its divisions are 32-bit ones unless the group has 2^32 tiles.
 template <int BN>
 struct TileFinder {
   const Params& p;
@@ -142,7 +142,7 @@ struct TileFinder {
   int64_t before = 0;       // output elements before it, in the chunk
   uint64_t chunk_tiles = 0;
   int64_t chunk_out = 0;
-  uint64_t qa = 0, va = 0, m = 0, nn = 0;
+  uint32_t qa = 0, va = 0, m = 0, nn = 0;  // its first query and row, how many
   bool bad = false;
 
   __device__ TileFinder(const Params& p_, int lane_) : p(p_), lane(lane_) { load(); }
@@ -156,19 +156,19 @@ struct TileFinder {
         if (q0 < 0 || q1 < q0 || (uint64_t)q1 > p.nq || v0 < 0 || v1 < v0 || (uint64_t)v1 > p.n) {
           bad = true;  // the group counts as empty
         } else {
-          qa = (uint64_t)q0;
-          va = (uint64_t)v0;
-          m = (uint64_t)(q1 - q0);
-          nn = (uint64_t)(v1 - v0);
+          qa = (uint32_t)q0;
+          va = (uint32_t)v0;
+          m = (uint32_t)(q1 - q0);
+          nn = (uint32_t)(v1 - v0);
         }
       } else {
-        m = p.nq;
-        nn = p.n;
+        m = (uint32_t)p.nq;
+        nn = (uint32_t)p.n;
       }
     }
-    tiles = ((m + BN - 1) / BN) * ((nn + kBM - 1) / kBM);
+    tiles = (uint64_t)((m + BN - 1) / BN) * ((nn + kBM - 1) / kBM);
     incl = tiles;
-    int64_t e = (int64_t)(m * nn);
+    int64_t e = (int64_t)m * nn;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint64_t t = __shfl_up_sync(0xffffffffu, incl, o);
@@ -178,43 +178,44 @@ struct TileFinder {
         e += x;
       }
     }
-    before = e - (int64_t)(m * nn);
+    before = e - (int64_t)m * nn;
     chunk_tiles = __shfl_sync(0xffffffffu, incl, 31);
     chunk_out = __shfl_sync(0xffffffffu, e, 31);
   }
 
-  // Tile t (rising between calls); qcnt 0 when there is none.
-  __device__ Tile find(uint64_t t) {
-    Tile r;
-    r.qcnt = 0;
+  // The lane whose group holds tile t (rising between calls); -1 when there is none.
+  __device__ int find(uint64_t t) {
     while (t >= first + chunk_tiles) {
+      if (g0 + 32 >= p.groups || g0 + 32 < g0) return -1;
       first += chunk_tiles;
       out0 += chunk_out;
-      if (g0 + 32 >= p.groups || g0 + 32 < g0) {
-        g0 = p.groups;
-        chunk_tiles = 0;
-        return r;
-      }
       g0 += 32;
       load();
     }
-    const uint32_t hit = __ballot_sync(0xffffffffu, t - first < incl);
-    const int s = __ffs(hit) - 1;
-    const uint64_t in = t - first - (__shfl_sync(0xffffffffu, incl, s) - __shfl_sync(0xffffffffu, tiles, s));
-    const uint64_t gm = __shfl_sync(0xffffffffu, m, s), gn = __shfl_sync(0xffffffffu, nn, s);
-    const uint64_t gq = __shfl_sync(0xffffffffu, qa, s), gv = __shfl_sync(0xffffffffu, va, s);
-    const int64_t go = out0 + __shfl_sync(0xffffffffu, before, s);
+    return __ffs(__ballot_sync(0xffffffffu, t - first < incl)) - 1;
+  }
+  // Tile t of this lane's group.
+  __device__ Tile tile(uint64_t t) const {
+    const uint64_t in = t - first - (incl - tiles);
     // bands of kBand query tiles; in a band, all its query tiles of one row tile before the next
-    const uint64_t mt = (gm + BN - 1) / BN, nt = (gn + kBM - 1) / kBM;
-    const uint64_t band = in / (kBand * nt), rest = in - band * kBand * nt;
-    const uint64_t wide = min(kBand, mt - band * kBand);
-    const uint64_t ti = rest / wide, qi = band * kBand + rest - ti * wide;
-    r.ld = p.qo ? (int64_t)gn : (int64_t)p.ld;
-    r.out = go + (int64_t)(qi * BN) * r.ld + (int64_t)(ti * kBM);
-    r.vrow = (uint32_t)(gv + ti * kBM);
-    r.qrow = (uint32_t)(gq + qi * BN);
-    r.vcnt = (uint32_t)min((uint64_t)kBM, gn - ti * kBM);
-    r.qcnt = (uint32_t)min((uint64_t)BN, gm - qi * BN);
+    const uint32_t mt = (m + BN - 1) / BN, nt = (nn + kBM - 1) / kBM;
+    uint32_t band, rest;
+    if (in >> 32) {
+      band = (uint32_t)(in / (kBand * nt));
+      rest = (uint32_t)(in - (uint64_t)band * kBand * nt);
+    } else {
+      band = mt <= kBand ? 0u : (uint32_t)in / (kBand * nt);
+      rest = (uint32_t)in - band * kBand * nt;
+    }
+    const uint32_t wide = min(kBand, mt - band * kBand);
+    const uint32_t ti = rest / wide, qi = band * kBand + rest - ti * wide;
+    Tile r;
+    r.ld = p.qo ? (int64_t)nn : (int64_t)p.ld;
+    r.out = out0 + before + (int64_t)(qi * BN) * r.ld + (int64_t)(ti * kBM);
+    r.vrow = va + ti * kBM;
+    r.qrow = qa + qi * BN;
+    r.vcnt = min((uint32_t)kBM, nn - ti * kBM);
+    r.qcnt = min((uint32_t)BN, m - qi * BN);
     return r;
   }
 };
@@ -230,13 +231,43 @@ struct TileReader {
   }
 };
 
-__device__ inline void store_score(void* out, int type, int64_t at, float v) {
-  if (type == kOutF32)
-    ((float*)out)[at] = v;
-  else if (type == kOutF16)
-    ((__half*)out)[at] = __float2half_rn(v);
-  else
-    ((__nv_bfloat16*)out)[at] = __float2bfloat16_rn(v);
+// 16 consecutive accumulator columns of this thread's lane, without waiting.
+__device__ inline void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];\n"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+}
+__device__ inline void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+
+__device__ inline void put(float* p, float v) { *p = v; }
+__device__ inline void put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ inline void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// One epilogue warp's share of a tile: columns first, first + 32, ... in pieces
+// of 16. `at`: this lane's score of query 0.
+template <typename T>
+__device__ inline void store_tile(T* at, int64_t ld, uint32_t acc, uint32_t first, uint32_t qcnt, bool row, float alpha,
+                                  float bias) {
+  for (uint32_t c = first; c < qcnt; c += 32) {
+    uint32_t v[16];
+    tmem_ld16(acc + c, v);
+    tmem_wait_ld();
+    if (row) {
+      T* o = at + (int64_t)c * ld;
+      if (c + 16 <= qcnt) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j, o += ld) put(o, fmaf(alpha, __uint_as_float(v[j]), bias));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j, o += ld)
+          if (c + j < qcnt) put(o, fmaf(alpha, __uint_as_float(v[j]), bias));
+      }
+    }
+    __syncwarp();
+  }
 }
 
 template <bool FP8, int BN>
@@ -268,7 +299,7 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), 4);
+      mbar_init(acc_empty(b), 8);
     }
     for (int i = 0; i < kInfo; ++i) {
       mbar_init(info_full(i), 1);
@@ -394,26 +425,30 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
       ok &= mbar_wait(drain, 0);
     }
   } else if (warp == 2) {  // tiles
-    TileFinder<BN> find(p, lane);
+    TileFinder<BN> finder(p, lane);
     TileReader wr;
     for (uint64_t t = blockIdx.x;; t += gridDim.x) {
-      const Tile r = find.find(t);
+      const int at = finder.find(t);
       const bool got = mbar_wait(info_empty(wr.slot), wr.phase ^ 1u);
       if (!__all_sync(0xffffffffu, got)) {
         ok = false;
         break;
       }
-      if (lane == 0) {
-        tiles[wr.slot] = r;
+      if (lane == max(at, 0)) {
+        if (at < 0)
+          tiles[wr.slot].qcnt = 0;
+        else
+          tiles[wr.slot] = finder.tile(t);
         mbar_arrive(info_full(wr.slot));
       }
       __syncwarp();
       wr.next();
-      if (r.qcnt == 0) break;
+      if (at < 0) break;
     }
-    if (__any_sync(0xffffffffu, find.bad) && lane == 0 && p.status) atomicOr(p.status, kStatusOffsets);
-  } else if (warp >= 4 && warp < 8) {  // epilogue
+    if (__any_sync(0xffffffffu, finder.bad) && lane == 0 && p.status) atomicOr(p.status, kStatusOffsets);
+  } else if (warp >= 4 && warp < 12) {  // epilogue: two warps per lane quadrant, 16 columns in turn
     const int quad = warp & 3;
+    const uint32_t first = warp < 8 ? 0u : 16u;
     const uint32_t r = (uint32_t)(quad * 32 + lane);
     const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
     TileReader rd;
@@ -446,25 +481,22 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
           if (lane == 0 && p.status) atomicOr(p.status, kStatusCapacity);
         }
       }
-      for (uint32_t c = 0; c < qcnt; c += 32) {
-        uint32_t v[32];
-        tmem_ld32(tmem + lane_base + b * BN + c, v);
-        if (r < t.vcnt) {
-          const int64_t at = t.out + (int64_t)c * t.ld + r;
-          const uint32_t m = min(32u, qcnt - c);
-#pragma unroll
-          for (uint32_t j = 0; j < 32; ++j)
-            if (j < m) store_score(p.out, p.out_type, at + (int64_t)j * t.ld, fmaf(p.alpha, __uint_as_float(v[j]), bias));
-        }
-        __syncwarp();
-      }
+      const uint32_t acc = tmem + lane_base + b * BN;
+      const int64_t at = t.out + r;
+      const bool row = r < t.vcnt;
+      if (p.out_type == kOutF32)
+        store_tile((float*)p.out + at, t.ld, acc, first, qcnt, row, p.alpha, bias);
+      else if (p.out_type == kOutF16)
+        store_tile((__half*)p.out + at, t.ld, acc, first, qcnt, row, p.alpha, bias);
+      else
+        store_tile((__nv_bfloat16*)p.out + at, t.ld, acc, first, qcnt, row, p.alpha, bias);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(acc_empty(b));
       b ^= 1u;
       bph ^= b == 0u;
     }
-  } else if (FP8 && warp >= 8) {  // exponents
+  } else if (FP8 && warp >= 12) {  // exponents
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     TileReader rd;
     uint32_t f = 0, fph = 0;
@@ -479,19 +511,19 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
       if (lane == 0) mbar_arrive(info_empty(rd.slot));
       rd.next();
       if (t.qcnt == 0) break;
+      // column j, lane i: the word of row 32 j + i (rows past the arrays' ends repeat the last one)
+      const uint8_t *ve[4], *qe[8];
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) ve[j] = p.ve + min((uint64_t)t.vrow + 32 * j + lane, p.n - 1) * p.ld_ve;
+#pragma unroll
+      for (uint32_t j = 0; j < BN / 32; ++j) qe[j] = p.qe + min((uint64_t)t.qrow + 32 * j + lane, p.nq - 1) * p.ld_qe;
       for (uint32_t kb = 0; kb < p.nkb; kb += 4) {
-        // column j, lane i: the word of row 32 j + i (rows past the arrays' ends repeat the last one)
-        uint32_t w[12];
+        uint32_t w[12] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-          const uint64_t row = min((uint64_t)t.vrow + 32 * j + lane, p.n - 1);
-          w[j] = *(const uint32_t*)(p.ve + row * p.ld_ve + kb);
-        }
+        for (uint32_t j = 0; j < 4; ++j) w[j] = *(const uint32_t*)(ve[j] + kb);
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) {
-          const uint64_t row = min((uint64_t)t.qrow + 32 * j + lane, p.nq - 1);
-          w[4 + j] = 32 * j < t.qcnt ? *(const uint32_t*)(p.qe + row * p.ld_qe + kb) : 0u;
-        }
+        for (uint32_t j = 0; j < BN / 32; ++j)
+          if (32 * j < t.qcnt) w[4 + j] = *(const uint32_t*)(qe[j] + kb);
         got = mbar_wait(sf_empty(f), fph ^ 1u);
         if (!__all_sync(0xffffffffu, got)) {
           ok = false;
@@ -502,9 +534,15 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
         asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(w[0]), "r"(w[1]),
                      "r"(w[2]), "r"(w[3])
                      : "memory");
-        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(at + 4),
-                     "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]), "r"(w[9]), "r"(w[10]), "r"(w[11])
-                     : "memory");
+        if constexpr (BN <= 32)
+          asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};\n" ::"r"(at + 4), "r"(w[4]) : "memory");
+        else if constexpr (BN <= 64)
+          asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};\n" ::"r"(at + 4), "r"(w[4]), "r"(w[5])
+                       : "memory");
+        else
+          asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(at + 4),
+                       "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]), "r"(w[9]), "r"(w[10]), "r"(w[11])
+                       : "memory");
         asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
         tc_fence_before();
         __syncwarp();

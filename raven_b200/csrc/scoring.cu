@@ -41,15 +41,23 @@ uint64_t type_size(int32_t t) {
 }
 bool aligned(const void* p, uint64_t a) { return (uintptr_t)p % a == 0; }
 
-// SMs of the current device.
+// SMs of the current device. On a device's first call its default memory pool
+// is told to keep freed scratch (as raven_index_upload does): a pool that gives
+// it back at every synchronisation makes the next call wait for an allocation.
 int sm_count(int* out) {
   static std::mutex mu;
   static int count[256] = {};
   int dev = 0;
   CU(cudaGetDevice(&dev));
-  std::lock_guard<std::mutex> lk(mu);
   if (dev < 0 || dev >= 256) return fail(RAVEN_EINVAL, "device ordinal out of range");
-  if (!count[dev]) CU(cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev));
+  std::lock_guard<std::mutex> lk(mu);
+  if (!count[dev]) {
+    CU(cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev));
+    cudaMemPool_t pool;
+    uint64_t keep = ~0ull;
+    if (cudaDeviceGetDefaultMemPool(&pool, dev) == cudaSuccess)
+      cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
+  }
   *out = count[dev];
   return RAVEN_OK;
 }
