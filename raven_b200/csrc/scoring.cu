@@ -527,21 +527,20 @@ int raven_topk_rows_device(const void* d_scores, int32_t type, uint64_t nq, uint
   p.starts = d_row_starts;
   p.total = n;
   p.k = k;
-  p.largest = largest != 0;
+  p.mul = largest ? 1u : ~0u;
+  p.add = largest ? 0x7fffffu : 0x7ffffeu;
   p.type = type == RAVEN_TYPE_F32 ? 0 : type == RAVEN_TYPE_F16 ? 1 : 2;
   p.vals = d_vals;
   p.ids = d_ids;
   p.counts = d_counts;
-  // A warp takes rows of up to 1024 scores (1024 rows of one wave's teams fill
-  // the GPU), a CTA longer ones; where rows are too few to fill the GPU twice
-  // over, each is split into parts of at least two tiles. Ragged rows go by
-  // their mean.
+  // A warp takes rows of up to 1024 scores, a CTA longer ones; where rows are
+  // too few to fill the GPU, each is split into parts of at least a tile.
+  // Ragged rows go by their mean.
   const uint64_t len = d_row_starts ? (n + nq - 1) / nq : n;
   const bool warp = len <= 1024;
-  uint64_t parts = 1;
   const uint64_t tile = raven_topk::kCtaThreads * 16ull;
-  if (!warp && nq < 4ull * sms) parts = std::max<uint64_t>(1, std::min<uint64_t>(8ull * sms / nq, len / (2 * tile)));
-  parts = std::min<uint64_t>(parts, 2ull * sms);
+  uint64_t parts = 1;
+  if (!warp && nq < 4ull * sms) parts = std::max<uint64_t>(1, std::min<uint64_t>((4ull * sms + nq - 1) / nq, len / tile));
   p.parts = (uint32_t)parts;
   uint64_t* tmp = nullptr;
   if (parts > 1) {

@@ -5,17 +5,18 @@
 // or smallest first); with the complement of its index below it, 64 bits order
 // the row totally, so the answer does not depend on how the row is split. A
 // team of threads (a warp for short rows, a CTA for long ones) streams its
-// part of a row once, a tile at a time in registers, and keeps the elements
-// above a threshold in shared memory:
-//   * first tile: the k-th best of the threads' own maxima is a bound that at
-//     least k elements reach, so about k elements are kept instead of all;
-//   * then: the k-th best kept so far; a later element must beat it, since an
-//     equal one has a higher index.
-// The kept ones are ranked when the tile that set them is done, when they fill
-// the buffer, and at the end. A tile whose survivors do not fit (rising data,
-// equal scores) is taken again slice by slice, ranked in between: slower, with
-// the same result. Few long rows are split into parts over the GPU; the parts'
-// lists are joined by the same code.
+// part of a row once, a tile of 16 elements per thread at a time in registers,
+// and keeps the elements above a bound in shared memory:
+//   * first tile: the k-th best of the threads' own maxima is reached by at
+//     least k elements, so little more than k of the tile are kept;
+//   * when many are kept, the k-th best of them is the new bound. A later
+//     element must beat it, since an equal one has a higher index.
+// Both k-th bests are found by one warp with the values in registers, a bit of
+// the key at a time from the highest one in which they differ. At the end the
+// few left over are ordered by counting. A tile whose survivors do not fit
+// (rising data, equal scores) is taken again slice by slice, pruned in between:
+// slower, with the same result. Few long rows are split into parts over the
+// GPU; the parts' lists are joined by the same code.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -38,7 +39,7 @@ struct Params {
   uint64_t total;             // ragged: scores in x
   uint32_t k;
   uint32_t parts;             // teams per row
-  int largest;
+  uint32_t mul, add;          // of the keys: 1, 0x7fffff, or for the smallest first -1, 0x7ffffe
   int type;                   // of the values written (lists need it too)
   uint64_t* lists;            // parts > 1: [nq][parts][k] entries, zero where there is none
   void* vals;
@@ -46,15 +47,19 @@ struct Params {
   uint32_t* counts;           // or null
 };
 
-// NaN is 1, below every number; 0 is no element.
-__device__ inline uint32_t key_of(float x, int largest) {
+// Keys: 0xffffffff for the best infinity down to kWorst for the worst one; NaN
+// (canonical after the addition) below it, and 0 for no element. With `up` the
+// usual order-preserving image of the bits, the key is up + 0x7fffff, or
+// ~up + 0x7fffff for the smallest first: one multiply-add.
+constexpr uint32_t kWorst = 0x00fffffeu;
+__device__ inline uint32_t key_of(float x, uint32_t mul, uint32_t add) {
   const uint32_t b = __float_as_uint(x + 0.0f);  // -0 counts as 0
-  const uint32_t up = (b & 0x80000000u) ? ~b : b | 0x80000000u;
-  return x != x ? 1u : largest ? up : ~up;
+  const uint32_t up = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  return up * mul + add;
 }
-__device__ inline float value_of(uint32_t key, int largest) {
-  const uint32_t up = largest ? key : ~key;
-  return key == 1u ? __int_as_float(0x7fc00000) : __uint_as_float((up & 0x80000000u) ? up & 0x7fffffffu : ~up);
+__device__ inline float value_of(uint32_t key, uint32_t mul, uint32_t add) {
+  const uint32_t up = (key - add) * mul;  // mul is 1 or -1: its own inverse
+  return key < kWorst ? __int_as_float(0x7fc00000) : __uint_as_float((up & 0x80000000u) ? up & 0x7fffffffu : ~up);
 }
 
 template <int TEAM>
@@ -71,7 +76,7 @@ struct Team {
 template <int TEAM>
 struct Shared {
   uint64_t buf[Team<TEAM>::kBuf];
-  uint32_t max[TEAM];
+  uint32_t top[TEAM];
   uint32_t count;
   uint32_t bound;
 };
@@ -93,67 +98,132 @@ struct Loader {
   }
 };
 
+// By one warp, N values per lane (0: none): the largest T that at least k of
+// them reach, 0 if fewer than k are there. `slack`: a T that is reached by up to
+// k + slack will do.
+template <int N>
+__device__ inline uint32_t kth_of_warp(const uint32_t (&v)[N], uint32_t k, uint32_t slack) {
+  uint32_t hi = 0, lo = 0xffffffffu;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    hi = max(hi, v[i]);
+    lo = min(lo, v[i]);
+  }
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  if (hi == lo) return hi;
+  int bit = 31 - __clz(hi ^ lo);
+  uint32_t t = bit < 31 ? hi & ~((2u << bit) - 1u) : 0u;
+  for (; bit >= 0; --bit) {
+    const uint32_t next = t | (1u << bit);
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) c += v[i] >= next;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (c >= k) {
+      t = next;
+      if (c <= k + slack) break;
+    }
+  }
+  return t;
+}
+
 template <int TEAM>
 struct Keeper {
   using TM = Team<TEAM>;
-  static constexpr uint32_t kRank = TEAM == 32 ? 128 : 384;  // up to here ranks are counted, above sorted
+  static constexpr uint32_t kPrune = 1024;  // entries that one warp prunes
+  static constexpr uint32_t kFew = 128;     // rows up to here need no bound
+  static_assert(kPrune <= (uint32_t)TM::kBuf && 2 * kMaxK <= kPrune / 2, "sizes");
   Shared<TEAM>& s;
   uint32_t tid, k;
   uint32_t above = 0;   // only keys over it can matter
   uint32_t held = 0;    // entries in the buffer (= s.count between calls)
-  bool ranked = true;   // they are the best so far in order, at most k
-  bool few;             // no more elements than are ranked by counting: no bound is needed
+  bool few;
 
-  __device__ Keeper(Shared<TEAM>& s_, uint32_t tid_, uint32_t k_, uint64_t n) : s(s_), tid(tid_), k(k_), few(n <= kRank) {
+  __device__ Keeper(Shared<TEAM>& s_, uint32_t tid_, uint32_t k_, uint64_t n) : s(s_), tid(tid_), k(k_), few(n <= kFew) {
     if (tid == 0) s.count = 0;
     TM::sync();
   }
 
-  // The buffer's best k, in order, at its front. Entry and exit are synchronised.
-  __device__ void rank() {
-    const uint32_t c = held;
-    if (c <= kRank) {
-      constexpr int kOwn = (kRank + TEAM - 1) / TEAM;
-      uint64_t own[kOwn];
-      uint32_t at[kOwn];
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) {
-        const uint32_t e = tid + i * TEAM;
-        own[i] = e < c ? s.buf[e] : 0;
-        at[i] = 0;
-      }
-      for (uint32_t j = 0; j < c; ++j) {
-        const uint64_t o = s.buf[j];
-#pragma unroll
-        for (int i = 0; i < kOwn; ++i) at[i] += o > own[i];
-      }
-      TM::sync();
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i)
-        if (tid + i * TEAM < c && at[i] < k) s.buf[at[i]] = own[i];
-    } else {
-      uint32_t p2 = 2 * TEAM;
-      while (p2 < c) p2 <<= 1;
-      for (uint32_t i = c + tid; i < p2; i += TEAM) s.buf[i] = 0;
-      TM::sync();
-      for (uint32_t w = 2; w <= p2; w <<= 1)
-        for (uint32_t h = w >> 1; h > 0; h >>= 1) {
-          for (uint32_t i = tid; i < p2 / 2; i += TEAM) {
-            const uint32_t a = 2 * i - (i & (h - 1)), b = a + h;
-            const uint64_t x = s.buf[a], y = s.buf[b];
-            if ((x < y) == ((a & w) == 0)) {
-              s.buf[a] = y;
-              s.buf[b] = x;
-            }
-          }
-          TM::sync();
-        }
+  // Drops entries below the k-th key. Entry and exit are synchronised.
+  __device__ void prune() {
+    if (held > kPrune) {
+      sort();
+      return;
     }
+    if (tid < 32) {
+      uint32_t t;
+      if (held <= kPrune / 4)
+        t = kth_of_held<kPrune / 128>();
+      else
+        t = kth_of_held<kPrune / 32>();
+      if (tid == 0) s.bound = t;
+    }
+    // in place: entries are moved towards the front a round of the team at a
+    // time, and a round's reads come before its writes
+    const uint32_t c = held;
+    if (tid == 0) s.count = 0;
+    TM::sync();
+    const uint32_t t = s.bound;
+    for (uint32_t i = 0; i < c; i += TEAM) {
+      const uint64_t e = i + tid < c ? s.buf[i + tid] : 0;
+      TM::sync();
+      if (e && (uint32_t)(e >> 32) >= t) s.buf[atomicAdd(&s.count, 1u)] = e;
+      TM::sync();
+    }
+    held = s.count;
+    TM::sync();
+    if (held >= k) above = max(above, t);
+    if (held > kPrune / 2) sort();  // many equals
+  }
+  template <int N>
+  __device__ uint32_t kth_of_held() const {
+    uint32_t v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = tid + 32 * i < held ? (uint32_t)(s.buf[tid + 32 * i] >> 32) : 0u;
+    return kth_of_warp(v, k, 0);
+  }
+
+  // The best k in order at the front, by sorting all.
+  __device__ void sort() {
+    const uint32_t c = held;
+    uint32_t p2 = 2 * TEAM;
+    while (p2 < c) p2 <<= 1;
+    for (uint32_t i = c + tid; i < p2; i += TEAM) s.buf[i] = 0;
+    TM::sync();
+    for (uint32_t w = 2; w <= p2; w <<= 1)
+      for (uint32_t h = w >> 1; h > 0; h >>= 1) {
+        for (uint32_t i = tid; i < p2 / 2; i += TEAM) {
+          const uint32_t a = 2 * i - (i & (h - 1)), b = a + h;
+          const uint64_t x = s.buf[a], y = s.buf[b];
+          if ((x < y) == ((a & w) == 0)) {
+            s.buf[a] = y;
+            s.buf[b] = x;
+          }
+        }
+        TM::sync();
+      }
     held = min(c, k);
-    ranked = true;
     if (tid == 0) s.count = held;
     TM::sync();
     if (c >= k) above = max(above, (uint32_t)(s.buf[k - 1] >> 32));
+  }
+
+  // The best k in order, at s.buf + the value returned.
+  __device__ uint32_t finish() {
+    if (held > k + 32) prune();
+    if (held > kPrune / 2) sort();
+    const uint32_t c = held;  // at most kPrune / 2: the other half takes the ordered ones
+    for (uint32_t e = tid; e < c; e += TEAM) {
+      const uint64_t own = s.buf[e];
+      uint32_t at = 0;
+#pragma unroll 4
+      for (uint32_t j = 0; j < c; ++j) at += s.buf[j] > own;
+      if (at < k) s.buf[kPrune / 2 + at] = own;
+    }
+    held = min(c, k);
+    TM::sync();
+    return kPrune / 2;
   }
 
   // Takes a tile: key[e] (0: none) with index idx(e). Indexes of a later tile
@@ -161,28 +231,29 @@ struct Keeper {
   template <int E, typename Idx>
   __device__ void take(const uint32_t (&key)[E], bool more, Idx idx) {
     const uint32_t old = held;
-    if (above == 0 && !few) bound(key);
-    if (!push(key, idx)) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) top = max(top, key[e]);
+    if (above == 0 && !few) bound(top);
+    if (!push(key, top, idx)) {
       undo(old);
-      bound(key);  // now from this tile
-      if (!push(key, idx)) {
+      bound(top);  // now from this tile
+      if (!push(key, top, idx)) {
         undo(old);
-        rank();
         slices(key, idx);
         return;
       }
     }
-    // when the first tile's survivors are ranked, the k-th is the threshold
-    if (more && held >= k && (old < k || held > (uint32_t)TM::kBuf / 2)) rank();
+    if (more && held > kPrune / 2) prune();
   }
 
   // Appends the keys over `above`; false if they do not fit. Exit is synchronised.
   template <int E, typename Idx>
-  __device__ bool push(const uint32_t (&key)[E], Idx idx) {
-    uint32_t mine = 0;
+  __device__ bool push(const uint32_t (&key)[E], uint32_t top, Idx idx) {
+    if (top > above) {
+      uint32_t mine = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) mine += key[e] > above;
-    if (mine) {
+      for (int e = 0; e < E; ++e) mine += key[e] > above;
       uint32_t p = atomicAdd(&s.count, mine);
       if (p + mine <= (uint32_t)TM::kBuf) {
 #pragma unroll
@@ -191,11 +262,9 @@ struct Keeper {
       }
     }
     TM::sync();
-    const uint32_t c = s.count;
+    held = s.count;
     TM::sync();  // read by all before the next append
-    ranked &= c == held;
-    held = c;
-    return c <= (uint32_t)TM::kBuf;
+    return held <= (uint32_t)TM::kBuf;
   }
   __device__ void undo(uint32_t old) {
     held = old;
@@ -203,7 +272,7 @@ struct Keeper {
     TM::sync();
   }
 
-  // The tile one element a thread at a time, ranked in between. Slices are not
+  // The tile one element a thread at a time, pruned in between. Slices are not
   // in the order of their indexes, so an equal of the k-th is kept until the end.
   template <int E, typename Idx>
   __device__ void slices(const uint32_t (&key)[E], Idx idx) {
@@ -212,7 +281,7 @@ struct Keeper {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       if (held + TEAM > (uint32_t)TM::kBuf) {
-        rank();
+        sort();
         lower = max(was, above - 1);
       }
       if (key[e] > lower) {
@@ -223,51 +292,47 @@ struct Keeper {
       held = s.count;
       TM::sync();
     }
-    rank();
+    if (held > k) sort();
   }
 
-  // A bound from the tile's own maxima: the k-th best of G of them is reached
-  // by at least k elements, so lower keys are out.
-  template <int E>
-  __device__ void bound(const uint32_t (&key)[E]) {
-    uint32_t g = 32;  // maxima: twice k, as far as there are threads
-    while (g < 2 * k && g < (uint32_t)TEAM) g <<= 1;
-    if (g < k) return;
-    uint32_t m = 0;
+  // A bound from the threads' maxima of a tile: k of them, so k elements, reach
+  // the k-th best of them.
+  __device__ void bound(uint32_t top) {
+    if (k > (uint32_t)TEAM) return;
+    uint32_t t;
+    if constexpr (TEAM == 32) {
+      const uint32_t v[1] = {top};
+      t = kth_of_warp(v, k, k / 4);
+    } else {
+      s.top[tid] = top;
+      TM::sync();
+      if (tid < 32) {
+        uint32_t v[TEAM / 32];
 #pragma unroll
-    for (int e = 0; e < E; ++e) m = max(m, key[e]);
-    for (uint32_t o = 1; o < (uint32_t)TEAM / g; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const uint32_t per = (uint32_t)TEAM / g;  // threads per maximum (at most 8: one warp's lanes)
-    if (tid % per == 0) s.max[tid / per] = m;
-    TM::sync();
-    if (tid < g) {
-      const uint32_t mine = s.max[tid];
-      uint32_t at = 0;
-      for (uint32_t j = 0; j < g; ++j) {
-        const uint32_t o = s.max[j];
-        at += o > mine || (o == mine && j < tid);
+        for (int i = 0; i < TEAM / 32; ++i) v[i] = s.top[tid + 32 * i];
+        t = kth_of_warp(v, k, k / 4);
+        if (tid == 0) s.bound = t;
       }
-      if (at == k - 1) s.bound = mine;
+      TM::sync();
+      t = s.bound;
+      TM::sync();
     }
-    TM::sync();
-    const uint32_t b = s.bound;
-    if (b > 1) above = max(above, b - 1);
-    TM::sync();
+    if (t > 1) above = max(above, t - 1);
   }
 };
 
 template <int TEAM>
 __device__ inline void write_out(const Params& p, Keeper<TEAM>& kp, uint64_t row, uint32_t part, uint32_t parts) {
-  if (!kp.ranked) kp.rank();
+  const uint64_t* best = kp.s.buf + kp.finish();
   const uint32_t c = kp.held;
   if (parts > 1) {
     uint64_t* o = p.lists + (row * parts + part) * p.k;
-    for (uint32_t i = kp.tid; i < p.k; i += TEAM) o[i] = i < c ? kp.s.buf[i] : 0;
+    for (uint32_t i = kp.tid; i < p.k; i += TEAM) o[i] = i < c ? best[i] : 0;
     return;
   }
   for (uint32_t i = kp.tid; i < p.k; i += TEAM) {
-    const uint64_t e = i < c ? kp.s.buf[i] : 0;
-    const float v = i < c ? value_of((uint32_t)(e >> 32), p.largest) : 0.0f;
+    const uint64_t e = i < c ? best[i] : 0;
+    const float v = i < c ? value_of((uint32_t)(e >> 32), p.mul, p.add) : 0.0f;
     const uint64_t at = row * p.k + i;
     if (p.type == 0)
       ((float*)p.vals)[at] = v;
@@ -296,33 +361,39 @@ __global__ void __launch_bounds__(kCtaThreads) topk_kernel(const Params p) {
     const uint64_t hi = b < 0 ? 0 : min((uint64_t)b, p.total);
     len = hi > lo ? min(hi - lo, (uint64_t)0xffffffffu) : 0;
   }
-  // this part's elements: [from, to) of the row
-  const uint64_t each = (len + p.parts - 1) / p.parts;
+  // this part's elements: [from, to) of the row. Parts are whole tiles less 16
+  // bytes, for a row that starts between 16-byte boundaries
+  using L = Loader<T>;
+  constexpr uint32_t kTile = TEAM * L::kE;
+  uint64_t each = len;
+  if (p.parts > 1) each = ((len + p.parts - 1) / p.parts + kTile + L::kPer - 1) / kTile * kTile - L::kPer;
   const uint64_t from = min(len, each * part), to = min(len, from + each);
   Keeper<TEAM> kp(*sh, tid, p.k, to - from);
-  using L = Loader<T>;
   // pieces of 16 bytes from the boundary at or before the first element: the
   // bytes around a row are in the same 16 as some of its own
   const uint8_t* base = (const uint8_t*)p.x + (lo + from) * sizeof(T);
   const uint32_t skip = (uint32_t)(((uintptr_t)base & 15) / sizeof(T));
-  const uint4* w = (const uint4*)((uintptr_t)base & ~(uintptr_t)15);
-  const uint64_t end = skip + (to - from);  // in elements from w
-  constexpr uint64_t kTile = (uint64_t)TEAM * L::kE;
-  for (uint64_t t = 0; to > from && t < end; t += kTile) {
-    uint4 v[L::kPieces];
-#pragma unroll
-    for (int i = 0; i < L::kPieces; ++i) {
-      const uint64_t e = t + (uint64_t)(i * TEAM + tid) * L::kPer;
-      v[i] = e < end ? __ldg(w + e / L::kPer) : make_uint4(0, 0, 0, 0);
-    }
+  const uint4* w = (const uint4*)((uintptr_t)base & ~(uintptr_t)15) + tid;
+  const uint64_t end = to > from ? skip + (to - from) : 0;  // in elements from the boundary
+  for (uint64_t t = 0; t < end; t += kTile, w += TEAM * L::kPieces) {
     uint32_t key[L::kE];
+    if ((t || !skip) && t + kTile <= end) {
+      uint4 v[L::kPieces];
 #pragma unroll
-    for (int i = 0; i < L::kPieces; ++i)
+      for (int i = 0; i < L::kPieces; ++i) v[i] = __ldg(w + i * TEAM);
 #pragma unroll
-      for (int c = 0; c < L::kPer; ++c) {
-        const uint64_t e = t + (uint64_t)(i * TEAM + tid) * L::kPer + c;
-        key[i * L::kPer + c] = e >= skip && e < end ? key_of(L::get(v[i], c), p.largest) : 0u;
+      for (int e = 0; e < L::kE; ++e) key[e] = key_of(L::get(v[e / L::kPer], e % L::kPer), p.mul, p.add);
+    } else {
+      const uint32_t lo_ = t ? 0 : skip, hi_ = (uint32_t)min(end - t, (uint64_t)kTile);
+#pragma unroll
+      for (int i = 0; i < L::kPieces; ++i) {
+        const uint32_t e0 = (i * TEAM + tid) * L::kPer;
+        const uint4 v = e0 < hi_ ? __ldg(w + i * TEAM) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < L::kPer; ++c)
+          key[i * L::kPer + c] = e0 + c >= lo_ && e0 + c < hi_ ? key_of(L::get(v, c), p.mul, p.add) : 0u;
       }
+    }
     const uint32_t i0 = (uint32_t)(from - skip + t) + tid * L::kPer;  // wraps where the element does not exist
     kp.take(key, t + kTile < end,
             [&](int e) { return i0 + (uint32_t)((e / L::kPer) * TEAM * L::kPer + e % L::kPer); });
