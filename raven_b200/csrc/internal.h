@@ -21,3 +21,14 @@ int fp8_encode_lane_major(const float* d_rows, uint64_t n, uint32_t dim, uint8_t
                           uint8_t* d_exps, uint64_t ld_exps, cudaStream_t st);
 
 }  // namespace raven_internal
+
+#ifdef __CUDACC__
+namespace raven_score {
+// Start of a kernel's memory accesses: the kernel before it in the stream is
+// done and its writes are seen; the kernel after it may be set up.
+__device__ inline void after_previous() {
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+}
+}  // namespace raven_score
+#endif

@@ -37,6 +37,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "internal.h"
 #include "knn_tc.cuh"
 
 namespace raven_score {
@@ -323,6 +324,7 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
+  after_previous();
 
   if (warp == 0) {
     if (lane == 0) {  // TMA

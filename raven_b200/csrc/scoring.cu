@@ -7,6 +7,7 @@
 #include <nvtx3/nvToolsExt.h>
 
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 
 #include "../../include/raven_gpu.h"
@@ -16,6 +17,8 @@
 
 using raven_internal::encode_tiled;
 using raven_internal::fail;
+
+using raven_score::after_previous;
 
 namespace {
 
@@ -62,6 +65,43 @@ int sm_count(int* out) {
   return RAVEN_OK;
 }
 
+// Launches `kern` so that it may start while the kernel before it in the stream
+// ends. Every kernel here waits for that one (after_previous) before it touches
+// memory, and lets its own successor start at once. `allowed`: devices (bits)
+// on which the kernel may already use `smem` bytes; the attribute is set again
+// when a launch is refused (a context replaced since).
+struct Allowed {
+  std::atomic<uint64_t> mask{0};
+};
+template <typename... K, typename... A>
+cudaError_t launch(void (*kern)(K...), uint64_t grid, int threads, uint32_t smem, Allowed& allowed, cudaStream_t st,
+                   A&&... args) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3((unsigned)grid);
+  c.blockDim = dim3((unsigned)threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &at;
+  c.numAttrs = 1;
+  for (int turn = 0;; ++turn) {
+    if (smem > 48 * 1024 && (turn || dev >= 64 || !(allowed.mask.load(std::memory_order_relaxed) & bit))) {
+      e = cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      if (e != cudaSuccess) return e;
+      allowed.mask.fetch_or(bit, std::memory_order_relaxed);
+    }
+    e = cudaLaunchKernelEx(&c, kern, args...);
+    if (e != cudaErrorInvalidValue || turn || smem <= 48 * 1024) return e;
+    (void)cudaGetLastError();
+  }
+}
+
 // ---------------------------------------------------------------------------
 // FP8 rows. Block b of a row: e = the least exponent with max|x| <= 448 * 2^e
 // over its finite values (0 when they are all zero, at least -127), code =
@@ -94,6 +134,7 @@ template <typename T, bool VEC, bool LANE>
 __global__ void __launch_bounds__(256) fp8_encode_kernel(const T* __restrict__ in, uint64_t n, uint32_t dim, uint64_t ld,
                                                          uint8_t* __restrict__ codes, uint64_t ld_codes,
                                                          uint8_t* __restrict__ exps, uint64_t ld_exps) {
+  after_previous();
   const int lane = threadIdx.x & 31;
   const uint32_t nb = (dim + kBlock - 1) / kBlock, nb4 = (nb + 3) / 4 * 4, dim16 = (dim + 15) / 16 * 16;
   const uint64_t units = n * nb;
@@ -141,6 +182,7 @@ __global__ void __launch_bounds__(256) fp8_encode_kernel(const T* __restrict__ i
 __global__ void __launch_bounds__(256) fp8_decode_kernel(const uint8_t* __restrict__ codes, uint64_t ld_codes,
                                                          const uint8_t* __restrict__ exps, uint64_t ld_exps, uint64_t n,
                                                          uint32_t dim, float* __restrict__ out, uint64_t ld) {
+  after_previous();
   const uint64_t total = n * dim;
   for (uint64_t t = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; t < total; t += (uint64_t)gridDim.x * blockDim.x) {
     const uint64_t row = t / dim;
@@ -156,11 +198,9 @@ cudaError_t launch_encode(const void* x, uint64_t n, uint32_t dim, uint64_t ld, 
   const uint64_t units = n * ((dim + kBlock - 1) / kBlock);
   const unsigned grid = (unsigned)std::min<uint64_t>((units + 7) / 8, (uint64_t)sms * 16);
   const bool vec = !LANE && ld % 4 == 0 && aligned(x, 4 * sizeof(T));
-  if (vec)
-    fp8_encode_kernel<T, true, LANE><<<grid, 256, 0, st>>>((const T*)x, n, dim, ld, codes, ld_codes, exps, ld_exps);
-  else
-    fp8_encode_kernel<T, false, LANE><<<grid, 256, 0, st>>>((const T*)x, n, dim, ld, codes, ld_codes, exps, ld_exps);
-  return cudaGetLastError();
+  static Allowed none;
+  return launch(vec ? fp8_encode_kernel<T, true, LANE> : fp8_encode_kernel<T, false, LANE>, grid, 256, 0, none, st,
+                (const T*)x, n, dim, ld, codes, ld_codes, exps, ld_exps);
 }
 
 int encode_rows(const void* x, int32_t type, uint64_t n, uint32_t dim, uint64_t ld, uint8_t* codes, uint64_t ld_codes,
@@ -214,11 +254,8 @@ template <bool FP8, int BN>
 cudaError_t launch_score(const CUtensorMap& q, const CUtensorMap& v, const raven_score::Params& p, unsigned grid,
                          cudaStream_t st) {
   using L = raven_score::Layout<FP8, BN>;
-  auto kern = raven_score::score_kernel<FP8, BN>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes);
-  if (e != cudaSuccess) return e;
-  kern<<<grid, L::kThreads, L::kBytes, st>>>(q, v, p);
-  return cudaGetLastError();
+  static Allowed allowed;
+  return launch(raven_score::score_kernel<FP8, BN>, grid, L::kThreads, L::kBytes, allowed, st, q, v, p);
 }
 
 template <bool FP8>
@@ -339,6 +376,7 @@ int run_scores(const raven_rows* q, const int64_t* qo, const raven_rows* v, cons
 __global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* __restrict__ qo, const int64_t* __restrict__ vo,
                                                          uint32_t groups, uint64_t nq, uint64_t n,
                                                          int64_t* __restrict__ starts, int* status) {
+  after_previous();
   __shared__ int64_t part[256];
   __shared__ int64_t gq[256], gm[256], gn[256];
   const uint32_t g0 = blockIdx.x * 256u, tid = threadIdx.x;
@@ -402,13 +440,11 @@ __global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* __restri
 template <typename T, int TEAM>
 cudaError_t launch_topk(const raven_topk::Params& p, cudaStream_t st) {
   using TM = raven_topk::Team<TEAM>;
-  auto kern = raven_topk::topk_kernel<T, TEAM>;
-  const int smem = TM::kTeams * (int)sizeof(raven_topk::Shared<TEAM>);
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
+  const uint32_t smem = TM::kTeams * (uint32_t)sizeof(raven_topk::Shared<TEAM>);
   const uint64_t units = p.nq * p.parts;
-  kern<<<(unsigned)((units + TM::kTeams - 1) / TM::kTeams), raven_topk::kCtaThreads, smem, st>>>(p);
-  return cudaGetLastError();
+  static Allowed allowed;
+  return launch(raven_topk::topk_kernel<T, TEAM>, (units + TM::kTeams - 1) / TM::kTeams, raven_topk::kCtaThreads, smem,
+                allowed, st, p);
 }
 template <int TEAM>
 cudaError_t dispatch_topk(int32_t type, const raven_topk::Params& p, cudaStream_t st) {
@@ -461,8 +497,9 @@ int raven_fp8_decode_device(const uint8_t* d_codes, uint64_t ld_codes, const uin
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   const unsigned grid = (unsigned)std::min<uint64_t>((n * dim + 255) / 256, (uint64_t)sms * 16);
-  fp8_decode_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(d_codes, ld_codes, d_exps, ld_exps, n, dim, d_out, ld);
-  CU(cudaGetLastError());
+  static Allowed none;
+  CU(launch(fp8_decode_kernel, grid, 256, 0, none, (cudaStream_t)stream, d_codes, ld_codes, d_exps, ld_exps, n, dim,
+            d_out, ld));
   return RAVEN_OK;
 }
 
@@ -493,9 +530,9 @@ int raven_group_rows_device(const int64_t* d_q_offsets, const int64_t* d_v_offse
   if (!d_q_offsets || !d_v_offsets || !d_row_starts) return fail(RAVEN_EINVAL, "null argument");
   if (!aligned(d_q_offsets, 8) || !aligned(d_v_offsets, 8) || !aligned(d_row_starts, 8))
     return fail(RAVEN_EINVAL, "offsets and row starts: not aligned to 64 bits");
-  group_rows_kernel<<<(groups + 255) / 256, 256, 0, (cudaStream_t)stream>>>(d_q_offsets, d_v_offsets, groups, nq, n,
-                                                                            d_row_starts, d_status);
-  CU(cudaGetLastError());
+  static Allowed none;
+  CU(launch(group_rows_kernel, (groups + 255) / 256, 256, 0, none, (cudaStream_t)stream, d_q_offsets, d_v_offsets,
+            groups, nq, n, d_row_starts, d_status));
   return RAVEN_OK;
 }
 
@@ -553,9 +590,9 @@ int raven_topk_rows_device(const void* d_scores, int32_t type, uint64_t nq, uint
     j.x = tmp;
     j.n = parts * k;
     j.parts = 1;
-    raven_topk::topk_join_kernel<<<(unsigned)nq, raven_topk::kCtaThreads,
-                                   sizeof(raven_topk::Shared<raven_topk::kCtaThreads>), st>>>(j);
-    e = cudaGetLastError();
+    static Allowed none;
+    e = launch(raven_topk::topk_join_kernel, nq, raven_topk::kCtaThreads,
+               (uint32_t)sizeof(raven_topk::Shared<raven_topk::kCtaThreads>), none, st, j);
   }
   if (tmp) cudaFreeAsync(tmp, st);
   if (e != cudaSuccess) return fail(RAVEN_ECUDA, std::string("topk: ") + cudaGetErrorString(e));

@@ -25,6 +25,8 @@
 
 #include <cstdint>
 
+#include "internal.h"
+
 namespace raven_topk {
 
 constexpr uint32_t kMaxK = 256;
@@ -348,6 +350,7 @@ __device__ inline void write_out(const Params& p, Keeper<TEAM>& kp, uint64_t row
 template <typename T, int TEAM>
 __global__ void __launch_bounds__(kCtaThreads) topk_kernel(const Params p) {
   extern __shared__ __align__(16) uint8_t raw[];
+  raven_score::after_previous();
   Shared<TEAM>* sh = (Shared<TEAM>*)raw + threadIdx.x / TEAM;
   const uint32_t tid = threadIdx.x % TEAM;
   const uint64_t unit = (uint64_t)blockIdx.x * Team<TEAM>::kTeams + threadIdx.x / TEAM;
@@ -405,6 +408,7 @@ __global__ void __launch_bounds__(kCtaThreads) topk_kernel(const Params p) {
 __global__ void __launch_bounds__(kCtaThreads) topk_join_kernel(const Params p) {
   constexpr int TEAM = kCtaThreads, E = 8;
   extern __shared__ __align__(16) uint8_t raw[];
+  raven_score::after_previous();
   const uint64_t row = blockIdx.x;
   Keeper<TEAM> kp(*(Shared<TEAM>*)raw, threadIdx.x, p.k, p.n);
   const uint64_t* x = (const uint64_t*)p.x + row * p.n;

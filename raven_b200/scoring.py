@@ -32,46 +32,53 @@ def _up(x: int, m: int) -> int:
     return -(-x // m) * m
 
 
-def _matrix(x, name: str) -> torch.Tensor:
+def _matrix(x, name: str) -> int:
+    """The row pitch of a matrix on a GPU with each row's values side by side."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise ValueError(f"{name} must be a 2-D tensor")
     if not x.is_cuda:
         raise ValueError(f"{name} must be on a GPU")
     if x.dtype not in _TYPES:
         raise ValueError(f"{name} must be float32, float16 or bfloat16, not {x.dtype}")
-    if x.shape[1] == 0:
+    (n, dim), (pitch, step) = x.shape, x.stride()
+    if dim == 0:
         raise ValueError(f"{name} has rows of no values")
     # one row, or rows of one value, may come with any strides
-    if (x.stride(1) != 1 and x.shape[1] > 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+    if (step != 1 and dim > 1) or (pitch < dim and n > 1):
         raise ValueError(f"{name} must hold each row's values side by side and its rows one after another")
-    return x
+    return pitch if n > 1 else max(pitch, dim)
 
 
 def _pitch(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
 
 
-def _on(device: torch.device, *tensors) -> None:
+def _on(device: int, *tensors) -> None:
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"all tensors must be on {device}, got one on {t.device}")
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"all tensors must be on cuda:{device}, got one on {t.device}")
 
 
-def _call(device: torch.device, fn, *args) -> None:
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def _call(device: int, fn, *args) -> None:
     """The library call with `device` current, on its current stream."""
-    if torch.cuda.current_device() == device.index:
-        L.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    if torch.cuda.current_device() == device:
+        rc = fn(*args, _stream(device))
     else:
         with torch.cuda.device(device):
-            L.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+            rc = fn(*args, _stream(device))
+    if rc:
+        L.check(rc)
 
 
 def aligned_rows(x: torch.Tensor) -> torch.Tensor:
     """The rows of `x` as `scores` takes 16-bit rows: starting on 16 bytes, 16
     bytes times a whole number apart. A copy where `x` is not laid out so."""
-    _matrix(x, "rows")
-    step = 16 // x.element_size()
-    if x.data_ptr() % 16 == 0 and _pitch(x) % step == 0:
+    pitch, step = _matrix(x, "rows"), 16 // x.element_size()
+    if x.data_ptr() % 16 == 0 and pitch % step == 0:
         return x
     out = x.new_empty(x.shape[0], _up(x.shape[1], step))[:, : x.shape[1]]
     out.copy_(x)
@@ -84,19 +91,25 @@ class Fp8Rows:
     2^(exps - 127) of its block of 128."""
 
     def __init__(self, codes: torch.Tensor, exps: torch.Tensor, dim: int):
-        for name, t, most in (("codes", codes, _up(dim, 16)), ("exps", exps, _up(-(-dim // BLOCK), 4))):
-            if t.dtype != torch.uint8 or t.dim() != 2 or not t.is_cuda or t.stride(1) != 1:
-                raise ValueError(f"{name} must be a 2-D uint8 tensor on a GPU, each row's bytes side by side")
-            if t.shape[1] < most:
-                raise ValueError(f"{name} must have at least {most} columns for dim {dim}, got {t.shape[1]}")
         if dim < 1:
             raise ValueError("dim must be at least 1")
-        if codes.shape[0] != exps.shape[0] or codes.device != exps.device:
+        pitch = []
+        for name, t, least in (("codes", codes, _up(dim, 16)), ("exps", exps, _up(-(-dim // BLOCK), 4))):
+            if t.dtype != torch.uint8 or t.dim() != 2 or not t.is_cuda or t.stride(1) != 1:
+                raise ValueError(f"{name} must be a 2-D uint8 tensor on a GPU, each row's bytes side by side")
+            if t.shape[1] < least:
+                raise ValueError(f"{name} must have at least {least} columns for dim {dim}, got {t.shape[1]}")
+            pitch.append(_pitch(t))
+        n = codes.shape[0]
+        self.device_index = codes.get_device()
+        if exps.shape[0] != n or exps.get_device() != self.device_index:
             raise ValueError("codes and exps must have the same rows and device")
-        self.codes, self.exps, self.dim = codes, exps, int(dim)
-        self.device = codes.device
-        self._rows = L.Rows(codes.data_ptr(), exps.data_ptr(), codes.shape[0], _pitch(codes), _pitch(exps),
-                            L.RAVEN_TYPE_FP8)
+        self.codes, self.exps, self.dim = codes, exps, dim
+        self._rows = L.Rows(codes.data_ptr(), exps.data_ptr(), n, pitch[0], pitch[1], L.RAVEN_TYPE_FP8)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
 
     def __len__(self) -> int:
         return self.codes.shape[0]
@@ -115,32 +128,32 @@ class Fp8Rows:
         even. The scale of a block is the least power of two that brings its
         values to at most 448; infinities and NaN become NaN. `out`: rows to
         write instead of new ones (len(x) of them)."""
-        _matrix(x, "x")
-        n, dim = x.shape
+        pitch = _matrix(x, "x")
+        (n, dim), device = x.shape, x.get_device()
         if out is None:
             out = Fp8Rows.empty(n, dim, x.device)
         elif len(out) != n or out.dim != dim:
             raise ValueError(f"out holds {len(out)} rows of {out.dim}, expected {n} of {dim}")
-        _on(x.device, out.codes)
+        if out.device_index != device:
+            raise ValueError(f"out must be on cuda:{device}")
         r = out._rows
-        _call(x.device, L.load().raven_fp8_encode_device, x.data_ptr(), _TYPES[x.dtype], n, dim, _pitch(x), r.data, r.ld,
-              r.exps, r.ld_exps)
+        _call(device, L.load().raven_fp8_encode_device, x.data_ptr(), _TYPES[x.dtype], n, dim, pitch, r.data, r.ld, r.exps,
+              r.ld_exps)
         return out
 
     @staticmethod
     def of_index(index) -> "Fp8Rows":
         """FP8 rows of the vectors of a `DeviceIndex`, on its GPU."""
-        device = torch.device("cuda", index.device)
-        out = Fp8Rows.empty(index.n, index.dim, device)
+        out = Fp8Rows.empty(index.n, index.dim, torch.device("cuda", index.device))
         r = out._rows
-        _call(device, L.load().raven_index_fp8_device, index._h, r.data, r.ld, r.exps, r.ld_exps)
+        _call(index.device, L.load().raven_index_fp8_device, index._h, r.data, r.ld, r.exps, r.ld_exps)
         return out
 
     def decode(self) -> torch.Tensor:
         """The values, float32 [n, dim] (exact)."""
         out = torch.empty(len(self), self.dim, dtype=torch.float32, device=self.device)
         r = self._rows
-        _call(self.device, L.load().raven_fp8_decode_device, r.data, r.ld, r.exps, r.ld_exps, len(self), self.dim,
+        _call(self.device_index, L.load().raven_fp8_decode_device, r.data, r.ld, r.exps, r.ld_exps, len(self), self.dim,
               out.data_ptr(), self.dim)
         return out
 
@@ -155,44 +168,49 @@ Rows = Union[torch.Tensor, Fp8Rows]
 
 
 def _operands(queries: Rows, vectors: Rows, dtype: torch.dtype, bias: Optional[torch.Tensor]):
-    """(device, dim, queries, vectors) as the library takes them, with what must stay alive."""
-    keep = None
-    if isinstance(vectors, Fp8Rows):
-        device, dim, v, n = vectors.device, vectors.dim, vectors._rows, len(vectors)
+    """(device, dim, nq, n, queries, vectors) as the library takes them, and what must stay alive until the call."""
+    fp8 = isinstance(vectors, Fp8Rows)
+    if fp8:
+        device, dim, v = vectors.device_index, vectors.dim, vectors._rows
+        n = v.rows
     else:
-        _matrix(vectors, "vectors")
+        pitch = _matrix(vectors, "vectors")
         if vectors.dtype == torch.float32:
             raise ValueError("vectors must be Fp8Rows, float16 or bfloat16 (Fp8Rows.encode holds float32 rows as FP8)")
-        device, (n, dim) = vectors.device, vectors.shape
-        if vectors.data_ptr() % 16 or _pitch(vectors) % 8:
+        (n, dim), device, at = vectors.shape, vectors.get_device(), vectors.data_ptr()
+        if at % 16 or pitch % 8:
             raise ValueError("16-bit vectors must start on 16 bytes, a multiple of 8 values apart "
                              "(aligned_rows makes them so)")
-        v = L.Rows(vectors.data_ptr(), None, n, _pitch(vectors), 0, _TYPES[vectors.dtype])
+        v = L.Rows(at, None, n, pitch, 0, _TYPES[vectors.dtype])
     if isinstance(queries, Fp8Rows):
-        if not isinstance(vectors, Fp8Rows):
+        if not fp8:
             raise ValueError("FP8 queries need FP8 vectors")
-        qdim, nq, q, qdev = queries.dim, len(queries), queries._rows, queries.device
+        qdim, q, qdevice = queries.dim, queries._rows, queries.device_index
+        nq = q.rows
     else:
-        _matrix(queries, "queries")
-        if not isinstance(vectors, Fp8Rows):
+        pitch = _matrix(queries, "queries")
+        if not fp8:
             if queries.dtype != vectors.dtype:
                 raise ValueError(f"queries must have the vectors' type {vectors.dtype}, got {queries.dtype}")
-            queries = aligned_rows(queries)
-        nq, qdim = queries.shape
-        q, qdev, keep = L.Rows(queries.data_ptr(), None, nq, _pitch(queries), 0, _TYPES[queries.dtype]), queries.device, queries
+            if pitch % 8 or queries.data_ptr() % 16:
+                queries = aligned_rows(queries)
+                pitch = _pitch(queries)
+        (nq, qdim), qdevice = queries.shape, queries.get_device()
+        q = L.Rows(queries.data_ptr(), None, nq, pitch, 0, _TYPES[queries.dtype])
     if qdim != dim:
         raise ValueError(f"dim mismatch: expected {dim}, got {qdim}")
-    if qdev != device:
-        raise ValueError(f"all tensors must be on {device}, got one on {qdev}")
+    if qdevice != device:
+        raise ValueError(f"queries and vectors must be on one GPU, got cuda:{qdevice} and cuda:{device}")
     if dtype not in _TYPES:
         raise ValueError(f"scores must be float32, float16 or bfloat16, not {dtype}")
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()):
-        raise ValueError(f"bias must be a contiguous float32 tensor of {n} values")
-    _on(device, bias)
-    return device, dim, nq, n, q, v, keep
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous():
+            raise ValueError(f"bias must be a contiguous float32 tensor of {n} values")
+        _on(device, bias)
+    return device, dim, nq, n, q, v, queries
 
 
-def _status(status: Optional[torch.Tensor], device) -> Optional[int]:
+def _status(status: Optional[torch.Tensor], device: int) -> Optional[int]:
     if status is None:
         return None
     if status.dtype != torch.int32 or status.numel() != 1:
@@ -214,17 +232,20 @@ def scores(queries: Rows, vectors: Rows, *, alpha: float = 1.0, bias: Optional[t
     bias ranks like squared distances. `out`: a matrix of `dtype` to write (any
     row pitch). `status`: an int32 that gets RAVEN_S_* bits."""
     device, dim, nq, n, q, v, keep = _operands(queries, vectors, dtype, bias)
+    pitch = n
     if out is None:
-        out = torch.empty(nq, n, dtype=dtype, device=device)
-    elif out.shape != (nq, n) or out.dtype != dtype or (n > 1 and out.stride(1) != 1) or (nq > 1 and out.stride(0) < n):
-        raise ValueError(f"out must be a {dtype} matrix of {nq} x {n}, each row's values side by side")
-    _on(device, out)
-    _call(device, L.load().raven_scores_device, q, v, dim, alpha, _ptr(bias), out.data_ptr(), _TYPES[dtype],
-          max(_pitch(out), 1), _status(status, device))
+        out = torch.empty((nq, n), dtype=dtype, device=vectors.device)
+    else:
+        if out.shape != (nq, n) or out.dtype != dtype or (n > 1 and out.stride(1) != 1) or (nq > 1 and out.stride(0) < n):
+            raise ValueError(f"out must be a {dtype} matrix of {nq} x {n}, each row's values side by side")
+        _on(device, out)
+        pitch = _pitch(out)
+    _call(device, L.load().raven_scores_device, q, v, dim, alpha, _ptr(bias), out.data_ptr(), _TYPES[dtype], pitch,
+          _status(status, device))
     return out
 
 
-def _offsets(name: str, t: torch.Tensor, device) -> int:
+def _offsets(name: str, t: torch.Tensor, device: int) -> int:
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int64 or t.dim() != 1 or t.numel() < 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous 1-D int64 tensor")
     _on(device, t)
@@ -251,10 +272,11 @@ def group_scores(queries: Rows, query_offsets: torch.Tensor, vectors: Rows, vect
     if out is None:
         if total is None:
             raise ValueError("total or out is needed: the number of scores is known on the GPU only")
-        out = torch.empty(total, dtype=dtype, device=device)
+        out = torch.empty(total, dtype=dtype, device=vectors.device)
     elif out.dim() != 1 or out.dtype != dtype or not out.is_contiguous() or (total is not None and out.numel() < total):
         raise ValueError(f"out must be a contiguous 1-D {dtype} tensor with room for the scores")
-    _on(device, out)
+    else:
+        _on(device, out)
     _call(device, L.load().raven_group_scores_device, q, query_offsets.data_ptr(), v, vector_offsets.data_ptr(), groups,
           dim, alpha, _ptr(bias), out.data_ptr(), _TYPES[dtype], out.numel(), _status(status, device))
     return out
@@ -264,7 +286,7 @@ def group_rows(query_offsets: torch.Tensor, vector_offsets: torch.Tensor, nq: in
                status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """int64 [nq + 1]: where each query's scores start in the output of
     `group_scores`, and its size; the row_starts of `top_k`."""
-    device = query_offsets.device
+    device = query_offsets.get_device()
     groups = _offsets("query_offsets", query_offsets, device)
     if _offsets("vector_offsets", vector_offsets, device) != groups:
         raise ValueError("query_offsets and vector_offsets must have the same length")
@@ -272,7 +294,7 @@ def group_rows(query_offsets: torch.Tensor, vector_offsets: torch.Tensor, nq: in
         raise ValueError("query_offsets must be on a GPU")
     if groups == 0 or nq < 0 or n < 0:
         raise ValueError("there must be at least one group, and nq and n must not be negative")
-    out = torch.empty(nq + 1, dtype=torch.int64, device=device)
+    out = torch.empty(nq + 1, dtype=torch.int64, device=query_offsets.device)
     _call(device, L.load().raven_group_rows_device, query_offsets.data_ptr(), vector_offsets.data_ptr(), groups, nq, n,
           out.data_ptr(), _status(status, device))
     return out
@@ -287,19 +309,21 @@ def top_k(scores: torch.Tensor, k: int, *, largest: bool = True,
     row's count (rows of fewer than k) are 0."""
     if not isinstance(scores, torch.Tensor) or not scores.is_cuda or scores.dtype not in _TYPES:
         raise ValueError("scores must be a float32, float16 or bfloat16 tensor on a GPU")
+    index, device = scores.get_device(), scores.device
     if row_starts is None:
-        if scores.dim() != 2 or (scores.shape[1] > 1 and scores.stride(1) != 1) or \
-                (scores.shape[0] > 1 and scores.stride(0) < scores.shape[1]):
-            raise ValueError("scores must be a matrix with each row's values side by side")
-        (nq, n), ld, starts = scores.shape, _pitch(scores), None
+        if scores.dim() != 2:
+            raise ValueError("scores must be a matrix, or packed with row_starts")
+        (nq, n), (ld, step), starts = scores.shape, scores.stride(), None
+        if (n > 1 and step != 1) or (nq > 1 and ld < n):
+            raise ValueError("scores must hold each row's values side by side and its rows one after another")
+        ld = max(ld, n)
     else:
         if scores.dim() != 1 or not scores.is_contiguous():
             raise ValueError("packed scores must be a contiguous 1-D tensor")
-        nq, n, ld, starts = _offsets("row_starts", row_starts, scores.device), scores.numel(), 0, row_starts.data_ptr()
-    device = scores.device
-    vals = torch.empty(nq, max(k, 0), dtype=scores.dtype, device=device)
-    ids = torch.empty(nq, max(k, 0), dtype=torch.int32, device=device)
+        nq, n, ld, starts = _offsets("row_starts", row_starts, index), scores.numel(), 0, row_starts.data_ptr()
+    vals = torch.empty((nq, max(k, 0)), dtype=scores.dtype, device=device)
+    ids = torch.empty((nq, max(k, 0)), dtype=torch.int32, device=device)
     counts = torch.empty(nq, dtype=torch.int32, device=device)
-    _call(device, L.load().raven_topk_rows_device, scores.data_ptr(), _TYPES[scores.dtype], nq, n, ld, starts, k,
+    _call(index, L.load().raven_topk_rows_device, scores.data_ptr(), _TYPES[scores.dtype], nq, n, ld, starts, k,
           int(largest), vals.data_ptr(), ids.data_ptr(), counts.data_ptr())
     return vals, ids, counts
