@@ -210,13 +210,16 @@ struct TileFinder {
     }
     const uint32_t wide = min(kBand, mt - band * kBand);
     const uint32_t ti = rest / wide, qi = band * kBand + rest - ti * wide;
+    // even query tiles (at most BN, so mt - 1 of them are less than m): with a
+    // short last one, the CTAs that always got that one had less to do
+    const uint32_t step = mt == 1 ? BN : ((m + mt - 1) / mt + 15) / 16 * 16;
     Tile r;
     r.ld = p.qo ? (int64_t)nn : (int64_t)p.ld;
-    r.out = out0 + before + (int64_t)(qi * BN) * r.ld + (int64_t)(ti * kBM);
+    r.out = out0 + before + (int64_t)(qi * step) * r.ld + (int64_t)(ti * kBM);
     r.vrow = va + ti * kBM;
-    r.qrow = qa + qi * BN;
+    r.qrow = qa + qi * step;
     r.vcnt = min((uint32_t)kBM, nn - ti * kBM);
-    r.qcnt = min((uint32_t)BN, m - qi * BN);
+    r.qcnt = min(step, m - qi * step);
     return r;
   }
 };
@@ -242,6 +245,16 @@ __device__ inline void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
       : "r"(taddr));
 }
 __device__ inline void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+
+__device__ inline bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(is)::"memory");
+  return is != 0;
+}
+// The whole warp waits; one answer for all lanes.
+__device__ inline bool warp_wait(uint32_t bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
 
 __device__ inline void put(float* p, float v) { *p = v; }
 __device__ inline void put(__half* p, float v) { *p = __float2half_rn(v); }
@@ -326,113 +339,121 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
   bool ok = true;
   after_previous();
 
-  if (warp == 0) {
-    if (lane == 0) {  // TMA
-      TileReader rd;
-      uint32_t s = 0, ph = 0, used = 0, last_ph = 0;
-      while (ok) {
-        if (!mbar_wait(info_full(rd.slot), rd.phase)) {
+  // Warps 0 and 1 run their loops as whole warps and elect a lane only where
+  // they issue: loop state then lives in uniform registers, which is what the
+  // copies and MMAs take their operands from. One lane looping alone moved
+  // every operand over at each use, about 500 cycles per K block.
+  if (warp == 0) {  // TMA
+    TileReader rd;
+    uint32_t s = 0, ph = 0, used = 0, last_ph = 0;
+    while (ok) {
+      if (!warp_wait(info_full(rd.slot), rd.phase)) {
+        ok = false;
+        break;
+      }
+      const uint32_t qcnt = tiles[rd.slot].qcnt, vrow = tiles[rd.slot].vrow, qrow = tiles[rd.slot].qrow;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(info_empty(rd.slot));
+      rd.next();
+      if (qcnt == 0) break;
+      const uint32_t boxes = (qcnt + kQBox - 1) / kQBox;
+      for (uint32_t kb = 0; kb < p.nkb; ++kb) {
+        if (!warp_wait(empty(s), ph ^ 1u)) {
           ok = false;
           break;
         }
-        const Tile t = tiles[rd.slot];
-        mbar_arrive(info_empty(rd.slot));
-        rd.next();
-        if (t.qcnt == 0) break;
-        const uint32_t boxes = (t.qcnt + kQBox - 1) / kQBox;
-        for (uint32_t kb = 0; kb < p.nkb; ++kb) {
-          if (!mbar_wait(empty(s), ph ^ 1u)) {
-            ok = false;
-            break;
-          }
+        if (elect_one()) {
           mbar_expect_tx(full(s), kABytes + boxes * kQBoxBytes);
           const uint32_t a = sbase + s * L::kStage;
           const int x = (int)(kb * (FP8 ? 128u : 64u));
-          tma_load_2d(a, &tm_v, x, (int)t.vrow, full(s));
+          tma_load_2d(a, &tm_v, x, (int)vrow, full(s));
           for (uint32_t b = 0; b < boxes; ++b)
-            tma_load_2d(a + kABytes + b * kQBoxBytes, &tm_q, x, (int)(t.qrow + b * kQBox), full(s));
-          used |= 1u << s;
-          last_ph = (last_ph & ~(1u << s)) | (ph << s);
-          if (++s == S) {
-            s = 0;
-            ph ^= 1u;
-          }
+            tma_load_2d(a + kABytes + b * kQBoxBytes, &tm_q, x, (int)(qrow + b * kQBox), full(s));
+        }
+        __syncwarp();
+        used |= 1u << s;
+        last_ph = (last_ph & ~(1u << s)) | (ph << s);
+        if (++s == S) {
+          s = 0;
+          ph ^= 1u;
         }
       }
-      // every load issued has landed (immediate unless a wait ran out)
-      for (uint32_t st = 0; st < S; ++st)
-        if ((used >> st) & 1u) ok &= mbar_wait(full(st), (last_ph >> st) & 1u);
     }
-  } else if (warp == 1) {
-    if (lane == 0) {  // MMA
-      TileReader rd;
-      uint32_t s = 0, ph = 0, b = 0, bph = 0, f = 0, fph = 0;
-      while (ok) {
-        if (!mbar_wait(info_full(rd.slot), rd.phase)) {
+    // every load issued has landed (immediate unless a wait ran out)
+    for (uint32_t st = 0; st < S; ++st)
+      if ((used >> st) & 1u) ok &= warp_wait(full(st), (last_ph >> st) & 1u);
+  } else if (warp == 1) {  // MMA
+    TileReader rd;
+    uint32_t s = 0, ph = 0, b = 0, bph = 0, f = 0, fph = 0;
+    while (ok) {
+      if (!warp_wait(info_full(rd.slot), rd.phase)) {
+        ok = false;
+        break;
+      }
+      const uint32_t qcnt = __shfl_sync(0xffffffffu, tiles[rd.slot].qcnt, 0);
+      if (lane == 0) mbar_arrive(info_empty(rd.slot));
+      rd.next();
+      if (qcnt == 0) break;
+      const uint32_t idesc = p.idesc | (((qcnt + 15u) / 16u * 2u) << 17);  // N, a multiple of 16, in eights
+      if (!warp_wait(acc_empty(b), bph ^ 1u)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t d = tmem + b * BN;
+      for (uint32_t kb = 0; kb < p.nkb; ++kb) {
+        if (FP8 && (kb & 3u) == 0 && !warp_wait(sf_full(f), fph)) {
           ok = false;
           break;
         }
-        const uint32_t qcnt = tiles[rd.slot].qcnt;
-        mbar_arrive(info_empty(rd.slot));
-        rd.next();
-        if (qcnt == 0) break;
-        const uint32_t idesc = p.idesc | (((qcnt + 15u) / 16u * 2u) << 17);  // N, a multiple of 16, in eights
-        if (!mbar_wait(acc_empty(b), bph ^ 1u)) {
+        if (!warp_wait(full(s), ph)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t d = tmem + b * BN;
-        for (uint32_t kb = 0; kb < p.nkb; ++kb) {
-          if (FP8 && (kb & 3u) == 0 && !mbar_wait(sf_full(f), fph)) {
-            ok = false;
-            break;
-          }
-          if (!mbar_wait(full(s), ph)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t a = sbase + s * L::kStage;
-          const uint64_t da = sw128_desc(a), db = sw128_desc(a + kABytes);
-          const uint32_t steps = kb + 1 == p.nkb ? p.last_k : 4u;
-          for (uint32_t k = 0; k < steps; ++k) {  // 32 bytes along the swizzled row
-            if constexpr (FP8) {
-              const uint32_t sel = kb & 3u;
-              mma_mxf8(d, da + 2 * k, db + 2 * k, idesc | (sel << 4) | (sel << 29), tmem + L::kAcc + f * kSfCols,
-                       tmem + L::kAcc + f * kSfCols + 4, (kb | k) != 0u);
-            } else {
+        const uint32_t a = sbase + s * L::kStage;
+        const uint64_t da = sw128_desc(a), db = sw128_desc(a + kABytes);
+        const bool last = kb + 1 == p.nkb;
+        const bool sf_done = FP8 && ((kb & 3u) == 3u || last);
+        const uint32_t steps = last ? p.last_k : 4u;
+        const uint32_t sel = kb & 3u;
+        const uint32_t sf = tmem + L::kAcc + f * kSfCols;
+        if (elect_one()) {
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k) {  // 32 bytes along the swizzled row
+            if (k >= steps) break;
+            if constexpr (FP8)
+              mma_mxf8(d, da + 2 * k, db + 2 * k, idesc | (sel << 4) | (sel << 29), sf, sf + 4, (kb | k) != 0u);
+            else
               mma_f16(d, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0u);
-            }
           }
           mma_commit(empty(s));
-          if (++s == S) {
-            s = 0;
-            ph ^= 1u;
-          }
-          if (FP8 && ((kb & 3u) == 3u || kb + 1 == p.nkb)) {
-            mma_commit(sf_empty(f));
-            if (++f == kSf) {
-              f = 0;
-              fph ^= 1u;
-            }
-          }
+          if (sf_done) mma_commit(sf_empty(f));
+          if (last) mma_commit(acc_full(b));
         }
-        if (!ok) break;
-        mma_commit(acc_full(b));
-        b ^= 1u;
-        bph ^= b == 0u;
+        __syncwarp();
+        if (++s == S) {
+          s = 0;
+          ph ^= 1u;
+        }
+        if (sf_done && ++f == kSf) {
+          f = 0;
+          fph ^= 1u;
+        }
       }
-      mma_commit(drain);  // every MMA issued has completed
-      ok &= mbar_wait(drain, 0);
+      if (!ok) break;
+      b ^= 1u;
+      bph ^= b == 0u;
     }
+    if (elect_one()) mma_commit(drain);  // every MMA issued has completed
+    __syncwarp();
+    ok &= warp_wait(drain, 0);
   } else if (warp == 2) {  // tiles
     TileFinder<BN> finder(p, lane);
     TileReader wr;
     for (uint64_t t = blockIdx.x;; t += gridDim.x) {
       const int at = finder.find(t);
-      const bool got = mbar_wait(info_empty(wr.slot), wr.phase ^ 1u);
-      if (!__all_sync(0xffffffffu, got)) {
+      if (!warp_wait(info_empty(wr.slot), wr.phase ^ 1u)) {
         ok = false;
         break;
       }
@@ -456,8 +477,7 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
     TileReader rd;
     uint32_t b = 0, bph = 0;
     while (true) {
-      bool got = mbar_wait(info_full(rd.slot), rd.phase);
-      if (!__all_sync(0xffffffffu, got)) {
+      if (!warp_wait(info_full(rd.slot), rd.phase)) {
         ok = false;
         break;
       }
@@ -467,8 +487,7 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
       rd.next();
       if (t.qcnt == 0) break;
       const float bias = p.bias && r < t.vcnt ? p.bias[t.vrow + r] : 0.0f;
-      got = mbar_wait(acc_full(b), bph);
-      if (!__all_sync(0xffffffffu, got)) {
+      if (!warp_wait(acc_full(b), bph)) {
         ok = false;
         break;
       }
@@ -503,8 +522,7 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
     TileReader rd;
     uint32_t f = 0, fph = 0;
     while (ok) {
-      bool got = mbar_wait(info_full(rd.slot), rd.phase);
-      if (!__all_sync(0xffffffffu, got)) {
+      if (!warp_wait(info_full(rd.slot), rd.phase)) {
         ok = false;
         break;
       }
@@ -526,8 +544,7 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
 #pragma unroll
         for (uint32_t j = 0; j < BN / 32; ++j)
           if (32 * j < t.qcnt) w[4 + j] = *(const uint32_t*)(qe[j] + kb);
-        got = mbar_wait(sf_empty(f), fph ^ 1u);
-        if (!__all_sync(0xffffffffu, got)) {
+        if (!warp_wait(sf_empty(f), fph ^ 1u)) {
           ok = false;
           break;
         }
