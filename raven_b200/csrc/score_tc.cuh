@@ -22,8 +22,9 @@
 //   warp 1      issues the MMAs
 //   warp 2      owns the tensor memory; finds the CTA's tiles
 //   warps 4-11  epilogue: one accumulator is stored while the next is filled
-//   warps 12-15 (FP8) bring the tile's exponents to tensor memory, each warp
-//               its 32 lanes (every lane quadrant holds a copy)
+//   warps 12-15 (FP8) gather the tile's exponents, which start at any row of
+//               a group, into the order that tensor memory takes; the MMA warp
+//               copies them there in line with its instructions
 // A tile's size is known on the device only (group sizes are device data): the
 // N of its instructions and the queries it loads follow the group.
 //
@@ -58,8 +59,9 @@ constexpr int kQBox = 32;              // queries per TMA box
 constexpr uint32_t kABytes = kBM * 128;
 constexpr uint32_t kQBoxBytes = kQBox * 128;
 constexpr int kInfo = 4;               // tiles found ahead
-constexpr int kSf = 4;                 // exponent buffers in tensor memory
+constexpr int kSf = 4;                 // exponent buffers, in shared and in tensor memory
 constexpr int kSfCols = 16;            // columns of one: 4 for the rows, 8 for the queries
+constexpr uint32_t kSfBytes = 512;     // 128 rows: 32 lanes x 4 columns
 constexpr uint32_t kBand = 8;          // query tiles walked together (they share a tile of v in L2)
 
 enum : int { kOutF32 = 0, kOutF16 = 1, kOutBf16 = 2 };
@@ -101,7 +103,9 @@ struct Layout {
   static constexpr uint32_t kBars = kStages * kStage;
   // full[S], empty[S], acc_full[2], acc_empty[2], info_full[I], info_empty[I], sf_full[F], sf_empty[F], drain
   static constexpr uint32_t kNumBars = 2 * kStages + 4 + 2 * kInfo + 2 * kSf + 1;
-  static constexpr uint32_t kTiles = (kBars + kNumBars * 8 + 15) / 16 * 16;
+  static constexpr uint32_t kExps = (kBars + kNumBars * 8 + 127) / 128 * 128;
+  static constexpr uint32_t kExpBuf = (1 + (BN + 127) / 128) * kSfBytes;
+  static constexpr uint32_t kTiles = kExps + (FP8 ? kSf * kExpBuf : 0);
   static constexpr uint32_t kSlot = kTiles + kInfo * (uint32_t)sizeof(Tile);
   static constexpr uint32_t kBytes = kSlot + 16 + 1024;
   static constexpr uint32_t kAcc = 2 * BN;  // accumulator columns
@@ -116,6 +120,12 @@ __device__ inline void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t ides
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
       : "memory");
+}
+// 512 bytes of exponents (32 lanes x 16 bytes) to four columns, the same in each
+// lane quadrant. Plain layout: groups of 8 lanes 128 bytes apart.
+__device__ inline void copy_exps(uint32_t taddr, uint32_t smem) {
+  const uint64_t desc = (uint64_t)((smem >> 4) & 0x3FFFu) | ((uint64_t)8 << 16) | ((uint64_t)8 << 32) | ((uint64_t)1 << 46);
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(taddr), "l"(desc) : "memory");
 }
 __device__ inline void mma_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                 uint32_t acc) {
@@ -251,8 +261,16 @@ __device__ inline bool elect_one() {
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(is)::"memory");
   return is != 0;
 }
-// The whole warp waits; one answer for all lanes.
+// The whole warp waits; one answer for all lanes. The clock is read only when
+// the first look does not find the phase complete.
 __device__ inline bool warp_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  if (__all_sync(0xffffffffu, done != 0)) return true;
   return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
 
@@ -419,6 +437,11 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
         const uint32_t sel = kb & 3u;
         const uint32_t sf = tmem + L::kAcc + f * kSfCols;
         if (elect_one()) {
+          if (FP8 && sel == 0) {  // in order before the MMAs that read them
+            const uint32_t e = sbase + L::kExps + f * L::kExpBuf;
+#pragma unroll
+            for (int j = 0; j < 1 + (BN + 127) / 128; ++j) copy_exps(sf + 4 * j, e + j * kSfBytes);
+          }
 #pragma unroll
           for (uint32_t k = 0; k < 4; ++k) {  // 32 bytes along the swizzled row
             if (k >= steps) break;
@@ -518,58 +541,58 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
       bph ^= b == 0u;
     }
   } else if (FP8 && warp >= 12) {  // exponents
-    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    // Thread r takes row r of the tile and queries r and r + 128: the word of
+    // row 32 j + i goes to lane i, column j. The next words are on their way
+    // while these are stored.
+    constexpr int kParts = 1 + (BN + 127) / 128;
+    const uint32_t r = threadIdx.x - 384;
     TileReader rd;
-    uint32_t f = 0, fph = 0;
-    while (ok) {
-      if (!warp_wait(info_full(rd.slot), rd.phase)) {
+    uint32_t kb = p.nkb;
+    const uint8_t* src[kParts];
+    auto load = [&](uint32_t (&w)[kParts]) {  // false: no more, or a wait ran out
+      kb += 4;
+      if (kb >= p.nkb) {
+        if (!warp_wait(info_full(rd.slot), rd.phase)) {
+          ok = false;
+          return false;
+        }
+        const uint32_t vrow = tiles[rd.slot].vrow, qrow = tiles[rd.slot].qrow, qcnt = tiles[rd.slot].qcnt;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(info_empty(rd.slot));
+        rd.next();
+        if (qcnt == 0) return false;
+        kb = 0;
+        // rows past the arrays' ends repeat the last one
+        src[0] = p.ve + min((uint64_t)vrow + r, p.n - 1) * p.ld_ve;
+#pragma unroll
+        for (int j = 1; j < kParts; ++j)
+          src[j] = p.qe + min((uint64_t)qrow + min(r + 128u * (j - 1), qcnt - 1), p.nq - 1) * p.ld_qe;
+      }
+#pragma unroll
+      for (int j = 0; j < kParts; ++j) w[j] = __ldg((const uint32_t*)(src[j] + kb));
+      return true;
+    };
+    uint32_t f = 0, fph = 0, w[kParts], next[kParts];
+    bool more = load(w);
+    while (more) {
+      more = load(next);
+      if (!ok) break;
+      if (!warp_wait(sf_empty(f), fph ^ 1u)) {
         ok = false;
         break;
       }
-      const Tile t = tiles[rd.slot];
+      uint8_t* to = smem + L::kExps + f * L::kExpBuf + (r % 32) * 16 + (r / 32) * 4;
+#pragma unroll
+      for (int j = 0; j < kParts; ++j) {
+        *(uint32_t*)(to + j * kSfBytes) = w[j];
+        w[j] = next[j];
+      }
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(info_empty(rd.slot));
-      rd.next();
-      if (t.qcnt == 0) break;
-      // column j, lane i: the word of row 32 j + i (rows past the arrays' ends repeat the last one)
-      const uint8_t *ve[4], *qe[8];
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) ve[j] = p.ve + min((uint64_t)t.vrow + 32 * j + lane, p.n - 1) * p.ld_ve;
-#pragma unroll
-      for (uint32_t j = 0; j < BN / 32; ++j) qe[j] = p.qe + min((uint64_t)t.qrow + 32 * j + lane, p.nq - 1) * p.ld_qe;
-      for (uint32_t kb = 0; kb < p.nkb; kb += 4) {
-        uint32_t w[12] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) w[j] = *(const uint32_t*)(ve[j] + kb);
-#pragma unroll
-        for (uint32_t j = 0; j < BN / 32; ++j)
-          if (32 * j < t.qcnt) w[4 + j] = *(const uint32_t*)(qe[j] + kb);
-        if (!warp_wait(sf_empty(f), fph ^ 1u)) {
-          ok = false;
-          break;
-        }
-        const uint32_t at = tmem + lane_base + L::kAcc + f * kSfCols;
-        tc_fence_after();
-        asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(w[0]), "r"(w[1]),
-                     "r"(w[2]), "r"(w[3])
-                     : "memory");
-        if constexpr (BN <= 32)
-          asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};\n" ::"r"(at + 4), "r"(w[4]) : "memory");
-        else if constexpr (BN <= 64)
-          asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};\n" ::"r"(at + 4), "r"(w[4]), "r"(w[5])
-                       : "memory");
-        else
-          asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(at + 4),
-                       "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]), "r"(w[9]), "r"(w[10]), "r"(w[11])
-                       : "memory");
-        asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sf_full(f));
-        if (++f == kSf) {
-          f = 0;
-          fph ^= 1u;
-        }
+      if (lane == 0) mbar_arrive(sf_full(f));
+      if (++f == kSf) {
+        f = 0;
+        fph ^= 1u;
       }
     }
   }
