@@ -13,16 +13,21 @@
 // the four instructions of a block name the same byte, and a column's four
 // bytes serve four blocks.
 //
-// Roles. 128 rows of v are the M side of an instruction (tensor-memory lanes),
-// up to BN queries the N side (columns): a lane then owns one row, and the 32
-// lanes of a warp store 32 consecutive scores of one query without a detour
-// through shared memory. One 128-byte swizzled row of shared memory is a block
-// of 128 codes or 64 16-bit values, so both types share one pipeline.
-//   warp 0      TMA: per K block 128 rows of v and the tile's queries
+// Two layouts. The M side of an instruction is 128 rows (tensor-memory lanes), the
+// N side up to BN rows (columns).
+//   rows    M = rows of v, N = queries: few queries cost the tensor cores and the
+//           shared memory little, and the 32 lanes of a warp write 32 consecutive
+//           scores of a query. For f32 scores, and for few queries.
+//   pairs   M = queries, N = rows of v: a lane owns a query and reads its scores in
+//           order, so it packs them into whole 32-byte sectors of the output,
+//           wherever a query's scores start. For 16-bit scores of many queries.
+// One 128-byte swizzled row of shared memory is a block of 128 codes or 64
+// 16-bit values, so both types share one pipeline. Warp roles:
+//   warp 0      TMA: per K block the tile's rows and queries
 //   warp 1      issues the MMAs
 //   warp 2      owns the tensor memory; finds the CTA's tiles
-//   warps 4-11  epilogue: one accumulator is stored while the next is filled
-//   warps 12-15 (FP8) gather the tile's exponents, which start at any row of
+//   next 8 (16) epilogue: one tile is stored while the next is computed
+//   last 4 (FP8) gather the tile's exponents, which start at any row of
 //               a group, into the order that tensor memory takes; the MMA warp
 //               copies them there in line with its instructions
 // A tile's size is known on the device only (group sizes are device data): the
@@ -38,6 +43,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "internal.h"
 #include "knn_tc.cuh"
 
@@ -46,7 +53,6 @@ namespace raven_score {
 using raven_tc::mbar_arrive;
 using raven_tc::mbar_expect_tx;
 using raven_tc::mbar_init;
-using raven_tc::mbar_wait;
 using raven_tc::mma_commit;
 using raven_tc::smem_u32;
 using raven_tc::sw128_desc;
@@ -54,13 +60,13 @@ using raven_tc::tc_fence_after;
 using raven_tc::tc_fence_before;
 using raven_tc::tma_load_2d;
 
-constexpr int kBM = 128;               // rows of v per tile
-constexpr int kQBox = 32;              // queries per TMA box
+constexpr int kBM = 128;               // rows of the M side
+constexpr int kQBox = 32;              // queries per TMA box where they are the N side
 constexpr uint32_t kABytes = kBM * 128;
-constexpr uint32_t kQBoxBytes = kQBox * 128;
+constexpr uint32_t kSleepNs = 1000000;  // how long a wait may sleep before it looks at the clock
 constexpr int kInfo = 4;               // tiles found ahead
 constexpr int kSf = 4;                 // exponent buffers, in shared and in tensor memory
-constexpr int kSfCols = 16;            // columns of one: 4 for the rows, 8 for the queries
+constexpr int kSfCols = 16;            // columns of one: 4 for the M side, 8 for the N side
 constexpr uint32_t kSfBytes = 512;     // 128 rows: 32 lanes x 4 columns
 constexpr uint32_t kBand = 8;          // query tiles walked together (they share a tile of v in L2)
 
@@ -71,6 +77,8 @@ struct Params {
   uint64_t nq, n;             // rows of q and v
   uint32_t nkb;               // 128-byte K blocks
   uint32_t last_k;            // instructions (32 bytes of K) in the last block
+  uint32_t subs;              // (rows) accumulators per tile: a tile has up to 128 * subs rows of v
+  uint32_t halo;              // (pairs) scores that a tile computes past its own, 0 where every query starts on a sector
   uint32_t groups;            // 1 with null offsets: dense
   const int64_t* qo;          // [groups + 1] or null
   const int64_t* vo;
@@ -92,14 +100,21 @@ struct Tile {
   int64_t ld;
   uint32_t vrow, qrow;        // first row and query
   uint32_t vcnt, qcnt;        // how many; qcnt 0: no more tiles
+  uint32_t vext;              // (pairs) rows computed: vcnt and up to a sector of the next tile's scores
+  uint32_t first;             // whether the tile starts its queries' scores
 };
 
-template <bool FP8, int BN>
+// BN: most rows of the N side. ROWS: the layout with rows of v as the M side.
+template <bool FP8, int BN, bool ROWS>
 struct Layout {
   static constexpr uint32_t kStage = kABytes + BN * 128;
-  static constexpr int kStages = (int)((204u * 1024) / kStage) < 10 ? (int)((204u * 1024) / kStage) : 10;
-  static constexpr int kThreads = FP8 ? 512 : 384;
-  static constexpr int kConsumers = FP8 ? 14 : 10;  // arrivals that free a tile slot
+  static constexpr int kStages = (int)(200u * 1024 / kStage);
+  static constexpr int kEpiWarps = ROWS ? 8 : 16;
+  static constexpr int kThreads = 32 * (4 + kEpiWarps + (FP8 ? 4 : 0));
+  static constexpr int kConsumers = 2 + kEpiWarps + (FP8 ? 4 : 0);  // arrivals that free a tile slot
+  static constexpr int kSubs = ROWS && BN < 128 ? 128 / BN : 1;              // most accumulators per tile
+  static constexpr uint32_t kTileQ = ROWS ? BN : kBM;                // queries per tile
+  static constexpr uint32_t kTileV = ROWS ? kBM : BN;                // rows of v per accumulator
   static constexpr uint32_t kBars = kStages * kStage;
   // full[S], empty[S], acc_full[2], acc_empty[2], info_full[I], info_empty[I], sf_full[F], sf_empty[F], drain
   static constexpr uint32_t kNumBars = 2 * kStages + 4 + 2 * kInfo + 2 * kSf + 1;
@@ -108,10 +123,12 @@ struct Layout {
   static constexpr uint32_t kTiles = kExps + (FP8 ? kSf * kExpBuf : 0);
   static constexpr uint32_t kSlot = kTiles + kInfo * (uint32_t)sizeof(Tile);
   static constexpr uint32_t kBytes = kSlot + 16 + 1024;
-  static constexpr uint32_t kAcc = 2 * BN;  // accumulator columns
+  static constexpr uint32_t kAccBuf = kSubs * BN;
+  static constexpr uint32_t kAcc = 2 * kAccBuf;  // accumulator columns
   static constexpr uint32_t kUsed = kAcc + (FP8 ? kSf * kSfCols : 0);
   static constexpr uint32_t kTmem = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
   static_assert(kUsed <= 512, "tensor memory has 512 columns");
+  static_assert(kBytes <= 227 * 1024, "shared memory of a CTA");
 };
 
 __device__ inline void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -141,8 +158,9 @@ __device__ inline void mma_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t ide
 // time (one per lane) and their tiles counted by a warp scan; a CTA's tiles
 // rise, so the groups are walked once. The lane that holds a tile's group works
 // out the tile. Its divisions are 32-bit ones unless the group has 2^32 tiles.
-template <int BN>
+template <typename L>
 struct TileFinder {
+  static constexpr uint32_t TQ = L::kTileQ;
   const Params& p;
   int lane;
   uint64_t first = 0;       // first tile of the chunk
@@ -154,9 +172,10 @@ struct TileFinder {
   uint64_t chunk_tiles = 0;
   int64_t chunk_out = 0;
   uint32_t qa = 0, va = 0, m = 0, nn = 0;  // its first query and row, how many
+  uint32_t rows;            // of v per tile
   bool bad = false;
 
-  __device__ TileFinder(const Params& p_, int lane_) : p(p_), lane(lane_) { load(); }
+  __device__ TileFinder(const Params& p_, int lane_) : p(p_), lane(lane_), rows(L::kTileV * p_.subs - p_.halo) { load(); }
 
   __device__ void load() {
     const uint32_t g = g0 + (uint32_t)lane;
@@ -177,7 +196,7 @@ struct TileFinder {
         nn = (uint32_t)p.n;
       }
     }
-    tiles = (uint64_t)((m + BN - 1) / BN) * ((nn + kBM - 1) / kBM);
+    tiles = (uint64_t)((m + TQ - 1) / TQ) * ((nn + rows - 1) / rows);
     incl = tiles;
     int64_t e = (int64_t)m * nn;
 #pragma unroll
@@ -209,7 +228,7 @@ struct TileFinder {
   __device__ Tile tile(uint64_t t) const {
     const uint64_t in = t - first - (incl - tiles);
     // bands of kBand query tiles; in a band, all its query tiles of one row tile before the next
-    const uint32_t mt = (m + BN - 1) / BN, nt = (nn + kBM - 1) / kBM;
+    const uint32_t mt = (m + TQ - 1) / TQ, nt = (nn + rows - 1) / rows;
     uint32_t band, rest;
     if (in >> 32) {
       band = (uint32_t)(in / (kBand * nt));
@@ -220,16 +239,18 @@ struct TileFinder {
     }
     const uint32_t wide = min(kBand, mt - band * kBand);
     const uint32_t ti = rest / wide, qi = band * kBand + rest - ti * wide;
-    // even query tiles (at most BN, so mt - 1 of them are less than m): with a
+    // even query tiles (at most TQ, so mt - 1 of them are less than m): with a
     // short last one, the CTAs that always got that one had less to do
-    const uint32_t step = mt == 1 ? BN : ((m + mt - 1) / mt + 15) / 16 * 16;
+    const uint32_t step = mt == 1 ? TQ : ((m + mt - 1) / mt + 15) / 16 * 16;
     Tile r;
     r.ld = p.qo ? (int64_t)nn : (int64_t)p.ld;
-    r.out = out0 + before + (int64_t)(qi * step) * r.ld + (int64_t)(ti * kBM);
-    r.vrow = va + ti * kBM;
+    r.out = out0 + before + (int64_t)(qi * step) * r.ld + (int64_t)ti * rows;
+    r.vrow = va + ti * rows;
     r.qrow = qa + qi * step;
-    r.vcnt = min((uint32_t)kBM, nn - ti * kBM);
+    r.vcnt = min(rows, nn - ti * rows);
     r.qcnt = min(step, m - qi * step);
+    r.vext = min(rows + p.halo, nn - ti * rows);
+    r.first = ti == 0;
     return r;
   }
 };
@@ -245,8 +266,13 @@ struct TileReader {
   }
 };
 
-// 16 consecutive accumulator columns of this thread's lane, without waiting.
-__device__ inline void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+// 8 or 16 consecutive accumulator columns of this thread's lane, without waiting.
+__device__ inline void tmem_ld(uint32_t taddr, uint32_t (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(taddr));
+}
+__device__ inline void tmem_ld(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
       "[%16];\n"
@@ -254,7 +280,13 @@ __device__ inline void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
         "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(taddr));
 }
-__device__ inline void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+// Waits for the loads; ties the registers to the wait.
+template <int N>
+__device__ inline void tmem_wait_ld(uint32_t (&v)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
+}
 
 __device__ inline bool elect_one() {
   uint32_t is;
@@ -262,51 +294,162 @@ __device__ inline bool elect_one() {
   return is != 0;
 }
 // The whole warp waits; one answer for all lanes. The clock is read only when
-// the first look does not find the phase complete.
+// the phase is not complete at the first look.
 __device__ inline bool warp_wait(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  if (__all_sync(0xffffffffu, done != 0)) return true;
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+  long long t0 = 0;
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity), "r"(kSleepNs)
+        : "memory");
+    if (__all_sync(0xffffffffu, done != 0)) return true;
+    const long long t = clock64();
+    if (t0 == 0) t0 = t;
+    if (__any_sync(0xffffffffu, t - t0 > raven_tc::kWaitCycles)) return false;
+  }
 }
 
+// The accumulators of a tile are read: the MMA warp may fill them again.
+__device__ inline void free_acc(uint32_t bar, uint32_t lane) {
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
 __device__ inline void put(float* p, float v) { *p = v; }
 __device__ inline void put(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ inline void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// One epilogue warp's share of a tile: columns first, first + 32, ... in pieces
-// of 16. `at`: this lane's score of query 0.
-template <typename T>
-__device__ inline void store_tile(T* at, int64_t ld, uint32_t acc, uint32_t first, uint32_t qcnt, bool row, float alpha,
-                                  float bias) {
-  for (uint32_t c = first; c < qcnt; c += 32) {
-    uint32_t v[16];
-    tmem_ld16(acc + c, v);
-    tmem_wait_ld();
-    if (row) {
-      T* o = at + (int64_t)c * ld;
-      if (c + 16 <= qcnt) {
+// Layout by rows: a lane holds one row of v. Two warps per lane quadrant take 16
+// queries in turn.
+template <int BN, typename T>
+__device__ inline void store_rows(T* out, const Tile& t, uint32_t qcnt, uint32_t acc, uint32_t warp, uint32_t lane,
+                                 float alpha, const float* bias, uint32_t acc_empty) {
+  const uint32_t r = (warp & 3) * 32 + lane, first = 16 * (warp >> 2);
+  const uint32_t subs = (t.vcnt + kBM - 1) / kBM;
+  for (uint32_t sub = 0; sub < subs && first < qcnt; ++sub) {
+    const bool row = r + sub * kBM < t.vcnt;
+    const float add = bias && row ? __ldg(bias + sub * kBM + r) : 0.0f;
+    T* o = out + t.out + sub * kBM + r + (int64_t)first * t.ld;
+    for (uint32_t c = first; c < qcnt; c += 32, o += 32 * t.ld) {
+      uint32_t v[16];
+      tmem_ld(acc + sub * BN + c, v);
+      tmem_wait_ld(v);
+      if (row) {
+        T* q = o;
+        if (c + 16 <= qcnt) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j, o += ld) put(o, fmaf(alpha, __uint_as_float(v[j]), bias));
-      } else {
+          for (int j = 0; j < 16; ++j, q += t.ld) put(q, fmaf(alpha, __uint_as_float(v[j]), add));
+        } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j, o += ld)
-          if (c + j < qcnt) put(o, fmaf(alpha, __uint_as_float(v[j]), bias));
+          for (int j = 0; j < 16; ++j, q += t.ld)
+            if (c + j < qcnt) put(q, fmaf(alpha, __uint_as_float(v[j]), add));
+        }
       }
+      __syncwarp();
     }
-    __syncwarp();
   }
+  free_acc(acc_empty, lane);
 }
 
-template <bool FP8, int BN>
-__global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
+__device__ inline uint32_t word_of(const uint32_t (&v)[16], int i, const __half*) {
+  const __half2 h = __floats2half2_rn(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+  return *(const uint32_t*)&h;
+}
+__device__ inline uint32_t word_of(const uint32_t (&v)[16], int i, const __nv_bfloat16*) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+  return *(const uint32_t*)&h;
+}
+
+// Layout by pairs, 16-bit scores: a lane holds one query; four warps per lane
+// quadrant share the columns. A step makes one 32-byte sector (16 scores) of each
+// query. Where a query's scores start inside a sector (after `lead` others), the
+// sector is put together from the words of this step and the last: selects move
+// the pair of them by 8, 4, 2 and 1 words, a funnel shift by half a word. A warp
+// writes the sectors that start among its own scores, and takes what the last
+// one needs from the columns after them (a tile computes that much of the next
+// one), so that only a query's first and last sectors are written in part:
+// 999 x 250007 scores took 460 us when every warp wrote its ends in part, and
+// 999 x 250000, where every sector is whole, 103. Halves of sectors are as bad
+// (2.1 TB/s for 16-byte stores alone, 4.9 for 32-byte ones).
+template <int BN, typename T>
+__device__ inline void store_pairs(T* out, const Tile& t, uint32_t qcnt, uint32_t acc, uint32_t warp, uint32_t lane,
+                                   float alpha, const float* bias, uint32_t acc_empty) {
+  static_assert(sizeof(T) == 2, "16-bit scores");
+  const uint32_t per = (t.vcnt + 63) / 64 * 16;  // columns per warp
+  const uint32_t first = (warp >> 2) * per, q = (warp & 3) * 32 + lane;
+  if ((warp & 3) * 32 >= qcnt || first >= t.vcnt) {
+    free_acc(acc_empty, lane);
+    return;
+  }
+  const uint32_t cols = min(per, t.vcnt - first), avail = t.vext - first;
+  const uint64_t start = (uint64_t)(uintptr_t)(out + t.out + (int64_t)q * t.ld + first);
+  const uint32_t lead = (uint32_t)(start & 31u) / 2;
+  const uint32_t shift = 16 - lead;  // scores from the last step's first to the sector's
+  const bool straight = !__any_sync(0xffffffffu, lead != 0);
+  const uint32_t steps = (cols + 15) / 16 + (straight ? 0 : 1);
+  const uint32_t own = q < qcnt ? lead + cols : 0;                   // sectors from here on are another's
+  const uint32_t from = t.first && first == 0 ? 0 : lead;            // and before here
+  uint64_t sector = start & ~(uint64_t)31;
+  uint32_t v[16], x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  tmem_ld(acc + first, v);
+  for (uint32_t k = 0; k < steps; ++k, sector += 32) {
+    tmem_wait_ld(v);
+    uint32_t w[8];
+    if (alpha != 1.0f || bias) {
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) {
+        const uint32_t c = 16 * k + i;
+        v[i] = __float_as_uint(fmaf(alpha, __uint_as_float(v[i]), bias && c < avail ? __ldg(bias + first + c) : 0.0f));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = word_of(v, i, (const T*)0);
+    if (k + 1 < steps)
+      tmem_ld(acc + min(first + 16 * (k + 1), (uint32_t)BN - 16), v);  // the last may have no columns left, nor use for them
+    if (!straight) {
+      uint32_t y[17];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y[i] = x[i];
+        y[8 + i] = x[i] = w[i];
+      }
+      y[16] = 0;
+      const uint32_t by = shift >> 1;  // 0..8: 8 takes this step's words as they are
+#pragma unroll
+      for (int i = 0; i < 9; ++i) y[i] = by & 8 ? y[i + 8] : y[i];
+#pragma unroll
+      for (int i = 0; i < 13; ++i) y[i] = by & 4 ? y[i + 4] : y[i];
+#pragma unroll
+      for (int i = 0; i < 11; ++i) y[i] = by & 2 ? y[i + 2] : y[i];
+#pragma unroll
+      for (int i = 0; i < 9; ++i) y[i] = by & 1 ? y[i + 1] : y[i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = __funnelshift_r(y[i], y[i + 1], (shift & 1) * 16);
+    }
+    const uint32_t at = 16 * k;  // scores from the first sector's start
+    if (at >= lead && at < own && at + 16 <= lead + avail) {
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(sector), "r"(w[0]), "r"(w[1]),
+                   "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                   : "memory");
+    } else if (at >= from && at < own) {  // a query's first or last sector
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {
+        const uint32_t h = at + 2 * i;
+        if (h >= lead && h < lead + avail) *(uint16_t*)(sector + 4 * i) = (uint16_t)w[i];
+        if (h + 1 >= lead && h + 1 < lead + avail) *(uint16_t*)(sector + 4 * i + 2) = (uint16_t)(w[i] >> 16);
+      }
+    }
+  }
+  free_acc(acc_empty, lane);
+}
+
+template <bool FP8, int BN, bool ROWS>
+__global__ void __launch_bounds__((Layout<FP8, BN, ROWS>::kThreads), 1)
     score_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_v, const Params p) {
-  using L = Layout<FP8, BN>;
-  constexpr int S = L::kStages;
+  using L = Layout<FP8, BN, ROWS>;
+  constexpr int S = L::kStages, kEpiWarps = L::kEpiWarps;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = smem_u32(smem);
@@ -331,7 +474,7 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), 8);
+      mbar_init(acc_empty(b), kEpiWarps);
     }
     for (int i = 0; i < kInfo; ++i) {
       mbar_init(info_full(i), 1);
@@ -369,33 +512,41 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
         ok = false;
         break;
       }
-      const uint32_t qcnt = tiles[rd.slot].qcnt, vrow = tiles[rd.slot].vrow, qrow = tiles[rd.slot].qrow;
+      const uint32_t qcnt = tiles[rd.slot].qcnt, vcnt = tiles[rd.slot].vcnt, qrow = tiles[rd.slot].qrow;
+      const uint32_t vrow = tiles[rd.slot].vrow;
       __syncwarp();
       if (lane == 0) mbar_arrive(info_empty(rd.slot));
       rd.next();
       if (qcnt == 0) break;
-      const uint32_t boxes = (qcnt + kQBox - 1) / kQBox;
-      for (uint32_t kb = 0; kb < p.nkb; ++kb) {
-        if (!warp_wait(empty(s), ph ^ 1u)) {
-          ok = false;
-          break;
+      const uint32_t boxes = (qcnt + kQBox - 1) / kQBox;  // (rows)
+      for (uint32_t sub = 0; sub * L::kTileV < vcnt && ok; ++sub)
+        for (uint32_t kb = 0; kb < p.nkb; ++kb) {
+          if (!warp_wait(empty(s), ph ^ 1u)) {
+            ok = false;
+            break;
+          }
+          if (elect_one()) {
+            const uint32_t a = sbase + s * L::kStage, bar = full(s);
+            const int x = (int)(kb * (FP8 ? 128u : 64u));
+            if constexpr (ROWS) {
+              mbar_expect_tx(bar, kABytes + boxes * (kQBox * 128));
+              tma_load_2d(a, &tm_v, x, (int)(vrow + sub * kBM), bar);
+              for (uint32_t b = 0; b < boxes; ++b)
+                tma_load_2d(a + kABytes + b * (kQBox * 128), &tm_q, x, (int)(qrow + b * kQBox), bar);
+            } else {
+              mbar_expect_tx(bar, L::kStage);
+              tma_load_2d(a, &tm_q, x, (int)qrow, bar);
+              tma_load_2d(a + kABytes, &tm_v, x, (int)vrow, bar);
+            }
+          }
+          __syncwarp();
+          used |= 1u << s;
+          last_ph = (last_ph & ~(1u << s)) | (ph << s);
+          if (++s == S) {
+            s = 0;
+            ph ^= 1u;
+          }
         }
-        if (elect_one()) {
-          mbar_expect_tx(full(s), kABytes + boxes * kQBoxBytes);
-          const uint32_t a = sbase + s * L::kStage;
-          const int x = (int)(kb * (FP8 ? 128u : 64u));
-          tma_load_2d(a, &tm_v, x, (int)vrow, full(s));
-          for (uint32_t b = 0; b < boxes; ++b)
-            tma_load_2d(a + kABytes + b * kQBoxBytes, &tm_q, x, (int)(qrow + b * kQBox), full(s));
-        }
-        __syncwarp();
-        used |= 1u << s;
-        last_ph = (last_ph & ~(1u << s)) | (ph << s);
-        if (++s == S) {
-          s = 0;
-          ph ^= 1u;
-        }
-      }
     }
     // every load issued has landed (immediate unless a wait ran out)
     for (uint32_t st = 0; st < S; ++st)
@@ -409,59 +560,62 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
         break;
       }
       const uint32_t qcnt = __shfl_sync(0xffffffffu, tiles[rd.slot].qcnt, 0);
+      const uint32_t vcnt = __shfl_sync(0xffffffffu, ROWS ? tiles[rd.slot].vcnt : tiles[rd.slot].vext, 0);
       if (lane == 0) mbar_arrive(info_empty(rd.slot));
       rd.next();
       if (qcnt == 0) break;
-      const uint32_t idesc = p.idesc | (((qcnt + 15u) / 16u * 2u) << 17);  // N, a multiple of 16, in eights
+      const uint32_t idesc = p.idesc | ((((ROWS ? qcnt : vcnt) + 15u) / 16u * 2u) << 17);  // N, a multiple of 16, in eights
       if (!warp_wait(acc_empty(b), bph ^ 1u)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const uint32_t d = tmem + b * BN;
-      for (uint32_t kb = 0; kb < p.nkb; ++kb) {
-        if (FP8 && (kb & 3u) == 0 && !warp_wait(sf_full(f), fph)) {
-          ok = false;
-          break;
-        }
-        if (!warp_wait(full(s), ph)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t a = sbase + s * L::kStage;
-        const uint64_t da = sw128_desc(a), db = sw128_desc(a + kABytes);
-        const bool last = kb + 1 == p.nkb;
-        const bool sf_done = FP8 && ((kb & 3u) == 3u || last);
-        const uint32_t steps = last ? p.last_k : 4u;
-        const uint32_t sel = kb & 3u;
-        const uint32_t sf = tmem + L::kAcc + f * kSfCols;
-        if (elect_one()) {
-          if (FP8 && sel == 0) {  // in order before the MMAs that read them
-            const uint32_t e = sbase + L::kExps + f * L::kExpBuf;
-#pragma unroll
-            for (int j = 0; j < 1 + (BN + 127) / 128; ++j) copy_exps(sf + 4 * j, e + j * kSfBytes);
+      for (uint32_t sub = 0; sub * L::kTileV < vcnt && ok; ++sub) {
+        const uint32_t d = tmem + b * L::kAccBuf + sub * BN;
+        const bool last_sub = (sub + 1) * L::kTileV >= vcnt;
+        for (uint32_t kb = 0; kb < p.nkb; ++kb) {
+          if (FP8 && (kb & 3u) == 0 && !warp_wait(sf_full(f), fph)) {
+            ok = false;
+            break;
           }
-#pragma unroll
-          for (uint32_t k = 0; k < 4; ++k) {  // 32 bytes along the swizzled row
-            if (k >= steps) break;
-            if constexpr (FP8)
-              mma_mxf8(d, da + 2 * k, db + 2 * k, idesc | (sel << 4) | (sel << 29), sf, sf + 4, (kb | k) != 0u);
-            else
-              mma_f16(d, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0u);
+          if (!warp_wait(full(s), ph)) {
+            ok = false;
+            break;
           }
-          mma_commit(empty(s));
-          if (sf_done) mma_commit(sf_empty(f));
-          if (last) mma_commit(acc_full(b));
-        }
-        __syncwarp();
-        if (++s == S) {
-          s = 0;
-          ph ^= 1u;
-        }
-        if (sf_done && ++f == kSf) {
-          f = 0;
-          fph ^= 1u;
+          const uint32_t a = sbase + s * L::kStage, done = empty(s);
+          const uint64_t da = sw128_desc(a), db = sw128_desc(a + kABytes);
+          const bool last = kb + 1 == p.nkb;
+          const bool sf_done = FP8 && ((kb & 3u) == 3u || last);
+          const uint32_t steps = last ? p.last_k : 4u;
+          const uint32_t sel = kb & 3u;
+          const uint32_t sf = tmem + L::kAcc + f * kSfCols;
+          if (++s == S) {
+            s = 0;
+            ph ^= 1u;
+          }
+          if (elect_one()) {
+            if (FP8 && sel == 0) {  // in order before the MMAs that read them
+              const uint32_t e = sbase + L::kExps + f * L::kExpBuf;
+#pragma unroll
+              for (int j = 0; j < 1 + (BN + 127) / 128; ++j) copy_exps(sf + 4 * j, e + j * kSfBytes);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {  // 32 bytes along the swizzled row
+              if (k >= steps) break;
+              if constexpr (FP8)
+                mma_mxf8(d, da + 2 * k, db + 2 * k, idesc | (sel << 4) | (sel << 29), sf, sf + 4, (kb | k) != 0u);
+              else
+                mma_f16(d, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0u);
+            }
+            mma_commit(done);
+            if (sf_done) mma_commit(sf_empty(f));
+            if (last && last_sub) mma_commit(acc_full(b));
+          }
+          __syncwarp();
+          if (sf_done && ++f == kSf) {
+            f = 0;
+            fph ^= 1u;
+          }
         }
       }
       if (!ok) break;
@@ -472,7 +626,7 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
     __syncwarp();
     ok &= warp_wait(drain, 0);
   } else if (warp == 2) {  // tiles
-    TileFinder<BN> finder(p, lane);
+    TileFinder<L> finder(p, lane);
     TileReader wr;
     for (uint64_t t = blockIdx.x;; t += gridDim.x) {
       const int at = finder.find(t);
@@ -492,11 +646,8 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
       if (at < 0) break;
     }
     if (__any_sync(0xffffffffu, finder.bad) && lane == 0 && p.status) atomicOr(p.status, kStatusOffsets);
-  } else if (warp >= 4 && warp < 12) {  // epilogue: two warps per lane quadrant, 16 columns in turn
-    const int quad = warp & 3;
-    const uint32_t first = warp < 8 ? 0u : 16u;
-    const uint32_t r = (uint32_t)(quad * 32 + lane);
-    const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+  } else if (warp >= 4 && warp < 4 + kEpiWarps) {  // epilogue
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     TileReader rd;
     uint32_t b = 0, bph = 0;
     while (true) {
@@ -509,64 +660,75 @@ __global__ void __launch_bounds__((Layout<FP8, BN>::kThreads), 1)
       if (lane == 0) mbar_arrive(info_empty(rd.slot));
       rd.next();
       if (t.qcnt == 0) break;
-      const float bias = p.bias && r < t.vcnt ? p.bias[t.vrow + r] : 0.0f;
+      // queries whose scores of this tile lie within the output (a sum of wild offsets may have wrapped)
+      uint32_t qcnt = t.qcnt;
+      if (p.qo && (t.out < 0 || t.out + (int64_t)(qcnt - 1) * t.ld + t.vext > (int64_t)p.capacity)) {
+        const int64_t room = (int64_t)p.capacity - t.out - (int64_t)t.vext;
+        qcnt = room < 0 || t.out < 0 ? 0u : (uint32_t)min(room / t.ld + 1, (int64_t)qcnt);
+        if (lane == 0 && p.status && qcnt < t.qcnt) atomicOr(p.status, kStatusCapacity);
+      }
       if (!warp_wait(acc_full(b), bph)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      // queries whose scores of this tile lie within the output
-      uint32_t qcnt = t.qcnt;
-      if (p.qo) {
-        const int64_t room = (int64_t)p.capacity - t.out - (int64_t)t.vcnt;
-        const int64_t fit = room < 0 || t.out < 0 ? 0 : room / t.ld + 1;  // a sum of wild offsets may have wrapped
-        if (fit < (int64_t)qcnt) {
-          qcnt = (uint32_t)fit;
-          if (lane == 0 && p.status) atomicOr(p.status, kStatusCapacity);
-        }
+      const uint32_t acc = tmem + lane_base + b * L::kAccBuf, w = (uint32_t)(warp - 4);
+      const float* bias = p.bias ? p.bias + t.vrow : nullptr;
+      if constexpr (ROWS) {
+        if (p.out_type == kOutF32)
+          store_rows<BN>((float*)p.out, t, qcnt, acc, w, lane, p.alpha, bias, acc_empty(b));
+        else if (p.out_type == kOutF16)
+          store_rows<BN>((__half*)p.out, t, qcnt, acc, w, lane, p.alpha, bias, acc_empty(b));
+        else
+          store_rows<BN>((__nv_bfloat16*)p.out, t, qcnt, acc, w, lane, p.alpha, bias, acc_empty(b));
+      } else {
+        if (p.out_type == kOutF16)
+          store_pairs<BN>((__half*)p.out, t, qcnt, acc, w, lane, p.alpha, bias, acc_empty(b));
+        else
+          store_pairs<BN>((__nv_bfloat16*)p.out, t, qcnt, acc, w, lane, p.alpha, bias, acc_empty(b));
       }
-      const uint32_t acc = tmem + lane_base + b * BN;
-      const int64_t at = t.out + r;
-      const bool row = r < t.vcnt;
-      if (p.out_type == kOutF32)
-        store_tile((float*)p.out + at, t.ld, acc, first, qcnt, row, p.alpha, bias);
-      else if (p.out_type == kOutF16)
-        store_tile((__half*)p.out + at, t.ld, acc, first, qcnt, row, p.alpha, bias);
-      else
-        store_tile((__nv_bfloat16*)p.out + at, t.ld, acc, first, qcnt, row, p.alpha, bias);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty(b));
       b ^= 1u;
       bph ^= b == 0u;
     }
-  } else if (FP8 && warp >= 12) {  // exponents
-    // Thread r takes row r of the tile and queries r and r + 128: the word of
-    // row 32 j + i goes to lane i, column j. The next words are on their way
-    // while these are stored.
+  } else if (FP8 && warp >= 4 + kEpiWarps) {  // exponents
+    // Thread r takes row r of the M side and rows r and r + 128 of the N side:
+    // the word of row 32 j + i goes to lane i, column j. The next words are on
+    // their way while these are stored.
     constexpr int kParts = 1 + (BN + 127) / 128;
-    const uint32_t r = threadIdx.x - 384;
+    const uint32_t r = threadIdx.x - 32 * (4 + kEpiWarps);
     TileReader rd;
-    uint32_t kb = p.nkb;
+    uint32_t kb = p.nkb, sub = 0, vrow = 0, vcnt = 0;
     const uint8_t* src[kParts];
     auto load = [&](uint32_t (&w)[kParts]) {  // false: no more, or a wait ran out
       kb += 4;
       if (kb >= p.nkb) {
-        if (!warp_wait(info_full(rd.slot), rd.phase)) {
-          ok = false;
-          return false;
-        }
-        const uint32_t vrow = tiles[rd.slot].vrow, qrow = tiles[rd.slot].qrow, qcnt = tiles[rd.slot].qcnt;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(info_empty(rd.slot));
-        rd.next();
-        if (qcnt == 0) return false;
         kb = 0;
-        // rows past the arrays' ends repeat the last one
-        src[0] = p.ve + min((uint64_t)vrow + r, p.n - 1) * p.ld_ve;
+        if (++sub * L::kTileV >= vcnt) {
+          if (!warp_wait(info_full(rd.slot), rd.phase)) {
+            ok = false;
+            return false;
+          }
+          const uint32_t qrow = tiles[rd.slot].qrow, qcnt = tiles[rd.slot].qcnt;
+          vrow = tiles[rd.slot].vrow;
+          vcnt = ROWS ? tiles[rd.slot].vcnt : tiles[rd.slot].vext;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(info_empty(rd.slot));
+          rd.next();
+          if (qcnt == 0) return false;
+          sub = 0;
+          // rows past what the tile or the array has repeat the last one
+          if constexpr (ROWS) {
 #pragma unroll
-        for (int j = 1; j < kParts; ++j)
-          src[j] = p.qe + min((uint64_t)qrow + min(r + 128u * (j - 1), qcnt - 1), p.nq - 1) * p.ld_qe;
+            for (int j = 1; j < kParts; ++j)
+              src[j] = p.qe + ((uint64_t)qrow + min(r + 128u * (j - 1), qcnt - 1)) * p.ld_qe;
+          } else {
+            src[0] = p.qe + ((uint64_t)qrow + min(r, qcnt - 1)) * p.ld_qe;
+#pragma unroll
+            for (int j = 1; j < kParts; ++j)
+              src[j] = p.ve + ((uint64_t)vrow + min(r + 128u * (j - 1), vcnt - 1)) * p.ld_ve;
+          }
+        }
+        if constexpr (ROWS) src[0] = p.ve + min((uint64_t)vrow + sub * kBM + r, p.n - 1) * p.ld_ve;
       }
 #pragma unroll
       for (int j = 0; j < kParts; ++j) w[j] = __ldg((const uint32_t*)(src[j] + kb));

@@ -250,21 +250,56 @@ bool rows_map(CUtensorMap* m, const void* base, int32_t type, uint32_t dim, uint
            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool FP8, int BN>
-cudaError_t launch_score(const CUtensorMap& q, const CUtensorMap& v, const raven_score::Params& p, unsigned grid,
-                         cudaStream_t st) {
-  using L = raven_score::Layout<FP8, BN>;
+struct Operands {
+  const raven_rows* q;
+  const raven_rows* v;
+  uint32_t dim;
+};
+
+template <bool FP8, int BN, bool ROWS>
+cudaError_t launch_score(const Operands& o, raven_score::Params p, int sms, cudaStream_t st) {
+  using L = raven_score::Layout<FP8, BN, ROWS>;
+  CUtensorMap mq, mv;
+  if (!rows_map(&mq, o.q->data, o.q->type, o.dim, o.q->rows, o.q->ld, ROWS ? raven_score::kQBox : raven_score::kBM) ||
+      !rows_map(&mv, o.v->data, o.v->type, o.dim, o.v->rows, o.v->ld, ROWS ? raven_score::kBM : BN))
+    return cudaErrorInvalidValue;
+  // Rows per tile, where M is the rows. A tile of few queries has little to do
+  // when K is short, and what it costs to find it, to hand it over and to start
+  // its epilogue shows: it takes several accumulators at once, as long as every
+  // SM keeps a few tiles (grouped: and a tile does not outgrow a mean group).
+  const uint64_t per = p.qo ? std::max<uint64_t>(p.n / p.groups, 1) : p.n;
+  uint64_t subs = p.nkb <= 4 ? L::kSubs : 1;
+  auto tiles = [&](uint64_t s) {
+    return (p.qo ? p.groups : 1) * ((per + s * L::kTileV - 1) / (s * L::kTileV)) *
+           (p.qo ? 1 : (p.nq + L::kTileQ - 1) / L::kTileQ);
+  };
+  while (subs > 1 && (tiles(subs) < 4ull * sms || (p.qo && subs * L::kTileV > 2 * per))) subs /= 2;
+  p.subs = (uint32_t)subs;
+  const bool whole = !p.qo && (uintptr_t)p.out % 32 == 0 && p.ld % 16 == 0;  // every query starts on a sector
+  p.halo = ROWS || whole ? 0 : 16;
+  const uint64_t grid = p.qo ? (uint64_t)sms : std::min<uint64_t>(tiles(subs), (uint64_t)sms);
   static Allowed allowed;
-  return launch(raven_score::score_kernel<FP8, BN>, grid, L::kThreads, L::kBytes, allowed, st, q, v, p);
+  return launch(raven_score::score_kernel<FP8, BN, ROWS>, grid, L::kThreads, L::kBytes, allowed, st, mq, mv, p);
 }
 
+// `want`: queries of a group, twice the mean where groups differ. The layout by
+// rows of v for f32 scores and up to 64 queries, its N side as wide as those need
+// and no wider than leaves every SM a tile. 16-bit scores of more queries: the
+// layout by pairs (in f32 its lanes, a query each, wrote 1024 x 250000 scores in
+// 385 us, the other in 223: 32 queries a megabyte apart are as many pages).
 template <bool FP8>
-cudaError_t dispatch_score(uint32_t bn, const CUtensorMap& q, const CUtensorMap& v, const raven_score::Params& p,
-                           unsigned grid, cudaStream_t st) {
-  if (bn <= 32) return launch_score<FP8, 32>(q, v, p, grid, st);
-  if (bn <= 64) return launch_score<FP8, 64>(q, v, p, grid, st);
-  if (bn <= 128) return launch_score<FP8, 128>(q, v, p, grid, st);
-  return launch_score<FP8, FP8 ? 192 : 256>(q, v, p, grid, st);
+cudaError_t dispatch_score(const Operands& o, const raven_score::Params& p, int sms, cudaStream_t st) {
+  const uint64_t want = p.qo ? 2 * ((p.nq + p.groups - 1) / p.groups) : p.nq;
+  if (want > 64 && p.out_type != raven_score::kOutF32) {
+    if (!p.qo && (p.nq + 127) / 128 * ((p.n + 223) / 224) < (uint64_t)sms)
+      return launch_score<FP8, 96, false>(o, p, sms, st);
+    return launch_score<FP8, 224, false>(o, p, sms, st);
+  }
+  const uint64_t vt = (p.n + raven_score::kBM - 1) / raven_score::kBM;
+  auto fills = [&](uint64_t bn) { return p.qo || vt * ((p.nq + bn - 1) / bn) >= (uint64_t)sms; };
+  if (want > 64 && fills(192)) return launch_score<FP8, 192, true>(o, p, sms, st);
+  if (want > 32 && fills(64)) return launch_score<FP8, 64, true>(o, p, sms, st);
+  return launch_score<FP8, 32, true>(o, p, sms, st);
 }
 
 int check_rows(const raven_rows* r, uint32_t dim, const char* what) {
@@ -350,21 +385,8 @@ int run_scores(const raven_rows* q, const int64_t* qo, const raven_rows* v, cons
   p.ld_qe = qq.ld_exps;
   p.ld_ve = v->ld_exps;
 
-  // Queries per tile: enough for a group (twice the mean where groups differ),
-  // and not so many that SMs are left without a tile.
-  uint64_t want = qo ? 2 * ((p.nq + groups - 1) / groups) : p.nq;
-  const uint64_t vt = (p.n + raven_score::kBM - 1) / raven_score::kBM;
-  uint32_t bn = want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 ? 128 : fp8 ? 192 : 256;
-  if (!qo)
-    while (bn > 32 && vt * ((p.nq + bn - 1) / bn) < (uint64_t)sms) bn = bn > 128 ? 128 : bn / 2;
-  const uint64_t most = qo ? (uint64_t)sms : vt * ((p.nq + bn - 1) / bn);
-  const unsigned grid = (unsigned)std::min<uint64_t>(most, (uint64_t)sms);
-
-  CUtensorMap mq, mv;
-  cudaError_t e = cudaErrorInvalidValue;
-  if (rows_map(&mq, qq.data, qq.type, dim, qq.rows, qq.ld, raven_score::kQBox) &&
-      rows_map(&mv, v->data, v->type, dim, v->rows, v->ld, raven_score::kBM))
-    e = fp8 ? dispatch_score<true>(bn, mq, mv, p, grid, st) : dispatch_score<false>(bn, mq, mv, p, grid, st);
+  const Operands o{&qq, v, dim};
+  const cudaError_t e = fp8 ? dispatch_score<true>(o, p, sms, st) : dispatch_score<false>(o, p, sms, st);
   if (tmp) cudaFreeAsync(tmp, st);
   if (e != cudaSuccess) return fail(RAVEN_ECUDA, std::string("scores: ") + cudaGetErrorString(e));
   return RAVEN_OK;
