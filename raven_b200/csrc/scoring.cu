@@ -108,74 +108,120 @@ cudaError_t launch(void (*kern)(K...), uint64_t grid, int threads, uint32_t smem
 // e4m3(x * 2^-e) to nearest even, exponent byte = e + 127. A power of two
 // scales exactly, so the only rounding is e4m3's own (half a step, 2^-4 of the
 // value; 2^-10 * 2^e below the type's normal range).
-// One warp per block: lane l holds values 4l..4l+3, so a block is read in one
-// piece of 512 or 256 bytes and written in one of 128.
+// A block is read by 32 lanes (f32) or 16 (16-bit), 16 bytes each, and each warp
+// has four such reads under way: bound by memory, 30000 x 768 f16 in 14 us
+// (4.9 TB/s), where one read of 8 bytes a lane at a time took 31.
 // ---------------------------------------------------------------------------
 __device__ inline float load_value(const float* p) { return *p; }
 __device__ inline float load_value(const __half* p) { return __half2float(*p); }
 __device__ inline float load_value(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
-template <typename T>
-__device__ inline void load4(const T* p, float (&x)[4]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 v = *(const float4*)p;
-    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-  } else {
-    const uint2 v = *(const uint2*)p;
-    const T* h = (const T*)&v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = load_value(h + i);
-  }
-}
+// A CTA takes a run of rows and gathers their exponents in shared memory: single
+// bytes of a 32-byte sector written at different times cost a read each.
+// VEC: pitch and address let 16 bytes be read at once. LANE: lane-major rows
+// (element e of the first 16C at (e % 16) * C + e / 16).
+constexpr uint32_t kExpBytes = 4096;  // of a run: rows x blocks padded to 4
 
-// VEC: pitch and address let four values be read at once. LANE: lane-major
-// rows (element e of the first 16C at (e % 16) * C + e / 16).
 template <typename T, bool VEC, bool LANE>
 __global__ void __launch_bounds__(256) fp8_encode_kernel(const T* __restrict__ in, uint64_t n, uint32_t dim, uint64_t ld,
                                                          uint8_t* __restrict__ codes, uint64_t ld_codes,
-                                                         uint8_t* __restrict__ exps, uint64_t ld_exps) {
+                                                         uint8_t* __restrict__ exps, uint64_t ld_exps, uint32_t run) {
+  constexpr int E = 16 / sizeof(T), G = (int)kBlock / E, U = 4;  // values per lane, lanes per block, blocks under way
+  __shared__ __align__(16) uint8_t se[kExpBytes];
   after_previous();
-  const int lane = threadIdx.x & 31;
+  const uint32_t sub = threadIdx.x % G, group = threadIdx.x / G;
   const uint32_t nb = (dim + kBlock - 1) / kBlock, nb4 = (nb + 3) / 4 * 4, dim16 = (dim + 15) / 16 * 16;
-  const uint64_t units = n * nb;
-  const uint64_t warps = (uint64_t)gridDim.x * (blockDim.x >> 5);
-  for (uint64_t u = (uint64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += warps) {
-    const uint64_t row = u / nb;
-    const uint32_t b = (uint32_t)(u - row * nb);
-    const uint32_t d = b * kBlock + 4 * lane;
-    const T* r = in + row * ld;
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (VEC && d + 4 <= dim) {
-      load4(r + d, x);
-    } else {
-      const uint32_t C = dim / 16;
+  for (uint64_t r0 = (uint64_t)blockIdx.x * run; r0 < n; r0 += (uint64_t)gridDim.x * run) {
+    const uint32_t rows = (uint32_t)min((uint64_t)run, n - r0), units = rows * nb;
+    if (nb4 != nb)
+      for (uint32_t i = threadIdx.x; i < rows * nb4 / 4; i += 256) ((uint32_t*)se)[i] = 0x7f7f7f7fu;
+    __syncthreads();
+    for (uint32_t u0 = 0; u0 < units; u0 += U * (256 / G)) {
+      uint32_t row[U], blk[U];
+      uint4 raw[U];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t e = d + i;
-        if (e < dim) x[i] = load_value(r + (LANE && e < 16 * C ? (e % 16) * C + e / 16 : e));
+      for (int k = 0; k < U; ++k) {
+        const uint32_t u = u0 + k * (256 / G) + group;
+        row[k] = u / nb;
+        blk[k] = u - row[k] * nb;
+        const uint32_t d = blk[k] * kBlock + E * sub;
+        raw[k] = make_uint4(0, 0, 0, 0);
+        if (u < units) {
+          const T* r = in + (r0 + row[k]) * ld;
+          if (VEC && d + E <= dim) {
+            raw[k] = *(const uint4*)(r + d);
+          } else {
+            const uint32_t C = dim / 16;
+            T* x = (T*)&raw[k];
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+              const uint32_t e = d + i;
+              if (e < dim) x[i] = r[LANE && e < 16 * C ? (e % 16) * C + e / 16 : e];
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const uint32_t u = u0 + k * (256 / G) + group;
+        float x[E];
+        uint32_t top = 0;  // largest magnitude, as bits
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          x[i] = load_value((const T*)&raw[k] + i);
+          top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+        }
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const bool odd = top >= 0x7f800000u;  // infinities or NaN among them: the largest finite one, then
+        if (__any_sync(0xffffffffu, odd)) {
+          top = 0;
+#pragma unroll
+          for (int i = 0; i < E; ++i) {
+            const uint32_t a = __float_as_uint(x[i]) & 0x7fffffffu;
+            if (a < 0x7f800000u) top = max(top, a);
+          }
+#pragma unroll
+          for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        }
+        // 448 = 1.75 * 2^8: one exponent more when the mantissa is above 1.75
+        int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+        e = top == 0 ? 0 : max(e, -127);
+        const float inv = e == -127 ? 1.7014118346046923e38f : __uint_as_float((uint32_t)(127 - e) << 23);  // 2^-e
+        uint32_t word[E / 4];
+#pragma unroll
+        for (int i = 0; i < E; i += 4) {
+          const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[i] * inv, x[i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+          const uint32_t hi =
+              __nv_cvt_float2_to_fp8x2(make_float2(x[i + 2] * inv, x[i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+          word[i / 4] = lo | (hi << 16);
+        }
+        if (odd) {
+#pragma unroll
+          for (int i = 0; i < E; ++i)
+            if ((__float_as_uint(x[i]) & 0x7fffffffu) >= 0x7f800000u)
+              word[i / 4] = (word[i / 4] & ~(0xffu << (8 * (i % 4)))) | (0x7fu << (8 * (i % 4)));
+        }
+        if (u < units) {
+          const uint32_t d = blk[k] * kBlock + E * sub;
+          if (d < dim16) {
+            uint8_t* c = codes + (r0 + row[k]) * ld_codes + d;
+            if constexpr (E == 4)
+              *(uint32_t*)c = word[0];
+            else
+              *(uint2*)c = make_uint2(word[0], word[1]);
+          }
+          if (sub == 0) se[row[k] * nb4 + blk[k]] = (uint8_t)(e + 127);
+        }
       }
     }
-    uint32_t top = 0;  // largest finite magnitude, as bits
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t a = __float_as_uint(x[i]) & 0x7fffffffu;
-      if (a < 0x7f800000u) top = max(top, a);
+    __syncthreads();
+    const uint32_t per = nb4 / 4;
+    for (uint32_t i = threadIdx.x; i < rows * per; i += 256) {
+      const uint32_t r = i / per;
+      *(uint32_t*)(exps + (r0 + r) * ld_exps + 4 * (i - r * per)) = ((const uint32_t*)se)[i];
     }
-    top = __reduce_max_sync(0xffffffffu, top);
-    // 448 = 1.75 * 2^8: one exponent more when the mantissa is above 1.75
-    int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-    e = top == 0 ? 0 : max(e, -127);
-    const float inv = e == -127 ? 1.7014118346046923e38f : __uint_as_float((uint32_t)(127 - e) << 23);  // 2^-e
-    uint32_t word = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool finite = (__float_as_uint(x[i]) & 0x7fffffffu) < 0x7f800000u;
-      const uint32_t c = finite ? (uint32_t)__nv_cvt_float_to_fp8(x[i] * inv, __NV_SATFINITE, __NV_E4M3) : 0x7fu;
-      word |= c << (8 * i);
-    }
-    if (d < dim16) *(uint32_t*)(codes + row * ld_codes + d) = word;
-    if (lane == 0) exps[row * ld_exps + b] = (uint8_t)(e + 127);
-    if (b + 1 == nb && lane < (int)(nb4 - nb)) exps[row * ld_exps + nb + lane] = 127;
+    __syncthreads();
   }
 }
 
@@ -195,12 +241,19 @@ __global__ void __launch_bounds__(256) fp8_decode_kernel(const uint8_t* __restri
 template <typename T, bool LANE>
 cudaError_t launch_encode(const void* x, uint64_t n, uint32_t dim, uint64_t ld, uint8_t* codes, uint64_t ld_codes,
                           uint8_t* exps, uint64_t ld_exps, int sms, cudaStream_t st) {
-  const uint64_t units = n * ((dim + kBlock - 1) / kBlock);
-  const unsigned grid = (unsigned)std::min<uint64_t>((units + 7) / 8, (uint64_t)sms * 16);
-  const bool vec = !LANE && ld % 4 == 0 && aligned(x, 4 * sizeof(T));
+  // rows of a run: a multiple of 8 (their exponents fill whole sectors), one read
+  // of the CTA's threads and more, up to four while SMs keep several runs
+  const uint32_t nb = (dim + kBlock - 1) / kBlock, nb4 = (nb + 3) / 4 * 4;
+  const uint32_t once = 256 * 16 / (kBlock * (uint32_t)sizeof(T));  // blocks the threads read at once
+  uint32_t run = std::max(1u, once / nb);
+  if (run > 8 || n >= 8ull * sms) run = (run + 7) / 8 * 8;
+  while (run * nb < 4 * once && n / run > 8ull * sms) run *= 2;
+  run = std::min(run, kExpBytes / nb4);
+  const uint64_t grid = std::min<uint64_t>((n + run - 1) / run, (uint64_t)sms * 8);
+  const bool vec = !LANE && ld * sizeof(T) % 16 == 0 && aligned(x, 16);
   static Allowed none;
   return launch(vec ? fp8_encode_kernel<T, true, LANE> : fp8_encode_kernel<T, false, LANE>, grid, 256, 0, none, st,
-                (const T*)x, n, dim, ld, codes, ld_codes, exps, ld_exps);
+                (const T*)x, n, dim, ld, codes, ld_codes, exps, ld_exps, run);
 }
 
 int encode_rows(const void* x, int32_t type, uint64_t n, uint32_t dim, uint64_t ld, uint8_t* codes, uint64_t ld_codes,
@@ -592,11 +645,13 @@ int raven_topk_rows_device(const void* d_scores, int32_t type, uint64_t nq, uint
   p.vals = d_vals;
   p.ids = d_ids;
   p.counts = d_counts;
-  // A warp takes rows of up to 1024 scores, a CTA longer ones; where rows are
-  // too few to fill the GPU, each is split into parts of at least a tile.
-  // Ragged rows go by their mean.
+  // A warp takes a row when rows are short, or so many that warps fill the GPU
+  // and k is small (no barriers, and every warp's loads overlap the others' work:
+  // 10000 x 10007, k = 10, 94 us, by CTAs 120; 4096 x 6667, k = 100, 88 us, by CTAs
+  // 77: a warp's 32 maxima bound k = 100 loosely); else a CTA does. Where rows are too few to fill the
+  // GPU, each is split into parts of at least a tile. Ragged rows go by their mean.
   const uint64_t len = d_row_starts ? (n + nq - 1) / nq : n;
-  const bool warp = len <= 1024;
+  const bool warp = len <= 1024 || (nq >= 16ull * sms && k <= 32);
   const uint64_t tile = raven_topk::kCtaThreads * 16ull;
   uint64_t parts = 1;
   if (!warp && nq < 4ull * sms) parts = std::max<uint64_t>(1, std::min<uint64_t>((4ull * sms + nq - 1) / nq, len / tile));

@@ -7,8 +7,9 @@
 // team of threads (a warp for short rows, a CTA for long ones) streams its
 // part of a row once, a tile of 16 elements per thread at a time in registers,
 // and keeps the elements above a bound in shared memory:
-//   * first tile: the k-th best of the threads' own maxima is reached by at
-//     least k elements, so little more than k of the tile are kept;
+//   * first tile: the k-th best of the threads' own maxima (of their quarters'
+//     maxima, when k is above the threads) is reached by at least k elements,
+//     so little more than k of the tile are kept;
 //   * when many are kept, the k-th best of them is the new bound. A later
 //     element must beat it, since an equal one has a higher index.
 // Both k-th bests are found by one warp with the values in registers, a bit of
@@ -232,10 +233,15 @@ struct Keeper {
   // are higher than those of an earlier one. `more`: this is not the last.
   template <int E, typename Idx>
   __device__ void take(const uint32_t (&key)[E], bool more, Idx idx) {
+    static_assert(E % 4 == 0, "quarters");
     const uint32_t old = held;
-    uint32_t top = 0;
+    uint32_t top[4];  // best of each quarter
 #pragma unroll
-    for (int e = 0; e < E; ++e) top = max(top, key[e]);
+    for (int g = 0; g < 4; ++g) {
+      top[g] = key[g * (E / 4)];
+#pragma unroll
+      for (int e = 1; e < E / 4; ++e) top[g] = max(top[g], key[g * (E / 4) + e]);
+    }
     if (above == 0 && !few) bound(top);
     if (!push(key, top, idx)) {
       undo(old);
@@ -246,21 +252,40 @@ struct Keeper {
         return;
       }
     }
-    if (more && held > kPrune / 2) prune();
+    if (more && held > (TEAM == 32 ? 2 * k + 16 : kPrune / 2)) prune();  // the k-th best so far bounds the next tiles
   }
 
-  // Appends the keys over `above`; false if they do not fit. Exit is synchronised.
+  // Appends the keys over `above`; false if they do not fit. Exit is
+  // synchronised. In a warp's small tiles few pass, so a quarter that holds none
+  // is skipped; in a CTA's, one addition reserves a thread's places (the other
+  // way round each was slower by a fifth).
   template <int E, typename Idx>
-  __device__ bool push(const uint32_t (&key)[E], uint32_t top, Idx idx) {
-    if (top > above) {
+  __device__ bool push(const uint32_t (&key)[E], const uint32_t (&top)[4], Idx idx) {
+    const uint32_t best = max(max(top[0], top[1]), max(top[2], top[3]));
+    if constexpr (TEAM == 32) {
+      if (__any_sync(0xffffffffu, best > above)) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          if (!__any_sync(0xffffffffu, top[g] > above)) continue;
+#pragma unroll
+          for (int i = 0; i < E / 4; ++i) {
+            const int e = g * (E / 4) + i;
+            if (key[e] > above) {
+              const uint32_t at = atomicAdd(&s.count, 1u);
+              if (at < (uint32_t)TM::kBuf) s.buf[at] = ((uint64_t)key[e] << 32) | (uint32_t)~idx(e);
+            }
+          }
+        }
+      }
+    } else if (best > above) {
       uint32_t mine = 0;
 #pragma unroll
       for (int e = 0; e < E; ++e) mine += key[e] > above;
-      uint32_t p = atomicAdd(&s.count, mine);
-      if (p + mine <= (uint32_t)TM::kBuf) {
+      uint32_t at = atomicAdd(&s.count, mine);
+      if (at + mine <= (uint32_t)TM::kBuf) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
-          if (key[e] > above) s.buf[p++] = ((uint64_t)key[e] << 32) | (uint32_t)~idx(e);
+          if (key[e] > above) s.buf[at++] = ((uint64_t)key[e] << 32) | (uint32_t)~idx(e);
       }
     }
     TM::sync();
@@ -297,16 +322,20 @@ struct Keeper {
     if (held > k) sort();
   }
 
-  // A bound from the threads' maxima of a tile: k of them, so k elements, reach
-  // the k-th best of them.
-  __device__ void bound(uint32_t top) {
-    if (k > (uint32_t)TEAM) return;
+  // A bound from the maxima of a tile, one for each thread or, where those are
+  // too few, four: k of them, so k elements, reach the k-th best of them.
+  __device__ void bound(const uint32_t (&top)[4]) {
+    if (k > (uint32_t)TEAM && (TEAM > 32 || k > 128)) return;
     uint32_t t;
     if constexpr (TEAM == 32) {
-      const uint32_t v[1] = {top};
-      t = kth_of_warp(v, k, k / 4);
+      if (k <= 32) {
+        const uint32_t v[1] = {max(max(top[0], top[1]), max(top[2], top[3]))};
+        t = kth_of_warp(v, k, k / 4);
+      } else {
+        t = kth_of_warp(top, k, k / 8);
+      }
     } else {
-      s.top[tid] = top;
+      s.top[tid] = max(max(top[0], top[1]), max(top[2], top[3]));
       TM::sync();
       if (tid < 32) {
         uint32_t v[TEAM / 32];
@@ -348,7 +377,7 @@ __device__ inline void write_out(const Params& p, Keeper<TEAM>& kp, uint64_t row
 }
 
 template <typename T, int TEAM>
-__global__ void __launch_bounds__(kCtaThreads) topk_kernel(const Params p) {
+__global__ void __launch_bounds__(kCtaThreads, TEAM == 32 ? 3 : 4) topk_kernel(const Params p) {
   extern __shared__ __align__(16) uint8_t raw[];
   raven_score::after_previous();
   Shared<TEAM>* sh = (Shared<TEAM>*)raw + threadIdx.x / TEAM;
@@ -378,24 +407,35 @@ __global__ void __launch_bounds__(kCtaThreads) topk_kernel(const Params p) {
   const uint32_t skip = (uint32_t)(((uintptr_t)base & 15) / sizeof(T));
   const uint4* w = (const uint4*)((uintptr_t)base & ~(uintptr_t)15) + tid;
   const uint64_t end = to > from ? skip + (to - from) : 0;  // in elements from the boundary
-  for (uint64_t t = 0; t < end; t += kTile, w += TEAM * L::kPieces) {
-    uint32_t key[L::kE];
-    if ((t || !skip) && t + kTile <= end) {
-      uint4 v[L::kPieces];
+  uint4 v[L::kPieces];
+  auto load = [&](uint64_t t) {  // pieces of the tile at t that hold an element
+    const uint64_t left = t < end ? end - t : 0;
 #pragma unroll
-      for (int i = 0; i < L::kPieces; ++i) v[i] = __ldg(w + i * TEAM);
+    for (int i = 0; i < L::kPieces; ++i)
+      if ((uint64_t)(i * TEAM + tid) * L::kPer < left) v[i] = __ldg(w + i * TEAM);
+    w += TEAM * L::kPieces;
+  };
+  load(0);
+  for (uint64_t t = 0; t < end; t += kTile) {
+    uint32_t key[L::kE];
+    if (t + kTile <= end) {
 #pragma unroll
       for (int e = 0; e < L::kE; ++e) key[e] = key_of(L::get(v[e / L::kPer], e % L::kPer), p.mul, p.add);
     } else {
-      const uint32_t lo_ = t ? 0 : skip, hi_ = (uint32_t)min(end - t, (uint64_t)kTile);
+      const uint32_t hi = (uint32_t)(end - t);
 #pragma unroll
       for (int i = 0; i < L::kPieces; ++i) {
         const uint32_t e0 = (i * TEAM + tid) * L::kPer;
-        const uint4 v = e0 < hi_ ? __ldg(w + i * TEAM) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int c = 0; c < L::kPer; ++c)
-          key[i * L::kPer + c] = e0 + c >= lo_ && e0 + c < hi_ ? key_of(L::get(v, c), p.mul, p.add) : 0u;
+          key[i * L::kPer + c] = e0 + c < hi ? key_of(L::get(v[i], c), p.mul, p.add) : 0u;
       }
+    }
+    load(t + kTile);  // on its way while this tile is taken
+    if (t == 0 && tid == 0) {  // what lies before the first element
+#pragma unroll
+      for (int c = 0; c < L::kPer; ++c)
+        if (c < (int)skip) key[c] = 0;
     }
     const uint32_t i0 = (uint32_t)(from - skip + t) + tid * L::kPer;  // wraps where the element does not exist
     kp.take(key, t + kTile < end,
