@@ -17,10 +17,11 @@
 // N side up to BN rows (columns).
 //   rows    M = rows of v, N = queries: few queries cost the tensor cores and the
 //           shared memory little, and the 32 lanes of a warp write 32 consecutive
-//           scores of a query. For f32 scores, and for few queries.
+//           scores of a query. For few queries, and for f32 scores that start on
+//           sectors.
 //   pairs   M = queries, N = rows of v: a lane owns a query and reads its scores in
 //           order, so it packs them into whole 32-byte sectors of the output,
-//           wherever a query's scores start. For 16-bit scores of many queries.
+//           wherever a query's scores start.
 // One 128-byte swizzled row of shared memory is a block of 128 codes or 64
 // 16-bit values, so both types share one pipeline. Warp roles:
 //   warp 0      TMA: per K block the tile's rows and queries
@@ -353,6 +354,7 @@ __device__ inline void store_rows(T* out, const Tile& t, uint32_t qcnt, uint32_t
   free_acc(acc_empty, lane);
 }
 
+__device__ inline uint32_t word_of(const uint32_t (&v)[8], int i, const float*) { return v[i]; }
 __device__ inline uint32_t word_of(const uint32_t (&v)[16], int i, const __half*) {
   const __half2 h = __floats2half2_rn(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
   return *(const uint32_t*)&h;
@@ -362,21 +364,21 @@ __device__ inline uint32_t word_of(const uint32_t (&v)[16], int i, const __nv_bf
   return *(const uint32_t*)&h;
 }
 
-// Layout by pairs, 16-bit scores: a lane holds one query; four warps per lane
-// quadrant share the columns. A step makes one 32-byte sector (16 scores) of each
-// query. Where a query's scores start inside a sector (after `lead` others), the
-// sector is put together from the words of this step and the last: selects move
-// the pair of them by 8, 4, 2 and 1 words, a funnel shift by half a word. A warp
+// Layout by pairs: a lane holds one query; four warps per lane quadrant share the
+// columns. A step makes one 32-byte sector (8 words, SC scores) of each query.
+// Where a query's scores start inside a sector (after `lead` others), the sector
+// is put together from the words of this step and the last: selects move the
+// pair of them by 8, 4, 2 and 1 words, a funnel shift by half a word. A warp
 // writes the sectors that start among its own scores, and takes what the last
 // one needs from the columns after them (a tile computes that much of the next
 // one), so that only a query's first and last sectors are written in part:
-// 999 x 250007 scores took 460 us when every warp wrote its ends in part, and
+// 999 x 250007 bf16 scores took 460 us when every warp wrote its ends in part, and
 // 999 x 250000, where every sector is whole, 103. Halves of sectors are as bad
 // (2.1 TB/s for 16-byte stores alone, 4.9 for 32-byte ones).
 template <int BN, typename T>
 __device__ inline void store_pairs(T* out, const Tile& t, uint32_t qcnt, uint32_t acc, uint32_t warp, uint32_t lane,
                                    float alpha, const float* bias, uint32_t acc_empty) {
-  static_assert(sizeof(T) == 2, "16-bit scores");
+  constexpr uint32_t SC = 32 / sizeof(T);
   const uint32_t per = (t.vcnt + 63) / 64 * 16;  // columns per warp
   const uint32_t first = (warp >> 2) * per, q = (warp & 3) * 32 + lane;
   if ((warp & 3) * 32 >= qcnt || first >= t.vcnt) {
@@ -385,29 +387,29 @@ __device__ inline void store_pairs(T* out, const Tile& t, uint32_t qcnt, uint32_
   }
   const uint32_t cols = min(per, t.vcnt - first), avail = t.vext - first;
   const uint64_t start = (uint64_t)(uintptr_t)(out + t.out + (int64_t)q * t.ld + first);
-  const uint32_t lead = (uint32_t)(start & 31u) / 2;
-  const uint32_t shift = 16 - lead;  // scores from the last step's first to the sector's
+  const uint32_t lead = (uint32_t)(start & 31u) / sizeof(T);
+  const uint32_t shift = SC - lead;  // scores from the last step's first to the sector's
   const bool straight = !__any_sync(0xffffffffu, lead != 0);
-  const uint32_t steps = (cols + 15) / 16 + (straight ? 0 : 1);
+  const uint32_t steps = (cols + SC - 1) / SC + (straight ? 0 : 1);
   const uint32_t own = q < qcnt ? lead + cols : 0;                   // sectors from here on are another's
   const uint32_t from = t.first && first == 0 ? 0 : lead;            // and before here
   uint64_t sector = start & ~(uint64_t)31;
-  uint32_t v[16], x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  uint32_t v[SC], x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   tmem_ld(acc + first, v);
   for (uint32_t k = 0; k < steps; ++k, sector += 32) {
     tmem_wait_ld(v);
     uint32_t w[8];
     if (alpha != 1.0f || bias) {
 #pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) {
-        const uint32_t c = 16 * k + i;
+      for (uint32_t i = 0; i < SC; ++i) {
+        const uint32_t c = SC * k + i;
         v[i] = __float_as_uint(fmaf(alpha, __uint_as_float(v[i]), bias && c < avail ? __ldg(bias + first + c) : 0.0f));
       }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = word_of(v, i, (const T*)0);
     if (k + 1 < steps)
-      tmem_ld(acc + min(first + 16 * (k + 1), (uint32_t)BN - 16), v);  // the last may have no columns left, nor use for them
+      tmem_ld(acc + min(first + SC * (k + 1), (uint32_t)BN - SC), v);  // the last may have no columns left, nor use for them
     if (!straight) {
       uint32_t y[17];
 #pragma unroll
@@ -416,7 +418,7 @@ __device__ inline void store_pairs(T* out, const Tile& t, uint32_t qcnt, uint32_
         y[8 + i] = x[i] = w[i];
       }
       y[16] = 0;
-      const uint32_t by = shift >> 1;  // 0..8: 8 takes this step's words as they are
+      const uint32_t by = shift * sizeof(T) / 4;  // words, 0..8: 8 takes this step's words as they are
 #pragma unroll
       for (int i = 0; i < 9; ++i) y[i] = by & 8 ? y[i + 8] : y[i];
 #pragma unroll
@@ -426,19 +428,23 @@ __device__ inline void store_pairs(T* out, const Tile& t, uint32_t qcnt, uint32_
 #pragma unroll
       for (int i = 0; i < 9; ++i) y[i] = by & 1 ? y[i + 1] : y[i];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = __funnelshift_r(y[i], y[i + 1], (shift & 1) * 16);
+      for (int i = 0; i < 8; ++i) w[i] = sizeof(T) == 2 ? __funnelshift_r(y[i], y[i + 1], (shift & 1) * 16) : y[i];
     }
-    const uint32_t at = 16 * k;  // scores from the first sector's start
-    if (at >= lead && at < own && at + 16 <= lead + avail) {
+    const uint32_t at = SC * k;  // scores from the first sector's start
+    if (at >= lead && at < own && at + SC <= lead + avail) {
       asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(sector), "r"(w[0]), "r"(w[1]),
                    "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                    : "memory");
     } else if (at >= from && at < own) {  // a query's first or last sector
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) {
-        const uint32_t h = at + 2 * i;
-        if (h >= lead && h < lead + avail) *(uint16_t*)(sector + 4 * i) = (uint16_t)w[i];
-        if (h + 1 >= lead && h + 1 < lead + avail) *(uint16_t*)(sector + 4 * i + 2) = (uint16_t)(w[i] >> 16);
+        if constexpr (sizeof(T) == 4) {
+          if (at + i >= lead && at + i < lead + avail) *(uint32_t*)(sector + 4 * i) = w[i];
+        } else {
+          const uint32_t h = at + 2 * i;
+          if (h >= lead && h < lead + avail) *(uint16_t*)(sector + 4 * i) = (uint16_t)w[i];
+          if (h + 1 >= lead && h + 1 < lead + avail) *(uint16_t*)(sector + 4 * i + 2) = (uint16_t)(w[i] >> 16);
+        }
       }
     }
   }
@@ -682,7 +688,9 @@ __global__ void __launch_bounds__((Layout<FP8, BN, ROWS>::kThreads), 1)
         else
           store_rows<BN>((__nv_bfloat16*)p.out, t, qcnt, acc, w, lane, p.alpha, bias, acc_empty(b));
       } else {
-        if (p.out_type == kOutF16)
+        if (p.out_type == kOutF32)
+          store_pairs<BN>((float*)p.out, t, qcnt, acc, w, lane, p.alpha, bias, acc_empty(b));
+        else if (p.out_type == kOutF16)
           store_pairs<BN>((__half*)p.out, t, qcnt, acc, w, lane, p.alpha, bias, acc_empty(b));
         else
           store_pairs<BN>((__nv_bfloat16*)p.out, t, qcnt, acc, w, lane, p.alpha, bias, acc_empty(b));

@@ -310,7 +310,7 @@ struct Operands {
 };
 
 template <bool FP8, int BN, bool ROWS>
-cudaError_t launch_score(const Operands& o, raven_score::Params p, int sms, cudaStream_t st) {
+cudaError_t launch_score(const Operands& o, raven_score::Params p, bool whole, int sms, cudaStream_t st) {
   using L = raven_score::Layout<FP8, BN, ROWS>;
   CUtensorMap mq, mv;
   if (!rows_map(&mq, o.q->data, o.q->type, o.dim, o.q->rows, o.q->ld, ROWS ? raven_score::kQBox : raven_score::kBM) ||
@@ -328,31 +328,39 @@ cudaError_t launch_score(const Operands& o, raven_score::Params p, int sms, cuda
   };
   while (subs > 1 && (tiles(subs) < 4ull * sms || (p.qo && subs * L::kTileV > 2 * per))) subs /= 2;
   p.subs = (uint32_t)subs;
-  const bool whole = !p.qo && (uintptr_t)p.out % 32 == 0 && p.ld % 16 == 0;  // every query starts on a sector
   p.halo = ROWS || whole ? 0 : 16;
   const uint64_t grid = p.qo ? (uint64_t)sms : std::min<uint64_t>(tiles(subs), (uint64_t)sms);
   static Allowed allowed;
   return launch(raven_score::score_kernel<FP8, BN, ROWS>, grid, L::kThreads, L::kBytes, allowed, st, mq, mv, p);
 }
 
-// `want`: queries of a group, twice the mean where groups differ. The layout by
-// rows of v for f32 scores and up to 64 queries, its N side as wide as those need
-// and no wider than leaves every SM a tile. 16-bit scores of more queries: the
-// layout by pairs (in f32 its lanes, a query each, wrote 1024 x 250000 scores in
-// 385 us, the other in 223: 32 queries a megabyte apart are as many pages).
+// `want`: queries of a group, twice the mean where groups differ. Up to 64: the
+// layout by rows of v. More: by pairs, whose sectors are whole wherever a query's
+// scores start (785 x 132491 f32 99 us, by rows 167; 999 x 250007 bf16 152, 271),
+// except
+//   f32 scores that all start on sectors: by rows, a warp writes whole lines;
+//   queries 1.5 MB apart and more: a lane of the layout by pairs comes back to
+//   its query's page for every sector, and the pages of 128 queries are too many
+//   (100 x 1000003 f32 323 us, by rows 131).
+// The N side is as wide as the queries need and no wider than leaves SMs a tile.
+constexpr uint64_t kFar = 3 << 19;
+
 template <bool FP8>
 cudaError_t dispatch_score(const Operands& o, const raven_score::Params& p, int sms, cudaStream_t st) {
   const uint64_t want = p.qo ? 2 * ((p.nq + p.groups - 1) / p.groups) : p.nq;
-  if (want > 64 && p.out_type != raven_score::kOutF32) {
+  const uint64_t size = p.out_type == raven_score::kOutF32 ? 4 : 2;
+  const bool whole = !p.qo && (uintptr_t)p.out % 32 == 0 && p.ld * size % 32 == 0;  // every query starts on a sector
+  const bool far = !p.qo && p.ld * size >= kFar;
+  if (want > 64 && !(whole && size == 4) && !far) {
     if (!p.qo && (p.nq + 127) / 128 * ((p.n + 223) / 224) < (uint64_t)sms)
-      return launch_score<FP8, 96, false>(o, p, sms, st);
-    return launch_score<FP8, 224, false>(o, p, sms, st);
+      return launch_score<FP8, 96, false>(o, p, whole, sms, st);
+    return launch_score<FP8, 224, false>(o, p, whole, sms, st);
   }
   const uint64_t vt = (p.n + raven_score::kBM - 1) / raven_score::kBM;
   auto fills = [&](uint64_t bn) { return p.qo || vt * ((p.nq + bn - 1) / bn) >= (uint64_t)sms; };
-  if (want > 64 && fills(192)) return launch_score<FP8, 192, true>(o, p, sms, st);
-  if (want > 32 && fills(64)) return launch_score<FP8, 64, true>(o, p, sms, st);
-  return launch_score<FP8, 32, true>(o, p, sms, st);
+  if (want > 64 && fills(192)) return launch_score<FP8, 192, true>(o, p, whole, sms, st);
+  if (want > 32 && fills(64)) return launch_score<FP8, 64, true>(o, p, whole, sms, st);
+  return launch_score<FP8, 32, true>(o, p, whole, sms, st);
 }
 
 int check_rows(const raven_rows* r, uint32_t dim, const char* what) {
@@ -512,20 +520,26 @@ __global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* __restri
 // ---------------------------------------------------------------------------
 // Top-k of rows.
 // ---------------------------------------------------------------------------
-template <typename T, int TEAM>
+template <typename T, int TEAM, bool BIG>
 cudaError_t launch_topk(const raven_topk::Params& p, cudaStream_t st) {
-  using TM = raven_topk::Team<TEAM>;
-  const uint32_t smem = TM::kTeams * (uint32_t)sizeof(raven_topk::Shared<TEAM>);
+  using TM = raven_topk::Team<TEAM, BIG>;
+  const uint32_t smem = TM::kTeams * (uint32_t)sizeof(raven_topk::Shared<TEAM, BIG>);
   const uint64_t units = p.nq * p.parts;
   static Allowed allowed;
-  return launch(raven_topk::topk_kernel<T, TEAM>, (units + TM::kTeams - 1) / TM::kTeams, raven_topk::kCtaThreads, smem,
-                allowed, st, p);
+  return launch(raven_topk::topk_kernel<T, TEAM, BIG>, (units + TM::kTeams - 1) / TM::kTeams, raven_topk::kCtaThreads,
+                smem, allowed, st, p);
 }
-template <int TEAM>
+template <int TEAM, bool BIG>
 cudaError_t dispatch_topk(int32_t type, const raven_topk::Params& p, cudaStream_t st) {
-  return type == RAVEN_TYPE_F32   ? launch_topk<float, TEAM>(p, st)
-         : type == RAVEN_TYPE_F16 ? launch_topk<__half, TEAM>(p, st)
-                                  : launch_topk<__nv_bfloat16, TEAM>(p, st);
+  return type == RAVEN_TYPE_F32   ? launch_topk<float, TEAM, BIG>(p, st)
+         : type == RAVEN_TYPE_F16 ? launch_topk<__half, TEAM, BIG>(p, st)
+                                  : launch_topk<__nv_bfloat16, TEAM, BIG>(p, st);
+}
+template <bool BIG>
+cudaError_t launch_join(const raven_topk::Params& p, cudaStream_t st) {
+  static Allowed none;
+  return launch(raven_topk::topk_join_kernel<BIG>, p.nq, raven_topk::kCtaThreads,
+                (uint32_t)sizeof(raven_topk::Shared<raven_topk::kCtaThreads, BIG>), none, st, p);
 }
 
 }  // namespace
@@ -661,15 +675,17 @@ int raven_topk_rows_device(const void* d_scores, int32_t type, uint64_t nq, uint
     CU(cudaMallocAsync((void**)&tmp, nq * parts * k * 8, st));
     p.lists = tmp;
   }
-  cudaError_t e = warp ? dispatch_topk<32>(type, p, st) : dispatch_topk<raven_topk::kCtaThreads>(type, p, st);
+  constexpr int kCta = raven_topk::kCtaThreads;
+  const bool big = 2 * k > (uint32_t)kCta;
+  cudaError_t e = warp  ? dispatch_topk<32, false>(type, p, st)
+                  : big ? dispatch_topk<kCta, true>(type, p, st)
+                        : dispatch_topk<kCta, false>(type, p, st);
   if (e == cudaSuccess && parts > 1) {
     raven_topk::Params j = p;
     j.x = tmp;
     j.n = parts * k;
     j.parts = 1;
-    static Allowed none;
-    e = launch(raven_topk::topk_join_kernel, nq, raven_topk::kCtaThreads,
-               (uint32_t)sizeof(raven_topk::Shared<raven_topk::kCtaThreads>), none, st, j);
+    e = big ? launch_join<true>(j, st) : launch_join<false>(j, st);
   }
   if (tmp) cudaFreeAsync(tmp, st);
   if (e != cudaSuccess) return fail(RAVEN_ECUDA, std::string("topk: ") + cudaGetErrorString(e));

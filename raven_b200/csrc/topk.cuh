@@ -7,14 +7,13 @@
 // team of threads (a warp for short rows, a CTA for long ones) streams its
 // part of a row once, a tile of 16 elements per thread at a time in registers,
 // and keeps the elements above a bound in shared memory:
-//   * first tile: the k-th best of the threads' own maxima (of their quarters'
-//     maxima, when k is above the threads) is reached by at least k elements,
-//     so little more than k of the tile are kept;
+//   * first tile: the k-th best of the threads' own maxima is reached by at
+//     least k elements, so little more than k of the tile are kept;
 //   * when many are kept, the k-th best of them is the new bound. A later
 //     element must beat it, since an equal one has a higher index.
 // Both k-th bests are found by one warp with the values in registers, a bit of
-// the key at a time from the highest one in which they differ. At the end the
-// few left over are ordered by counting. A tile whose survivors do not fit
+// the key at a time from the highest one in which they differ. At the end one
+// warp orders the few left over in registers. A tile whose survivors do not fit
 // (rising data, equal scores) is taken again slice by slice, pruned in between:
 // slower, with the same result. Few long rows are split into parts over the
 // GPU; the parts' lists are joined by the same code.
@@ -65,7 +64,10 @@ __device__ inline float value_of(uint32_t key, uint32_t mul, uint32_t add) {
   return key < kWorst ? __int_as_float(0x7fc00000) : __uint_as_float((up & 0x80000000u) ? up & 0x7fffffffu : ~up);
 }
 
-template <int TEAM>
+// BIG: k above half of a CTA's threads, whose least maximum bounds nothing; the
+// bound is then found among their quarters' maxima. A kernel of its own: the
+// registers that takes cost the others a fifth.
+template <int TEAM, bool BIG>
 struct Team {
   static constexpr int kBuf = TEAM == 32 ? 1024 : 2048;
   static constexpr int kTeams = kCtaThreads / TEAM;
@@ -76,10 +78,10 @@ struct Team {
       __syncthreads();
   }
 };
-template <int TEAM>
+template <int TEAM, bool BIG>
 struct Shared {
-  uint64_t buf[Team<TEAM>::kBuf];
-  uint32_t top[TEAM];
+  uint64_t buf[Team<TEAM, BIG>::kBuf];
+  uint32_t top[TEAM == 32 ? 1 : BIG ? 4 * TEAM : TEAM];
   uint32_t count;
   uint32_t bound;
 };
@@ -131,19 +133,53 @@ __device__ inline uint32_t kth_of_warp(const uint32_t (&v)[N], uint32_t k, uint3
   return t;
 }
 
-template <int TEAM>
+// By one warp: v (element 32 i + lane in v[i]) in descending order. A bitonic sort
+// of 32 N entries with 5 exchanges between lanes for each power of two above 32
+// and none through memory: 100 entries cost 600 instructions of one warp, where
+// counting each one's place among the others cost 1800.
+template <int N>
+__device__ inline void sort_of_warp(uint64_t (&v)[N], uint32_t lane) {
+#pragma unroll
+  for (uint32_t w = 2; w <= 32 * N; w <<= 1)
+#pragma unroll
+    for (uint32_t h = w >> 1; h > 0; h >>= 1) {
+      if (h >= 32) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int j = i ^ (int)(h / 32);
+          if (j > i) {
+            const bool down = (((uint32_t)i * 32) & w) == 0;  // w > 32 here
+            const uint64_t a = v[i], b = v[j];
+            const bool swap = (a < b) == down;
+            v[i] = swap ? b : a;
+            v[j] = swap ? a : b;
+          }
+        }
+      } else {
+        const bool low = (lane & h) == 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const bool down = (((uint32_t)i * 32 + lane) & w) == 0;
+          const uint64_t a = v[i], b = __shfl_xor_sync(0xffffffffu, a, h);
+          v[i] = (a < b) == (low == down) ? b : a;
+        }
+      }
+    }
+}
+
+template <int TEAM, bool BIG>
 struct Keeper {
-  using TM = Team<TEAM>;
+  using TM = Team<TEAM, BIG>;
   static constexpr uint32_t kPrune = 1024;  // entries that one warp prunes
   static constexpr uint32_t kFew = 128;     // rows up to here need no bound
-  static_assert(kPrune <= (uint32_t)TM::kBuf && 2 * kMaxK <= kPrune / 2, "sizes");
-  Shared<TEAM>& s;
+  static_assert(kPrune <= (uint32_t)TM::kBuf && kMaxK <= 256, "sizes");
+  Shared<TEAM, BIG>& s;
   uint32_t tid, k;
   uint32_t above = 0;   // only keys over it can matter
   uint32_t held = 0;    // entries in the buffer (= s.count between calls)
   bool few;
 
-  __device__ Keeper(Shared<TEAM>& s_, uint32_t tid_, uint32_t k_, uint64_t n) : s(s_), tid(tid_), k(k_), few(n <= kFew) {
+  __device__ Keeper(Shared<TEAM, BIG>& s_, uint32_t tid_, uint32_t k_, uint64_t n) : s(s_), tid(tid_), k(k_), few(n <= kFew) {
     if (tid == 0) s.count = 0;
     TM::sync();
   }
@@ -212,28 +248,39 @@ struct Keeper {
     if (c >= k) above = max(above, (uint32_t)(s.buf[k - 1] >> 32));
   }
 
-  // The best k in order, at s.buf + the value returned.
-  __device__ uint32_t finish() {
-    if (held > k + 32) prune();
-    if (held > kPrune / 2) sort();
-    const uint32_t c = held;  // at most kPrune / 2: the other half takes the ordered ones
-    for (uint32_t e = tid; e < c; e += TEAM) {
-      const uint64_t own = s.buf[e];
-      uint32_t at = 0;
-#pragma unroll 4
-      for (uint32_t j = 0; j < c; ++j) at += s.buf[j] > own;
-      if (at < k) s.buf[kPrune / 2 + at] = own;
+  // The best k in order, at the front of the buffer.
+  __device__ void finish() {
+    if (held > 256) prune();
+    if (held > 256) sort();  // many equals
+    if (tid < 32) {
+      if (held <= 32)
+        order<1>();
+      else if (held <= 64)
+        order<2>();
+      else if (held <= 128)
+        order<4>();
+      else
+        order<8>();
     }
-    held = min(c, k);
+    held = min(held, k);
     TM::sync();
-    return kPrune / 2;
+  }
+  template <int N>
+  __device__ void order() {
+    uint64_t v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = tid + 32 * i < held ? s.buf[tid + 32 * i] : 0;
+    sort_of_warp(v, tid);
+#pragma unroll
+    for (int i = 0; i < N; ++i) s.buf[tid + 32 * i] = v[i];  // the warp has read what it writes over
   }
 
-  // Takes a tile: key[e] (0: none) with index idx(e). Indexes of a later tile
-  // are higher than those of an earlier one. `more`: this is not the last.
-  template <int E, typename Idx>
-  __device__ void take(const uint32_t (&key)[E], bool more, Idx idx) {
-    static_assert(E % 4 == 0, "quarters");
+  // Takes a tile: key[e] (0: none) with index idx(e), and again(e) the key from
+  // where it came. Indexes of a later tile are higher than those of an earlier
+  // one. `more`: this is not the last.
+  template <int E, typename Idx, typename Again>
+  __device__ void take(const uint32_t (&key)[E], bool more, Idx idx, Again again) {
+    static_assert(E % 4 == 0 && E <= 32, "quarters, bits");
     const uint32_t old = held;
     uint32_t top[4];  // best of each quarter
 #pragma unroll
@@ -242,11 +289,11 @@ struct Keeper {
 #pragma unroll
       for (int e = 1; e < E / 4; ++e) top[g] = max(top[g], key[g * (E / 4) + e]);
     }
-    if (above == 0 && !few) bound(top);
-    if (!push(key, top, idx)) {
+    if (above == 0 && !few) bound(key, top);
+    if (!push(key, top, idx, again)) {
       undo(old);
-      bound(top);  // now from this tile
-      if (!push(key, top, idx)) {
+      bound(key, top);  // now from this tile
+      if (!push(key, top, idx, again)) {
         undo(old);
         slices(key, idx);
         return;
@@ -256,36 +303,32 @@ struct Keeper {
   }
 
   // Appends the keys over `above`; false if they do not fit. Exit is
-  // synchronised. In a warp's small tiles few pass, so a quarter that holds none
-  // is skipped; in a CTA's, one addition reserves a thread's places (the other
-  // way round each was slower by a fifth).
-  template <int E, typename Idx>
-  __device__ bool push(const uint32_t (&key)[E], const uint32_t (&top)[4], Idx idx) {
-    const uint32_t best = max(max(top[0], top[1]), max(top[2], top[3]));
-    if constexpr (TEAM == 32) {
-      if (__any_sync(0xffffffffu, best > above)) {
+  // synchronised. In a warp's tiles few pass: a thread marks its own and fetches
+  // those again. In a CTA's tiles, with as many as k of them and 64 registers, it
+  // walks its keys (either way round each was slower by a tenth to a fifth).
+  template <int E, typename Idx, typename Again>
+  __device__ bool push(const uint32_t (&key)[E], const uint32_t (&top)[4], Idx idx, Again again) {
+    if (max(max(top[0], top[1]), max(top[2], top[3])) > above) {
+      if constexpr (TEAM == 32) {
+        uint32_t mine = 0;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          if (!__any_sync(0xffffffffu, top[g] > above)) continue;
-#pragma unroll
-          for (int i = 0; i < E / 4; ++i) {
-            const int e = g * (E / 4) + i;
-            if (key[e] > above) {
-              const uint32_t at = atomicAdd(&s.count, 1u);
-              if (at < (uint32_t)TM::kBuf) s.buf[at] = ((uint64_t)key[e] << 32) | (uint32_t)~idx(e);
-            }
+        for (int e = 0; e < E; ++e) mine |= key[e] > above ? 1u << e : 0u;
+        uint32_t at = atomicAdd(&s.count, (uint32_t)__popc(mine));
+        if (at + __popc(mine) <= (uint32_t)TM::kBuf)
+          for (; mine; mine &= mine - 1) {
+            const int e = __ffs(mine) - 1;
+            s.buf[at++] = ((uint64_t)again(e) << 32) | (uint32_t)~idx(e);
           }
+      } else {
+        uint32_t mine = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) mine += key[e] > above;
+        uint32_t at = atomicAdd(&s.count, mine);
+        if (at + mine <= (uint32_t)TM::kBuf) {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (key[e] > above) s.buf[at++] = ((uint64_t)key[e] << 32) | (uint32_t)~idx(e);
         }
-      }
-    } else if (best > above) {
-      uint32_t mine = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) mine += key[e] > above;
-      uint32_t at = atomicAdd(&s.count, mine);
-      if (at + mine <= (uint32_t)TM::kBuf) {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (key[e] > above) s.buf[at++] = ((uint64_t)key[e] << 32) | (uint32_t)~idx(e);
       }
     }
     TM::sync();
@@ -322,25 +365,32 @@ struct Keeper {
     if (held > k) sort();
   }
 
-  // A bound from the maxima of a tile, one for each thread or, where those are
-  // too few, four: k of them, so k elements, reach the k-th best of them.
-  __device__ void bound(const uint32_t (&top)[4]) {
-    if (k > (uint32_t)TEAM && (TEAM > 32 || k > 128)) return;
+  // A bound from a tile: the k-th best of its threads' maxima, which k of them
+  // and so k elements reach; where k is above a warp's threads, of its elements.
+  template <int E>
+  __device__ void bound(const uint32_t (&key)[E], const uint32_t (&top)[4]) {
+    if (k > (uint32_t)TEAM && TEAM > 32) return;
     uint32_t t;
     if constexpr (TEAM == 32) {
       if (k <= 32) {
         const uint32_t v[1] = {max(max(top[0], top[1]), max(top[2], top[3]))};
         t = kth_of_warp(v, k, k / 4);
       } else {
-        t = kth_of_warp(top, k, k / 8);
+        t = kth_of_warp(key, k, k / 8);
       }
     } else {
-      s.top[tid] = max(max(top[0], top[1]), max(top[2], top[3]));
+      constexpr int PER = BIG ? 4 : 1;
+      if constexpr (BIG) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.top[tid + i * TEAM] = top[i];
+      } else {
+        s.top[tid] = max(max(top[0], top[1]), max(top[2], top[3]));
+      }
       TM::sync();
       if (tid < 32) {
-        uint32_t v[TEAM / 32];
+        uint32_t v[PER * TEAM / 32];
 #pragma unroll
-        for (int i = 0; i < TEAM / 32; ++i) v[i] = s.top[tid + 32 * i];
+        for (int i = 0; i < PER * TEAM / 32; ++i) v[i] = s.top[tid + 32 * i];
         t = kth_of_warp(v, k, k / 4);
         if (tid == 0) s.bound = t;
       }
@@ -352,9 +402,10 @@ struct Keeper {
   }
 };
 
-template <int TEAM>
-__device__ inline void write_out(const Params& p, Keeper<TEAM>& kp, uint64_t row, uint32_t part, uint32_t parts) {
-  const uint64_t* best = kp.s.buf + kp.finish();
+template <int TEAM, bool BIG>
+__device__ inline void write_out(const Params& p, Keeper<TEAM, BIG>& kp, uint64_t row, uint32_t part, uint32_t parts) {
+  kp.finish();
+  const uint64_t* best = kp.s.buf;
   const uint32_t c = kp.held;
   if (parts > 1) {
     uint64_t* o = p.lists + (row * parts + part) * p.k;
@@ -376,13 +427,13 @@ __device__ inline void write_out(const Params& p, Keeper<TEAM>& kp, uint64_t row
   if (p.counts && kp.tid == 0) p.counts[row] = c;
 }
 
-template <typename T, int TEAM>
+template <typename T, int TEAM, bool BIG>
 __global__ void __launch_bounds__(kCtaThreads, TEAM == 32 ? 3 : 4) topk_kernel(const Params p) {
   extern __shared__ __align__(16) uint8_t raw[];
   raven_score::after_previous();
-  Shared<TEAM>* sh = (Shared<TEAM>*)raw + threadIdx.x / TEAM;
+  Shared<TEAM, BIG>* sh = (Shared<TEAM, BIG>*)raw + threadIdx.x / TEAM;
   const uint32_t tid = threadIdx.x % TEAM;
-  const uint64_t unit = (uint64_t)blockIdx.x * Team<TEAM>::kTeams + threadIdx.x / TEAM;
+  const uint64_t unit = (uint64_t)blockIdx.x * Team<TEAM, BIG>::kTeams + threadIdx.x / TEAM;
   const uint64_t row = unit / p.parts;
   if (row >= p.nq) return;  // a whole team
   const uint32_t part = (uint32_t)(unit - row * p.parts);
@@ -400,7 +451,7 @@ __global__ void __launch_bounds__(kCtaThreads, TEAM == 32 ? 3 : 4) topk_kernel(c
   uint64_t each = len;
   if (p.parts > 1) each = ((len + p.parts - 1) / p.parts + kTile + L::kPer - 1) / kTile * kTile - L::kPer;
   const uint64_t from = min(len, each * part), to = min(len, from + each);
-  Keeper<TEAM> kp(*sh, tid, p.k, to - from);
+  Keeper<TEAM, BIG> kp(*sh, tid, p.k, to - from);
   // pieces of 16 bytes from the boundary at or before the first element: the
   // bytes around a row are in the same 16 as some of its own
   const uint8_t* base = (const uint8_t*)p.x + (lo + from) * sizeof(T);
@@ -438,32 +489,38 @@ __global__ void __launch_bounds__(kCtaThreads, TEAM == 32 ? 3 : 4) topk_kernel(c
         if (c < (int)skip) key[c] = 0;
     }
     const uint32_t i0 = (uint32_t)(from - skip + t) + tid * L::kPer;  // wraps where the element does not exist
-    kp.take(key, t + kTile < end,
-            [&](int e) { return i0 + (uint32_t)((e / L::kPer) * TEAM * L::kPer + e % L::kPer); });
+    const T* x0 = (const T*)((uintptr_t)base & ~(uintptr_t)15) + t + tid * L::kPer;
+    auto place = [&](int e) { return (uint32_t)((e / L::kPer) * TEAM * L::kPer + e % L::kPer); };
+    kp.take(
+        key, t + kTile < end, [&](int e) { return i0 + place(e); },
+        [&](int e) { return key_of((float)x0[place(e)], p.mul, p.add); });
   }
-  write_out<TEAM>(p, kp, row, part, p.parts);
+  write_out(p, kp, row, part, p.parts);
 }
 
 // Joins a row's lists (p.x: [nq][n] entries, n = lists x k).
+template <bool BIG>
 __global__ void __launch_bounds__(kCtaThreads) topk_join_kernel(const Params p) {
   constexpr int TEAM = kCtaThreads, E = 8;
   extern __shared__ __align__(16) uint8_t raw[];
   raven_score::after_previous();
   const uint64_t row = blockIdx.x;
-  Keeper<TEAM> kp(*(Shared<TEAM>*)raw, threadIdx.x, p.k, p.n);
+  Keeper<TEAM, BIG> kp(*(Shared<TEAM, BIG>*)raw, threadIdx.x, p.k, p.n);
   const uint64_t* x = (const uint64_t*)p.x + row * p.n;
   for (uint64_t t = 0; t < p.n; t += (uint64_t)TEAM * E) {
-    uint32_t key[E], id[E];
+    uint32_t key[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const uint64_t at = t + (uint64_t)e * TEAM + threadIdx.x;
       const uint64_t v = at < p.n ? x[at] : 0;
       key[e] = (uint32_t)(v >> 32);
-      id[e] = ~(uint32_t)v;
     }
-    kp.take(key, t + (uint64_t)TEAM * E < p.n, [&](int e) { return id[e]; });
+    auto again = [&](int e) { return x[t + (uint64_t)e * TEAM + threadIdx.x]; };
+    kp.take(
+        key, t + (uint64_t)TEAM * E < p.n, [&](int e) { return ~(uint32_t)again(e); },
+        [&](int e) { return (uint32_t)(again(e) >> 32); });
   }
-  write_out<TEAM>(p, kp, row, 0, 1);
+  write_out(p, kp, row, 0, 1);
 }
 
 }  // namespace raven_topk
