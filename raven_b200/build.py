@@ -18,7 +18,7 @@ LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libraven_gpu.so")
 
 SOURCES = ["raven_gpu.cu", "scoring.cu", "host_index.cpp"]
-DEPS = SOURCES + ["search_kernel.cuh", "search_cta.cuh", "knn_tc.cuh", "score_tc.cuh", "topk.cuh", "internal.h",
+DEPS = SOURCES + ["search_kernel.cuh", "search_cta.cuh", "knn_tc.cuh", "score_tc.cuh", "topk.cuh", "fp8.cuh", "internal.h",
                   "host_index.h"]
 
 

@@ -3,7 +3,6 @@
 // grouped, score_tc.cuh) and the best k of each row of scores (topk.cuh).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 #include <nvtx3/nvToolsExt.h>
 
 #include <algorithm>
@@ -11,6 +10,7 @@
 #include <mutex>
 
 #include "../../include/raven_gpu.h"
+#include "fp8.cuh"
 #include "internal.h"
 #include "score_tc.cuh"
 #include "topk.cuh"
@@ -112,9 +112,7 @@ cudaError_t launch(void (*kern)(K...), uint64_t grid, int threads, uint32_t smem
 // has four such reads under way: bound by memory, 30000 x 768 f16 in 14 us
 // (4.9 TB/s), where one read of 8 bytes a lane at a time took 31.
 // ---------------------------------------------------------------------------
-__device__ inline float load_value(const float* p) { return *p; }
-__device__ inline float load_value(const __half* p) { return __half2float(*p); }
-__device__ inline float load_value(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+using raven_fp8::load_value;
 
 // A CTA takes a run of rows and gathers their exponents in shared memory: single
 // bytes of a 32-byte sector written at different times cost a read each.
@@ -184,24 +182,11 @@ __global__ void __launch_bounds__(256) fp8_encode_kernel(const T* __restrict__ i
 #pragma unroll
           for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         }
-        // 448 = 1.75 * 2^8: one exponent more when the mantissa is above 1.75
-        int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-        e = top == 0 ? 0 : max(e, -127);
-        const float inv = e == -127 ? 1.7014118346046923e38f : __uint_as_float((uint32_t)(127 - e) << 23);  // 2^-e
+        const int e = raven_fp8::exponent_of(top);
+        const float inv = raven_fp8::inverse_of(e);
         uint32_t word[E / 4];
 #pragma unroll
-        for (int i = 0; i < E; i += 4) {
-          const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[i] * inv, x[i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-          const uint32_t hi =
-              __nv_cvt_float2_to_fp8x2(make_float2(x[i + 2] * inv, x[i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-          word[i / 4] = lo | (hi << 16);
-        }
-        if (odd) {
-#pragma unroll
-          for (int i = 0; i < E; ++i)
-            if ((__float_as_uint(x[i]) & 0x7fffffffu) >= 0x7f800000u)
-              word[i / 4] = (word[i / 4] & ~(0xffu << (8 * (i % 4)))) | (0x7fu << (8 * (i % 4)));
-        }
+        for (int i = 0; i < E; i += 4) word[i / 4] = raven_fp8::codes_of(x + i, inv);
         if (u < units) {
           const uint32_t d = blk[k] * kBlock + E * sub;
           if (d < dim16) {
@@ -309,11 +294,12 @@ struct Operands {
   uint32_t dim;
 };
 
-template <bool FP8, int BN, bool ROWS>
+template <bool FP8, int BN, bool ROWS, bool HELD = false>
 cudaError_t launch_score(const Operands& o, raven_score::Params p, bool whole, int sms, cudaStream_t st) {
-  using L = raven_score::Layout<FP8, BN, ROWS>;
-  CUtensorMap mq, mv;
-  if (!rows_map(&mq, o.q->data, o.q->type, o.dim, o.q->rows, o.q->ld, ROWS ? raven_score::kQBox : raven_score::kBM) ||
+  using L = raven_score::Layout<FP8, BN, ROWS, HELD>;
+  CUtensorMap mq{}, mv;
+  if ((!HELD &&
+       !rows_map(&mq, o.q->data, o.q->type, o.dim, o.q->rows, o.q->ld, ROWS ? raven_score::kQBox : raven_score::kBM)) ||
       !rows_map(&mv, o.v->data, o.v->type, o.dim, o.v->rows, o.v->ld, ROWS ? raven_score::kBM : BN))
     return cudaErrorInvalidValue;
   // Rows per tile, where M is the rows. A tile of few queries has little to do
@@ -331,7 +317,7 @@ cudaError_t launch_score(const Operands& o, raven_score::Params p, bool whole, i
   p.halo = ROWS || whole ? 0 : 16;
   const uint64_t grid = p.qo ? (uint64_t)sms : std::min<uint64_t>(tiles(subs), (uint64_t)sms);
   static Allowed allowed;
-  return launch(raven_score::score_kernel<FP8, BN, ROWS>, grid, L::kThreads, L::kBytes, allowed, st, mq, mv, p);
+  return launch(raven_score::score_kernel<FP8, BN, ROWS, HELD>, grid, L::kThreads, L::kBytes, allowed, st, mq, mv, p);
 }
 
 // `want`: queries of a group, twice the mean where groups differ. Up to 64: the
@@ -356,6 +342,8 @@ cudaError_t dispatch_score(const Operands& o, const raven_score::Params& p, int 
       return launch_score<FP8, 96, false>(o, p, whole, sms, st);
     return launch_score<FP8, 224, false>(o, p, whole, sms, st);
   }
+  if constexpr (FP8)
+    if (p.qx) return launch_score<FP8, 32, true, true>(o, p, whole, sms, st);
   const uint64_t vt = (p.n + raven_score::kBM - 1) / raven_score::kBM;
   auto fills = [&](uint64_t bn) { return p.qo || vt * ((p.nq + bn - 1) / bn) >= (uint64_t)sms; };
   if (want > 64 && fills(192)) return launch_score<FP8, 192, true>(o, p, whole, sms, st);
@@ -427,7 +415,13 @@ int run_scores(const raven_rows* q, const int64_t* qo, const raven_rows* v, cons
 
   raven_rows qq = *q;
   uint8_t* tmp = nullptr;
-  if (encode) {  // the queries' codes live until the product is done, in stream order
+  if (encode && !qo && q->rows <= 32 && p.nkb <= raven_score::kHeldBlocks && q->rows * p.nkb <= raven_score::kHeldUnits) {
+    p.qx = q->data;  // every CTA encodes them for itself
+    p.q_type = q->type == RAVEN_TYPE_F32 ? raven_score::kOutF32
+               : q->type == RAVEN_TYPE_F16 ? raven_score::kOutF16 : raven_score::kOutBf16;
+    p.dim = dim;
+    p.ld_qx = q->ld;
+  } else if (encode) {  // the queries' codes live until the product is done, in stream order
     qq.type = RAVEN_TYPE_FP8;
     qq.ld = codes_pitch(dim);
     qq.ld_exps = exps_pitch(dim);

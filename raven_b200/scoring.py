@@ -93,19 +93,23 @@ class Fp8Rows:
     def __init__(self, codes: torch.Tensor, exps: torch.Tensor, dim: int):
         if dim < 1:
             raise ValueError("dim must be at least 1")
-        pitch = []
-        for name, t, least in (("codes", codes, _up(dim, 16)), ("exps", exps, _up(-(-dim // BLOCK), 4))):
-            if t.dtype != torch.uint8 or t.dim() != 2 or not t.is_cuda or t.stride(1) != 1:
-                raise ValueError(f"{name} must be a 2-D uint8 tensor on a GPU, each row's bytes side by side")
-            if t.shape[1] < least:
-                raise ValueError(f"{name} must have at least {least} columns for dim {dim}, got {t.shape[1]}")
-            pitch.append(_pitch(t))
-        n = codes.shape[0]
+        if codes.dim() != 2 or exps.dim() != 2 or codes.dtype != torch.uint8 or exps.dtype != torch.uint8 or \
+                not codes.is_cuda:
+            raise ValueError("codes and exps must be 2-D uint8 tensors on a GPU")
+        (n, wide), (pitch, step) = codes.shape, codes.stride()
+        (en, ewide), (epitch, estep) = exps.shape, exps.stride()
+        if step != 1 or estep != 1:
+            raise ValueError("codes and exps must hold each row's bytes side by side")
+        if wide < -(-dim // 16) * 16 or ewide < -(-dim // 512) * 4:
+            raise ValueError(f"dim {dim} needs {_up(dim, 16)} columns of codes and {_up(-(-dim // BLOCK), 4)} of exps, "
+                             f"got {wide} and {ewide}")
         self.device_index = codes.get_device()
-        if exps.shape[0] != n or exps.get_device() != self.device_index:
+        if en != n or exps.get_device() != self.device_index:
             raise ValueError("codes and exps must have the same rows and device")
+        if n == 1:  # one row may come with any pitch
+            pitch, epitch = max(pitch, wide), max(epitch, ewide)
         self.codes, self.exps, self.dim = codes, exps, dim
-        self._rows = L.Rows(codes.data_ptr(), exps.data_ptr(), n, pitch[0], pitch[1], L.RAVEN_TYPE_FP8)
+        self._rows = L.Rows(codes.data_ptr(), exps.data_ptr(), n, pitch, epitch, L.RAVEN_TYPE_FP8)
 
     @property
     def device(self) -> torch.device:
