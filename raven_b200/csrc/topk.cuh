@@ -250,7 +250,7 @@ struct Keeper {
 
   // The best k in order, at the front of the buffer.
   __device__ void finish() {
-    if (held > 256) prune();
+    if (held > 256 || (held > 128 && k <= 128)) prune();  // half the entries cost less than half to order
     if (held > 256) sort();  // many equals
     if (tid < 32) {
       if (held <= 32)
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(kCtaThreads, TEAM == 32 ? 3 : 4) topk_kernel(c
   Shared<TEAM, BIG>* sh = (Shared<TEAM, BIG>*)raw + threadIdx.x / TEAM;
   const uint32_t tid = threadIdx.x % TEAM;
   const uint64_t unit = (uint64_t)blockIdx.x * Team<TEAM, BIG>::kTeams + threadIdx.x / TEAM;
-  const uint64_t row = unit / p.parts;
+  const uint64_t row = p.parts == 1 ? unit : unit / p.parts;
   if (row >= p.nq) return;  // a whole team
   const uint32_t part = (uint32_t)(unit - row * p.parts);
   uint64_t lo = row * p.ld, len = p.n;
@@ -477,9 +477,14 @@ __global__ void __launch_bounds__(kCtaThreads, TEAM == 32 ? 3 : 4) topk_kernel(c
 #pragma unroll
       for (int i = 0; i < L::kPieces; ++i) {
         const uint32_t e0 = (i * TEAM + tid) * L::kPer;
+        if (e0 + L::kPer <= hi) {
 #pragma unroll
-        for (int c = 0; c < L::kPer; ++c)
-          key[i * L::kPer + c] = e0 + c < hi ? key_of(L::get(v[i], c), p.mul, p.add) : 0u;
+          for (int c = 0; c < L::kPer; ++c) key[i * L::kPer + c] = key_of(L::get(v[i], c), p.mul, p.add);
+        } else {
+#pragma unroll
+          for (int c = 0; c < L::kPer; ++c)
+            key[i * L::kPer + c] = e0 + c < hi ? key_of(L::get(v[i], c), p.mul, p.add) : 0u;
+        }
       }
     }
     load(t + kTile);  // on its way while this tile is taken

@@ -325,7 +325,7 @@ def top_k(scores: torch.Tensor, k: int, *, largest: bool = True,
         if scores.dim() != 1 or not scores.is_contiguous():
             raise ValueError("packed scores must be a contiguous 1-D tensor")
         nq, n, ld, starts = _offsets("row_starts", row_starts, index), scores.numel(), 0, row_starts.data_ptr()
-    vals = torch.empty((nq, max(k, 0)), dtype=scores.dtype, device=device)
+    vals = scores.new_empty((nq, max(k, 0)))
     ids = torch.empty((nq, max(k, 0)), dtype=torch.int32, device=device)
     counts = torch.empty(nq, dtype=torch.int32, device=device)
     _call(index, L.load().raven_topk_rows_device, scores.data_ptr(), _TYPES[scores.dtype], nq, n, ld, starts, k,
