@@ -24,11 +24,14 @@ __device__ inline float inverse_of(int e) {
   return e == -127 ? 1.7014118346046923e38f : __uint_as_float((uint32_t)(127 - e) << 23);
 }
 __device__ inline bool odd_value(float x) { return (__float_as_uint(x) & 0x7fffffffu) >= 0x7f800000u; }  // infinite or NaN
-// Four codes, the first lowest, rounded to nearest even; the NaN code for what is not finite.
+// Four codes, the first lowest, rounded to nearest even.
 __device__ inline uint32_t codes_of(const float* x, float inv) {
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * inv, x[1] * inv), __NV_SATFINITE, __NV_E4M3);
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2] * inv, x[3] * inv), __NV_SATFINITE, __NV_E4M3);
-  uint32_t w = lo | (hi << 16);
+  return lo | (hi << 16);
+}
+// The same with the NaN code for what is not finite (the conversion saturates infinities).
+__device__ inline uint32_t with_nan(uint32_t w, const float* x) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (odd_value(x[i])) w = (w & ~(0xffu << (8 * i))) | (0x7fu << (8 * i));

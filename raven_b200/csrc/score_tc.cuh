@@ -120,7 +120,12 @@ template <bool FP8, int BN, bool ROWS, bool HELD>
 struct Layout {
   static_assert(!HELD || (FP8 && ROWS && BN == 32), "one box of queries");
   static constexpr uint32_t kHeld = HELD ? kHeldBlocks * BN * 128 : 0;
-  static constexpr uint32_t kStage = kABytes + (HELD ? 0 : BN * 128);
+  // K blocks per stage: with few queries a block is so little work that handing
+  // it over took longer (256 groups of FP8, 32 x 1024 x 512 on average: 37.6 us with
+  // one block, 34.5 with two)
+  static constexpr uint32_t kPer = ROWS && BN <= 64 ? 2 : 1;
+  static constexpr uint32_t kBlockBytes = kABytes + (HELD ? 0 : BN * 128);
+  static constexpr uint32_t kStage = kPer * kBlockBytes;
   static constexpr int kStages = (int)((200u * 1024 - kHeld) / kStage);
   static constexpr int kEpiWarps = ROWS ? 8 : 16;
   static constexpr int kThreads = 32 * (4 + kEpiWarps + (FP8 ? 4 : 0));
@@ -489,7 +494,7 @@ __device__ inline void hold_queries(const Params& p, uint8_t* held, uint8_t* exp
       if (a < 0x7f800000u) top = max(top, a);
     }
     const int e = raven_fp8::exponent_of(__reduce_max_sync(0xffffffffu, top));
-    const uint32_t word = raven_fp8::codes_of(x[k], raven_fp8::inverse_of(e));
+    const uint32_t word = raven_fp8::with_nan(raven_fp8::codes_of(x[k], raven_fp8::inverse_of(e)), x[k]);
     *(uint32_t*)(held + b * (32 * 128) + row * 128 + ((lane / 4) ^ (row & 7)) * 16 + (lane % 4) * 4) = word;
     if (lane == 0) exps[row * kHeldBlocks + b] = (uint8_t)(e + 127);
   }
@@ -573,24 +578,31 @@ __global__ void __launch_bounds__((Layout<FP8, BN, ROWS, HELD>::kThreads), 1)
       if (qcnt == 0) break;
       const uint32_t boxes = (qcnt + kQBox - 1) / kQBox;  // (rows)
       for (uint32_t sub = 0; sub * L::kTileV < vcnt && ok; ++sub)
-        for (uint32_t kb = 0; kb < p.nkb; ++kb) {
+        for (uint32_t kb = 0; kb < p.nkb; kb += L::kPer) {
           if (!warp_wait(empty(s), ph ^ 1u)) {
             ok = false;
             break;
           }
           if (elect_one()) {
-            const uint32_t a = sbase + s * L::kStage, bar = full(s);
-            const int x = (int)(kb * (FP8 ? 128u : 64u));
-            if constexpr (ROWS) {
-              mbar_expect_tx(bar, kABytes + (HELD ? 0 : boxes * (kQBox * 128)));
-              tma_load_2d(a, &tm_v, x, (int)(vrow + sub * kBM), bar);
-              if constexpr (!HELD)
-                for (uint32_t b = 0; b < boxes; ++b)
-                  tma_load_2d(a + kABytes + b * (kQBox * 128), &tm_q, x, (int)(qrow + b * kQBox), bar);
-            } else {
-              mbar_expect_tx(bar, L::kStage);
-              tma_load_2d(a, &tm_q, x, (int)qrow, bar);
-              tma_load_2d(a + kABytes, &tm_v, x, (int)vrow, bar);
+            const uint32_t bar = full(s), blocks = min(L::kPer, p.nkb - kb);
+            if constexpr (ROWS)
+              mbar_expect_tx(bar, blocks * (kABytes + (HELD ? 0 : boxes * (kQBox * 128))));
+            else
+              mbar_expect_tx(bar, blocks * L::kBlockBytes);
+#pragma unroll
+            for (uint32_t j = 0; j < L::kPer; ++j) {
+              if (j >= blocks) break;
+              const uint32_t a = sbase + s * L::kStage + j * L::kBlockBytes;
+              const int x = (int)((kb + j) * (FP8 ? 128u : 64u));
+              if constexpr (ROWS) {
+                tma_load_2d(a, &tm_v, x, (int)(vrow + sub * kBM), bar);
+                if constexpr (!HELD)
+                  for (uint32_t b = 0; b < boxes; ++b)
+                    tma_load_2d(a + kABytes + b * (kQBox * 128), &tm_q, x, (int)(qrow + b * kQBox), bar);
+              } else {
+                tma_load_2d(a, &tm_q, x, (int)qrow, bar);
+                tma_load_2d(a + kABytes, &tm_v, x, (int)vrow, bar);
+              }
             }
           }
           __syncwarp();
@@ -628,7 +640,7 @@ __global__ void __launch_bounds__((Layout<FP8, BN, ROWS, HELD>::kThreads), 1)
       for (uint32_t sub = 0; sub * L::kTileV < vcnt && ok; ++sub) {
         const uint32_t d = tmem + b * L::kAccBuf + sub * BN;
         const bool last_sub = (sub + 1) * L::kTileV >= vcnt;
-        for (uint32_t kb = 0; kb < p.nkb; ++kb) {
+        for (uint32_t kb = 0; kb < p.nkb; kb += L::kPer) {
           if (FP8 && (kb & 3u) == 0 && !warp_wait(sf_full(f), fph)) {
             ok = false;
             break;
@@ -637,30 +649,34 @@ __global__ void __launch_bounds__((Layout<FP8, BN, ROWS, HELD>::kThreads), 1)
             ok = false;
             break;
           }
-          const uint32_t a = sbase + s * L::kStage, done = empty(s);
-          const uint64_t da = sw128_desc(a), db = sw128_desc(HELD ? held_at + kb * (BN * 128) : a + kABytes);
-          const bool last = kb + 1 == p.nkb;
-          const bool sf_done = FP8 && ((kb & 3u) == 3u || last);
-          const uint32_t steps = last ? p.last_k : 4u;
-          const uint32_t sel = kb & 3u;
+          const uint32_t a0 = sbase + s * L::kStage, done = empty(s);
+          const bool last = kb + L::kPer >= p.nkb;
+          const bool sf_done = FP8 && ((kb & 3u) == 4u - L::kPer || last);
           const uint32_t sf = tmem + L::kAcc + f * kSfCols;
           if (++s == S) {
             s = 0;
             ph ^= 1u;
           }
           if (elect_one()) {
-            if (FP8 && sel == 0) {  // in order before the MMAs that read them
+            if (FP8 && (kb & 3u) == 0) {  // in order before the MMAs that read them
               const uint32_t e = sbase + L::kExps + f * L::kExpBuf;
 #pragma unroll
               for (int j = 0; j < 1 + (BN + 127) / 128; ++j) copy_exps(sf + 4 * j, e + j * kSfBytes);
             }
 #pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) {  // 32 bytes along the swizzled row
-              if (k >= steps) break;
-              if constexpr (FP8)
-                mma_mxf8(d, da + 2 * k, db + 2 * k, idesc | (sel << 4) | (sel << 29), sf, sf + 4, (kb | k) != 0u);
-              else
-                mma_f16(d, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0u);
+            for (uint32_t j = 0; j < L::kPer; ++j) {
+              if (kb + j >= p.nkb) break;
+              const uint32_t a = a0 + j * L::kBlockBytes;
+              const uint64_t da = sw128_desc(a), db = sw128_desc(HELD ? held_at + (kb + j) * (BN * 128) : a + kABytes);
+              const uint32_t steps = kb + j + 1 == p.nkb ? p.last_k : 4u, sel = (kb + j) & 3u;
+#pragma unroll
+              for (uint32_t k = 0; k < 4; ++k) {  // 32 bytes along the swizzled row
+                if (k >= steps) break;
+                if constexpr (FP8)
+                  mma_mxf8(d, da + 2 * k, db + 2 * k, idesc | (sel << 4) | (sel << 29), sf, sf + 4, (kb | j | k) != 0u);
+                else
+                  mma_f16(d, da + 2 * k, db + 2 * k, idesc, (kb | j | k) != 0u);
+              }
             }
             mma_commit(done);
             if (sf_done) mma_commit(sf_empty(f));

@@ -108,9 +108,10 @@ cudaError_t launch(void (*kern)(K...), uint64_t grid, int threads, uint32_t smem
 // e4m3(x * 2^-e) to nearest even, exponent byte = e + 127. A power of two
 // scales exactly, so the only rounding is e4m3's own (half a step, 2^-4 of the
 // value; 2^-10 * 2^e below the type's normal range).
-// A block is read by 32 lanes (f32) or 16 (16-bit), 16 bytes each, and each warp
-// has four such reads under way: bound by memory, 30000 x 768 f16 in 14 us
-// (4.9 TB/s), where one read of 8 bytes a lane at a time took 31.
+// A block is read by 32 lanes (f32) or 16 (16-bit), 16 bytes each, and a warp has
+// two such reads under way (30000 x 768 f16 17 us, 4.0 TB/s, 1000000 x 128 f32 139 us,
+// 4.6; four, with half the warps, were
+// slower, and 8 bytes a lane, one read at a time, took half as long again).
 // ---------------------------------------------------------------------------
 using raven_fp8::load_value;
 
@@ -121,10 +122,10 @@ using raven_fp8::load_value;
 constexpr uint32_t kExpBytes = 4096;  // of a run: rows x blocks padded to 4
 
 template <typename T, bool VEC, bool LANE>
-__global__ void __launch_bounds__(256) fp8_encode_kernel(const T* __restrict__ in, uint64_t n, uint32_t dim, uint64_t ld,
+__global__ void __launch_bounds__(256, 8) fp8_encode_kernel(const T* __restrict__ in, uint64_t n, uint32_t dim, uint64_t ld,
                                                          uint8_t* __restrict__ codes, uint64_t ld_codes,
                                                          uint8_t* __restrict__ exps, uint64_t ld_exps, uint32_t run) {
-  constexpr int E = 16 / sizeof(T), G = (int)kBlock / E, U = 4;  // values per lane, lanes per block, blocks under way
+  constexpr int E = 16 / sizeof(T), G = (int)kBlock / E, U = 2;  // values per lane, lanes per block, blocks under way
   __shared__ __align__(16) uint8_t se[kExpBytes];
   after_previous();
   const uint32_t sub = threadIdx.x % G, group = threadIdx.x / G;
@@ -171,8 +172,8 @@ __global__ void __launch_bounds__(256) fp8_encode_kernel(const T* __restrict__ i
         }
 #pragma unroll
         for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const bool odd = top >= 0x7f800000u;  // infinities or NaN among them: the largest finite one, then
-        if (__any_sync(0xffffffffu, odd)) {
+        const bool odd = __any_sync(0xffffffffu, top >= 0x7f800000u);  // infinities or NaN: the largest finite one, then
+        if (odd) {
           top = 0;
 #pragma unroll
           for (int i = 0; i < E; ++i) {
@@ -186,7 +187,10 @@ __global__ void __launch_bounds__(256) fp8_encode_kernel(const T* __restrict__ i
         const float inv = raven_fp8::inverse_of(e);
         uint32_t word[E / 4];
 #pragma unroll
-        for (int i = 0; i < E; i += 4) word[i / 4] = raven_fp8::codes_of(x + i, inv);
+        for (int i = 0; i < E; i += 4) {
+          word[i / 4] = raven_fp8::codes_of(x + i, inv);
+          if (odd) word[i / 4] = raven_fp8::with_nan(word[i / 4], x + i);
+        }
         if (u < units) {
           const uint32_t d = blk[k] * kBlock + E * sub;
           if (d < dim16) {
@@ -234,7 +238,7 @@ cudaError_t launch_encode(const void* x, uint64_t n, uint32_t dim, uint64_t ld, 
   if (run > 8 || n >= 8ull * sms) run = (run + 7) / 8 * 8;
   while (run * nb < 4 * once && n / run > 8ull * sms) run *= 2;
   run = std::min(run, kExpBytes / nb4);
-  const uint64_t grid = std::min<uint64_t>((n + run - 1) / run, (uint64_t)sms * 8);
+  const uint64_t grid = std::min<uint64_t>((n + run - 1) / run, (uint64_t)sms * 64);
   const bool vec = !LANE && ld * sizeof(T) % 16 == 0 && aligned(x, 16);
   static Allowed none;
   return launch(vec ? fp8_encode_kernel<T, true, LANE> : fp8_encode_kernel<T, false, LANE>, grid, 256, 0, none, st,
