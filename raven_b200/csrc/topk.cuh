@@ -11,6 +11,8 @@
 //     least k elements, so little more than k of the tile are kept;
 //   * when many are kept, the k-th best of them is the new bound. A later
 //     element must beat it, since an equal one has a higher index.
+// Once there is a bound, a tile costs one minimum or maximum per score (one for two
+// 16-bit ones) and one comparison per thread: keys are made only for what passes.
 // Both k-th bests are found by one warp with the values in registers, a bit of
 // the key at a time from the highest one in which they differ. At the end one
 // warp orders the few left over in registers. A tile whose survivors do not fit
@@ -24,6 +26,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "internal.h"
 
@@ -102,6 +105,41 @@ struct Loader {
     }
   }
 };
+
+// The best score of a thread's pieces, NaN ignored (all NaN: the worst infinity).
+__device__ inline float best_of(const uint4 (&v)[4], bool largest, const float*) {
+  const uint32_t* u = (const uint32_t*)v;
+  float m = largest ? -__int_as_float(0x7f800000) : __int_as_float(0x7f800000);
+  if (largest) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) m = fmaxf(m, __uint_as_float(u[e]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) m = fminf(m, __uint_as_float(u[e]));
+  }
+  return m;
+}
+template <typename H2, typename H>
+__device__ inline float best_of_pairs(const uint4 (&v)[2], bool largest, uint32_t worst) {
+  const uint32_t* u = (const uint32_t*)v;
+  H2 m = *(const H2*)&worst;
+  if (largest) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = __hmax2(m, *(const H2*)&u[e]);
+    m.x = __hmax(m.x, m.y);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = __hmin2(m, *(const H2*)&u[e]);
+    m.x = __hmin(m.x, m.y);
+  }
+  return (float)m.x;
+}
+__device__ inline float best_of(const uint4 (&v)[2], bool largest, const __half*) {
+  return best_of_pairs<__half2, __half>(v, largest, largest ? 0xfc00fc00u : 0x7c007c00u);
+}
+__device__ inline float best_of(const uint4 (&v)[2], bool largest, const __nv_bfloat16*) {
+  return best_of_pairs<__nv_bfloat162, __nv_bfloat16>(v, largest, largest ? 0xff80ff80u : 0x7f807f80u);
+}
 
 // By one warp, N values per lane (0: none): the largest T that at least k of
 // them reach, 0 if fewer than k are there. `slack`: a T that is reached by up to
@@ -192,7 +230,9 @@ struct Keeper {
     }
     if (tid < 32) {
       uint32_t t;
-      if (held <= kPrune / 4)
+      if (held <= 64)
+        t = kth_of_held<2>();
+      else if (held <= kPrune / 4)
         t = kth_of_held<kPrune / 128>();
       else
         t = kth_of_held<kPrune / 32>();
@@ -275,6 +315,60 @@ struct Keeper {
     for (int i = 0; i < N; ++i) s.buf[tid + 32 * i] = v[i];  // the warp has read what it writes over
   }
 
+  // Takes a tile as it was loaded, elements that do not exist being the worst
+  // infinity. key(e): the key of an element in registers, 0 if it does not exist.
+  template <typename T, int P, typename Key, typename Idx, typename Again>
+  __device__ void take_raw(const uint4 (&v)[P], bool more, uint32_t mul, uint32_t add, Key key, Idx idx, Again again) {
+    constexpr int E = Loader<T>::kE;
+    const bool largest = mul == 1u;
+    const float best = best_of(v, largest, (const T*)0);
+    if constexpr (!BIG)
+      if (above == 0 && !few && (TEAM > 32 || k <= 32)) bound_of(key_of(best, mul, add));
+    // a bound over the worst infinity excludes NaN, as comparisons do
+    if (above >= kWorst) {
+      // the least value over the bound; no value is over the best infinity
+      const float least = above == 0xffffffffu ? __int_as_float(0x7fc00000) : value_of(above + 1, mul, add);
+      const uint32_t old = held;
+      if (largest ? best >= least : best <= least) {
+        uint32_t mine = 0;
+        if (largest) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) mine |= Loader<T>::get(v[e / Loader<T>::kPer], e % Loader<T>::kPer) >= least ? 1u << e : 0u;
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) mine |= Loader<T>::get(v[e / Loader<T>::kPer], e % Loader<T>::kPer) <= least ? 1u << e : 0u;
+        }
+        append(mine, idx, again);
+      }
+      if (appended()) {
+        if (more && held > (TEAM == 32 ? 2 * k + 16 : kPrune / 2)) prune();  // the k-th best so far bounds the next tiles
+        return;
+      }
+      undo(old);
+    }
+    uint32_t keys[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) keys[e] = key(e);
+    take(keys, more, idx, again);
+  }
+  // Appends the marked elements of a thread, if they fit.
+  template <typename Idx, typename Again>
+  __device__ void append(uint32_t mine, Idx idx, Again again) {
+    uint32_t at = atomicAdd(&s.count, (uint32_t)__popc(mine));
+    if (at + __popc(mine) <= (uint32_t)TM::kBuf)
+      for (; mine; mine &= mine - 1) {
+        const int e = __ffs(mine) - 1;
+        s.buf[at++] = ((uint64_t)again(e) << 32) | (uint32_t)~idx(e);
+      }
+  }
+  // Synchronises, and whether all fitted.
+  __device__ bool appended() {
+    TM::sync();
+    held = s.count;
+    TM::sync();  // read by all before the next append
+    return held <= (uint32_t)TM::kBuf;
+  }
+
   // Takes a tile: key[e] (0: none) with index idx(e), and again(e) the key from
   // where it came. Indexes of a later tile are higher than those of an earlier
   // one. `more`: this is not the last.
@@ -302,39 +396,16 @@ struct Keeper {
     if (more && held > (TEAM == 32 ? 2 * k + 16 : kPrune / 2)) prune();  // the k-th best so far bounds the next tiles
   }
 
-  // Appends the keys over `above`; false if they do not fit. Exit is
-  // synchronised. In a warp's tiles few pass: a thread marks its own and fetches
-  // those again. In a CTA's tiles, with as many as k of them and 64 registers, it
-  // walks its keys (either way round each was slower by a tenth to a fifth).
+  // Appends the keys over `above`; false if they do not fit. Exit is synchronised.
   template <int E, typename Idx, typename Again>
   __device__ bool push(const uint32_t (&key)[E], const uint32_t (&top)[4], Idx idx, Again again) {
     if (max(max(top[0], top[1]), max(top[2], top[3])) > above) {
-      if constexpr (TEAM == 32) {
-        uint32_t mine = 0;
+      uint32_t mine = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) mine |= key[e] > above ? 1u << e : 0u;
-        uint32_t at = atomicAdd(&s.count, (uint32_t)__popc(mine));
-        if (at + __popc(mine) <= (uint32_t)TM::kBuf)
-          for (; mine; mine &= mine - 1) {
-            const int e = __ffs(mine) - 1;
-            s.buf[at++] = ((uint64_t)again(e) << 32) | (uint32_t)~idx(e);
-          }
-      } else {
-        uint32_t mine = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) mine += key[e] > above;
-        uint32_t at = atomicAdd(&s.count, mine);
-        if (at + mine <= (uint32_t)TM::kBuf) {
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (key[e] > above) s.buf[at++] = ((uint64_t)key[e] << 32) | (uint32_t)~idx(e);
-        }
-      }
+      for (int e = 0; e < E; ++e) mine |= key[e] > above ? 1u << e : 0u;
+      append(mine, idx, again);
     }
-    TM::sync();
-    held = s.count;
-    TM::sync();  // read by all before the next append
-    return held <= (uint32_t)TM::kBuf;
+    return appended();
   }
   __device__ void undo(uint32_t old) {
     held = old;
@@ -369,36 +440,46 @@ struct Keeper {
   // and so k elements reach; where k is above a warp's threads, of its elements.
   template <int E>
   __device__ void bound(const uint32_t (&key)[E], const uint32_t (&top)[4]) {
-    if (k > (uint32_t)TEAM && TEAM > 32) return;
-    uint32_t t;
-    if constexpr (TEAM == 32) {
-      if (k <= 32) {
-        const uint32_t v[1] = {max(max(top[0], top[1]), max(top[2], top[3]))};
-        t = kth_of_warp(v, k, k / 4);
-      } else {
-        t = kth_of_warp(key, k, k / 8);
-      }
+    if constexpr (BIG) {
+      if (k > (uint32_t)TEAM) return;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s.top[tid + i * TEAM] = top[i];
+      TM::sync();
+      bound_of_tops<4>();
+    } else if (TEAM == 32 && k > 32) {
+      const uint32_t t = kth_of_warp(key, k, k / 8);
+      if (t > 1) above = max(above, t - 1);
     } else {
-      constexpr int PER = BIG ? 4 : 1;
-      if constexpr (BIG) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s.top[tid + i * TEAM] = top[i];
-      } else {
-        s.top[tid] = max(max(top[0], top[1]), max(top[2], top[3]));
-      }
-      TM::sync();
-      if (tid < 32) {
-        uint32_t v[PER * TEAM / 32];
-#pragma unroll
-        for (int i = 0; i < PER * TEAM / 32; ++i) v[i] = s.top[tid + 32 * i];
-        t = kth_of_warp(v, k, k / 4);
-        if (tid == 0) s.bound = t;
-      }
-      TM::sync();
-      t = s.bound;
-      TM::sync();
+      bound_of(max(max(top[0], top[1]), max(top[2], top[3])));
     }
-    if (t > 1) above = max(above, t - 1);
+  }
+  // The same from each thread's best key.
+  __device__ void bound_of(uint32_t top) {
+    if constexpr (TEAM == 32) {
+      const uint32_t v[1] = {top};
+      const uint32_t t = kth_of_warp(v, k, k / 4);
+      if (t > kWorst) above = max(above, t - 1);
+    } else {
+      if (k > (uint32_t)TEAM) return;
+      s.top[tid] = top;
+      TM::sync();
+      bound_of_tops<1>();
+    }
+  }
+  template <int PER>
+  __device__ void bound_of_tops() {
+    if (tid < 32) {
+      uint32_t v[PER * TEAM / 32];
+#pragma unroll
+      for (int i = 0; i < PER * TEAM / 32; ++i) v[i] = s.top[tid + 32 * i];
+      const uint32_t t = kth_of_warp(v, k, k / 4);
+      if (tid == 0) s.bound = t;
+    }
+    TM::sync();
+    const uint32_t t = s.bound;
+    TM::sync();
+    // not among NaN or the worst infinity: a thread without a number counts as that
+    if (t > kWorst) above = max(above, t - 1);
   }
 };
 
@@ -458,46 +539,52 @@ __global__ void __launch_bounds__(kCtaThreads, TEAM == 32 ? 3 : 4) topk_kernel(c
   const uint32_t skip = (uint32_t)(((uintptr_t)base & 15) / sizeof(T));
   const uint4* w = (const uint4*)((uintptr_t)base & ~(uintptr_t)15) + tid;
   const uint64_t end = to > from ? skip + (to - from) : 0;  // in elements from the boundary
-  uint4 v[L::kPieces];
+  // the worst infinity, for what does not exist
+  const uint32_t inf = sizeof(T) == 4                            ? 0x7f800000u
+                       : std::is_same<T, __half>::value ? 0x7c007c00u
+                                                        : 0x7f807f80u;
+  const uint32_t none = p.mul == 1u ? inf | (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : inf;
+  uint4 v[L::kPieces], ahead[L::kPieces];
   auto load = [&](uint64_t t) {  // pieces of the tile at t that hold an element
-    const uint64_t left = t < end ? end - t : 0;
+    if (t + kTile <= end) {
 #pragma unroll
-    for (int i = 0; i < L::kPieces; ++i)
-      if ((uint64_t)(i * TEAM + tid) * L::kPer < left) v[i] = __ldg(w + i * TEAM);
+      for (int i = 0; i < L::kPieces; ++i) ahead[i] = __ldg(w + i * TEAM);
+    } else {
+      const uint32_t left = t < end ? (uint32_t)(end - t) : 0;
+#pragma unroll
+      for (int i = 0; i < L::kPieces; ++i)
+        ahead[i] = (i * TEAM + tid) * L::kPer < left ? __ldg(w + i * TEAM) : make_uint4(none, none, none, none);
+    }
     w += TEAM * L::kPieces;
   };
   load(0);
   for (uint64_t t = 0; t < end; t += kTile) {
-    uint32_t key[L::kE];
-    if (t + kTile <= end) {
+    const uint32_t lo_ = t ? 0 : skip, hi_ = (uint32_t)min(end - t, (uint64_t)kTile);  // elements of the tile that exist
 #pragma unroll
-      for (int e = 0; e < L::kE; ++e) key[e] = key_of(L::get(v[e / L::kPer], e % L::kPer), p.mul, p.add);
-    } else {
-      const uint32_t hi = (uint32_t)(end - t);
+    for (int i = 0; i < L::kPieces; ++i) v[i] = ahead[i];
+    if (lo_ || hi_ < kTile) {  // pieces at the row's edges
 #pragma unroll
       for (int i = 0; i < L::kPieces; ++i) {
         const uint32_t e0 = (i * TEAM + tid) * L::kPer;
-        if (e0 + L::kPer <= hi) {
-#pragma unroll
-          for (int c = 0; c < L::kPer; ++c) key[i * L::kPer + c] = key_of(L::get(v[i], c), p.mul, p.add);
-        } else {
+        if (e0 < lo_ || (e0 < hi_ && e0 + L::kPer > hi_)) {
+          T* x = (T*)&v[i];
 #pragma unroll
           for (int c = 0; c < L::kPer; ++c)
-            key[i * L::kPer + c] = e0 + c < hi ? key_of(L::get(v[i], c), p.mul, p.add) : 0u;
+            if (e0 + c < lo_ || e0 + c >= hi_) x[c] = *(const T*)&none;
         }
       }
     }
     load(t + kTile);  // on its way while this tile is taken
-    if (t == 0 && tid == 0) {  // what lies before the first element
-#pragma unroll
-      for (int c = 0; c < L::kPer; ++c)
-        if (c < (int)skip) key[c] = 0;
-    }
     const uint32_t i0 = (uint32_t)(from - skip + t) + tid * L::kPer;  // wraps where the element does not exist
     const T* x0 = (const T*)((uintptr_t)base & ~(uintptr_t)15) + t + tid * L::kPer;
     auto place = [&](int e) { return (uint32_t)((e / L::kPer) * TEAM * L::kPer + e % L::kPer); };
-    kp.take(
-        key, t + kTile < end, [&](int e) { return i0 + place(e); },
+    kp.template take_raw<T>(
+        v, t + kTile < end, p.mul, p.add,
+        [&](int e) {
+          const uint32_t at = tid * L::kPer + place(e);
+          return at >= lo_ && at < hi_ ? key_of(L::get(v[e / L::kPer], e % L::kPer), p.mul, p.add) : 0u;
+        },
+        [&](int e) { return i0 + place(e); },
         [&](int e) { return key_of((float)x0[place(e)], p.mul, p.add); });
   }
   write_out(p, kp, row, part, p.parts);
