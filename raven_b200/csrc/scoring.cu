@@ -524,8 +524,8 @@ cudaError_t launch_topk(const raven_topk::Params& p, cudaStream_t st) {
   const uint32_t smem = TM::kTeams * (uint32_t)sizeof(raven_topk::Shared<TEAM, BIG>);
   const uint64_t units = p.nq * p.parts;
   static Allowed allowed;
-  return launch(raven_topk::topk_kernel<T, TEAM, BIG>, (units + TM::kTeams - 1) / TM::kTeams, raven_topk::kCtaThreads,
-                smem, allowed, st, p);
+  return launch(raven_topk::topk_kernel<T, TEAM, BIG>, (units + TM::kTeams - 1) / TM::kTeams, TM::kThreads, smem, allowed,
+                st, p);
 }
 template <int TEAM, bool BIG>
 cudaError_t dispatch_topk(int32_t type, const raven_topk::Params& p, cudaStream_t st) {
@@ -675,9 +675,15 @@ int raven_topk_rows_device(const void* d_scores, int32_t type, uint64_t nq, uint
   }
   constexpr int kCta = raven_topk::kCtaThreads;
   const bool big = 2 * k > (uint32_t)kCta;
-  cudaError_t e = warp  ? dispatch_topk<32, false>(type, p, st)
-                  : big ? dispatch_topk<kCta, true>(type, p, st)
-                        : dispatch_topk<kCta, false>(type, p, st);
+  // With k above a warp's threads, selecting and ordering k is a chain of one warp
+  // while its CTA waits: with rows enough, CTAs of half the threads keep twice as
+  // many such chains going (10000 x 10007, k = 100, 220 to 175 us).
+  const bool half = parts == 1 && k > 32 && nq >= 8ull * sms;
+  cudaError_t e = warp                  ? dispatch_topk<32, false>(type, p, st)
+                  : half && 2 * k > 128 ? dispatch_topk<128, true>(type, p, st)
+                  : half                ? dispatch_topk<128, false>(type, p, st)
+                  : big                 ? dispatch_topk<kCta, true>(type, p, st)
+                                        : dispatch_topk<kCta, false>(type, p, st);
   if (e == cudaSuccess && parts > 1) {
     raven_topk::Params j = p;
     j.x = tmp;

@@ -67,13 +67,15 @@ __device__ inline float value_of(uint32_t key, uint32_t mul, uint32_t add) {
   return key < kWorst ? __int_as_float(0x7fc00000) : __uint_as_float((up & 0x80000000u) ? up & 0x7fffffffu : ~up);
 }
 
+// A team of 32 is a warp, a larger one a CTA.
 // BIG: k above half of a CTA's threads, whose least maximum bounds nothing; the
 // bound is then found among their quarters' maxima. A kernel of its own: the
 // registers that takes cost the others a fifth.
 template <int TEAM, bool BIG>
 struct Team {
   static constexpr int kBuf = TEAM == 32 ? 1024 : 2048;
-  static constexpr int kTeams = kCtaThreads / TEAM;
+  static constexpr int kThreads = TEAM == 32 ? kCtaThreads : TEAM;  // of a CTA
+  static constexpr int kTeams = kThreads / TEAM;
   __device__ static void sync() {
     if constexpr (TEAM == 32)
       __syncwarp();
@@ -440,8 +442,7 @@ struct Keeper {
   // and so k elements reach; where k is above a warp's threads, of its elements.
   template <int E>
   __device__ void bound(const uint32_t (&key)[E], const uint32_t (&top)[4]) {
-    if constexpr (BIG) {
-      if (k > (uint32_t)TEAM) return;
+    if constexpr (BIG) {  // k <= kMaxK <= 4 * TEAM
 #pragma unroll
       for (int i = 0; i < 4; ++i) s.top[tid + i * TEAM] = top[i];
       TM::sync();
@@ -509,7 +510,7 @@ __device__ inline void write_out(const Params& p, Keeper<TEAM, BIG>& kp, uint64_
 }
 
 template <typename T, int TEAM, bool BIG>
-__global__ void __launch_bounds__(kCtaThreads, TEAM == 32 ? 3 : 4) topk_kernel(const Params p) {
+__global__ void __launch_bounds__((Team<TEAM, BIG>::kThreads), TEAM == 32 ? 3 : 1024 / TEAM) topk_kernel(const Params p) {
   extern __shared__ __align__(16) uint8_t raw[];
   raven_score::after_previous();
   Shared<TEAM, BIG>* sh = (Shared<TEAM, BIG>*)raw + threadIdx.x / TEAM;
