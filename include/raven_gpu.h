@@ -255,7 +255,7 @@ RAVEN_API int raven_merge_topk_gathered_device(const void* d_gathered, uint32_t 
 /* bits of *d_status, which calls only ever set (the caller clears it) */
 #define RAVEN_S_OFFSETS 1  /* a group's offsets fall or leave the rows: it counted as empty */
 #define RAVEN_S_CAPACITY 2 /* scores past the output's capacity were not written */
-#define RAVEN_S_WAIT 4     /* a wait inside the kernel ran out: the scores are not valid */
+#define RAVEN_S_WAIT 4     /* a wait inside the kernel (each is bounded) ran out: the scores are not valid */
 
 /* Rows of `dim` values, row i at data + i * ld values (codes). FP8 rows also
  * have exponent bytes, row i at exps + i * ld_exps, one per 128 values: a value
@@ -303,9 +303,9 @@ RAVEN_API int raven_scores_device(const raven_rows* q, const raven_rows* v, uint
  * [d_v_offsets[g], d_v_offsets[g + 1]), for g < groups; both offset arrays
  * (groups + 1 each, on the device) rise, and groups may be empty on either
  * side. Output packed: groups in order, in a group its queries in order, for
- * each the scores of the group's vectors. At most `capacity` elements are
- * written: a query's scores in a tile of 128 vectors are written when they fit
- * whole. Queries outside every group have no scores. */
+ * each the scores of the group's vectors. Nothing past `capacity` elements is
+ * written: queries whose scores all fit have them, of the next one some may be
+ * there. Queries outside every group have no scores. */
 RAVEN_API int raven_group_scores_device(const raven_rows* q, const int64_t* d_q_offsets, const raven_rows* v,
                                         const int64_t* d_v_offsets, uint32_t groups, uint32_t dim, float alpha,
                                         const float* d_bias, void* d_out, int32_t out_type, uint64_t capacity,
@@ -321,7 +321,7 @@ RAVEN_API int raven_group_rows_device(const int64_t* d_q_offsets, const int64_t*
  * smallest with largest = 0), equal scores by the lower index, NaN after every
  * number, -0 equal to 0. Rows are n scores at pitch ld, or with d_row_starts
  * (nq + 1 values on the device) the scores [d_row_starts[i], d_row_starts[i + 1])
- * of n in all. d_ids: indexes within the row; d_counts (may be NULL): min(k, row
+ * of n in all (fewer than 2^32 in a row). d_ids: indexes within the row; d_counts (may be NULL): min(k, row
  * length); slots past the count are 0. Values have the scores' type. */
 RAVEN_API int raven_topk_rows_device(const void* d_scores, int32_t type, uint64_t nq, uint64_t n, uint64_t ld,
                                      const int64_t* d_row_starts, uint32_t k, int32_t largest, void* d_vals,

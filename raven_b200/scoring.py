@@ -10,9 +10,14 @@
 * `group_rows`   — where each query's scores start in grouped scores.
 * `top_k`        — the best k of each row of scores, dense or packed.
 
+    rows = Fp8Rows.encode(X)                              # or Fp8Rows.of_index(searcher.device_index)
+    near = scores(Q, rows, alpha=-2.0, bias=(rows.decode() ** 2).sum(1))
+    dist, ids, _ = top_k(near, 10, largest=False)         # squared distances less |q|^2
+
 Everything runs in libraven_gpu.so on the current stream of the tensors'
-device and returns without waiting. The reference has no counterpart: it
-scores every vector only in its tests (test_pybinding.py:16-18), by numpy.
+device and returns without waiting; nothing is differentiable. The reference
+has no counterpart: it scores every vector only in its tests
+(test_pybinding.py:16-18), by numpy.
 """
 from __future__ import annotations
 
@@ -268,7 +273,8 @@ def group_scores(queries: Rows, query_offsets: torch.Tensor, vectors: Rows, vect
 
     `total` is the number of scores (the program that made the groups knows it:
     the sum of queries times vectors; the last of `group_rows`), or `out` a 1-D
-    tensor with room for them. No more than that is written."""
+    tensor with room for them. Nothing is written past it: queries whose scores
+    all fit have them, and `status` gets RAVEN_S_CAPACITY."""
     device, dim, nq, n, q, v, keep = _operands(queries, vectors, dtype, bias)
     groups = _offsets("query_offsets", query_offsets, device)
     if _offsets("vector_offsets", vector_offsets, device) != groups:

@@ -503,3 +503,113 @@ def test_refusals(S):
                  lambda: S.Fp8Rows.encode(f(2, 65537))):
         with pytest.raises(RavenError):
             call()
+
+
+# ---- each layout and team, at the sizes where the choice between them changes ---------
+
+
+def _check_on_gpu(got, q, v, t, alpha=1.0, bias=None):
+    """_check with the 64-bit products on the GPU, for large outputs."""
+    torch = _torch()
+    for at in range(0, q.shape[0], 64):
+        a = q[at:at + 64].double()
+        exact = alpha * (a @ v.double().T) + (0.0 if bias is None else bias.double())
+        mags = a.abs() @ v.double().abs().T
+        off = abs(alpha) * (q.shape[1] + 1) * 2.0 ** -23 * mags + 2.0 ** -23 * exact.abs()
+        if bias is not None:
+            off = off + 2.0 ** -23 * bias.double().abs()
+        lim = off + torch.finfo(_dt(t)).eps / 2 * (exact.abs() + off) + 1e-37
+        assert bool(((got[at:at + 64].double() - exact).abs() <= lim).all())
+
+
+LAYOUTS = [(300, 30_011, 40), (300, 30_016, 40), (130, 20_007, 300), (129, 33_001, 128), (65, 25_003, 17),
+           (70, 400_003, 16), (70, 400_000, 16), (66, 800_001, 16), (40, 50_001, 900), (33, 150_001, 16),
+           (32, 9_001, 128), (4, 20_001, 1024), (4, 20_001, 1025), (1, 300_001, 100), (2000, 1_503, 96), (1000, 209, 64)]
+
+
+@pytest.mark.parametrize("nq,n,dim", LAYOUTS)
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("fp8", [True, False])
+def test_scores_layouts(S, nq, n, dim, t, fp8):
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(nq + n + dim)
+    q = torch.randn(nq, dim, generator=g, device="cuda").half()
+    v = torch.randn(n, dim, generator=g, device="cuda").half()
+    bias = torch.randn(n, generator=g, device="cuda")
+    if fp8:
+        rows, qv = S.Fp8Rows.encode(v), S.Fp8Rows.encode(q).decode()
+        vv = rows.decode()
+    else:
+        q, rows = S.aligned_rows(q), S.aligned_rows(v)
+        qv, vv = q, rows
+    # scores that start anywhere: a pitch and a start of their own, and the bytes around them untouched
+    for room, left in ((n, 0), (n + 13, 5)):
+        big = torch.full((nq, room), 9.0, dtype=_dt(t), device="cuda")
+        out = big[:, left:left + n]
+        with_bias = left > 0
+        S.scores(q, rows, dtype=_dt(t), out=out, alpha=0.5 if with_bias else 1.0, bias=bias if with_bias else None)
+        _check_on_gpu(out, qv, vv, t, 0.5 if with_bias else 1.0, bias if with_bias else None)
+        assert bool((big[:, :left] == 9.0).all()) and bool((big[:, left + n:] == 9.0).all())
+
+
+@pytest.mark.parametrize("t,out", [("fp8", "bf16"), ("fp8", "f32"), ("bf16", "f16"), ("f16", "f32")])
+def test_group_scores_large_groups(S, t, out):
+    """Groups of more than 64 queries on average: the layout by pairs, with packed
+    scores that start anywhere."""
+    _grouped(S, t, out, 4, 700, 1500, 136, 11)
+    _grouped(S, t, out, 3, 400, 901, 72, 12, alpha=-1.5, with_bias=True)
+
+
+def test_group_scores_capacity_by_pairs(S):
+    torch = _torch()
+    q, v = _gpu(_data(200, 64, 1, 1.0), "bf16"), _gpu(_data(301, 64, 2, 1.0), "bf16")
+    qo, vo = torch.tensor([0, 200], device="cuda"), torch.tensor([0, 301], device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for fit in (0, 1, 57, 199):
+        status.zero_()
+        room = torch.full((200 * 301,), 5.0, device="cuda")
+        S.group_scores(q, qo, v, vo, out=room[:fit * 301 + 100], status=status)
+        assert int(status) == 2
+        if fit:
+            _check(room[:fit * 301].view(fit, 301), _np(q)[:fit], _np(v), "f32")
+        assert bool((room[fit * 301 + 100:] == 5.0).all())
+
+
+def test_fp8_bytes_past_the_values_do_not_matter(S):
+    """Code bytes past dim and exponent bytes past the last block are not read as values."""
+    torch = _torch()
+    for nq, n, dim in ((3, 300, 200), (40, 300, 200), (200, 1000, 520)):
+        rows, q = S.Fp8Rows.encode(_gpu(_data(n, dim, 1, 1.0))), S.Fp8Rows.encode(_gpu(_data(nq, dim, 2, 1.0)))
+        want = S.scores(q, rows)
+        for r in (rows, q):
+            r.codes[:, dim:] = 0x7F  # NaN
+            r.exps[:, -(-dim // 128):] = 255
+        assert bool((S.scores(q, rows) == want).all())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("nq,n,k", [(1300, 1500, 100), (1300, 1500, 40), (1300, 2100, 256), (2500, 1200, 20),
+                                    (2500, 1100, 33), (1, 70_000, 200), (3, 4097, 129), (5000, 30, 30), (5000, 900, 200)])
+def test_top_k_teams(S, t, nq, n, k):
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(n + k)
+    for x in (torch.randn(nq, n, generator=g, device="cuda"),
+              torch.randint(0, 40, (nq, n), generator=g, device="cuda").float()):
+        x[0], x[-1, : n // 2] = float("nan"), float("nan")
+        x[nq // 2, ::3], x[nq // 2, 1::3] = float("inf"), float("-inf")
+        x = x.to(_dt(t))
+        for largest in (True, False):
+            vals, ids, counts = S.top_k(x, k, largest=largest)
+            # by a stable sort of the values with NaN behind the worst infinity
+            key = torch.where(x.isnan(), torch.full_like(x, float("nan")), x).float()
+            order = torch.sort(torch.where(key.isnan(), torch.full_like(key, float("inf")), -key if largest else key),
+                               dim=1, stable=True)
+            idx = order.indices
+            # NaN after infinities of the same place: a second stable sort by whether it is NaN
+            idx = idx.gather(1, torch.sort(key.gather(1, idx).isnan().to(torch.int8), dim=1, stable=True).indices)
+            c = min(k, n)
+            assert bool((counts == c).all())
+            assert bool((ids[:, :c].long() == idx[:, :c]).all())
+            want = x.gather(1, idx[:, :c])
+            assert bool(((vals[:, :c] == want) | (vals[:, :c].isnan() & want.isnan())).all())
+            assert bool((ids[:, c:] == 0).all()) and bool((vals[:, c:] == 0).all())
