@@ -25,7 +25,9 @@ int fp8_encode_lane_major(const float* d_rows, uint64_t n, uint32_t dim, uint8_t
 #ifdef __CUDACC__
 namespace raven_score {
 // Start of a kernel's memory accesses: the kernel before it in the stream is
-// done and its writes are seen; the kernel after it may be set up.
+// done and its writes are seen; the kernel after it may be set up. A kernel that
+// begins before its inputs are written reads them by ordinary loads, never as
+// data that is constant while it runs (__ldg, const __restrict__).
 __device__ inline void after_previous() {
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   asm volatile("griddepcontrol.wait;\n" ::: "memory");

@@ -115,7 +115,7 @@ struct Tile {
 // BN: most rows of the N side. ROWS: the layout with rows of v as the M side.
 // HELD: a handful of queries, not encoded yet: every CTA encodes them into its
 // shared memory and keeps them there. Saves the launch and the scratch of an
-// encoding before (1 x 100000 x 128: 10.5 to 8.5 us).
+// encoding before (1 x 100000 x 128: 10.5 to 8.0 us).
 template <bool FP8, int BN, bool ROWS, bool HELD>
 struct Layout {
   static_assert(!HELD || (FP8 && ROWS && BN == 32), "one box of queries");
@@ -349,7 +349,7 @@ __device__ inline void store_rows(T* out, const Tile& t, uint32_t qcnt, uint32_t
   const uint32_t subs = (t.vcnt + kBM - 1) / kBM;
   for (uint32_t sub = 0; sub < subs && first < qcnt; ++sub) {
     const bool row = r + sub * kBM < t.vcnt;
-    const float add = bias && row ? __ldg(bias + sub * kBM + r) : 0.0f;
+    const float add = bias && row ? bias[sub * kBM + r] : 0.0f;
     T* o = out + t.out + sub * kBM + r + (int64_t)first * t.ld;
     for (uint32_t c = first; c < qcnt; c += 32, o += 32 * t.ld) {
       uint32_t v[16];
@@ -421,7 +421,7 @@ __device__ inline void store_pairs(T* out, const Tile& t, uint32_t qcnt, uint32_
 #pragma unroll
       for (uint32_t i = 0; i < SC; ++i) {
         const uint32_t c = SC * k + i;
-        v[i] = __float_as_uint(fmaf(alpha, __uint_as_float(v[i]), bias && c < avail ? __ldg(bias + first + c) : 0.0f));
+        v[i] = __float_as_uint(fmaf(alpha, __uint_as_float(v[i]), bias && c < avail ? bias[first + c] : 0.0f));
       }
     }
 #pragma unroll
@@ -819,7 +819,7 @@ __global__ void __launch_bounds__((Layout<FP8, BN, ROWS, HELD>::kThreads), 1)
       }
 #pragma unroll
       for (int j = 0; j < kParts; ++j)
-        w[j] = HELD && j ? *(const uint32_t*)(src[j] + kb) : __ldg((const uint32_t*)(src[j] + kb));
+        w[j] = *(const uint32_t*)(src[j] + kb);
       return true;
     };
     uint32_t f = 0, fph = 0, w[kParts], next[kParts];

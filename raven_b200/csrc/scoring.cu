@@ -44,6 +44,15 @@ uint64_t type_size(int32_t t) {
 }
 bool aligned(const void* p, uint64_t a) { return (uintptr_t)p % a == 0; }
 
+// What a device's first call sets up is no part of a stream's work: this thread
+// does it although one of its streams is being captured, which otherwise ends
+// the capture.
+struct Apart {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  Apart() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~Apart() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 // SMs of the current device. On a device's first call its default memory pool
 // is told to keep freed scratch (as raven_index_upload does): a pool that gives
 // it back at every synchronisation makes the next call wait for an allocation.
@@ -56,6 +65,7 @@ int sm_count(int* out) {
   std::lock_guard<std::mutex> lk(mu);
   if (!count[dev]) {
     CU(cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev));
+    Apart apart;
     cudaMemPool_t pool;
     uint64_t keep = ~0ull;
     if (cudaDeviceGetDefaultMemPool(&pool, dev) == cudaSuccess)
@@ -92,6 +102,7 @@ cudaError_t launch(void (*kern)(K...), uint64_t grid, int threads, uint32_t smem
   c.numAttrs = 1;
   for (int turn = 0;; ++turn) {
     if (smem > 48 * 1024 && (turn || dev >= 64 || !(allowed.mask.load(std::memory_order_relaxed) & bit))) {
+      Apart apart;
       e = cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
       if (e != cudaSuccess) return e;
       allowed.mask.fetch_or(bit, std::memory_order_relaxed);
@@ -122,9 +133,9 @@ using raven_fp8::load_value;
 constexpr uint32_t kExpBytes = 4096;  // of a run: rows x blocks padded to 4
 
 template <typename T, bool VEC, bool LANE>
-__global__ void __launch_bounds__(256, 8) fp8_encode_kernel(const T* __restrict__ in, uint64_t n, uint32_t dim, uint64_t ld,
-                                                         uint8_t* __restrict__ codes, uint64_t ld_codes,
-                                                         uint8_t* __restrict__ exps, uint64_t ld_exps, uint32_t run) {
+__global__ void __launch_bounds__(256, 8) fp8_encode_kernel(const T* in, uint64_t n, uint32_t dim, uint64_t ld,
+                                                         uint8_t* codes, uint64_t ld_codes, uint8_t* exps,
+                                                         uint64_t ld_exps, uint32_t run) {
   constexpr int E = 16 / sizeof(T), G = (int)kBlock / E, U = 2;  // values per lane, lanes per block, blocks under way
   __shared__ __align__(16) uint8_t se[kExpBytes];
   after_previous();
@@ -214,9 +225,9 @@ __global__ void __launch_bounds__(256, 8) fp8_encode_kernel(const T* __restrict_
   }
 }
 
-__global__ void __launch_bounds__(256) fp8_decode_kernel(const uint8_t* __restrict__ codes, uint64_t ld_codes,
-                                                         const uint8_t* __restrict__ exps, uint64_t ld_exps, uint64_t n,
-                                                         uint32_t dim, float* __restrict__ out, uint64_t ld) {
+__global__ void __launch_bounds__(256) fp8_decode_kernel(const uint8_t* codes, uint64_t ld_codes, const uint8_t* exps,
+                                                         uint64_t ld_exps, uint64_t n, uint32_t dim, float* out,
+                                                         uint64_t ld) {
   after_previous();
   const uint64_t total = n * dim;
   for (uint64_t t = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; t < total; t += (uint64_t)gridDim.x * blockDim.x) {
@@ -383,7 +394,7 @@ int run_scores(const raven_rows* q, const int64_t* qo, const raven_rows* v, cons
   if (out_type != RAVEN_TYPE_F32 && out_type != RAVEN_TYPE_F16 && out_type != RAVEN_TYPE_BF16)
     return fail(RAVEN_EINVAL, "scores: type must be f32, f16 or bf16");
   if (q->rows == 0 || v->rows == 0 || groups == 0) return RAVEN_OK;
-  if (!out) return fail(RAVEN_EINVAL, "scores: null output");
+  if (!out && !(qo && capacity == 0)) return fail(RAVEN_EINVAL, "scores: null output");
   if (!aligned(out, type_size(out_type))) return fail(RAVEN_EINVAL, "scores: output is not aligned to its type");
   if (!qo && ld < v->rows) return fail(RAVEN_EINVAL, "scores: output pitch below the number of vectors");
   const bool encode = fp8 && q->type != RAVEN_TYPE_FP8;
@@ -454,9 +465,8 @@ int run_scores(const raven_rows* q, const int64_t* qo, const raven_rows* v, cons
 // Where each query's scores start in grouped scores: starts[i] for query i of
 // group g is sum over earlier groups of m h_n plus its place times n_g. Blocks
 // take runs of 256 groups; each sums the groups before its run by itself.
-__global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* __restrict__ qo, const int64_t* __restrict__ vo,
-                                                         uint32_t groups, uint64_t nq, uint64_t n,
-                                                         int64_t* __restrict__ starts, int* status) {
+__global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* qo, const int64_t* vo, uint32_t groups,
+                                                         uint64_t nq, uint64_t n, int64_t* starts, int* status) {
   after_previous();
   __shared__ int64_t part[256];
   __shared__ int64_t gq[256], gm[256], gn[256];
@@ -604,7 +614,7 @@ int raven_group_scores_device(const raven_rows* q, const int64_t* d_q_offsets, c
   if (groups && (!d_q_offsets || !d_v_offsets)) return fail(RAVEN_EINVAL, "offsets: null");
   if (groups && (!aligned(d_q_offsets, 8) || !aligned(d_v_offsets, 8)))
     return fail(RAVEN_EINVAL, "offsets: not aligned to 64 bits");
-  if (capacity == 0) groups = 0;
+  if (capacity == 0 && !d_status) groups = 0;  // nothing to write, nor anyone to tell
   return run_scores(q, d_q_offsets, v, d_v_offsets, groups, dim, alpha, d_bias, d_out, out_type, 0, capacity, d_status,
                     stream);
 }

@@ -549,12 +549,12 @@ __global__ void __launch_bounds__((Team<TEAM, BIG>::kThreads), TEAM == 32 ? 3 : 
   auto load = [&](uint64_t t) {  // pieces of the tile at t that hold an element
     if (t + kTile <= end) {
 #pragma unroll
-      for (int i = 0; i < L::kPieces; ++i) ahead[i] = __ldg(w + i * TEAM);
+      for (int i = 0; i < L::kPieces; ++i) ahead[i] = w[i * TEAM];
     } else {
       const uint32_t left = t < end ? (uint32_t)(end - t) : 0;
 #pragma unroll
       for (int i = 0; i < L::kPieces; ++i)
-        ahead[i] = (i * TEAM + tid) * L::kPer < left ? __ldg(w + i * TEAM) : make_uint4(none, none, none, none);
+        ahead[i] = (i * TEAM + tid) * L::kPer < left ? w[i * TEAM] : make_uint4(none, none, none, none);
     }
     w += TEAM * L::kPieces;
   };

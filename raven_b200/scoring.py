@@ -249,7 +249,7 @@ def scores(queries: Rows, vectors: Rows, *, alpha: float = 1.0, bias: Optional[t
             raise ValueError(f"out must be a {dtype} matrix of {nq} x {n}, each row's values side by side")
         _on(device, out)
         pitch = _pitch(out)
-    _call(device, L.load().raven_scores_device, q, v, dim, alpha, _ptr(bias), out.data_ptr(), _TYPES[dtype], pitch,
+    _call(device, L.load().raven_scores_device, q, v, dim, float(alpha), _ptr(bias), out.data_ptr(), _TYPES[dtype], pitch,
           _status(status, device))
     return out
 
@@ -288,7 +288,7 @@ def group_scores(queries: Rows, query_offsets: torch.Tensor, vectors: Rows, vect
     else:
         _on(device, out)
     _call(device, L.load().raven_group_scores_device, q, query_offsets.data_ptr(), v, vector_offsets.data_ptr(), groups,
-          dim, alpha, _ptr(bias), out.data_ptr(), _TYPES[dtype], out.numel(), _status(status, device))
+          dim, float(alpha), _ptr(bias), out.data_ptr(), _TYPES[dtype], out.numel(), _status(status, device))
     return out
 
 
@@ -319,7 +319,7 @@ def top_k(scores: torch.Tensor, k: int, *, largest: bool = True,
     row's count (rows of fewer than k) are 0."""
     if not isinstance(scores, torch.Tensor) or not scores.is_cuda or scores.dtype not in _TYPES:
         raise ValueError("scores must be a float32, float16 or bfloat16 tensor on a GPU")
-    index, device = scores.get_device(), scores.device
+    index, device, k = scores.get_device(), scores.device, int(k)
     if row_starts is None:
         if scores.dim() != 2:
             raise ValueError("scores must be a matrix, or packed with row_starts")

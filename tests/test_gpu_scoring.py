@@ -613,3 +613,105 @@ def test_top_k_teams(S, t, nq, n, k):
             want = x.gather(1, idx[:, :c])
             assert bool(((vals[:, :c] == want) | (vals[:, :c].isnan() & want.isnan())).all())
             assert bool((ids[:, c:] == 0).all()) and bool((vals[:, c:] == 0).all())
+
+
+def test_group_scores_without_room_tell(S):
+    torch = _torch()
+    q, v = _gpu(_data(20, 64, 1, 1.0), "bf16"), _gpu(_data(30, 64, 2, 1.0), "bf16")
+    qo, vo = torch.tensor([0, 20], device="cuda"), torch.tensor([0, 30], device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    S.group_scores(q, qo, v, vo, total=0, status=status)
+    assert int(status) == 2
+    status.zero_()
+    S.group_scores(q, torch.zeros_like(qo), v, vo, total=0, status=status)  # no scores: nothing is missing
+    assert int(status) == 0
+
+
+def test_inputs_written_just_before(S):
+    """Every operator on what the one before it has just written, in one stream
+    without a wait, the buffers the same each time and their contents not."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rows = S.Fp8Rows.empty(3000, 200, "cuda")
+    out, back = torch.empty(70, 3000, device="cuda"), torch.empty(70, 200, device="cuda")
+    x, q = torch.empty(3000, 200, device="cuda"), torch.empty(70, 200, device="cuda")
+    got, inputs = [], []
+    for i in range(12):
+        x.normal_(generator=g)
+        q.normal_(generator=g)
+        S.Fp8Rows.encode(x, out=rows)
+        S.scores(q, rows, out=out)
+        vals, ids, _ = S.top_k(out, 7)
+        again = S.Fp8Rows.encode(out)  # scores as rows: reads what the product wrote
+        got.append((vals, ids, S.scores(again, again), S.top_k(S.scores(q[:3], rows), 5)[1]))
+        inputs.append((x.clone(), q.clone()))
+    torch.cuda.synchronize()
+    for (vals, ids, self_scores, few), (x, q) in zip(got, inputs):
+        rows = S.Fp8Rows.encode(x)
+        torch.cuda.synchronize()
+        out = S.scores(q, rows)
+        torch.cuda.synchronize()
+        want = S.top_k(out, 7)
+        again = S.Fp8Rows.encode(out)
+        torch.cuda.synchronize()
+        assert bool((vals == want[0]).all()) and bool((ids == want[1]).all())
+        assert bool((self_scores == S.scores(again, again)).all())
+        few_out = S.scores(q[:3], rows)
+        torch.cuda.synchronize()
+        assert bool((few == S.top_k(few_out, 5)[1]).all())
+
+
+def test_first_call_inside_a_capture(raven_lib):
+    """A process whose first calls of the library are captured."""
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from raven_b200 import scoring as S
+x, q = torch.randn(5000, 96, device="cuda"), torch.randn(64, 96, device="cuda")
+long = torch.randn(2, 100_000, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = S.top_k(S.scores(q, S.Fp8Rows.encode(x)), 9)
+    got_long = S.top_k(long, 9)
+for _ in range(3):
+    x.normal_(); q.normal_(); long.normal_()
+    graph.replay()
+    want, want_long = S.top_k(S.scores(q, S.Fp8Rows.encode(x)), 9), S.top_k(long, 9)
+    torch.cuda.synchronize()
+    assert all(bool((a == b).all()) for a, b in zip(got, want)) and all(bool((a == b).all()) for a, b in zip(got_long, want_long))
+print("captured")
+"""
+    import os
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_two_threads(S):
+    """Calls from two threads, each on a stream of its own."""
+    import threading
+
+    torch = _torch()
+    rows = S.Fp8Rows.encode(_gpu(_data(4000, 160, 1, 1.0)))
+    qs = [_gpu(_data(100, 160, 20 + i, 1.0)) for i in range(2)]
+    want = [S.top_k(S.scores(q, rows), 12) for q in qs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(40):
+                got = S.top_k(S.scores(qs[i], rows), 12)
+            torch.cuda.current_stream().synchronize()
+            if not all(bool((a == b).all()) for a, b in zip(got, want[i])):
+                bad.append(i)
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad
