@@ -301,8 +301,8 @@ RAVEN_API int raven_scores_device(const raven_rows* q, const raven_rows* v, uint
 
 /* Scores by group: queries [d_q_offsets[g], d_q_offsets[g + 1]) against vectors
  * [d_v_offsets[g], d_v_offsets[g + 1]), for g < groups; both offset arrays
- * (groups + 1 each, on the device) rise, and groups may be empty on either
- * side. Output packed: groups in order, in a group its queries in order, for
+ * (groups + 1 each, on the device; fewer than 2^31) rise, and groups may be
+ * empty on either side. Output packed: groups in order, in a group its queries in order, for
  * each the scores of the group's vectors. Nothing past `capacity` elements is
  * written: queries whose scores all fit have them, of the next one some may be
  * there. Queries outside every group have no scores. */

@@ -77,6 +77,25 @@ constexpr uint32_t kHeldUnits = 32;    // and query blocks that it encodes
 enum : int { kOutF32 = 0, kOutF16 = 1, kOutBf16 = 2 };
 enum : int { kStatusOffsets = 1, kStatusCapacity = 2, kStatusWait = 4 };
 
+// Sums over the groups before a chunk of 32 groups: their tiles, their scores.
+struct alignas(16) Chunk {
+  int64_t tiles, out;
+};
+constexpr uint32_t kChunk = 32;
+
+// Group g's first query and row, how many of each; false, and an empty group,
+// where its offsets are not within the arrays or fall.
+__device__ inline bool group_of(const int64_t* qo, const int64_t* vo, uint32_t g, uint64_t nq, uint64_t n, int64_t& q0,
+                                int64_t& v0, int64_t& m, int64_t& nn) {
+  const int64_t a = qo[g], q1 = qo[g + 1], b = vo[g], v1 = vo[g + 1];
+  const bool ok = a >= 0 && q1 >= a && (uint64_t)q1 <= nq && b >= 0 && v1 >= b && (uint64_t)v1 <= n;
+  q0 = ok ? a : 0;
+  v0 = ok ? b : 0;
+  m = ok ? q1 - a : 0;
+  nn = ok ? v1 - b : 0;
+  return ok;
+}
+
 struct Params {
   uint64_t nq, n;             // rows of q and v
   uint32_t nkb;               // 128-byte K blocks
@@ -84,6 +103,8 @@ struct Params {
   uint32_t subs;              // (rows) accumulators per tile: a tile has up to 128 * subs rows of v
   uint32_t halo;              // (pairs) scores that a tile computes past its own, 0 where every query starts on a sector
   uint32_t groups;            // 1 with null offsets: dense
+  uint32_t nchunks;           // many groups: chunks[nchunks + 1], else null
+  const Chunk* chunks;
   const int64_t* qo;          // [groups + 1] or null
   const int64_t* vo;
   const uint8_t* qe;          // exponents (FP8)
@@ -173,18 +194,35 @@ __device__ inline void mma_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t ide
       : "memory");
 }
 
+// The last chunk with at most t tiles before it (t is less than all their tiles),
+// 32 guesses at a time.
+__device__ __noinline__ uint32_t chunk_of_tile(const Chunk* chunks, uint32_t count, uint64_t t) {
+  uint32_t lo = 0;
+  while (count > 1) {
+    const uint32_t step = (count + 31) / 32, c = (threadIdx.x & 31) * step;
+    const uint32_t at = 31 - __clz(__ballot_sync(0xffffffffu, c < count && (uint64_t)chunks[lo + c].tiles <= t));
+    lo += at * step;
+    count = min(step, count - at * step);
+  }
+  return lo;
+}
+
 // Finds the tiles of one CTA, in order, by one warp: groups are read 32 at a
 // time (one per lane) and their tiles counted by a warp scan; a CTA's tiles
-// rise, so the groups are walked once. The lane that holds a tile's group works
-// out the tile. Its divisions are 32-bit ones unless the group has 2^32 tiles.
-template <typename L>
+// rise, so the groups are walked once. MANY groups, whose walk would take longer
+// than the tiles: the sums before each chunk of 32 groups are there, a tile's
+// chunk is searched for, and a CTA takes runs of up to 32 consecutive tiles,
+// which mostly share a chunk (65536 groups of 1 x 8 scores 1400 to 313 us).
+// The lane that holds a tile's group works out the tile. Its divisions are 32-bit
+// ones unless the group has 2^32 tiles.
+template <typename L, bool MANY>
 struct TileFinder {
   static constexpr uint32_t TQ = L::kTileQ;
   const Params& p;
   int lane;
   uint64_t first = 0;       // first tile of the chunk
   int64_t out0 = 0;         // output elements before the chunk
-  uint32_t g0 = 0;          // its first group
+  uint32_t g0 = 0u - kChunk;  // its first group
   uint64_t incl = 0;        // this lane's group: tiles up to and with it, in the chunk
   uint64_t tiles = 0;
   int64_t before = 0;       // output elements before it, in the chunk
@@ -192,24 +230,40 @@ struct TileFinder {
   int64_t chunk_out = 0;
   uint32_t qa = 0, va = 0, m = 0, nn = 0;  // its first query and row, how many
   uint32_t rows;            // of v per tile
+  uint64_t t;               // the CTA's next tile
+  uint64_t skip;            // from the last tile of a run to the next run
+  uint32_t run = 1, left;   // consecutive tiles that the CTA takes, how many are left
   bool bad = false;
 
-  __device__ TileFinder(const Params& p_, int lane_) : p(p_), lane(lane_), rows(L::kTileV * p_.subs - p_.halo) { load(); }
+  __device__ TileFinder(const Params& p_, int lane_) : p(p_), lane(lane_), rows(L::kTileV * p_.subs - p_.halo) {
+    if constexpr (MANY) {
+      const uint64_t total = (uint64_t)p.chunks[p.nchunks].tiles;
+      run = (uint32_t)max((uint64_t)1, min((uint64_t)kChunk, total / (8 * (uint64_t)gridDim.x)));
+    }
+    left = run;
+    t = (uint64_t)blockIdx.x * run;
+    skip = (uint64_t)(gridDim.x - 1) * run + 1;
+  }
+  __device__ void next() {
+    if (MANY && --left) {
+      ++t;
+    } else {
+      t += skip;
+      left = run;
+    }
+  }
 
   __device__ void load() {
     const uint32_t g = g0 + (uint32_t)lane;
     qa = va = m = nn = 0;
     if (g < p.groups) {
       if (p.qo) {
-        const int64_t q0 = p.qo[g], q1 = p.qo[g + 1], v0 = p.vo[g], v1 = p.vo[g + 1];
-        if (q0 < 0 || q1 < q0 || (uint64_t)q1 > p.nq || v0 < 0 || v1 < v0 || (uint64_t)v1 > p.n) {
-          bad = true;  // the group counts as empty
-        } else {
-          qa = (uint32_t)q0;
-          va = (uint32_t)v0;
-          m = (uint32_t)(q1 - q0);
-          nn = (uint32_t)(v1 - v0);
-        }
+        int64_t q0, v0, mq, mv;
+        bad |= !group_of(p.qo, p.vo, g, p.nq, p.n, q0, v0, mq, mv);
+        qa = (uint32_t)q0;
+        va = (uint32_t)v0;
+        m = (uint32_t)mq;
+        nn = (uint32_t)mv;
       } else {
         m = (uint32_t)p.nq;
         nn = (uint32_t)p.n;
@@ -220,10 +274,10 @@ struct TileFinder {
     int64_t e = (int64_t)m * nn;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t t = __shfl_up_sync(0xffffffffu, incl, o);
+      const uint64_t y = __shfl_up_sync(0xffffffffu, incl, o);
       const int64_t x = __shfl_up_sync(0xffffffffu, e, o);
       if (lane >= o) {
-        incl += t;
+        incl += y;
         e += x;
       }
     }
@@ -232,19 +286,28 @@ struct TileFinder {
     chunk_out = __shfl_sync(0xffffffffu, e, 31);
   }
 
-  // The lane whose group holds tile t (rising between calls); -1 when there is none.
-  __device__ int find(uint64_t t) {
+  // The lane whose group holds tile t; -1 when there is none.
+  __device__ int find() {
     while (t >= first + chunk_tiles) {
-      if (g0 + 32 >= p.groups || g0 + 32 < g0) return -1;
+      uint32_t g = g0 + kChunk;
       first += chunk_tiles;
       out0 += chunk_out;
-      g0 += 32;
+      if constexpr (MANY) {
+        if (t >= (uint64_t)p.chunks[p.nchunks].tiles) return -1;
+        const uint32_t c = chunk_of_tile(p.chunks, p.nchunks, t);
+        g = c * kChunk;
+        first = (uint64_t)p.chunks[c].tiles;
+        out0 = p.chunks[c].out;
+      }
+      if (g >= p.groups) return -1;
+      g0 = g;
       load();
+      if (MANY) break;  // it is this one
     }
     return __ffs(__ballot_sync(0xffffffffu, t - first < incl)) - 1;
   }
   // Tile t of this lane's group.
-  __device__ Tile tile(uint64_t t) const {
+  __device__ Tile tile() const {
     const uint64_t in = t - first - (incl - tiles);
     // bands of kBand query tiles; in a band, all its query tiles of one row tile before the next
     const uint32_t mt = (m + TQ - 1) / TQ, nt = (nn + rows - 1) / rows;
@@ -697,26 +760,31 @@ __global__ void __launch_bounds__((Layout<FP8, BN, ROWS, HELD>::kThreads), 1)
     __syncwarp();
     ok &= warp_wait(drain, 0);
   } else if (warp == 2) {  // tiles
-    TileFinder<L> finder(p, lane);
-    TileReader wr;
-    for (uint64_t t = blockIdx.x;; t += gridDim.x) {
-      const int at = finder.find(t);
-      if (!warp_wait(info_empty(wr.slot), wr.phase ^ 1u)) {
-        ok = false;
-        break;
+    auto find_tiles = [&](auto finder) {
+      TileReader wr;
+      for (;; finder.next()) {
+        const int at = finder.find();
+        if (!warp_wait(info_empty(wr.slot), wr.phase ^ 1u)) {
+          ok = false;
+          break;
+        }
+        if (lane == max(at, 0)) {
+          if (at < 0)
+            tiles[wr.slot].qcnt = 0;
+          else
+            tiles[wr.slot] = finder.tile();
+          mbar_arrive(info_full(wr.slot));
+        }
+        __syncwarp();
+        wr.next();
+        if (at < 0) break;
       }
-      if (lane == max(at, 0)) {
-        if (at < 0)
-          tiles[wr.slot].qcnt = 0;
-        else
-          tiles[wr.slot] = finder.tile(t);
-        mbar_arrive(info_full(wr.slot));
-      }
-      __syncwarp();
-      wr.next();
-      if (at < 0) break;
-    }
-    if (__any_sync(0xffffffffu, finder.bad) && lane == 0 && p.status) atomicOr(p.status, kStatusOffsets);
+      if (__any_sync(0xffffffffu, finder.bad) && lane == 0 && p.status) atomicOr(p.status, kStatusOffsets);
+    };
+    if (p.chunks)
+      find_tiles(TileFinder<L, true>(p, lane));
+    else
+      find_tiles(TileFinder<L, false>(p, lane));
   } else if (warp >= 4 && warp < 4 + kEpiWarps) {  // epilogue
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     if constexpr (HELD) {

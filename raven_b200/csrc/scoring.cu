@@ -303,6 +303,102 @@ bool rows_map(CUtensorMap* m, const void* base, int32_t type, uint32_t dim, uint
            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// ---------------------------------------------------------------------------
+// Many groups: sums over the groups before each chunk of 32, so that neither a
+// tile's group nor a query's place is found by walking them all.
+// ---------------------------------------------------------------------------
+using raven_score::Chunk;
+using raven_score::kChunk;
+// From how many groups on: the sums' two launches take 4 us and more, and a walk
+// is partly hidden by the tiles (1000 groups of 1 x 8 scores 22 us walked, 18 with
+// sums, but 1000 of 10 x 1000 44 and 49; 2000 of 20 x 300 59 and 45). The blocks of
+// group_rows, which sum what is before them by themselves, reach that later (4096
+// groups 11.5 us, 13.0 with sums; 65536: 50, 19).
+constexpr uint32_t kManyGroups = 1536, kManyGroupRows = 8192;
+
+// Per chunk, the tiles (of tq queries and `rows` rows of v) and scores of its groups.
+__global__ void __launch_bounds__(256) group_chunks_kernel(const int64_t* qo, const int64_t* vo, uint32_t groups,
+                                                           uint64_t nq, uint64_t n, uint32_t tq, uint32_t rows,
+                                                           Chunk* chunks, int* status) {
+  after_previous();
+  const uint32_t g = blockIdx.x * 256u + threadIdx.x, lane = threadIdx.x & 31;
+  int64_t a, b, m = 0, nn = 0;
+  const bool bad = g < groups && !raven_score::group_of(qo, vo, g, nq, n, a, b, m, nn);
+  int64_t tiles = (m + tq - 1) / tq * ((nn + rows - 1) / rows), out = m * nn;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    out += __shfl_xor_sync(0xffffffffu, out, o);
+  }
+  if (lane == 0 && g < groups) chunks[g / kChunk] = Chunk{tiles, out};
+  if (__any_sync(0xffffffffu, bad) && lane == 0 && status) atomicOr(status, raven_score::kStatusOffsets);
+}
+
+// Chunks' sums to sums over the chunks before; chunks[count]: over all. One CTA.
+__global__ void __launch_bounds__(1024) group_scan_kernel(Chunk* chunks, uint32_t count) {
+  constexpr uint32_t N = 4;  // chunks of a thread at once
+  __shared__ Chunk part[32];
+  after_previous();
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  Chunk before{0, 0};
+  for (uint32_t base = 0; base < count; base += 1024 * N) {
+    Chunk x[N], sum{0, 0};
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) {
+      const uint32_t c = base + tid * N + i;
+      x[i] = c < count ? chunks[c] : Chunk{0, 0};
+      sum.tiles += x[i].tiles;
+      sum.out += x[i].out;
+    }
+    Chunk up = sum;
+    auto scan = [&](Chunk& s) {
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t t = __shfl_up_sync(0xffffffffu, s.tiles, o), u = __shfl_up_sync(0xffffffffu, s.out, o);
+        if ((int)lane >= o) {
+          s.tiles += t;
+          s.out += u;
+        }
+      }
+    };
+    scan(up);
+    if (lane == 31) part[warp] = up;
+    __syncthreads();
+    if (warp == 0) {
+      Chunk s = part[lane];
+      scan(s);
+      part[lane] = s;
+    }
+    __syncthreads();
+    Chunk at{before.tiles + up.tiles - sum.tiles, before.out + up.out - sum.out};
+    if (warp) {
+      at.tiles += part[warp - 1].tiles;
+      at.out += part[warp - 1].out;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) {
+      const uint32_t c = base + tid * N + i;
+      if (c < count) chunks[c] = at;
+      at.tiles += x[i].tiles;
+      at.out += x[i].out;
+    }
+    before.tiles += part[31].tiles;
+    before.out += part[31].out;
+    __syncthreads();
+  }
+  if (tid == 0) chunks[count] = before;
+}
+
+uint32_t chunks_of(uint32_t groups) { return (groups + kChunk - 1) / kChunk; }
+
+cudaError_t launch_chunks(const int64_t* qo, const int64_t* vo, uint32_t groups, uint64_t nq, uint64_t n, uint32_t tq,
+                          uint32_t rows, Chunk* chunks, int* status, cudaStream_t st) {
+  static Allowed none, none_scan;
+  const cudaError_t e = launch(group_chunks_kernel, (groups + 255) / 256, 256, 0, none, st, qo, vo, groups, nq, n, tq,
+                               rows, chunks, status);
+  return e != cudaSuccess ? e : launch(group_scan_kernel, 1, 1024, 0, none_scan, st, chunks, chunks_of(groups));
+}
+
 struct Operands {
   const raven_rows* q;
   const raven_rows* v;
@@ -331,8 +427,19 @@ cudaError_t launch_score(const Operands& o, raven_score::Params p, bool whole, i
   p.subs = (uint32_t)subs;
   p.halo = ROWS || whole ? 0 : 16;
   const uint64_t grid = p.qo ? (uint64_t)sms : std::min<uint64_t>(tiles(subs), (uint64_t)sms);
+  Chunk* chunks = nullptr;
+  cudaError_t e = cudaSuccess;
+  if (p.groups > kManyGroups) {
+    p.nchunks = chunks_of(p.groups);
+    if ((e = cudaMallocAsync((void**)&chunks, (p.nchunks + 1ull) * sizeof(Chunk), st)) != cudaSuccess) return e;
+    p.chunks = chunks;
+    e = launch_chunks(p.qo, p.vo, p.groups, p.nq, p.n, L::kTileQ, L::kTileV * p.subs - p.halo, chunks, p.status, st);
+  }
   static Allowed allowed;
-  return launch(raven_score::score_kernel<FP8, BN, ROWS, HELD>, grid, L::kThreads, L::kBytes, allowed, st, mq, mv, p);
+  if (e == cudaSuccess)
+    e = launch(raven_score::score_kernel<FP8, BN, ROWS, HELD>, grid, L::kThreads, L::kBytes, allowed, st, mq, mv, p);
+  if (chunks) cudaFreeAsync(chunks, st);
+  return e;
 }
 
 // `want`: queries of a group, twice the mean where groups differ. Up to 64: the
@@ -464,24 +571,22 @@ int run_scores(const raven_rows* q, const int64_t* qo, const raven_rows* v, cons
 
 // Where each query's scores start in grouped scores: starts[i] for query i of
 // group g is sum over earlier groups of m h_n plus its place times n_g. Blocks
-// take runs of 256 groups; each sums the groups before its run by itself.
+// take runs of 256 groups; each sums the groups before its run by itself, unless
+// the sums are given (many groups).
 __global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* qo, const int64_t* vo, uint32_t groups,
-                                                         uint64_t nq, uint64_t n, int64_t* starts, int* status) {
+                                                         uint64_t nq, uint64_t n, const Chunk* chunks, int64_t* starts,
+                                                         int* status) {
   after_previous();
   __shared__ int64_t part[256];
   __shared__ int64_t gq[256], gm[256], gn[256];
   const uint32_t g0 = blockIdx.x * 256u, tid = threadIdx.x;
   bool bad = false;
   auto read = [&](uint32_t g, int64_t& a, int64_t& m, int64_t& c) {
-    const int64_t q0 = qo[g], q1 = qo[g + 1], v0 = vo[g], v1 = vo[g + 1];
-    const bool ok = q0 >= 0 && q1 >= q0 && (uint64_t)q1 <= nq && v0 >= 0 && v1 >= v0 && (uint64_t)v1 <= n;
-    bad |= !ok;
-    a = ok ? q0 : 0;
-    m = ok ? q1 - q0 : 0;
-    c = ok ? v1 - v0 : 0;
+    int64_t v0;
+    bad |= !raven_score::group_of(qo, vo, g, nq, n, a, v0, m, c);
   };
   int64_t sum = 0, a, m, c;
-  for (uint32_t g = tid; g < g0; g += 256) {
+  for (uint32_t g = tid; g < g0 && !chunks; g += 256) {
     read(g, a, m, c);
     sum += m * c;
   }
@@ -491,7 +596,7 @@ __global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* qo, cons
     if ((int)tid < o) part[tid] += part[tid + o];
     __syncthreads();
   }
-  const int64_t before = part[0];
+  const int64_t before = chunks ? chunks[g0 / kChunk].out : part[0];
   __syncthreads();
   a = m = c = 0;
   if (g0 + tid < groups) read(g0 + tid, a, m, c);
@@ -614,6 +719,7 @@ int raven_group_scores_device(const raven_rows* q, const int64_t* d_q_offsets, c
   if (groups && (!d_q_offsets || !d_v_offsets)) return fail(RAVEN_EINVAL, "offsets: null");
   if (groups && (!aligned(d_q_offsets, 8) || !aligned(d_v_offsets, 8)))
     return fail(RAVEN_EINVAL, "offsets: not aligned to 64 bits");
+  if (groups > kMaxRows) return fail(RAVEN_ELIMIT, "more than 2^31 - 1 groups");
   if (capacity == 0 && !d_status) groups = 0;  // nothing to write, nor anyone to tell
   return run_scores(q, d_q_offsets, v, d_v_offsets, groups, dim, alpha, d_bias, d_out, out_type, 0, capacity, d_status,
                     stream);
@@ -627,9 +733,22 @@ int raven_group_rows_device(const int64_t* d_q_offsets, const int64_t* d_v_offse
   if (!d_q_offsets || !d_v_offsets || !d_row_starts) return fail(RAVEN_EINVAL, "null argument");
   if (!aligned(d_q_offsets, 8) || !aligned(d_v_offsets, 8) || !aligned(d_row_starts, 8))
     return fail(RAVEN_EINVAL, "offsets and row starts: not aligned to 64 bits");
+  if (groups > kMaxRows) return fail(RAVEN_ELIMIT, "more than 2^31 - 1 groups");
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  Chunk* chunks = nullptr;
+  cudaError_t e = cudaSuccess;
+  if (groups > kManyGroupRows) {
+    CU(cudaMallocAsync((void**)&chunks, (chunks_of(groups) + 1ull) * sizeof(Chunk), st));
+    e = launch_chunks(d_q_offsets, d_v_offsets, groups, nq, n, 1, 1, chunks, d_status, st);
+  }
   static Allowed none;
-  CU(launch(group_rows_kernel, (groups + 255) / 256, 256, 0, none, (cudaStream_t)stream, d_q_offsets, d_v_offsets,
-            groups, nq, n, d_row_starts, d_status));
+  if (e == cudaSuccess)
+    e = launch(group_rows_kernel, (groups + 255) / 256, 256, 0, none, st, d_q_offsets, d_v_offsets, groups, nq, n, chunks,
+               d_row_starts, d_status);
+  if (chunks) cudaFreeAsync(chunks, st);
+  CU(e);
   return RAVEN_OK;
 }
 

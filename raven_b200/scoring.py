@@ -22,6 +22,7 @@ has no counterpart: it scores every vector only in its tests
 from __future__ import annotations
 
 import ctypes as C
+import operator
 from typing import Optional, Tuple, Union
 
 import torch
@@ -319,7 +320,7 @@ def top_k(scores: torch.Tensor, k: int, *, largest: bool = True,
     row's count (rows of fewer than k) are 0."""
     if not isinstance(scores, torch.Tensor) or not scores.is_cuda or scores.dtype not in _TYPES:
         raise ValueError("scores must be a float32, float16 or bfloat16 tensor on a GPU")
-    index, device, k = scores.get_device(), scores.device, int(k)
+    index, device, k = scores.get_device(), scores.device, operator.index(k)
     if row_starts is None:
         if scores.dim() != 2:
             raise ValueError("scores must be a matrix, or packed with row_starts")

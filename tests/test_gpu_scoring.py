@@ -715,3 +715,70 @@ def test_two_threads(S):
     for t in ts:
         t.join()
     assert not bad
+
+
+@pytest.mark.parametrize("t,groups,nq,n,even", [("bf16", 1600, 3000, 20000, False), ("fp8", 1900, 1000, 9000, False),
+                                                ("f16", 2000, 2000, 20000, True)])
+def test_group_scores_many_groups(S, t, groups, nq, n, even):
+    _grouped(S, t, "f32", groups, nq, n, 72, 5, even, alpha=0.5, with_bias=True)
+
+
+@pytest.mark.parametrize("groups,most_q,most_v,empty", [(1536, 9, 300, 0.3), (1537, 9, 300, 0.3), (5000, 300, 40, 0.2),
+                                                        (150_000, 4, 20, 0.5), (150_000, 2, 9, 0.999), (40_000, 1, 3, 1.0)])
+def test_many_groups_exactly(S, groups, most_q, most_v, empty):
+    """Small integers, whose products and sums are exact: every score as it is."""
+    torch = _torch()
+    r = np.random.default_rng(groups + most_q)
+    m, c = r.integers(0, most_q + 1, groups), r.integers(0, most_v + 1, groups)
+    m[r.random(groups) < empty] = 0
+    m[groups // 3: groups // 2] = 0  # chunks without a score
+    c[r.random(groups) < 0.1] = 0
+    qo, vo = np.concatenate([[0], np.cumsum(m)]), np.concatenate([[0], np.cumsum(c)])
+    nq, n, total = int(qo[-1]) + 3, int(vo[-1]) + 5, int((m * c).sum())
+    g = torch.Generator(device="cuda").manual_seed(groups)
+    q = torch.randint(-3, 4, (nq, 40), device="cuda", generator=g).half()
+    v = torch.randint(-3, 4, (n, 40), device="cuda", generator=g).half()
+    tq, tv = torch.from_numpy(qo).cuda(), torch.from_numpy(vo).cuda()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    starts = S.group_rows(tq, tv, nq, n, status=status)
+    room = torch.full((total + 64,), 5.0, device="cuda")
+    S.group_scores(q, tq, v, tv, out=room, status=status)
+    assert int(status) == 0
+    want = np.concatenate([[0], np.cumsum(np.repeat(c, m)), [total] * 3])
+    np.testing.assert_array_equal(starts.cpu().numpy(), want)
+    at = torch.arange(total, device="cuda")
+    query = torch.searchsorted(starts, at, right=True) - 1
+    group = torch.searchsorted(tq, query, right=True) - 1
+    row = tv[group] + at - starts[query]
+    for a in range(0, total, 1 << 20):
+        b = slice(a, min(total, a + (1 << 20)))
+        assert bool((room[b] == (q[query[b]].float() * v[row[b]].float()).sum(1)).all())
+    assert bool((room[total:] == 5.0).all())
+
+
+def test_many_groups_bad_offsets(S):
+    """A bad group among many sets the status, wherever it is, and has no scores."""
+    torch = _torch()
+    groups = 4000
+    q, v = _gpu(_data(groups, 64, 1, 1.0), "bf16"), _gpu(_data(groups, 64, 2, 1.0), "bf16")
+    o = np.arange(groups + 1)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for at, value in ((0, -1), (1700, groups + 1), (groups, groups + 1), (2500, 7)):
+        bad = o.copy()
+        bad[at] = value
+        good, tb = torch.from_numpy(o).cuda(), torch.from_numpy(bad).cuda()
+        ok = (bad[:-1] >= 0) & (bad[1:] >= bad[:-1]) & (bad[1:] <= groups)
+        width = (bad[1:] - bad[:-1])[ok]
+        status.zero_()
+        room = torch.full((2 * groups,), 5.0, device="cuda")
+        S.group_scores(q, good, v, tb, out=room, status=status)
+        assert int(status) & 1
+        status.zero_()
+        starts = S.group_rows(good, tb, groups, groups, status=status)
+        assert int(status) & 1 and int(starts[-1]) == int(width.sum())
+        rows = np.concatenate([bad[g] + np.arange(bad[g + 1] - bad[g]) for g in np.flatnonzero(ok)])
+        want = (_np(q)[np.repeat(np.flatnonzero(ok), width)] * _np(v)[rows]).sum(1)
+        size = (np.abs(_np(q))[np.repeat(np.flatnonzero(ok), width)] * np.abs(_np(v)[rows])).sum(1)
+        # 64 products, exact in f32, summed with at most one rounding or truncation each
+        assert np.all(np.abs(_np(room[:len(want)]) - want) <= 64 * 2.0 ** -23 * size)
+        assert bool((room[len(want):] == 5.0).all())

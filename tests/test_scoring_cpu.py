@@ -54,6 +54,7 @@ def test_scores_refusals(raven_lib):
     assert group(4096, 4100, 1, 10) == EINVAL
     assert group(4096, 4096, 0, 10) == 0
     assert group(4096, 4096, 3, 0) == 0
+    assert group(4096, 4096, 1 << 31, 10) == L.RAVEN_ELIMIT
 
 
 def test_encode_decode_refusals(raven_lib):
@@ -89,6 +90,7 @@ def test_topk_and_group_rows_refusals(raven_lib):
     def rows(qo=4096, vo=4096, groups=2, nq=5, n=5, out=4096):
         return raven_lib.raven_group_rows_device(qo, vo, groups, nq, n, out, None, None)
 
+    assert rows(groups=1 << 31) == L.RAVEN_ELIMIT
     assert rows(qo=None) == L.RAVEN_EINVAL and rows(groups=0) == L.RAVEN_EINVAL and rows(out=4100) == L.RAVEN_EINVAL
     assert rows(nq=1 << 31) == L.RAVEN_ELIMIT
 
