@@ -97,6 +97,9 @@ struct Loader {
   static constexpr int kPer = 16 / (int)sizeof(T);
   static constexpr int kPieces = 16 / kPer;
   static constexpr int kE = 16;
+  // Low bits of a key that tell no values of the type apart: zeros of the f32
+  // image, ones of a negative's, and a sum with them.
+  static constexpr int kLow = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 13 : 16;
   __device__ static float get(const uint4& w, int c) {
     const uint32_t* u = &w.x;
     if constexpr (sizeof(T) == 4) {
@@ -144,9 +147,10 @@ __device__ inline float best_of(const uint4 (&v)[2], bool largest, const __nv_bf
 }
 
 // By one warp, N values per lane (0: none): the largest T that at least k of
-// them reach, 0 if fewer than k are there. `slack`: a T that is reached by up to
+// them reach, 0 if fewer than k are there. Bits below LOW tell no values apart
+// and are not tried (4096 rows of 6667 f16, k = 100: 67 to 63 us). `slack`: a T that is reached by up to
 // k + slack will do.
-template <int N>
+template <int LOW, int N>
 __device__ inline uint32_t kth_of_warp(const uint32_t (&v)[N], uint32_t k, uint32_t slack) {
   uint32_t hi = 0, lo = 0xffffffffu;
 #pragma unroll
@@ -159,7 +163,7 @@ __device__ inline uint32_t kth_of_warp(const uint32_t (&v)[N], uint32_t k, uint3
   if (hi == lo) return hi;
   int bit = 31 - __clz(hi ^ lo);
   uint32_t t = bit < 31 ? hi & ~((2u << bit) - 1u) : 0u;
-  for (; bit >= 0; --bit) {
+  for (; bit >= LOW; --bit) {
     const uint32_t next = t | (1u << bit);
     uint32_t c = 0;
 #pragma unroll
@@ -169,6 +173,13 @@ __device__ inline uint32_t kth_of_warp(const uint32_t (&v)[N], uint32_t k, uint3
       t = next;
       if (c <= k + slack) break;
     }
+  }
+  if (LOW && t) {  // a value there
+    uint32_t least = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (v[i] >= t) least = min(least, v[i]);
+    t = __reduce_min_sync(0xffffffffu, least);
   }
   return t;
 }
@@ -207,7 +218,7 @@ __device__ inline void sort_of_warp(uint64_t (&v)[N], uint32_t lane) {
     }
 }
 
-template <int TEAM, bool BIG>
+template <int TEAM, bool BIG, int LOW>
 struct Keeper {
   using TM = Team<TEAM, BIG>;
   static constexpr uint32_t kPrune = 1024;  // entries that one warp prunes
@@ -236,24 +247,37 @@ struct Keeper {
         t = kth_of_held<2>();
       else if (held <= kPrune / 4)
         t = kth_of_held<kPrune / 128>();
+      else if (held <= kPrune / 2)
+        t = kth_of_held<kPrune / 64>();
       else
         t = kth_of_held<kPrune / 32>();
-      if (tid == 0) s.bound = t;
+      // in place, 64 entries at a time, read before any of them is written over;
+      // the whole team did it slower (20000 rows of 500 f32, k = 30: 57, 53 us)
+      constexpr uint32_t U = 2;
+      uint32_t c = 0;
+      for (uint32_t i = tid; i < held + tid; i += 32 * U) {
+        uint64_t e[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) e[u] = i + 32 * u < held ? s.buf[i + 32 * u] : 0;
+        __syncwarp();
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+          const bool keep = e[u] && (uint32_t)(e[u] >> 32) >= t;
+          const uint32_t all = __ballot_sync(0xffffffffu, keep);
+          if (keep) s.buf[c + __popc(all & ((1u << tid) - 1u))] = e[u];
+          c += __popc(all);
+        }
+        __syncwarp();
+      }
+      if (tid == 0) {
+        s.bound = t;
+        s.count = c;
+      }
     }
-    // in place: entries are moved towards the front a round of the team at a
-    // time, and a round's reads come before its writes
-    const uint32_t c = held;
-    if (tid == 0) s.count = 0;
     TM::sync();
     const uint32_t t = s.bound;
-    for (uint32_t i = 0; i < c; i += TEAM) {
-      const uint64_t e = i + tid < c ? s.buf[i + tid] : 0;
-      TM::sync();
-      if (e && (uint32_t)(e >> 32) >= t) s.buf[atomicAdd(&s.count, 1u)] = e;
-      TM::sync();
-    }
     held = s.count;
-    TM::sync();
+    TM::sync();  // read by all before the next append
     if (held >= k) above = max(above, t);
     if (held > kPrune / 2) sort();  // many equals
   }
@@ -262,7 +286,7 @@ struct Keeper {
     uint32_t v[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = tid + 32 * i < held ? (uint32_t)(s.buf[tid + 32 * i] >> 32) : 0u;
-    return kth_of_warp(v, k, 0);
+    return kth_of_warp<LOW>(v, k, 0);
   }
 
   // The best k in order at the front, by sorting all.
@@ -448,7 +472,7 @@ struct Keeper {
       TM::sync();
       bound_of_tops<4>();
     } else if (TEAM == 32 && k > 32) {
-      const uint32_t t = kth_of_warp(key, k, k / 8);
+      const uint32_t t = kth_of_warp<LOW>(key, k, k / 8);
       if (t > 1) above = max(above, t - 1);
     } else {
       bound_of(max(max(top[0], top[1]), max(top[2], top[3])));
@@ -458,7 +482,7 @@ struct Keeper {
   __device__ void bound_of(uint32_t top) {
     if constexpr (TEAM == 32) {
       const uint32_t v[1] = {top};
-      const uint32_t t = kth_of_warp(v, k, k / 4);
+      const uint32_t t = kth_of_warp<LOW>(v, k, k / 4);
       if (t > kWorst) above = max(above, t - 1);
     } else {
       if (k > (uint32_t)TEAM) return;
@@ -473,7 +497,7 @@ struct Keeper {
       uint32_t v[PER * TEAM / 32];
 #pragma unroll
       for (int i = 0; i < PER * TEAM / 32; ++i) v[i] = s.top[tid + 32 * i];
-      const uint32_t t = kth_of_warp(v, k, k / 4);
+      const uint32_t t = kth_of_warp<LOW>(v, k, k / 4);
       if (tid == 0) s.bound = t;
     }
     TM::sync();
@@ -484,8 +508,8 @@ struct Keeper {
   }
 };
 
-template <int TEAM, bool BIG>
-__device__ inline void write_out(const Params& p, Keeper<TEAM, BIG>& kp, uint64_t row, uint32_t part, uint32_t parts) {
+template <int TEAM, bool BIG, int LOW>
+__device__ inline void write_out(const Params& p, Keeper<TEAM, BIG, LOW>& kp, uint64_t row, uint32_t part, uint32_t parts) {
   kp.finish();
   const uint64_t* best = kp.s.buf;
   const uint32_t c = kp.held;
@@ -533,7 +557,7 @@ __global__ void __launch_bounds__((Team<TEAM, BIG>::kThreads), TEAM == 32 ? 3 : 
   uint64_t each = len;
   if (p.parts > 1) each = ((len + p.parts - 1) / p.parts + kTile + L::kPer - 1) / kTile * kTile - L::kPer;
   const uint64_t from = min(len, each * part), to = min(len, from + each);
-  Keeper<TEAM, BIG> kp(*sh, tid, p.k, to - from);
+  Keeper<TEAM, BIG, Loader<T>::kLow> kp(*sh, tid, p.k, to - from);
   // pieces of 16 bytes from the boundary at or before the first element: the
   // bytes around a row are in the same 16 as some of its own
   const uint8_t* base = (const uint8_t*)p.x + (lo + from) * sizeof(T);
@@ -598,7 +622,7 @@ __global__ void __launch_bounds__(kCtaThreads) topk_join_kernel(const Params p) 
   extern __shared__ __align__(16) uint8_t raw[];
   raven_score::after_previous();
   const uint64_t row = blockIdx.x;
-  Keeper<TEAM, BIG> kp(*(Shared<TEAM, BIG>*)raw, threadIdx.x, p.k, p.n);
+  Keeper<TEAM, BIG, 0> kp(*(Shared<TEAM, BIG>*)raw, threadIdx.x, p.k, p.n);
   const uint64_t* x = (const uint64_t*)p.x + row * p.n;
   for (uint64_t t = 0; t < p.n; t += (uint64_t)TEAM * E) {
     uint32_t key[E];

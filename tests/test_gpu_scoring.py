@@ -782,3 +782,17 @@ def test_many_groups_bad_offsets(S):
         # 64 products, exact in f32, summed with at most one rounding or truncation each
         assert np.all(np.abs(_np(room[:len(want)]) - want) <= 64 * 2.0 ** -23 * size)
         assert bool((room[len(want):] == 5.0).all())
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("largest", [True, False])
+@pytest.mark.parametrize("k", [10, 40, 100, 256])
+def test_top_k_every_16_bit_value(S, t, largest, k):
+    """Rows of all values of a type, infinities, NaN and both zeros among them,
+    and rows of those nearest to zero, several of each."""
+    torch = _torch()
+    r = np.random.default_rng(k)
+    every = torch.from_numpy(np.arange(65536).astype(np.uint16).view(np.int16)).view(_dt(t)).double().numpy()
+    _top(S, np.stack([r.permutation(every) for _ in range(3)]), k, largest, t, False)
+    small = np.concatenate([every[:40], every[0x8000:0x8000 + 40]])
+    _top(S, np.stack([r.choice(small, 4000) for _ in range(1300)]), k, largest, t, False)
