@@ -500,6 +500,7 @@ int run_scores(const raven_rows* q, const int64_t* qo, const raven_rows* v, cons
   if (!fp8 && q->type != v->type) return fail(RAVEN_EINVAL, "queries must have the vectors' type");
   if (out_type != RAVEN_TYPE_F32 && out_type != RAVEN_TYPE_F16 && out_type != RAVEN_TYPE_BF16)
     return fail(RAVEN_EINVAL, "scores: type must be f32, f16 or bf16");
+  if (!aligned(bias, 4) || !aligned(status, 4)) return fail(RAVEN_EINVAL, "scores: bias and status must start on 4 bytes");
   if (q->rows == 0 || v->rows == 0 || groups == 0) return RAVEN_OK;
   if (!out && !(qo && capacity == 0)) return fail(RAVEN_EINVAL, "scores: null output");
   if (!aligned(out, type_size(out_type))) return fail(RAVEN_EINVAL, "scores: output is not aligned to its type");
@@ -733,6 +734,7 @@ int raven_group_rows_device(const int64_t* d_q_offsets, const int64_t* d_v_offse
   if (!d_q_offsets || !d_v_offsets || !d_row_starts) return fail(RAVEN_EINVAL, "null argument");
   if (!aligned(d_q_offsets, 8) || !aligned(d_v_offsets, 8) || !aligned(d_row_starts, 8))
     return fail(RAVEN_EINVAL, "offsets and row starts: not aligned to 64 bits");
+  if (!aligned(d_status, 4)) return fail(RAVEN_EINVAL, "status must start on 4 bytes");
   if (groups > kMaxRows) return fail(RAVEN_ELIMIT, "more than 2^31 - 1 groups");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;

@@ -55,6 +55,8 @@ def test_scores_refusals(raven_lib):
     assert group(4096, 4096, 0, 10) == 0
     assert group(4096, 4096, 3, 0) == 0
     assert group(4096, 4096, 1 << 31, 10) == L.RAVEN_ELIMIT
+    for bias, status in ((4098, None), (None, 4097)):
+        assert raven_lib.raven_scores_device(ok(), ok(), 128, 1.0, bias, 4096, 0, 8, status, None) == EINVAL
 
 
 def test_encode_decode_refusals(raven_lib):
@@ -91,6 +93,7 @@ def test_topk_and_group_rows_refusals(raven_lib):
         return raven_lib.raven_group_rows_device(qo, vo, groups, nq, n, out, None, None)
 
     assert rows(groups=1 << 31) == L.RAVEN_ELIMIT
+    assert raven_lib.raven_group_rows_device(4096, 4096, 2, 5, 5, 4096, 4098, None) == L.RAVEN_EINVAL
     assert rows(qo=None) == L.RAVEN_EINVAL and rows(groups=0) == L.RAVEN_EINVAL and rows(out=4100) == L.RAVEN_EINVAL
     assert rows(nq=1 << 31) == L.RAVEN_ELIMIT
 
