@@ -790,9 +790,10 @@ int raven_topk_rows_device(const void* d_scores, int32_t type, uint64_t nq, uint
   p.counts = d_counts;
   // A warp takes a row when rows are short, or so many that warps fill the GPU
   // and k is small (no barriers, and every warp's loads overlap the others' work:
-  // 10000 x 10007, k = 10, 94 us, by CTAs 120; 4096 x 6667, k = 100, 88 us, by CTAs
-  // 77: a warp's 32 maxima bound k = 100 loosely); else a CTA does. Where rows are too few to fill the
-  // GPU, each is split into parts of at least a tile. Ragged rows go by their mean.
+  // 10000 x 10007, k = 10, took 94 us by warps and 120 by CTAs, 4096 x 6667, k = 100,
+  // 88 and 77, since a warp's 32 maxima bound k = 100 loosely; those taken are at 82 and 61 by now); else
+  // a CTA does. Where rows are too few to fill the GPU, each is split into parts of
+  // at least a tile. Ragged rows go by their mean.
   const uint64_t len = d_row_starts ? (n + nq - 1) / nq : n;
   const bool warp = len <= 1024 || (nq >= 16ull * sms && k <= 32);
   const uint64_t tile = raven_topk::kCtaThreads * 16ull;
@@ -808,7 +809,7 @@ int raven_topk_rows_device(const void* d_scores, int32_t type, uint64_t nq, uint
   const bool big = 2 * k > (uint32_t)kCta;
   // With k above a warp's threads, selecting and ordering k is a chain of one warp
   // while its CTA waits: with rows enough, CTAs of half the threads keep twice as
-  // many such chains going (10000 x 10007, k = 100, 220 to 175 us).
+  // many such chains going (10000 x 10007 f32, k = 100, 220 to 179 us).
   const bool half = parts == 1 && k > 32 && nq >= 8ull * sms;
   cudaError_t e = warp                  ? dispatch_topk<32, false>(type, p, st)
                   : half && 2 * k > 128 ? dispatch_topk<128, true>(type, p, st)

@@ -148,8 +148,8 @@ __device__ inline float best_of(const uint4 (&v)[2], bool largest, const __nv_bf
 
 // By one warp, N values per lane (0: none): the largest T that at least k of
 // them reach, 0 if fewer than k are there. Bits below LOW tell no values apart
-// and are not tried (4096 rows of 6667 f16, k = 100: 67 to 63 us). `slack`: a T that is reached by up to
-// k + slack will do.
+// and are not tried (4096 rows of 6667 f16, k = 100: 67 to 63 us). `slack`: a T
+// that is reached by up to k + slack will do.
 template <int LOW, int N>
 __device__ inline uint32_t kth_of_warp(const uint32_t (&v)[N], uint32_t k, uint32_t slack) {
   uint32_t hi = 0, lo = 0xffffffffu;
