@@ -796,3 +796,36 @@ def test_top_k_every_16_bit_value(S, t, largest, k):
     _top(S, np.stack([r.permutation(every) for _ in range(3)]), k, largest, t, False)
     small = np.concatenate([every[:40], every[0x8000:0x8000 + 40]])
     _top(S, np.stack([r.choice(small, 4000) for _ in range(1300)]), k, largest, t, False)
+
+
+def test_many_groups_captured(S):
+    """Offsets that change between replays of one captured run over many groups."""
+    torch = _torch()
+    groups, nq, n = 10_000, 12_000, 30_000
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randint(-3, 4, (nq, 64), device="cuda", generator=g).bfloat16()
+    v = torch.randint(-3, 4, (n, 64), device="cuda", generator=g).bfloat16()
+
+    def offsets(total):
+        cuts = torch.randint(0, total + 1, (groups - 1,), device="cuda", generator=g).sort().values
+        return torch.cat([cuts.new_zeros(1), cuts, cuts.new_full((1,), total)])
+
+    qo, vo = offsets(nq), offsets(n)
+    out = torch.empty(400_000, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        S.group_scores(q, qo, v, vo, out=out, status=status)
+        starts = S.group_rows(qo, vo, nq, n)
+    for _ in range(3):
+        qo.copy_(offsets(nq))
+        vo.copy_(offsets(n))
+        graph.replay()
+        want = S.group_rows(qo, vo, nq, n)
+        total = int(want[-1])
+        assert total <= out.numel() and int(status) == 0
+        assert bool((starts == want).all())
+        at = torch.arange(total, device="cuda")
+        query = torch.searchsorted(want, at, right=True) - 1
+        row = vo[torch.searchsorted(qo, query, right=True) - 1] + at - want[query]
+        assert bool((out[:total] == (q[query].float() * v[row].float()).sum(1)).all())
