@@ -312,8 +312,12 @@ RAVEN_API int raven_group_scores_device(const raven_rows* q, const int64_t* d_q_
                                         int32_t* d_status, void* stream);
 
 /* d_row_starts[i] (nq + 1 values) = where query i's scores start in the packed
- * output; the last one is its size. Queries before the first group start at 0,
- * those behind the last group at the size. */
+ * output; the last one is its size. They rise. Queries before the first group
+ * start at 0, those behind the last group at the size, and those of a group that
+ * counts as empty where the scores of the groups before it end: none of them has
+ * scores. Where query offsets fall, a query that several groups cover has its
+ * place in one of them, the same every time, and a row that ends there may hold
+ * scores of the others too. */
 RAVEN_API int raven_group_rows_device(const int64_t* d_q_offsets, const int64_t* d_v_offsets, uint32_t groups,
                                       uint64_t nq, uint64_t n, int64_t* d_row_starts, int32_t* d_status, void* stream);
 

@@ -570,22 +570,59 @@ int run_scores(const raven_rows* q, const int64_t* qo, const raven_rows* v, cons
   return RAVEN_OK;
 }
 
+// A query's group is where a bisection of the offsets for it ends: by the first
+// offset (queries before it have no group), then bit by bit from the highest one
+// of the group's number, right of offset s where qo[s] <= i. So every query has
+// one place, a group with qo[g] <= i < qo[g + 1] or, as number `groups`, what is
+// behind the last, where offsets fall too (several groups cover a query there),
+// and places rise with their queries. Which offsets lead to place x does not
+// depend on the query; they bound its queries [lo, hi). By one warp, a bit of x
+// from `low` on per lane (one lane after the other took 2 to 3 us of a call more).
+__device__ inline void queries_of(const int64_t* qo, uint32_t groups, int64_t nq, uint32_t x, uint32_t low, int64_t& lo,
+                                  int64_t& hi) {
+  const uint32_t bit = threadIdx.x & 31, s = (x >> bit | 1u) << bit;
+  lo = max((int64_t)0, qo[0]);
+  hi = nq;
+  if (bit >= low && s <= groups) {
+    if (x >> bit & 1u)
+      lo = max(lo, qo[s]);
+    else
+      hi = min(hi, qo[s]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    lo = max(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = min(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+}
+
 // Where each query's scores start in grouped scores: starts[i] for query i of
-// group g is sum over earlier groups of m h_n plus its place times n_g. Blocks
-// take runs of 256 groups; each sums the groups before its run by itself, unless
-// the sums are given (many groups).
+// group g is sum over earlier groups of m h_n plus its place times n_g; a group
+// that counts as empty gives its queries the sum alone. Blocks take runs of 256
+// groups; each sums the groups before its run by itself, unless the sums are
+// given (many groups).
 __global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* qo, const int64_t* vo, uint32_t groups,
                                                          uint64_t nq, uint64_t n, const Chunk* chunks, int64_t* starts,
                                                          int* status) {
   after_previous();
   __shared__ int64_t part[256];
-  __shared__ int64_t gq[256], gm[256], gn[256];
+  __shared__ int64_t edge[256], ends[2][2];  // the run's offsets; its queries by the bits above it, those behind the last group
   const uint32_t g0 = blockIdx.x * 256u, tid = threadIdx.x;
   bool bad = false;
   auto read = [&](uint32_t g, int64_t& a, int64_t& m, int64_t& c) {
     int64_t v0;
     bad |= !raven_score::group_of(qo, vo, g, nq, n, a, v0, m, c);
   };
+  const bool last = g0 + 256 >= groups;
+  if (tid < 32 || (last && tid < 64)) {
+    int64_t lo, hi;
+    queries_of(qo, groups, (int64_t)nq, tid < 32 ? g0 : groups, tid < 32 ? 8 : 0, lo, hi);
+    if ((tid & 31) == 0) {
+      ends[tid >> 5][0] = lo;
+      ends[tid >> 5][1] = hi;
+    }
+  }
+  edge[tid] = g0 + tid <= groups ? qo[g0 + tid] : INT64_MAX;
   int64_t sum = 0, a, m, c;
   for (uint32_t g = tid; g < g0 && !chunks; g += 256) {
     read(g, a, m, c);
@@ -599,11 +636,21 @@ __global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* qo, cons
   }
   const int64_t before = chunks ? chunks[g0 / kChunk].out : part[0];
   __syncthreads();
+  int64_t lo = 0, hi = 0;
   a = m = c = 0;
-  if (g0 + tid < groups) read(g0 + tid, a, m, c);
-  gq[tid] = a;
-  gm[tid] = m;
-  gn[tid] = c;
+  if (g0 + tid < groups) {
+    read(g0 + tid, a, m, c);
+    lo = ends[0][0];
+    hi = ends[0][1];
+#pragma unroll
+    for (uint32_t bit = 0; bit < 8; ++bit) {
+      const int64_t x = edge[(tid >> bit | 1u) << bit];
+      if (tid >> bit & 1u)
+        lo = max(lo, x);
+      else
+        hi = min(hi, x);
+    }
+  }
   part[tid] = m * c;
   __syncthreads();
   for (int o = 1; o < 256; o <<= 1) {
@@ -612,22 +659,23 @@ __global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* qo, cons
     part[tid] += x;
     __syncthreads();
   }
-  for (uint32_t j = tid >> 5; j < 256; j += 8) {  // a warp per group
-    const int64_t base = before + part[j] - gm[j] * gn[j];
-    for (int64_t i = tid & 31; i < gm[j]; i += 32) starts[gq[j] + i] = base + i * gn[j];
+  const int64_t base = before + part[tid] - m * c - a * c;  // less what i * c below has too much
+  const bool few = hi - lo <= 8;  // queries of a group, written by its thread; more by its warp
+  for (int64_t i = lo; few && i < hi; ++i) starts[i] = base + i * c;
+  for (uint32_t left = __ballot_sync(0xffffffffu, !few); left; left &= left - 1) {
+    const int j = __ffs(left) - 1;
+    const int64_t end = __shfl_sync(0xffffffffu, hi, j), at = __shfl_sync(0xffffffffu, base, j);
+    const int64_t width = __shfl_sync(0xffffffffu, c, j);
+    for (int64_t i = __shfl_sync(0xffffffffu, lo, j) + (tid & 31); i < end; i += 32) starts[i] = at + i * width;
   }
   // queries before the first group start at 0, those behind the last one at the end
-  if (g0 + 256 >= groups) {
+  if (last) {
     const int64_t total = before + part[255];
-    int64_t last = qo[groups];
-    last = last < 0 ? 0 : last > (int64_t)nq ? (int64_t)nq : last;
-    for (int64_t i = last + tid; i <= (int64_t)nq; i += 256) starts[i] = total;
+    for (int64_t i = ends[1][0] + tid; i < ends[1][1]; i += 256) starts[i] = total;
+    if (tid == 0) starts[nq] = total;
   }
-  if (blockIdx.x == 0) {
-    int64_t first = qo[0];
-    first = first < 0 ? 0 : first > (int64_t)nq ? (int64_t)nq : first;
-    for (int64_t i = tid; i < first; i += 256) starts[i] = 0;
-  }
+  if (blockIdx.x == 0)
+    for (int64_t i = tid; i < min(qo[0], (int64_t)nq); i += 256) starts[i] = 0;
   if (bad && status) atomicOr(status, raven_score::kStatusOffsets);
 }
 

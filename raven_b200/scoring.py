@@ -296,7 +296,8 @@ def group_scores(queries: Rows, query_offsets: torch.Tensor, vectors: Rows, vect
 def group_rows(query_offsets: torch.Tensor, vector_offsets: torch.Tensor, nq: int, n: int,
                status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """int64 [nq + 1]: where each query's scores start in the output of
-    `group_scores`, and its size; the row_starts of `top_k`."""
+    `group_scores`, and its size; the row_starts of `top_k`. Queries of no group,
+    or of one whose offsets fall or leave the rows, have rows of no scores."""
     device = query_offsets.get_device()
     groups = _offsets("query_offsets", query_offsets, device)
     if _offsets("vector_offsets", vector_offsets, device) != groups:

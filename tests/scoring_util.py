@@ -69,3 +69,17 @@ def top_k(rows, k, largest):
         vals[i, : order.size] = r[order]
         ids[i, : order.size] = order
     return vals, ids, counts
+
+
+def group_starts(qo, vo, nq, n):
+    """Where each query's scores start, from the definition, for query offsets
+    that never fall: groups whose offsets fall or leave the rows have no scores."""
+    at, starts = 0, np.zeros(nq + 1, np.int64)
+    for g in range(len(qo) - 1):
+        a, b, c, d = (int(x) for x in (qo[g], qo[g + 1], vo[g], vo[g + 1]))
+        width = d - c if 0 <= a and b <= nq and 0 <= c <= d <= n else 0
+        for i in range(max(a, 0), min(b, nq)):
+            starts[i] = at + (i - a) * width
+        at += (b - a) * width
+        starts[max(min(b, nq), 0):] = at
+    return starts

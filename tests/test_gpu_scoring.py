@@ -829,3 +829,85 @@ def test_many_groups_captured(S):
         query = torch.searchsorted(want, at, right=True) - 1
         row = vo[torch.searchsorted(qo, query, right=True) - 1] + at - want[query]
         assert bool((out[:total] == (q[query].float() * v[row].float()).sum(1)).all())
+
+
+# ---- rows beside malformed groups -----------------------------------------------------
+
+
+def _poisoned_starts(S, qo, vo, nq, n):
+    """The row starts written over memory that holds something else, and the status."""
+    torch = _torch()
+    from raven_b200 import _lib as L
+
+    out = torch.full((nq + 1,), -12345, dtype=torch.int64, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    tq, tv = torch.from_numpy(np.asarray(qo, np.int64)).cuda(), torch.from_numpy(np.asarray(vo, np.int64)).cuda()
+    L.check(L.load().raven_group_rows_device(tq.data_ptr(), tv.data_ptr(), len(qo) - 1, nq, n, out.data_ptr(),
+                                             status.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    return out, int(status)
+
+
+@pytest.mark.parametrize("qo,vo", [([0, 10, 20], [0, 30, 20]), ([0, 10, 25], [0, 10, 20]), ([-5, 4, 20], [0, 10, 20]),
+                                   ([0, 5, 5, 12, 20], [0, 31, 8, 8, 30]), ([0, 7, 20], [-1, 4, 1 << 62]),
+                                   ([21, 30, 40], [0, 4, 5]), ([-9, -3, -1], [0, 4, 5]),
+                                   ([3, 9, 14], [4, 2, 9]), ([-(1 << 60), 20, 1 << 62], [0, 30, 30])])
+def test_group_rows_beside_malformed_groups(S, qo, vo):
+    """Every start is written, and the queries of sound groups have the rows of theirs."""
+    torch = _torch()
+    starts, status = _poisoned_starts(S, qo, vo, 20, 30)
+    np.testing.assert_array_equal(starts.cpu().numpy(), U.group_starts(qo, vo, 20, 30))
+    assert status == int(any(a > b or a < 0 or b > lim for o, lim in ((qo, 20), (vo, 30)) for a, b in zip(o[:-1], o[1:])))
+    # the neighbours' best scores are those of their own group's vectors
+    q, v = _gpu(_data(20, 64, 1, 1.0), "bf16"), _gpu(_data(30, 64, 2, 1.0), "bf16")
+    packed = S.group_scores(q, torch.tensor(qo, device="cuda"), v, torch.tensor(vo, device="cuda"), total=int(starts[-1]))
+    vals, ids, counts = S.top_k(packed, 4, row_starts=starts)
+    full = S.scores(q, v)
+    for g in range(len(qo) - 1):
+        sound = 0 <= qo[g] <= qo[g + 1] <= 20 and 0 <= vo[g] <= vo[g + 1] <= 30
+        for i in range(max(qo[g], 0), min(qo[g + 1], 20)):
+            part = _np(full[i, vo[g]:vo[g + 1]]) if sound else np.zeros(0)
+            wv, wi, wc = U.top_k([part], 4, True)
+            assert int(counts[i]) == wc[0]
+            np.testing.assert_array_equal(ids[i].cpu().numpy(), wi[0])
+            np.testing.assert_array_equal(_np(vals[i]), wv[0])
+
+
+@pytest.mark.parametrize("groups", [700, 8192, 9000])
+def test_group_rows_beside_malformed_groups_among_many(S, groups):
+    r = np.random.default_rng(groups)
+    for _ in range(3):
+        qo = np.concatenate([[0], np.cumsum(r.integers(0, 5, groups))])
+        vo = np.concatenate([[0], np.cumsum(r.integers(0, 40, groups))])
+        nq, n = int(qo[-1]) - 3, int(vo[-1]) - 30  # the last groups leave the rows
+        vo[r.integers(1, groups, 20)] = r.integers(-5, n + 5, 20)
+        starts, status = _poisoned_starts(S, qo, vo, nq, n)
+        assert status == 1
+        np.testing.assert_array_equal(starts.cpu().numpy(), U.group_starts(qo, vo, nq, n))
+
+
+@pytest.mark.parametrize("groups", [3, 40, 900, 9000])
+def test_group_rows_where_query_offsets_fall(S, groups):
+    """Several groups cover a query: its place is in one of them, the same every
+    time, starts rise, and none is left as it was."""
+    r = np.random.default_rng(groups)
+    nq, n = 500, 50
+    for turn in range(6):
+        qo = r.integers(-20, nq + 20, groups + 1)
+        qo[: groups // 2] = np.sort(qo[: groups // 2])
+        vo = np.sort(r.integers(0, n + 1, groups + 1))
+        starts, status = _poisoned_starts(S, qo, vo, nq, n)
+        got = starts.cpu().numpy()
+        for _ in range(3):
+            np.testing.assert_array_equal(_poisoned_starts(S, qo, vo, nq, n)[0].cpu().numpy(), got)
+        assert status == int(np.any(qo[1:] < qo[:-1]) or qo.min() < 0 or qo.max() > nq)
+        assert got[0] >= 0 and np.all(np.diff(got) >= 0)
+        sound = (qo[:-1] >= 0) & (qo[1:] >= qo[:-1]) & (qo[1:] <= nq)
+        size = np.where(sound, (qo[1:] - qo[:-1]) * (vo[1:] - vo[:-1]), 0)
+        base = np.concatenate([[0], np.cumsum(size)])
+        assert got[nq] == base[-1]
+        for i in range(nq):
+            may = {0} if i < qo[0] else set()
+            may |= {int(base[-1])} if i >= qo[-1] else set()
+            for g in np.flatnonzero((qo[:-1] <= i) & (i < qo[1:])):
+                may.add(int(base[g] + ((i - qo[g]) * (vo[g + 1] - vo[g]) if sound[g] else 0)))
+            assert int(got[i]) in may
