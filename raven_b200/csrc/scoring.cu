@@ -529,7 +529,7 @@ int run_scores(const raven_rows* q, const int64_t* qo, const raven_rows* v, cons
   p.out_type = out_type == RAVEN_TYPE_F32 ? raven_score::kOutF32
                : out_type == RAVEN_TYPE_F16 ? raven_score::kOutF16 : raven_score::kOutBf16;
   p.ld = ld;
-  p.capacity = capacity;
+  p.capacity = std::min<uint64_t>(capacity, 1ull << 62);  // signed on the device; no output is larger
   p.status = status;
   // instruction descriptor, M = 128. FP8: types e4m3 (0), exponent scales (bit 23);
   // 16-bit: f32 accumulator (bit 4), types f16 (0) or bf16 (1)

@@ -911,3 +911,20 @@ def test_group_rows_where_query_offsets_fall(S, groups):
             for g in np.flatnonzero((qo[:-1] <= i) & (i < qo[1:])):
                 may.add(int(base[g] + ((i - qo[g]) * (vo[g + 1] - vo[g]) if sound[g] else 0)))
             assert int(got[i]) in may
+
+
+@pytest.mark.parametrize("capacity", [35, (1 << 63) - 1, 1 << 63, (1 << 64) - 1])
+def test_group_scores_any_capacity(S, capacity):
+    """A caller who knows that the output is large enough may give any capacity."""
+    torch = _torch()
+    from raven_b200 import _lib as L
+
+    q, v = _gpu(_data(5, 64, 1, 1.0), "f16"), _gpu(_data(7, 64, 2, 1.0), "f16")
+    qo, vo = torch.tensor([0, 5], device="cuda"), torch.tensor([0, 7], device="cuda")
+    out, status = torch.full((36,), 9.0, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    rows = [L.Rows(x.data_ptr(), None, len(x), 64, 0, L.RAVEN_TYPE_F16) for x in (q, v)]
+    L.check(L.load().raven_group_scores_device(rows[0], qo.data_ptr(), rows[1], vo.data_ptr(), 1, 64, 1.0, None,
+                                               out.data_ptr(), L.RAVEN_TYPE_F32, capacity, status.data_ptr(),
+                                               torch.cuda.current_stream().cuda_stream))
+    assert int(status) == 0 and float(out[35]) == 9.0
+    assert bool((out[:35].view(5, 7) == S.scores(q, v)).all())
