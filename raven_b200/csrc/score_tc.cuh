@@ -215,6 +215,10 @@ __device__ __noinline__ uint32_t chunk_of_tile(const Chunk* chunks, uint32_t cou
 // which mostly share a chunk (65536 groups of 1 x 8 scores 1400 to 313 us).
 // The lane that holds a tile's group works out the tile. Its divisions are 32-bit
 // ones unless the group has 2^32 tiles.
+// A group whose scores start past the output's capacity ends the CTA's tiles:
+// what they hold cannot be stored, and offsets that fall again and again could
+// ask for any amount of it. It also keeps the place of a tile's scores below
+// 2^62 plus a group's, so sums with it do not wrap.
 template <typename L, bool MANY>
 struct TileFinder {
   static constexpr uint32_t TQ = L::kTileQ;
@@ -233,7 +237,8 @@ struct TileFinder {
   uint64_t t;               // the CTA's next tile
   uint64_t skip;            // from the last tile of a run to the next run
   uint32_t run = 1, left;   // consecutive tiles that the CTA takes, how many are left
-  bool bad = false;
+  uint32_t open = 0;        // lanes whose group's scores start within the output
+  bool bad = false, past = false;
 
   __device__ TileFinder(const Params& p_, int lane_) : p(p_), lane(lane_), rows(L::kTileV * p_.subs - p_.halo) {
     if constexpr (MANY) {
@@ -282,6 +287,8 @@ struct TileFinder {
       }
     }
     before = e - (int64_t)m * nn;
+    // (unsigned: a sum of wild offsets that has wrapped is past it too)
+    open = __ballot_sync(0xffffffffu, !p.qo || (uint64_t)out0 + (uint64_t)before < p.capacity);
     chunk_tiles = __shfl_sync(0xffffffffu, incl, 31);
     chunk_out = __shfl_sync(0xffffffffu, e, 31);
   }
@@ -304,7 +311,15 @@ struct TileFinder {
       load();
       if (MANY) break;  // it is this one
     }
-    return __ffs(__ballot_sync(0xffffffffu, t - first < incl)) - 1;
+    const int at = __ffs(__ballot_sync(0xffffffffu, t - first < incl)) - 1;
+    if (at < 0 || (open >> at & 1u)) return at;
+    past = true;
+    if (!MANY)  // the offsets behind it are looked at all the same
+      for (uint32_t g = g0 + kChunk; g < p.groups; g += kChunk) {
+        g0 = g;
+        load();
+      }
+    return -1;
   }
   // Tile t of this lane's group.
   __device__ Tile tile() const {
@@ -779,7 +794,8 @@ __global__ void __launch_bounds__((Layout<FP8, BN, ROWS, HELD>::kThreads), 1)
         wr.next();
         if (at < 0) break;
       }
-      if (__any_sync(0xffffffffu, finder.bad) && lane == 0 && p.status) atomicOr(p.status, kStatusOffsets);
+      const int bits = (__any_sync(0xffffffffu, finder.bad) ? kStatusOffsets : 0) | (finder.past ? kStatusCapacity : 0);
+      if (bits && lane == 0 && p.status) atomicOr(p.status, bits);
     };
     if (p.chunks)
       find_tiles(TileFinder<L, true>(p, lane));
@@ -811,11 +827,11 @@ __global__ void __launch_bounds__((Layout<FP8, BN, ROWS, HELD>::kThreads), 1)
       if (lane == 0) mbar_arrive(info_empty(rd.slot));
       rd.next();
       if (t.qcnt == 0) break;
-      // queries whose scores of this tile lie within the output (a sum of wild offsets may have wrapped)
+      // queries whose scores of this tile lie within the output
       uint32_t qcnt = t.qcnt;
-      if (p.qo && (t.out < 0 || t.out + (int64_t)(qcnt - 1) * t.ld + t.vext > (int64_t)p.capacity)) {
+      if (p.qo && t.out + (int64_t)(qcnt - 1) * t.ld + t.vext > (int64_t)p.capacity) {
         const int64_t room = (int64_t)p.capacity - t.out - (int64_t)t.vext;
-        qcnt = room < 0 || t.out < 0 ? 0u : (uint32_t)min(room / t.ld + 1, (int64_t)qcnt);
+        qcnt = room < 0 ? 0u : (uint32_t)min(room / t.ld + 1, (int64_t)qcnt);
         if (lane == 0 && p.status && qcnt < t.qcnt) atomicOr(p.status, kStatusCapacity);
       }
       if (!warp_wait(acc_full(b), bph)) {

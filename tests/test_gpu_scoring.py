@@ -928,3 +928,37 @@ def test_group_scores_any_capacity(S, capacity):
                                                torch.cuda.current_stream().cuda_stream))
     assert int(status) == 0 and float(out[35]) == 9.0
     assert bool((out[:35].view(5, 7) == S.scores(q, v)).all())
+
+
+@pytest.mark.parametrize("groups", [1501, 3001])
+def test_group_scores_end_at_the_capacity(S, groups):
+    """Offsets that fall again and again, so that hundreds of groups cover all
+    rows: the work is that of the groups that reach into the output, not of all."""
+    torch = _torch()
+    nq = n = 60_000
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randint(-3, 4, (nq, 64), device="cuda", generator=g).half()
+    v = torch.randint(-3, 4, (n, 64), device="cuda", generator=g).half()
+    fit = 9 * n + 50
+    out = torch.full((fit + 100,), 5.0, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def run(offsets, want_status):
+        o = torch.tensor(offsets, device="cuda")
+        for timed in (False, True):
+            out.fill_(5.0)
+            status.zero_()
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            S.group_scores(q, o, v, o, out=out[:fit], status=status)
+            b.record()
+            b.synchronize()
+        assert int(status) == want_status
+        assert bool((out[:9 * n].view(9, n) == q[:9].float() @ v.float().T).all()) and bool((out[fit:] == 5.0).all())
+        return a.elapsed_time(b)
+
+    one = run([0, nq], 2)
+    many = run([0, nq] * ((groups + 1) // 2), 3)
+    assert many <= 50 * one + 5.0, (one, many)  # (groups + 1) / 2 times one if all were computed
+    # a bad group far behind the output's end is still told of
+    assert run([0, nq] + [nq] * (groups - 2) + [nq + 1], 3) <= 50 * one + 5.0
