@@ -252,7 +252,9 @@ RAVEN_API int raven_merge_topk_gathered_device(const void* d_gathered, uint32_t 
 #define RAVEN_TYPE_BF16 2
 #define RAVEN_TYPE_FP8 3 /* e4m3 codes, one power-of-two scale per 128 values */
 
-/* bits of *d_status, which calls only ever set (the caller clears it) */
+/* bits of *d_status, which calls only ever set (the caller clears it). Calls with
+ * a NULL d_status set them in a word of the device that raven_scoring_status_device
+ * takes: nothing else tells of them, since calls do not wait for their kernels. */
 #define RAVEN_S_OFFSETS 1  /* a group's offsets fall or leave the rows: it counted as empty */
 #define RAVEN_S_CAPACITY 2 /* scores past the output's capacity were not written */
 #define RAVEN_S_WAIT 4     /* a wait inside the kernel (each is bounded) ran out: the scores are not valid */
@@ -294,7 +296,7 @@ RAVEN_API int raven_index_fp8_device(raven_index* ix, uint8_t* d_codes, uint64_t
  * in f32 on the tensor cores and rounded once to out_type (f32, f16, bf16).
  * alpha = -2 with d_bias[j] = |v_j|^2 gives squared distances less |q_i|^2.
  * Vectors are FP8, f16 or bf16; queries have the same type, or, with FP8
- * vectors, any type (they are encoded first). d_status may be NULL. */
+ * vectors, any type (they are encoded first). */
 RAVEN_API int raven_scores_device(const raven_rows* q, const raven_rows* v, uint32_t dim, float alpha,
                                   const float* d_bias, void* d_out, int32_t out_type, uint64_t ld_out,
                                   int32_t* d_status, void* stream);
@@ -305,7 +307,8 @@ RAVEN_API int raven_scores_device(const raven_rows* q, const raven_rows* v, uint
  * empty on either side. Output packed: groups in order, in a group its queries in order, for
  * each the scores of the group's vectors. Nothing past `capacity` elements is
  * written: queries whose scores all fit have them, of the next one some may be
- * there. Queries outside every group have no scores. */
+ * there. Queries outside every group have no scores. A call with no capacity and
+ * no d_status does nothing, nor does one without queries or vectors. */
 RAVEN_API int raven_group_scores_device(const raven_rows* q, const int64_t* d_q_offsets, const raven_rows* v,
                                         const int64_t* d_v_offsets, uint32_t groups, uint32_t dim, float alpha,
                                         const float* d_bias, void* d_out, int32_t out_type, uint64_t capacity,
@@ -320,6 +323,11 @@ RAVEN_API int raven_group_scores_device(const raven_rows* q, const int64_t* d_q_
  * scores of the others too. */
 RAVEN_API int raven_group_rows_device(const int64_t* d_q_offsets, const int64_t* d_v_offsets, uint32_t groups,
                                       uint64_t nq, uint64_t n, int64_t* d_row_starts, int32_t* d_status, void* stream);
+
+/* Sets in *d_status (on the current device) the bits that calls without a
+ * d_status have set on this device since they were last taken, in `stream`'s
+ * order, and clears those. */
+RAVEN_API int raven_scoring_status_device(int32_t* d_status, void* stream);
 
 /* The best k (1..256) scores of each of nq rows, best first (largest, or
  * smallest with largest = 0), equal scores by the lower index, NaN after every

@@ -170,6 +170,7 @@ SIGNATURES = {
                                             C.c_void_p, C.c_void_p]),
     "raven_group_rows_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint64, C.c_uint64, C.c_void_p,
                                           C.c_void_p, C.c_void_p]),
+    "raven_scoring_status_device": (C.c_int, [C.c_void_p, C.c_void_p]),
     "raven_topk_rows_device": (C.c_int, [C.c_void_p, C.c_int32, C.c_uint64, C.c_uint64, C.c_uint64, C.c_void_p,
                                          C.c_uint32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "raven_limits": (None, [C.POINTER(Limits)]),

@@ -77,6 +77,11 @@ constexpr uint32_t kHeldUnits = 32;    // and query blocks that it encodes
 enum : int { kOutF32 = 0, kOutF16 = 1, kOutBf16 = 2 };
 enum : int { kStatusOffsets = 1, kStatusCapacity = 2, kStatusWait = 4 };
 
+// The status of calls that are given no word for it, per device, until it is taken
+// (raven_scoring_status_device).
+__device__ int g_status;
+__device__ inline void tell(int* status, int bits) { atomicOr(status ? status : &g_status, bits); }
+
 // Sums over the groups before a chunk of 32 groups: their tiles, their scores.
 struct alignas(16) Chunk {
   int64_t tiles, out;
@@ -121,7 +126,7 @@ struct Params {
   int out_type;
   uint64_t ld;                // dense: output pitch; grouped: the pitch is the group's rows
   uint64_t capacity;          // grouped: output elements
-  int* status;                // or null
+  int* status;                // null: g_status
 };
 
 struct Tile {
@@ -795,7 +800,7 @@ __global__ void __launch_bounds__((Layout<FP8, BN, ROWS, HELD>::kThreads), 1)
         if (at < 0) break;
       }
       const int bits = (__any_sync(0xffffffffu, finder.bad) ? kStatusOffsets : 0) | (finder.past ? kStatusCapacity : 0);
-      if (bits && lane == 0 && p.status) atomicOr(p.status, bits);
+      if (bits && lane == 0) tell(p.status, bits);
     };
     if (p.chunks)
       find_tiles(TileFinder<L, true>(p, lane));
@@ -832,7 +837,7 @@ __global__ void __launch_bounds__((Layout<FP8, BN, ROWS, HELD>::kThreads), 1)
       if (p.qo && t.out + (int64_t)(qcnt - 1) * t.ld + t.vext > (int64_t)p.capacity) {
         const int64_t room = (int64_t)p.capacity - t.out - (int64_t)t.vext;
         qcnt = room < 0 ? 0u : (uint32_t)min(room / t.ld + 1, (int64_t)qcnt);
-        if (lane == 0 && p.status && qcnt < t.qcnt) atomicOr(p.status, kStatusCapacity);
+        if (lane == 0 && qcnt < t.qcnt) tell(p.status, kStatusCapacity);
       }
       if (!warp_wait(acc_full(b), bph)) {
         ok = false;
@@ -931,7 +936,7 @@ __global__ void __launch_bounds__((Layout<FP8, BN, ROWS, HELD>::kThreads), 1)
       }
     }
   }
-  if (!ok && lane == 0 && p.status) atomicOr(p.status, kStatusWait);
+  if (!ok && lane == 0) tell(p.status, kStatusWait);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(256) group_chunks_kernel(const int64_t* qo, co
     out += __shfl_xor_sync(0xffffffffu, out, o);
   }
   if (lane == 0 && g < groups) chunks[g / kChunk] = Chunk{tiles, out};
-  if (__any_sync(0xffffffffu, bad) && lane == 0 && status) atomicOr(status, raven_score::kStatusOffsets);
+  if (__any_sync(0xffffffffu, bad) && lane == 0) raven_score::tell(status, raven_score::kStatusOffsets);
 }
 
 // Chunks' sums to sums over the chunks before; chunks[count]: over all. One CTA.
@@ -676,7 +676,12 @@ __global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* qo, cons
   }
   if (blockIdx.x == 0)
     for (int64_t i = tid; i < min(qo[0], (int64_t)nq); i += 256) starts[i] = 0;
-  if (bad && status) atomicOr(status, raven_score::kStatusOffsets);
+  if (bad) raven_score::tell(status, raven_score::kStatusOffsets);
+}
+
+__global__ void status_kernel(int* status) {
+  after_previous();
+  atomicOr(status, atomicExch(&raven_score::g_status, 0));
 }
 
 // ---------------------------------------------------------------------------
@@ -769,7 +774,7 @@ int raven_group_scores_device(const raven_rows* q, const int64_t* d_q_offsets, c
   if (groups && (!aligned(d_q_offsets, 8) || !aligned(d_v_offsets, 8)))
     return fail(RAVEN_EINVAL, "offsets: not aligned to 64 bits");
   if (groups > kMaxRows) return fail(RAVEN_ELIMIT, "more than 2^31 - 1 groups");
-  if (capacity == 0 && !d_status) groups = 0;  // nothing to write, nor anyone to tell
+  if (capacity == 0 && !d_status) groups = 0;  // a call for nothing
   return run_scores(q, d_q_offsets, v, d_v_offsets, groups, dim, alpha, d_bias, d_out, out_type, 0, capacity, d_status,
                     stream);
 }
@@ -799,6 +804,15 @@ int raven_group_rows_device(const int64_t* d_q_offsets, const int64_t* d_v_offse
                d_row_starts, d_status);
   if (chunks) cudaFreeAsync(chunks, st);
   CU(e);
+  return RAVEN_OK;
+}
+
+int raven_scoring_status_device(int32_t* d_status, void* stream) {
+  NvtxRange nvtx_range("raven.scoring_status");
+  if (!d_status) return fail(RAVEN_EINVAL, "null status");
+  if (!aligned(d_status, 4)) return fail(RAVEN_EINVAL, "status must start on 4 bytes");
+  static Allowed none;
+  CU(launch(status_kernel, 1, 1, 0, none, (cudaStream_t)stream, d_status));
   return RAVEN_OK;
 }
 

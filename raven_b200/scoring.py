@@ -9,6 +9,7 @@
                    collection, or one projection per group.
 * `group_rows`   — where each query's scores start in grouped scores.
 * `top_k`        — the best k of each row of scores, dense or packed.
+* `take_status`  — what went wrong on a device in calls without a status.
 
     rows = Fp8Rows.encode(X)                              # or Fp8Rows.of_index(searcher.device_index)
     near = scores(Q, rows, alpha=-2.0, bias=(rows.decode() ** 2).sum(1))
@@ -240,7 +241,8 @@ def scores(queries: Rows, vectors: Rows, *, alpha: float = 1.0, bias: Optional[t
     summed in float32 on the tensor cores, rounded once. Float queries against
     FP8 rows are encoded first. alpha = -2 with the vectors' squared norms as
     bias ranks like squared distances. `out`: a matrix of `dtype` to write (any
-    row pitch). `status`: an int32 that gets RAVEN_S_* bits."""
+    row pitch). `status`: an int32 that gets RAVEN_S_* bits; without it
+    `take_status` tells whether the scores are valid."""
     device, dim, nq, n, q, v, keep = _operands(queries, vectors, dtype, bias)
     pitch = n
     if out is None:
@@ -275,7 +277,9 @@ def group_scores(queries: Rows, query_offsets: torch.Tensor, vectors: Rows, vect
     `total` is the number of scores (the program that made the groups knows it:
     the sum of queries times vectors; the last of `group_rows`), or `out` a 1-D
     tensor with room for them. Nothing is written past it: queries whose scores
-    all fit have them, and `status` gets RAVEN_S_CAPACITY."""
+    all fit have them, and `status` gets RAVEN_S_CAPACITY. Groups whose offsets fall
+    or leave the rows have no scores, and it gets RAVEN_S_OFFSETS; without a
+    `status`, `take_status` tells of both."""
     device, dim, nq, n, q, v, keep = _operands(queries, vectors, dtype, bias)
     groups = _offsets("query_offsets", query_offsets, device)
     if _offsets("vector_offsets", vector_offsets, device) != groups:
@@ -310,6 +314,18 @@ def group_rows(query_offsets: torch.Tensor, vector_offsets: torch.Tensor, nq: in
     _call(device, L.load().raven_group_rows_device, query_offsets.data_ptr(), vector_offsets.data_ptr(), groups, nq, n,
           out.data_ptr(), _status(status, device))
     return out
+
+
+def take_status(device=None) -> int:
+    """The RAVEN_S_* bits that calls without a `status` have set on a GPU (the
+    current one) since they were last taken: 0 when all went well. Waits for the
+    current stream; calls on others may add theirs later."""
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError("device must be a GPU")
+    bits = torch.zeros(1, dtype=torch.int32, device=device)
+    _call(bits.get_device(), L.load().raven_scoring_status_device, bits.data_ptr())
+    return int(bits)
 
 
 def top_k(scores: torch.Tensor, k: int, *, largest: bool = True,

@@ -962,3 +962,43 @@ def test_group_scores_end_at_the_capacity(S, groups):
     assert many <= 50 * one + 5.0, (one, many)  # (groups + 1) / 2 times one if all were computed
     # a bad group far behind the output's end is still told of
     assert run([0, nq] + [nq] * (groups - 2) + [nq + 1], 3) <= 50 * one + 5.0
+
+
+def test_status_of_calls_without_one(S):
+    """What goes wrong in calls without a status is kept until it is taken."""
+    torch = _torch()
+    q, v = _gpu(_data(20, 64, 1, 1.0), "bf16"), _gpu(_data(30, 64, 2, 1.0), "bf16")
+    o = lambda *x: torch.tensor(x, device="cuda")  # noqa: E731
+    S.take_status()
+    S.scores(q, v)
+    S.group_scores(q, o(0, 20), v, o(0, 30), total=600)
+    S.group_rows(o(0, 20), o(0, 30), 20, 30)
+    assert S.take_status() == 0
+    S.group_scores(q, o(0, 20), v, o(0, 30), total=599)
+    S.group_scores(q, o(0, 20), v, o(0, 30), total=600)  # does not clear it
+    assert S.take_status("cuda:0") == 2 and S.take_status() == 0
+    S.group_scores(q, o(0, 20), v, o(0, 30), total=0)  # asks for nothing
+    assert S.take_status() == 0
+    S.group_scores(q, o(0, 10, 5), v, o(0, 10, 20), total=600)
+    assert S.take_status() == 1
+    S.group_rows(o(0, 20), o(0, 31), 20, 30)
+    assert S.take_status() == 1
+    falls = torch.arange(3002, device="cuda").flip(0)  # many groups
+    S.group_scores(q, falls, v, falls, total=600)
+    assert S.take_status() == 1
+    # a call with a status of its own says nothing here
+    own = torch.zeros(1, dtype=torch.int32, device="cuda")
+    S.group_scores(q, o(0, 20), v, o(0, 31), total=600, status=own)
+    assert int(own) == 1 and S.take_status() == 0
+    # in a captured run
+    qo, vo = o(0, 20), o(0, 30)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        S.group_scores(q, qo, v, vo, total=600)
+    graph.replay()
+    assert S.take_status() == 0
+    vo[1] = 31
+    graph.replay()
+    assert S.take_status() == 1
+    with pytest.raises(ValueError):
+        S.take_status("cpu")

@@ -143,3 +143,10 @@ def test_definitions():
     assert U.fp8_exponents(np.array([[448.0], [449.0], [0.0], [224.0], [1e-42]])).ravel().tolist() == [0, 1, 0, -1, -127]
     vals, ids, counts = U.top_k([[1.0, np.nan, 1.0, np.inf], []], 3, True)
     assert ids.tolist() == [[3, 0, 2], [0, 0, 0]] and counts.tolist() == [3, 0]
+
+
+def test_status_refusals(raven_lib):
+    from raven_b200 import _lib as L
+
+    assert raven_lib.raven_scoring_status_device(None, None) == L.RAVEN_EINVAL
+    assert raven_lib.raven_scoring_status_device(4098, None) == L.RAVEN_EINVAL
