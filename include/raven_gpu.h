@@ -261,7 +261,8 @@ RAVEN_API int raven_merge_topk_gathered_device(const void* d_gathered, uint32_t 
 
 /* Rows of `dim` values, row i at data + i * ld values (codes). FP8 rows also
  * have exponent bytes, row i at exps + i * ld_exps, one per 128 values: a value
- * is its code times 2^(byte - 127). Layout of FP8 rows: codes start on 16 bytes
+ * is its code times 2^(byte - 127), or NaN where the byte is 255 (encoding never
+ * makes one; the largest is 247). Layout of FP8 rows: codes start on 16 bytes
  * and ld is a multiple of 16; exps start on 4 bytes and ld_exps is a multiple
  * of 4, at least ceil(dim / 128). f16 and bf16 rows start on 16 bytes and ld is
  * a multiple of 8; queries that a call encodes may have any ld >= dim. */

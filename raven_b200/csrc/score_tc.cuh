@@ -5,7 +5,7 @@
 //   S[i, j] = alpha * sum_t q[i, t] v[j, t] + bias[j]
 //
 // FP8 rows are e4m3 codes with one exponent byte per block of 128 values
-// (value = code * 2^(byte - 127)). The block's exponents go to the tensor core
+// (value = code * 2^(byte - 127), byte 255 NaN). The block's exponents go to the tensor core
 // beside the codes (kind::mxf8f6f4 with block scaling): a power of two scales a
 // product exactly, so all blocks of a row sum in one f32 accumulator and
 // nothing is rescaled in registers. The instruction takes an exponent for each

@@ -234,7 +234,9 @@ __global__ void __launch_bounds__(256) fp8_decode_kernel(const uint8_t* codes, u
     const uint64_t row = t / dim;
     const uint32_t d = (uint32_t)(t - row * dim);
     const __half_raw h = __nv_cvt_fp8_to_halfraw(codes[row * ld_codes + d], __NV_E4M3);
-    out[row * ld + d] = ldexpf(__half2float(*(const __half*)&h), (int)exps[row * ld_exps + d / kBlock] - 127);
+    const int e = exps[row * ld_exps + d / kBlock];
+    // 255 is the scales' NaN, as the tensor cores take it
+    out[row * ld + d] = e == 255 ? __int_as_float(0x7fc00000) : ldexpf(__half2float(*(const __half*)&h), e - 127);
   }
 }
 

@@ -95,7 +95,7 @@ def aligned_rows(x: torch.Tensor) -> torch.Tensor:
 class Fp8Rows:
     """Rows held as FP8: `codes` uint8 [n, roundup(dim, 16)] (e4m3) and `exps`
     uint8 [n, roundup(ceil(dim / 128), 4)]; a value is its code times
-    2^(exps - 127) of its block of 128."""
+    2^(exps - 127) of its block of 128, and NaN where that byte is 255."""
 
     def __init__(self, codes: torch.Tensor, exps: torch.Tensor, dim: int):
         if dim < 1:

@@ -1002,3 +1002,23 @@ def test_status_of_calls_without_one(S):
     assert S.take_status() == 1
     with pytest.raises(ValueError):
         S.take_status("cpu")
+
+
+@pytest.mark.parametrize("nq", [2, 40, 200])
+def test_fp8_every_scale(S, nq):
+    """The least, the largest and the NaN exponent byte mean the same to the
+    products and to decode, block by block."""
+    torch = _torch()
+    q, v = S.Fp8Rows.empty(nq, 256, "cuda"), S.Fp8Rows.empty(300, 256, "cuda")
+    q.codes.fill_(0x38)  # 1
+    v.codes.fill_(0x38)
+    q.exps.fill_(127)
+    v.exps.fill_(127)
+    for a, b in ((254, 0), (0, 254), (254, 1), (0, 127), (127, 0), (120, 134), (255, 0), (0, 255), (127, 255)):
+        q.exps[:, 0], v.exps[:, 0] = 127, 127
+        q.exps[1, 0], v.exps[131, 0] = a, b
+        assert bool((q.decode()[1, :128] == 2.0 ** (a - 127)).all()) != (a == 255)
+        assert bool(v.decode()[131, :128].isnan().all()) == (b == 255)
+        want = q.decode().double() @ v.decode().double().T  # what is far below the largest vanishes
+        got = S.scores(q, v)
+        assert bool(((got.double() == want.float().double()) | (got.isnan() & want.isnan())).all()), (a, b)
