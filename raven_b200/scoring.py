@@ -95,9 +95,13 @@ def aligned_rows(x: torch.Tensor) -> torch.Tensor:
 class Fp8Rows:
     """Rows held as FP8: `codes` uint8 [n, roundup(dim, 16)] (e4m3) and `exps`
     uint8 [n, roundup(ceil(dim / 128), 4)]; a value is its code times
-    2^(exps - 127) of its block of 128, and NaN where that byte is 255."""
+    2^(exps - 127) of its block of 128, and NaN where that byte is 255. Their
+    contents may change, the two tensors stay: other ones make other rows."""
 
     def __init__(self, codes: torch.Tensor, exps: torch.Tensor, dim: int):
+        self._hold(codes, exps, dim)
+
+    def _hold(self, codes: torch.Tensor, exps: torch.Tensor, dim: int) -> None:
         if dim < 1:
             raise ValueError("dim must be at least 1")
         if codes.dim() != 2 or exps.dim() != 2 or codes.dtype != torch.uint8 or exps.dtype != torch.uint8 or \
@@ -115,15 +119,35 @@ class Fp8Rows:
             raise ValueError("codes and exps must have the same rows and device")
         if n == 1:  # one row may come with any pitch
             pitch, epitch = max(pitch, wide), max(epitch, ewide)
-        self.codes, self.exps, self.dim = codes, exps, dim
-        self._rows = L.Rows(codes.data_ptr(), exps.data_ptr(), n, pitch, epitch, L.RAVEN_TYPE_FP8)
+        self._codes, self._exps, self._dim = codes, exps, dim
+        self._n, self._at, self._exps_at = n, codes.data_ptr(), exps.data_ptr()
+        self._held = L.Rows(self._at, self._exps_at, n, pitch, epitch, L.RAVEN_TYPE_FP8)
+
+    @property
+    def _rows(self) -> L.Rows:
+        """The rows as the library takes them, where the tensors are now (resize_ and set_ move them)."""
+        if self._codes.data_ptr() != self._at or self._exps.data_ptr() != self._exps_at:
+            self._hold(self._codes, self._exps, self._dim)
+        return self._held
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._codes
+
+    @property
+    def exps(self) -> torch.Tensor:
+        return self._exps
+
+    @property
+    def dim(self) -> int:
+        return self._dim
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self._codes.device
 
     def __len__(self) -> int:
-        return self.codes.shape[0]
+        return self._rows.rows
 
     @staticmethod
     def empty(n: int, dim: int, device) -> "Fp8Rows":
@@ -182,8 +206,8 @@ def _operands(queries: Rows, vectors: Rows, dtype: torch.dtype, bias: Optional[t
     """(device, dim, nq, n, queries, vectors) as the library takes them, and what must stay alive until the call."""
     fp8 = isinstance(vectors, Fp8Rows)
     if fp8:
-        device, dim, v = vectors.device_index, vectors.dim, vectors._rows
-        n = v.rows
+        device, dim, v = vectors.device_index, vectors._dim, vectors._rows
+        n = vectors._n
     else:
         pitch = _matrix(vectors, "vectors")
         if vectors.dtype == torch.float32:
@@ -196,8 +220,8 @@ def _operands(queries: Rows, vectors: Rows, dtype: torch.dtype, bias: Optional[t
     if isinstance(queries, Fp8Rows):
         if not fp8:
             raise ValueError("FP8 queries need FP8 vectors")
-        qdim, q, qdevice = queries.dim, queries._rows, queries.device_index
-        nq = q.rows
+        qdim, q, qdevice = queries._dim, queries._rows, queries.device_index
+        nq = queries._n
     else:
         pitch = _matrix(queries, "queries")
         if not fp8:
@@ -246,7 +270,7 @@ def scores(queries: Rows, vectors: Rows, *, alpha: float = 1.0, bias: Optional[t
     device, dim, nq, n, q, v, keep = _operands(queries, vectors, dtype, bias)
     pitch = n
     if out is None:
-        out = torch.empty((nq, n), dtype=dtype, device=vectors.device)
+        out = (vectors._codes if isinstance(vectors, Fp8Rows) else vectors).new_empty((nq, n), dtype=dtype)
     else:
         if out.shape != (nq, n) or out.dtype != dtype or (n > 1 and out.stride(1) != 1) or (nq > 1 and out.stride(0) < n):
             raise ValueError(f"out must be a {dtype} matrix of {nq} x {n}, each row's values side by side")

@@ -1022,3 +1022,23 @@ def test_fp8_every_scale(S, nq):
         want = q.decode().double() @ v.decode().double().T  # what is far below the largest vanishes
         got = S.scores(q, v)
         assert bool(((got.double() == want.float().double()) | (got.isnan() & want.isnan())).all()), (a, b)
+
+
+def test_fp8_rows_keep_no_old_memory(S):
+    """Rows follow their tensors, which cannot be exchanged for others."""
+    torch = _torch()
+    a, b = S.Fp8Rows.encode(_gpu(_data(50, 200, 1, 1.0))), S.Fp8Rows.encode(_gpu(_data(80, 200, 2, 1.0)))
+    q = _gpu(_data(9, 200, 3, 1.0))
+    want = S.scores(q, b)
+    for name, value in (("codes", b.codes), ("exps", b.exps), ("dim", 100)):
+        with pytest.raises(AttributeError):
+            setattr(a, name, value)
+    a.codes.set_(b.codes.clone())
+    with pytest.raises(ValueError):  # 80 rows of codes, 50 of exponents
+        S.scores(q, a)
+    a.exps.set_(b.exps.clone())
+    assert len(a) == 80 and bool((S.scores(q, a) == want).all()) and bool((a.decode() == b.decode()).all())
+    assert bool((S.scores(a.rows(3, 5), a) == S.scores(b.rows(3, 5), b)).all())
+    x = _gpu(_data(80, 200, 4, 1.0))
+    S.Fp8Rows.encode(x, out=a)
+    assert bool((a.decode() == S.Fp8Rows.encode(x).decode()).all()) and bool((S.scores(q, b) == want).all())
