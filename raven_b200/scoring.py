@@ -53,7 +53,7 @@ def _matrix(x, name: str) -> int:
     # one row, or rows of one value, may come with any strides
     if (step != 1 and dim > 1) or (pitch < dim and n > 1):
         raise ValueError(f"{name} must hold each row's values side by side and its rows one after another")
-    return pitch if n > 1 else max(pitch, dim)
+    return pitch if n > 1 else _up(dim, 8)
 
 
 def _pitch(x: torch.Tensor) -> int:
@@ -118,7 +118,7 @@ class Fp8Rows:
         if en != n or exps.get_device() != self.device_index:
             raise ValueError("codes and exps must have the same rows and device")
         if n == 1:  # one row may come with any pitch
-            pitch, epitch = max(pitch, wide), max(epitch, ewide)
+            pitch, epitch = _up(dim, 16), _up(-(-dim // BLOCK), 4)
         self._codes, self._exps, self._dim = codes, exps, dim
         self._n, self._at, self._exps_at = n, codes.data_ptr(), exps.data_ptr()
         self._held = L.Rows(self._at, self._exps_at, n, pitch, epitch, L.RAVEN_TYPE_FP8)

@@ -1042,3 +1042,23 @@ def test_fp8_rows_keep_no_old_memory(S):
     x = _gpu(_data(80, 200, 4, 1.0))
     S.Fp8Rows.encode(x, out=a)
     assert bool((a.decode() == S.Fp8Rows.encode(x).decode()).all()) and bool((S.scores(q, b) == want).all())
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_one_row_has_no_pitch(S, t):
+    """A single row may come with any strides: nothing is a pitch away from it."""
+    torch = _torch()
+    x, q = _gpu(_data(3, 100, 1, 1.0), t), _gpu(_data(4, 100, 2, 1.0), t)
+    want = S.scores(q, S.aligned_rows(x))
+    for row in (x[:1], x[0].as_strided((1, 100), (1 << 45, 1)), x[0].as_strided((1, 100), (3, 1))):
+        assert bool((S.scores(q, row) == want[:, :1]).all())
+        assert bool((S.scores(row, S.aligned_rows(q))[0] == S.scores(x, S.aligned_rows(q))[0]).all())
+        assert bool((S.Fp8Rows.encode(row).decode() == S.Fp8Rows.encode(x).decode()[:1]).all())
+    rows = S.Fp8Rows.encode(x)
+    codes, exps = rows.codes[:1, :112].as_strided((1, 112), (1 << 45, 1)), rows.exps[:1].as_strided((1, 4), (5, 1))
+    one = S.Fp8Rows(codes, exps, 100)
+    assert bool((S.scores(q, one) == S.scores(q, rows)[:, :1]).all()) and bool((one.decode() == rows.decode()[:1]).all())
+    out = torch.empty(700, device="cuda").as_strided((1, 4), (1 << 45, 1))
+    assert bool((S.scores(x[:1], S.aligned_rows(q), out=out) == S.scores(x, S.aligned_rows(q))[:1]).all())
+    vals, ids, _ = S.top_k(torch.arange(9.0, device="cuda").as_strided((1, 9), (1 << 45, 1)), 2)
+    assert ids.tolist() == [[8, 7]] and vals.tolist() == [[8.0, 7.0]]
