@@ -32,6 +32,8 @@ RAVEN_TYPE_F16 = 1
 RAVEN_TYPE_BF16 = 2
 RAVEN_TYPE_FP8 = 3
 
+RAVEN_MAX_TOP_K = 256  # of raven_topk_rows_device
+
 RAVEN_S_OFFSETS = 1
 RAVEN_S_CAPACITY = 2
 RAVEN_S_WAIT = 4

@@ -39,6 +39,11 @@ def _up(x: int, m: int) -> int:
     return -(-x // m) * m
 
 
+def _u32(x: int) -> int:
+    """x as the library's 32-bit arguments take it: what they cannot hold stays out of every limit."""
+    return x if 0 <= x < 1 << 32 else (1 << 32) - 1
+
+
 def _matrix(x, name: str) -> int:
     """The row pitch of a matrix on a GPU with each row's values side by side."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
@@ -172,8 +177,8 @@ class Fp8Rows:
         if out.device_index != device:
             raise ValueError(f"out must be on cuda:{device}")
         r = out._rows
-        _call(device, L.load().raven_fp8_encode_device, x.data_ptr(), _TYPES[x.dtype], n, dim, pitch, r.data, r.ld, r.exps,
-              r.ld_exps)
+        _call(device, L.load().raven_fp8_encode_device, x.data_ptr(), _TYPES[x.dtype], n, _u32(dim), pitch, r.data, r.ld,
+              r.exps, r.ld_exps)
         return out
 
     @staticmethod
@@ -188,8 +193,8 @@ class Fp8Rows:
         """The values, float32 [n, dim] (exact)."""
         out = torch.empty(len(self), self.dim, dtype=torch.float32, device=self.device)
         r = self._rows
-        _call(self.device_index, L.load().raven_fp8_decode_device, r.data, r.ld, r.exps, r.ld_exps, len(self), self.dim,
-              out.data_ptr(), self.dim)
+        _call(self.device_index, L.load().raven_fp8_decode_device, r.data, r.ld, r.exps, r.ld_exps, len(self),
+              _u32(self.dim), out.data_ptr(), self.dim)
         return out
 
     def rows(self, first: int, count: int) -> "Fp8Rows":
@@ -276,7 +281,7 @@ def scores(queries: Rows, vectors: Rows, *, alpha: float = 1.0, bias: Optional[t
             raise ValueError(f"out must be a {dtype} matrix of {nq} x {n}, each row's values side by side")
         _on(device, out)
         pitch = _pitch(out)
-    _call(device, L.load().raven_scores_device, q, v, dim, float(alpha), _ptr(bias), out.data_ptr(), _TYPES[dtype], pitch,
+    _call(device, L.load().raven_scores_device, q, v, _u32(dim), float(alpha), _ptr(bias), out.data_ptr(), _TYPES[dtype], pitch,
           _status(status, device))
     return out
 
@@ -316,8 +321,8 @@ def group_scores(queries: Rows, query_offsets: torch.Tensor, vectors: Rows, vect
         raise ValueError(f"out must be a contiguous 1-D {dtype} tensor with room for the scores")
     else:
         _on(device, out)
-    _call(device, L.load().raven_group_scores_device, q, query_offsets.data_ptr(), v, vector_offsets.data_ptr(), groups,
-          dim, float(alpha), _ptr(bias), out.data_ptr(), _TYPES[dtype], out.numel(), _status(status, device))
+    _call(device, L.load().raven_group_scores_device, q, query_offsets.data_ptr(), v, vector_offsets.data_ptr(),
+          _u32(groups), _u32(dim), float(alpha), _ptr(bias), out.data_ptr(), _TYPES[dtype], out.numel(), _status(status, device))
     return out
 
 
@@ -335,8 +340,8 @@ def group_rows(query_offsets: torch.Tensor, vector_offsets: torch.Tensor, nq: in
     if groups == 0 or nq < 0 or n < 0:
         raise ValueError("there must be at least one group, and nq and n must not be negative")
     out = torch.empty(nq + 1, dtype=torch.int64, device=query_offsets.device)
-    _call(device, L.load().raven_group_rows_device, query_offsets.data_ptr(), vector_offsets.data_ptr(), groups, nq, n,
-          out.data_ptr(), _status(status, device))
+    _call(device, L.load().raven_group_rows_device, query_offsets.data_ptr(), vector_offsets.data_ptr(), _u32(groups), nq,
+          _u32(n), out.data_ptr(), _status(status, device))
     return out
 
 
@@ -373,9 +378,10 @@ def top_k(scores: torch.Tensor, k: int, *, largest: bool = True,
         if scores.dim() != 1 or not scores.is_contiguous():
             raise ValueError("packed scores must be a contiguous 1-D tensor")
         nq, n, ld, starts = _offsets("row_starts", row_starts, index), scores.numel(), 0, row_starts.data_ptr()
-    vals = scores.new_empty((nq, max(k, 0)))
-    ids = torch.empty((nq, max(k, 0)), dtype=torch.int32, device=device)
+    wide = k if 0 < k <= L.RAVEN_MAX_TOP_K else 0  # other k are refused before anything is written
+    vals = scores.new_empty((nq, wide))
+    ids = torch.empty((nq, wide), dtype=torch.int32, device=device)
     counts = torch.empty(nq, dtype=torch.int32, device=device)
-    _call(index, L.load().raven_topk_rows_device, scores.data_ptr(), _TYPES[scores.dtype], nq, n, ld, starts, k,
+    _call(index, L.load().raven_topk_rows_device, scores.data_ptr(), _TYPES[scores.dtype], nq, n, ld, starts, _u32(k),
           int(largest), vals.data_ptr(), ids.data_ptr(), counts.data_ptr())
     return vals, ids, counts

@@ -1062,3 +1062,30 @@ def test_one_row_has_no_pitch(S, t):
     assert bool((S.scores(x[:1], S.aligned_rows(q), out=out) == S.scores(x, S.aligned_rows(q))[:1]).all())
     vals, ids, _ = S.top_k(torch.arange(9.0, device="cuda").as_strided((1, 9), (1 << 45, 1)), 2)
     assert ids.tolist() == [[8, 7]] and vals.tolist() == [[8.0, 7.0]]
+
+
+def test_sizes_past_32_bits_are_refused(S):
+    """Sizes that the library takes as 32 bits are not cut to their low ones."""
+    torch = _torch()
+    from raven_b200 import RavenError
+
+    x = torch.randn(2, 9, device="cuda")
+    off = torch.tensor([0, 2], device="cuda")
+    for k in ((1 << 32) + 3, (1 << 64) + 3, 3 - (1 << 32), -1, 257, 1 << 31):
+        with pytest.raises(RavenError):
+            S.top_k(x, k)
+        with pytest.raises(RavenError):
+            S.top_k(x[:0], k)
+    for n in ((1 << 32) + 2, (1 << 64) + 2):
+        with pytest.raises(RavenError):
+            S.group_rows(off, off, 2, n)
+    # a row of 2^32 + 16 codes, which are never read
+    codes = torch.empty((1, (1 << 32) + 16), dtype=torch.uint8, device="cuda")
+    rows = S.Fp8Rows(codes, torch.empty((1, (1 << 25) + 4), dtype=torch.uint8, device="cuda"), (1 << 32) + 16)
+    with pytest.raises(RavenError):
+        S.scores(rows, rows)
+    with pytest.raises(RavenError):
+        S.group_scores(rows, off, rows, off, total=4)
+    wide = codes[:, : (1 << 32) + 16].view(torch.float16)  # 2^31 + 8 values
+    with pytest.raises(RavenError):
+        S.Fp8Rows.encode(wide)
