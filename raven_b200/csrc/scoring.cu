@@ -401,6 +401,8 @@ cudaError_t launch_chunks(const int64_t* qo, const int64_t* vo, uint32_t groups,
   return e != cudaSuccess ? e : launch(group_scan_kernel, 1, 1024, 0, none_scan, st, chunks, chunks_of(groups));
 }
 
+constexpr uint32_t kHalo = 16;  // scores that a tile by pairs computes past its own: a sector of 16-bit ones
+
 struct Operands {
   const raven_rows* q;
   const raven_rows* v;
@@ -421,13 +423,14 @@ cudaError_t launch_score(const Operands& o, raven_score::Params p, bool whole, i
   // SM keeps a few tiles (grouped: and a tile does not outgrow a mean group).
   const uint64_t per = p.qo ? std::max<uint64_t>(p.n / p.groups, 1) : p.n;
   uint64_t subs = p.nkb <= 4 ? L::kSubs : 1;
+  p.halo = ROWS || whole ? 0 : kHalo;
   auto tiles = [&](uint64_t s) {
-    return (p.qo ? p.groups : 1) * ((per + s * L::kTileV - 1) / (s * L::kTileV)) *
+    const uint64_t rows = s * L::kTileV - p.halo;
+    return (p.qo ? p.groups : 1) * ((per + rows - 1) / rows) *
            (p.qo ? 1 : (p.nq + L::kTileQ - 1) / L::kTileQ);
   };
   while (subs > 1 && (tiles(subs) < 4ull * sms || (p.qo && subs * L::kTileV > 2 * per))) subs /= 2;
   p.subs = (uint32_t)subs;
-  p.halo = ROWS || whole ? 0 : 16;
   const uint64_t grid = p.qo ? (uint64_t)sms : std::min<uint64_t>(tiles(subs), (uint64_t)sms);
   Chunk* chunks = nullptr;
   cudaError_t e = cudaSuccess;
@@ -462,7 +465,8 @@ cudaError_t dispatch_score(const Operands& o, const raven_score::Params& p, int 
   const bool whole = !p.qo && (uintptr_t)p.out % 32 == 0 && p.ld * size % 32 == 0;  // every query starts on a sector
   const bool far = !p.qo && p.ld * size >= kFar;
   if (want > 64 && !(whole && size == 4) && !far) {
-    if (!p.qo && (p.nq + 127) / 128 * ((p.n + 223) / 224) < (uint64_t)sms)
+    const uint64_t rows = 224 - (whole ? 0 : kHalo);
+    if (!p.qo && (p.nq + 127) / 128 * ((p.n + rows - 1) / rows) < (uint64_t)sms)
       return launch_score<FP8, 96, false>(o, p, whole, sms, st);
     return launch_score<FP8, 224, false>(o, p, whole, sms, st);
   }

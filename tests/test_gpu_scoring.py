@@ -1089,3 +1089,24 @@ def test_sizes_past_32_bits_are_refused(S):
     wide = codes[:, : (1 << 32) + 16].view(torch.float16)  # 2^31 + 8 values
     with pytest.raises(RavenError):
         S.Fp8Rows.encode(wide)
+
+
+@pytest.mark.parametrize("nq,n,rows", [(100, 10_001, 80), (100, 10_000, 80), (128, 7_008, 96), (70, 32_001, 208), (300, 3_001, 80)])
+def test_scores_take_a_cta_per_tile(S, nq, n, rows):
+    """Up to the number of SMs there are as many CTAs as tiles of 128 queries and
+    `rows` rows; where scores start between sectors a tile keeps 16 rows less."""
+    torch = _torch()
+    driver = pytest.importorskip("cuda.bindings.driver")
+    q, v = _gpu(_data(nq, 64, 1, 1.0), "f16"), _gpu(_data(n, 64, 2, 1.0), "f16")
+    t = torch.float32 if rows in (80, 208) else torch.bfloat16  # 16-bit scores that start on sectors: whole tiles
+    room = torch.empty(nq, -(-n // 16) * 16 + (1 if rows in (80, 208) else 0), dtype=t, device="cuda")
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        S.scores(q, v, dtype=t, out=room[:, :n])
+    _, _, count = driver.cuGraphGetNodes(driver.CUgraph(graph.raw_cuda_graph()), 0)
+    _, nodes, _ = driver.cuGraphGetNodes(driver.CUgraph(graph.raw_cuda_graph()), count)
+    grids = [driver.cuGraphKernelNodeGetParams(x)[1].gridDimX for x in nodes[:count]]
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert grids == [min(sms, -(-n // rows) * -(-nq // 128))]
+    graph.replay()
+    _check(room[:, :n], _np(q), _np(v), "f32" if t == torch.float32 else "bf16")
