@@ -1110,3 +1110,42 @@ def test_scores_take_a_cta_per_tile(S, nq, n, rows):
     assert grids == [min(sms, -(-n // rows) * -(-nq // 128))]
     graph.replay()
     _check(room[:, :n], _np(q), _np(v), "f32" if t == torch.float32 else "bf16")
+
+
+# ---- long rows, exactly ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dim", [1000, 4095, 8192, 8200, 65_535, 65_536])
+@pytest.mark.parametrize("nq,n", [(1, 300), (2, 500), (40, 300), (70, 300), (130, 1000)])
+@pytest.mark.parametrize("t", ["f16", "bf16", "fp8", "fp8 from f32"])
+def test_scores_of_long_rows_exactly(S, nq, n, dim, t):
+    """Whole numbers of at most 3 in magnitude, with a scale of its own for each
+    block: products and sums (of at most 9 * 65536 * 4 < 2^24 in units of the
+    least product) are exact in f32 and the codes are exact, so a value that is
+    dropped, doubled or given another block's scale shows in every score."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(dim + nq)
+    blocks = -(-dim // 128)
+
+    def make(rows):
+        x = torch.randint(1, 4, (rows, dim), device="cuda", generator=g).float()
+        x *= torch.randint(0, 2, (rows, dim), device="cuda", generator=g) * 2 - 1
+        scale = torch.randint(0, 2, (rows, blocks), device="cuda", generator=g).float().exp2()
+        return x * scale.repeat_interleave(128, 1)[:, :dim]
+
+    q, v = make(nq), make(n)
+    if t.startswith("fp8"):
+        rows, ops = S.Fp8Rows.encode(v), (q if t != "fp8" else S.Fp8Rows.encode(q))
+        assert bool((rows.decode() == v).all())
+    else:
+        rows, ops = S.aligned_rows(v.to(_dt(t))), S.aligned_rows(q.to(_dt(t)))
+    want = q.double() @ v.double().T
+    assert bool((S.scores(ops, rows).double() == want).all())
+    room = torch.empty(nq, n + 3, device="cuda")  # scores between sectors
+    assert bool((S.scores(ops, rows, out=room[:, 1:n + 1]).double() == want).all())
+    # the same in two groups
+    a, b = nq // 2, n // 3
+    qo, vo = torch.tensor([0, a, nq], device="cuda"), torch.tensor([0, b, n], device="cuda")
+    got = S.group_scores(ops, qo, rows, vo, total=a * b + (nq - a) * (n - b))
+    assert bool((got[:a * b].view(a, b).double() == want[:a, :b]).all())
+    assert bool((got[a * b:].view(nq - a, n - b).double() == want[a:, b:]).all())
