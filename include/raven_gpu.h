@@ -334,7 +334,7 @@ RAVEN_API int raven_scoring_status_device(int32_t* d_status, void* stream);
  * smallest with largest = 0), equal scores by the lower index, NaN after every
  * number, -0 equal to 0. Rows are n scores at pitch ld, or with d_row_starts
  * (nq + 1 values on the device) the scores [d_row_starts[i], d_row_starts[i + 1])
- * of n in all (fewer than 2^32 in a row). d_ids: indexes within the row; d_counts (may be NULL): min(k, row
+ * of n in all (of a row, the first 2^32 - 1). d_ids: indexes within the row; d_counts (may be NULL): min(k, row
  * length); slots past the count are 0. Values have the scores' type. */
 RAVEN_API int raven_topk_rows_device(const void* d_scores, int32_t type, uint64_t nq, uint64_t n, uint64_t ld,
                                      const int64_t* d_row_starts, uint32_t k, int32_t largest, void* d_vals,

@@ -362,8 +362,10 @@ def top_k(scores: torch.Tensor, k: int, *, largest: bool = True,
     """(values [nq, k], ids [nq, k] int32, counts [nq] int32) of the best k
     (1..256) of each row, best first, equal scores by the lower index, NaN after
     every number. Rows are those of a matrix, or with `row_starts` (int64, nq + 1
-    values) pieces of a packed 1-D tensor; ids count within the row. Slots past a
-    row's count (rows of fewer than k) are 0."""
+    values) pieces of a packed 1-D tensor; ids count within the row (in rows of
+    2^31 scores and more, which only packed ones can be, their bits are unsigned;
+    scores from 2^32 - 1 on are not looked at). Slots past a row's count (rows of
+    fewer than k) are 0."""
     if not isinstance(scores, torch.Tensor) or not scores.is_cuda or scores.dtype not in _TYPES:
         raise ValueError("scores must be a float32, float16 or bfloat16 tensor on a GPU")
     index, device, k = scores.get_device(), scores.device, operator.index(k)

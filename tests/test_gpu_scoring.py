@@ -1149,3 +1149,16 @@ def test_scores_of_long_rows_exactly(S, nq, n, dim, t):
     got = S.group_scores(ops, qo, rows, vo, total=a * b + (nq - a) * (n - b))
     assert bool((got[:a * b].view(a, b).double() == want[:a, :b]).all())
     assert bool((got[a * b:].view(nq - a, n - b).double() == want[a:, b:]).all())
+
+
+@pytest.mark.parametrize("dim", [7, 16, 100, 130, 256])
+def test_fp8_of_index_of_any_dimension(S, raven_lib, dim):
+    """The index holds its vectors in an order of its own; their FP8 rows are in the caller's."""
+    from raven_b200.index import DeviceIndex, Graph
+
+    base = _data(300, dim, dim, 2.0).astype(np.float32)
+    g = Graph.build(base, r=16, l=32, alpha=1.2, seed=1)
+    rows = S.Fp8Rows.of_index(DeviceIndex(g, base))
+    want = S.Fp8Rows.encode(_gpu(base))
+    assert len(rows) == 300 and rows.dim == dim
+    assert bool((rows.codes == want.codes).all()) and bool((rows.exps == want.exps).all())
