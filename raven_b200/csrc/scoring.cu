@@ -314,9 +314,9 @@ using raven_score::kChunk;
 // From how many groups on: the sums' two launches take 4 us and more, and a walk
 // is partly hidden by the tiles (1000 groups of 1 x 8 scores 22 us walked, 18 with
 // sums, but 1000 of 10 x 1000 44 and 49; 2000 of 20 x 300 59 and 45). The blocks of
-// group_rows, which sum what is before them by themselves, reach that later (4096
-// groups 11.5 us, 13.0 with sums; 65536: 50, 19).
-constexpr uint32_t kManyGroups = 1536, kManyGroupRows = 8192;
+// group_rows, which sum what is before them by themselves, reach that later (16384
+// groups 12.0 us a call, 14.6 with sums; 32768: 21.3, 14.4; 65536: 39.9, 14.4).
+constexpr uint32_t kManyGroups = 1536, kManyGroupRows = 16384;
 
 // Per chunk, the tiles (of tq queries and `rows` rows of v) and scores of its groups.
 __global__ void __launch_bounds__(256) group_chunks_kernel(const int64_t* qo, const int64_t* vo, uint32_t groups,

@@ -872,7 +872,7 @@ def test_group_rows_beside_malformed_groups(S, qo, vo):
             np.testing.assert_array_equal(_np(vals[i]), wv[0])
 
 
-@pytest.mark.parametrize("groups", [700, 8192, 9000])
+@pytest.mark.parametrize("groups", [700, 8192, 9000, 20_000])
 def test_group_rows_beside_malformed_groups_among_many(S, groups):
     r = np.random.default_rng(groups)
     for _ in range(3):
@@ -885,7 +885,7 @@ def test_group_rows_beside_malformed_groups_among_many(S, groups):
         np.testing.assert_array_equal(starts.cpu().numpy(), U.group_starts(qo, vo, nq, n))
 
 
-@pytest.mark.parametrize("groups", [3, 40, 900, 9000])
+@pytest.mark.parametrize("groups", [3, 40, 900, 9000, 20_000])
 def test_group_rows_where_query_offsets_fall(S, groups):
     """Several groups cover a query: its place is in one of them, the same every
     time, starts rise, and none is left as it was."""
