@@ -234,9 +234,12 @@ __global__ void __launch_bounds__(256) fp8_decode_kernel(const uint8_t* codes, u
     const uint64_t row = t / dim;
     const uint32_t d = (uint32_t)(t - row * dim);
     const __half_raw h = __nv_cvt_fp8_to_halfraw(codes[row * ld_codes + d], __NV_E4M3);
-    const int e = exps[row * ld_exps + d / kBlock];
-    // 255 is the scales' NaN, as the tensor cores take it
-    out[row * ld + d] = e == 255 ? __int_as_float(0x7fc00000) : ldexpf(__half2float(*(const __half*)&h), e - 127);
+    // the scale as f32 bits: 0 is 2^-127, below the normal range, and 255 the scales'
+    // NaN, as the tensor cores take it; the product with a power of two is rounded as
+    // ldexpf would (infinite from 2^128)
+    const uint32_t e = exps[row * ld_exps + d / kBlock];
+    const float scale = __uint_as_float(e == 0 ? 0x400000u : e == 255 ? 0x7fc00000u : e << 23);
+    out[row * ld + d] = __half2float(*(const __half*)&h) * scale;
   }
 }
 

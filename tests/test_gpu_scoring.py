@@ -1162,3 +1162,21 @@ def test_fp8_of_index_of_any_dimension(S, raven_lib, dim):
     want = S.Fp8Rows.encode(_gpu(base))
     assert len(rows) == 300 and rows.dim == dim
     assert bool((rows.codes == want.codes).all()) and bool((rows.exps == want.exps).all())
+
+
+def test_fp8_decode_every_code_and_scale(S):
+    """All 256 codes under all 256 exponent bytes, rounded to f32 where a value is
+    below its normal range."""
+    torch = _torch()
+    rows = S.Fp8Rows.empty(256, 256, "cuda")
+    rows.codes.copy_(torch.arange(256, device="cuda").to(torch.uint8).expand(256, 256))
+    rows.exps.copy_(torch.arange(256, device="cuda").to(torch.uint8)[:, None].expand(256, 4))
+    c = np.arange(256)
+    mag = np.where((c & 127) >> 3 == 0, (c & 7) * 2.0 ** -9, (8 + (c & 7)) * 2.0 ** (((c & 127) >> 3) - 10.0))
+    value = np.where((c & 127) == 127, np.nan, np.where(c > 127, -mag, mag))
+    scale = np.where(c == 255, np.nan, 2.0 ** (c - 127.0))
+    with np.errstate(over="ignore"):
+        want = (scale[:, None] * value[None, :]).astype(np.float32)
+    got = rows.decode().cpu().numpy()
+    np.testing.assert_array_equal(got, want)
+    assert np.array_equal(np.signbit(got[:255, :127]), np.signbit(want[:255, :127]))
