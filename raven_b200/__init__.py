@@ -3,6 +3,7 @@
 The engine itself is libraven_gpu.so (hand-written CUDA for sm_100a behind the
 C ABI in include/raven_gpu.h). This package is its host side: a ctypes binding
 and the `Index` / `Searcher` / `GraphSearcher` surface of the reference.
+`raven_b200.scoring` (which needs torch) has exhaustive scores on torch tensors.
 """
 from .index import AdaptiveEfConfig, DeviceIndex, Graph, GraphSearcher, Index, Searcher  # noqa: F401
 from ._lib import RavenError, SearchParams  # noqa: F401

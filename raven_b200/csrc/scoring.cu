@@ -318,7 +318,7 @@ using raven_score::kChunk;
 // is partly hidden by the tiles (1000 groups of 1 x 8 scores 22 us walked, 18 with
 // sums, but 1000 of 10 x 1000 44 and 49; 2000 of 20 x 300 59 and 45). The blocks of
 // group_rows, which sum what is before them by themselves, reach that later (16384
-// groups 12.0 us a call, 14.6 with sums; 32768: 21.3, 14.4; 65536: 39.9, 14.4).
+// groups 10.8 us a call, 14.6 with sums; 32768: 21.3, 14; 65536: 39.9, 14).
 constexpr uint32_t kManyGroups = 1536, kManyGroupRows = 16384;
 
 // Per chunk, the tiles (of tq queries and `rows` rows of v) and scores of its groups.
@@ -603,6 +603,8 @@ __device__ inline void queries_of(const int64_t* qo, uint32_t groups, int64_t nq
     lo = max(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     hi = min(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
+  lo = min(lo, nq);
+  hi = max(hi, lo);
 }
 
 // Where each query's scores start in grouped scores: starts[i] for query i of
@@ -615,6 +617,8 @@ __global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* qo, cons
                                                          int* status) {
   after_previous();
   __shared__ int64_t part[256];
+  __shared__ int64_t from[256], size[256], start[256], per[256];  // groups of many queries
+  __shared__ uint32_t large, huge;
   __shared__ int64_t edge[256], ends[2][2];  // the run's offsets; its queries by the bits above it, those behind the last group
   const uint32_t g0 = blockIdx.x * 256u, tid = threadIdx.x;
   bool bad = false;
@@ -631,6 +635,7 @@ __global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* qo, cons
       ends[tid >> 5][1] = hi;
     }
   }
+  if (tid == 0) large = huge = 0;
   edge[tid] = g0 + tid <= groups ? qo[g0 + tid] : INT64_MAX;
   int64_t sum = 0, a, m, c;
   for (uint32_t g = tid; g < g0 && !chunks; g += 256) {
@@ -659,6 +664,8 @@ __global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* qo, cons
       else
         hi = min(hi, x);
     }
+    lo = min(lo, (int64_t)nq);
+    hi = max(hi, lo);  // [lo, hi) within the queries whatever the offsets are: sums with them do not wrap
   }
   part[tid] = m * c;
   __syncthreads();
@@ -668,15 +675,32 @@ __global__ void __launch_bounds__(256) group_rows_kernel(const int64_t* qo, cons
     part[tid] += x;
     __syncthreads();
   }
-  const int64_t base = before + part[tid] - m * c - a * c;  // less what i * c below has too much
-  const bool few = hi - lo <= 8;  // queries of a group, written by its thread; more by its warp
-  for (int64_t i = lo; few && i < hi; ++i) starts[i] = base + i * c;
-  for (uint32_t left = __ballot_sync(0xffffffffu, !few); left; left &= left - 1) {
-    const int j = __ffs(left) - 1;
-    const int64_t end = __shfl_sync(0xffffffffu, hi, j), at = __shfl_sync(0xffffffffu, base, j);
-    const int64_t width = __shfl_sync(0xffffffffu, c, j);
-    for (int64_t i = __shfl_sync(0xffffffffu, lo, j) + (tid & 31); i < end; i += 32) starts[i] = at + i * width;
+  // a group of up to 64 queries is written by 8 lanes, of up to 4096 by a warp, a larger one by all
+  const uint32_t lane = tid & 31;
+  const int64_t count = hi - lo, base = before + part[tid] - m * c + (lo - a) * c;  // of the first query that is its own
+  auto write = [&](int64_t first, int64_t n, int64_t at, int64_t width, uint32_t i, uint32_t step) {
+    int64_t* to = starts + first;
+    at += i * width;
+    width *= step;
+#pragma unroll 4
+    for (; i < n; i += step, at += width) to[i] = at;
+  };
+#pragma unroll 2
+  for (int r = 0; r < 8; ++r) {
+    const int64_t first = __shfl_sync(0xffffffffu, lo, r, 8), at = __shfl_sync(0xffffffffu, base, r, 8);
+    const int64_t width = __shfl_sync(0xffffffffu, c, r, 8);
+    write(first, __shfl_sync(0xffffffffu, count <= 64 ? (int)count : 0, r, 8), at, width, lane & 7, 8);
   }
+  if (count > 64) {  // in any order: each is written by itself
+    const uint32_t k = count <= 4096 ? atomicAdd(&large, 1u) : 255u - atomicAdd(&huge, 1u);
+    from[k] = lo;
+    size[k] = count;
+    start[k] = base;
+    per[k] = c;
+  }
+  __syncthreads();
+  for (uint32_t k = tid / 32; k < large; k += 8) write(from[k], size[k], start[k], per[k], lane, 32);
+  for (uint32_t k = 256 - huge; k < 256; ++k) write(from[k], size[k], start[k], per[k], tid, 256);
   // queries before the first group start at 0, those behind the last one at the end
   if (last) {
     const int64_t total = before + part[255];

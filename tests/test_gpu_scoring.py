@@ -850,7 +850,9 @@ def _poisoned_starts(S, qo, vo, nq, n):
 @pytest.mark.parametrize("qo,vo", [([0, 10, 20], [0, 30, 20]), ([0, 10, 25], [0, 10, 20]), ([-5, 4, 20], [0, 10, 20]),
                                    ([0, 5, 5, 12, 20], [0, 31, 8, 8, 30]), ([0, 7, 20], [-1, 4, 1 << 62]),
                                    ([21, 30, 40], [0, 4, 5]), ([-9, -3, -1], [0, 4, 5]),
-                                   ([3, 9, 14], [4, 2, 9]), ([-(1 << 60), 20, 1 << 62], [0, 30, 30])])
+                                   ([3, 9, 14], [4, 2, 9]), ([-(1 << 60), 20, 1 << 62], [0, 30, 30]),
+                                   ([0, 1 << 62, (1 << 62) + 20], [0, 10, 30]),
+                                   ([-(1 << 63), -(1 << 63) + 20, (1 << 63) - 1], [0, 10, 30])])
 def test_group_rows_beside_malformed_groups(S, qo, vo):
     """Every start is written, and the queries of sound groups have the rows of theirs."""
     torch = _torch()
@@ -1180,3 +1182,57 @@ def test_fp8_decode_every_code_and_scale(S):
     got = rows.decode().cpu().numpy()
     np.testing.assert_array_equal(got, want)
     assert np.array_equal(np.signbit(got[:255, :127]), np.signbit(want[:255, :127]))
+
+
+@pytest.mark.parametrize("groups", [2, 60, 9000, 20_000])
+def test_group_rows_of_wild_offsets(S, groups):
+    """Offsets near the ends of 64 bits, in any order: every start is written, none beside them."""
+    r = np.random.default_rng(groups)
+    nq, n = 300, 50
+    ends = np.array([-(1 << 63), -(1 << 63) + 1, -(1 << 62), -1, 0, 7, 299, 300, 301, (1 << 31) + 5, (1 << 32) + 9, 1 << 62,
+                     (1 << 63) - 2, (1 << 63) - 1], np.int64)
+    for turn in range(8):
+        qo, vo = r.choice(ends, groups + 1), r.choice(ends, groups + 1)
+        if turn % 2:
+            qo.sort()
+        if turn < 4:
+            vo = np.sort(r.integers(0, n + 1, groups + 1))
+        starts, _ = _poisoned_starts(S, qo, vo, nq, n)
+        got = starts.cpu().numpy()
+        assert got[0] >= 0 and np.all(np.diff(got) >= 0)
+        if turn % 2:
+            np.testing.assert_array_equal(got, U.group_starts(qo, vo, nq, n))
+
+
+@pytest.mark.parametrize("groups", [2, 60, 1536, 9000])
+def test_group_scores_of_wild_offsets(S, groups):
+    """Sound groups among offsets near the ends of 64 bits have their scores, and
+    nothing is written past the output."""
+    torch = _torch()
+    r = np.random.default_rng(groups)
+    g = torch.Generator(device="cuda").manual_seed(groups)
+    q = torch.randint(-3, 4, (300, 64), device="cuda", generator=g).half()
+    v = torch.randint(-3, 4, (50, 64), device="cuda", generator=g).half()
+    full = (q.float() @ v.float().T).cpu().numpy()
+    ends = np.array([-(1 << 63), -1, 0, 7, 9, 20, 50, 299, 300, 301, (1 << 31) + 5, 1 << 62, (1 << 63) - 1], np.int64)
+    cap = 40_000
+    for turn in range(4):
+        qo, vo = r.choice(ends, groups + 1), r.choice(ends, groups + 1)
+        want = []
+        for i in range(groups):
+            a, b, c, d = (int(x) for x in (qo[i], qo[i + 1], vo[i], vo[i + 1]))
+            if 0 <= a <= b <= 300 and 0 <= c <= d <= 50:
+                want.append(full[a:b, c:d].ravel())
+        want = np.concatenate(want) if want else np.zeros(0, np.float32)
+        room = torch.full((cap + 100,), 5.0, device="cuda")
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        S.group_scores(q, torch.from_numpy(qo).cuda(), v, torch.from_numpy(vo).cuda(), out=room[:cap], status=status)
+        got = room.cpu().numpy()
+        assert np.all(got[cap:] == 5.0)
+        assert int(status) == (1 if groups > 2 or np.any(qo[1:] < qo[:-1]) or np.any(vo[1:] < vo[:-1]) or
+                               qo.min() < 0 or qo.max() > 300 or vo.min() < 0 or vo.max() > 50 else 0) + 2 * (len(want) > cap)
+        if len(want) <= cap:
+            np.testing.assert_array_equal(got[:len(want)], want)
+            assert np.all(got[len(want):] == 5.0)
+        else:
+            np.testing.assert_array_equal(got[:cap - 50], want[:cap - 50])  # all but a query that does not fit
