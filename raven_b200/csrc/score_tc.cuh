@@ -474,7 +474,7 @@ __device__ inline uint32_t word_of(const uint32_t (&v)[16], int i, const __nv_bf
 // one needs from the columns after them (a tile computes that much of the next
 // one), so that only a query's first and last sectors are written in part:
 // 999 x 250007 bf16 scores took 460 us when every warp wrote its ends in part, and
-// 999 x 250000, where every sector is whole, 103. Halves of sectors are as bad
+// 999 x 250000, where every sector is whole, 124. Halves of sectors are as bad
 // (2.1 TB/s for 16-byte stores alone, 4.9 for 32-byte ones).
 template <int BN, typename T>
 __device__ inline void store_pairs(T* out, const Tile& t, uint32_t qcnt, uint32_t acc, uint32_t warp, uint32_t lane,
