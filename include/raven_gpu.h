@@ -251,6 +251,9 @@ RAVEN_API int raven_merge_topk_gathered_device(const void* d_gathered, uint32_t 
 #define RAVEN_TYPE_F16 1
 #define RAVEN_TYPE_BF16 2
 #define RAVEN_TYPE_FP8 3 /* e4m3 codes, one power-of-two scale per 128 values */
+#define RAVEN_TYPE_INT4_32 4  /* 4-bit codes, one scale word per 32 values */
+#define RAVEN_TYPE_INT4_64 5  /* the same per 64 */
+#define RAVEN_TYPE_INT4_128 6 /* the same per 128 */
 
 /* bits of *d_status, which calls only ever set (the caller clears it). Calls with
  * a NULL d_status set them in a word of the device that raven_scoring_status_device
@@ -258,6 +261,7 @@ RAVEN_API int raven_merge_topk_gathered_device(const void* d_gathered, uint32_t 
 #define RAVEN_S_OFFSETS 1  /* a group's offsets fall or leave the rows: it counted as empty */
 #define RAVEN_S_CAPACITY 2 /* scores past the output's capacity were not written */
 #define RAVEN_S_WAIT 4     /* a wait inside the kernel (each is bounded) ran out: the scores are not valid */
+#define RAVEN_S_IDS 8      /* a slot, an id or a filter's number was not below what there is */
 
 /* Rows of `dim` values, row i at data + i * ld values (codes). FP8 rows also
  * have exponent bytes, row i at exps + i * ld_exps, one per 128 values: a value
@@ -268,10 +272,10 @@ RAVEN_API int raven_merge_topk_gathered_device(const void* d_gathered, uint32_t 
  * a multiple of 8; queries that a call encodes may have any ld >= dim. */
 typedef struct {
   const void* data;
-  const uint8_t* exps; /* FP8 only */
+  const uint8_t* exps; /* FP8: exponent bytes; 4 bits: scale words */
   uint64_t rows;       /* < 2^31 */
   uint64_t ld;
-  uint64_t ld_exps; /* FP8 only */
+  uint64_t ld_exps; /* FP8: bytes; 4 bits: words */
   int32_t type;     /* RAVEN_TYPE_* */
 } raven_rows;
 
@@ -293,11 +297,49 @@ RAVEN_API int raven_fp8_decode_device(const uint8_t* d_codes, uint64_t ld_codes,
 RAVEN_API int raven_index_fp8_device(raven_index* ix, uint8_t* d_codes, uint64_t ld_codes, uint8_t* d_exps,
                                      uint64_t ld_exps, void* stream);
 
+/* 4-bit rows (RAVEN_TYPE_INT4_*): row i's codes at data + i * ld bytes, its scale
+ * words at (const uint32_t*)exps + i * ld_exps, one per group of 32, 64 or 128
+ * values. With the low 8 bits of a word as a signed number z, and the f32 that the
+ * word is without them as the step, a value is (code + z) * step: NaN for a whole
+ * group whose word is one. Codes start on 16 bytes, ld is a multiple of 16 of at
+ * least 16 * ceil(dim / 32). Words are held by whole blocks of 128 values (W = 4,
+ * 2 or 1 of them): they start on 4 * W bytes, ld_exps is a multiple of W of at
+ * least W * ceil(dim / 128), those past the last group are not looked at.
+ * Layout of codes: the eight values from 8i on are one 32-bit word, the first in
+ * its lowest 4 bits. 16 words are a block (128 values, four units of 32); the last
+ * block has u <= 4 units. Word 4 * unit + quarter of a block (in the order of
+ * values) is its word u * quarter + unit.
+ *
+ * Writes m rows of f32, f16 or bf16 values (any ld >= dim, dim in 1..65536) into
+ * `out`: row i as row d_slots[i], or as row i with NULL d_slots. Rows with a slot
+ * below 0 are left out, as are those with one of out->rows and more
+ * (RAVEN_S_IDS); of rows with the same slot the last is held. For a group of
+ * values from lo to hi, the step is max((hi - lo) / 15, max|x| / 127), rounded up
+ * to 16 significant bits, z = lo / step and code = x / step - z, both quotients
+ * rounded to nearest even, the code at most 15. A group with an infinity or a NaN
+ * is NaN as a whole. Codes past dim, up to a multiple of 32 values, and words past
+ * the last group, up to a multiple of W, are 0; what is behind them is left. */
+RAVEN_API int raven_int4_write_device(const void* d_rows, int32_t type, uint64_t m, uint32_t dim, uint64_t ld,
+                                      const int32_t* d_slots, const raven_rows* out, int32_t* d_status, void* stream);
+/* The values that m of the rows stand for, rounded once to out_type (f32, in
+ * which they are exact unless they overflow, f16, bf16): those of d_ids, or the
+ * first m with NULL d_ids. Rows of an id that is not one of the rows' are 0 (one
+ * that is not below them, but not one below 0, sets RAVEN_S_IDS). */
+RAVEN_API int raven_int4_read_device(const raven_rows* rows, uint32_t dim, const int32_t* d_ids, uint64_t m, void* d_out,
+                                     int32_t out_type, uint64_t ld, int32_t* d_status, void* stream);
+/* 4-bit rows of an index's uploaded vectors (n x dim, in the caller's order of
+ * values), on the index's device. */
+RAVEN_API int raven_index_int4_device(raven_index* ix, const raven_rows* out, void* stream);
+
 /* out[i * ld_out + j] = alpha * <q_i, v_j> + (d_bias ? d_bias[j] : 0), summed
  * in f32 on the tensor cores and rounded once to out_type (f32, f16, bf16).
  * alpha = -2 with d_bias[j] = |v_j|^2 gives squared distances less |q_i|^2.
  * Vectors are FP8, f16 or bf16; queries have the same type, or, with FP8
- * vectors, any type (they are encoded first). */
+ * vectors, any type (they are encoded first).
+ * With 4-bit vectors they are f32, f16 or bf16 rows at any ld >= dim; nothing is
+ * rounded before the sums but f32 queries, to 22 bits of each value, and what is
+ * below 2^-34 of a query's largest; a query with an infinity or a NaN has
+ * scores of NaN. */
 RAVEN_API int raven_scores_device(const raven_rows* q, const raven_rows* v, uint32_t dim, float alpha,
                                   const float* d_bias, void* d_out, int32_t out_type, uint64_t ld_out,
                                   int32_t* d_status, void* stream);
@@ -339,6 +381,39 @@ RAVEN_API int raven_scoring_status_device(int32_t* d_status, void* stream);
 RAVEN_API int raven_topk_rows_device(const void* d_scores, int32_t type, uint64_t nq, uint64_t n, uint64_t ld,
                                      const int64_t* d_row_starts, uint32_t k, int32_t largest, void* d_vals,
                                      uint32_t* d_ids, uint32_t* d_counts, void* stream);
+
+/* What scores are adjusted by: arrays on the device, NULL for what does not apply. */
+typedef struct {
+  const float* bias;          /* n values, of query i at bias + i * ld_bias (0: the same for all) */
+  uint64_t ld_bias;
+  const uint32_t* allow;      /* filters: vector j's bit is bit j % 32 of word j / 32, filter f at allow + f * ld_allow */
+  uint64_t allow_count;
+  uint64_t ld_allow;          /* at least ceil(n / 32) */
+  const int32_t* allow_rows;  /* the filter of each query, below 0: none; NULL: the one filter, or its own of nq */
+  const int32_t* seen;        /* vectors that query i has seen: [seen_starts[i], seen_starts[i + 1]) of these ids, */
+  uint64_t seen_total;        /* each as often as it is there */
+  const int64_t* seen_starts; /* nq + 1 */
+  const float* repetition;    /* of each query (nq values); NULL: the one below */
+  const float* presence;
+  const float* frequency;
+  float repetition_all, presence_all, frequency_all;
+} raven_adjustments;
+
+/* Scores (nq x n at pitch ld, f32, f16 or bf16) put right before the best are
+ * taken, into d_out (the same type, nq x n at ld_out; it may be d_scores at ld,
+ * and must not overlap it otherwise). In f32, each operation rounded:
+ *   s of a vector that the query has seen c > 0 times:
+ *     largest: s = (s > 0 ? s / repetition : s * repetition) - (presence + frequency * c)
+ *     else:    s = (s > 0 ? s * repetition : s / repetition) + (presence + frequency * c)
+ *   s = s + bias
+ *   s = -infinity (largest; else infinity) where the query's filter has no bit
+ * rounded once to the type. Ids below 0 count for nothing, nor do those of n and
+ * more (RAVEN_S_IDS); a history whose starts fall or leave `seen` counts as empty
+ * (RAVEN_S_OFFSETS); a query with a filter of allow_count and more may see nothing
+ * (RAVEN_S_IDS). */
+RAVEN_API int raven_adjust_scores_device(const void* d_scores, int32_t type, uint64_t nq, uint64_t n, uint64_t ld,
+                                         const raven_adjustments* by, int32_t largest, void* d_out, uint64_t ld_out,
+                                         int32_t* d_status, void* stream);
 
 typedef struct {
   uint32_t max_ef;      /* largest pool capacity (fixed ef or adaptive max) */

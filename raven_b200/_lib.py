@@ -31,12 +31,16 @@ RAVEN_TYPE_F32 = 0
 RAVEN_TYPE_F16 = 1
 RAVEN_TYPE_BF16 = 2
 RAVEN_TYPE_FP8 = 3
+RAVEN_TYPE_INT4_32 = 4
+RAVEN_TYPE_INT4_64 = 5
+RAVEN_TYPE_INT4_128 = 6
 
 RAVEN_MAX_TOP_K = 256  # of raven_topk_rows_device
 
 RAVEN_S_OFFSETS = 1
 RAVEN_S_CAPACITY = 2
 RAVEN_S_WAIT = 4
+RAVEN_S_IDS = 8
 
 u32p = C.POINTER(C.c_uint32)
 f32p = C.POINTER(C.c_float)
@@ -130,6 +134,26 @@ class Rows(C.Structure):
     ]
 
 
+class Adjustments(C.Structure):
+    _fields_ = [
+        ("bias", C.c_void_p),
+        ("ld_bias", C.c_uint64),
+        ("allow", C.c_void_p),
+        ("allow_count", C.c_uint64),
+        ("ld_allow", C.c_uint64),
+        ("allow_rows", C.c_void_p),
+        ("seen", C.c_void_p),
+        ("seen_total", C.c_uint64),
+        ("seen_starts", C.c_void_p),
+        ("repetition", C.c_void_p),
+        ("presence", C.c_void_p),
+        ("frequency", C.c_void_p),
+        ("repetition_all", C.c_float),
+        ("presence_all", C.c_float),
+        ("frequency_all", C.c_float),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/raven_gpu.h
 SIGNATURES = {
     "raven_graph_build": (C.c_int, [f32p, C.c_uint64, C.c_uint32, C.POINTER(BuildConfig), C.POINTER(C.c_void_p)]),
@@ -165,6 +189,11 @@ SIGNATURES = {
     "raven_fp8_decode_device": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint32,
                                           C.c_void_p, C.c_uint64, C.c_void_p]),
     "raven_index_fp8_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "raven_int4_write_device": (C.c_int, [C.c_void_p, C.c_int32, C.c_uint64, C.c_uint32, C.c_uint64, C.c_void_p,
+                                          C.POINTER(Rows), C.c_void_p, C.c_void_p]),
+    "raven_int4_read_device": (C.c_int, [C.POINTER(Rows), C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p, C.c_int32,
+                                         C.c_uint64, C.c_void_p, C.c_void_p]),
+    "raven_index_int4_device": (C.c_int, [C.c_void_p, C.POINTER(Rows), C.c_void_p]),
     "raven_scores_device": (C.c_int, [C.POINTER(Rows), C.POINTER(Rows), C.c_uint32, C.c_float, C.c_void_p, C.c_void_p,
                                       C.c_int32, C.c_uint64, C.c_void_p, C.c_void_p]),
     "raven_group_scores_device": (C.c_int, [C.POINTER(Rows), C.c_void_p, C.POINTER(Rows), C.c_void_p, C.c_uint32,
@@ -175,6 +204,9 @@ SIGNATURES = {
     "raven_scoring_status_device": (C.c_int, [C.c_void_p, C.c_void_p]),
     "raven_topk_rows_device": (C.c_int, [C.c_void_p, C.c_int32, C.c_uint64, C.c_uint64, C.c_uint64, C.c_void_p,
                                          C.c_uint32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "raven_adjust_scores_device": (C.c_int, [C.c_void_p, C.c_int32, C.c_uint64, C.c_uint64, C.c_uint64,
+                                             C.POINTER(Adjustments), C.c_int32, C.c_void_p, C.c_uint64, C.c_void_p,
+                                             C.c_void_p]),
     "raven_limits": (None, [C.POINTER(Limits)]),
     "raven_index_set_tuning": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32]),
     "raven_index_set_small_batch": (C.c_int, [C.c_void_p, C.c_uint64]),

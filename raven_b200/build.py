@@ -17,9 +17,9 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libraven_gpu.so")
 
-SOURCES = ["raven_gpu.cu", "scoring.cu", "host_index.cpp"]
-DEPS = SOURCES + ["search_kernel.cuh", "search_cta.cuh", "knn_tc.cuh", "score_tc.cuh", "topk.cuh", "fp8.cuh", "internal.h",
-                  "host_index.h"]
+SOURCES = ["raven_gpu.cu", "scoring.cu", "rows4.cu", "host_index.cpp"]
+DEPS = SOURCES + ["search_kernel.cuh", "search_cta.cuh", "knn_tc.cuh", "score_tc.cuh", "topk.cuh", "fp8.cuh",
+                  "int4.cuh", "adjust.cuh", "status.cuh", "launch.h", "internal.h", "host_index.h"]
 
 
 def nvcc_path() -> str:

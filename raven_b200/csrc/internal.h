@@ -8,6 +8,8 @@
 #include <cstdint>
 #include <string>
 
+#include "../../include/raven_gpu.h"
+
 namespace raven_internal {
 
 // Sets the calling thread's raven_last_error() message and returns `code`.
@@ -19,6 +21,16 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_tiled();
 // FP8 codes of f32 rows held in the index's lane-major order (pitch dim).
 int fp8_encode_lane_major(const float* d_rows, uint64_t n, uint32_t dim, uint8_t* d_codes, uint64_t ld_codes,
                           uint8_t* d_exps, uint64_t ld_exps, cudaStream_t st);
+
+// Values under one scale word of 4-bit rows of a type, 0 for other types.
+uint32_t int4_group(int32_t type);
+// raven_scores_device with 4-bit vectors.
+int int4_scores(const raven_rows* q, const raven_rows* v, uint32_t dim, float alpha, const float* d_bias, void* d_out,
+                int32_t out_type, uint64_t ld, int32_t* d_status, void* stream);
+// Takes the status of the operators of rows4.cu (raven_scoring_status_device).
+int rows4_status(int* d_status, cudaStream_t st);
+// 4-bit rows of f32 rows held in the index's lane-major order.
+int int4_write_lane_major(const float* d_rows, uint64_t n, uint32_t dim, const raven_rows* out, cudaStream_t st);
 
 }  // namespace raven_internal
 

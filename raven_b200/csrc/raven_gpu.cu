@@ -1726,6 +1726,14 @@ int raven_index_fp8_device(raven_index* ix, uint8_t* d_codes, uint64_t ld_codes,
                                                (cudaStream_t)stream);
 }
 
+int raven_index_int4_device(raven_index* ix, const raven_rows* out, void* stream) {
+  NvtxRange nvtx_range("raven.index_int4");
+  if (!ix) return fail(RAVEN_EINVAL, "null index");
+  CU(cudaSetDevice(ix->device));
+  if (ix->n == 0) return RAVEN_OK;
+  return raven_internal::int4_write_lane_major(ix->d_vec, ix->n, ix->dim, out, (cudaStream_t)stream);
+}
+
 int raven_index_set_small_batch(raven_index* ix, uint64_t max_nq) {
   if (!ix) return fail(RAVEN_EINVAL, "null index");
   ix->small_batch_max = max_nq;

@@ -1,0 +1,309 @@
+// Operators of the C ABI (include/raven_gpu.h) on 4-bit rows: written, read back
+// and scored against (int4.cuh); and scores put right for what a query has seen, a
+// bias and filters (adjust.cuh).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "../../include/raven_gpu.h"
+#include "internal.h"
+#include "launch.h"
+#include "status.cuh"
+#include "adjust.cuh"
+#include "int4.cuh"
+
+using namespace raven_launch;
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// 4-bit rows.
+// ---------------------------------------------------------------------------
+using raven_internal::int4_group;
+using raven_int4::kBlock;
+
+int kind_of(int32_t t) { return t == RAVEN_TYPE_F32 ? 0 : t == RAVEN_TYPE_F16 ? 1 : 2; }
+
+int check_int4(const raven_rows* r, uint32_t dim, const char* what) {
+  const std::string w(what);
+  if (!r) return fail(RAVEN_EINVAL, w + ": null");
+  const uint64_t group = int4_group(r->type);
+  if (!group) return fail(RAVEN_EINVAL, w + ": type must be 4 bits");
+  if (r->rows > kMaxRows) return fail(RAVEN_ELIMIT, w + ": more than 2^31 - 1 rows");
+  if (r->rows == 0) return RAVEN_OK;
+  if (!r->data || !r->exps) return fail(RAVEN_EINVAL, w + ": 4-bit rows need codes and scale words");
+  if (!aligned(r->data, 16) || r->ld % 16 || r->ld < (dim + 31ull) / 32 * 16)
+    return fail(RAVEN_EINVAL, w + ": 4-bit codes must start on 16 bytes, their pitch a multiple of 16 of at least dim / 2");
+  const uint64_t per = kBlock / group;
+  if (!aligned(r->exps, 4 * per) || r->ld_exps % per || r->ld_exps < (dim + kBlock - 1ull) / kBlock * per)
+    return fail(RAVEN_EINVAL, w + ": scale words must start on those of 128 values, their pitch a multiple of them");
+  return RAVEN_OK;
+}
+
+template <typename T, bool LANE>
+cudaError_t launch_write(raven_int4::Write p, int sms, cudaStream_t st) {
+  const bool vec = !LANE && p.ld * sizeof(T) % 16 == 0 && aligned(p.x, 16);
+  const uint64_t grid = std::min<uint64_t>((p.m + p.run - 1) / p.run, (uint64_t)sms * 64);
+  static Allowed none;
+  return launch(vec ? raven_int4::write_kernel<T, true, LANE> : raven_int4::write_kernel<T, false, LANE>, grid, 256, 0,
+                none, st, p);
+}
+
+// Up to here every CTA looks for its slots among the later ones.
+constexpr uint64_t kFewSlots = 4096;
+constexpr uint64_t kMaxSlots = 1ull << 30;
+
+int write_rows(const void* x, int32_t type, uint64_t m, uint32_t dim, uint64_t ld, bool lane, const int32_t* slots,
+               const raven_rows* out, int32_t* status, cudaStream_t st) {
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  raven_int4::Write p{};
+  p.x = x;
+  p.m = m;
+  p.ld = ld;
+  p.dim = dim;
+  p.group = int4_group(out->type);
+  p.units = (dim + 31) / 32;
+  p.codes = (uint8_t*)out->data;
+  p.words = (uint32_t*)out->exps;
+  p.n = out->rows;
+  p.ld_codes = out->ld;
+  p.ld_words = out->ld_exps;
+  p.slots = slots;
+  p.status = status;
+  const uint32_t per = (dim + p.group - 1) / p.group * (p.group / 8);
+  p.run = std::min(raven_int4::kRun, std::max(1u, 256 / per));
+  raven_int4::Claim* table = nullptr;
+  cudaError_t e = cudaSuccess;
+  if (slots && m > kFewSlots) {
+    while ((1ull << p.bits) < 2 * m) ++p.bits;
+    CU(cudaMallocAsync((void**)&table, sizeof(raven_int4::Claim) << p.bits, st));
+    p.table = table;
+    static Allowed none;
+    e = cudaMemsetAsync(table, 0xff, sizeof(raven_int4::Claim) << p.bits, st);
+    if (e == cudaSuccess)
+      e = launch(raven_int4::claim_kernel, (m + 255) / 256, 256, 0, none, st, slots, (uint32_t)m, p.n, table, p.bits);
+  }
+  if (e == cudaSuccess)
+    e = type == RAVEN_TYPE_F32   ? (lane ? launch_write<float, true>(p, sms, st) : launch_write<float, false>(p, sms, st))
+        : type == RAVEN_TYPE_F16 ? launch_write<__half, false>(p, sms, st)
+                                 : launch_write<__nv_bfloat16, false>(p, sms, st);
+  if (table) cudaFreeAsync(table, st);
+  if (e != cudaSuccess) return fail(RAVEN_ECUDA, std::string("4-bit rows: ") + cudaGetErrorString(e));
+  return RAVEN_OK;
+}
+
+template <typename T>
+cudaError_t launch_read(const raven_int4::Read& p, int sms, cudaStream_t st) {
+  const bool vec = p.ld * sizeof(T) % 16 == 0 && aligned(p.out, 16);
+  constexpr uint64_t V = 16 / sizeof(T);
+  const uint64_t items = p.m * ((p.dim + V - 1) / V);
+  const uint64_t grid = std::min<uint64_t>((items + 255) / 256, (uint64_t)sms * 32);
+  static Allowed none;
+  return launch(vec ? raven_int4::read_kernel<T, true> : raven_int4::read_kernel<T, false>, grid, 256, 0, none, st, p);
+}
+
+// ---------------------------------------------------------------------------
+// Adjusted scores.
+// ---------------------------------------------------------------------------
+template <typename T>
+cudaError_t launch_adjust(const raven_adjust::Params& p, bool largest, cudaStream_t st) {
+  static Allowed allowed[2];
+  const uint32_t smem = p.seen ? p.tile * 4 + (p.tile + 31) / 32 * 4 : 0;
+  return launch(largest ? raven_adjust::adjust_kernel<T, true> : raven_adjust::adjust_kernel<T, false>, p.nq * p.tiles, 256,
+                smem, allowed[largest], st, p);
+}
+
+__global__ void status_kernel(int* status) {
+  raven_score::after_previous();
+  atomicOr(status, atomicExch(&raven_score::g_status, 0));
+}
+
+}  // namespace
+
+namespace raven_internal {
+
+uint32_t int4_group(int32_t t) {
+  return t == RAVEN_TYPE_INT4_32 ? 32 : t == RAVEN_TYPE_INT4_64 ? 64 : t == RAVEN_TYPE_INT4_128 ? 128 : 0;
+}
+
+int rows4_status(int* d_status, cudaStream_t st) {
+  static Allowed none;
+  CU(launch(status_kernel, 1, 1, 0, none, st, d_status));
+  return RAVEN_OK;
+}
+
+int int4_scores(const raven_rows* q, const raven_rows* v, uint32_t dim, float alpha, const float* bias, void* out,
+                int32_t out_type, uint64_t ld, int32_t* status, void* stream) {
+  if (int rc = check_dim(dim)) return rc;
+  if (int rc = check_int4(v, dim, "vectors")) return rc;
+  if (!q || !float_type(q->type)) return fail(RAVEN_EINVAL, "queries: type must be f32, f16 or bf16 with 4-bit vectors");
+  if (q->rows > kMaxRows) return fail(RAVEN_ELIMIT, "queries: more than 2^31 - 1 rows");
+  if (q->rows && (!q->data || !aligned(q->data, type_size(q->type))))
+    return fail(RAVEN_EINVAL, "queries: null or not aligned to their type");
+  if (q->rows && q->ld < dim) return fail(RAVEN_EINVAL, "queries: pitch below dim");
+  if (!float_type(out_type)) return fail(RAVEN_EINVAL, "scores: type must be f32, f16 or bf16");
+  if (!aligned(bias, 4) || !aligned(status, 4)) return fail(RAVEN_EINVAL, "scores: bias and status must start on 4 bytes");
+  if (q->rows == 0 || v->rows == 0) return RAVEN_OK;
+  if (!out) return fail(RAVEN_EINVAL, "scores: null output");
+  if (!aligned(out, type_size(out_type))) return fail(RAVEN_EINVAL, "scores: output is not aligned to its type");
+  if (ld < v->rows) return fail(RAVEN_EINVAL, "scores: output pitch below the number of vectors");
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  raven_int4::Scores p{};
+  p.q = q->data;
+  p.q_type = kind_of(q->type);
+  p.nq = q->rows;
+  p.ld_q = q->ld;
+  p.codes = (const uint8_t*)v->data;
+  p.words = (const uint32_t*)v->exps;
+  p.n = v->rows;
+  p.ld_codes = v->ld;
+  p.ld_words = v->ld_exps;
+  p.dim = dim;
+  p.group = int4_group(v->type);
+  p.units = (dim + 31) / 32;
+  p.alpha = alpha;
+  p.bias = bias;
+  p.out = out;
+  p.out_type = kind_of(out_type);
+  p.ld = ld;
+  static Allowed none;
+  const uint64_t grid = std::min<uint64_t>((p.n * ((p.nq + 7) / 8) + 7) / 8, (uint64_t)sms * 64);
+  CU(launch(q->type == RAVEN_TYPE_F32   ? raven_int4::scores_kernel<float>
+            : q->type == RAVEN_TYPE_F16 ? raven_int4::scores_kernel<__half>
+                                        : raven_int4::scores_kernel<__nv_bfloat16>,
+            grid, 256, 0, none, st, p));
+  return RAVEN_OK;
+}
+
+int int4_write_lane_major(const float* d_rows, uint64_t n, uint32_t dim, const raven_rows* out, cudaStream_t st) {
+  if (int rc = check_int4(out, dim, "out")) return rc;
+  if (out->rows < n) return fail(RAVEN_EINVAL, "out: fewer rows than the index");
+  return write_rows(d_rows, RAVEN_TYPE_F32, n, dim, dim, true, nullptr, out, nullptr, st);
+}
+
+}  // namespace raven_internal
+
+extern "C" {
+
+int raven_int4_write_device(const void* d_rows, int32_t type, uint64_t m, uint32_t dim, uint64_t ld,
+                            const int32_t* d_slots, const raven_rows* out, int32_t* d_status, void* stream) {
+  NvtxRange nvtx_range("raven.int4_write");
+  if (int rc = check_dim(dim)) return rc;
+  if (!float_type(type)) return fail(RAVEN_EINVAL, "rows: type must be f32, f16 or bf16");
+  if (int rc = check_int4(out, dim, "out")) return rc;
+  if (!aligned(d_slots, 4) || !aligned(d_status, 4)) return fail(RAVEN_EINVAL, "slots and status must start on 4 bytes");
+  if (m == 0) return RAVEN_OK;
+  if (m > (d_slots ? kMaxSlots : kMaxRows)) return fail(RAVEN_ELIMIT, "rows: more than 2^31 - 1, or 2^30 with slots");
+  if (!d_rows) return fail(RAVEN_EINVAL, "rows: null");
+  if (ld < dim) return fail(RAVEN_EINVAL, "rows: pitch below dim");
+  if (!aligned(d_rows, type_size(type))) return fail(RAVEN_EINVAL, "rows: not aligned to their type");
+  if (!d_slots && m > out->rows) return fail(RAVEN_EINVAL, "out: fewer rows than are written");
+  return write_rows(d_rows, type, m, dim, ld, false, d_slots, out, d_status, (cudaStream_t)stream);
+}
+
+int raven_int4_read_device(const raven_rows* rows, uint32_t dim, const int32_t* d_ids, uint64_t m, void* d_out,
+                           int32_t out_type, uint64_t ld, int32_t* d_status, void* stream) {
+  NvtxRange nvtx_range("raven.int4_read");
+  if (int rc = check_dim(dim)) return rc;
+  if (int rc = check_int4(rows, dim, "rows")) return rc;
+  if (!float_type(out_type)) return fail(RAVEN_EINVAL, "output: type must be f32, f16 or bf16");
+  if (!aligned(d_ids, 4) || !aligned(d_status, 4)) return fail(RAVEN_EINVAL, "ids and status must start on 4 bytes");
+  if (m == 0) return RAVEN_OK;
+  if (m > kMaxRows) return fail(RAVEN_ELIMIT, "output: more than 2^31 - 1 rows");
+  if (!d_out || !aligned(d_out, type_size(out_type))) return fail(RAVEN_EINVAL, "output: null or not aligned to its type");
+  if (ld < dim) return fail(RAVEN_EINVAL, "output: pitch below dim");
+  if (!d_ids && m > rows->rows) return fail(RAVEN_EINVAL, "rows: fewer than are read");
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  raven_int4::Read p{};
+  p.codes = (const uint8_t*)rows->data;
+  p.words = (const uint32_t*)rows->exps;
+  p.n = rows->rows;
+  p.ld_codes = rows->ld;
+  p.ld_words = rows->ld_exps;
+  p.dim = dim;
+  p.group = raven_internal::int4_group(rows->type);
+  p.units = (dim + 31) / 32;
+  p.ids = d_ids;
+  p.m = m;
+  p.out = d_out;
+  p.ld = ld;
+  p.status = d_status;
+  cudaStream_t st = (cudaStream_t)stream;
+  CU(out_type == RAVEN_TYPE_F32   ? launch_read<float>(p, sms, st)
+     : out_type == RAVEN_TYPE_F16 ? launch_read<__half>(p, sms, st)
+                                  : launch_read<__nv_bfloat16>(p, sms, st));
+  return RAVEN_OK;
+}
+
+int raven_adjust_scores_device(const void* d_scores, int32_t type, uint64_t nq, uint64_t n, uint64_t ld,
+                               const raven_adjustments* by, int32_t largest, void* d_out, uint64_t ld_out,
+                               int32_t* d_status, void* stream) {
+  NvtxRange nvtx_range("raven.adjust_scores");
+  if (!by) return fail(RAVEN_EINVAL, "null adjustments");
+  if (!float_type(type)) return fail(RAVEN_EINVAL, "scores: type must be f32, f16 or bf16");
+  if (nq > kMaxRows || n > kMaxRows) return fail(RAVEN_ELIMIT, "more than 2^31 - 1 queries or vectors");
+  if (nq == 0 || n == 0) return RAVEN_OK;
+  const uint64_t size = type_size(type);
+  if (!d_scores || !d_out) return fail(RAVEN_EINVAL, "scores: null");
+  if (!aligned(d_scores, size) || !aligned(d_out, size)) return fail(RAVEN_EINVAL, "scores: not aligned to their type");
+  if (nq == 1) ld = ld_out = n;
+  if (ld < n || ld_out < n) return fail(RAVEN_EINVAL, "scores: pitch below the row length");
+  if (ld > 1ull << 40 || ld_out > 1ull << 40) return fail(RAVEN_ELIMIT, "scores: pitch above 2^40");
+  const uintptr_t a = (uintptr_t)d_scores, b = (uintptr_t)d_out;
+  const uint64_t wide = ((nq - 1) * ld + n) * size, wide_out = ((nq - 1) * ld_out + n) * size;
+  if (a < b + wide_out && b < a + wide && !(a == b && ld == ld_out))
+    return fail(RAVEN_EINVAL, "scores: the output overlaps them, but is not the same");
+  if (!aligned(by->bias, 4) || !aligned(by->allow, 4) || !aligned(by->allow_rows, 4) || !aligned(by->seen, 4) ||
+      !aligned(by->seen_starts, 8) || !aligned(by->repetition, 4) || !aligned(by->presence, 4) ||
+      !aligned(by->frequency, 4) || !aligned(d_status, 4))
+    return fail(RAVEN_EINVAL, "an argument is not aligned to its type");
+  if (by->bias && by->ld_bias && by->ld_bias < n) return fail(RAVEN_EINVAL, "bias: pitch below the row length");
+  if (by->allow) {
+    if (by->allow_count == 0 || by->allow_count > kMaxRows) return fail(RAVEN_EINVAL, "filters: 1 to 2^31 - 1 of them");
+    if (by->ld_allow < (n + 31) / 32 && by->allow_count > 1) return fail(RAVEN_EINVAL, "filters: pitch below n / 32 words");
+    if (!by->allow_rows && by->allow_count != 1 && by->allow_count != nq)
+      return fail(RAVEN_EINVAL, "filters: one, or one for each query, without allow_rows");
+  }
+  if (by->seen_starts && !by->seen && by->seen_total) return fail(RAVEN_EINVAL, "seen: null");
+  if (by->seen && !by->seen_starts) return fail(RAVEN_EINVAL, "seen: needs its starts");
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  raven_adjust::Params p{};
+  p.x = d_scores;
+  p.out = d_out;
+  p.nq = nq;
+  p.n = n;
+  p.ld = ld;
+  p.ld_out = ld_out;
+  p.bias = by->bias;
+  p.ld_bias = by->ld_bias;
+  p.allow = by->allow;
+  p.allow_count = by->allow_count;
+  p.ld_allow = by->ld_allow;
+  p.allow_rows = by->allow_rows;
+  p.seen = by->seen;
+  p.seen_total = by->seen_total;
+  p.starts = by->seen_starts;
+  p.repetition = by->repetition;
+  p.presence = by->presence;
+  p.frequency = by->frequency;
+  p.repetition_all = by->repetition_all;
+  p.presence_all = by->presence_all;
+  p.frequency_all = by->frequency_all;
+  p.status = d_status;
+  p.tile = 4096;
+  p.tiles = (n + p.tile - 1) / p.tile;
+  if (nq * p.tiles > kMaxRows) return fail(RAVEN_ELIMIT, "scores: more tiles than a launch holds");
+  cudaStream_t st = (cudaStream_t)stream;
+  CU(type == RAVEN_TYPE_F32   ? launch_adjust<float>(p, largest != 0, st)
+     : type == RAVEN_TYPE_F16 ? launch_adjust<__half>(p, largest != 0, st)
+                              : launch_adjust<__nv_bfloat16>(p, largest != 0, st));
+  return RAVEN_OK;
+}
+
+}  // extern "C"

@@ -48,6 +48,7 @@
 
 #include "fp8.cuh"
 #include "internal.h"
+#include "status.cuh"
 #include "knn_tc.cuh"
 
 namespace raven_score {
@@ -75,12 +76,6 @@ constexpr uint32_t kBand = 8;          // query tiles walked together (they shar
 constexpr uint32_t kHeldBlocks = 8;    // (HELD) K blocks of queries that a CTA holds
 constexpr uint32_t kHeldUnits = 32;    // and query blocks that it encodes
 enum : int { kOutF32 = 0, kOutF16 = 1, kOutBf16 = 2 };
-enum : int { kStatusOffsets = 1, kStatusCapacity = 2, kStatusWait = 4 };
-
-// The status of calls that are given no word for it, per device, until it is taken
-// (raven_scoring_status_device).
-__device__ int g_status;
-__device__ inline void tell(int* status, int bits) { atomicOr(status ? status : &g_status, bits); }
 
 // Sums over the groups before a chunk of 32 groups: their tiles, their scores.
 struct alignas(16) Chunk {

@@ -3,115 +3,23 @@
 // grouped, score_tc.cuh) and the best k of each row of scores (topk.cuh).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <nvtx3/nvToolsExt.h>
 
 #include <algorithm>
-#include <atomic>
-#include <mutex>
 
 #include "../../include/raven_gpu.h"
 #include "fp8.cuh"
 #include "internal.h"
+#include "launch.h"
 #include "score_tc.cuh"
 #include "topk.cuh"
 
 using raven_internal::encode_tiled;
-using raven_internal::fail;
 
 using raven_score::after_previous;
 
+using namespace raven_launch;
+
 namespace {
-
-struct NvtxRange {
-  explicit NvtxRange(const char* name) { nvtxRangePushA(name); }
-  ~NvtxRange() { nvtxRangePop(); }
-  NvtxRange(const NvtxRange&) = delete;
-  NvtxRange& operator=(const NvtxRange&) = delete;
-};
-
-#define CU(call)                                                                        \
-  do {                                                                                  \
-    cudaError_t e_ = (call);                                                            \
-    if (e_ != cudaSuccess) return fail(RAVEN_ECUDA, std::string(#call ": ") + cudaGetErrorString(e_)); \
-  } while (0)
-
-constexpr uint64_t kMaxRows = 0x7fffffffull;  // rows are TMA coordinates (int32)
-constexpr uint32_t kMaxDim = 65536;
-constexpr uint32_t kBlock = 128;              // values under one scale
-
-uint64_t type_size(int32_t t) {
-  return t == RAVEN_TYPE_F32 ? 4 : t == RAVEN_TYPE_F16 || t == RAVEN_TYPE_BF16 ? 2 : t == RAVEN_TYPE_FP8 ? 1 : 0;
-}
-bool aligned(const void* p, uint64_t a) { return (uintptr_t)p % a == 0; }
-
-// What a device's first call sets up is no part of a stream's work: this thread
-// does it although one of its streams is being captured, which otherwise ends
-// the capture.
-struct Apart {
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  Apart() { cudaThreadExchangeStreamCaptureMode(&mode); }
-  ~Apart() { cudaThreadExchangeStreamCaptureMode(&mode); }
-};
-
-// SMs of the current device. On a device's first call its default memory pool
-// is told to keep freed scratch (as raven_index_upload does): a pool that gives
-// it back at every synchronisation makes the next call wait for an allocation.
-int sm_count(int* out) {
-  static std::mutex mu;
-  static int count[256] = {};
-  int dev = 0;
-  CU(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 256) return fail(RAVEN_EINVAL, "device ordinal out of range");
-  std::lock_guard<std::mutex> lk(mu);
-  if (!count[dev]) {
-    CU(cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev));
-    Apart apart;
-    cudaMemPool_t pool;
-    uint64_t keep = ~0ull;
-    if (cudaDeviceGetDefaultMemPool(&pool, dev) == cudaSuccess)
-      cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
-  }
-  *out = count[dev];
-  return RAVEN_OK;
-}
-
-// Launches `kern` so that it may start while the kernel before it in the stream
-// ends. Every kernel here waits for that one (after_previous) before it touches
-// memory, and lets its own successor start at once. `allowed`: devices (bits)
-// on which the kernel may already use `smem` bytes; the attribute is set again
-// when a launch is refused (a context replaced since).
-struct Allowed {
-  std::atomic<uint64_t> mask{0};
-};
-template <typename... K, typename... A>
-cudaError_t launch(void (*kern)(K...), uint64_t grid, int threads, uint32_t smem, Allowed& allowed, cudaStream_t st,
-                   A&&... args) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  const uint64_t bit = 1ull << (dev & 63);
-  cudaLaunchConfig_t c{};
-  c.gridDim = dim3((unsigned)grid);
-  c.blockDim = dim3((unsigned)threads);
-  c.dynamicSmemBytes = smem;
-  c.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  c.attrs = &at;
-  c.numAttrs = 1;
-  for (int turn = 0;; ++turn) {
-    if (smem > 48 * 1024 && (turn || dev >= 64 || !(allowed.mask.load(std::memory_order_relaxed) & bit))) {
-      Apart apart;
-      e = cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      if (e != cudaSuccess) return e;
-      allowed.mask.fetch_or(bit, std::memory_order_relaxed);
-    }
-    e = cudaLaunchKernelEx(&c, kern, args...);
-    if (e != cudaErrorInvalidValue || turn || smem <= 48 * 1024) return e;
-    (void)cudaGetLastError();
-  }
-}
 
 // ---------------------------------------------------------------------------
 // FP8 rows. Block b of a row: e = the least exponent with max|x| <= 448 * 2^e
@@ -277,10 +185,6 @@ int encode_rows(const void* x, int32_t type, uint64_t n, uint32_t dim, uint64_t 
 uint64_t exps_pitch(uint32_t dim) { return ((dim + kBlock - 1) / kBlock + 3) / 4 * 4; }
 uint64_t codes_pitch(uint32_t dim) { return (dim + 15) / 16 * 16; }
 
-int check_dim(uint32_t dim) {
-  if (dim == 0 || dim > kMaxDim) return fail(RAVEN_ELIMIT, "dim must be in 1..65536");
-  return RAVEN_OK;
-}
 int check_fp8(const uint8_t* codes, uint64_t ld_codes, const uint8_t* exps, uint64_t ld_exps, uint32_t dim) {
   if (!codes || !exps) return fail(RAVEN_EINVAL, "FP8 rows need codes and exponents");
   if (!aligned(codes, 16) || ld_codes % 16 || ld_codes < codes_pitch(dim))
@@ -795,6 +699,8 @@ int raven_fp8_decode_device(const uint8_t* d_codes, uint64_t ld_codes, const uin
 int raven_scores_device(const raven_rows* q, const raven_rows* v, uint32_t dim, float alpha, const float* d_bias,
                         void* d_out, int32_t out_type, uint64_t ld_out, int32_t* d_status, void* stream) {
   NvtxRange nvtx_range("raven.scores");
+  if (v && raven_internal::int4_group(v->type))
+    return raven_internal::int4_scores(q, v, dim, alpha, d_bias, d_out, out_type, ld_out, d_status, stream);
   return run_scores(q, nullptr, v, nullptr, 1, dim, alpha, d_bias, d_out, out_type, ld_out, 0, d_status, stream);
 }
 
@@ -803,6 +709,7 @@ int raven_group_scores_device(const raven_rows* q, const int64_t* d_q_offsets, c
                               const float* d_bias, void* d_out, int32_t out_type, uint64_t capacity, int32_t* d_status,
                               void* stream) {
   NvtxRange nvtx_range("raven.group_scores");
+  if (v && raven_internal::int4_group(v->type)) return fail(RAVEN_EINVAL, "vectors: grouped scores take f16, bf16 or FP8 rows");
   if (groups && (!d_q_offsets || !d_v_offsets)) return fail(RAVEN_EINVAL, "offsets: null");
   if (groups && (!aligned(d_q_offsets, 8) || !aligned(d_v_offsets, 8)))
     return fail(RAVEN_EINVAL, "offsets: not aligned to 64 bits");
@@ -846,7 +753,7 @@ int raven_scoring_status_device(int32_t* d_status, void* stream) {
   if (!aligned(d_status, 4)) return fail(RAVEN_EINVAL, "status must start on 4 bytes");
   static Allowed none;
   CU(launch(status_kernel, 1, 1, 0, none, (cudaStream_t)stream, d_status));
-  return RAVEN_OK;
+  return raven_internal::rows4_status(d_status, (cudaStream_t)stream);
 }
 
 int raven_topk_rows_device(const void* d_scores, int32_t type, uint64_t nq, uint64_t n, uint64_t ld,

@@ -3,17 +3,29 @@
 * `Fp8Rows`      — embedding rows as e4m3 codes with one power-of-two scale per
                    128 values (a quarter of f32, like the SQ8 codes, but with a
                    scale for each block of each row): encode / decode / of_index.
-* `scores`       — every query against every row (FP8, f16 or bf16 rows).
+* `Int4Rows`     — rows as 4-bit codes with a step and an offset per group of 32,
+                   64 or 128 values (an eighth of f32): encode, write (rows of a
+                   collection in place), decode (all, or those of some ids),
+                   of_index.
+* `scores`       — every query against every row (4-bit, FP8, f16 or bf16 rows).
 * `group_scores` — the queries of each group against the rows of that group,
                    groups of any size: partitions (tenants, lists) of a
                    collection, or one projection per group.
 * `group_rows`   — where each query's scores start in grouped scores.
+* `adjust`       — scores put right before the best are taken: less for rows that
+                   a query has seen, a bias per row, filters.
 * `top_k`        — the best k of each row of scores, dense or packed.
 * `take_status`  — what went wrong on a device in calls without a status.
 
     rows = Fp8Rows.encode(X)                              # or Fp8Rows.of_index(searcher.device_index)
     near = scores(Q, rows, alpha=-2.0, bias=(rows.decode() ** 2).sum(1))
     dist, ids, _ = top_k(near, 10, largest=False)         # squared distances less |q|^2
+
+    held = Int4Rows.encode(X, group=64)                   # a collection that is kept up to date in place
+    held.write(changed, slots)
+    s = adjust(scores(Q, held), allow=filters, allow_rows=tenant, seen=history, seen_starts=starts, presence=1.0)
+    best, ids, _ = top_k(s, 100)
+    near = held.decode(ids.reshape(-1))                   # the candidates, for ranking
 
 Everything runs in libraven_gpu.so on the current stream of the tensors'
 device and returns without waiting; nothing is differentiable. The reference
@@ -204,19 +216,178 @@ class Fp8Rows:
         return Fp8Rows(self.codes[first:first + count], self.exps[first:first + count], self.dim)
 
 
-Rows = Union[torch.Tensor, Fp8Rows]
+_GROUPS = {32: L.RAVEN_TYPE_INT4_32, 64: L.RAVEN_TYPE_INT4_64, 128: L.RAVEN_TYPE_INT4_128}
+
+
+def _ids(name: str, t: torch.Tensor, device: int) -> int:
+    """How many of a 1-D int32 tensor of ids or slots on a GPU."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous 1-D int32 tensor")
+    _on(device, t)
+    return t.numel()
+
+
+class Int4Rows:
+    """Rows held in 4 bits: `codes` uint8 [n, 16 * ceil(dim / 32)] and `scales`
+    int32 [n, ceil(dim / 128) * (128 / group)], a word for each `group` (32, 64
+    or 128) of a row's values that holds a step and an offset of -127..127
+    steps; a value is (code + offset) * step. include/raven_gpu.h has the layout
+    of both. Their contents may change, the two tensors stay."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, dim: int, group: int = 64):
+        self._hold(codes, scales, dim, group)
+
+    def _hold(self, codes: torch.Tensor, scales: torch.Tensor, dim: int, group: int) -> None:
+        if dim < 1:
+            raise ValueError("dim must be at least 1")
+        if group not in _GROUPS:
+            raise ValueError(f"group must be 32, 64 or 128, not {group}")
+        if codes.dim() != 2 or scales.dim() != 2 or codes.dtype != torch.uint8 or scales.dtype != torch.int32 or \
+                not codes.is_cuda:
+            raise ValueError("codes and scales must be 2-D uint8 and int32 tensors on a GPU")
+        (n, wide), (pitch, step) = codes.shape, codes.stride()
+        (sn, swide), (spitch, sstep) = scales.shape, scales.stride()
+        need, sneed = 16 * -(-dim // 32), -(-dim // BLOCK) * (BLOCK // group)
+        if wide < need or swide < sneed:
+            raise ValueError(f"dim {dim} needs {need} columns of codes and {sneed} of scales, got {wide} and {swide}")
+        if step != 1 or (sstep != 1 and swide > 1):
+            raise ValueError("codes and scales must hold each row's values side by side")
+        self.device_index = codes.get_device()
+        if sn != n or scales.get_device() != self.device_index:
+            raise ValueError("codes and scales must have the same rows and device")
+        if n <= 1:  # one row may come with any pitch
+            pitch, spitch = need, sneed
+        self._codes, self._scales, self._dim, self._group = codes, scales, dim, group
+        self._n, self._at, self._scales_at = n, codes.data_ptr(), scales.data_ptr()
+        self._held = L.Rows(self._at, self._scales_at, n, pitch, spitch, _GROUPS[group])
+
+    @property
+    def _rows(self) -> L.Rows:
+        """The rows as the library takes them, where the tensors are now (resize_ and set_ move them)."""
+        if self._codes.data_ptr() != self._at or self._scales.data_ptr() != self._scales_at:
+            self._hold(self._codes, self._scales, self._dim, self._group)
+        return self._held
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
+
+    @property
+    def dim(self) -> int:
+        return self._dim
+
+    @property
+    def group(self) -> int:
+        return self._group
+
+    @property
+    def device(self) -> torch.device:
+        return self._codes.device
+
+    def __len__(self) -> int:
+        return self._rows.rows
+
+    @staticmethod
+    def empty(n: int, dim: int, device, group: int = 64) -> "Int4Rows":
+        """Room for n rows, uninitialised."""
+        if dim < 1 or n < 0:
+            raise ValueError("n must not be negative and dim at least 1")
+        if group not in _GROUPS:
+            raise ValueError(f"group must be 32, 64 or 128, not {group}")
+        return Int4Rows(torch.empty(n, 16 * -(-dim // 32), dtype=torch.uint8, device=device),
+                        torch.empty(n, -(-dim // BLOCK) * (BLOCK // group), dtype=torch.int32, device=device), dim, group)
+
+    @staticmethod
+    def encode(x: torch.Tensor, group: int = 64, out: Optional["Int4Rows"] = None) -> "Int4Rows":
+        """The rows of a float32, float16 or bfloat16 matrix. A group's step is
+        the least, of 16 significant bits, whose 15 multiples cover the group's
+        range (and 127 its largest magnitude); values are rounded to the nearest
+        multiple, halves to even. A group with an infinity or a NaN is NaN as a
+        whole. `out`: rows to write instead of new ones (len(x) of them)."""
+        pitch = _matrix(x, "x")
+        n, dim = x.shape
+        if out is None:
+            out = Int4Rows.empty(n, dim, x.device, group)
+        elif len(out) != n or out.dim != dim:
+            raise ValueError(f"out holds {len(out)} rows of {out.dim}, expected {n} of {dim}")
+        out._write(x, pitch, None, None)
+        return out
+
+    def write(self, x: torch.Tensor, slots: torch.Tensor, status: Optional[torch.Tensor] = None) -> "Int4Rows":
+        """Rows of x as rows slots[i] (int32, on the GPU), as `encode` makes them.
+        Negative slots leave theirs out; of rows with the same slot the last is
+        held. Rows with a slot of len(self) and more are left out too, and
+        `status` (or `take_status`) gets RAVEN_S_IDS."""
+        pitch = _matrix(x, "x")
+        if x.shape[1] != self._dim:
+            raise ValueError(f"dim mismatch: expected {self._dim}, got {x.shape[1]}")
+        if _ids("slots", slots, self.device_index) != x.shape[0]:
+            raise ValueError(f"{x.shape[0]} rows need as many slots, got {slots.numel()}")
+        self._write(x, pitch, slots, status)
+        return self
+
+    def _write(self, x, pitch, slots, status) -> None:
+        device = self.device_index
+        if x.get_device() != device:
+            raise ValueError(f"x must be on cuda:{device}")
+        _call(device, L.load().raven_int4_write_device, x.data_ptr(), _TYPES[x.dtype], x.shape[0], _u32(self._dim), pitch,
+              _ptr(slots), self._rows, _status(status, device))
+
+    @staticmethod
+    def of_index(index, group: int = 64) -> "Int4Rows":
+        """4-bit rows of the vectors of a `DeviceIndex`, on its GPU."""
+        out = Int4Rows.empty(index.n, index.dim, torch.device("cuda", index.device), group)
+        _call(index.device, L.load().raven_index_int4_device, index._h, out._rows)
+        return out
+
+    def decode(self, ids: Optional[torch.Tensor] = None, *, dtype: torch.dtype = torch.float32,
+               out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The values, [n, dim], or those of the rows `ids` (int32, on the GPU):
+        float32 (exact), float16 or bfloat16 (rounded once). Rows of ids below 0
+        are 0; so are those of ids of len(self) and more, and `status` (or
+        `take_status`) gets RAVEN_S_IDS. `out`: a matrix to write."""
+        rows, device = self._rows, self.device_index
+        m = rows.rows if ids is None else _ids("ids", ids, device)
+        if out is not None:
+            dtype = out.dtype
+        if dtype not in _TYPES:
+            raise ValueError(f"values must be float32, float16 or bfloat16, not {dtype}")
+        pitch = self._dim
+        if out is None:
+            out = torch.empty(m, self._dim, dtype=dtype, device=self.device)
+        else:
+            if out.shape != (m, self._dim):
+                raise ValueError(f"out must be a matrix of {m} x {self._dim}")
+            pitch = _matrix(out, "out")
+            _on(device, out)
+        _call(device, L.load().raven_int4_read_device, rows, _u32(self._dim), _ptr(ids), m, out.data_ptr(), _TYPES[dtype],
+              pitch, _status(status, device))
+        return out
+
+    def rows(self, first: int, count: int) -> "Int4Rows":
+        """Rows [first, first + count), without a copy."""
+        if first < 0 or count < 0 or first + count > len(self):
+            raise ValueError(f"rows [{first}, {first + count}) of {len(self)}")
+        return Int4Rows(self.codes[first:first + count], self.scales[first:first + count], self.dim, self.group)
+
+
+Rows = Union[torch.Tensor, Fp8Rows, Int4Rows]
 
 
 def _operands(queries: Rows, vectors: Rows, dtype: torch.dtype, bias: Optional[torch.Tensor]):
     """(device, dim, nq, n, queries, vectors) as the library takes them, and what must stay alive until the call."""
-    fp8 = isinstance(vectors, Fp8Rows)
-    if fp8:
+    fp8, int4 = isinstance(vectors, Fp8Rows), isinstance(vectors, Int4Rows)
+    if fp8 or int4:
         device, dim, v = vectors.device_index, vectors._dim, vectors._rows
         n = vectors._n
     else:
         pitch = _matrix(vectors, "vectors")
         if vectors.dtype == torch.float32:
-            raise ValueError("vectors must be Fp8Rows, float16 or bfloat16 (Fp8Rows.encode holds float32 rows as FP8)")
+            raise ValueError("vectors must be Fp8Rows, Int4Rows, float16 or bfloat16 (Fp8Rows.encode holds float32 rows as FP8)")
         (n, dim), device, at = vectors.shape, vectors.get_device(), vectors.data_ptr()
         if at % 16 or pitch % 8:
             raise ValueError("16-bit vectors must start on 16 bytes, a multiple of 8 values apart "
@@ -227,9 +398,11 @@ def _operands(queries: Rows, vectors: Rows, dtype: torch.dtype, bias: Optional[t
             raise ValueError("FP8 queries need FP8 vectors")
         qdim, q, qdevice = queries._dim, queries._rows, queries.device_index
         nq = queries._n
+    elif isinstance(queries, Int4Rows):
+        raise ValueError("queries must be a matrix or Fp8Rows")
     else:
         pitch = _matrix(queries, "queries")
-        if not fp8:
+        if not fp8 and not int4:
             if queries.dtype != vectors.dtype:
                 raise ValueError(f"queries must have the vectors' type {vectors.dtype}, got {queries.dtype}")
             if pitch % 8 or queries.data_ptr() % 16:
@@ -268,14 +441,14 @@ def scores(queries: Rows, vectors: Rows, *, alpha: float = 1.0, bias: Optional[t
            status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """alpha * <query, vector> + bias[vector] for every pair, [nq, n] of `dtype`:
     summed in float32 on the tensor cores, rounded once. Float queries against
-    FP8 rows are encoded first. alpha = -2 with the vectors' squared norms as
+    FP8 rows are encoded first; against 4-bit rows they are taken as they are. alpha = -2 with the vectors' squared norms as
     bias ranks like squared distances. `out`: a matrix of `dtype` to write (any
     row pitch). `status`: an int32 that gets RAVEN_S_* bits; without it
     `take_status` tells whether the scores are valid."""
     device, dim, nq, n, q, v, keep = _operands(queries, vectors, dtype, bias)
     pitch = n
     if out is None:
-        out = (vectors._codes if isinstance(vectors, Fp8Rows) else vectors).new_empty((nq, n), dtype=dtype)
+        out = (vectors if isinstance(vectors, torch.Tensor) else vectors._codes).new_empty((nq, n), dtype=dtype)
     else:
         if out.shape != (nq, n) or out.dtype != dtype or (n > 1 and out.stride(1) != 1) or (nq > 1 and out.stride(0) < n):
             raise ValueError(f"out must be a {dtype} matrix of {nq} x {n}, each row's values side by side")
@@ -309,6 +482,8 @@ def group_scores(queries: Rows, query_offsets: torch.Tensor, vectors: Rows, vect
     all fit have them, and `status` gets RAVEN_S_CAPACITY. Groups whose offsets fall
     or leave the rows have no scores, and it gets RAVEN_S_OFFSETS; without a
     `status`, `take_status` tells of both."""
+    if isinstance(vectors, Int4Rows):
+        raise ValueError("grouped scores take Fp8Rows, float16 or bfloat16 vectors")
     device, dim, nq, n, q, v, keep = _operands(queries, vectors, dtype, bias)
     groups = _offsets("query_offsets", query_offsets, device)
     if _offsets("vector_offsets", vector_offsets, device) != groups:
@@ -355,6 +530,105 @@ def take_status(device=None) -> int:
     bits = torch.zeros(1, dtype=torch.int32, device=device)
     _call(bits.get_device(), L.load().raven_scoring_status_device, bits.data_ptr())
     return int(bits)
+
+
+def _scores_matrix(x: torch.Tensor, name: str) -> int:
+    """The row pitch of a matrix of scores."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or not x.is_cuda or x.dtype not in _TYPES:
+        raise ValueError(f"{name} must be a float32, float16 or bfloat16 matrix on a GPU")
+    (nq, n), (ld, step) = x.shape, x.stride()
+    if (n > 1 and step != 1) or (nq > 1 and ld < n):
+        raise ValueError(f"{name} must hold each row's values side by side and its rows one after another")
+    return max(ld, n)
+
+
+def _per_query(name: str, x, nq: int, device: int):
+    """(address, number) of a penalty: one number, or a float32 tensor of one for each query."""
+    if isinstance(x, torch.Tensor):
+        if x.dtype != torch.float32 or x.shape != (nq,) or not x.is_contiguous():
+            raise ValueError(f"{name} must be a number or a contiguous float32 tensor of {nq}")
+        _on(device, x)
+        return x.data_ptr(), 0.0
+    return None, float(x)
+
+
+def adjust(scores: torch.Tensor, *, bias: Optional[torch.Tensor] = None, allow: Optional[torch.Tensor] = None,
+           allow_rows: Optional[torch.Tensor] = None, seen: Optional[torch.Tensor] = None,
+           seen_starts: Optional[torch.Tensor] = None, repetition: Union[float, torch.Tensor] = 1.0,
+           presence: Union[float, torch.Tensor] = 0.0, frequency: Union[float, torch.Tensor] = 0.0,
+           largest: bool = True, out: Optional[torch.Tensor] = None,
+           status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Scores [nq, n] put right before `top_k` takes the best. In float32, and
+    rounded once to the scores' type:
+
+    1. What a query has seen (int32 ids seen[seen_starts[i]:seen_starts[i + 1]],
+       starts int64 [nq + 1], both on the GPU) c > 0 times becomes worse: a
+       positive score is divided by `repetition`, another one is multiplied by
+       it, and presence + frequency * c is taken off (with `largest` false, where
+       the smallest are best: multiplied, divided, added). The three are numbers,
+       or float32 tensors of one for each query.
+    2. `bias` is added: float32 [n], or [nq, n].
+    3. Where the query's filter has no bit the score is -infinity (with `largest`
+       false, infinity). `allow` holds filters as bits, int32 [filters, ceil(n /
+       32)] (or 1-D: one filter), vector j bit j % 32 of word j // 32;
+       `allow_rows` (int32 [nq]) is each query's filter, -1 for none. Without it
+       there is one filter, or one for each query.
+
+    `out`: a matrix to write, `scores` itself among them. Ids below 0 count for
+    nothing; nor do ids of n and more, and a query with a filter that is not there
+    may see nothing: `status` (or `take_status`) gets RAVEN_S_IDS. Histories whose
+    starts fall or leave `seen` count as empty: RAVEN_S_OFFSETS."""
+    ld = _scores_matrix(scores, "scores")
+    (nq, n), device = scores.shape, scores.get_device()
+    by = L.Adjustments()
+    if bias is not None:
+        if not isinstance(bias, torch.Tensor) or bias.dtype != torch.float32 or bias.shape not in ((n,), (nq, n)) or \
+                (n > 1 and bias.stride(-1) != 1) or (bias.dim() == 2 and nq > 1 and n > 0 and bias.stride(0) < n):
+            raise ValueError(f"bias must be a float32 tensor of {n} values, or {nq} x {n}, each row's side by side")
+        _on(device, bias)
+        by.bias, by.ld_bias = bias.data_ptr(), 0 if bias.dim() == 1 or nq == 1 else bias.stride(0)
+    words = -(-n // 32)
+    if allow is not None:
+        if not isinstance(allow, torch.Tensor) or allow.dtype != torch.int32 or allow.dim() not in (1, 2) or \
+                allow.shape[-1] < words or (words > 1 and allow.stride(-1) != 1) or \
+                (allow.dim() == 2 and allow.shape[0] > 1 and allow.stride(0) < words):
+            raise ValueError(f"allow must be an int32 tensor with {words} words for each filter, side by side")
+        _on(device, allow)
+        count = allow.shape[0] if allow.dim() == 2 else 1
+        if count == 0:
+            raise ValueError("allow holds no filter")
+        if allow_rows is None:
+            if count not in (1, nq):
+                raise ValueError(f"allow holds {count} filters: without allow_rows there must be one, or {nq}")
+        elif _ids("allow_rows", allow_rows, device) != nq:
+            raise ValueError(f"allow_rows must hold {nq} numbers of filters")
+        by.allow, by.allow_count = allow.data_ptr(), count
+        by.ld_allow, by.allow_rows = allow.stride(0) if count > 1 else words, _ptr(allow_rows)
+    elif allow_rows is not None:
+        raise ValueError("allow_rows without allow")
+    if (seen is None) != (seen_starts is None):
+        raise ValueError("seen and seen_starts come together")
+    if seen is not None:
+        by.seen_total = _ids("seen", seen, device)
+        if _offsets("seen_starts", seen_starts, device) != nq:
+            raise ValueError(f"seen_starts must hold {nq + 1} values")
+        by.seen, by.seen_starts = seen.data_ptr(), seen_starts.data_ptr()
+    by.repetition, by.repetition_all = _per_query("repetition", repetition, nq, device)
+    by.presence, by.presence_all = _per_query("presence", presence, nq, device)
+    by.frequency, by.frequency_all = _per_query("frequency", frequency, nq, device)
+    if by.repetition is None and not by.repetition_all > 0.0:
+        raise ValueError("repetition must be above 0")
+    if out is None:
+        out = torch.empty((nq, n), dtype=scores.dtype, device=scores.device)
+        ld_out = n
+    else:
+        ld_out = _scores_matrix(out, "out")
+        if out.shape != (nq, n) or out.dtype != scores.dtype:
+            raise ValueError(f"out must be a {scores.dtype} matrix of {nq} x {n}")
+        _on(device, out)
+    _call(device, L.load().raven_adjust_scores_device, scores.data_ptr(), _TYPES[scores.dtype], nq, n, ld, by, int(largest),
+          out.data_ptr(), ld_out, _status(status, device))
+    return out
 
 
 def top_k(scores: torch.Tensor, k: int, *, largest: bool = True,
