@@ -255,68 +255,4 @@ __global__ void __launch_bounds__(256) read_kernel(const Read p) {
   }
 }
 
-// ---------------------------------------------------------------------------
-// Scores of queries against 4-bit rows:
-//   S[i, j] = alpha * sum_g step_jg (sum_k code_jk q_ik + z_jg sum_k q_ik) + bias[j]
-// ---------------------------------------------------------------------------
-struct Scores {
-  const void* q;
-  int q_type;  // 0 f32, 1 f16, 2 bf16
-  uint64_t nq, ld_q;
-  const uint8_t* codes;
-  const uint32_t* words;
-  uint64_t n, ld_codes, ld_words;
-  uint32_t dim, group, units;
-  float alpha;
-  const float* bias;
-  void* out;
-  int out_type;
-  uint64_t ld;
-};
-
-template <typename T>
-__device__ inline float value_at(const void* x, uint64_t i) {
-  return raven_fp8::load_value((const T*)x + i);
-}
-__device__ inline void put(void* out, int type, uint64_t i, float v) {
-  if (type == 0)
-    ((float*)out)[i] = v;
-  else if (type == 1)
-    ((__half*)out)[i] = __float2half_rn(v);
-  else
-    ((__nv_bfloat16*)out)[i] = __float2bfloat16_rn(v);
-}
-
-// A warp takes a row and up to eight queries; lanes take words.
-template <typename T>
-__global__ void __launch_bounds__(256) scores_kernel(const Scores p) {
-  constexpr int NQ = 8;
-  after_previous();
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t chunks = (p.nq + NQ - 1) / NQ, total = p.n * chunks;
-  for (uint64_t u = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / 32; u < total; u += (uint64_t)gridDim.x * 8) {
-    const uint64_t j = u / chunks, q0 = (u - j * chunks) * NQ;
-    float sum[NQ] = {};
-    for (uint32_t i = lane; 8 * i < p.dim; i += 32) {
-      const uint32_t w = p.words[j * p.ld_words + 8 * i / p.group];
-      const uint32_t word = *(const uint32_t*)(p.codes + j * p.ld_codes + 4 * word_at(i, p.units));
-      const float step = step_of(w), z = zero_of(w);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (8 * i + k >= p.dim) break;
-        const float v = ((float)((word >> (4 * k)) & 15u) + z) * step;
-        for (int q = 0; q < NQ; ++q)
-          if (q0 + q < p.nq) {
-            const float x = value_at<T>(p.q, (q0 + q) * p.ld_q + 8 * i + k);
-            sum[q] = fmaf(v, x, fmaf(x, 0.f, sum[q]));  // NaN for an infinity too
-          }
-      }
-    }
-    for (int q = 0; q < NQ; ++q) {
-      for (int o = 16; o > 0; o >>= 1) sum[q] += __shfl_xor_sync(0xffffffffu, sum[q], o);
-      if (lane == 0 && q0 + q < p.nq) put(p.out, p.out_type, (q0 + q) * p.ld + j, p.alpha * sum[q] + (p.bias ? p.bias[j] : 0.f));
-    }
-  }
-}
-
 }  // namespace raven_int4

@@ -76,6 +76,8 @@ inline int sm_count(int* out) {
 // when a launch is refused (a context replaced since).
 struct Allowed {
   std::atomic<uint64_t> mask{0};
+  const uint32_t most;  // of a kernel whose launches differ in size: the largest
+  explicit Allowed(uint32_t m = 0) : most(m) {}
 };
 template <typename... K, typename... A>
 cudaError_t launch(void (*kern)(K...), uint64_t grid, int threads, uint32_t smem, Allowed& allowed, cudaStream_t st,
@@ -97,7 +99,8 @@ cudaError_t launch(void (*kern)(K...), uint64_t grid, int threads, uint32_t smem
   for (int turn = 0;; ++turn) {
     if (smem > 48 * 1024 && (turn || dev >= 64 || !(allowed.mask.load(std::memory_order_relaxed) & bit))) {
       Apart apart;
-      e = cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      e = cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)(smem > allowed.most ? smem : allowed.most));
       if (e != cudaSuccess) return e;
       allowed.mask.fetch_or(bit, std::memory_order_relaxed);
     }

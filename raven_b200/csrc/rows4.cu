@@ -12,6 +12,7 @@
 #include "status.cuh"
 #include "adjust.cuh"
 #include "int4.cuh"
+#include "score4.cuh"
 
 using namespace raven_launch;
 
@@ -105,6 +106,65 @@ cudaError_t launch_read(const raven_int4::Read& p, int sms, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------------------
+// Scores.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kMostShared = 227 * 1024;
+constexpr uint64_t kOwnLayout = 16384;  // values that each CTA lays out for itself
+
+template <int NT, int PARTS, int G, bool HELD, typename O>
+cudaError_t launch_score4(const raven_score4::Params& p, int sms, cudaStream_t st) {
+  using namespace raven_score4;
+  const uint64_t smem = Smem<NT, PARTS, G, HELD>::bytes(p.units, p.groups, p.split);
+  const uint64_t resident = (uint64_t)sms * (NT == 1 ? std::max<uint64_t>(1, std::min<uint64_t>(2, kMostShared / smem)) : 1);
+  const uint64_t columns = std::max<uint64_t>(1, std::min<uint64_t>(p.tiles, resident / p.chunks));
+  static Allowed allowed(kMostShared);
+  return launch(score4_kernel<NT, PARTS, G, HELD, O>, columns * p.chunks, kThreads, (uint32_t)smem, allowed, st, p);
+}
+
+template <int NT, int PARTS, int G>
+cudaError_t run_score4(raven_score4::Params p, int sms, cudaStream_t st) {
+  using namespace raven_score4;
+  using Q = Laid<NT, PARTS>;
+  p.chunks = (uint32_t)((p.nq + NT * 8 - 1) / (NT * 8));
+  // rows of a CTA's tile: as many as leave every SM one
+  p.split = 1;
+  while (p.split < kWarps && 2 * p.split <= p.blocks && p.n * p.chunks < (uint64_t)sms * 2 * kRows * (kWarps / p.split)) p.split *= 2;
+  const uint64_t rows = kRows * (kWarps / p.split);
+  p.tiles = (p.n + rows - 1) / rows;
+  const bool held = Smem<NT, PARTS, G, true>::bytes(p.units, p.groups, p.split) <= kMostShared;
+  uint8_t* laid = nullptr;
+  cudaError_t e = cudaSuccess;
+  if (!held || (uint64_t)NT * 8 * p.dim > kOwnLayout) {
+    if ((e = cudaMallocAsync((void**)&laid, p.chunks * Q::bytes(p.units, p.groups), st)) != cudaSuccess) return e;
+    static Allowed none;
+    e = launch(lay_out_kernel<NT, PARTS, G>, ((uint64_t)p.chunks * NT * 8 + kWarps - 1) / kWarps, kThreads, 0, none, st, p,
+               laid);
+    p.q = nullptr;
+    p.laid = laid;
+  }
+  auto go = [&](auto o) {
+    using O = decltype(o);
+    return held ? launch_score4<NT, PARTS, G, true, O>(p, sms, st) : launch_score4<NT, PARTS, G, false, O>(p, sms, st);
+  };
+  if (e == cudaSuccess) e = p.out_type == 0 ? go(float()) : p.out_type == 1 ? go(__half()) : go(__nv_bfloat16());
+  if (laid) cudaFreeAsync(laid, st);
+  return e;
+}
+
+template <int NT, int PARTS>
+cudaError_t group_score4(const raven_score4::Params& p, uint32_t group, int sms, cudaStream_t st) {
+  return group == 32   ? run_score4<NT, PARTS, 32>(p, sms, st)
+         : group == 64 ? run_score4<NT, PARTS, 64>(p, sms, st)
+                       : run_score4<NT, PARTS, 128>(p, sms, st);
+}
+
+cudaError_t dispatch_score4(const raven_score4::Params& p, uint32_t group, int sms, cudaStream_t st) {
+  if (p.q_type == 0)
+    return p.nq <= 8 ? group_score4<1, 2>(p, group, sms, st) : group_score4<4, 2>(p, group, sms, st);
+  return p.nq <= 8 ? group_score4<1, 1>(p, group, sms, st) : group_score4<4, 1>(p, group, sms, st);
+}
+
+// ---------------------------------------------------------------------------
 // Adjusted scores.
 // ---------------------------------------------------------------------------
 template <typename T>
@@ -152,7 +212,7 @@ int int4_scores(const raven_rows* q, const raven_rows* v, uint32_t dim, float al
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
-  raven_int4::Scores p{};
+  raven_score4::Params p{};
   p.q = q->data;
   p.q_type = kind_of(q->type);
   p.nq = q->rows;
@@ -163,19 +223,17 @@ int int4_scores(const raven_rows* q, const raven_rows* v, uint32_t dim, float al
   p.ld_codes = v->ld;
   p.ld_words = v->ld_exps;
   p.dim = dim;
-  p.group = int4_group(v->type);
   p.units = (dim + 31) / 32;
+  p.blocks = (dim + raven_int4::kBlock - 1) / raven_int4::kBlock;
+  const uint32_t group = int4_group(v->type);
+  p.groups = (dim + group - 1) / group;
   p.alpha = alpha;
   p.bias = bias;
   p.out = out;
   p.out_type = kind_of(out_type);
   p.ld = ld;
-  static Allowed none;
-  const uint64_t grid = std::min<uint64_t>((p.n * ((p.nq + 7) / 8) + 7) / 8, (uint64_t)sms * 64);
-  CU(launch(q->type == RAVEN_TYPE_F32   ? raven_int4::scores_kernel<float>
-            : q->type == RAVEN_TYPE_F16 ? raven_int4::scores_kernel<__half>
-                                        : raven_int4::scores_kernel<__nv_bfloat16>,
-            grid, 256, 0, none, st, p));
+  p.whole = aligned(out, 4 * type_size(out_type)) && (ld % 4 == 0 || p.nq == 1);
+  CU(dispatch_score4(p, group, sms, st));
   return RAVEN_OK;
 }
 
