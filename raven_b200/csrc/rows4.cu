@@ -111,57 +111,85 @@ cudaError_t launch_read(const raven_int4::Read& p, int sms, cudaStream_t st) {
 constexpr uint32_t kMostShared = 227 * 1024;
 constexpr uint64_t kOwnLayout = 16384;  // values that each CTA lays out for itself
 
-template <int NT, int PARTS, int G, bool HELD, typename O>
-cudaError_t launch_score4(const raven_score4::Params& p, int sms, cudaStream_t st) {
+template <int NT, int G, bool F32, bool HELD, typename O>
+cudaError_t launch_score4(const CUtensorMap& map, const raven_score4::Params& p, uint64_t ctas, cudaStream_t st) {
   using namespace raven_score4;
-  const uint64_t smem = Smem<NT, PARTS, G, HELD>::bytes(p.units, p.groups, p.split);
-  const uint64_t resident = (uint64_t)sms * (NT == 1 ? std::max<uint64_t>(1, std::min<uint64_t>(2, kMostShared / smem)) : 1);
-  const uint64_t columns = std::max<uint64_t>(1, std::min<uint64_t>(p.tiles, resident / p.chunks));
+  using L = Layout<NT, G>;
   static Allowed allowed(kMostShared);
-  return launch(score4_kernel<NT, PARTS, G, HELD, O>, columns * p.chunks, kThreads, (uint32_t)smem, allowed, st, p);
+  return launch(score4_kernel<NT, G, F32, HELD, O>, ctas, L::kThreads,
+                (uint32_t)L::bytes(p.units, p.groups, p.split, p.depth, HELD), allowed, st, map, p);
 }
 
-template <int NT, int PARTS, int G>
-cudaError_t run_score4(raven_score4::Params p, int sms, cudaStream_t st) {
+template <int NT, int G, bool F32>
+cudaError_t run_score4(const CUtensorMap& map, raven_score4::Params p, int out_type, int sms, cudaStream_t st) {
   using namespace raven_score4;
-  using Q = Laid<NT, PARTS>;
-  p.chunks = (uint32_t)((p.nq + NT * 8 - 1) / (NT * 8));
-  // rows of a CTA's tile: as many as leave every SM one
-  p.split = 1;
-  while (p.split < kWarps && 2 * p.split <= p.blocks && p.n * p.chunks < (uint64_t)sms * 2 * kRows * (kWarps / p.split)) p.split *= 2;
-  const uint64_t rows = kRows * (kWarps / p.split);
-  p.tiles = (p.n + rows - 1) / rows;
-  const bool held = Smem<NT, PARTS, G, true>::bytes(p.units, p.groups, p.split) <= kMostShared;
+  using L = Layout<NT, G>;
+  using Q = Laid<NT>;
+  constexpr uint32_t kQueries = F32 ? NT * 4 : NT * 8;
+  p.chunks = (uint32_t)((p.nq + kQueries - 1) / kQueries);
+  const uint64_t columns = std::max<uint64_t>(1, (uint64_t)sms / p.chunks);  // CTAs of a chunk
+  // Warps that share a row: as few as keep them evenly busy. In blocks of 128 values, what the busiest warp takes,
+  // with a block's time for sums that meet.
+  uint64_t best = ~0ull;
+  for (uint32_t split = 1; split <= L::kWarps && split <= p.blocks; split *= 2) {
+    const uint64_t rows = kRows * (L::kWarps / split), tiles = (p.n + rows - 1) / rows;
+    const uint64_t time = (tiles + columns - 1) / columns * ((p.blocks + split - 1) / split + (split > 1 ? 1 : 0));
+    if (time < best) {
+      best = time;
+      p.split = split;
+      p.tiles = tiles;
+    }
+  }
+  // three tiles under way at least, beside the queries
+  const bool held = L::bytes(p.units, p.groups, p.split, 3, true) <= kMostShared;
+  p.depth = kMaxDepth;
+  while (L::bytes(p.units, p.groups, p.split, p.depth, held) > kMostShared) --p.depth;
   uint8_t* laid = nullptr;
   cudaError_t e = cudaSuccess;
-  if (!held || (uint64_t)NT * 8 * p.dim > kOwnLayout) {
+  if (!held || (uint64_t)kQueries * p.dim > kOwnLayout) {
     if ((e = cudaMallocAsync((void**)&laid, p.chunks * Q::bytes(p.units, p.groups), st)) != cudaSuccess) return e;
     static Allowed none;
-    e = launch(lay_out_kernel<NT, PARTS, G>, ((uint64_t)p.chunks * NT * 8 + kWarps - 1) / kWarps, kThreads, 0, none, st, p,
-               laid);
+    e = launch(lay_out_kernel<NT, G, F32>, (uint64_t)p.chunks * kQueries, 256, 0, none, st, p, laid);
     p.q = nullptr;
     p.laid = laid;
   }
+  const uint64_t ctas = std::min(columns, p.tiles) * p.chunks;
   auto go = [&](auto o) {
     using O = decltype(o);
-    return held ? launch_score4<NT, PARTS, G, true, O>(p, sms, st) : launch_score4<NT, PARTS, G, false, O>(p, sms, st);
+    return held ? launch_score4<NT, G, F32, true, O>(map, p, ctas, st) : launch_score4<NT, G, F32, false, O>(map, p, ctas, st);
   };
-  if (e == cudaSuccess) e = p.out_type == 0 ? go(float()) : p.out_type == 1 ? go(__half()) : go(__nv_bfloat16());
+  if (e == cudaSuccess) e = out_type == 0 ? go(float()) : out_type == 1 ? go(__half()) : go(__nv_bfloat16());
   if (laid) cudaFreeAsync(laid, st);
   return e;
 }
 
-template <int NT, int PARTS>
-cudaError_t group_score4(const raven_score4::Params& p, uint32_t group, int sms, cudaStream_t st) {
-  return group == 32   ? run_score4<NT, PARTS, 32>(p, sms, st)
-         : group == 64 ? run_score4<NT, PARTS, 64>(p, sms, st)
-                       : run_score4<NT, PARTS, 128>(p, sms, st);
+template <int NT, bool F32>
+cudaError_t group_score4(const CUtensorMap& map, const raven_score4::Params& p, uint32_t group, int out_type, int sms,
+                         cudaStream_t st) {
+  return group == 32   ? run_score4<NT, 32, F32>(map, p, out_type, sms, st)
+         : group == 64 ? run_score4<NT, 64, F32>(map, p, out_type, sms, st)
+                       : run_score4<NT, 128, F32>(map, p, out_type, sms, st);
 }
 
-cudaError_t dispatch_score4(const raven_score4::Params& p, uint32_t group, int sms, cudaStream_t st) {
-  if (p.q_type == 0)
-    return p.nq <= 8 ? group_score4<1, 2>(p, group, sms, st) : group_score4<4, 2>(p, group, sms, st);
-  return p.nq <= 8 ? group_score4<1, 1>(p, group, sms, st) : group_score4<4, 1>(p, group, sms, st);
+template <bool F32>
+cudaError_t dispatch_score4(const CUtensorMap& map, const raven_score4::Params& p, uint32_t group, int out_type, int sms,
+                            cudaStream_t st) {
+  const uint64_t columns = F32 ? 2 * p.nq : p.nq;
+  return columns <= 8    ? group_score4<1, F32>(map, p, group, out_type, sms, st)
+         : columns <= 16 ? group_score4<2, F32>(map, p, group, out_type, sms, st)
+                         : group_score4<4, F32>(map, p, group, out_type, sms, st);
+}
+
+// Codes as boxes of up to 64 bytes (a block) x a warp's rows; what is past a row's end or the last row reads 0.
+bool codes_map(CUtensorMap* m, const raven_rows* v, uint32_t units) {
+  PFN_cuTensorMapEncodeTiled_v12000 f = raven_internal::encode_tiled();
+  if (!f) return false;
+  cuuint64_t gdim[2] = {16ull * units, v->rows};
+  cuuint64_t gstride[1] = {v->ld};
+  cuuint32_t box[2] = {std::min(64u, 16 * units), raven_score4::kRows};
+  cuuint32_t es[2] = {1, 1};
+  return f(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)v->data, gdim, gstride, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // ---------------------------------------------------------------------------
@@ -217,10 +245,9 @@ int int4_scores(const raven_rows* q, const raven_rows* v, uint32_t dim, float al
   p.q_type = kind_of(q->type);
   p.nq = q->rows;
   p.ld_q = q->ld;
-  p.codes = (const uint8_t*)v->data;
+  p.whole_q = aligned(q->data, 16) && (q->ld * type_size(q->type) % 16 == 0 || p.nq == 1);
   p.words = (const uint32_t*)v->exps;
   p.n = v->rows;
-  p.ld_codes = v->ld;
   p.ld_words = v->ld_exps;
   p.dim = dim;
   p.units = (dim + 31) / 32;
@@ -230,10 +257,13 @@ int int4_scores(const raven_rows* q, const raven_rows* v, uint32_t dim, float al
   p.alpha = alpha;
   p.bias = bias;
   p.out = out;
-  p.out_type = kind_of(out_type);
   p.ld = ld;
   p.whole = aligned(out, 4 * type_size(out_type)) && (ld % 4 == 0 || p.nq == 1);
-  CU(dispatch_score4(p, group, sms, st));
+  p.status = status;
+  CUtensorMap map;
+  if (!codes_map(&map, v, p.units)) return fail(RAVEN_ECUDA, "scores: no tensor map of the vectors");
+  CU(q->type == RAVEN_TYPE_F32 ? dispatch_score4<true>(map, p, group, kind_of(out_type), sms, st)
+                               : dispatch_score4<false>(map, p, group, kind_of(out_type), sms, st));
   return RAVEN_OK;
 }
 

@@ -17,13 +17,16 @@
 // z * sum(q), and its step is applied in f32 when the group ends: the scale is
 // never rounded into an operand.
 //
-// What bounds it: reading the codes. Each warp has its own ring of copies to shared
-// memory (cp.async) for tiles of 32 rows x 128 values (2 KB); a lane reads back
-// what it copied, so only the scale words, which the lanes of a row share, need
-// the warp to meet. Few rows of many values are split over K between the warps of
-// a CTA, which add up in a fixed order.
+// Two parts of an f32 query are two columns of the N side, added up at the end.
+//
+// What bounds it: reading the codes. Each warp has its own ring of tiles of 32 rows
+// x 128 values in shared memory: one TMA copy of 2 KB, and a copy of 4 to 16 bytes
+// a lane for the scale words. Where a CTA's tiles are few or large, warps share a
+// tile's rows and take its blocks of 128 values in turn; their sums meet in shared
+// memory and are added up in a fixed order.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -33,44 +36,51 @@
 #include "fp8.cuh"
 #include "int4.cuh"
 #include "internal.h"
+#include "knn_tc.cuh"
+#include "status.cuh"
 
 namespace raven_score4 {
 
 using raven_int4::kBlock;
 using raven_int4::kUnit;
 using raven_score::after_previous;
+using raven_tc::mbar_expect_tx;
+using raven_tc::mbar_init;
+using raven_tc::smem_u32;
+using raven_tc::tma_load_2d;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kMT = 2;                  // M tiles of a warp
-constexpr uint32_t kRows = 16 * kMT;    // rows of a warp's tile
-constexpr int kDepth = 4;               // tiles under way per warp
+constexpr int kMT = 2;                // M tiles of a warp
+constexpr uint32_t kRows = 16 * kMT;  // rows of a warp's tile
+constexpr uint32_t kMaxDepth = 6;     // tiles under way per warp, at most
 
 struct Params {
   const void* q;      // queries that each CTA lays out for itself, or null: `laid` holds them
   const uint8_t* laid;
   int q_type;         // 0 f32, 1 f16, 2 bf16
   uint64_t nq, ld_q;
-  const uint8_t* codes;
+  bool whole_q;       // 16 bytes of a query can be read at once
   const uint32_t* words;
-  uint64_t n, ld_codes, ld_words;
+  uint64_t n, ld_words;
   uint32_t dim, units, blocks, groups;  // of a row
-  uint32_t split;     // warps of a CTA that share a row's blocks
-  uint32_t chunks;    // of NT * 8 queries
+  uint32_t split;     // warps that share a row's blocks
+  uint32_t depth;     // of the rings
+  uint32_t chunks;    // of the queries
   uint64_t tiles;     // of a CTA's rows
   float alpha;
   const float* bias;
   void* out;
-  int out_type;
   uint64_t ld;
   bool whole;         // four scores of a query can be written at once
+  int* status;
 };
 
-// A chunk of queries as the kernel takes it: fragments (for each unit, N tile and
-// part 16 bytes a lane), then per group the sums of the queries' values, then per
-// query two powers of two whose product brings sums back.
-template <int NT, int PARTS>
+// A chunk of queries as the kernel takes it, NT * 8 columns: fragments (for each
+// unit and N tile 16 bytes a lane), then per group the columns' sums, then per
+// column two powers of two whose product brings sums back. f32 queries have two
+// columns side by side, the second for what the first leaves and without sums.
+template <int NT>
 struct Laid {
-  static constexpr uint32_t kUnitBytes = NT * PARTS * 512;
+  static constexpr uint32_t kUnitBytes = NT * 512;
   __host__ __device__ static uint64_t frags(uint32_t units) { return (uint64_t)units * kUnitBytes; }
   __host__ __device__ static uint64_t sums(uint32_t groups) { return (uint64_t)groups * NT * 8 * 4; }
   __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t groups) {
@@ -80,90 +90,140 @@ struct Laid {
 
 __device__ inline float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
 
-// Column `col` of a chunk from query `x` (null: none, zeros), by one warp.
-template <int NT, int PARTS, int G, typename T>
-__device__ inline void lay_out(const T* x, uint32_t dim, uint32_t units, uint32_t groups, uint32_t col, uint8_t* to) {
-  const uint32_t lane = threadIdx.x & 31;
-  float* sums = (float*)(to + Laid<NT, PARTS>::frags(units));
-  float* back = sums + groups * NT * 8;
-  uint32_t top = 0;
-  if (x)
-    for (uint32_t d = lane; d < dim; d += 32) top = max(top, __float_as_uint(raven_fp8::load_value(x + d)) & 0x7fffffffu);
+template <typename T>
+__device__ inline void eight(const T* x, uint32_t d, uint32_t dim, bool whole, float (&v)[8]) {
+  if (whole && d + 8 <= dim) {
+    __align__(16) T raw[8];
+    ((uint4*)raw)[0] = *(const uint4*)(x + d);
+    if constexpr (sizeof(T) == 4) ((uint4*)raw)[1] = *(const uint4*)(x + d + 4);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const bool bad = top >= 0x7f800000u;
-  const int e = top == 0 || bad ? 14 : 14 - (ilogbf(__uint_as_float(top)));  // -113 .. 163
-  const float m0 = pow2(e / 2), m1 = pow2(e - e / 2);
-  const bool none = x == nullptr || bad;
+    for (int k = 0; k < 8; ++k) v[k] = raven_fp8::load_value(raw + k);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = d + k < dim ? raven_fp8::load_value(x + d + k) : 0.f;
+  }
+}
+
+// Queries [first, first + count) as columns from `col` on, by all of a CTA's
+// threads. top: `count` words of shared memory.
+template <int NT, int G, typename T>
+__device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, uint32_t col, uint8_t* to, uint32_t* top) {
+  constexpr bool F32 = std::is_same<T, float>::value;
   constexpr uint32_t L = G / 8;
-  const uint32_t n8 = (units * 4 + L - 1) / L * L;  // eights, up to whole groups
-  for (uint32_t i0 = 0; i0 < n8; i0 += 32) {
-    const uint32_t i = i0 + lane;
+  float* sums = (float*)(to + Laid<NT>::frags(p.units));
+  float* back = sums + p.groups * NT * 8;
+  const uint32_t n8 = (p.units * 4 + L - 1) / L * L;  // eights, up to whole groups
+  const uint32_t items = count * n8;
+  auto load = [&](uint32_t q, uint32_t i, float(&v)[8]) {
+    if (first + q < p.nq) {
+      eight((const T*)p.q + (first + q) * p.ld_q, 8 * i, p.dim, p.whole_q, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = 0.f;
+    }
+  };
+  for (uint32_t i = threadIdx.x; i < count; i += blockDim.x) top[i] = 0;
+  __syncthreads();
+  for (uint32_t u = threadIdx.x; u < items; u += blockDim.x) {
+    const uint32_t q = u / n8;
+    float v[8];
+    load(q, u - q * n8, v);
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
+    atomicMax(&top[q], m);
+  }
+  __syncthreads();
+  for (uint32_t u0 = 0; u0 < items; u0 += blockDim.x) {
+    const uint32_t u = u0 + threadIdx.x, q = min(u / n8, count - 1), i = u - q * n8;  // past the last item: past the last unit
+    const bool bad = top[q] >= 0x7f800000u;
+    const int e = top[q] == 0 || bad ? 14 : 14 - ilogbf(__uint_as_float(top[q]));  // -113 .. 163
+    const float m0 = pow2(e / 2), m1 = pow2(e - e / 2);
     float v[8], sum = 0.f;
+    load(q, i, v);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const uint32_t d = 8 * i + k;
-      v[k] = !none && d < dim ? raven_fp8::load_value(x + d) * m0 * m1 : 0.f;
+      v[k] = bad ? 0.f : v[k] * m0 * m1;
       sum += v[k];
     }
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (i % L == 0 && i / L < groups) sums[i / L * (NT * 8) + col] = sum * 0x1p-24f;
-    if (i < units * 4) {
-      const uint32_t unit = i >> 2, at = (unit * NT + col / 8) * PARTS * 512 + ((col & 7) * 4 + (i & 3)) * 16;
-      __align__(16) __half part[PARTS][8];
+    const uint32_t c = col + (F32 ? 2 * q : q);
+    if (i % L == 0 && i / L < p.groups) {
+      sums[i / L * (NT * 8) + c] = sum * 0x1p-24f;
+      if (F32) sums[i / L * (NT * 8) + c + 1] = 0.f;
+    }
+    if (i < p.units * 4) {
+      __align__(16) __half part[F32 ? 2 : 1][8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float w = k & 1 ? v[k] * 0.0625f : v[k];
         const int s = (k & 3) * 2 + (k >> 2);
         part[0][s] = __float2half_rn(w);
-        if constexpr (PARTS == 2) part[1][s] = __float2half_rn(w - __half2float(part[0][s]));
+        if constexpr (F32) part[1][s] = __float2half_rn(w - __half2float(part[0][s]));
       }
 #pragma unroll
-      for (int p = 0; p < PARTS; ++p) *(uint4*)(to + at + p * 512) = *(const uint4*)part[p];
+      for (int h = 0; h < (F32 ? 2 : 1); ++h)
+        *(uint4*)(to + ((i >> 2) * NT + (c + h) / 8) * 512 + (((c + h) & 7) * 4 + (i & 3)) * 16) = *(const uint4*)part[h];
+    }
+    if (i == 0) {
+      const int b = 24 - e;  // -139 .. 137
+#pragma unroll
+      for (int h = 0; h < (F32 ? 2 : 1); ++h) {
+        back[2 * (c + h)] = bad ? __uint_as_float(0x7fc00000u) : pow2(b / 2);
+        back[2 * (c + h) + 1] = pow2(b - b / 2);
+      }
     }
   }
-  if (lane == 0) {
-    const int b = 24 - e;  // -139 .. 137
-    back[2 * col] = bad ? __uint_as_float(0x7fc00000u) : pow2(b / 2);
-    back[2 * col + 1] = pow2(b - b / 2);
-  }
 }
 
-template <int NT, int PARTS, int G>
-__device__ inline void lay_out_any(const Params& p, uint64_t query, uint32_t col, uint8_t* to) {
-  const bool there = query < p.nq;
-  const uint64_t at = query * p.ld_q;
-  if (p.q_type == 0)
-    lay_out<NT, PARTS, G>(there ? (const float*)p.q + at : nullptr, p.dim, p.units, p.groups, col, to);
+template <int NT, int G, bool F32>
+__device__ inline void lay_out_any(const Params& p, uint64_t first, uint32_t count, uint32_t col, uint8_t* to, uint32_t* top) {
+  if constexpr (F32)
+    lay_out<NT, G, float>(p, first, count, col, to, top);
   else if (p.q_type == 1)
-    lay_out<NT, PARTS, G>(there ? (const __half*)p.q + at : nullptr, p.dim, p.units, p.groups, col, to);
+    lay_out<NT, G, __half>(p, first, count, col, to, top);
   else
-    lay_out<NT, PARTS, G>(there ? (const __nv_bfloat16*)p.q + at : nullptr, p.dim, p.units, p.groups, col, to);
+    lay_out<NT, G, __nv_bfloat16>(p, first, count, col, to, top);
 }
 
-// All chunks, a warp per column.
-template <int NT, int PARTS, int G>
-__global__ void __launch_bounds__(kThreads) lay_out_kernel(const Params p, uint8_t* to) {
+// All chunks, a CTA per query.
+template <int NT, int G, bool F32>
+__global__ void __launch_bounds__(256) lay_out_kernel(const Params p, uint8_t* to) {
+  constexpr uint32_t Q = F32 ? NT * 4 : NT * 8;
+  __shared__ uint32_t top[1];
   after_previous();
-  const uint64_t w = (uint64_t)blockIdx.x * kWarps + threadIdx.x / 32;
-  const uint64_t chunk = w / (NT * 8);
-  if (chunk >= p.chunks) return;
-  const uint32_t col = (uint32_t)(w - chunk * (NT * 8));
-  lay_out_any<NT, PARTS, G>(p, w, col, to + chunk * Laid<NT, PARTS>::bytes(p.units, p.groups));
+  const uint32_t chunk = blockIdx.x / Q, q = blockIdx.x - chunk * Q;
+  lay_out_any<NT, G, F32>(p, blockIdx.x, 1, F32 ? 2 * q : q, to + chunk * Laid<NT>::bytes(p.units, p.groups), top);
 }
 
 template <int B>
 __device__ inline void copy_async(uint32_t to, const void* from) {
-  if constexpr (B == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to), "l"(from) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(to), "l"(from), "n"(B) : "memory");
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(to), "l"(from), "n"(B) : "memory");
 }
-__device__ inline void copies_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int N>
-__device__ inline void copies_wait() {
-  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+// Arrives at the barrier when this thread's copies have landed.
+__device__ inline void copies_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(bar) : "memory");
+}
+// Waits for a phase of the barrier; false after about two seconds.
+__device__ inline bool wait(uint32_t bar, uint32_t parity) {
+  auto done = [&]() {
+    uint32_t d;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(d)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return d != 0;
+  };
+  if (done()) return true;
+  const long long t0 = clock64();
+  while (clock64() - t0 < raven_tc::kWaitCycles)
+    if (done()) return true;
+  return false;
+}
+__device__ inline void meet(uint32_t id, uint32_t threads) {
+  asm volatile("bar.sync %0, %1;\n" ::"r"(id), "r"(threads) : "memory");
 }
 
 __device__ inline void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -173,14 +233,19 @@ __device__ inline void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int NT, int PARTS, int G, bool HELD>
-struct Smem {
-  static constexpr uint32_t kWords = kBlock / G;                          // scale words of a row's block
-  static constexpr uint32_t kStage = kMT * 2 * 512 + kRows * kWords * 4;  // codes, 16 bytes a lane and row; words by row
-  static constexpr uint32_t kRing = kWarps * kDepth * kStage;
-  static constexpr uint32_t kPart = 32 * 4 * kMT * NT * 4;                // a warp's sums
-  __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t groups, uint32_t split) {
-    return kRing + (split > 1 ? kWarps * kPart : kWarps * 32 * 9 * 4) + (HELD ? Laid<NT, PARTS>::bytes(units, groups) : 0);
+template <int NT, int G>
+struct Layout {
+  static constexpr uint32_t kWarps = NT <= 2 ? 16 : 8;    // as many as their registers allow
+  static constexpr uint32_t kThreads = kWarps * 32;
+  static constexpr uint32_t kWords = kBlock / G;          // scale words of a row's block
+  static constexpr uint32_t kCodeBytes = kRows * 64, kWordBytes = kRows * kWords * 4;
+  static constexpr uint32_t kPart = 32 * 4 * kMT * NT * 4;  // a warp's sums
+  static constexpr uint32_t kBars = kWarps * kMaxDepth * 8;  // in front of the rings
+  static constexpr uint32_t kTops = NT * 8 * 4;
+  __host__ __device__ static uint64_t ring(uint32_t depth) { return (uint64_t)kWarps * depth * (kCodeBytes + kWordBytes); }
+  __host__ __device__ static uint64_t shared(uint32_t split) { return split > 1 ? kWarps * kPart : 0; }
+  __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t groups, uint32_t split, uint32_t depth, bool held) {
+    return kBars + ring(depth) + kTops + shared(split) + (held ? Laid<NT>::bytes(units, groups) : 0);
   }
 };
 
@@ -195,63 +260,63 @@ __device__ inline T rounded(float v) {
 }
 
 // HELD: the chunk's queries are in shared memory; else read through L1.
-template <int NT, int PARTS, int G, bool HELD, typename O>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) score4_kernel(const Params p) {
-  using S = Smem<NT, PARTS, G, HELD>;
-  using Q = Laid<NT, PARTS>;
-  extern __shared__ __align__(16) uint8_t smem[];
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32, g = lane >> 2, t = lane & 3;
-  uint8_t* ring = smem + warp * kDepth * S::kStage;
-  float* scratch = (float*)(smem + S::kRing);
-  const uint32_t scratch_bytes = p.split > 1 ? kWarps * S::kPart : kWarps * 32 * 9 * 4;
-  uint8_t* held = smem + S::kRing + scratch_bytes;
-  const uint32_t kw = warp % p.split, wr = warp / p.split, across = kWarps / p.split;
-  const uint64_t chunk = blockIdx.x % p.chunks, step = gridDim.x / p.chunks;
-  const uint64_t first = blockIdx.x / p.chunks;
+template <int NT, int G, bool F32, bool HELD, typename O>
+__global__ void __launch_bounds__(Layout<NT, G>::kThreads, 1) score4_kernel(const __grid_constant__ CUtensorMap map,
+                                                                            const Params p) {
+  using S = Layout<NT, G>;
+  using Q = Laid<NT>;
+  constexpr uint32_t kQueries = F32 ? NT * 4 : NT * 8;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32, g = lane >> 2, t = lane & 3, odd = g & 1;
+  const uint32_t bars = smem_u32(smem) + warp * kMaxDepth * 8;
+  uint8_t* codes = smem + S::kBars + warp * p.depth * S::kCodeBytes;
+  uint8_t* words = smem + S::kBars + S::kWarps * p.depth * S::kCodeBytes + warp * p.depth * S::kWordBytes;
+  uint8_t* after = smem + S::kBars + S::ring(p.depth);
+  uint32_t* tops = (uint32_t*)after;
+  float* shared = (float*)(after + S::kTops);
+  uint8_t* held = after + S::kTops + S::shared(p.split);
+  const uint32_t kw = warp % p.split, wr = warp / p.split, across = S::kWarps / p.split;
+  const uint64_t chunk = blockIdx.x % p.chunks, step = gridDim.x / p.chunks, first = blockIdx.x / p.chunks;
+  const uint32_t pitch = min(64u, 16 * p.units);  // of a tile's rows of codes
+  if (lane < p.depth) mbar_init(bars + 8 * lane, 33);
+  asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  __syncwarp();
   after_previous();
 
   // the ring: what is copied next
   uint64_t ahead = first;
-  uint32_t ahead_b = kw, slot = 0;
-  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  uint32_t ahead_b = kw, slot = 0, pending = 0;
+  const uint32_t codes_at = smem_u32(codes), words_at = smem_u32(words);
   auto copy_next = [&]() {
     if (ahead < p.tiles) {
       const uint64_t row0 = (ahead * across + wr) * kRows;
-      const uint32_t at = ring_at + slot * S::kStage;
-      const uint32_t u = min(4u, p.units - 4 * ahead_b);
-#pragma unroll
-      for (int r = 0; r < 2 * kMT; ++r) {
-        const uint64_t row = min(row0 + g * (2 * kMT) + r, p.n - 1);
-        const uint8_t* from = p.codes + row * p.ld_codes + 64 * ahead_b + 4 * u * t;
-        const uint32_t to = at + r * 512 + lane * 16;
-        if (u == 4)
-          copy_async<16>(to, from);
-        else
-          for (uint32_t w = 0; w < u; ++w) copy_async<4>(to + 4 * w, from + 4 * w);
-        if (t == (uint32_t)r % 4)
-          copy_async<4 * S::kWords>(at + kMT * 1024 + (g * 2 * kMT + r) * S::kWords * 4,
-                                    p.words + row * p.ld_words + ahead_b * S::kWords);
+      const uint32_t bar = bars + 8 * slot;
+      copy_async<4 * S::kWords>(words_at + slot * S::kWordBytes + lane * (4 * S::kWords),
+                                p.words + min(row0 + lane, p.n - 1) * p.ld_words + ahead_b * S::kWords);
+      copies_arrive(bar);
+      if (lane == 0) {
+        mbar_expect_tx(bar, kRows * pitch);
+        tma_load_2d(codes_at + slot * S::kCodeBytes, &map, (int)(64 * ahead_b), (int)min(row0, p.n), bar);
       }
+      pending |= 1u << slot;
+      slot = slot + 1 == p.depth ? 0 : slot + 1;
       ahead_b += p.split;
       if (ahead_b >= p.blocks) {
         ahead_b = kw;
         ahead += step;
       }
     }
-    copies_commit();
-    slot = slot + 1 == kDepth ? 0 : slot + 1;
   };
-#pragma unroll
-  for (int i = 0; i < kDepth - 1; ++i) copy_next();
+  for (uint32_t i = 0; i + 1 < p.depth; ++i) copy_next();
 
   const uint8_t* laid = held;
   if constexpr (HELD) {
     if (p.q) {
-      for (uint32_t col = warp; col < NT * 8; col += kWarps) lay_out_any<NT, PARTS, G>(p, chunk * NT * 8 + col, col, held);
+      lay_out_any<NT, G, F32>(p, chunk * kQueries, kQueries, 0, held, tops);
     } else {
-      const uint64_t bytes = Q::bytes(p.units, p.groups);
+      const uint32_t bytes = (uint32_t)Q::bytes(p.units, p.groups);
       const uint8_t* from = p.laid + chunk * bytes;
-      for (uint64_t i = threadIdx.x * 16; i < bytes; i += kThreads * 16) *(uint4*)(held + i) = *(const uint4*)(from + i);
+      for (uint32_t i = threadIdx.x * 16; i < bytes; i += S::kThreads * 16) *(uint4*)(held + i) = *(const uint4*)(from + i);
     }
     __syncthreads();
   } else {
@@ -260,20 +325,38 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) score4_kernel(const
   const float* sums = (const float*)(laid + Q::frags(p.units));
   const float* back = sums + p.groups * NT * 8;
 
-  uint32_t now = 0;  // the stage that is taken next
+  bool ok = true;  // no wait has run out
+  uint32_t now = 0, phases = 0;  // the stage that is taken next; parities of the stages
+  // row m * 16 + g (+ 8) of the fragments is row 8 (g / 2) + g % 2 + 4 m (+ 2) of the tile: two lanes next to one
+  // another in g read 128 bytes side by side
+  const uint32_t my_row = 8 * (g >> 1) + odd;
   for (uint64_t tile = first; tile < p.tiles; tile += step) {
     float total[kMT][NT][4] = {};
     for (uint32_t b = kw; b < p.blocks; b += p.split) {
-      copies_wait<kDepth - 2>();
+      if (ok && !__all_sync(0xffffffffu, wait(bars + 8 * now, phases >> now & 1u))) {
+        ok = false;
+        if (lane == 0) raven_score::tell(p.status, raven_score::kStatusWait);
+      }
+      if (!ok) continue;  // but meets the warps it shares rows with
       __syncwarp();
+      const uint8_t* stage = codes + now * S::kCodeBytes;
+      const uint32_t* word = (const uint32_t*)(words + now * S::kWordBytes) + my_row * S::kWords;
+      phases ^= 1u << now;
+      pending &= ~(1u << now);
+      now = now + 1 == p.depth ? 0 : now + 1;
       copy_next();  // into the stage that every lane is done with
-      const uint8_t* stage = ring + now * S::kStage;
-      now = now + 1 == kDepth ? 0 : now + 1;
-      uint4 code[kMT][2];
-#pragma unroll
-      for (int r = 0; r < 2 * kMT; ++r) code[r / 2][r % 2] = *(const uint4*)(stage + r * 512 + lane * 16);
-      const uint32_t* words = (const uint32_t*)(stage + kMT * 1024) + g * 2 * kMT * S::kWords;
       const uint32_t u = min(4u, p.units - 4 * b);
+      uint4 code[kMT][2];
+      if (u == 4) {
+#pragma unroll
+        for (int r = 0; r < 2 * kMT; ++r) code[r / 2][r % 2] = *(const uint4*)(stage + (my_row + 2 * r) * 64 + 16 * t);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 2 * kMT; ++r) {
+          const uint32_t* c = (const uint32_t*)(stage + (my_row + 2 * r) * pitch + 4 * u * t);
+          code[r / 2][r % 2] = make_uint4(c[0], u > 1 ? c[1] : 0, u > 2 ? c[2] : 0, 0);
+        }
+      }
 #pragma unroll
       for (uint32_t gi = 0; gi < S::kWords; ++gi) {
         constexpr uint32_t U = G / kUnit;
@@ -285,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) score4_kernel(const
             float z[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t w = words[(2 * m + h) * S::kWords + gi];
+              const uint32_t w = word[(4 * m + 2 * h) * S::kWords + gi];
               sc[m][h] = raven_int4::step_of(w);
               z[h] = raven_int4::zero_of(w);
             }
@@ -293,9 +376,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) score4_kernel(const
             for (int j = 0; j < NT; ++j) {
               const float2 x = *(const float2*)(gs + 8 * j);
               acc[m][j][0] = z[0] * x.x;
-              acc[m][j][1] = z[0] * x.y;
               acc[m][j][2] = z[1] * x.x;
-              acc[m][j][3] = z[1] * x.y;
+              acc[m][j][1] = F32 ? 0.f : z[0] * x.y;
+              acc[m][j][3] = F32 ? 0.f : z[1] * x.y;
             }
           }
 #pragma unroll
@@ -316,18 +399,16 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) score4_kernel(const
                   a[m][h][2] = (w >> 8) & 0x000f000fu;
                   a[m][h][3] = (w >> 8) & 0x00f000f0u;
                 }
-              const uint8_t* f = laid + (uint64_t)(4 * b + unit) * Q::kUnitBytes + lane * 16;
+              const uint8_t* f = laid + (4 * b + unit) * Q::kUnitBytes + lane * 16;
 #pragma unroll
-              for (int j = 0; j < NT; ++j)
+              for (int j = 0; j < NT; ++j) {
+                const uint4 x = *(const uint4*)(f + j * 512);
 #pragma unroll
-                for (int q = PARTS - 1; q >= 0; --q) {
-                  const uint4 x = *(const uint4*)(f + (j * PARTS + q) * 512);
-#pragma unroll
-                  for (int m = 0; m < kMT; ++m) {
-                    mma(acc[m][j], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], x.x, x.y);
-                    mma(acc[m][j], a[m][0][2], a[m][1][2], a[m][0][3], a[m][1][3], x.z, x.w);
-                  }
+                for (int m = 0; m < kMT; ++m) {
+                  mma(acc[m][j], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], x.x, x.y);
+                  mma(acc[m][j], a[m][0][2], a[m][1][2], a[m][0][3], a[m][1][3], x.z, x.w);
                 }
+              }
             }
           }
 #pragma unroll
@@ -339,52 +420,69 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1) score4_kernel(const
         }
       }
     }
-    // the warps that shared the rows add up, the first one's sums last
+    // The sums of a column (of two, F32) for this lane's four rows, from one warp after the other where several
+    // shared them; lanes next to one another in g swap two, so that each has four rows side by side.
+    const uint64_t row = (tile * across + wr) * kRows + 4 * g;
+    float* mine = shared + warp * (S::kPart / 4) + lane;
     if (p.split > 1) {
-      float* mine = scratch + warp * (S::kPart / 4) + lane;
-      if (kw > 0) {
 #pragma unroll
-        for (int i = 0; i < kMT * NT * 4; ++i) mine[32 * i] = ((const float*)total)[i];
-      }
-      __syncthreads();
-      if (kw == 0) {
-        for (uint32_t k = 1; k < p.split; ++k)
-#pragma unroll
-          for (int i = 0; i < kMT * NT * 4; ++i) ((float*)total)[i] += mine[k * (S::kPart / 4) + 32 * i];
-      }
-      __syncthreads();
-      if (kw > 0) continue;
+      for (int i = 0; i < kMT * NT * 4; ++i) mine[32 * i] = total[i / (4 * NT)][i / 4 % NT][i % 4];
+      meet(1 + wr, 32 * p.split);
     }
-    // row m * 16 + g (+ 8) of the fragments is row g * 4 + 2 m (+ 1) of the tile: a lane holds four rows side by side
-    const uint64_t row = (tile * across + wr) * kRows + g * (2 * kMT);
+    const float* theirs = shared + wr * p.split * (S::kPart / 4) + lane;
     float bias[2 * kMT];
 #pragma unroll
     for (int r = 0; r < 2 * kMT; ++r) bias[r] = p.bias && row + r < p.n ? p.bias[row + r] : 0.f;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint32_t col = 8 * j + 2 * t + c;
-        const uint64_t query = chunk * NT * 8 + col;
-        if (query >= p.nq) continue;
-        const float b0 = back[2 * col], b1 = back[2 * col + 1];
-        __align__(16) O v[2 * kMT];
+      for (int c = 0; c < (F32 ? 1 : 2); ++c) {
+        float v[2 * kMT];
+        if (p.split > 1) {
+          if ((j * (F32 ? 1 : 2) + c) % p.split != kw) continue;
 #pragma unroll
-        for (int r = 0; r < 2 * kMT; ++r) v[r] = rounded<O>(fmaf(p.alpha, total[r / 2][j][2 * (r % 2) + c] * b0 * b1, bias[r]));
-        O* to = (O*)p.out + query * p.ld + row;
-        if (p.whole && row + 2 * kMT <= p.n) {
-          if constexpr (sizeof(O) == 4)
-            *(uint4*)to = *(const uint4*)v;
-          else
-            *(uint2*)to = *(const uint2*)v;
+          for (int r = 0; r < 2 * kMT; ++r) v[r] = 0.f;
+          for (uint32_t k = 0; k < p.split; ++k) {
+            const float* from = theirs + k * (S::kPart / 4);
+#pragma unroll
+            for (int r = 0; r < 2 * kMT; ++r) {
+              const float* x = from + 32 * (((r / 2) * NT + j) * 4 + 2 * (r % 2) + c);
+              v[r] += F32 ? x[0] + x[32] : x[0];
+            }
+          }
         } else {
 #pragma unroll
           for (int r = 0; r < 2 * kMT; ++r)
-            if (row + r < p.n) to[r] = v[r];
+            v[r] = F32 ? total[r / 2][j][2 * (r % 2)] + total[r / 2][j][2 * (r % 2) + 1] : total[r / 2][j][2 * (r % 2) + c];
+        }
+        const float s0 = __shfl_xor_sync(0xffffffffu, odd ? v[0] : v[2], 4), s1 = __shfl_xor_sync(0xffffffffu, odd ? v[1] : v[3], 4);
+        const float y[4] = {odd ? s0 : v[0], odd ? v[2] : s0, odd ? s1 : v[1], odd ? v[3] : s1};
+        const uint32_t col = 8 * j + 2 * t + c;
+        const uint64_t query = chunk * kQueries + (F32 ? col / 2 : col);
+        if (query < p.nq) {
+          const float b0 = back[2 * col], b1 = back[2 * col + 1];
+          __align__(16) O o[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[r] = rounded<O>(fmaf(p.alpha, y[r] * b0 * b1, bias[r]));
+          O* to = (O*)p.out + query * p.ld + row;
+          if (p.whole && row + 4 <= p.n) {
+            if constexpr (sizeof(O) == 4)
+              *(uint4*)to = *(const uint4*)o;
+            else
+              *(uint2*)to = *(const uint2*)o;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (row + r < p.n) to[r] = o[r];
+          }
         }
       }
+    if (p.split > 1) meet(1 + wr, 32 * p.split);
   }
-  copies_wait<0>();
+  // a wait ran out: no copy is under way any more when the CTA ends
+  if (!ok)
+    for (uint32_t i = 0; i < p.depth; ++i)
+      if (pending >> i & 1u) wait(bars + 8 * i, phases >> i & 1u);
 }
 
 }  // namespace raven_score4
