@@ -44,7 +44,8 @@ __device__ inline uint32_t word_at(uint32_t i, uint32_t units) {
 }
 
 __device__ inline float step_of(uint32_t word) { return __uint_as_float(word & 0xffffff00u); }
-__device__ inline float zero_of(uint32_t word) { return (float)(int8_t)(word & 0xffu); }
+// z: as the low bits of an f32 of 2^23, offset by 128
+__device__ inline float zero_of(uint32_t word) { return __uint_as_float((word & 0xffu) ^ 0x4b000080u) - 8388736.f; }
 
 // ---------------------------------------------------------------------------
 // Slots named more than once: the last of their rows is the one that is held.
@@ -87,22 +88,55 @@ struct Write {
   const Claim* table;      // null: few rows
   uint32_t bits;
   uint32_t run;            // rows of a CTA at once
+  uint32_t per, magic;     // eights of a row, and what divides by them
   int* status;
 };
 
 constexpr uint32_t kRun = 64;  // most rows of a run
+constexpr int kItems = 4;      // eights of a lane at once
+
+// u / per for u * per < 2^32; magic: 2^32 / per rounded up, 0 for 1.
+__device__ inline uint32_t divided(uint32_t u, uint32_t magic) { return magic ? __umulhi(u, magic) : u; }
+
+// The step of a group of values from lo to hi, as bits: the least with 16
+// significant bits for which hi - lo <= 15 * step and the largest magnitude <=
+// 127 * step. That is (hi - lo) / 15 and m / 127 in 64 bits, rounded up: 15 * step
+// is exact there, and a difference above it by a unit in its last place has a
+// quotient above the step by more than half of one. 127 * step is exact in f32. From an
+// estimate a little below, at most three units of 16 bits too low.
+__device__ inline uint32_t step_bits(float lo, float hi) {
+  const float m = fmaxf(hi, -lo);
+  if (m == 0.f) return 0;
+  const double range = (double)hi - (double)lo;
+  const float near = fmaxf(__double2float_rn(range * (1.0 / 15.0)), m * (1.f / 127.f));
+  uint32_t bits = __float_as_uint(near * (1.f - 0x1p-20f)) & ~255u;
+  for (int i = 0; i < 4; ++i) {
+    const float s = __uint_as_float(bits);
+    if (range <= 15.0 * (double)s && m <= 127.f * s) break;
+    bits += 256;
+  }
+  return bits;
+}
+__device__ inline float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
 // A lane takes eight values (two 16-byte loads of f32, one of 16-bit types), the
-// group / 8 lanes of a group share its range by shuffles.
+// L = group / 8 lanes of a group share its range by shuffles, and of four such
+// pieces at once every group's word is worked out by a lane of its own (64-bit
+// arithmetic that 16 lanes did alike took as long as the reading).
 // VEC: pitch and address let 16 bytes be read at once. LANE: lane-major rows
 // (element e of the first 16C at (e % 16) * C + e / 16).
-template <typename T, bool VEC, bool LANE>
-__global__ void __launch_bounds__(256) write_kernel(const Write p) {
+template <typename T, uint32_t L, bool VEC, bool LANE>
+__global__ void __launch_bounds__(256, 3) write_kernel(const Write p) {
   __shared__ int32_t dest[kRun];
   __shared__ uint32_t later[kRun];
   after_previous();
-  const uint32_t lanes = p.group / 8, ng = (p.dim + p.group - 1) / p.group, per = ng * lanes;
-  const uint32_t wide = (p.dim + kBlock - 1) / kBlock * (kBlock / p.group);  // words of a row as it is held
+  constexpr uint32_t G = 8 * L, kGroups = 32 / L;  // groups of a warp's piece
+  const uint32_t ng = (p.dim + G - 1) / G, lane = threadIdx.x & 31;
+  const uint32_t wide = (p.dim + kBlock - 1) / kBlock * (kBlock / G);  // words of a row as it is held
   for (uint64_t r0 = (uint64_t)blockIdx.x * p.run; r0 < p.m; r0 += (uint64_t)gridDim.x * p.run) {
     const uint32_t rows = (uint32_t)min((uint64_t)p.run, p.m - r0);
     if (threadIdx.x < rows) {
@@ -129,69 +163,105 @@ __global__ void __launch_bounds__(256) write_kernel(const Write p) {
       }
       __syncthreads();
     }
-    const uint32_t items = rows * per;
-    for (uint32_t u0 = 0; u0 < items; u0 += 256) {
-      const uint32_t u = u0 + threadIdx.x, r = u / per, i = u - r * per, d = 8 * i;
-      const int64_t to = u < items && !later[r] ? dest[r] : -1;
-      float x[8];
-      uint32_t top = 0;
-      float lo = INFINITY, hi = -INFINITY;
-      if (to >= 0) {
-        const T* row = (const T*)p.x + (r0 + r) * p.ld;
-        if (VEC && d + 8 <= p.dim) {
-          __align__(16) T raw[8];
-          ((uint4*)raw)[0] = *(const uint4*)(row + d);
-          if constexpr (sizeof(T) == 4) ((uint4*)raw)[1] = *(const uint4*)(row + d + 4);
+    const uint32_t items = rows * p.per;
+    for (uint32_t u0 = 0; u0 < items; u0 += 256 * kItems) {
+      float x[kItems][8], lo[kItems], hi[kItems];
+      int32_t to[kItems];
+      uint32_t at[kItems];
+      bool odd[kItems];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] = raven_fp8::load_value(raw + k);
+      for (int n = 0; n < kItems; ++n) {
+        const uint32_t u = u0 + n * 256 + threadIdx.x, r = divided(u, p.magic), i = u - r * p.per, d = 8 * i;
+        to[n] = u < items && !later[r] ? dest[r] : -1;
+        at[n] = i;
+        if (to[n] >= 0) {
+          const T* row = (const T*)p.x + (r0 + r) * p.ld;
+          if (VEC && d + 8 <= p.dim) {
+            __align__(16) T raw[8];
+            ((uint4*)raw)[0] = *(const uint4*)(row + d);
+            if constexpr (sizeof(T) == 4) ((uint4*)raw)[1] = *(const uint4*)(row + d + 4);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[n][k] = raven_fp8::load_value(raw + k);
+          } else {
+            const uint32_t C = p.dim / 16;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              // past the row its last value again, which changes no range
+              const uint32_t e = min(d + k, p.dim - 1);
+              x[n][k] = raven_fp8::load_value(row + (LANE && e < 16 * C ? (e % 16) * C + e / 16 : e));
+            }
+          }
         } else {
-          const uint32_t C = p.dim / 16;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t e = d + k;
-            x[k] = e < p.dim ? raven_fp8::load_value(row + (LANE && e < 16 * C ? (e % 16) * C + e / 16 : e)) : 0.f;
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (d + k < p.dim) {
-            top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
-            lo = fminf(lo, x[k]);
-            hi = fmaxf(hi, x[k]);
-          }
-      }
-      for (uint32_t o = lanes / 2; o > 0; o >>= 1) {
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      }
-      if (to < 0) continue;
-      uint32_t word = 0, scale = kNaN;
-      if (top < 0x7f800000u) {
-        const double need = fmax(((double)hi - (double)lo) / 15.0, (double)fmaxf(hi, -lo) / 127.0);
-        const uint32_t bits = (__float_as_uint(__double2float_ru(need)) + 255u) & ~255u;
-        const float step = __uint_as_float(bits), inv = 1.f / step;
-        scale = bits;
-        if (bits) {
-          const int z = (int)rintf(__fdiv_rn(lo, step));
-          scale = bits | ((uint32_t)z & 255u);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            // x * inv is off by less than 2^-15 here: near a border the quotient itself decides. It is an
-            // f32 rounded once, and between a value and a border that differ at least half a unit of it lies.
-            const float q = x[k] * inv;
-            float t = rintf(q);
-            if (!(fabsf(q - t) < 0.5f - 0x1p-12f)) t = rintf(__fdiv_rn(x[k], step));
-            const int c = min(max((int)t - z, 0), 15);
-            word |= (d + k < p.dim ? (uint32_t)c : 0u) << (4 * k);
-          }
+          for (int k = 0; k < 8; ++k) x[n][k] = 0.f;
         }
       }
-      if (i < 4 * p.units) *(uint32_t*)(p.codes + to * p.ld_codes + 4 * word_at(i, p.units)) = word;
-      uint32_t* words = p.words + to * p.ld_words;
-      if (i % lanes == 0) words[i / lanes] = scale;
-      if (i == 0)
-        for (uint32_t g = ng; g < wide; ++g) words[g] = 0;
+#pragma unroll
+      for (int n = 0; n < kItems; ++n) {
+        uint32_t top = 0;
+        lo[n] = hi[n] = x[n][0];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          top = max(top, __float_as_uint(x[n][k]) & 0x7fffffffu);
+          lo[n] = fminf(lo[n], x[n][k]);
+          hi[n] = fmaxf(hi[n], x[n][k]);
+        }
+        const uint32_t votes = __ballot_sync(0xffffffffu, top >= 0x7f800000u);
+        odd[n] = votes >> (lane & ~(L - 1)) & ((1u << L) - 1);
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) {
+          lo[n] = fminf(lo[n], __shfl_xor_sync(0xffffffffu, lo[n], o));
+          hi[n] = fmaxf(hi[n], __shfl_xor_sync(0xffffffffu, hi[n], o));
+        }
+      }
+      // lane n * kGroups + g: group g of piece n
+      float glo = 0.f, ghi = 0.f;
+#pragma unroll
+      for (int n = 0; n < kItems; ++n) {
+        const float a = __shfl_sync(0xffffffffu, lo[n], lane % kGroups * L), b = __shfl_sync(0xffffffffu, hi[n], lane % kGroups * L);
+        if (lane / kGroups == n) {
+          glo = a;
+          ghi = b;
+        }
+      }
+      const uint32_t bits = step_bits(glo, ghi);
+      const uint32_t scale = bits ? bits | ((uint32_t)(int)rintf(__fdiv_rn(glo, __uint_as_float(bits))) & 255u) : 0u;
+#pragma unroll
+      for (int n = 0; n < kItems; ++n) {
+        uint32_t w = __shfl_sync(0xffffffffu, scale, n * kGroups + lane / L);
+        if (to[n] < 0) continue;
+        const uint32_t i = at[n], d = 8 * i;
+        uint32_t word = 0;
+        if (odd[n]) {
+          w = kNaN;
+        } else if (w & ~255u) {
+          const float step = step_of(w), inv = reciprocal(step);
+          const int z = (int)(int8_t)(w & 0xffu);
+          uint32_t near = 0;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            // x * inv is off by less than 2^-15 here (infinite or NaN for the smallest steps): next to a border the
+            // quotient itself decides. It is an f32 rounded once, and a value and a border that differ do so by more
+            // than its rounding.
+            // Rounding by adding 1.5 * 2^23, whose low bits are then the whole number.
+            const float q = x[n][k] * inv, t = q + 12582912.f;
+            near |= !(fabsf(q - (t - 12582912.f)) < 0.5f - 0x1p-12f) ? 1u << k : 0u;
+            const int c = min(max(__float_as_int(t) - 0x4b400000 - z, 0), 15);
+            word |= d + k < p.dim ? (uint32_t)c << (4 * k) : 0u;
+          }
+          if (near) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if ((near >> k & 1u) && d + k < p.dim)
+                word = (word & ~(15u << (4 * k))) | (uint32_t)min((int)rintf(__fdiv_rn(x[n][k], step)) - z, 15) << (4 * k);
+          }
+        }
+        if (i < 4 * p.units) *(uint32_t*)(p.codes + to[n] * p.ld_codes + 4 * word_at(i, p.units)) = word;
+        uint32_t* words = p.words + to[n] * p.ld_words;
+        if (i % L == 0) words[i / L] = w;
+        if (i == 0)
+          for (uint32_t g = ng; g < wide; ++g) words[g] = 0;
+      }
     }
     __syncthreads();
   }
@@ -199,15 +269,17 @@ __global__ void __launch_bounds__(256) write_kernel(const Write p) {
 
 // ---------------------------------------------------------------------------
 // Reading: a lane writes 16 bytes of the output, half a word of f32 or a whole one
-// of 16-bit values. Rows of no id are 0.
+// of 16-bit values, four such pieces at once. Rows of no id are 0.
 // ---------------------------------------------------------------------------
 struct Read {
   const uint8_t* codes;
   const uint32_t* words;
   uint64_t n, ld_codes, ld_words;
   uint32_t dim, group, units;
-  const int32_t* ids;  // null: row i
+  const int32_t* ids;   // null: row i
   uint64_t m;
+  uint32_t run;         // rows of a CTA at once
+  uint32_t per, magic;  // pieces of a row
   void* out;
   uint64_t ld;
   int* status;
@@ -217,40 +289,51 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) read_kernel(const Read p) {
   constexpr uint32_t V = 16 / sizeof(T);
   after_previous();
-  const uint32_t per = (p.dim + V - 1) / V;
-  const uint64_t total = p.m * per;
-  for (uint64_t u = (uint64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += (uint64_t)gridDim.x * 256) {
-    const uint64_t r = u / per;
-    const uint32_t d = (uint32_t)(u - r * per) * V;
-    const int64_t from = p.ids ? (int64_t)p.ids[r] : (int64_t)r;
-    const bool there = from >= 0 && from < (int64_t)p.n;
-    if (from >= (int64_t)p.n && d == 0) raven_score::tell(p.status, kStatusIds);
-    float step = 0.f, z = 0.f;
-    uint32_t word = 0;
-    if (there) {
-      const uint32_t w = p.words[from * p.ld_words + d / p.group];
-      step = step_of(w);
-      z = zero_of(w);
-      word = *(const uint32_t*)(p.codes + from * p.ld_codes + 4 * word_at(d / 8, p.units)) >> (4 * (d % 8));
-    }
-    __align__(16) T v[V];
+  const uint32_t shift = 31 - __clz(p.group);
+  for (uint64_t r0 = (uint64_t)blockIdx.x * p.run; r0 < p.m; r0 += (uint64_t)gridDim.x * p.run) {
+    const uint32_t rows = (uint32_t)min((uint64_t)p.run, p.m - r0), items = rows * p.per;
+    for (uint32_t u0 = 0; u0 < items; u0 += 256 * kItems) {
+      uint32_t word[kItems], scale[kItems];
 #pragma unroll
-    for (uint32_t k = 0; k < V; ++k) {
-      const float f = there ? ((float)((word >> (4 * k)) & 15u) + z) * step : 0.f;
-      if constexpr (sizeof(T) == 4)
-        v[k] = f;
-      else if constexpr (std::is_same<T, __half>::value)
-        v[k] = __float2half_rn(f);
-      else
-        v[k] = __float2bfloat16_rn(f);
-    }
-    T* to = (T*)p.out + r * p.ld + d;
-    if (VEC && d + V <= p.dim) {
-      *(uint4*)to = *(const uint4*)v;
-    } else {
+      for (int n = 0; n < kItems; ++n) {
+        const uint32_t u = u0 + n * 256 + threadIdx.x, r = divided(u, p.magic), d = (u - r * p.per) * V;
+        word[n] = scale[n] = 0;
+        if (u < items) {
+          const int64_t from = p.ids ? (int64_t)p.ids[r0 + r] : (int64_t)(r0 + r);
+          if (from >= 0 && from < (int64_t)p.n) {
+            scale[n] = p.words[from * p.ld_words + (d >> shift)];
+            word[n] = *(const uint32_t*)(p.codes + from * p.ld_codes + 4 * word_at(d / 8, p.units)) >> (4 * (d % 8));
+          } else if (from >= 0 && d == 0) {
+            raven_score::tell(p.status, kStatusIds);
+          }
+        }
+      }
 #pragma unroll
-      for (uint32_t k = 0; k < V; ++k)
-        if (d + k < p.dim) to[k] = v[k];
+      for (int n = 0; n < kItems; ++n) {
+        const uint32_t u = u0 + n * 256 + threadIdx.x, r = divided(u, p.magic), d = (u - r * p.per) * V;
+        if (u >= items) continue;
+        // code + z: the code as the low bits of 2^23, all exact
+        const float step = step_of(scale[n]), z = zero_of(scale[n]) - 8388608.f;
+        __align__(16) T v[V];
+#pragma unroll
+        for (uint32_t k = 0; k < V; ++k) {
+          const float f = (__uint_as_float((word[n] >> (4 * k) & 15u) | 0x4b000000u) + z) * step;
+          if constexpr (sizeof(T) == 4)
+            v[k] = f;
+          else if constexpr (std::is_same<T, __half>::value)
+            v[k] = __float2half_rn(f);
+          else
+            v[k] = __float2bfloat16_rn(f);
+        }
+        T* to = (T*)p.out + (r0 + r) * p.ld + d;
+        if (VEC && d + V <= p.dim) {
+          *(uint4*)to = *(const uint4*)v;
+        } else {
+#pragma unroll
+          for (uint32_t k = 0; k < V; ++k)
+            if (d + k < p.dim) to[k] = v[k];
+        }
+      }
     }
   }
 }

@@ -42,13 +42,28 @@ int check_int4(const raven_rows* r, uint32_t dim, const char* what) {
   return RAVEN_OK;
 }
 
-template <typename T, bool LANE>
+// Rows of a CTA at once: kItems pieces a thread, as long as every SM gets rows. Sets what divides by `per`.
+uint32_t rows_at_once(uint64_t m, uint32_t per, int sms, uint32_t most, uint32_t* magic) {
+  *magic = per > 1 ? (uint32_t)((0x100000000ull + per - 1) / per) : 0;
+  const uint64_t fair = (m + 2ull * sms - 1) / (2ull * sms);
+  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({256 * raven_int4::kItems / per, most, fair}));
+}
+
+template <typename T, uint32_t L, bool LANE>
 cudaError_t launch_write(raven_int4::Write p, int sms, cudaStream_t st) {
   const bool vec = !LANE && p.ld * sizeof(T) % 16 == 0 && aligned(p.x, 16);
+  p.per = (p.dim + 8 * L - 1) / (8 * L) * L;
+  p.run = rows_at_once(p.m, p.per, sms, raven_int4::kRun, &p.magic);
   const uint64_t grid = std::min<uint64_t>((p.m + p.run - 1) / p.run, (uint64_t)sms * 64);
   static Allowed none;
-  return launch(vec ? raven_int4::write_kernel<T, true, LANE> : raven_int4::write_kernel<T, false, LANE>, grid, 256, 0,
+  return launch(vec ? raven_int4::write_kernel<T, L, true, LANE> : raven_int4::write_kernel<T, L, false, LANE>, grid, 256, 0,
                 none, st, p);
+}
+template <typename T, bool LANE>
+cudaError_t group_write(const raven_int4::Write& p, int sms, cudaStream_t st) {
+  return p.group == 32   ? launch_write<T, 4, LANE>(p, sms, st)
+         : p.group == 64 ? launch_write<T, 8, LANE>(p, sms, st)
+                         : launch_write<T, 16, LANE>(p, sms, st);
 }
 
 // Up to here every CTA looks for its slots among the later ones.
@@ -73,8 +88,6 @@ int write_rows(const void* x, int32_t type, uint64_t m, uint32_t dim, uint64_t l
   p.ld_words = out->ld_exps;
   p.slots = slots;
   p.status = status;
-  const uint32_t per = (dim + p.group - 1) / p.group * (p.group / 8);
-  p.run = std::min(raven_int4::kRun, std::max(1u, 256 / per));
   raven_int4::Claim* table = nullptr;
   cudaError_t e = cudaSuccess;
   if (slots && m > kFewSlots) {
@@ -87,20 +100,21 @@ int write_rows(const void* x, int32_t type, uint64_t m, uint32_t dim, uint64_t l
       e = launch(raven_int4::claim_kernel, (m + 255) / 256, 256, 0, none, st, slots, (uint32_t)m, p.n, table, p.bits);
   }
   if (e == cudaSuccess)
-    e = type == RAVEN_TYPE_F32   ? (lane ? launch_write<float, true>(p, sms, st) : launch_write<float, false>(p, sms, st))
-        : type == RAVEN_TYPE_F16 ? launch_write<__half, false>(p, sms, st)
-                                 : launch_write<__nv_bfloat16, false>(p, sms, st);
+    e = type == RAVEN_TYPE_F32   ? (lane ? group_write<float, true>(p, sms, st) : group_write<float, false>(p, sms, st))
+        : type == RAVEN_TYPE_F16 ? group_write<__half, false>(p, sms, st)
+                                 : group_write<__nv_bfloat16, false>(p, sms, st);
   if (table) cudaFreeAsync(table, st);
   if (e != cudaSuccess) return fail(RAVEN_ECUDA, std::string("4-bit rows: ") + cudaGetErrorString(e));
   return RAVEN_OK;
 }
 
 template <typename T>
-cudaError_t launch_read(const raven_int4::Read& p, int sms, cudaStream_t st) {
+cudaError_t launch_read(raven_int4::Read p, int sms, cudaStream_t st) {
   const bool vec = p.ld * sizeof(T) % 16 == 0 && aligned(p.out, 16);
-  constexpr uint64_t V = 16 / sizeof(T);
-  const uint64_t items = p.m * ((p.dim + V - 1) / V);
-  const uint64_t grid = std::min<uint64_t>((items + 255) / 256, (uint64_t)sms * 32);
+  constexpr uint32_t V = 16 / sizeof(T);
+  p.per = (p.dim + V - 1) / V;
+  p.run = rows_at_once(p.m, p.per, sms, 256 * raven_int4::kItems, &p.magic);
+  const uint64_t grid = std::min<uint64_t>((p.m + p.run - 1) / p.run, (uint64_t)sms * 64);
   static Allowed none;
   return launch(vec ? raven_int4::read_kernel<T, true> : raven_int4::read_kernel<T, false>, grid, 256, 0, none, st, p);
 }
@@ -111,85 +125,112 @@ cudaError_t launch_read(const raven_int4::Read& p, int sms, cudaStream_t st) {
 constexpr uint32_t kMostShared = 227 * 1024;
 constexpr uint64_t kOwnLayout = 16384;  // values that each CTA lays out for itself
 
-template <int NT, int G, bool F32, bool HELD, typename O>
-cudaError_t launch_score4(const CUtensorMap& map, const raven_score4::Params& p, uint64_t ctas, cudaStream_t st) {
+// Codes as boxes of up to 64 bytes (a block) x `rows` rows; what is past a row's end or the last row reads 0.
+bool codes_map(CUtensorMap* m, const raven_rows* v, uint32_t units, uint32_t rows) {
+  PFN_cuTensorMapEncodeTiled_v12000 f = raven_internal::encode_tiled();
+  if (!f) return false;
+  cuuint64_t gdim[2] = {16ull * units, v->rows};
+  cuuint64_t gstride[1] = {v->ld};
+  cuuint32_t box[2] = {std::min(64u, 16 * units), rows};
+  cuuint32_t es[2] = {1, 1};
+  return f(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)v->data, gdim, gstride, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int NT, int G, bool F32, typename O>
+cudaError_t launch_score4(const CUtensorMap& map, const raven_score4::Params& p, uint64_t ctas, uint64_t smem, cudaStream_t st) {
   using namespace raven_score4;
-  using L = Layout<NT, G>;
   static Allowed allowed(kMostShared);
-  return launch(score4_kernel<NT, G, F32, HELD, O>, ctas, L::kThreads,
-                (uint32_t)L::bytes(p.units, p.groups, p.split, p.depth, HELD), allowed, st, map, p);
+  return launch(score4_kernel<NT, G, F32, O>, ctas, Layout<NT, G>::kThreads, (uint32_t)smem, allowed, st, map, p);
 }
 
 template <int NT, int G, bool F32>
-cudaError_t run_score4(const CUtensorMap& map, raven_score4::Params p, int out_type, int sms, cudaStream_t st) {
+cudaError_t run_score4(const raven_rows* v, raven_score4::Params p, int out_type, int sms, cudaStream_t st) {
   using namespace raven_score4;
   using L = Layout<NT, G>;
   using Q = Laid<NT>;
   constexpr uint32_t kQueries = F32 ? NT * 4 : NT * 8;
   p.chunks = (uint32_t)((p.nq + kQueries - 1) / kQueries);
-  const uint64_t columns = std::max<uint64_t>(1, (uint64_t)sms / p.chunks);  // CTAs of a chunk
+  // slices of a row: as few as let a CTA hold its queries beside its rings
+  p.slices = 1;
+  p.slice = p.blocks;
+  while (L::bytes(std::min(4 * p.slice, p.units), std::min(p.slice * L::kWords, p.groups), std::min(L::kWarps, p.slice),
+                  L::kLeast) >
+         kMostShared) {
+    ++p.slices;
+    p.slice = (p.blocks + p.slices - 1) / p.slices;
+  }
+  p.slices = (p.blocks + p.slice - 1) / p.slice;
+  const uint32_t shares = p.chunks * p.slices;
+  const uint64_t columns = std::max<uint64_t>(1, (uint64_t)sms / shares);  // CTAs of a share
   // Warps that share a row: as few as keep them evenly busy. In blocks of 128 values, what the busiest warp takes,
   // with a block's time for sums that meet.
   uint64_t best = ~0ull;
-  for (uint32_t split = 1; split <= L::kWarps && split <= p.blocks; split *= 2) {
-    const uint64_t rows = kRows * (L::kWarps / split), tiles = (p.n + rows - 1) / rows;
-    const uint64_t time = (tiles + columns - 1) / columns * ((p.blocks + split - 1) / split + (split > 1 ? 1 : 0));
+  for (uint32_t split = 1; split <= p.slice && L::kWarps % split == 0; split *= 2) {
+    const uint64_t rows = L::kRows * (L::kWarps / split), tiles = (p.n + rows - 1) / rows;
+    const uint64_t time = (tiles + columns - 1) / columns * ((p.slice + split - 1) / split + (split > 1 ? 1 : 0));
     if (time < best) {
       best = time;
       p.split = split;
-      p.tiles = tiles;
+      p.tiles = (uint32_t)tiles;
     }
   }
-  // three tiles under way at least, beside the queries
-  const bool held = L::bytes(p.units, p.groups, p.split, 3, true) <= kMostShared;
+  const uint32_t units = std::min(4 * p.slice, p.units), groups = std::min(p.slice * L::kWords, p.groups);
   p.depth = kMaxDepth;
-  while (L::bytes(p.units, p.groups, p.split, p.depth, held) > kMostShared) --p.depth;
-  uint8_t* laid = nullptr;
+  while (L::bytes(units, groups, p.split, p.depth) > kMostShared) --p.depth;
+  uint8_t* tmp = nullptr;
   cudaError_t e = cudaSuccess;
-  if (!held || (uint64_t)kQueries * p.dim > kOwnLayout) {
-    if ((e = cudaMallocAsync((void**)&laid, p.chunks * Q::bytes(p.units, p.groups), st)) != cudaSuccess) return e;
+  const bool lay = p.slices > 1 || (uint64_t)kQueries * p.dim > kOwnLayout;
+  const uint64_t laid = lay ? (p.chunks * Q::bytes(p.units, p.groups) + 255) / 256 * 256 : 0;
+  const uint64_t wide = (p.n + 3) / 4 * 4, sums = p.slices > 1 ? p.slices * p.nq * wide * 4 : 0;
+  if (laid + sums && (e = cudaMallocAsync((void**)&tmp, laid + sums, st)) != cudaSuccess) return e;
+  if (lay) {
     static Allowed none;
-    e = launch(lay_out_kernel<NT, G, F32>, (uint64_t)p.chunks * kQueries, 256, 0, none, st, p, laid);
+    e = launch(lay_out_kernel<NT, G, F32>, (uint64_t)p.chunks * kQueries, 256, 0, none, st, p, tmp);
     p.q = nullptr;
-    p.laid = laid;
+    p.laid = tmp;
   }
-  const uint64_t ctas = std::min(columns, p.tiles) * p.chunks;
-  auto go = [&](auto o) {
-    using O = decltype(o);
-    return held ? launch_score4<NT, G, F32, true, O>(map, p, ctas, st) : launch_score4<NT, G, F32, false, O>(map, p, ctas, st);
-  };
-  if (e == cudaSuccess) e = out_type == 0 ? go(float()) : out_type == 1 ? go(__half()) : go(__nv_bfloat16());
-  if (laid) cudaFreeAsync(laid, st);
+  Join j{(const float*)(tmp + laid), wide, p.nq * wide, p.slices, p.nq, p.n, p.alpha, p.bias, p.out, p.ld};
+  if (p.slices > 1) {
+    p.out = tmp + laid;
+    p.ld = wide;
+    p.ld_slice = p.nq * wide;
+    p.alpha = 1.f;
+    p.bias = nullptr;
+  }
+  p.whole = aligned(p.out, 16) && (p.nq == 1 || p.ld % (16 / (p.slices > 1 || out_type == 0 ? 4 : 2)) == 0);
+  CUtensorMap map;
+  if (e == cudaSuccess && !codes_map(&map, v, p.units, L::kRows)) e = cudaErrorInvalidValue;
+  const uint64_t ctas = std::min<uint64_t>(columns, p.tiles) * shares, smem = L::bytes(units, groups, p.split, p.depth);
+  if (e == cudaSuccess)
+    e = p.slices > 1 || out_type == 0 ? launch_score4<NT, G, F32, float>(map, p, ctas, smem, st)
+        : out_type == 1               ? launch_score4<NT, G, F32, __half>(map, p, ctas, smem, st)
+                                      : launch_score4<NT, G, F32, __nv_bfloat16>(map, p, ctas, smem, st);
+  if (p.slices > 1 && e == cudaSuccess) {
+    static Allowed none;
+    const uint64_t grid = std::min<uint64_t>((p.nq * (wide / 4) + 255) / 256, (uint64_t)sms * 32);
+    e = launch(out_type == 0 ? join_kernel<float> : out_type == 1 ? join_kernel<__half> : join_kernel<__nv_bfloat16>, grid, 256,
+               0, none, st, j);
+  }
+  if (tmp) cudaFreeAsync(tmp, st);
   return e;
 }
 
 template <int NT, bool F32>
-cudaError_t group_score4(const CUtensorMap& map, const raven_score4::Params& p, uint32_t group, int out_type, int sms,
+cudaError_t group_score4(const raven_rows* v, const raven_score4::Params& p, uint32_t group, int out_type, int sms,
                          cudaStream_t st) {
-  return group == 32   ? run_score4<NT, 32, F32>(map, p, out_type, sms, st)
-         : group == 64 ? run_score4<NT, 64, F32>(map, p, out_type, sms, st)
-                       : run_score4<NT, 128, F32>(map, p, out_type, sms, st);
+  return group == 32   ? run_score4<NT, 32, F32>(v, p, out_type, sms, st)
+         : group == 64 ? run_score4<NT, 64, F32>(v, p, out_type, sms, st)
+                       : run_score4<NT, 128, F32>(v, p, out_type, sms, st);
 }
 
 template <bool F32>
-cudaError_t dispatch_score4(const CUtensorMap& map, const raven_score4::Params& p, uint32_t group, int out_type, int sms,
+cudaError_t dispatch_score4(const raven_rows* v, const raven_score4::Params& p, uint32_t group, int out_type, int sms,
                             cudaStream_t st) {
   const uint64_t columns = F32 ? 2 * p.nq : p.nq;
-  return columns <= 8    ? group_score4<1, F32>(map, p, group, out_type, sms, st)
-         : columns <= 16 ? group_score4<2, F32>(map, p, group, out_type, sms, st)
-                         : group_score4<4, F32>(map, p, group, out_type, sms, st);
-}
-
-// Codes as boxes of up to 64 bytes (a block) x a warp's rows; what is past a row's end or the last row reads 0.
-bool codes_map(CUtensorMap* m, const raven_rows* v, uint32_t units) {
-  PFN_cuTensorMapEncodeTiled_v12000 f = raven_internal::encode_tiled();
-  if (!f) return false;
-  cuuint64_t gdim[2] = {16ull * units, v->rows};
-  cuuint64_t gstride[1] = {v->ld};
-  cuuint32_t box[2] = {std::min(64u, 16 * units), raven_score4::kRows};
-  cuuint32_t es[2] = {1, 1};
-  return f(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)v->data, gdim, gstride, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-           CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return columns <= 8    ? group_score4<1, F32>(v, p, group, out_type, sms, st)
+         : columns <= 16 ? group_score4<2, F32>(v, p, group, out_type, sms, st)
+                         : group_score4<4, F32>(v, p, group, out_type, sms, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -197,10 +238,10 @@ bool codes_map(CUtensorMap* m, const raven_rows* v, uint32_t units) {
 // ---------------------------------------------------------------------------
 template <typename T>
 cudaError_t launch_adjust(const raven_adjust::Params& p, bool largest, cudaStream_t st) {
-  static Allowed allowed[2];
-  const uint32_t smem = p.seen ? p.tile * 4 + (p.tile + 31) / 32 * 4 : 0;
+  static Allowed none;
+  const uint32_t smem = p.seen ? raven_adjust::shared_bytes(p.tile) : 0;
   return launch(largest ? raven_adjust::adjust_kernel<T, true> : raven_adjust::adjust_kernel<T, false>, p.nq * p.tiles, 256,
-                smem, allowed[largest], st, p);
+                smem, none, st, p);
 }
 
 __global__ void status_kernel(int* status) {
@@ -258,12 +299,9 @@ int int4_scores(const raven_rows* q, const raven_rows* v, uint32_t dim, float al
   p.bias = bias;
   p.out = out;
   p.ld = ld;
-  p.whole = aligned(out, 4 * type_size(out_type)) && (ld % 4 == 0 || p.nq == 1);
   p.status = status;
-  CUtensorMap map;
-  if (!codes_map(&map, v, p.units)) return fail(RAVEN_ECUDA, "scores: no tensor map of the vectors");
-  CU(q->type == RAVEN_TYPE_F32 ? dispatch_score4<true>(map, p, group, kind_of(out_type), sms, st)
-                               : dispatch_score4<false>(map, p, group, kind_of(out_type), sms, st));
+  CU(q->type == RAVEN_TYPE_F32 ? dispatch_score4<true>(v, p, group, kind_of(out_type), sms, st)
+                               : dispatch_score4<false>(v, p, group, kind_of(out_type), sms, st));
   return RAVEN_OK;
 }
 
@@ -384,8 +422,11 @@ int raven_adjust_scores_device(const void* d_scores, int32_t type, uint64_t nq, 
   p.presence_all = by->presence_all;
   p.frequency_all = by->frequency_all;
   p.status = d_status;
-  p.tile = 4096;
-  p.tiles = (n + p.tile - 1) / p.tile;
+  // the largest tiles, since each scans its row's history, that leave every SM four
+  const uint64_t most = 16 / size - 1;  // columns before a row's first
+  p.tile = 8192;
+  while (p.tile > 1024 && nq * ((n + most + p.tile - 1) / p.tile) < 4ull * sms) p.tile /= 2;
+  p.tiles = (n + most + p.tile - 1) / p.tile;
   if (nq * p.tiles > kMaxRows) return fail(RAVEN_ELIMIT, "scores: more tiles than a launch holds");
   cudaStream_t st = (cudaStream_t)stream;
   CU(type == RAVEN_TYPE_F32   ? launch_adjust<float>(p, largest != 0, st)

@@ -19,11 +19,13 @@
 //
 // Two parts of an f32 query are two columns of the N side, added up at the end.
 //
-// What bounds it: reading the codes. Each warp has its own ring of tiles of 32 rows
-// x 128 values in shared memory: one TMA copy of 2 KB, and a copy of 4 to 16 bytes
-// a lane for the scale words. Where a CTA's tiles are few or large, warps share a
-// tile's rows and take its blocks of 128 values in turn; their sums meet in shared
-// memory and are added up in a fixed order.
+// What bounds it: reading the codes. Each warp has its own ring of tiles of 32 or 64
+// rows x 128 values in shared memory: one TMA copy of 2 or 4 KB, and a copy of 4 to
+// 16 bytes a row for the scale words. Where a CTA's tiles are few or large, warps
+// share a tile's rows and take its blocks of 128 values in turn; their sums meet in
+// shared memory and are added up in a fixed order. A CTA holds its queries in shared
+// memory; where rows are too long for that, CTAs take slices of them, and a second
+// kernel adds up their sums.
 #pragma once
 
 #include <cuda.h>
@@ -49,9 +51,7 @@ using raven_tc::mbar_init;
 using raven_tc::smem_u32;
 using raven_tc::tma_load_2d;
 
-constexpr int kMT = 2;                // M tiles of a warp
-constexpr uint32_t kRows = 16 * kMT;  // rows of a warp's tile
-constexpr uint32_t kMaxDepth = 6;     // tiles under way per warp, at most
+constexpr uint32_t kMaxDepth = 6;  // tiles under way per warp, at most
 
 struct Params {
   const void* q;      // queries that each CTA lays out for itself, or null: `laid` holds them
@@ -62,14 +62,16 @@ struct Params {
   const uint32_t* words;
   uint64_t n, ld_words;
   uint32_t dim, units, blocks, groups;  // of a row
+  uint32_t slices;    // of a row's blocks, `slice` blocks each but the last
+  uint32_t slice;
   uint32_t split;     // warps that share a row's blocks
   uint32_t depth;     // of the rings
   uint32_t chunks;    // of the queries
-  uint64_t tiles;     // of a CTA's rows
+  uint32_t tiles;     // of a CTA's rows
   float alpha;
   const float* bias;
-  void* out;
-  uint64_t ld;
+  void* out;          // of slice s at out + s * ld_slice
+  uint64_t ld, ld_slice;
   bool whole;         // four scores of a query can be written at once
   int* status;
 };
@@ -227,7 +229,7 @@ __device__ inline void meet(uint32_t id, uint32_t threads) {
 }
 
 __device__ inline void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -235,17 +237,30 @@ __device__ inline void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
 
 template <int NT, int G>
 struct Layout {
-  static constexpr uint32_t kWarps = NT <= 2 ? 16 : 8;    // as many as their registers allow
+#ifndef MT1
+#define MT1 4
+#define W1 16
+#define W2 16
+#endif
+  static constexpr int kMT = NT == 1 ? MT1 : 2;           // M tiles of a warp: few queries leave registers for four
+  static constexpr int kAtOnce = NT == 4 ? kMT : 1;       // M tiles that go through a block together
+  static constexpr uint32_t kRows = 16 * kMT;             // rows of its tile
+  static constexpr uint32_t kWarps = NT == 1 ? W1 : NT == 2 ? W2 : 8;    // as many as their registers allow
   static constexpr uint32_t kThreads = kWarps * 32;
   static constexpr uint32_t kWords = kBlock / G;          // scale words of a row's block
   static constexpr uint32_t kCodeBytes = kRows * 64, kWordBytes = kRows * kWords * 4;
   static constexpr uint32_t kPart = 32 * 4 * kMT * NT * 4;  // a warp's sums
   static constexpr uint32_t kBars = kWarps * kMaxDepth * 8;  // in front of the rings
   static constexpr uint32_t kTops = NT * 8 * 4;
+  static_assert(kBars % 128 == 0 && kCodeBytes % 128 == 0, "a TMA copy's place in shared memory");
+  static constexpr uint32_t kLeast = NT == 1 ? 2 : 3;      // stages of a ring
+  // what every call needs: rings, a block of queries, sums that meet
+  static_assert(kBars + kLeast * (uint64_t)kWarps * (kCodeBytes + kWordBytes) + kTops + kWarps * kPart + 4 * Laid<NT>::kUnitBytes +
+                kWords * NT * 32 + NT * 64 <= 227 * 1024, "shared memory of a CTA");
   __host__ __device__ static uint64_t ring(uint32_t depth) { return (uint64_t)kWarps * depth * (kCodeBytes + kWordBytes); }
   __host__ __device__ static uint64_t shared(uint32_t split) { return split > 1 ? kWarps * kPart : 0; }
-  __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t groups, uint32_t split, uint32_t depth, bool held) {
-    return kBars + ring(depth) + kTops + shared(split) + (held ? Laid<NT>::bytes(units, groups) : 0);
+  __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t groups, uint32_t split, uint32_t depth) {
+    return kBars + ring(depth) + kTops + shared(split) + Laid<NT>::bytes(units, groups);
   }
 };
 
@@ -259,12 +274,12 @@ __device__ inline T rounded(float v) {
     return __float2bfloat16_rn(v);
 }
 
-// HELD: the chunk's queries are in shared memory; else read through L1.
-template <int NT, int G, bool F32, bool HELD, typename O>
+template <int NT, int G, bool F32, typename O>
 __global__ void __launch_bounds__(Layout<NT, G>::kThreads, 1) score4_kernel(const __grid_constant__ CUtensorMap map,
                                                                             const Params p) {
   using S = Layout<NT, G>;
   using Q = Laid<NT>;
+  constexpr int MT = S::kMT, R = 2 * MT;  // rows of a lane
   constexpr uint32_t kQueries = F32 ? NT * 4 : NT * 8;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32, g = lane >> 2, t = lane & 3, odd = g & 1;
@@ -276,7 +291,12 @@ __global__ void __launch_bounds__(Layout<NT, G>::kThreads, 1) score4_kernel(cons
   float* shared = (float*)(after + S::kTops);
   uint8_t* held = after + S::kTops + S::shared(p.split);
   const uint32_t kw = warp % p.split, wr = warp / p.split, across = S::kWarps / p.split;
-  const uint64_t chunk = blockIdx.x % p.chunks, step = gridDim.x / p.chunks, first = blockIdx.x / p.chunks;
+  // this CTA's queries, slice of the blocks, tiles
+  const uint32_t shares = p.chunks * p.slices, share = blockIdx.x % shares;
+  const uint32_t step = gridDim.x / shares, first = blockIdx.x / shares;
+  const uint32_t slice = share % p.slices;
+  const uint64_t chunk = share / p.slices;
+  const uint32_t b0 = slice * p.slice, blocks = min(p.slice, p.blocks - b0);
   const uint32_t pitch = min(64u, 16 * p.units);  // of a tile's rows of codes
   if (lane < p.depth) mbar_init(bars + 8 * lane, 33);
   asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -284,55 +304,152 @@ __global__ void __launch_bounds__(Layout<NT, G>::kThreads, 1) score4_kernel(cons
   after_previous();
 
   // the ring: what is copied next
-  uint64_t ahead = first;
-  uint32_t ahead_b = kw, slot = 0, pending = 0;
-  const uint32_t codes_at = smem_u32(codes), words_at = smem_u32(words);
+  uint32_t ahead = first, ahead_b = kw, slot = 0, pending = 0;
+  const uint32_t codes_at = smem_u32(codes), words_at = smem_u32(words) + lane * (4 * S::kWords);
+  int ahead_y = 0;
+  const uint32_t* ahead_words[S::kRows / 32];
+  auto aim = [&]() {
+    const uint64_t row0 = ((uint64_t)ahead * across + wr) * S::kRows;
+    ahead_y = (int)min(row0, p.n);
+#pragma unroll
+    for (uint32_t i = 0; i < S::kRows / 32; ++i)
+      ahead_words[i] = p.words + min(row0 + lane + 32 * i, p.n - 1) * p.ld_words + b0 * S::kWords;
+  };
   auto copy_next = [&]() {
     if (ahead < p.tiles) {
-      const uint64_t row0 = (ahead * across + wr) * kRows;
       const uint32_t bar = bars + 8 * slot;
-      copy_async<4 * S::kWords>(words_at + slot * S::kWordBytes + lane * (4 * S::kWords),
-                                p.words + min(row0 + lane, p.n - 1) * p.ld_words + ahead_b * S::kWords);
+#pragma unroll
+      for (uint32_t i = 0; i < S::kRows / 32; ++i)
+        copy_async<4 * S::kWords>(words_at + slot * S::kWordBytes + i * (128 * S::kWords), ahead_words[i] + ahead_b * S::kWords);
       copies_arrive(bar);
       if (lane == 0) {
-        mbar_expect_tx(bar, kRows * pitch);
-        tma_load_2d(codes_at + slot * S::kCodeBytes, &map, (int)(64 * ahead_b), (int)min(row0, p.n), bar);
+        mbar_expect_tx(bar, S::kRows * pitch);
+        tma_load_2d(codes_at + slot * S::kCodeBytes, &map, (int)(64 * (b0 + ahead_b)), ahead_y, bar);
       }
       pending |= 1u << slot;
       slot = slot + 1 == p.depth ? 0 : slot + 1;
       ahead_b += p.split;
-      if (ahead_b >= p.blocks) {
+      if (ahead_b >= blocks) {
         ahead_b = kw;
         ahead += step;
+        aim();
       }
     }
   };
+  if (kw >= blocks) ahead = p.tiles;  // a last slice of fewer blocks than warps
+  aim();
   for (uint32_t i = 0; i + 1 < p.depth; ++i) copy_next();
 
-  const uint8_t* laid = held;
-  if constexpr (HELD) {
-    if (p.q) {
-      lay_out_any<NT, G, F32>(p, chunk * kQueries, kQueries, 0, held, tops);
-    } else {
-      const uint32_t bytes = (uint32_t)Q::bytes(p.units, p.groups);
-      const uint8_t* from = p.laid + chunk * bytes;
-      for (uint32_t i = threadIdx.x * 16; i < bytes; i += S::kThreads * 16) *(uint4*)(held + i) = *(const uint4*)(from + i);
-    }
-    __syncthreads();
+  const uint32_t units = min(4 * p.slice, p.units - 4 * b0), groups = min(p.slice * S::kWords, p.groups - b0 * S::kWords);
+  float* sums = (float*)(held + Q::frags(units));
+  float* back = sums + groups * NT * 8;
+  if (p.q) {
+    lay_out_any<NT, G, F32>(p, chunk * kQueries, kQueries, 0, held, tops);
   } else {
-    laid = p.laid + chunk * Q::bytes(p.units, p.groups);
+    const uint8_t* from = p.laid + chunk * Q::bytes(p.units, p.groups);
+    auto bring = [&](void* to, const uint8_t* what, uint32_t bytes) {
+      for (uint32_t i = threadIdx.x * 16; i < bytes; i += S::kThreads * 16)
+        *(uint4*)((uint8_t*)to + i) = *(const uint4*)(what + i);
+    };
+    bring(held, from + Q::frags(4 * b0), (uint32_t)Q::frags(units));
+    from += Q::frags(p.units);
+    bring(sums, from + Q::sums(b0 * S::kWords), (uint32_t)Q::sums(groups));
+    bring(back, from + Q::sums(p.groups), NT * 8 * 8);
   }
-  const float* sums = (const float*)(laid + Q::frags(p.units));
-  const float* back = sums + p.groups * NT * 8;
+  __syncthreads();
 
   bool ok = true;  // no wait has run out
   uint32_t now = 0, phases = 0;  // the stage that is taken next; parities of the stages
-  // row m * 16 + g (+ 8) of the fragments is row 8 (g / 2) + g % 2 + 4 m (+ 2) of the tile: two lanes next to one
-  // another in g read 128 bytes side by side
-  const uint32_t my_row = 8 * (g >> 1) + odd;
-  for (uint64_t tile = first; tile < p.tiles; tile += step) {
-    float total[kMT][NT][4] = {};
-    for (uint32_t b = kw; b < p.blocks; b += p.split) {
+  // Row 16 m + g (+ 8) of the fragments is row R (g / 2) * 2 + g % 2 + 4 m (+ 2) of the tile: two lanes next to one
+  // another in g read 128 bytes side by side.
+  const uint32_t my_row = 2 * R * (g >> 1) + odd;
+  for (uint32_t tile = first; tile < p.tiles; tile += step) {
+    float total[MT][NT][4] = {};
+    auto block = [&](auto full, const uint8_t* stage, const uint32_t* word, uint32_t b, uint32_t u) {
+      constexpr bool FULL = decltype(full)::value;
+      constexpr int MG = S::kAtOnce;  // M tiles at once
+      uint4 x[4][NT];                 // the queries' fragments
+      auto fetch = [&](uint32_t unit) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          if (FULL || unit < u) x[unit][j] = *(const uint4*)(held + (4 * b + unit) * Q::kUnitBytes + lane * 16 + j * 512);
+      };
+      if constexpr (MG < MT) {
+#pragma unroll
+        for (uint32_t unit = 0; unit < 4; ++unit) fetch(unit);
+      }
+#pragma unroll
+      for (int m0 = 0; m0 < MT; m0 += MG) {
+        uint4 code[MG][2];
+#pragma unroll
+        for (int m = 0; m < MG; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t r = my_row + 4 * (m0 + m) + 2 * h;
+            if constexpr (FULL) {
+              code[m][h] = *(const uint4*)(stage + r * 64 + 16 * t);
+            } else {
+              const uint32_t* c = (const uint32_t*)(stage + r * pitch + 4 * u * t);
+              code[m][h] = make_uint4(c[0], u > 1 ? c[1] : 0, u > 2 ? c[2] : 0, 0);
+            }
+          }
+#pragma unroll
+        for (uint32_t gi = 0; gi < S::kWords; ++gi) {
+          constexpr uint32_t U = G / kUnit;
+          if (!FULL && gi * U >= u) break;
+          float sc[MG][2], acc[MG][NT][4];
+          const float* gs = sums + (b * S::kWords + gi) * (NT * 8) + 2 * t;
+#pragma unroll
+          for (int m = 0; m < MG; ++m) {
+            float z[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t w = word[(4 * (m0 + m) + 2 * h) * S::kWords + gi];
+              sc[m][h] = raven_int4::step_of(w);
+              z[h] = raven_int4::zero_of(w);
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              const float2 q = *(const float2*)(gs + 8 * j);
+              acc[m][j][0] = z[0] * q.x;
+              acc[m][j][2] = z[1] * q.x;
+              acc[m][j][1] = F32 ? 0.f : z[0] * q.y;
+              acc[m][j][3] = F32 ? 0.f : z[1] * q.y;
+            }
+          }
+#pragma unroll
+          for (uint32_t uu = 0; uu < U; ++uu) {
+            const uint32_t unit = gi * U + uu;
+            if (!FULL && unit >= u) break;
+            if constexpr (MG == MT) fetch(unit);
+#pragma unroll
+            for (int m = 0; m < MG; ++m) {
+              uint32_t a[2][4];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint4 c = code[m][h];
+                const uint32_t w = unit == 0 ? c.x : unit == 1 ? c.y : unit == 2 ? c.z : c.w;
+                a[h][0] = w & 0x000f000fu;
+                a[h][1] = w & 0x00f000f0u;
+                a[h][2] = (w >> 8) & 0x000f000fu;
+                a[h][3] = (w >> 8) & 0x00f000f0u;
+              }
+#pragma unroll
+              for (int j = 0; j < NT; ++j) mma(acc[m][j], a[0][0], a[1][0], a[0][1], a[1][1], x[unit][j].x, x[unit][j].y);
+#pragma unroll
+              for (int j = 0; j < NT; ++j) mma(acc[m][j], a[0][2], a[1][2], a[0][3], a[1][3], x[unit][j].z, x[unit][j].w);
+            }
+          }
+#pragma unroll
+          for (int m = 0; m < MG; ++m)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) total[m0 + m][j][i] = fmaf(sc[m][i / 2], acc[m][j][i], total[m0 + m][j][i]);
+        }
+      }
+    };
+    for (uint32_t b = kw; b < blocks; b += p.split) {
       if (ok && !__all_sync(0xffffffffu, wait(bars + 8 * now, phases >> now & 1u))) {
         ok = false;
         if (lane == 0) raven_score::tell(p.status, raven_score::kStatusWait);
@@ -345,134 +462,80 @@ __global__ void __launch_bounds__(Layout<NT, G>::kThreads, 1) score4_kernel(cons
       pending &= ~(1u << now);
       now = now + 1 == p.depth ? 0 : now + 1;
       copy_next();  // into the stage that every lane is done with
-      const uint32_t u = min(4u, p.units - 4 * b);
-      uint4 code[kMT][2];
-      if (u == 4) {
-#pragma unroll
-        for (int r = 0; r < 2 * kMT; ++r) code[r / 2][r % 2] = *(const uint4*)(stage + (my_row + 2 * r) * 64 + 16 * t);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 2 * kMT; ++r) {
-          const uint32_t* c = (const uint32_t*)(stage + (my_row + 2 * r) * pitch + 4 * u * t);
-          code[r / 2][r % 2] = make_uint4(c[0], u > 1 ? c[1] : 0, u > 2 ? c[2] : 0, 0);
-        }
-      }
-#pragma unroll
-      for (uint32_t gi = 0; gi < S::kWords; ++gi) {
-        constexpr uint32_t U = G / kUnit;
-        if (gi * U < u) {
-          float sc[kMT][2], acc[kMT][NT][4];
-          const float* gs = sums + (b * S::kWords + gi) * (NT * 8) + 2 * t;
-#pragma unroll
-          for (int m = 0; m < kMT; ++m) {
-            float z[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t w = word[(4 * m + 2 * h) * S::kWords + gi];
-              sc[m][h] = raven_int4::step_of(w);
-              z[h] = raven_int4::zero_of(w);
-            }
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              const float2 x = *(const float2*)(gs + 8 * j);
-              acc[m][j][0] = z[0] * x.x;
-              acc[m][j][2] = z[1] * x.x;
-              acc[m][j][1] = F32 ? 0.f : z[0] * x.y;
-              acc[m][j][3] = F32 ? 0.f : z[1] * x.y;
-            }
-          }
-#pragma unroll
-          for (uint32_t uu = 0; uu < U; ++uu) {
-            const uint32_t unit = gi * U + uu;
-            if (unit < u) {
-              uint32_t a[kMT][2][4];
-#pragma unroll
-              for (int m = 0; m < kMT; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  const uint32_t w = unit == 0   ? code[m][h].x
-                                     : unit == 1 ? code[m][h].y
-                                     : unit == 2 ? code[m][h].z
-                                                 : code[m][h].w;
-                  a[m][h][0] = w & 0x000f000fu;
-                  a[m][h][1] = w & 0x00f000f0u;
-                  a[m][h][2] = (w >> 8) & 0x000f000fu;
-                  a[m][h][3] = (w >> 8) & 0x00f000f0u;
-                }
-              const uint8_t* f = laid + (4 * b + unit) * Q::kUnitBytes + lane * 16;
-#pragma unroll
-              for (int j = 0; j < NT; ++j) {
-                const uint4 x = *(const uint4*)(f + j * 512);
-#pragma unroll
-                for (int m = 0; m < kMT; ++m) {
-                  mma(acc[m][j], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], x.x, x.y);
-                  mma(acc[m][j], a[m][0][2], a[m][1][2], a[m][0][3], a[m][1][3], x.z, x.w);
-                }
-              }
-            }
-          }
-#pragma unroll
-          for (int m = 0; m < kMT; ++m)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) total[m][j][i] = fmaf(sc[m][i / 2], acc[m][j][i], total[m][j][i]);
-        }
-      }
+      const uint32_t u = units - 4 * b;
+      if (u >= 4)
+        block(std::true_type(), stage, word, b, 4);
+      else
+        block(std::false_type(), stage, word, b, u);
     }
-    // The sums of a column (of two, F32) for this lane's four rows, from one warp after the other where several
-    // shared them; lanes next to one another in g swap two, so that each has four rows side by side.
-    const uint64_t row = (tile * across + wr) * kRows + 4 * g;
-    float* mine = shared + warp * (S::kPart / 4) + lane;
+    // The sums of a column (of two, F32) for this lane's rows, from one warp after the other where several shared
+    // them; lanes next to one another in g swap half of theirs, so that each has rows side by side.
+    const uint64_t row = ((uint64_t)tile * across + wr) * S::kRows + R * g;
     if (p.split > 1) {
+      float* mine = shared + warp * (S::kPart / 4) + lane;
 #pragma unroll
-      for (int i = 0; i < kMT * NT * 4; ++i) mine[32 * i] = total[i / (4 * NT)][i / 4 % NT][i % 4];
+      for (int i = 0; i < MT * NT * 4; ++i) mine[32 * i] = total[i / (4 * NT)][i / 4 % NT][i % 4];
       meet(1 + wr, 32 * p.split);
     }
     const float* theirs = shared + wr * p.split * (S::kPart / 4) + lane;
-    float bias[2 * kMT];
+    float bias[R];
 #pragma unroll
-    for (int r = 0; r < 2 * kMT; ++r) bias[r] = p.bias && row + r < p.n ? p.bias[row + r] : 0.f;
+    for (int r = 0; r < R; ++r) bias[r] = 0.f;
+    if (p.bias) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (row + r < p.n) bias[r] = p.bias[row + r];
+    }
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int c = 0; c < (F32 ? 1 : 2); ++c) {
-        float v[2 * kMT];
+        if (chunk * kQueries + (F32 ? 4 * j : 8 * j + c) >= p.nq) continue;  // no lane has a query
+        float v[R];
         if (p.split > 1) {
           if ((j * (F32 ? 1 : 2) + c) % p.split != kw) continue;
 #pragma unroll
-          for (int r = 0; r < 2 * kMT; ++r) v[r] = 0.f;
+          for (int r = 0; r < R; ++r) v[r] = 0.f;
           for (uint32_t k = 0; k < p.split; ++k) {
             const float* from = theirs + k * (S::kPart / 4);
 #pragma unroll
-            for (int r = 0; r < 2 * kMT; ++r) {
+            for (int r = 0; r < R; ++r) {
               const float* x = from + 32 * (((r / 2) * NT + j) * 4 + 2 * (r % 2) + c);
               v[r] += F32 ? x[0] + x[32] : x[0];
             }
           }
         } else {
 #pragma unroll
-          for (int r = 0; r < 2 * kMT; ++r)
+          for (int r = 0; r < R; ++r)
             v[r] = F32 ? total[r / 2][j][2 * (r % 2)] + total[r / 2][j][2 * (r % 2) + 1] : total[r / 2][j][2 * (r % 2) + c];
         }
-        const float s0 = __shfl_xor_sync(0xffffffffu, odd ? v[0] : v[2], 4), s1 = __shfl_xor_sync(0xffffffffu, odd ? v[1] : v[3], 4);
-        const float y[4] = {odd ? s0 : v[0], odd ? v[2] : s0, odd ? s1 : v[1], odd ? v[3] : s1};
+        float y[R];
+#pragma unroll
+        for (int i = 0; i < R / 2; ++i) {
+          const float s = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[R / 2 + i], 4);
+          y[2 * i] = odd ? s : v[i];
+          y[2 * i + 1] = odd ? v[R / 2 + i] : s;
+        }
         const uint32_t col = 8 * j + 2 * t + c;
         const uint64_t query = chunk * kQueries + (F32 ? col / 2 : col);
         if (query < p.nq) {
-          const float b0 = back[2 * col], b1 = back[2 * col + 1];
-          __align__(16) O o[4];
+          const float k0 = back[2 * col], k1 = back[2 * col + 1];
+          __align__(16) O o[R];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[r] = rounded<O>(fmaf(p.alpha, y[r] * b0 * b1, bias[r]));
-          O* to = (O*)p.out + query * p.ld + row;
-          if (p.whole && row + 4 <= p.n) {
-            if constexpr (sizeof(O) == 4)
-              *(uint4*)to = *(const uint4*)o;
-            else
-              *(uint2*)to = *(const uint2*)o;
+          for (int r = 0; r < R; ++r) o[r] = rounded<O>(fmaf(p.alpha, y[r] * k0 * k1, bias[r]));
+          O* to = (O*)p.out + slice * p.ld_slice + query * p.ld + row;
+          if (p.whole && row + R <= p.n) {
+            constexpr int B = R * sizeof(O) >= 16 ? 16 : 8;
+#pragma unroll
+            for (int i = 0; i < (int)(R * sizeof(O)) / B; ++i) {
+              if constexpr (B == 16)
+                ((uint4*)to)[i] = ((const uint4*)o)[i];
+              else
+                ((uint2*)to)[i] = ((const uint2*)o)[i];
+            }
           } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < R; ++r)
               if (row + r < p.n) to[r] = o[r];
           }
         }
@@ -483,6 +546,39 @@ __global__ void __launch_bounds__(Layout<NT, G>::kThreads, 1) score4_kernel(cons
   if (!ok)
     for (uint32_t i = 0; i < p.depth; ++i)
       if (pending >> i & 1u) wait(bars + 8 * i, phases >> i & 1u);
+}
+
+// Scores from the slices' sums, in order: four at a time, pitch ld_slice / nq a multiple of 4.
+struct Join {
+  const float* part;
+  uint64_t ld, ld_slice;  // of the sums
+  uint32_t slices;
+  uint64_t nq, n;
+  float alpha;
+  const float* bias;
+  void* out;
+  uint64_t ld_out;
+};
+template <typename O>
+__global__ void __launch_bounds__(256) join_kernel(const Join p) {
+  after_previous();
+  const uint64_t per = (p.n + 3) / 4, total = p.nq * per;
+  for (uint64_t u = (uint64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += (uint64_t)gridDim.x * 256) {
+    const uint64_t q = u / per, j = 4 * (u - q * per);
+    const float* from = p.part + q * p.ld + j;
+    float4 v = *(const float4*)from;
+    for (uint32_t s = 1; s < p.slices; ++s) {
+      const float4 x = *(const float4*)(from + s * p.ld_slice);
+      v.x += x.x;
+      v.y += x.y;
+      v.z += x.z;
+      v.w += x.w;
+    }
+    const float y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (j + r < p.n) ((O*)p.out)[q * p.ld_out + j + r] = rounded<O>(fmaf(p.alpha, y[r], p.bias ? p.bias[j + r] : 0.f));
+  }
 }
 
 }  // namespace raven_score4
