@@ -38,31 +38,21 @@ struct Params {
   const float *repetition, *presence, *frequency;
   float repetition_all, presence_all, frequency_all;
   uint32_t tile;    // columns of a CTA
-  uint64_t tiles;   // of a row
+  uint32_t tiles;   // of a row
   int* status;
 };
 
-constexpr uint32_t kHits = 2048;  // seen ids of a tile that are kept between the scan and the counts
-constexpr int kBatch = 4;         // vectors of a thread that are read together
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kMostPlaces = 8192;  // of a tile
+constexpr uint32_t kHits = 2048;        // seen ids of a tile that are kept between the scan and the counts
+constexpr uint32_t kBatch = 4;          // vectors of a thread that are read together
 
-// Shared memory of a tile: a count per column, a bit per column that says whether
-// its count is there, the ids found.
-__host__ __device__ inline uint32_t shared_bytes(uint32_t tile) { return tile * 4 + tile / 8 + kHits * 2; }
-
-template <typename T, int V>
-__device__ inline void put(T* to, const float (&v)[V]) {
-  __align__(16) T o[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    if constexpr (sizeof(T) == 4)
-      o[k] = v[k];
-    else if constexpr (std::is_same<T, __half>::value)
-      o[k] = __float2half_rn(v[k]);
-    else
-      o[k] = __float2bfloat16_rn(v[k]);
-  }
-  *(uint4*)to = *(const uint4*)o;
+// Shared memory of a tile: a word per place (how often it was seen, then its
+// finished score), per 32 places which were seen and which are hidden, the ids found.
+__host__ __device__ inline uint32_t shared_bytes(uint32_t tile, bool seen) {
+  return tile / 4 + (seen ? tile * 4 + kHits * 2 : 0);
 }
+
 template <typename T>
 __device__ inline T one(float v) {
   if constexpr (sizeof(T) == 4)
@@ -72,79 +62,114 @@ __device__ inline T one(float v) {
   else
     return __float2bfloat16_rn(v);
 }
+// A score as its bits, in the low half of a word where it has 16.
+template <typename T>
+__device__ inline uint32_t bits_of(T v) {
+  if constexpr (sizeof(T) == 4)
+    return __float_as_uint(v);
+  else
+    return *(const uint16_t*)&v;
+}
+
+// 16 bytes of scores as four words: what is done to them.
+template <typename T>
+struct Vector {
+  static constexpr uint32_t V = 16 / sizeof(T);
+  uint32_t w[4];
+
+  // V values from b[S] on; each sum is rounded to f32 and to the type.
+  template <int S>
+  __device__ void add(const float* from) {
+    const float* b = from + S;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        w[j] = __float_as_uint(__fadd_rn(__uint_as_float(w[j]), b[j]));
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const float2 v = __half22float2(*(const __half2*)&w[j]);
+        const __half2 r = __floats2half2_rn(__fadd_rn(v.x, b[2 * j]), __fadd_rn(v.y, b[2 * j + 1]));
+        w[j] = *(const uint32_t*)&r;
+      } else {
+        const float x = __uint_as_float(w[j] << 16), y = __uint_as_float(w[j] & 0xffff0000u);
+        const __nv_bfloat162 r = __floats2bfloat162_rn(__fadd_rn(x, b[2 * j]), __fadd_rn(y, b[2 * j + 1]));
+        w[j] = *(const uint32_t*)&r;
+      }
+    }
+  }
+  __device__ void set(uint32_t k, uint32_t bits) {  // k: known when compiled
+    if constexpr (sizeof(T) == 4)
+      w[k] = bits;
+    else
+      w[k / 2] = __byte_perm(w[k / 2], bits, k & 1 ? 0x5410 : 0x3254);
+  }
+  // Places whose bit is set become `bits` (two of them a word where they have 16).
+  __device__ void hide(uint32_t hidden, uint32_t bits) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        if (hidden >> j & 1u) w[j] = bits;
+      } else {
+        // the two bits at the tops of two bytes, each copied over half a word
+        uint32_t m;
+        asm("prmt.b32 %0, %1, 0, 0x9988;" : "=r"(m) : "r"((hidden >> (2 * j) & 3u) * 0x4080u));
+        w[j] = (w[j] & ~m) | (bits & m);
+      }
+    }
+  }
+};
 
 // A CTA takes a tile of a row, 16 bytes a thread at a time. Rows may start
-// anywhere: columns are counted from the last 16-byte boundary before the row
-// (`shift` columns before its first), so that vectors are whole but for the row's
-// ends. What it has beside the scores (bias, filter) is read at any alignment.
+// anywhere: places are counted from the last 16-byte boundary before the row (its
+// first column is place `shift`), so that vectors are whole but for the row's ends.
+// What it has beside the scores (bias, filter) is read at any alignment.
 //
-// How often each column was seen is counted in shared memory: one scan over the
-// history keeps the ids within the tile (16 bits each), their counts are set to 0,
-// then counted; a bit per column says which counts are there, so that no table is
-// cleared and columns that were not seen cost a bit of a word.
+// What a query has seen is worked out before: one scan over the history keeps the
+// ids within the tile (16 bits each), their counts are set to 0, then counted; a
+// bit per place says which counts are there, so that no table is cleared. Then each
+// id's score takes the place of its count. Scores that were not seen cost a bit of a
+// word, and the division is done for seen ones alone (where each thread did it for
+// its own vectors, a warp took the branch for nearly every one: 256 x 250007 bf16
+// 216 us). The first vectors are on their way meanwhile.
 template <typename T, bool LARGEST>
-__global__ void __launch_bounds__(256) adjust_kernel(const Params p) {
-  constexpr int V = 16 / sizeof(T);
-  extern __shared__ uint32_t shared[];
+__global__ void __launch_bounds__(kThreads, 4) adjust_kernel(const Params p) {
+  constexpr uint32_t V = 16 / sizeof(T);
+  extern __shared__ uint2 shared[];
   __shared__ uint32_t found;
-  uint32_t* count = shared;
-  uint32_t* mark = shared + p.tile;
-  uint16_t* hits = (uint16_t*)(mark + p.tile / 32);
+  uint2* bits = shared;  // x: seen, y: hidden
+  uint32_t* count = (uint32_t*)(bits + p.tile / 32);  // then the bits of a score
+  uint16_t* hits = (uint16_t*)(count + p.tile);
   after_previous();
-  const uint64_t row = blockIdx.x / p.tiles;
+  const uint32_t row = blockIdx.x / p.tiles;  // 32-bit: the 64-bit division took as long as a vector
   const T* x = (const T*)p.x + row * p.ld;
   T* out = (T*)p.out + row * p.ld_out;
   const uint32_t shift = (uint32_t)((uintptr_t)x % 16 / sizeof(T));
-  // columns [c0, c0 + tile) of the row, c0 <= 0 in the first tile
-  const int64_t c0 = (int64_t)(blockIdx.x - row * p.tiles) * p.tile - shift;
-  if (c0 >= (int64_t)p.n) return;  // a row that needs no last tile
-  bool some = false;
+  x -= shift;
+  out -= shift;
+  // places [first, last) of the row, of which the tile has those from t0 on
+  const uint32_t first = shift, last = (uint32_t)p.n + shift, t0 = (blockIdx.x - row * p.tiles) * p.tile;
+  if (t0 >= last) return;  // a row that needs no last tile
+  const uint32_t worst = bits_of(one<T>(LARGEST ? -INFINITY : INFINITY)) * (V == 8 ? 0x10001u : 1u);
+  const bool inner = t0 >= first + 4 && t0 + p.tile + 4 <= last;  // the row's ends, and what is beside them, are elsewhere
+  int64_t a = 0, b = 0;
   if (p.seen) {
-    for (uint32_t i = threadIdx.x; i < p.tile / 32; i += 256) mark[i] = 0;
-    if (threadIdx.x == 0) found = 0;
-    int64_t a = p.starts[row], b = p.starts[row + 1];
-    if (a < 0 || b < a || (uint64_t)b > p.seen_total) {
-      if (threadIdx.x == 0) raven_score::tell(p.status, kStatusOffsets);
-      a = b = 0;
-    }
-    // an id's place in the tile is below `cols` where the tile has it, at least `from` where the row has it
-    const uint32_t cols = (uint32_t)min((int64_t)p.tile, (int64_t)p.n - c0), from = c0 < 0 ? shift : 0;
-    const bool first = c0 <= 0 && p.tile + c0 > 0;
-    auto place = [&](int32_t id) { return (uint32_t)((int64_t)id - c0); };
-    __syncthreads();
-#pragma unroll 4
-    for (int64_t i = a + threadIdx.x; i < b; i += 256) {
-      const int32_t id = p.seen[i];
-      const uint32_t at = place(id);
-      if (first && id >= 0 && (uint32_t)id >= p.n) raven_score::tell(p.status, kStatusIds);
-      if (id >= 0 && at < cols && at >= from) {
-        const uint32_t k = atomicAdd(&found, 1u);
-        if (k < kHits) hits[k] = (uint16_t)at;
-        count[at] = 0;
-      }
-    }
-    __syncthreads();
-    const uint32_t n = found;
-    some = n > 0;
-    auto add = [&](uint32_t at) {
-      atomicAdd(&count[at], 1u);
-      atomicOr(&mark[at / 32], 1u << (at % 32));
-    };
-    if (n <= kHits) {
-      for (uint32_t i = threadIdx.x; i < n; i += 256) add(hits[i]);
-    } else {
-      for (int64_t i = a + threadIdx.x; i < b; i += 256) {
-        const int32_t id = p.seen[i];
-        const uint32_t at = place(id);
-        if (id >= 0 && at < cols && at >= from) add(at);
-      }
-    }
-    if (some) __syncthreads();
+    a = p.starts[row];
+    b = p.starts[row + 1];
   }
-  const float rep = p.repetition ? p.repetition[row] : p.repetition_all;
-  const float pre = p.presence ? p.presence[row] : p.presence_all;
-  const float freq = p.frequency ? p.frequency[row] : p.frequency_all;
-  const float* bias = p.bias ? p.bias + row * p.ld_bias : nullptr;
+  const float* bias = p.bias ? p.bias + row * p.ld_bias - shift : nullptr;  // of place 0
+  const uint32_t skew = (uint32_t)((uintptr_t)bias / 4 % 4);                // of a vector's first bias from 16 bytes
+  // The scores of the thread's first vectors are on their way from here on.
+  uint4 raw[kBatch];
+  auto read = [&](auto in, uint32_t l0) {
+#pragma unroll
+    for (uint32_t i = 0; i < kBatch; ++i) {
+      const uint32_t l = l0 + i * kThreads * V, c = t0 + l;
+      if (l < p.tile && (decltype(in)::value || (c >= first && c + V <= last))) raw[i] = *(const uint4*)(x + c);
+    }
+  };
+  if (inner)
+    read(std::true_type(), threadIdx.x * V);
+  else
+    read(std::false_type(), threadIdx.x * V);
   const uint32_t* allow = nullptr;
   bool none = false;
   if (p.allow) {
@@ -153,93 +178,164 @@ __global__ void __launch_bounds__(256) adjust_kernel(const Params p) {
     if (none && threadIdx.x == 0) raven_score::tell(p.status, kStatusIds);
     if (f >= 0 && !none) allow = p.allow + f * p.ld_allow;
   }
-  constexpr float kHidden = LARGEST ? -INFINITY : INFINITY;
-  auto seen_before = [&](float v, uint32_t at) {
-    const float by = __fadd_rn(pre, __fmul_rn(freq, (float)count[at]));
-    v = (v > 0.f) == LARGEST ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-    return LARGEST ? __fsub_rn(v, by) : __fadd_rn(v, by);
-  };
-  const bool same = (uintptr_t)x % 16 == (uintptr_t)out % 16;
-  const uint32_t skew = bias ? (uint32_t)(((uintptr_t)bias / 4 + 4 - shift % 4) % 4) : 0;  // of the bias of a vector's first column
-  for (uint32_t l0 = threadIdx.x * V; l0 < p.tile; l0 += 256 * V * kBatch) {
-    uint4 raw[kBatch];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const uint32_t l = l0 + i * 256 * V;
-      const int64_t c = c0 + l;
-      if (l < p.tile && c >= 0 && c + V <= (int64_t)p.n) raw[i] = *(const uint4*)(x + c);
+  for (uint32_t i = threadIdx.x; i < p.tile / 32; i += kThreads) {
+    uint32_t hidden = none ? ~0u : 0u;
+    if (allow) {
+      // places from t0 + 32 i on are columns from c on: the bits of two words
+      const int64_t c = (int64_t)t0 + 32 * i - shift;
+      const int64_t w = c >> 5, words = ((int64_t)p.n + 31) / 32;
+      const uint32_t a = w >= 0 && w < words ? allow[w] : 0, b = (c & 31) && w + 1 < words ? allow[w + 1] : 0;
+      hidden = ~__funnelshift_r(a, b, (uint32_t)c & 31);
     }
+    bits[i] = make_uint2(0, hidden);
+  }
+  if (threadIdx.x == 0) found = 0;
+  __syncthreads();
+  if (p.seen) {
+    if (a < 0 || b < a || (uint64_t)b > p.seen_total) {
+      if (threadIdx.x == 0) raven_score::tell(p.status, kStatusOffsets);
+      a = b = 0;
+    }
+    const uint32_t ends = min(p.tile, last - t0);
+    // false for what is no column of the tile; `at`: its place there
+    auto within = [&](int32_t id, uint32_t& at) {
+      at = (uint32_t)id + shift - t0;
+      return id >= 0 && (uint32_t)id < (uint32_t)p.n && at < ends;
+    };
+    constexpr int kIds = 8;  // of a thread at once
+    for (int64_t i0 = a + threadIdx.x; i0 < b; i0 += kIds * kThreads) {
+      int32_t id[kIds];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const uint32_t l = l0 + i * 256 * V;
-      const int64_t c = c0 + l;
-      if (l >= p.tile || c >= (int64_t)p.n || c + V <= 0) continue;
-      const uint32_t marks = some ? mark[l / 32] >> (l % 32) & ((1u << V) - 1) : 0;
-      if (c >= 0 && c + V <= (int64_t)p.n) {
-        float v[V];
-        const T* r = (const T*)&raw[i];
+      for (int k = 0; k < kIds; ++k) id[k] = i0 + k * kThreads < b ? p.seen[i0 + k * kThreads] : -1;
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = raven_fp8::load_value(r + k);
-        if (marks) {
-#pragma unroll
-          for (int k = 0; k < V; ++k)
-            if (marks >> k & 1u) v[k] = seen_before(v[k], l + k);
-        }
-        if (bias) {
-          // from the 16 bytes that hold the first one on; at the ends one by one
-          if (c >= 4 && c + V + 4 <= (int64_t)p.n) {
-            float b[V + 4];
-            const float4* from = (const float4*)(bias + c - skew);
-#pragma unroll
-            for (int k = 0; k < V / 4; ++k) ((float4*)b)[k] = from[k];
-            if (skew) ((float4*)b)[V / 4] = from[V / 4];
-            auto shifted = [&](auto s) {
-#pragma unroll
-              for (int k = 0; k < V; ++k) v[k] = __fadd_rn(v[k], b[k + decltype(s)::value]);
-            };
-            if (skew == 0)
-              shifted(std::integral_constant<int, 0>());
-            else if (skew == 1)
-              shifted(std::integral_constant<int, 1>());
-            else if (skew == 2)
-              shifted(std::integral_constant<int, 2>());
-            else
-              shifted(std::integral_constant<int, 3>());
-          } else {
-#pragma unroll
-            for (int k = 0; k < V; ++k) v[k] = __fadd_rn(v[k], bias[c + k]);
-          }
-        }
-        if (allow) {
-          const uint64_t w = (uint64_t)c / 32, w1 = ((uint64_t)c + V - 1) / 32;
-          const uint32_t lo = allow[w], bits = __funnelshift_r(lo, w1 != w ? allow[w1] : lo, (uint32_t)c % 32);
-#pragma unroll
-          for (int k = 0; k < V; ++k)
-            if (!(bits >> k & 1u)) v[k] = kHidden;
-        }
-        if (none) {
-#pragma unroll
-          for (int k = 0; k < V; ++k) v[k] = kHidden;
-        }
-        if (same) {
-          put<T, V>(out + c, v);
-        } else {
-#pragma unroll
-          for (int k = 0; k < V; ++k) out[c + k] = one<T>(v[k]);
-        }
-      } else {
-        for (int k = 0; k < V; ++k) {
-          const int64_t e = c + k;
-          if (e < 0 || e >= (int64_t)p.n) continue;
-          float v = raven_fp8::load_value(x + e);
-          if (marks >> k & 1u) v = seen_before(v, l + k);
-          if (bias) v = __fadd_rn(v, bias[e]);
-          if (none || (allow && !(allow[e / 32] >> (e % 32) & 1u))) v = kHidden;
-          out[e] = one<T>(v);
+      for (int k = 0; k < kIds; ++k) {
+        uint32_t at;
+        if (within(id[k], at)) {
+          const uint32_t h = atomicAdd(&found, 1u);
+          if (h < kHits) hits[h] = (uint16_t)at;
+          count[at] = 0;
+        } else if (t0 == 0 && id[k] >= 0 && (uint32_t)id[k] >= (uint32_t)p.n) {
+          raven_score::tell(p.status, kStatusIds);
         }
       }
     }
+    __syncthreads();
+    const uint32_t n = found;
+    if (n) {
+      auto add = [&](uint32_t at) {
+        atomicAdd(&count[at], 1u);
+        atomicOr(&bits[at / 32].x, 1u << (at % 32));
+      };
+      if (n <= kHits) {
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) add(hits[i]);
+      } else {
+        for (int64_t i = a + threadIdx.x; i < b; i += kThreads) {
+          uint32_t at;
+          if (within(p.seen[i], at)) add(at);
+        }
+      }
+      __syncthreads();
+      const float rep = p.repetition ? p.repetition[row] : p.repetition_all;
+      const float pre = p.presence ? p.presence[row] : p.presence_all;
+      const float freq = p.frequency ? p.frequency[row] : p.frequency_all;
+      auto worse = [&](uint32_t at) {
+        const float v = raven_fp8::load_value(x + t0 + at);
+        const float by = __fadd_rn(pre, __fmul_rn(freq, (float)count[at]));
+        float y = (v > 0.f) == LARGEST ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+        y = LARGEST ? __fsub_rn(y, by) : __fadd_rn(y, by);
+        return bits_of(one<T>(bias ? __fadd_rn(y, bias[t0 + at]) : y));
+      };
+      if (n <= kHits) {
+        uint32_t y[kHits / kThreads];  // an id that is there twice: both read its count before either writes
+#pragma unroll
+        for (uint32_t i = 0; i < kHits / kThreads; ++i)
+          if (threadIdx.x + kThreads * i < n) y[i] = worse(hits[threadIdx.x + kThreads * i]);
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < kHits / kThreads; ++i)
+          if (threadIdx.x + kThreads * i < n) count[hits[threadIdx.x + kThreads * i]] = y[i];
+      } else {
+#pragma unroll 8
+        for (uint32_t at = threadIdx.x; at < p.tile; at += kThreads)
+          if (bits[at / 32].x >> (at % 32) & 1u) count[at] = worse(at);
+      }
+      __syncthreads();
+    }
   }
+  const bool same = (uintptr_t)x % 16 == (uintptr_t)out % 16;
+  // IN: all the tile's places are the row's, and so are four more on either side.
+  auto finish = [&](auto in) {
+    constexpr bool IN = decltype(in)::value;
+    for (uint32_t l0 = threadIdx.x * V; l0 < p.tile; l0 += kBatch * kThreads * V) {
+      if (l0 >= kBatch * kThreads * V) read(in, l0);
+      // Biases of two vectors are read before either is written: the compiler cannot know that they lie apart.
+#pragma unroll
+      for (uint32_t i0 = 0; i0 < kBatch; i0 += 2) {
+        float b[2][V + 4];
+        if (bias) {
+#pragma unroll
+          for (uint32_t h = 0; h < 2; ++h) {
+            const uint32_t l = l0 + (i0 + h) * kThreads * V, c = t0 + l;
+            if (l >= p.tile || (!IN && (c < first || c + V > last))) continue;
+            if (IN || (c >= first + 4 && c + V + 4 <= last)) {
+              // the 16 bytes that hold the first one, and those after them
+              const float4* from = (const float4*)(bias + c - skew);
+#pragma unroll
+              for (uint32_t k = 0; k < V / 4; ++k) ((float4*)b[h])[k] = from[k];
+              if (skew) ((float4*)b[h])[V / 4] = from[V / 4];
+            } else {
+#pragma unroll
+              for (uint32_t k = 0; k < V + 4; ++k) b[h][k] = k >= skew && k < skew + V ? bias[c + k - skew] : 0.f;
+            }
+          }
+        }
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+          const uint32_t l = l0 + (i0 + h) * kThreads * V, c = t0 + l;
+          if (l >= p.tile || (!IN && c >= last)) continue;
+          const uint2 m = bits[l / 32];
+          const uint32_t seen = m.x >> (l % 32) & ((1u << V) - 1), hidden = m.y >> (l % 32);
+          if (IN || (c >= first && c + V <= last)) {
+            Vector<T> v{{raw[i0 + h].x, raw[i0 + h].y, raw[i0 + h].z, raw[i0 + h].w}};
+            if (bias) {
+              if (skew == 0)
+                v.template add<0>(b[h]);
+              else if (skew == 1)
+                v.template add<1>(b[h]);
+              else if (skew == 2)
+                v.template add<2>(b[h]);
+              else
+                v.template add<3>(b[h]);
+            }
+            if (seen) {
+#pragma unroll
+              for (uint32_t k = 0; k < V; ++k)
+                if (seen >> k & 1u) v.set(k, count[l + k]);
+            }
+            if (p.allow) v.hide(hidden, worst);
+            if (same) {
+              *(uint4*)(out + c) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+            } else {
+#pragma unroll
+              for (uint32_t k = 0; k < V; ++k) out[c + k] = ((const T*)v.w)[k];
+            }
+          } else {
+            for (uint32_t k = 0; k < V; ++k)
+              if (c + k >= first && c + k < last) {
+                const float f = raven_fp8::load_value(x + c + k);
+                T o = one<T>(bias ? __fadd_rn(f, bias[c + k]) : f);
+                if (seen >> k & 1u) o = *(const T*)&count[l + k];
+                out[c + k] = hidden >> k & 1u ? *(const T*)&worst : o;
+              }
+          }
+        }
+      }
+    }
+  };
+  if (inner)
+    finish(std::true_type());
+  else
+    finish(std::false_type());
 }
 
 }  // namespace raven_adjust

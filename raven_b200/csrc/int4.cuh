@@ -43,6 +43,12 @@ __device__ inline uint32_t word_at(uint32_t i, uint32_t units) {
   return 16 * block + min(4u, units - 4 * block) * quarter + unit;
 }
 
+// Row `row` at a pitch: one multiply-add.
+template <typename T>
+__device__ inline T* row_at(T* base, uint32_t row, uint32_t pitch) {
+  return base + (uint64_t)row * pitch;
+}
+
 __device__ inline float step_of(uint32_t word) { return __uint_as_float(word & 0xffffff00u); }
 // z: as the low bits of an f32 of 2^23, offset by 128
 __device__ inline float zero_of(uint32_t word) { return __uint_as_float((word & 0xffu) ^ 0x4b000080u) - 8388736.f; }
@@ -79,11 +85,11 @@ __global__ void __launch_bounds__(256) claim_kernel(const int32_t* slots, uint32
 
 struct Write {
   const void* x;
-  uint64_t m, ld;          // rows and their pitch in values
+  uint32_t m, ld;          // rows and their pitch in values
   uint32_t dim, group, units;
   uint8_t* codes;
   uint32_t* words;
-  uint64_t n, ld_codes, ld_words;  // rows held, pitches in bytes and words
+  uint32_t n, ld_codes, ld_words;  // rows held, pitches in bytes and words
   const int32_t* slots;    // null: row i is held as row i
   const Claim* table;      // null: few rows
   uint32_t bits;
@@ -123,6 +129,33 @@ __device__ inline float reciprocal(float x) {
   return r;
 }
 
+// The codes of eight values: rint(x / step) - z, at most 15, the first lowest.
+// The quotient has to be x / step rounded to f32: of values that differ from a
+// border between two codes (a multiple of step / 2 of up to 24 bits, so an f32) it
+// lies on the right side of it then, and on it for those that do not, which go to
+// the even code. q = x * inv is off by a unit or two in its last place; its
+// remainder is exact (18 bits), and what that adds is off by 2^-22 of such a unit,
+// where a value next to a border is at least 2^-17 of one further from it than half
+// a unit. Rounding is adding 1.5 * 2^23, whose low bits are then the whole number;
+// sums of them, 4 bits apart, are a word of codes (mod 2^32). Steps are whole
+// numbers of up to 16 bits times a power of two.
+__device__ inline uint32_t codes_of(float (&x)[8], float step, int z) {
+  if (step < 0x1p-80f) {  // remainders and reciprocals stay within f32's range; all values are below 2^-73
+    step *= 0x1p64f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] *= 0x1p64f;
+  }
+  constexpr float kRound = 12582912.f;
+  const float inv = reciprocal(step), most = kRound + (float)(z + 15);
+  uint32_t word = 0u - (0x4b400000u + (uint32_t)z) * 0x11111111u;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float q = x[k] * inv, t = fmaf(fmaf(-q, step, x[k]), inv, q) + kRound;
+    word += __float_as_uint(fminf(t, most)) << (4 * k);
+  }
+  return word;
+}
+
 // A lane takes eight values (two 16-byte loads of f32, one of 16-bit types), the
 // L = group / 8 lanes of a group share its range by shuffles, and of four such
 // pieces at once every group's word is worked out by a lane of its own (64-bit
@@ -138,44 +171,18 @@ __global__ void __launch_bounds__(256, 3) write_kernel(const Write p) {
   const uint32_t ng = (p.dim + G - 1) / G, lane = threadIdx.x & 31;
   const uint32_t wide = (p.dim + kBlock - 1) / kBlock * (kBlock / G);  // words of a row as it is held
   for (uint64_t r0 = (uint64_t)blockIdx.x * p.run; r0 < p.m; r0 += (uint64_t)gridDim.x * p.run) {
-    const uint32_t rows = (uint32_t)min((uint64_t)p.run, p.m - r0);
-    if (threadIdx.x < rows) {
-      int64_t s = p.slots ? (int64_t)p.slots[r0 + threadIdx.x] : (int64_t)(r0 + threadIdx.x);
-      if (s >= (int64_t)p.n) {
-        raven_score::tell(p.status, kStatusIds);
-        s = -1;
-      }
-      if (s >= 0 && p.table) {
-        uint32_t h = claim_hash((uint32_t)s) >> (32 - p.bits);
-        for (uint32_t tries = 0; tries >> p.bits == 0 && p.table[h].slot != (uint32_t)s; ++tries)
-          h = (h + 1) & ((1u << p.bits) - 1);
-        if (p.table[h].row != (int32_t)(r0 + threadIdx.x)) s = -1;
-      }
-      dest[threadIdx.x] = s < 0 ? -1 : (int32_t)s;
-      later[threadIdx.x] = 0;
-    }
-    __syncthreads();
-    if (p.slots && !p.table) {
-      for (uint64_t j = r0 + 1 + threadIdx.x; j < p.m; j += 256) {
-        const int32_t s = p.slots[j];
-        for (uint32_t k = 0; k < rows && r0 + k < j; ++k)
-          if (dest[k] == s) later[k] = 1;
-      }
-      __syncthreads();
-    }
-    const uint32_t items = rows * p.per;
-    for (uint32_t u0 = 0; u0 < items; u0 += 256 * kItems) {
-      float x[kItems][8], lo[kItems], hi[kItems];
-      int32_t to[kItems];
-      uint32_t at[kItems];
-      bool odd[kItems];
+    const uint32_t rows = (uint32_t)min((uint64_t)p.run, p.m - r0), items = rows * p.per;
+    float x[kItems][8];
+    uint32_t from[kItems], at[kItems];  // a piece's row of the run, which of its eights
+    auto load = [&](uint32_t u0) {
 #pragma unroll
       for (int n = 0; n < kItems; ++n) {
-        const uint32_t u = u0 + n * 256 + threadIdx.x, r = divided(u, p.magic), i = u - r * p.per, d = 8 * i;
-        to[n] = u < items && !later[r] ? dest[r] : -1;
-        at[n] = i;
-        if (to[n] >= 0) {
-          const T* row = (const T*)p.x + (r0 + r) * p.ld;
+        const uint32_t u = u0 + n * 256 + threadIdx.x;
+        from[n] = divided(u, p.magic);
+        at[n] = u - from[n] * p.per;
+        const uint32_t d = 8 * at[n];
+        if (u < items) {
+          const T* row = row_at((const T*)p.x, (uint32_t)r0 + from[n], p.ld);
           if (VEC && d + 8 <= p.dim) {
             __align__(16) T raw[8];
             ((uint4*)raw)[0] = *(const uint4*)(row + d);
@@ -196,17 +203,52 @@ __global__ void __launch_bounds__(256, 3) write_kernel(const Write p) {
           for (int k = 0; k < 8; ++k) x[n][k] = 0.f;
         }
       }
+    };
+    load(0);  // on the way while the slots are settled
+    if (threadIdx.x < rows) {
+      int64_t s = p.slots ? (int64_t)p.slots[r0 + threadIdx.x] : (int64_t)(r0 + threadIdx.x);
+      if (s >= (int64_t)p.n) {
+        raven_score::tell(p.status, kStatusIds);
+        s = -1;
+      }
+      if (s >= 0 && p.table) {
+        uint32_t h = claim_hash((uint32_t)s) >> (32 - p.bits);
+        for (uint32_t tries = 0; tries >> p.bits == 0; ++tries) {
+          const Claim c = p.table[h];
+          if (c.slot == (uint32_t)s) {
+            if (c.row != (int32_t)(r0 + threadIdx.x)) s = -1;
+            break;
+          }
+          h = (h + 1) & ((1u << p.bits) - 1);
+        }
+      }
+      dest[threadIdx.x] = s < 0 ? -1 : (int32_t)s;
+      later[threadIdx.x] = 0;
+    }
+    __syncthreads();
+    if (p.slots && !p.table) {
+      for (uint64_t j = r0 + 1 + threadIdx.x; j < p.m; j += 256) {
+        const int32_t s = p.slots[j];
+        for (uint32_t k = 0; k < rows && r0 + k < j; ++k)
+          if (dest[k] == s) later[k] = 1;
+      }
+      __syncthreads();
+    }
+    for (uint32_t u0 = 0; u0 < items; u0 += 256 * kItems) {
+      if (u0) load(u0);
+      float lo[kItems], hi[kItems];
+      bool odd[kItems];
 #pragma unroll
       for (int n = 0; n < kItems; ++n) {
-        uint32_t top = 0;
+        float not_finite = 0.f;  // NaN after an infinity or a NaN
         lo[n] = hi[n] = x[n][0];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          top = max(top, __float_as_uint(x[n][k]) & 0x7fffffffu);
+          not_finite = fmaf(x[n][k], 0.f, not_finite);
           lo[n] = fminf(lo[n], x[n][k]);
           hi[n] = fmaxf(hi[n], x[n][k]);
         }
-        const uint32_t votes = __ballot_sync(0xffffffffu, top >= 0x7f800000u);
+        const uint32_t votes = __ballot_sync(0xffffffffu, not_finite != 0.f);
         odd[n] = votes >> (lane & ~(L - 1)) & ((1u << L) - 1);
 #pragma unroll
         for (int o = L / 2; o > 0; o >>= 1) {
@@ -229,35 +271,18 @@ __global__ void __launch_bounds__(256, 3) write_kernel(const Write p) {
 #pragma unroll
       for (int n = 0; n < kItems; ++n) {
         uint32_t w = __shfl_sync(0xffffffffu, scale, n * kGroups + lane / L);
-        if (to[n] < 0) continue;
         const uint32_t i = at[n], d = 8 * i;
+        const int32_t to = u0 + n * 256 + threadIdx.x < items && !later[from[n]] ? dest[from[n]] : -1;
+        if (to < 0) continue;
         uint32_t word = 0;
         if (odd[n]) {
           w = kNaN;
         } else if (w & ~255u) {
-          const float step = step_of(w), inv = reciprocal(step);
-          const int z = (int)(int8_t)(w & 0xffu);
-          uint32_t near = 0;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            // x * inv is off by less than 2^-15 here (infinite or NaN for the smallest steps): next to a border the
-            // quotient itself decides. It is an f32 rounded once, and a value and a border that differ do so by more
-            // than its rounding.
-            // Rounding by adding 1.5 * 2^23, whose low bits are then the whole number.
-            const float q = x[n][k] * inv, t = q + 12582912.f;
-            near |= !(fabsf(q - (t - 12582912.f)) < 0.5f - 0x1p-12f) ? 1u << k : 0u;
-            const int c = min(max(__float_as_int(t) - 0x4b400000 - z, 0), 15);
-            word |= d + k < p.dim ? (uint32_t)c << (4 * k) : 0u;
-          }
-          if (near) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if ((near >> k & 1u) && d + k < p.dim)
-                word = (word & ~(15u << (4 * k))) | (uint32_t)min((int)rintf(__fdiv_rn(x[n][k], step)) - z, 15) << (4 * k);
-          }
+          word = codes_of(x[n], step_of(w), (int)(int8_t)(w & 0xffu));
+          if (d + 8 > p.dim) word &= d < p.dim ? (1u << (4 * (p.dim - d))) - 1 : 0u;
         }
-        if (i < 4 * p.units) *(uint32_t*)(p.codes + to[n] * p.ld_codes + 4 * word_at(i, p.units)) = word;
-        uint32_t* words = p.words + to[n] * p.ld_words;
+        if (i < 4 * p.units) *(uint32_t*)(row_at(p.codes, to, p.ld_codes) + 4 * word_at(i, p.units)) = word;
+        uint32_t* words = row_at(p.words, to, p.ld_words);
         if (i % L == 0) words[i / L] = w;
         if (i == 0)
           for (uint32_t g = ng; g < wide; ++g) words[g] = 0;
@@ -274,14 +299,14 @@ __global__ void __launch_bounds__(256, 3) write_kernel(const Write p) {
 struct Read {
   const uint8_t* codes;
   const uint32_t* words;
-  uint64_t n, ld_codes, ld_words;
+  uint32_t n, ld_codes, ld_words;
   uint32_t dim, group, units;
   const int32_t* ids;   // null: row i
-  uint64_t m;
+  uint32_t m;
   uint32_t run;         // rows of a CTA at once
   uint32_t per, magic;  // pieces of a row
   void* out;
-  uint64_t ld;
+  uint32_t ld;
   int* status;
 };
 
@@ -293,31 +318,38 @@ __global__ void __launch_bounds__(256) read_kernel(const Read p) {
   for (uint64_t r0 = (uint64_t)blockIdx.x * p.run; r0 < p.m; r0 += (uint64_t)gridDim.x * p.run) {
     const uint32_t rows = (uint32_t)min((uint64_t)p.run, p.m - r0), items = rows * p.per;
     for (uint32_t u0 = 0; u0 < items; u0 += 256 * kItems) {
-      uint32_t word[kItems], scale[kItems];
+      uint32_t word[kItems], scale[kItems], at[kItems], to_row[kItems];
+      int32_t from[kItems];
 #pragma unroll
       for (int n = 0; n < kItems; ++n) {
-        const uint32_t u = u0 + n * 256 + threadIdx.x, r = divided(u, p.magic), d = (u - r * p.per) * V;
+        const uint32_t u = u0 + n * 256 + threadIdx.x, r = divided(u, p.magic);
+        at[n] = (u - r * p.per) * V;
+        to_row[n] = (uint32_t)r0 + r;
+        from[n] = -1;
+        if (u < items) from[n] = p.ids ? p.ids[to_row[n]] : (int32_t)to_row[n];
+      }
+#pragma unroll
+      for (int n = 0; n < kItems; ++n) {
+        const uint32_t d = at[n];
         word[n] = scale[n] = 0;
-        if (u < items) {
-          const int64_t from = p.ids ? (int64_t)p.ids[r0 + r] : (int64_t)(r0 + r);
-          if (from >= 0 && from < (int64_t)p.n) {
-            scale[n] = p.words[from * p.ld_words + (d >> shift)];
-            word[n] = *(const uint32_t*)(p.codes + from * p.ld_codes + 4 * word_at(d / 8, p.units)) >> (4 * (d % 8));
-          } else if (from >= 0 && d == 0) {
-            raven_score::tell(p.status, kStatusIds);
-          }
+        if ((uint32_t)from[n] < p.n) {
+          scale[n] = row_at(p.words, from[n], p.ld_words)[d >> shift];
+          word[n] = *(const uint32_t*)(row_at(p.codes, from[n], p.ld_codes) + 4 * word_at(d / 8, p.units)) >> (4 * (d % 8));
+        } else if (from[n] >= 0 && d == 0) {
+          raven_score::tell(p.status, kStatusIds);
         }
       }
 #pragma unroll
       for (int n = 0; n < kItems; ++n) {
-        const uint32_t u = u0 + n * 256 + threadIdx.x, r = divided(u, p.magic), d = (u - r * p.per) * V;
-        if (u >= items) continue;
-        // code + z: the code as the low bits of 2^23, all exact
-        const float step = step_of(scale[n]), z = zero_of(scale[n]) - 8388608.f;
+        if (u0 + n * 256 + threadIdx.x >= items) continue;
+        const uint32_t d = at[n];
+        // code + z, exactly: four bits at place 4 k of an f32's significand are a code on top of 2^(23 - 4 k)
+        const float step = step_of(scale[n]), z = zero_of(scale[n]);
         __align__(16) T v[V];
 #pragma unroll
         for (uint32_t k = 0; k < V; ++k) {
-          const float f = (__uint_as_float((word[n] >> (4 * k) & 15u) | 0x4b000000u) + z) * step;
+          const uint32_t at = 4 * (k % 4), w = k < 4 ? word[n] : word[n] >> 16;
+          const float f = (__uint_as_float((w & (15u << at)) | (150u - at) << 23) + (z - (float)(8388608u >> at))) * step;
           if constexpr (sizeof(T) == 4)
             v[k] = f;
           else if constexpr (std::is_same<T, __half>::value)
@@ -325,7 +357,7 @@ __global__ void __launch_bounds__(256) read_kernel(const Read p) {
           else
             v[k] = __float2bfloat16_rn(f);
         }
-        T* to = (T*)p.out + (r0 + r) * p.ld + d;
+        T* to = row_at((T*)p.out, to_row[n], p.ld) + d;
         if (VEC && d + V <= p.dim) {
           *(uint4*)to = *(const uint4*)v;
         } else {

@@ -26,6 +26,8 @@ using raven_int4::kBlock;
 
 int kind_of(int32_t t) { return t == RAVEN_TYPE_F32 ? 0 : t == RAVEN_TYPE_F16 ? 1 : 2; }
 
+constexpr uint64_t kMaxPitch = 0xffffffffull;  // pitches are 32-bit factors
+
 int check_int4(const raven_rows* r, uint32_t dim, const char* what) {
   const std::string w(what);
   if (!r) return fail(RAVEN_EINVAL, w + ": null");
@@ -36,6 +38,7 @@ int check_int4(const raven_rows* r, uint32_t dim, const char* what) {
   if (!r->data || !r->exps) return fail(RAVEN_EINVAL, w + ": 4-bit rows need codes and scale words");
   if (!aligned(r->data, 16) || r->ld % 16 || r->ld < (dim + 31ull) / 32 * 16)
     return fail(RAVEN_EINVAL, w + ": 4-bit codes must start on 16 bytes, their pitch a multiple of 16 of at least dim / 2");
+  if (r->ld > kMaxPitch || r->ld_exps > kMaxPitch) return fail(RAVEN_ELIMIT, w + ": pitch of 2^32 and more");
   const uint64_t per = kBlock / group;
   if (!aligned(r->exps, 4 * per) || r->ld_exps % per || r->ld_exps < (dim + kBlock - 1ull) / kBlock * per)
     return fail(RAVEN_EINVAL, w + ": scale words must start on those of 128 values, their pitch a multiple of them");
@@ -51,13 +54,14 @@ uint32_t rows_at_once(uint64_t m, uint32_t per, int sms, uint32_t most, uint32_t
 
 template <typename T, uint32_t L, bool LANE>
 cudaError_t launch_write(raven_int4::Write p, int sms, cudaStream_t st) {
-  const bool vec = !LANE && p.ld * sizeof(T) % 16 == 0 && aligned(p.x, 16);
+  const bool vec = p.ld * sizeof(T) % 16 == 0 && aligned(p.x, 16);
   p.per = (p.dim + 8 * L - 1) / (8 * L) * L;
   p.run = rows_at_once(p.m, p.per, sms, raven_int4::kRun, &p.magic);
   const uint64_t grid = std::min<uint64_t>((p.m + p.run - 1) / p.run, (uint64_t)sms * 64);
   static Allowed none;
-  return launch(vec ? raven_int4::write_kernel<T, L, true, LANE> : raven_int4::write_kernel<T, L, false, LANE>, grid, 256, 0,
-                none, st, p);
+  if constexpr (!LANE)
+    if (vec) return launch(raven_int4::write_kernel<T, L, true, false>, grid, 256, 0, none, st, p);
+  return launch(raven_int4::write_kernel<T, L, false, LANE>, grid, 256, 0, none, st, p);
 }
 template <typename T, bool LANE>
 cudaError_t group_write(const raven_int4::Write& p, int sms, cudaStream_t st) {
@@ -76,16 +80,16 @@ int write_rows(const void* x, int32_t type, uint64_t m, uint32_t dim, uint64_t l
   if (int rc = sm_count(&sms)) return rc;
   raven_int4::Write p{};
   p.x = x;
-  p.m = m;
-  p.ld = ld;
+  p.m = (uint32_t)m;
+  p.ld = (uint32_t)ld;
   p.dim = dim;
   p.group = int4_group(out->type);
   p.units = (dim + 31) / 32;
   p.codes = (uint8_t*)out->data;
   p.words = (uint32_t*)out->exps;
-  p.n = out->rows;
-  p.ld_codes = out->ld;
-  p.ld_words = out->ld_exps;
+  p.n = (uint32_t)out->rows;
+  p.ld_codes = (uint32_t)out->ld;
+  p.ld_words = (uint32_t)out->ld_exps;
   p.slots = slots;
   p.status = status;
   raven_int4::Claim* table = nullptr;
@@ -239,9 +243,9 @@ cudaError_t dispatch_score4(const raven_rows* v, const raven_score4::Params& p, 
 template <typename T>
 cudaError_t launch_adjust(const raven_adjust::Params& p, bool largest, cudaStream_t st) {
   static Allowed none;
-  const uint32_t smem = p.seen ? raven_adjust::shared_bytes(p.tile) : 0;
-  return launch(largest ? raven_adjust::adjust_kernel<T, true> : raven_adjust::adjust_kernel<T, false>, p.nq * p.tiles, 256,
-                smem, none, st, p);
+  const uint32_t smem = raven_adjust::shared_bytes(p.tile, p.seen != nullptr);
+  return launch(largest ? raven_adjust::adjust_kernel<T, true> : raven_adjust::adjust_kernel<T, false>, p.nq * p.tiles,
+                raven_adjust::kThreads, smem, none, st, p);
 }
 
 __global__ void status_kernel(int* status) {
@@ -326,6 +330,7 @@ int raven_int4_write_device(const void* d_rows, int32_t type, uint64_t m, uint32
   if (m > (d_slots ? kMaxSlots : kMaxRows)) return fail(RAVEN_ELIMIT, "rows: more than 2^31 - 1, or 2^30 with slots");
   if (!d_rows) return fail(RAVEN_EINVAL, "rows: null");
   if (ld < dim) return fail(RAVEN_EINVAL, "rows: pitch below dim");
+  if (ld > kMaxPitch) return fail(RAVEN_ELIMIT, "rows: pitch of 2^32 and more");
   if (!aligned(d_rows, type_size(type))) return fail(RAVEN_EINVAL, "rows: not aligned to their type");
   if (!d_slots && m > out->rows) return fail(RAVEN_EINVAL, "out: fewer rows than are written");
   return write_rows(d_rows, type, m, dim, ld, false, d_slots, out, d_status, (cudaStream_t)stream);
@@ -342,22 +347,23 @@ int raven_int4_read_device(const raven_rows* rows, uint32_t dim, const int32_t* 
   if (m > kMaxRows) return fail(RAVEN_ELIMIT, "output: more than 2^31 - 1 rows");
   if (!d_out || !aligned(d_out, type_size(out_type))) return fail(RAVEN_EINVAL, "output: null or not aligned to its type");
   if (ld < dim) return fail(RAVEN_EINVAL, "output: pitch below dim");
+  if (ld > kMaxPitch) return fail(RAVEN_ELIMIT, "output: pitch of 2^32 and more");
   if (!d_ids && m > rows->rows) return fail(RAVEN_EINVAL, "rows: fewer than are read");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   raven_int4::Read p{};
   p.codes = (const uint8_t*)rows->data;
   p.words = (const uint32_t*)rows->exps;
-  p.n = rows->rows;
-  p.ld_codes = rows->ld;
-  p.ld_words = rows->ld_exps;
+  p.n = (uint32_t)rows->rows;
+  p.ld_codes = (uint32_t)rows->ld;
+  p.ld_words = (uint32_t)rows->ld_exps;
   p.dim = dim;
   p.group = raven_internal::int4_group(rows->type);
   p.units = (dim + 31) / 32;
   p.ids = d_ids;
-  p.m = m;
+  p.m = (uint32_t)m;
   p.out = d_out;
-  p.ld = ld;
+  p.ld = (uint32_t)ld;
   p.status = d_status;
   cudaStream_t st = (cudaStream_t)stream;
   CU(out_type == RAVEN_TYPE_F32   ? launch_read<float>(p, sms, st)
@@ -424,9 +430,9 @@ int raven_adjust_scores_device(const void* d_scores, int32_t type, uint64_t nq, 
   p.status = d_status;
   // the largest tiles, since each scans its row's history, that leave every SM four
   const uint64_t most = 16 / size - 1;  // columns before a row's first
-  p.tile = 8192;
+  p.tile = raven_adjust::kMostPlaces;
   while (p.tile > 1024 && nq * ((n + most + p.tile - 1) / p.tile) < 4ull * sms) p.tile /= 2;
-  p.tiles = (n + most + p.tile - 1) / p.tile;
+  p.tiles = (uint32_t)((n + most + p.tile - 1) / p.tile);
   if (nq * p.tiles > kMaxRows) return fail(RAVEN_ELIMIT, "scores: more tiles than a launch holds");
   cudaStream_t st = (cudaStream_t)stream;
   CU(type == RAVEN_TYPE_F32   ? launch_adjust<float>(p, largest != 0, st)
