@@ -13,6 +13,7 @@
 #include "adjust.cuh"
 #include "int4.cuh"
 #include "score4.cuh"
+#include "score4_wide.cuh"
 
 using namespace raven_launch;
 
@@ -129,16 +130,16 @@ cudaError_t launch_read(raven_int4::Read p, int sms, cudaStream_t st) {
 constexpr uint32_t kMostShared = 227 * 1024;
 constexpr uint64_t kOwnLayout = 16384;  // values that each CTA lays out for itself
 
-// Codes as boxes of up to 64 bytes (a block) x `rows` rows; what is past a row's end or the last row reads 0.
-bool codes_map(CUtensorMap* m, const raven_rows* v, uint32_t units, uint32_t rows) {
+// Codes as boxes of `wide` bytes (64: a block) x `rows` rows; what is past a row's end or the last row reads 0.
+bool codes_map(CUtensorMap* m, const raven_rows* v, uint32_t units, uint32_t wide, uint32_t rows, CUtensorMapSwizzle swizzle) {
   PFN_cuTensorMapEncodeTiled_v12000 f = raven_internal::encode_tiled();
   if (!f) return false;
   cuuint64_t gdim[2] = {16ull * units, v->rows};
   cuuint64_t gstride[1] = {v->ld};
-  cuuint32_t box[2] = {std::min(64u, 16 * units), rows};
+  cuuint32_t box[2] = {wide, rows};
   cuuint32_t es[2] = {1, 1};
   return f(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)v->data, gdim, gstride, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-           CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+           swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int NT, int G, bool F32, typename O>
@@ -146,6 +147,14 @@ cudaError_t launch_score4(const CUtensorMap& map, const raven_score4::Params& p,
   using namespace raven_score4;
   static Allowed allowed(kMostShared);
   return launch(score4_kernel<NT, G, F32, O>, ctas, Layout<NT, G>::kThreads, (uint32_t)smem, allowed, st, map, p);
+}
+
+cudaError_t launch_join(const raven_score4::Join& j, int out_type, int sms, cudaStream_t st) {
+  using namespace raven_score4;
+  static Allowed none;
+  const uint64_t grid = std::min<uint64_t>((j.nq * (j.ld / 4) + 255) / 256, (uint64_t)sms * 32);
+  return launch(out_type == 0 ? join_kernel<float> : out_type == 1 ? join_kernel<__half> : join_kernel<__nv_bfloat16>, grid, 256,
+                0, none, st, j);
 }
 
 template <int NT, int G, bool F32>
@@ -188,12 +197,6 @@ cudaError_t run_score4(const raven_rows* v, raven_score4::Params p, int out_type
   const uint64_t laid = lay ? (p.chunks * Q::bytes(p.units, p.groups) + 255) / 256 * 256 : 0;
   const uint64_t wide = (p.n + 3) / 4 * 4, sums = p.slices > 1 ? p.slices * p.nq * wide * 4 : 0;
   if (laid + sums && (e = cudaMallocAsync((void**)&tmp, laid + sums, st)) != cudaSuccess) return e;
-  if (lay) {
-    static Allowed none;
-    e = launch(lay_out_kernel<NT, G, F32>, (uint64_t)p.chunks * kQueries, 256, 0, none, st, p, tmp);
-    p.q = nullptr;
-    p.laid = tmp;
-  }
   Join j{(const float*)(tmp + laid), wide, p.nq * wide, p.slices, p.nq, p.n, p.alpha, p.bias, p.out, p.ld};
   if (p.slices > 1) {
     p.out = tmp + laid;
@@ -202,39 +205,111 @@ cudaError_t run_score4(const raven_rows* v, raven_score4::Params p, int out_type
     p.alpha = 1.f;
     p.bias = nullptr;
   }
+  if (lay) {
+    static Allowed none;
+    e = launch(lay_out_kernel<Q, G, F32>, (uint64_t)p.chunks * kQueries, 256, 0, none, st, p, tmp);
+    p.q = nullptr;
+    p.laid = tmp;
+  }
   p.whole = aligned(p.out, 16) && (p.nq == 1 || p.ld % (16 / (p.slices > 1 || out_type == 0 ? 4 : 2)) == 0);
   CUtensorMap map;
-  if (e == cudaSuccess && !codes_map(&map, v, p.units, L::kRows)) e = cudaErrorInvalidValue;
+  if (e == cudaSuccess && !codes_map(&map, v, p.units, std::min(64u, 16 * p.units), L::kRows, CU_TENSOR_MAP_SWIZZLE_NONE)) e = cudaErrorInvalidValue;
   const uint64_t ctas = std::min<uint64_t>(columns, p.tiles) * shares, smem = L::bytes(units, groups, p.split, p.depth);
   if (e == cudaSuccess)
     e = p.slices > 1 || out_type == 0 ? launch_score4<NT, G, F32, float>(map, p, ctas, smem, st)
         : out_type == 1               ? launch_score4<NT, G, F32, __half>(map, p, ctas, smem, st)
                                       : launch_score4<NT, G, F32, __nv_bfloat16>(map, p, ctas, smem, st);
-  if (p.slices > 1 && e == cudaSuccess) {
-    static Allowed none;
-    const uint64_t grid = std::min<uint64_t>((p.nq * (wide / 4) + 255) / 256, (uint64_t)sms * 32);
-    e = launch(out_type == 0 ? join_kernel<float> : out_type == 1 ? join_kernel<__half> : join_kernel<__nv_bfloat16>, grid, 256,
-               0, none, st, j);
-  }
+  if (p.slices > 1 && e == cudaSuccess) e = launch_join(j, out_type, sms, st);
   if (tmp) cudaFreeAsync(tmp, st);
   return e;
 }
 
-template <int NT, bool F32>
-cudaError_t group_score4(const raven_rows* v, const raven_score4::Params& p, uint32_t group, int out_type, int sms,
-                         cudaStream_t st) {
-  return group == 32   ? run_score4<NT, 32, F32>(v, p, out_type, sms, st)
-         : group == 64 ? run_score4<NT, 64, F32>(v, p, out_type, sms, st)
-                       : run_score4<NT, 128, F32>(v, p, out_type, sms, st);
+template <int NC, int G, bool F32, typename O>
+cudaError_t launch_wide(const CUtensorMap& map, const raven_score4::Params& p, uint64_t ctas, uint64_t smem, cudaStream_t st) {
+  static Allowed allowed(kMostShared);
+  return launch(raven_score4::wide_kernel<NC, G, F32, O>, ctas, raven_score4::kWideThreads, (uint32_t)smem, allowed, st, map, p);
+}
+
+template <int NC, int G, bool F32>
+cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, int sms, cudaStream_t st) {
+  using namespace raven_score4;
+  using L = Wide<NC>;
+  using Q = WideLaid<NC>;
+  constexpr uint32_t kQueries = F32 ? NC / 2 : NC, W = kBlock / G;
+  p.chunks = (uint32_t)((p.nq + kQueries - 1) / kQueries);
+  p.tiles = (uint32_t)((p.n + kWideRows - 1) / kWideRows);
+  // Slices of a row, whole fours of blocks (the sums of four groups share a block): those that take least time, in
+  // blocks of a team (half a microsecond), with a block and a half a tile for its end and what the sums' join costs.
+  auto bytes = [&](uint32_t slice, uint32_t depth) {
+    return L::bytes(std::min(4 * slice, p.units), std::min(slice * W, p.groups), depth);
+  };
+  double best = 0;
+  uint64_t columns = 1;
+  for (uint32_t n = 1; n <= std::max(1u, (p.blocks + 3) / 4); ++n) {
+    const uint32_t slice = n == 1 ? p.blocks : ((p.blocks + n - 1) / n + 3) / 4 * 4, slices = (p.blocks + slice - 1) / slice;
+    if (slices != n || bytes(slice, 2) > kMostShared) continue;
+    const uint64_t shares = (uint64_t)p.chunks * slices, c = std::max<uint64_t>(1, (uint64_t)sms / shares);
+    const uint64_t rounds = (p.tiles + kWideTeams * c - 1) / (kWideTeams * c) * ((shares + sms - 1) / sms);
+    const double time = rounds * (slice + 1.5) + (slices > 1 ? 6 + 4e-6 * p.nq * p.n * slices : 0);
+    if (best == 0 || time < best) {
+      best = time;
+      columns = c;
+      p.slice = slice;
+      p.slices = slices;
+    }
+    if (n >= 64 && best > 0) break;
+  }
+  const uint32_t shares = p.chunks * p.slices;
+  p.depth = kWideDepth;
+  while (bytes(p.slice, p.depth) > kMostShared) --p.depth;
+  uint8_t* tmp = nullptr;
+  cudaError_t e = cudaSuccess;
+  const bool lay = p.slices > 1 || (uint64_t)kQueries * p.dim > kOwnLayout;
+  const uint64_t laid = lay ? (p.chunks * Q::bytes(p.units, p.groups) + 255) / 256 * 256 : 0;
+  const uint64_t wide = (p.n + 3) / 4 * 4, sums = p.slices > 1 ? p.slices * p.nq * wide * 4 : 0;
+  if (laid + sums && (e = cudaMallocAsync((void**)&tmp, laid + sums, st)) != cudaSuccess) return e;
+  Join j{(const float*)(tmp + laid), wide, p.nq * wide, p.slices, p.nq, p.n, p.alpha, p.bias, p.out, p.ld};
+  if (p.slices > 1) {
+    p.out = tmp + laid;
+    p.ld = wide;
+    p.ld_slice = p.nq * wide;
+    p.alpha = 1.f;
+    p.bias = nullptr;
+  }
+  if (lay) {
+    static Allowed none;
+    e = launch(lay_out_kernel<Q, G, F32>, (uint64_t)p.chunks * kQueries, 256, 0, none, st, p, tmp);
+    p.q = nullptr;
+    p.laid = tmp;
+  }
+  CUtensorMap map;
+  if (e == cudaSuccess && !codes_map(&map, v, p.units, 64, kWideRows, CU_TENSOR_MAP_SWIZZLE_64B)) e = cudaErrorInvalidValue;
+  const uint64_t ctas = std::min<uint64_t>(columns, (p.tiles + kWideTeams - 1) / kWideTeams) * shares;
+  if (e == cudaSuccess)
+    e = p.slices > 1 || out_type == 0 ? launch_wide<NC, G, F32, float>(map, p, ctas, bytes(p.slice, p.depth), st)
+        : out_type == 1               ? launch_wide<NC, G, F32, __half>(map, p, ctas, bytes(p.slice, p.depth), st)
+                                      : launch_wide<NC, G, F32, __nv_bfloat16>(map, p, ctas, bytes(p.slice, p.depth), st);
+  if (p.slices > 1 && e == cudaSuccess) e = launch_join(j, out_type, sms, st);
+  if (tmp) cudaFreeAsync(tmp, st);
+  return e;
+}
+
+// Columns are queries, two for one of f32.
+template <int G, bool F32>
+cudaError_t group_score4(const raven_rows* v, const raven_score4::Params& p, int out_type, int sms, cudaStream_t st) {
+  const uint64_t columns = F32 ? 2 * p.nq : p.nq;
+  return columns <= 8    ? run_score4<1, G, F32>(v, p, out_type, sms, st)
+         : columns <= 16 ? run_score4<2, G, F32>(v, p, out_type, sms, st)
+         : columns <= 32 ? run_wide<32, G, F32>(v, p, out_type, sms, st)
+                         : run_wide<64, G, F32>(v, p, out_type, sms, st);
 }
 
 template <bool F32>
 cudaError_t dispatch_score4(const raven_rows* v, const raven_score4::Params& p, uint32_t group, int out_type, int sms,
                             cudaStream_t st) {
-  const uint64_t columns = F32 ? 2 * p.nq : p.nq;
-  return columns <= 8    ? group_score4<1, F32>(v, p, group, out_type, sms, st)
-         : columns <= 16 ? group_score4<2, F32>(v, p, group, out_type, sms, st)
-                         : group_score4<4, F32>(v, p, group, out_type, sms, st);
+  return group == 32   ? group_score4<32, F32>(v, p, out_type, sms, st)
+         : group == 64 ? group_score4<64, F32>(v, p, out_type, sms, st)
+                       : group_score4<128, F32>(v, p, out_type, sms, st);
 }
 
 // ---------------------------------------------------------------------------

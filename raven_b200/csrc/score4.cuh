@@ -78,15 +78,24 @@ struct Params {
 
 // A chunk of queries as the kernel takes it, NT * 8 columns: fragments (for each
 // unit and N tile 16 bytes a lane), then per group the columns' sums, then per
-// column two powers of two whose product brings sums back. f32 queries have two
-// columns side by side, the second for what the first leaves and without sums.
+// column what brings its sums back: alpha times a power of two, or where that is no
+// f32 a NaN, and the power as two factors. f32 queries have two columns side by
+// side, the second for what the first leaves and without sums.
 template <int NT>
 struct Laid {
+  static constexpr uint32_t kColumns = NT * 8;
   static constexpr uint32_t kUnitBytes = NT * 512;
   __host__ __device__ static uint64_t frags(uint32_t units) { return (uint64_t)units * kUnitBytes; }
   __host__ __device__ static uint64_t sums(uint32_t groups) { return (uint64_t)groups * NT * 8 * 4; }
   __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t groups) {
-    return frags(units) + sums(groups) + NT * 8 * 8;
+    return frags(units) + sums(groups) + NT * 8 * 16;
+  }
+  // Where a quarter of a unit of a column is; a group's sum (times 2^-24), where `to` are the sums.
+  __device__ static uint32_t frag_at(uint32_t unit, uint32_t quarter, uint32_t col) {
+    return (unit * NT + col / 8) * 512 + ((col & 7) * 4 + quarter) * 16;
+  }
+  __device__ static void put_sum(uint8_t* to, uint32_t group, uint32_t col, float sum) {
+    ((float*)to)[group * (NT * 8) + col] = sum;
   }
 };
 
@@ -108,12 +117,12 @@ __device__ inline void eight(const T* x, uint32_t d, uint32_t dim, bool whole, f
 
 // Queries [first, first + count) as columns from `col` on, by all of a CTA's
 // threads. top: `count` words of shared memory.
-template <int NT, int G, typename T>
+template <class Q, int G, typename T>
 __device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, uint32_t col, uint8_t* to, uint32_t* top) {
   constexpr bool F32 = std::is_same<T, float>::value;
   constexpr uint32_t L = G / 8;
-  float* sums = (float*)(to + Laid<NT>::frags(p.units));
-  float* back = sums + p.groups * NT * 8;
+  uint8_t* sums = to + Q::frags(p.units);
+  float* back = (float*)(sums + Q::sums(p.groups));
   const uint32_t n8 = (p.units * 4 + L - 1) / L * L;  // eights, up to whole groups
   const uint32_t items = count * n8;
   auto load = [&](uint32_t q, uint32_t i, float(&v)[8]) {
@@ -152,8 +161,8 @@ __device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, 
     for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const uint32_t c = col + (F32 ? 2 * q : q);
     if (i % L == 0 && i / L < p.groups) {
-      sums[i / L * (NT * 8) + c] = sum * 0x1p-24f;
-      if (F32) sums[i / L * (NT * 8) + c + 1] = 0.f;
+      Q::put_sum(sums, i / L, c, sum * 0x1p-24f);
+      if (F32) Q::put_sum(sums, i / L, c + 1, 0.f);
     }
     if (i < p.units * 4) {
       __align__(16) __half part[F32 ? 2 : 1][8];
@@ -166,37 +175,41 @@ __device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, 
       }
 #pragma unroll
       for (int h = 0; h < (F32 ? 2 : 1); ++h)
-        *(uint4*)(to + ((i >> 2) * NT + (c + h) / 8) * 512 + (((c + h) & 7) * 4 + (i & 3)) * 16) = *(const uint4*)part[h];
+        *(uint4*)(to + Q::frag_at(i >> 2, i & 3, c + h)) = *(const uint4*)part[h];
     }
     if (i == 0) {
       const int b = 24 - e;  // -139 .. 137
 #pragma unroll
       for (int h = 0; h < (F32 ? 2 : 1); ++h) {
-        back[2 * (c + h)] = bad ? __uint_as_float(0x7fc00000u) : pow2(b / 2);
-        back[2 * (c + h) + 1] = pow2(b - b / 2);
+        // exact where alpha's exponent leaves it among the normal numbers
+        const int a = p.alpha == 0.f ? 0 : ilogbf(p.alpha) + b;
+        const bool plain = a >= -120 && a <= 120 && (p.alpha == 0.f || fabsf(p.alpha) < INFINITY) && b >= -126 && b <= 127;
+        const float k0 = bad ? __uint_as_float(0x7fc00000u) : pow2(b / 2), k1 = pow2(b - b / 2);
+        *(float4*)(back + 4 * (c + h)) = make_float4(plain && !bad ? p.alpha * k0 * k1 : __uint_as_float(0x7fc00000u), k0, k1,
+                                                     plain || bad ? 0.f : 1.f);
       }
     }
   }
 }
 
-template <int NT, int G, bool F32>
+template <class Q, int G, bool F32>
 __device__ inline void lay_out_any(const Params& p, uint64_t first, uint32_t count, uint32_t col, uint8_t* to, uint32_t* top) {
   if constexpr (F32)
-    lay_out<NT, G, float>(p, first, count, col, to, top);
+    lay_out<Q, G, float>(p, first, count, col, to, top);
   else if (p.q_type == 1)
-    lay_out<NT, G, __half>(p, first, count, col, to, top);
+    lay_out<Q, G, __half>(p, first, count, col, to, top);
   else
-    lay_out<NT, G, __nv_bfloat16>(p, first, count, col, to, top);
+    lay_out<Q, G, __nv_bfloat16>(p, first, count, col, to, top);
 }
 
 // All chunks, a CTA per query.
-template <int NT, int G, bool F32>
+template <class Q, int G, bool F32>
 __global__ void __launch_bounds__(256) lay_out_kernel(const Params p, uint8_t* to) {
-  constexpr uint32_t Q = F32 ? NT * 4 : NT * 8;
+  constexpr uint32_t kQueries = F32 ? Q::kColumns / 2 : Q::kColumns;
   __shared__ uint32_t top[1];
   after_previous();
-  const uint32_t chunk = blockIdx.x / Q, q = blockIdx.x - chunk * Q;
-  lay_out_any<NT, G, F32>(p, blockIdx.x, 1, F32 ? 2 * q : q, to + chunk * Laid<NT>::bytes(p.units, p.groups), top);
+  const uint32_t chunk = blockIdx.x / kQueries, q = blockIdx.x - chunk * kQueries;
+  lay_out_any<Q, G, F32>(p, blockIdx.x, 1, F32 ? 2 * q : q, to + chunk * Q::bytes(p.units, p.groups), top);
 }
 
 template <int B>
@@ -237,15 +250,10 @@ __device__ inline void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
 
 template <int NT, int G>
 struct Layout {
-#ifndef MT1
-#define MT1 4
-#define W1 16
-#define W2 16
-#endif
-  static constexpr int kMT = NT == 1 ? MT1 : 2;           // M tiles of a warp: few queries leave registers for four
-  static constexpr int kAtOnce = NT == 4 ? kMT : 1;       // M tiles that go through a block together
+  static constexpr int kMT = NT == 1 ? 4 : 2;             // M tiles of a warp: as many as its registers allow
+  static constexpr int kAtOnce = NT == 1 ? 1 : kMT;       // M tiles that go through a block together
   static constexpr uint32_t kRows = 16 * kMT;             // rows of its tile
-  static constexpr uint32_t kWarps = NT == 1 ? W1 : NT == 2 ? W2 : 8;    // as many as their registers allow
+  static constexpr uint32_t kWarps = 16;
   static constexpr uint32_t kThreads = kWarps * 32;
   static constexpr uint32_t kWords = kBlock / G;          // scale words of a row's block
   static constexpr uint32_t kCodeBytes = kRows * 64, kWordBytes = kRows * kWords * 4;
@@ -344,7 +352,7 @@ __global__ void __launch_bounds__(Layout<NT, G>::kThreads, 1) score4_kernel(cons
   float* sums = (float*)(held + Q::frags(units));
   float* back = sums + groups * NT * 8;
   if (p.q) {
-    lay_out_any<NT, G, F32>(p, chunk * kQueries, kQueries, 0, held, tops);
+    lay_out_any<Q, G, F32>(p, chunk * kQueries, kQueries, 0, held, tops);
   } else {
     const uint8_t* from = p.laid + chunk * Q::bytes(p.units, p.groups);
     auto bring = [&](void* to, const uint8_t* what, uint32_t bytes) {
@@ -354,9 +362,11 @@ __global__ void __launch_bounds__(Layout<NT, G>::kThreads, 1) score4_kernel(cons
     bring(held, from + Q::frags(4 * b0), (uint32_t)Q::frags(units));
     from += Q::frags(p.units);
     bring(sums, from + Q::sums(b0 * S::kWords), (uint32_t)Q::sums(groups));
-    bring(back, from + Q::sums(p.groups), NT * 8 * 8);
+    bring(back, from + Q::sums(p.groups), NT * 8 * 16);
   }
   __syncthreads();
+  bool plain = true;  // every column has one factor
+  for (uint32_t c = 0; c < NT * 8; ++c) plain &= back[4 * c + 3] == 0.f;
 
   bool ok = true;  // no wait has run out
   uint32_t now = 0, phases = 0;  // the stage that is taken next; parities of the stages
@@ -519,19 +529,27 @@ __global__ void __launch_bounds__(Layout<NT, G>::kThreads, 1) score4_kernel(cons
         const uint32_t col = 8 * j + 2 * t + c;
         const uint64_t query = chunk * kQueries + (F32 ? col / 2 : col);
         if (query < p.nq) {
-          const float k0 = back[2 * col], k1 = back[2 * col + 1];
           __align__(16) O o[R];
+          if (plain) {
+            const float f = back[4 * col];
 #pragma unroll
-          for (int r = 0; r < R; ++r) o[r] = rounded<O>(fmaf(p.alpha, y[r] * k0 * k1, bias[r]));
+            for (int r = 0; r < R; ++r) o[r] = rounded<O>(fmaf(f, y[r], bias[r]));
+          } else {
+            const float k0 = back[4 * col + 1], k1 = back[4 * col + 2];
+#pragma unroll
+            for (int r = 0; r < R; ++r) o[r] = rounded<O>(fmaf(p.alpha, y[r] * k0 * k1, bias[r]));
+          }
           O* to = (O*)p.out + slice * p.ld_slice + query * p.ld + row;
           if (p.whole && row + R <= p.n) {
-            constexpr int B = R * sizeof(O) >= 16 ? 16 : 8;
+            constexpr int B = R * sizeof(O) >= 16 ? 16 : R * sizeof(O);
 #pragma unroll
             for (int i = 0; i < (int)(R * sizeof(O)) / B; ++i) {
               if constexpr (B == 16)
                 ((uint4*)to)[i] = ((const uint4*)o)[i];
-              else
+              else if constexpr (B == 8)
                 ((uint2*)to)[i] = ((const uint2*)o)[i];
+              else
+                ((uint32_t*)to)[i] = ((const uint32_t*)o)[i];
             }
           } else {
 #pragma unroll

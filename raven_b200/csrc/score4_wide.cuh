@@ -1,0 +1,342 @@
+// Scores of more than a few queries against 4-bit rows: as score4.cuh, with the sums
+// by tcgen05.mma. 32 or 64 columns (queries; two for one of f32) are the N side, 128
+// rows the M side. What a warp of mma.sync instructions does per query (fragments
+// from shared memory, sums in registers) took more instructions than the codes
+// themselves from 16 columns on.
+//
+// A group of four warps takes a tile of 128 rows, a row a thread. Codes come by TMA;
+// a thread turns its row's 128 codes of a block into f16 operands (five
+// instructions per eight codes, see score4.cuh) and writes them to tensor memory,
+// which the instruction reads its M side from: shared memory holds queries only,
+// and its bandwidth goes to them. A scale group is a chain of instructions of its
+// own, the last of which adds z * sum(q): three operands z * 2^-10 against the sum in
+// three f16 parts. The thread then reads its row's sums of the group and adds them,
+// times the group's step, to its own in registers. Three such groups of warps per SM
+// work on tiles of their own, so that one's instructions and waits are hidden by the
+// others'. A thread has all scores of its row, and a warp writes 32 scores of a query
+// side by side, wherever the query's scores start.
+#pragma once
+
+#include "score4.cuh"
+
+namespace raven_score4 {
+
+// A chunk of queries: K blocks of 64 values (two units), for each column 128 bytes
+// in the 128-byte swizzle; then blocks of four groups' sums laid out the same way,
+// 16 operands a group, of which three are its sum; then what brings sums back.
+template <int NC>
+struct WideLaid {
+  static constexpr uint32_t kColumns = NC;
+  static constexpr uint32_t kBlockBytes = NC * 128;
+  __host__ __device__ static uint64_t frags(uint32_t units) { return (uint64_t)((units + 1) / 2) * kBlockBytes; }
+  __host__ __device__ static uint64_t sums(uint32_t groups) { return (uint64_t)((groups + 3) / 4) * kBlockBytes; }
+  __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t groups) {
+    return frags(units) + sums(groups) + NC * 16;
+  }
+  __device__ static uint32_t frag_at(uint32_t unit, uint32_t quarter, uint32_t col) {
+    return unit / 2 * kBlockBytes + col * 128 + ((((unit & 1) * 4 + quarter) ^ (col & 7)) * 16);
+  }
+  // sum: times 2^-24; against z * 2^-10 it has to be 2^10 times that. Below 2^8, so three parts leave less than 2^-24.
+  __device__ static void put_sum(uint8_t* to, uint32_t group, uint32_t col, float sum) {
+    const float x = sum * 0x1p10f;
+    const __half hi = __float2half_rn(x);
+    const float r = x - __half2float(hi);
+    const __half mid = __float2half_rn(r), lo = __float2half_rn(r - __half2float(mid));
+    __align__(16) __half part[8] = {hi, mid, lo, __half(0.f), __half(0.f), __half(0.f), __half(0.f), __half(0.f)};
+    uint8_t* at = to + group / 4 * kBlockBytes + col * 128;
+    *(uint4*)(at + ((((group & 3) * 2) ^ (col & 7)) * 16)) = *(const uint4*)part;
+    *(uint4*)(at + ((((group & 3) * 2 + 1) ^ (col & 7)) * 16)) = make_uint4(0, 0, 0, 0);
+  }
+};
+
+constexpr uint32_t kWideRows = 128, kWideTeams = 3;  // rows of a tile; groups of four warps
+constexpr uint32_t kWideThreads = kWideTeams * 128;
+constexpr uint32_t kWideDepth = 4;                   // tiles under way per team, at most
+constexpr uint32_t kWideStage = kWideRows * 64;
+
+template <int NC>
+struct Wide {
+  // tensor memory of a team: operands of a block, of its groups' z, a group's sums
+  static constexpr uint32_t kZ = 64, kAcc = 96, kTeam = 160;
+  static_assert(kAcc + NC <= kTeam && kWideTeams * kTeam <= 512, "tensor memory has 512 columns");
+  static constexpr uint32_t kHead = 1024;  // barriers, the place of the tensor memory; TMA's places start on 1024 bytes
+  static constexpr uint32_t kTops = NC * 4;
+  __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t groups, uint32_t depth) {
+    return 1024 + kHead + (uint64_t)kWideTeams * depth * kWideStage + WideLaid<NC>::bytes(units, groups) + kTops;
+  }
+};
+
+template <int N>
+__device__ inline void tmem_st(uint32_t at, const uint32_t* v);
+template <>
+__device__ inline void tmem_st<2>(uint32_t at, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};\n" ::"r"(at), "r"(v[0]), "r"(v[1]) : "memory");
+}
+template <>
+__device__ inline void tmem_st<8>(uint32_t at, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(at), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+template <>
+__device__ inline void tmem_st<16>(uint32_t at, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};\n" ::"r"(at),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ inline void tmem_ld16(uint32_t at, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];\n"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(at));
+}
+// Waits for the loads; ties the registers to the wait.
+template <int N>
+__device__ inline void tmem_wait_ld(uint32_t (&v)[N][16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(v[j][i]));
+}
+// M side in tensor memory, N side in shared memory.
+__device__ inline void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(add)
+      : "memory");
+}
+// All lanes of a warp wait; one answer.
+__device__ inline bool warp_waits(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); }
+
+template <int NC, int G, bool F32, typename O>
+__global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
+  using Q = WideLaid<NC>;
+  using S = Wide<NC>;
+  constexpr uint32_t kQueries = F32 ? NC / 2 : NC, W = kBlock / G, U = G / kUnit;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31, team = warp / 4, row_of = tid & 127;
+  const uint32_t bars = smem_u32(smem) + team * 64;  // full[depth], done
+  const uint32_t done = bars + 8 * kWideDepth;
+  volatile uint32_t* slot_of_tmem = (volatile uint32_t*)(smem + 512);
+  uint8_t* ring = smem + S::kHead + team * p.depth * kWideStage;
+  uint8_t* held = smem + S::kHead + kWideTeams * p.depth * kWideStage;
+  const uint32_t shares = p.chunks * p.slices, share = blockIdx.x % shares;
+  const uint32_t step = gridDim.x / shares * kWideTeams, first = blockIdx.x / shares * kWideTeams + team;
+  const uint32_t slice = share % p.slices;
+  const uint64_t chunk = share / p.slices;
+  const uint32_t b0 = slice * p.slice, blocks = min(p.slice, p.blocks - b0);
+  const uint32_t units = min(4 * p.slice, p.units - 4 * b0), groups = min(p.slice * W, p.groups - b0 * W);
+  if (row_of == 0) {
+    for (uint32_t i = 0; i < kWideDepth + 1; ++i) mbar_init(bars + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32((void*)slot_of_tmem)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  raven_tc::tc_fence_before();
+  __syncthreads();
+  raven_tc::tc_fence_after();
+  const uint32_t tmem = *slot_of_tmem + team * S::kTeam;
+  const uint32_t mine = tmem + ((warp & 3) << 21);  // this warp's 32 lanes
+  after_previous();
+
+  // copies: by the team's first thread
+  uint32_t ahead = first, ahead_b = 0, slot = 0, pending = 0;
+  auto copy_next = [&]() {
+    if (ahead < p.tiles) {
+      mbar_expect_tx(bars + 8 * slot, kWideStage);
+      tma_load_2d(smem_u32(ring) + slot * kWideStage, &map, (int)(64 * (b0 + ahead_b)),
+                  (int)min((uint64_t)ahead * kWideRows, p.n), bars + 8 * slot);
+      pending |= 1u << slot;
+      slot = slot + 1 == p.depth ? 0 : slot + 1;
+      if (++ahead_b == blocks) {
+        ahead_b = 0;
+        ahead += step;
+      }
+    }
+  };
+  if (row_of == 0)
+    for (uint32_t i = 0; i < p.depth; ++i) copy_next();
+
+  uint8_t* sums = held + Q::frags(units);
+  float* back = (float*)(sums + Q::sums(groups));
+  if (p.q) {
+    lay_out_any<Q, G, F32>(p, chunk * kQueries, kQueries, 0, held, (uint32_t*)(back + 4 * NC));
+  } else {
+    const uint8_t* from = p.laid + chunk * Q::bytes(p.units, p.groups);
+    auto bring = [&](void* to, const uint8_t* what, uint32_t bytes) {
+      for (uint32_t i = tid * 16; i < bytes; i += kWideThreads * 16) *(uint4*)((uint8_t*)to + i) = *(const uint4*)(what + i);
+    };
+    bring(held, from + Q::frags(4 * b0), (uint32_t)Q::frags(units));
+    from += Q::frags(p.units);
+    bring(sums, from + Q::sums(b0 * W), (uint32_t)Q::sums(groups));
+    bring(back, from + Q::sums(p.groups), NC * 16);
+  }
+  {  // the operands behind a group's three z stay 0
+    const uint32_t zero[8] = {};
+#pragma unroll
+    for (uint32_t g = 0; g < W; ++g) tmem_st<8>(mine + S::kZ + 8 * g, zero);
+  }
+  asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // the queries, to the instructions
+  __syncthreads();
+  bool plain = true;  // every column has one factor
+  for (uint32_t c = 0; c < NC; ++c) plain &= back[4 * c + 3] == 0.f;
+  const uint64_t b_desc = raven_tc::sw128_desc(smem_u32(held)), z_desc = raven_tc::sw128_desc(smem_u32(sums));
+  constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(NC >> 3) << 17) | (8u << 24);  // f32 sums, f16 operands
+
+  bool ok = true;
+  uint32_t now = 0, phases = 0, done_phase = 0;
+  // the words of the thread's row, one block ahead
+  uint32_t next[W];
+  auto fetch = [&](uint32_t tile, uint32_t b) {
+    const uint32_t* from = p.words + min((uint64_t)tile * kWideRows + row_of, p.n - 1) * p.ld_words + (b0 + b) * W;
+    if constexpr (W == 4) {
+      const uint4 v = *(const uint4*)from;
+      next[0] = v.x, next[1] = v.y, next[2] = v.z, next[3] = v.w;
+    } else if constexpr (W == 2) {
+      const uint2 v = *(const uint2*)from;
+      next[0] = v.x, next[1] = v.y;
+    } else {
+      next[0] = *from;
+    }
+  };
+  if (first < p.tiles) fetch(first, 0);
+  for (uint32_t tile = first; tile < p.tiles; tile += step) {
+    float total[NC] = {};
+    for (uint32_t b = 0; b < blocks; ++b) {
+      const uint32_t u = min(4u, units - 4 * b);
+      uint32_t word[W];
+#pragma unroll
+      for (uint32_t g = 0; g < W; ++g) word[g] = next[g];
+      if (b + 1 < blocks)
+        fetch(tile, b + 1);
+      else if (tile + step < p.tiles)
+        fetch(tile + step, 0);
+      if (ok && !warp_waits(bars + 8 * now, phases >> now & 1u)) ok = false;
+      if (ok) {
+        // 64 bytes of the row, 16 at a time in the 64-byte swizzle
+        const uint8_t* stage = ring + now * kWideStage + row_of * 64;
+        uint32_t c[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *(uint4*)&c[4 * i] = *(const uint4*)(stage + ((i ^ ((row_of >> 1) & 3)) * 16));
+        // word u * quarter + unit of a block of u units
+        auto put_unit = [&](uint32_t unit, uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3) {
+          const uint32_t w[4] = {c0, c1, c2, c3};
+          uint32_t a[16];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            a[4 * i] = w[i] & 0x000f000fu;
+            a[4 * i + 1] = w[i] & 0x00f000f0u;
+            a[4 * i + 2] = (w[i] >> 8) & 0x000f000fu;
+            a[4 * i + 3] = (w[i] >> 8) & 0x00f000f0u;
+          }
+          tmem_st<16>(mine + 16 * unit, a);
+        };
+        if (u == 4) {
+          put_unit(0, c[0], c[4], c[8], c[12]);
+          put_unit(1, c[1], c[5], c[9], c[13]);
+          put_unit(2, c[2], c[6], c[10], c[14]);
+          put_unit(3, c[3], c[7], c[11], c[15]);
+        } else if (u == 3) {
+          put_unit(0, c[0], c[3], c[6], c[9]);
+          put_unit(1, c[1], c[4], c[7], c[10]);
+          put_unit(2, c[2], c[5], c[8], c[11]);
+        } else if (u == 2) {
+          put_unit(0, c[0], c[2], c[4], c[6]);
+          put_unit(1, c[1], c[3], c[5], c[7]);
+        } else {
+          put_unit(0, c[0], c[1], c[2], c[3]);
+        }
+#pragma unroll
+        for (uint32_t g = 0; g < W; ++g) {
+          const __half2 z = __float2half2_rn(raven_int4::zero_of(word[g]) * 0x1p-10f);
+          const uint32_t v = *(const uint32_t*)&z, three[2] = {v, v & 0xffffu};
+          tmem_st<2>(mine + S::kZ + 8 * g, three);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+      }
+      const uint32_t taken = now;
+      phases ^= 1u << now;
+      now = now + 1 == p.depth ? 0 : now + 1;
+#pragma unroll
+      for (uint32_t g = 0; g < W; ++g) {
+        if (g * U >= u) break;
+        raven_tc::tc_fence_before();
+        meet(1 + team, 128);  // operands are written, the sums before them read
+        if (row_of == 0 && ok) {
+          if (g == 0) {
+            pending &= ~(1u << taken);
+            copy_next();  // into the stage that every thread has read
+          }
+          raven_tc::tc_fence_after();
+          uint32_t add = 0;
+#pragma unroll
+          for (uint32_t uu = 0; uu < U; ++uu) {
+            const uint32_t unit = g * U + uu;
+            if (unit >= u) break;
+            const uint64_t at = b_desc + ((4 * b + unit) / 2 * Q::kBlockBytes >> 4) + (unit & 1) * 4;
+            mma_ts(tmem + S::kAcc, tmem + 16 * unit, at, idesc, add);
+            mma_ts(tmem + S::kAcc, tmem + 16 * unit + 8, at + 2, idesc, 1);
+            add = 1;
+          }
+          const uint32_t group = b * W + g;
+          mma_ts(tmem + S::kAcc, tmem + S::kZ + 8 * g, z_desc + (group / 4 * Q::kBlockBytes >> 4) + (group & 3) * 2, idesc, 1);
+          raven_tc::mma_commit(done);
+        }
+        if (ok && !warp_waits(done, done_phase)) ok = false;
+        done_phase ^= 1u;
+        raven_tc::tc_fence_after();
+        const float sc = raven_int4::step_of(word[g]);
+#pragma unroll
+        for (int j = 0; j < NC / 32; ++j) {
+          uint32_t v[2][16];
+          tmem_ld16(mine + S::kAcc + 32 * j, v[0]);
+          tmem_ld16(mine + S::kAcc + 32 * j + 16, v[1]);
+          tmem_wait_ld(v);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) total[32 * j + i] = fmaf(sc, __uint_as_float(v[i / 16][i % 16]), total[32 * j + i]);
+        }
+      }
+    }
+    const uint64_t row = (uint64_t)tile * kWideRows + row_of;
+    if (row < p.n) {
+      const float bias = p.bias ? p.bias[row] : 0.f;
+      O* to = (O*)p.out + slice * p.ld_slice + chunk * kQueries * p.ld + row;
+      const uint32_t here = (uint32_t)min((uint64_t)kQueries, p.nq - chunk * kQueries);
+#pragma unroll
+      for (uint32_t q = 0; q < kQueries; ++q) {
+        if (q >= here) break;
+        const uint32_t c = F32 ? 2 * q : q;
+        const float y = F32 ? total[c] + total[c + 1] : total[c];
+        *to = rounded<O>(plain ? fmaf(back[4 * c], y, bias) : fmaf(p.alpha, y * back[4 * c + 1] * back[4 * c + 2], bias));
+        to += p.ld;
+      }
+    }
+  }
+  if (!ok && lane == 0) raven_score::tell(p.status, raven_score::kStatusWait);
+  // a wait ran out: neither a copy nor an instruction of this team is under way any more
+  if (!ok && row_of == 0) {
+    for (uint32_t i = 0; i < p.depth; ++i)
+      if (pending >> i & 1u) wait(bars + 8 * i, phases >> i & 1u);
+    raven_tc::mma_commit(done);
+    wait(done, done_phase);
+  }
+  raven_tc::tc_fence_before();
+  __syncthreads();
+  raven_tc::tc_fence_after();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(*slot_of_tmem), "r"(512) : "memory");
+}
+
+}  // namespace raven_score4
