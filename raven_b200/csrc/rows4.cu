@@ -227,7 +227,7 @@ cudaError_t run_score4(const raven_rows* v, raven_score4::Params p, int out_type
 template <int NC, int G, bool F32, typename O>
 cudaError_t launch_wide(const CUtensorMap& map, const raven_score4::Params& p, uint64_t ctas, uint64_t smem, cudaStream_t st) {
   static Allowed allowed(kMostShared);
-  return launch(raven_score4::wide_kernel<NC, G, F32, O>, ctas, raven_score4::kWideThreads, (uint32_t)smem, allowed, st, map, p);
+  return launch(raven_score4::wide_kernel<NC, G, F32, O>, ctas, raven_score4::Wide<NC>::kThreads, (uint32_t)smem, allowed, st, map, p);
 }
 
 template <int NC, int G, bool F32>
@@ -249,7 +249,7 @@ cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, 
     const uint32_t slice = n == 1 ? p.blocks : ((p.blocks + n - 1) / n + 3) / 4 * 4, slices = (p.blocks + slice - 1) / slice;
     if (slices != n || bytes(slice, 2) > kMostShared) continue;
     const uint64_t shares = (uint64_t)p.chunks * slices, c = std::max<uint64_t>(1, (uint64_t)sms / shares);
-    const uint64_t rounds = (p.tiles + kWideTeams * c - 1) / (kWideTeams * c) * ((shares + sms - 1) / sms);
+    const uint64_t rounds = (p.tiles + L::kTeams * c - 1) / (L::kTeams * c) * ((shares + sms - 1) / sms);
     const double time = rounds * (slice + 1.5) + (slices > 1 ? 6 + 4e-6 * p.nq * p.n * slices : 0);
     if (best == 0 || time < best) {
       best = time;
@@ -284,7 +284,7 @@ cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, 
   }
   CUtensorMap map;
   if (e == cudaSuccess && !codes_map(&map, v, p.units, 64, kWideRows, CU_TENSOR_MAP_SWIZZLE_64B)) e = cudaErrorInvalidValue;
-  const uint64_t ctas = std::min<uint64_t>(columns, (p.tiles + kWideTeams - 1) / kWideTeams) * shares;
+  const uint64_t ctas = std::min<uint64_t>(columns, (p.tiles + L::kTeams - 1) / L::kTeams) * shares;
   if (e == cudaSuccess)
     e = p.slices > 1 || out_type == 0 ? launch_wide<NC, G, F32, float>(map, p, ctas, bytes(p.slice, p.depth), st)
         : out_type == 1               ? launch_wide<NC, G, F32, __half>(map, p, ctas, bytes(p.slice, p.depth), st)
@@ -294,14 +294,16 @@ cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, 
   return e;
 }
 
-// Columns are queries, two for one of f32.
+// Columns are queries, two for one of f32. An instruction of 96 columns takes no longer than one of 64, but each
+// column has its additions, and its scores: as few chunks as there can be, the narrower ones where they do.
 template <int G, bool F32>
 cudaError_t group_score4(const raven_rows* v, const raven_score4::Params& p, int out_type, int sms, cudaStream_t st) {
   const uint64_t columns = F32 ? 2 * p.nq : p.nq;
   return columns <= 8    ? run_score4<1, G, F32>(v, p, out_type, sms, st)
          : columns <= 16 ? run_score4<2, G, F32>(v, p, out_type, sms, st)
          : columns <= 32 ? run_wide<32, G, F32>(v, p, out_type, sms, st)
-                         : run_wide<64, G, F32>(v, p, out_type, sms, st);
+         : (columns + 63) / 64 > (columns + 95) / 96 ? run_wide<96, G, F32>(v, p, out_type, sms, st)
+                                                     : run_wide<64, G, F32>(v, p, out_type, sms, st);
 }
 
 template <bool F32>

@@ -78,7 +78,7 @@ struct Params {
 
 // A chunk of queries as the kernel takes it, NT * 8 columns: fragments (for each
 // unit and N tile 16 bytes a lane), then per group the columns' sums, then per
-// column what brings its sums back: alpha times a power of two, or where that is no
+// query what brings its sums back: alpha times a power of two, or where that is no
 // f32 a NaN, and the power as two factors. f32 queries have two columns side by
 // side, the second for what the first leaves and without sums.
 template <int NT>
@@ -90,12 +90,17 @@ struct Laid {
   __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t groups) {
     return frags(units) + sums(groups) + NT * 8 * 16;
   }
-  // Where a quarter of a unit of a column is; a group's sum (times 2^-24), where `to` are the sums.
+  // Where a quarter of a unit of a column is; a group's sum (times 2^-24), where `to` are the sums (of a block's groups
+  // so many).
   __device__ static uint32_t frag_at(uint32_t unit, uint32_t quarter, uint32_t col) {
     return (unit * NT + col / 8) * 512 + ((col & 7) * 4 + quarter) * 16;
   }
-  __device__ static void put_sum(uint8_t* to, uint32_t group, uint32_t col, float sum) {
+  __device__ static void put_sum(uint8_t* to, uint32_t group, uint32_t, uint32_t col, float sum) {
     ((float*)to)[group * (NT * 8) + col] = sum;
+  }
+  // What brings query q's sums back: a factor, two, a flag.
+  __device__ static void put_back(float* back, uint32_t q, float f, float k0, float k1, float flag) {
+    *(float4*)(back + 4 * q) = make_float4(f, k0, k1, flag);
   }
 };
 
@@ -161,8 +166,8 @@ __device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, 
     for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const uint32_t c = col + (F32 ? 2 * q : q);
     if (i % L == 0 && i / L < p.groups) {
-      Q::put_sum(sums, i / L, c, sum * 0x1p-24f);
-      if (F32) Q::put_sum(sums, i / L, c + 1, 0.f);
+      Q::put_sum(sums, i / L, kBlock / G, c, sum * 0x1p-24f);
+      if (F32) Q::put_sum(sums, i / L, kBlock / G, c + 1, 0.f);
     }
     if (i < p.units * 4) {
       __align__(16) __half part[F32 ? 2 : 1][8];
@@ -179,15 +184,11 @@ __device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, 
     }
     if (i == 0) {
       const int b = 24 - e;  // -139 .. 137
-#pragma unroll
-      for (int h = 0; h < (F32 ? 2 : 1); ++h) {
-        // exact where alpha's exponent leaves it among the normal numbers
-        const int a = p.alpha == 0.f ? 0 : ilogbf(p.alpha) + b;
-        const bool plain = a >= -120 && a <= 120 && (p.alpha == 0.f || fabsf(p.alpha) < INFINITY) && b >= -126 && b <= 127;
-        const float k0 = bad ? __uint_as_float(0x7fc00000u) : pow2(b / 2), k1 = pow2(b - b / 2);
-        *(float4*)(back + 4 * (c + h)) = make_float4(plain && !bad ? p.alpha * k0 * k1 : __uint_as_float(0x7fc00000u), k0, k1,
-                                                     plain || bad ? 0.f : 1.f);
-      }
+      // exact where alpha's exponent leaves it among the normal numbers
+      const int a = p.alpha == 0.f ? 0 : ilogbf(p.alpha) + b;
+      const bool plain = a >= -120 && a <= 120 && (p.alpha == 0.f || fabsf(p.alpha) < INFINITY) && b >= -126 && b <= 127;
+      const float none = __uint_as_float(0x7fc00000u), k0 = bad ? none : pow2(b / 2), k1 = pow2(b - b / 2);
+      Q::put_back(back, F32 ? c / 2 : c, plain && !bad ? p.alpha * k0 * k1 : none, k0, k1, plain || bad ? 0.f : 1.f);
     }
   }
 }
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(Layout<NT, G>::kThreads, 1) score4_kernel(cons
   }
   __syncthreads();
   bool plain = true;  // every column has one factor
-  for (uint32_t c = 0; c < NT * 8; ++c) plain &= back[4 * c + 3] == 0.f;
+  for (uint32_t q = 0; q < kQueries; ++q) plain &= back[4 * q + 3] == 0.f;
 
   bool ok = true;  // no wait has run out
   uint32_t now = 0, phases = 0;  // the stage that is taken next; parities of the stages
@@ -531,11 +532,11 @@ __global__ void __launch_bounds__(Layout<NT, G>::kThreads, 1) score4_kernel(cons
         if (query < p.nq) {
           __align__(16) O o[R];
           if (plain) {
-            const float f = back[4 * col];
+            const float f = back[4 * (F32 ? col / 2 : col)];
 #pragma unroll
             for (int r = 0; r < R; ++r) o[r] = rounded<O>(fmaf(f, y[r], bias[r]));
           } else {
-            const float k0 = back[4 * col + 1], k1 = back[4 * col + 2];
+            const float k0 = back[4 * (F32 ? col / 2 : col) + 1], k1 = back[4 * (F32 ? col / 2 : col) + 2];
 #pragma unroll
             for (int r = 0; r < R; ++r) o[r] = rounded<O>(fmaf(p.alpha, y[r] * k0 * k1, bias[r]));
           }

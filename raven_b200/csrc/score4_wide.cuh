@@ -11,10 +11,14 @@
 // and its bandwidth goes to them. A scale group is a chain of instructions of its
 // own, the last of which adds z * sum(q): three operands z * 2^-10 against the sum in
 // three f16 parts. The thread then reads its row's sums of the group and adds them,
-// times the group's step, to its own in registers. Three such groups of warps per SM
-// work on tiles of their own, so that one's instructions and waits are hidden by the
-// others'. A thread has all scores of its row, and a warp writes 32 scores of a query
-// side by side, wherever the query's scores start.
+// times the group's step, to its own in registers. Three or four such groups of warps
+// per SM (teams) work on tiles of their own, so that one's instructions and waits are
+// hidden by the others'. A thread has all scores of its row, and a warp writes 32
+// scores of a query side by side, wherever the query's scores start.
+//
+// An instruction of 16 values takes about 64 cycles up to 96 columns, since that is
+// how long its M side takes to come from tensor memory: 576 for a block, of which
+// teams that wait for one another's make 1000.
 #pragma once
 
 #include "score4.cuh"
@@ -23,7 +27,8 @@ namespace raven_score4 {
 
 // A chunk of queries: K blocks of 64 values (two units), for each column 128 bytes
 // in the 128-byte swizzle; then blocks of four groups' sums laid out the same way,
-// 16 operands a group, of which three are its sum; then what brings sums back.
+// 16 operands a group: its sum's three parts at four times its number in its block of
+// values, zeros against the z of the others; then what brings sums back.
 template <int NC>
 struct WideLaid {
   static constexpr uint32_t kColumns = NC;
@@ -36,33 +41,45 @@ struct WideLaid {
   __device__ static uint32_t frag_at(uint32_t unit, uint32_t quarter, uint32_t col) {
     return unit / 2 * kBlockBytes + col * 128 + ((((unit & 1) * 4 + quarter) ^ (col & 7)) * 16);
   }
+  // What brings query q's sums back: a factor, or two and a flag.
+  __device__ static void put_back(float* back, uint32_t q, float f, float k0, float k1, float flag) {
+    back[q] = f;
+    back[NC + 2 * q] = k0;
+    back[NC + 2 * q + 1] = k1;
+    back[3 * NC + q] = flag;
+  }
   // sum: times 2^-24; against z * 2^-10 it has to be 2^10 times that. Below 2^8, so three parts leave less than 2^-24.
-  __device__ static void put_sum(uint8_t* to, uint32_t group, uint32_t col, float sum) {
+  __device__ static void put_sum(uint8_t* to, uint32_t group, uint32_t per, uint32_t col, float sum) {
     const float x = sum * 0x1p10f;
     const __half hi = __float2half_rn(x);
     const float r = x - __half2float(hi);
     const __half mid = __float2half_rn(r), lo = __float2half_rn(r - __half2float(mid));
-    __align__(16) __half part[8] = {hi, mid, lo, __half(0.f), __half(0.f), __half(0.f), __half(0.f), __half(0.f)};
+    const __half zero = __half(0.f);
+    const uint32_t place = group % per;  // in its block of values
+    const bool odd = place & 1;
+    __align__(16) __half part[8] = {odd ? zero : hi, odd ? zero : mid, odd ? zero : lo, zero,
+                                    odd ? hi : zero, odd ? mid : zero, odd ? lo : zero, zero};
     uint8_t* at = to + group / 4 * kBlockBytes + col * 128;
-    *(uint4*)(at + ((((group & 3) * 2) ^ (col & 7)) * 16)) = *(const uint4*)part;
-    *(uint4*)(at + ((((group & 3) * 2 + 1) ^ (col & 7)) * 16)) = make_uint4(0, 0, 0, 0);
+    const uint32_t in = (group & 3) * 2, half = place / 2;
+    *(uint4*)(at + (((in + half) ^ (col & 7)) * 16)) = *(const uint4*)part;
+    *(uint4*)(at + (((in + 1 - half) ^ (col & 7)) * 16)) = make_uint4(0, 0, 0, 0);
   }
 };
 
-constexpr uint32_t kWideRows = 128, kWideTeams = 3;  // rows of a tile; groups of four warps
-constexpr uint32_t kWideThreads = kWideTeams * 128;
-constexpr uint32_t kWideDepth = 4;                   // tiles under way per team, at most
+constexpr uint32_t kWideRows = 128;  // of a tile
+constexpr uint32_t kWideDepth = 4;   // tiles under way per team, at most
 constexpr uint32_t kWideStage = kWideRows * 64;
 
 template <int NC>
 struct Wide {
-  // tensor memory of a team: operands of a block, of its groups' z, a group's sums
-  static constexpr uint32_t kZ = 64, kAcc = 96, kTeam = 160;
-  static_assert(kAcc + NC <= kTeam && kWideTeams * kTeam <= 512, "tensor memory has 512 columns");
+  // tensor memory of a team: operands of a block, a group's sums; in its last columns, the z of a block's groups
+  static constexpr uint32_t kAcc = 64, kTeam = kAcc + NC, kZ = 480;
+  static constexpr uint32_t kTeams = NC == 32 ? 4 : 3, kThreads = kTeams * 128;
+  static_assert(kTeams * kTeam <= kZ && kZ + 8 * kTeams <= 512, "tensor memory has 512 columns");
   static constexpr uint32_t kHead = 1024;  // barriers, the place of the tensor memory; TMA's places start on 1024 bytes
   static constexpr uint32_t kTops = NC * 4;
   __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t groups, uint32_t depth) {
-    return 1024 + kHead + (uint64_t)kWideTeams * depth * kWideStage + WideLaid<NC>::bytes(units, groups) + kTops;
+    return 1024 + kHead + (uint64_t)kTeams * depth * kWideStage + WideLaid<NC>::bytes(units, groups) + kTops;
   }
 };
 
@@ -71,6 +88,12 @@ __device__ inline void tmem_st(uint32_t at, const uint32_t* v);
 template <>
 __device__ inline void tmem_st<2>(uint32_t at, const uint32_t* v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};\n" ::"r"(at), "r"(v[0]), "r"(v[1]) : "memory");
+}
+template <>
+__device__ inline void tmem_st<4>(uint32_t at, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3])
+               : "memory");
 }
 template <>
 __device__ inline void tmem_st<8>(uint32_t at, const uint32_t* v) {
@@ -116,7 +139,7 @@ __device__ inline void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc
 __device__ inline bool warp_waits(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); }
 
 template <int NC, int G, bool F32, typename O>
-__global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
+__global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
   using Q = WideLaid<NC>;
   using S = Wide<NC>;
   constexpr uint32_t kQueries = F32 ? NC / 2 : NC, W = kBlock / G, U = G / kUnit;
@@ -127,9 +150,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
   const uint32_t done = bars + 8 * kWideDepth;
   volatile uint32_t* slot_of_tmem = (volatile uint32_t*)(smem + 512);
   uint8_t* ring = smem + S::kHead + team * p.depth * kWideStage;
-  uint8_t* held = smem + S::kHead + kWideTeams * p.depth * kWideStage;
+  uint8_t* held = smem + S::kHead + S::kTeams * p.depth * kWideStage;
   const uint32_t shares = p.chunks * p.slices, share = blockIdx.x % shares;
-  const uint32_t step = gridDim.x / shares * kWideTeams, first = blockIdx.x / shares * kWideTeams + team;
+  const uint32_t step = gridDim.x / shares * S::kTeams, first = blockIdx.x / shares * S::kTeams + team;
   const uint32_t slice = share % p.slices;
   const uint64_t chunk = share / p.slices;
   const uint32_t b0 = slice * p.slice, blocks = min(p.slice, p.blocks - b0);
@@ -147,8 +170,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
   raven_tc::tc_fence_before();
   __syncthreads();
   raven_tc::tc_fence_after();
-  const uint32_t tmem = *slot_of_tmem + team * S::kTeam;
-  const uint32_t mine = tmem + ((warp & 3) << 21);  // this warp's 32 lanes
+  const uint32_t tmem = *slot_of_tmem + team * S::kTeam, tmem_z = *slot_of_tmem + S::kZ + 8 * team;
+  const uint32_t lanes = (warp & 3) << 21, mine = tmem + lanes;  // this warp's 32 lanes
   after_previous();
 
   // copies: by the team's first thread
@@ -176,22 +199,21 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
   } else {
     const uint8_t* from = p.laid + chunk * Q::bytes(p.units, p.groups);
     auto bring = [&](void* to, const uint8_t* what, uint32_t bytes) {
-      for (uint32_t i = tid * 16; i < bytes; i += kWideThreads * 16) *(uint4*)((uint8_t*)to + i) = *(const uint4*)(what + i);
+      for (uint32_t i = tid * 16; i < bytes; i += S::kThreads * 16) *(uint4*)((uint8_t*)to + i) = *(const uint4*)(what + i);
     };
     bring(held, from + Q::frags(4 * b0), (uint32_t)Q::frags(units));
     from += Q::frags(p.units);
     bring(sums, from + Q::sums(b0 * W), (uint32_t)Q::sums(groups));
     bring(back, from + Q::sums(p.groups), NC * 16);
   }
-  {  // the operands behind a group's three z stay 0
+  {  // of the operands beside the z that are written, those of groups that are not there stay 0
     const uint32_t zero[8] = {};
-#pragma unroll
-    for (uint32_t g = 0; g < W; ++g) tmem_st<8>(mine + S::kZ + 8 * g, zero);
+    tmem_st<8>(tmem_z + lanes, zero);
   }
   asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // the queries, to the instructions
   __syncthreads();
   bool plain = true;  // every column has one factor
-  for (uint32_t c = 0; c < NC; ++c) plain &= back[4 * c + 3] == 0.f;
+  for (uint32_t q = 0; q < kQueries; ++q) plain &= back[3 * NC + q] == 0.f;
   const uint64_t b_desc = raven_tc::sw128_desc(smem_u32(held)), z_desc = raven_tc::sw128_desc(smem_u32(sums));
   constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(NC >> 3) << 17) | (8u << 24);  // f32 sums, f16 operands
 
@@ -258,12 +280,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
         } else {
           put_unit(0, c[0], c[1], c[2], c[3]);
         }
+        uint32_t zs[2 * W];
 #pragma unroll
         for (uint32_t g = 0; g < W; ++g) {
           const __half2 z = __float2half2_rn(raven_int4::zero_of(word[g]) * 0x1p-10f);
-          const uint32_t v = *(const uint32_t*)&z, three[2] = {v, v & 0xffffu};
-          tmem_st<2>(mine + S::kZ + 8 * g, three);
+          zs[2 * g] = *(const uint32_t*)&z;
+          zs[2 * g + 1] = zs[2 * g] & 0xffffu;
         }
+        tmem_st<2 * W>(tmem_z + lanes, zs);
         asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
       }
       const uint32_t taken = now;
@@ -291,7 +315,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
             add = 1;
           }
           const uint32_t group = b * W + g;
-          mma_ts(tmem + S::kAcc, tmem + S::kZ + 8 * g, z_desc + (group / 4 * Q::kBlockBytes >> 4) + (group & 3) * 2, idesc, 1);
+          mma_ts(tmem + S::kAcc, tmem_z, z_desc + (group / 4 * Q::kBlockBytes >> 4) + (group & 3) * 2, idesc, 1);
           raven_tc::mma_commit(done);
         }
         if (ok && !warp_waits(done, done_phase)) ok = false;
@@ -314,13 +338,28 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       const float bias = p.bias ? p.bias[row] : 0.f;
       O* to = (O*)p.out + slice * p.ld_slice + chunk * kQueries * p.ld + row;
       const uint32_t here = (uint32_t)min((uint64_t)kQueries, p.nq - chunk * kQueries);
+      if (plain && here == kQueries) {  // four at a time, without a branch between them
 #pragma unroll
-      for (uint32_t q = 0; q < kQueries; ++q) {
-        if (q >= here) break;
-        const uint32_t c = F32 ? 2 * q : q;
-        const float y = F32 ? total[c] + total[c + 1] : total[c];
-        *to = rounded<O>(plain ? fmaf(back[4 * c], y, bias) : fmaf(p.alpha, y * back[4 * c + 1] * back[4 * c + 2], bias));
-        to += p.ld;
+        for (uint32_t q = 0; q < kQueries; q += 4) {
+          const float4 f = *(const float4*)(back + q);
+          const float by[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k) {
+            const float y = F32 ? total[2 * (q + k)] + total[2 * (q + k) + 1] : total[q + k];
+            *to = rounded<O>(fmaf(by[k], y, bias));
+            to += p.ld;
+          }
+        }
+      } else {
+#pragma unroll
+        for (uint32_t q = 0; q < kQueries; ++q) {
+          if (q < here) {
+            const float y = F32 ? total[2 * q] + total[2 * q + 1] : total[q];
+            *to = rounded<O>(plain ? fmaf(back[q], y, bias)
+                                   : fmaf(p.alpha, y * back[NC + 2 * q] * back[NC + 2 * q + 1], bias));
+            to += p.ld;
+          }
+        }
       }
     }
   }
