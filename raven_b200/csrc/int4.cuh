@@ -164,13 +164,38 @@ __device__ inline uint32_t codes_of(float (&x)[8], float step, int z) {
 // (element e of the first 16C at (e % 16) * C + e / 16).
 template <typename T, uint32_t L, bool VEC, bool LANE>
 __global__ void __launch_bounds__(256, 3) write_kernel(const Write p) {
-  __shared__ int32_t dest[kRun];
+  __shared__ int32_t dest[2][kRun];  // where the rows of a run, and of the next one, are held; -1: nowhere
   __shared__ uint32_t later[kRun];
   after_previous();
+  // With a table the next run's rows are settled while this one's are worked on: two reads far apart, one after the other.
+  auto settle = [&](uint64_t r0, int32_t* to) {
+    if (r0 + threadIdx.x >= p.m || threadIdx.x >= p.run) return;
+    int64_t s = (int64_t)p.slots[r0 + threadIdx.x];
+    if (s >= (int64_t)p.n) {
+      raven_score::tell(p.status, kStatusIds);
+      s = -1;
+    }
+    if (s >= 0 && p.table) {
+      uint32_t h = claim_hash((uint32_t)s) >> (32 - p.bits);
+      for (uint32_t tries = 0; tries >> p.bits == 0; ++tries) {
+        const Claim c = p.table[h];
+        if (c.slot == (uint32_t)s) {
+          if (c.row != (int32_t)(r0 + threadIdx.x)) s = -1;
+          break;
+        }
+        h = (h + 1) & ((1u << p.bits) - 1);
+      }
+    }
+    to[threadIdx.x] = s < 0 ? -1 : (int32_t)s;
+    later[threadIdx.x] = 0;
+  };
+  const uint64_t stride = (uint64_t)gridDim.x * p.run;
+  uint32_t cur = 0;
+  if (p.slots) settle((uint64_t)blockIdx.x * p.run, dest[0]);
   constexpr uint32_t G = 8 * L, kGroups = 32 / L;  // groups of a warp's piece
   const uint32_t ng = (p.dim + G - 1) / G, lane = threadIdx.x & 31;
   const uint32_t wide = (p.dim + kBlock - 1) / kBlock * (kBlock / G);  // words of a row as it is held
-  for (uint64_t r0 = (uint64_t)blockIdx.x * p.run; r0 < p.m; r0 += (uint64_t)gridDim.x * p.run) {
+  for (uint64_t r0 = (uint64_t)blockIdx.x * p.run; r0 < p.m; r0 += stride) {
     const uint32_t rows = (uint32_t)min((uint64_t)p.run, p.m - r0), items = rows * p.per;
     float x[kItems][8];
     uint32_t from[kItems], at[kItems];  // a piece's row of the run, which of its eights
@@ -205,34 +230,18 @@ __global__ void __launch_bounds__(256, 3) write_kernel(const Write p) {
       }
     };
     load(0);  // on the way while the slots are settled
-    if (threadIdx.x < rows) {
-      int64_t s = p.slots ? (int64_t)p.slots[r0 + threadIdx.x] : (int64_t)(r0 + threadIdx.x);
-      if (s >= (int64_t)p.n) {
-        raven_score::tell(p.status, kStatusIds);
-        s = -1;
-      }
-      if (s >= 0 && p.table) {
-        uint32_t h = claim_hash((uint32_t)s) >> (32 - p.bits);
-        for (uint32_t tries = 0; tries >> p.bits == 0; ++tries) {
-          const Claim c = p.table[h];
-          if (c.slot == (uint32_t)s) {
-            if (c.row != (int32_t)(r0 + threadIdx.x)) s = -1;
-            break;
-          }
-          h = (h + 1) & ((1u << p.bits) - 1);
-        }
-      }
-      dest[threadIdx.x] = s < 0 ? -1 : (int32_t)s;
-      later[threadIdx.x] = 0;
-    }
-    __syncthreads();
-    if (p.slots && !p.table) {
-      for (uint64_t j = r0 + 1 + threadIdx.x; j < p.m; j += 256) {
-        const int32_t s = p.slots[j];
-        for (uint32_t k = 0; k < rows && r0 + k < j; ++k)
-          if (dest[k] == s) later[k] = 1;
-      }
+    if (p.slots) {
       __syncthreads();
+      if (p.table) {
+        settle(r0 + stride, dest[cur ^ 1]);
+      } else {
+        for (uint64_t j = r0 + 1 + threadIdx.x; j < p.m; j += 256) {
+          const int32_t s = p.slots[j];
+          for (uint32_t k = 0; k < rows && r0 + k < j; ++k)
+            if (dest[cur][k] == s) later[k] = 1;
+        }
+        __syncthreads();
+      }
     }
     for (uint32_t u0 = 0; u0 < items; u0 += 256 * kItems) {
       if (u0) load(u0);
@@ -272,7 +281,9 @@ __global__ void __launch_bounds__(256, 3) write_kernel(const Write p) {
       for (int n = 0; n < kItems; ++n) {
         uint32_t w = __shfl_sync(0xffffffffu, scale, n * kGroups + lane / L);
         const uint32_t i = at[n], d = 8 * i;
-        const int32_t to = u0 + n * 256 + threadIdx.x < items && !later[from[n]] ? dest[from[n]] : -1;
+        int32_t to = -1;
+        if (u0 + n * 256 + threadIdx.x < items)
+          to = !p.slots ? (int32_t)(r0 + from[n]) : later[from[n]] ? -1 : dest[cur][from[n]];
         if (to < 0) continue;
         uint32_t word = 0;
         if (odd[n]) {
@@ -288,7 +299,11 @@ __global__ void __launch_bounds__(256, 3) write_kernel(const Write p) {
           for (uint32_t g = ng; g < wide; ++g) words[g] = 0;
       }
     }
-    __syncthreads();
+    if (p.slots && !p.table) {
+      __syncthreads();
+      settle(r0 + stride, dest[cur ^ 1]);
+    }
+    cur ^= 1;
   }
 }
 

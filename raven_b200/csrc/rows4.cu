@@ -128,7 +128,7 @@ cudaError_t launch_read(raven_int4::Read p, int sms, cudaStream_t st) {
 // Scores.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kMostShared = 227 * 1024;
-constexpr uint64_t kOwnLayout = 16384;  // values that each CTA lays out for itself
+constexpr uint64_t kOwnLayout = 16384;  // values of queries that each CTA lays out for itself
 
 // Codes as boxes of `wide` bytes (64: a block) x `rows` rows; what is past a row's end or the last row reads 0.
 bool codes_map(CUtensorMap* m, const raven_rows* v, uint32_t units, uint32_t wide, uint32_t rows, CUtensorMapSwizzle swizzle) {
@@ -142,11 +142,11 @@ bool codes_map(CUtensorMap* m, const raven_rows* v, uint32_t units, uint32_t wid
            swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NT, int G, bool F32, typename O>
+template <int NT, int MT, int G, bool F32, typename O>
 cudaError_t launch_score4(const CUtensorMap& map, const raven_score4::Params& p, uint64_t ctas, uint64_t smem, cudaStream_t st) {
   using namespace raven_score4;
   static Allowed allowed(kMostShared);
-  return launch(score4_kernel<NT, G, F32, O>, ctas, Layout<NT, G>::kThreads, (uint32_t)smem, allowed, st, map, p);
+  return launch(score4_kernel<NT, MT, G, F32, O>, ctas, Layout<NT, MT, G>::kThreads, (uint32_t)smem, allowed, st, map, p);
 }
 
 cudaError_t launch_join(const raven_score4::Join& j, int out_type, int sms, cudaStream_t st) {
@@ -157,10 +157,10 @@ cudaError_t launch_join(const raven_score4::Join& j, int out_type, int sms, cuda
                 0, none, st, j);
 }
 
-template <int NT, int G, bool F32>
+template <int NT, int MT, int G, bool F32>
 cudaError_t run_score4(const raven_rows* v, raven_score4::Params p, int out_type, int sms, cudaStream_t st) {
   using namespace raven_score4;
-  using L = Layout<NT, G>;
+  using L = Layout<NT, MT, G>;
   using Q = Laid<NT>;
   constexpr uint32_t kQueries = F32 ? NT * 4 : NT * 8;
   p.chunks = (uint32_t)((p.nq + kQueries - 1) / kQueries);
@@ -176,12 +176,12 @@ cudaError_t run_score4(const raven_rows* v, raven_score4::Params p, int out_type
   p.slices = (p.blocks + p.slice - 1) / p.slice;
   const uint32_t shares = p.chunks * p.slices;
   const uint64_t columns = std::max<uint64_t>(1, (uint64_t)sms / shares);  // CTAs of a share
-  // Warps that share a row: as few as keep them evenly busy. In blocks of 128 values, what the busiest warp takes,
-  // with a block's time for sums that meet.
+  // Warps that share a row: those that leave the busiest SM least, in blocks of a warp's tile, with half a block of
+  // each warp for a tile's end and sums that meet.
   uint64_t best = ~0ull;
   for (uint32_t split = 1; split <= p.slice && L::kWarps % split == 0; split *= 2) {
     const uint64_t rows = L::kRows * (L::kWarps / split), tiles = (p.n + rows - 1) / rows;
-    const uint64_t time = (tiles + columns - 1) / columns * ((p.slice + split - 1) / split + (split > 1 ? 1 : 0));
+    const uint64_t time = (tiles + columns - 1) / columns * (2 * ((p.slice + split - 1) / split) + 1);
     if (time < best) {
       best = time;
       p.split = split;
@@ -193,7 +193,7 @@ cudaError_t run_score4(const raven_rows* v, raven_score4::Params p, int out_type
   while (L::bytes(units, groups, p.split, p.depth) > kMostShared) --p.depth;
   uint8_t* tmp = nullptr;
   cudaError_t e = cudaSuccess;
-  const bool lay = p.slices > 1 || (uint64_t)kQueries * p.dim > kOwnLayout;
+  const bool lay = std::min<uint64_t>(p.nq, kQueries) * p.dim > kOwnLayout;
   const uint64_t laid = lay ? (p.chunks * Q::bytes(p.units, p.groups) + 255) / 256 * 256 : 0;
   const uint64_t wide = (p.n + 3) / 4 * 4, sums = p.slices > 1 ? p.slices * p.nq * wide * 4 : 0;
   if (laid + sums && (e = cudaMallocAsync((void**)&tmp, laid + sums, st)) != cudaSuccess) return e;
@@ -216,9 +216,9 @@ cudaError_t run_score4(const raven_rows* v, raven_score4::Params p, int out_type
   if (e == cudaSuccess && !codes_map(&map, v, p.units, std::min(64u, 16 * p.units), L::kRows, CU_TENSOR_MAP_SWIZZLE_NONE)) e = cudaErrorInvalidValue;
   const uint64_t ctas = std::min<uint64_t>(columns, p.tiles) * shares, smem = L::bytes(units, groups, p.split, p.depth);
   if (e == cudaSuccess)
-    e = p.slices > 1 || out_type == 0 ? launch_score4<NT, G, F32, float>(map, p, ctas, smem, st)
-        : out_type == 1               ? launch_score4<NT, G, F32, __half>(map, p, ctas, smem, st)
-                                      : launch_score4<NT, G, F32, __nv_bfloat16>(map, p, ctas, smem, st);
+    e = p.slices > 1 || out_type == 0 ? launch_score4<NT, MT, G, F32, float>(map, p, ctas, smem, st)
+        : out_type == 1               ? launch_score4<NT, MT, G, F32, __half>(map, p, ctas, smem, st)
+                                      : launch_score4<NT, MT, G, F32, __nv_bfloat16>(map, p, ctas, smem, st);
   if (p.slices > 1 && e == cudaSuccess) e = launch_join(j, out_type, sms, st);
   if (tmp) cudaFreeAsync(tmp, st);
   return e;
@@ -264,7 +264,7 @@ cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, 
   while (bytes(p.slice, p.depth) > kMostShared) --p.depth;
   uint8_t* tmp = nullptr;
   cudaError_t e = cudaSuccess;
-  const bool lay = p.slices > 1 || (uint64_t)kQueries * p.dim > kOwnLayout;
+  const bool lay = std::min<uint64_t>(p.nq, kQueries) * p.dim > kOwnLayout;
   const uint64_t laid = lay ? (p.chunks * Q::bytes(p.units, p.groups) + 255) / 256 * 256 : 0;
   const uint64_t wide = (p.n + 3) / 4 * 4, sums = p.slices > 1 ? p.slices * p.nq * wide * 4 : 0;
   if (laid + sums && (e = cudaMallocAsync((void**)&tmp, laid + sums, st)) != cudaSuccess) return e;
@@ -299,8 +299,13 @@ cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, 
 template <int G, bool F32>
 cudaError_t group_score4(const raven_rows* v, const raven_score4::Params& p, int out_type, int sms, cudaStream_t st) {
   const uint64_t columns = F32 ? 2 * p.nq : p.nq;
-  return columns <= 8    ? run_score4<1, G, F32>(v, p, out_type, sms, st)
-         : columns <= 16 ? run_score4<2, G, F32>(v, p, out_type, sms, st)
+  if (columns <= 8) {  // four M tiles a warp, but where rows are so long that a CTA could not hold its queries beside them
+    using namespace raven_score4;
+    using L = Layout<1, 4, G>;
+    const bool fits = L::bytes(p.units, p.groups, std::min(L::kWarps, p.blocks), L::kLeast) <= kMostShared;
+    return fits ? run_score4<1, 4, G, F32>(v, p, out_type, sms, st) : run_score4<1, 2, G, F32>(v, p, out_type, sms, st);
+  }
+  return columns <= 16 ? run_score4<2, 2, G, F32>(v, p, out_type, sms, st)
          : columns <= 32 ? run_wide<32, G, F32>(v, p, out_type, sms, st)
          : (columns + 63) / 64 > (columns + 95) / 96 ? run_wide<96, G, F32>(v, p, out_type, sms, st)
                                                      : run_wide<64, G, F32>(v, p, out_type, sms, st);

@@ -121,15 +121,17 @@ __device__ inline void eight(const T* x, uint32_t d, uint32_t dim, bool whole, f
 }
 
 // Queries [first, first + count) as columns from `col` on, by all of a CTA's
-// threads. top: `count` words of shared memory.
+// threads: of their values a slice of whole blocks, `units` from unit `unit0` on
+// with so many groups. top: `count` words of shared memory.
 template <class Q, int G, typename T>
-__device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, uint32_t col, uint8_t* to, uint32_t* top) {
+__device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, uint32_t col, uint32_t unit0, uint32_t units,
+                               uint32_t groups, uint8_t* to, uint32_t* top) {
   constexpr bool F32 = std::is_same<T, float>::value;
   constexpr uint32_t L = G / 8;
-  uint8_t* sums = to + Q::frags(p.units);
-  float* back = (float*)(sums + Q::sums(p.groups));
-  const uint32_t n8 = (p.units * 4 + L - 1) / L * L;  // eights, up to whole groups
-  const uint32_t items = count * n8;
+  uint8_t* sums = to + Q::frags(units);
+  float* back = (float*)(sums + Q::sums(groups));
+  const uint32_t all = (p.dim + 7) / 8, n8 = (units * 4 + L - 1) / L * L;  // eights: of a query, of the slice up to whole groups
+  const uint32_t there = (uint32_t)min((uint64_t)count, p.nq > first ? p.nq - first : 0);
   auto load = [&](uint32_t q, uint32_t i, float(&v)[8]) {
     if (first + q < p.nq) {
       eight((const T*)p.q + (first + q) * p.ld_q, 8 * i, p.dim, p.whole_q, v);
@@ -140,23 +142,31 @@ __device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, 
   };
   for (uint32_t i = threadIdx.x; i < count; i += blockDim.x) top[i] = 0;
   __syncthreads();
-  for (uint32_t u = threadIdx.x; u < items; u += blockDim.x) {
-    const uint32_t q = u / n8;
-    float v[8];
-    load(q, u - q * n8, v);
+  for (uint32_t u0 = 0; u0 < there * all; u0 += blockDim.x) {
+    const uint32_t u = u0 + threadIdx.x, q = min(u / all, there - 1);
     uint32_t m = 0;
+    if (u < there * all) {
+      float v[8];
+      load(q, u - q * all, v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
-    atomicMax(&top[q], m);
+      for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
+    }
+    // one of a warp's lanes where they have one query
+    if (__all_sync(0xffffffffu, q == __shfl_sync(0xffffffffu, q, 0))) {
+      m = __reduce_max_sync(0xffffffffu, m);
+      if ((threadIdx.x & 31) == 0) atomicMax(&top[q], m);
+    } else {
+      atomicMax(&top[q], m);
+    }
   }
   __syncthreads();
-  for (uint32_t u0 = 0; u0 < items; u0 += blockDim.x) {
+  for (uint32_t u0 = 0; u0 < count * n8; u0 += blockDim.x) {
     const uint32_t u = u0 + threadIdx.x, q = min(u / n8, count - 1), i = u - q * n8;  // past the last item: past the last unit
     const bool bad = top[q] >= 0x7f800000u;
     const int e = top[q] == 0 || bad ? 14 : 14 - ilogbf(__uint_as_float(top[q]));  // -113 .. 163
     const float m0 = pow2(e / 2), m1 = pow2(e - e / 2);
     float v[8], sum = 0.f;
-    load(q, i, v);
+    load(q, 4 * unit0 + i, v);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       v[k] = bad ? 0.f : v[k] * m0 * m1;
@@ -165,11 +175,11 @@ __device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, 
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const uint32_t c = col + (F32 ? 2 * q : q);
-    if (i % L == 0 && i / L < p.groups) {
+    if (i % L == 0 && i / L < groups) {
       Q::put_sum(sums, i / L, kBlock / G, c, sum * 0x1p-24f);
       if (F32) Q::put_sum(sums, i / L, kBlock / G, c + 1, 0.f);
     }
-    if (i < p.units * 4) {
+    if (i < units * 4) {
       __align__(16) __half part[F32 ? 2 : 1][8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -194,13 +204,14 @@ __device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, 
 }
 
 template <class Q, int G, bool F32>
-__device__ inline void lay_out_any(const Params& p, uint64_t first, uint32_t count, uint32_t col, uint8_t* to, uint32_t* top) {
+__device__ inline void lay_out_any(const Params& p, uint64_t first, uint32_t count, uint32_t col, uint32_t unit0, uint32_t units,
+                                   uint32_t groups, uint8_t* to, uint32_t* top) {
   if constexpr (F32)
-    lay_out<Q, G, float>(p, first, count, col, to, top);
+    lay_out<Q, G, float>(p, first, count, col, unit0, units, groups, to, top);
   else if (p.q_type == 1)
-    lay_out<Q, G, __half>(p, first, count, col, to, top);
+    lay_out<Q, G, __half>(p, first, count, col, unit0, units, groups, to, top);
   else
-    lay_out<Q, G, __nv_bfloat16>(p, first, count, col, to, top);
+    lay_out<Q, G, __nv_bfloat16>(p, first, count, col, unit0, units, groups, to, top);
 }
 
 // All chunks, a CTA per query.
@@ -210,7 +221,7 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const Params p, uint8_t* t
   __shared__ uint32_t top[1];
   after_previous();
   const uint32_t chunk = blockIdx.x / kQueries, q = blockIdx.x - chunk * kQueries;
-  lay_out_any<Q, G, F32>(p, blockIdx.x, 1, F32 ? 2 * q : q, to + chunk * Q::bytes(p.units, p.groups), top);
+  lay_out_any<Q, G, F32>(p, blockIdx.x, 1, F32 ? 2 * q : q, 0, p.units, p.groups, to + chunk * Q::bytes(p.units, p.groups), top);
 }
 
 template <int B>
@@ -249,20 +260,19 @@ __device__ inline void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int NT, int G>
+template <int NT, int MT, int G>  // MT: M tiles of a warp, as many as its registers allow
 struct Layout {
-  static constexpr int kMT = NT == 1 ? 4 : 2;             // M tiles of a warp: as many as its registers allow
-  static constexpr int kAtOnce = NT == 1 ? 1 : kMT;       // M tiles that go through a block together
-  static constexpr uint32_t kRows = 16 * kMT;             // rows of its tile
+  static constexpr int kAtOnce = NT == 1 ? 1 : MT;       // M tiles that go through a block together
+  static constexpr uint32_t kRows = 16 * MT;             // rows of its tile
   static constexpr uint32_t kWarps = 16;
   static constexpr uint32_t kThreads = kWarps * 32;
   static constexpr uint32_t kWords = kBlock / G;          // scale words of a row's block
   static constexpr uint32_t kCodeBytes = kRows * 64, kWordBytes = kRows * kWords * 4;
-  static constexpr uint32_t kPart = 32 * 4 * kMT * NT * 4;  // a warp's sums
+  static constexpr uint32_t kPart = 32 * 4 * MT * NT * 4;  // a warp's sums
   static constexpr uint32_t kBars = kWarps * kMaxDepth * 8;  // in front of the rings
   static constexpr uint32_t kTops = NT * 8 * 4;
   static_assert(kBars % 128 == 0 && kCodeBytes % 128 == 0, "a TMA copy's place in shared memory");
-  static constexpr uint32_t kLeast = NT == 1 ? 2 : 3;      // stages of a ring
+  static constexpr uint32_t kLeast = MT == 4 ? 2 : 3;      // stages of a ring
   // what every call needs: rings, a block of queries, sums that meet
   static_assert(kBars + kLeast * (uint64_t)kWarps * (kCodeBytes + kWordBytes) + kTops + kWarps * kPart + 4 * Laid<NT>::kUnitBytes +
                 kWords * NT * 32 + NT * 64 <= 227 * 1024, "shared memory of a CTA");
@@ -283,12 +293,12 @@ __device__ inline T rounded(float v) {
     return __float2bfloat16_rn(v);
 }
 
-template <int NT, int G, bool F32, typename O>
-__global__ void __launch_bounds__(Layout<NT, G>::kThreads, 1) score4_kernel(const __grid_constant__ CUtensorMap map,
+template <int NT, int MT, int G, bool F32, typename O>
+__global__ void __launch_bounds__(Layout<NT, MT, G>::kThreads, 1) score4_kernel(const __grid_constant__ CUtensorMap map,
                                                                             const Params p) {
-  using S = Layout<NT, G>;
+  using S = Layout<NT, MT, G>;
   using Q = Laid<NT>;
-  constexpr int MT = S::kMT, R = 2 * MT;  // rows of a lane
+  constexpr int R = 2 * MT;  // rows of a lane
   constexpr uint32_t kQueries = F32 ? NT * 4 : NT * 8;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32, g = lane >> 2, t = lane & 3, odd = g & 1;
@@ -353,7 +363,7 @@ __global__ void __launch_bounds__(Layout<NT, G>::kThreads, 1) score4_kernel(cons
   float* sums = (float*)(held + Q::frags(units));
   float* back = sums + groups * NT * 8;
   if (p.q) {
-    lay_out_any<Q, G, F32>(p, chunk * kQueries, kQueries, 0, held, tops);
+    lay_out_any<Q, G, F32>(p, chunk * kQueries, kQueries, 0, 4 * b0, units, groups, held, tops);
   } else {
     const uint8_t* from = p.laid + chunk * Q::bytes(p.units, p.groups);
     auto bring = [&](void* to, const uint8_t* what, uint32_t bytes) {

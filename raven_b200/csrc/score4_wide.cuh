@@ -73,9 +73,9 @@ constexpr uint32_t kWideStage = kWideRows * 64;
 template <int NC>
 struct Wide {
   // tensor memory of a team: operands of a block, a group's sums; in its last columns, the z of a block's groups
-  static constexpr uint32_t kAcc = 64, kTeam = kAcc + NC, kZ = 480;
-  static constexpr uint32_t kTeams = NC == 32 ? 4 : 3, kThreads = kTeams * 128;
-  static_assert(kTeams * kTeam <= kZ && kZ + 8 * kTeams <= 512, "tensor memory has 512 columns");
+  static constexpr uint32_t kAcc = 64, kTeam = kAcc + NC;
+  static constexpr uint32_t kTeams = NC == 32 ? 4 : 3, kThreads = kTeams * 128, kZ = 512 - 8 * kTeams;
+  static_assert(kTeams * kTeam <= kZ, "tensor memory has 512 columns");
   static constexpr uint32_t kHead = 1024;  // barriers, the place of the tensor memory; TMA's places start on 1024 bytes
   static constexpr uint32_t kTops = NC * 4;
   __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t groups, uint32_t depth) {
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
   uint8_t* sums = held + Q::frags(units);
   float* back = (float*)(sums + Q::sums(groups));
   if (p.q) {
-    lay_out_any<Q, G, F32>(p, chunk * kQueries, kQueries, 0, held, (uint32_t*)(back + 4 * NC));
+    lay_out_any<Q, G, F32>(p, chunk * kQueries, kQueries, 0, 4 * b0, units, groups, held, (uint32_t*)(back + 4 * NC));
   } else {
     const uint8_t* from = p.laid + chunk * Q::bytes(p.units, p.groups);
     auto bring = [&](void* to, const uint8_t* what, uint32_t bytes) {
@@ -322,14 +322,16 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
         done_phase ^= 1u;
         raven_tc::tc_fence_after();
         const float sc = raven_int4::step_of(word[g]);
+        constexpr int P = 2;  // pieces of 16 columns at once
 #pragma unroll
-        for (int j = 0; j < NC / 32; ++j) {
-          uint32_t v[2][16];
-          tmem_ld16(mine + S::kAcc + 32 * j, v[0]);
-          tmem_ld16(mine + S::kAcc + 32 * j + 16, v[1]);
+        for (int j = 0; j < NC / (16 * P); ++j) {
+          uint32_t v[P][16];
+#pragma unroll
+          for (int k = 0; k < P; ++k) tmem_ld16(mine + S::kAcc + 16 * (P * j + k), v[k]);
           tmem_wait_ld(v);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) total[32 * j + i] = fmaf(sc, __uint_as_float(v[i / 16][i % 16]), total[32 * j + i]);
+          for (int i = 0; i < 16 * P; ++i)
+            total[16 * P * j + i] = fmaf(sc, __uint_as_float(v[i / 16][i % 16]), total[16 * P * j + i]);
         }
       }
     }
