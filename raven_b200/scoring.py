@@ -221,9 +221,10 @@ _GROUPS = {32: L.RAVEN_TYPE_INT4_32, 64: L.RAVEN_TYPE_INT4_64, 128: L.RAVEN_TYPE
 
 def _ids(name: str, t: torch.Tensor, device: int) -> int:
     """How many of a 1-D int32 tensor of ids or slots on a GPU."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous 1-D int32 tensor")
-    _on(device, t)
+    if t.get_device() != device:
+        _on(device, t)
     return t.numel()
 
 
@@ -358,7 +359,7 @@ class Int4Rows:
             raise ValueError(f"values must be float32, float16 or bfloat16, not {dtype}")
         pitch = self._dim
         if out is None:
-            out = torch.empty(m, self._dim, dtype=dtype, device=self.device)
+            out = self._codes.new_empty((m, self._dim), dtype=dtype)
         else:
             if out.shape != (m, self._dim):
                 raise ValueError(f"out must be a matrix of {m} x {self._dim}")
@@ -539,15 +540,18 @@ def _scores_matrix(x: torch.Tensor, name: str) -> int:
     (nq, n), (ld, step) = x.shape, x.stride()
     if (n > 1 and step != 1) or (nq > 1 and ld < n):
         raise ValueError(f"{name} must hold each row's values side by side and its rows one after another")
-    return max(ld, n)
+    return ld if ld > n else n
 
 
 def _per_query(name: str, x, nq: int, device: int):
     """(address, number) of a penalty: one number, or a float32 tensor of one for each query."""
+    if type(x) is float:
+        return None, x
     if isinstance(x, torch.Tensor):
-        if x.dtype != torch.float32 or x.shape != (nq,) or not x.is_contiguous():
+        if x.dtype is not torch.float32 or x.dim() != 1 or x.numel() != nq or not x.is_contiguous():
             raise ValueError(f"{name} must be a number or a contiguous float32 tensor of {nq}")
-        _on(device, x)
+        if x.get_device() != device:
+            _on(device, x)
         return x.data_ptr(), 0.0
     return None, float(x)
 
@@ -580,16 +584,17 @@ def adjust(scores: torch.Tensor, *, bias: Optional[torch.Tensor] = None, allow: 
     starts fall or leave `seen` count as empty: RAVEN_S_OFFSETS."""
     ld = _scores_matrix(scores, "scores")
     (nq, n), device = scores.shape, scores.get_device()
-    by = L.Adjustments()
+    bias_at, ld_bias = None, 0
     if bias is not None:
-        if not isinstance(bias, torch.Tensor) or bias.dtype != torch.float32 or bias.shape not in ((n,), (nq, n)) or \
+        if not isinstance(bias, torch.Tensor) or bias.dtype is not torch.float32 or bias.shape not in ((n,), (nq, n)) or \
                 (n > 1 and bias.stride(-1) != 1) or (bias.dim() == 2 and nq > 1 and n > 0 and bias.stride(0) < n):
             raise ValueError(f"bias must be a float32 tensor of {n} values, or {nq} x {n}, each row's side by side")
         _on(device, bias)
-        by.bias, by.ld_bias = bias.data_ptr(), 0 if bias.dim() == 1 or nq == 1 else bias.stride(0)
+        bias_at, ld_bias = bias.data_ptr(), 0 if bias.dim() == 1 or nq == 1 else bias.stride(0)
     words = -(-n // 32)
+    allow_at, count, ld_allow, rows_at = None, 0, 0, None
     if allow is not None:
-        if not isinstance(allow, torch.Tensor) or allow.dtype != torch.int32 or allow.dim() not in (1, 2) or \
+        if not isinstance(allow, torch.Tensor) or allow.dtype is not torch.int32 or allow.dim() not in (1, 2) or \
                 allow.shape[-1] < words or (words > 1 and allow.stride(-1) != 1) or \
                 (allow.dim() == 2 and allow.shape[0] > 1 and allow.stride(0) < words):
             raise ValueError(f"allow must be an int32 tensor with {words} words for each filter, side by side")
@@ -602,30 +607,34 @@ def adjust(scores: torch.Tensor, *, bias: Optional[torch.Tensor] = None, allow: 
                 raise ValueError(f"allow holds {count} filters: without allow_rows there must be one, or {nq}")
         elif _ids("allow_rows", allow_rows, device) != nq:
             raise ValueError(f"allow_rows must hold {nq} numbers of filters")
-        by.allow, by.allow_count = allow.data_ptr(), count
-        by.ld_allow, by.allow_rows = allow.stride(0) if count > 1 else words, _ptr(allow_rows)
+        else:
+            rows_at = allow_rows.data_ptr()
+        allow_at, ld_allow = allow.data_ptr(), allow.stride(0) if count > 1 else words
     elif allow_rows is not None:
         raise ValueError("allow_rows without allow")
     if (seen is None) != (seen_starts is None):
         raise ValueError("seen and seen_starts come together")
+    seen_at, total, starts_at = None, 0, None
     if seen is not None:
-        by.seen_total = _ids("seen", seen, device)
+        total = _ids("seen", seen, device)
         if _offsets("seen_starts", seen_starts, device) != nq:
             raise ValueError(f"seen_starts must hold {nq + 1} values")
-        by.seen, by.seen_starts = seen.data_ptr(), seen_starts.data_ptr()
-    by.repetition, by.repetition_all = _per_query("repetition", repetition, nq, device)
-    by.presence, by.presence_all = _per_query("presence", presence, nq, device)
-    by.frequency, by.frequency_all = _per_query("frequency", frequency, nq, device)
-    if by.repetition is None and not by.repetition_all > 0.0:
+        seen_at, starts_at = seen.data_ptr(), seen_starts.data_ptr()
+    rep_at, rep = _per_query("repetition", repetition, nq, device)
+    pre_at, pre = _per_query("presence", presence, nq, device)
+    freq_at, freq = _per_query("frequency", frequency, nq, device)
+    if rep_at is None and not rep > 0.0:
         raise ValueError("repetition must be above 0")
     if out is None:
-        out = torch.empty((nq, n), dtype=scores.dtype, device=scores.device)
+        out = torch.empty_like(scores) if scores.is_contiguous() else scores.new_empty((nq, n))
         ld_out = n
     else:
         ld_out = _scores_matrix(out, "out")
         if out.shape != (nq, n) or out.dtype != scores.dtype:
             raise ValueError(f"out must be a {scores.dtype} matrix of {nq} x {n}")
         _on(device, out)
+    by = L.Adjustments(bias_at, ld_bias, allow_at, count, ld_allow, rows_at, seen_at, total, starts_at, rep_at, pre_at, freq_at,
+                       rep, pre, freq)
     _call(device, L.load().raven_adjust_scores_device, scores.data_ptr(), _TYPES[scores.dtype], nq, n, ld, by, int(largest),
           out.data_ptr(), ld_out, _status(status, device))
     return out
