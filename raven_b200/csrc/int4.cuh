@@ -99,7 +99,8 @@ struct Write {
 };
 
 constexpr uint32_t kRun = 64;  // most rows of a run
-constexpr int kItems = 4;      // eights of a lane at once
+constexpr int kEights = 2;     // of a lane at once, written (four, with three CTAs an SM, 30000 x 768 f16 took 51 us, two 44)
+constexpr int kItems = 4;      // pieces of a lane at once, read
 
 // u / per for u * per < 2^32; magic: 2^32 / per rounded up, 0 for 1.
 __device__ inline uint32_t divided(uint32_t u, uint32_t magic) { return magic ? __umulhi(u, magic) : u; }
@@ -157,13 +158,13 @@ __device__ inline uint32_t codes_of(float (&x)[8], float step, int z) {
 }
 
 // A lane takes eight values (two 16-byte loads of f32, one of 16-bit types), the
-// L = group / 8 lanes of a group share its range by shuffles, and of four such
+// L = group / 8 lanes of a group share its range by shuffles, and of two such
 // pieces at once every group's word is worked out by a lane of its own (64-bit
 // arithmetic that 16 lanes did alike took as long as the reading).
 // VEC: pitch and address let 16 bytes be read at once. LANE: lane-major rows
 // (element e of the first 16C at (e % 16) * C + e / 16).
 template <typename T, uint32_t L, bool VEC, bool LANE>
-__global__ void __launch_bounds__(256, 3) write_kernel(const Write p) {
+__global__ void __launch_bounds__(256, 5) write_kernel(const Write p) {
   __shared__ int32_t dest[2][kRun];  // where the rows of a run, and of the next one, are held; -1: nowhere
   __shared__ uint32_t later[kRun];
   after_previous();
@@ -197,11 +198,11 @@ __global__ void __launch_bounds__(256, 3) write_kernel(const Write p) {
   const uint32_t wide = (p.dim + kBlock - 1) / kBlock * (kBlock / G);  // words of a row as it is held
   for (uint64_t r0 = (uint64_t)blockIdx.x * p.run; r0 < p.m; r0 += stride) {
     const uint32_t rows = (uint32_t)min((uint64_t)p.run, p.m - r0), items = rows * p.per;
-    float x[kItems][8];
-    uint32_t from[kItems], at[kItems];  // a piece's row of the run, which of its eights
+    float x[kEights][8];
+    uint32_t from[kEights], at[kEights];  // a piece's row of the run, which of its eights
     auto load = [&](uint32_t u0) {
 #pragma unroll
-      for (int n = 0; n < kItems; ++n) {
+      for (int n = 0; n < kEights; ++n) {
         const uint32_t u = u0 + n * 256 + threadIdx.x;
         from[n] = divided(u, p.magic);
         at[n] = u - from[n] * p.per;
@@ -243,12 +244,12 @@ __global__ void __launch_bounds__(256, 3) write_kernel(const Write p) {
         __syncthreads();
       }
     }
-    for (uint32_t u0 = 0; u0 < items; u0 += 256 * kItems) {
+    for (uint32_t u0 = 0; u0 < items; u0 += 256 * kEights) {
       if (u0) load(u0);
-      float lo[kItems], hi[kItems];
-      bool odd[kItems];
+      float lo[kEights], hi[kEights];
+      bool odd[kEights];
 #pragma unroll
-      for (int n = 0; n < kItems; ++n) {
+      for (int n = 0; n < kEights; ++n) {
         float not_finite = 0.f;  // NaN after an infinity or a NaN
         lo[n] = hi[n] = x[n][0];
 #pragma unroll
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(256, 3) write_kernel(const Write p) {
       // lane n * kGroups + g: group g of piece n
       float glo = 0.f, ghi = 0.f;
 #pragma unroll
-      for (int n = 0; n < kItems; ++n) {
+      for (int n = 0; n < kEights; ++n) {
         const float a = __shfl_sync(0xffffffffu, lo[n], lane % kGroups * L), b = __shfl_sync(0xffffffffu, hi[n], lane % kGroups * L);
         if (lane / kGroups == n) {
           glo = a;
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(256, 3) write_kernel(const Write p) {
       const uint32_t bits = step_bits(glo, ghi);
       const uint32_t scale = bits ? bits | ((uint32_t)(int)rintf(__fdiv_rn(glo, __uint_as_float(bits))) & 255u) : 0u;
 #pragma unroll
-      for (int n = 0; n < kItems; ++n) {
+      for (int n = 0; n < kEights; ++n) {
         uint32_t w = __shfl_sync(0xffffffffu, scale, n * kGroups + lane / L);
         const uint32_t i = at[n], d = 8 * i;
         int32_t to = -1;

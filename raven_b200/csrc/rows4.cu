@@ -46,18 +46,18 @@ int check_int4(const raven_rows* r, uint32_t dim, const char* what) {
   return RAVEN_OK;
 }
 
-// Rows of a CTA at once: kItems pieces a thread, as long as every SM gets rows. Sets what divides by `per`.
-uint32_t rows_at_once(uint64_t m, uint32_t per, int sms, uint32_t most, uint32_t* magic) {
+// Rows of a CTA at once: `items` pieces a thread, as long as every SM gets rows. Sets what divides by `per`.
+uint32_t rows_at_once(uint64_t m, uint32_t per, uint32_t items, int sms, uint32_t most, uint32_t* magic) {
   *magic = per > 1 ? (uint32_t)((0x100000000ull + per - 1) / per) : 0;
   const uint64_t fair = (m + 2ull * sms - 1) / (2ull * sms);
-  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({256 * raven_int4::kItems / per, most, fair}));
+  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({256 * items / per, most, fair}));
 }
 
 template <typename T, uint32_t L, bool LANE>
 cudaError_t launch_write(raven_int4::Write p, int sms, cudaStream_t st) {
   const bool vec = p.ld * sizeof(T) % 16 == 0 && aligned(p.x, 16);
   p.per = (p.dim + 8 * L - 1) / (8 * L) * L;
-  p.run = rows_at_once(p.m, p.per, sms, raven_int4::kRun, &p.magic);
+  p.run = rows_at_once(p.m, p.per, raven_int4::kEights, sms, raven_int4::kRun, &p.magic);
   const uint64_t grid = std::min<uint64_t>((p.m + p.run - 1) / p.run, (uint64_t)sms * 64);
   static Allowed none;
   if constexpr (!LANE)
@@ -118,7 +118,7 @@ cudaError_t launch_read(raven_int4::Read p, int sms, cudaStream_t st) {
   const bool vec = p.ld * sizeof(T) % 16 == 0 && aligned(p.out, 16);
   constexpr uint32_t V = 16 / sizeof(T);
   p.per = (p.dim + V - 1) / V;
-  p.run = rows_at_once(p.m, p.per, sms, 256 * raven_int4::kItems, &p.magic);
+  p.run = rows_at_once(p.m, p.per, raven_int4::kItems, sms, 256 * raven_int4::kItems, &p.magic);
   const uint64_t grid = std::min<uint64_t>((p.m + p.run - 1) / p.run, (uint64_t)sms * 64);
   static Allowed none;
   return launch(vec ? raven_int4::read_kernel<T, true> : raven_int4::read_kernel<T, false>, grid, 256, 0, none, st, p);
@@ -235,18 +235,18 @@ cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, 
   using namespace raven_score4;
   using L = Wide<NC>;
   using Q = WideLaid<NC>;
-  constexpr uint32_t kQueries = F32 ? NC / 2 : NC, W = kBlock / G;
+  constexpr uint32_t kQueries = F32 ? NC / 2 : NC;
   p.chunks = (uint32_t)((p.nq + kQueries - 1) / kQueries);
   p.tiles = (uint32_t)((p.n + kWideRows - 1) / kWideRows);
-  // Slices of a row, whole fours of blocks (the sums of four groups share a block): those that take least time, in
-  // blocks of a team (half a microsecond), with a block and a half a tile for its end and what the sums' join costs.
+  // Slices of a row: those that take least time, in blocks of a team (half a microsecond), with a block and a half a
+  // tile for its end and what the sums' join costs.
   auto bytes = [&](uint32_t slice, uint32_t depth) {
-    return L::bytes(std::min(4 * slice, p.units), std::min(slice * W, p.groups), depth);
+    return L::bytes(std::min(4 * slice, p.units), depth);
   };
   double best = 0;
   uint64_t columns = 1;
-  for (uint32_t n = 1; n <= std::max(1u, (p.blocks + 3) / 4); ++n) {
-    const uint32_t slice = n == 1 ? p.blocks : ((p.blocks + n - 1) / n + 3) / 4 * 4, slices = (p.blocks + slice - 1) / slice;
+  for (uint32_t n = 1; n <= p.blocks; ++n) {
+    const uint32_t slice = (p.blocks + n - 1) / n, slices = (p.blocks + slice - 1) / slice;
     if (slices != n || bytes(slice, 2) > kMostShared) continue;
     const uint64_t shares = (uint64_t)p.chunks * slices, c = std::max<uint64_t>(1, (uint64_t)sms / shares);
     const uint64_t rounds = (p.tiles + L::kTeams * c - 1) / (L::kTeams * c) * ((shares + sms - 1) / sms);
@@ -265,7 +265,7 @@ cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, 
   uint8_t* tmp = nullptr;
   cudaError_t e = cudaSuccess;
   const bool lay = std::min<uint64_t>(p.nq, kQueries) * p.dim > kOwnLayout;
-  const uint64_t laid = lay ? (p.chunks * Q::bytes(p.units, p.groups) + 255) / 256 * 256 : 0;
+  const uint64_t laid = lay ? (p.chunks * Q::bytes(p.units, 0) + 255) / 256 * 256 : 0;
   const uint64_t wide = (p.n + 3) / 4 * 4, sums = p.slices > 1 ? p.slices * p.nq * wide * 4 : 0;
   if (laid + sums && (e = cudaMallocAsync((void**)&tmp, laid + sums, st)) != cudaSuccess) return e;
   Join j{(const float*)(tmp + laid), wide, p.nq * wide, p.slices, p.nq, p.n, p.alpha, p.bias, p.out, p.ld};

@@ -90,12 +90,11 @@ struct Laid {
   __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t groups) {
     return frags(units) + sums(groups) + NT * 8 * 16;
   }
-  // Where a quarter of a unit of a column is; a group's sum (times 2^-24), where `to` are the sums (of a block's groups
-  // so many).
+  // Where a quarter of a unit of a column is; a group's sum (times 2^-24), where `to` are the sums.
   __device__ static uint32_t frag_at(uint32_t unit, uint32_t quarter, uint32_t col) {
     return (unit * NT + col / 8) * 512 + ((col & 7) * 4 + quarter) * 16;
   }
-  __device__ static void put_sum(uint8_t* to, uint32_t group, uint32_t, uint32_t col, float sum) {
+  __device__ static void put_sum(uint8_t* to, uint32_t group, uint32_t col, float sum) {
     ((float*)to)[group * (NT * 8) + col] = sum;
   }
   // What brings query q's sums back: a factor, two, a flag.
@@ -176,8 +175,8 @@ __device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, 
     for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const uint32_t c = col + (F32 ? 2 * q : q);
     if (i % L == 0 && i / L < groups) {
-      Q::put_sum(sums, i / L, kBlock / G, c, sum * 0x1p-24f);
-      if (F32) Q::put_sum(sums, i / L, kBlock / G, c + 1, 0.f);
+      Q::put_sum(sums, i / L, c, sum * 0x1p-24f);
+      if (F32) Q::put_sum(sums, i / L, c + 1, 0.f);
     }
     if (i < units * 4) {
       __align__(16) __half part[F32 ? 2 : 1][8];

@@ -5,19 +5,19 @@
 // themselves from 16 columns on.
 //
 // A group of four warps takes a tile of 128 rows, a row a thread. Codes come by TMA;
-// a thread turns its row's 128 codes of a block into f16 operands (five
-// instructions per eight codes, see score4.cuh) and writes them to tensor memory,
+// a thread turns its row's 128 codes of a block into f16 operands code + z (nine
+// instructions per eight codes: those of score4.cuh, and an f16 addition of z * 2^-24 or
+// z * 2^-20 to every two, which is exact) and writes them to tensor memory,
 // which the instruction reads its M side from: shared memory holds queries only,
 // and its bandwidth goes to them. A scale group is a chain of instructions of its
-// own, the last of which adds z * sum(q): three operands z * 2^-10 against the sum in
-// three f16 parts. The thread then reads its row's sums of the group and adds them,
+// own; the thread then reads its row's sums of the group and adds them,
 // times the group's step, to its own in registers. Three or four such groups of warps
 // per SM (teams) work on tiles of their own, so that one's instructions and waits are
 // hidden by the others'. A thread has all scores of its row, and a warp writes 32
 // scores of a query side by side, wherever the query's scores start.
 //
 // An instruction of 16 values takes about 64 cycles up to 96 columns, since that is
-// how long its M side takes to come from tensor memory: 576 for a block, of which
+// how long its M side takes to come from tensor memory: 512 for a block, of which
 // teams that wait for one another's make 1000.
 #pragma once
 
@@ -26,43 +26,24 @@
 namespace raven_score4 {
 
 // A chunk of queries: K blocks of 64 values (two units), for each column 128 bytes
-// in the 128-byte swizzle; then blocks of four groups' sums laid out the same way,
-// 16 operands a group: its sum's three parts at four times its number in its block of
-// values, zeros against the z of the others; then what brings sums back.
+// in the 128-byte swizzle; then what brings sums back.
 template <int NC>
 struct WideLaid {
   static constexpr uint32_t kColumns = NC;
   static constexpr uint32_t kBlockBytes = NC * 128;
   __host__ __device__ static uint64_t frags(uint32_t units) { return (uint64_t)((units + 1) / 2) * kBlockBytes; }
-  __host__ __device__ static uint64_t sums(uint32_t groups) { return (uint64_t)((groups + 3) / 4) * kBlockBytes; }
-  __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t groups) {
-    return frags(units) + sums(groups) + NC * 16;
-  }
+  __host__ __device__ static uint64_t sums(uint32_t) { return 0; }  // z is added to the codes
+  __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t) { return frags(units) + NC * 16; }
   __device__ static uint32_t frag_at(uint32_t unit, uint32_t quarter, uint32_t col) {
     return unit / 2 * kBlockBytes + col * 128 + ((((unit & 1) * 4 + quarter) ^ (col & 7)) * 16);
   }
+  __device__ static void put_sum(uint8_t*, uint32_t, uint32_t, float) {}
   // What brings query q's sums back: a factor, or two and a flag.
   __device__ static void put_back(float* back, uint32_t q, float f, float k0, float k1, float flag) {
     back[q] = f;
     back[NC + 2 * q] = k0;
     back[NC + 2 * q + 1] = k1;
     back[3 * NC + q] = flag;
-  }
-  // sum: times 2^-24; against z * 2^-10 it has to be 2^10 times that. Below 2^8, so three parts leave less than 2^-24.
-  __device__ static void put_sum(uint8_t* to, uint32_t group, uint32_t per, uint32_t col, float sum) {
-    const float x = sum * 0x1p10f;
-    const __half hi = __float2half_rn(x);
-    const float r = x - __half2float(hi);
-    const __half mid = __float2half_rn(r), lo = __float2half_rn(r - __half2float(mid));
-    const __half zero = __half(0.f);
-    const uint32_t place = group % per;  // in its block of values
-    const bool odd = place & 1;
-    __align__(16) __half part[8] = {odd ? zero : hi, odd ? zero : mid, odd ? zero : lo, zero,
-                                    odd ? hi : zero, odd ? mid : zero, odd ? lo : zero, zero};
-    uint8_t* at = to + group / 4 * kBlockBytes + col * 128;
-    const uint32_t in = (group & 3) * 2, half = place / 2;
-    *(uint4*)(at + (((in + half) ^ (col & 7)) * 16)) = *(const uint4*)part;
-    *(uint4*)(at + (((in + 1 - half) ^ (col & 7)) * 16)) = make_uint4(0, 0, 0, 0);
   }
 };
 
@@ -72,37 +53,42 @@ constexpr uint32_t kWideStage = kWideRows * 64;
 
 template <int NC>
 struct Wide {
-  // tensor memory of a team: operands of a block, a group's sums; in its last columns, the z of a block's groups
+  // tensor memory of a team: operands of a block, a group's sums
   static constexpr uint32_t kAcc = 64, kTeam = kAcc + NC;
-  static constexpr uint32_t kTeams = NC == 32 ? 4 : 3, kThreads = kTeams * 128, kZ = 512 - 8 * kTeams;
-  static_assert(kTeams * kTeam <= kZ, "tensor memory has 512 columns");
+  static constexpr uint32_t kTeams = NC == 32 ? 4 : 3, kThreads = kTeams * 128;
+  static_assert(kTeams * kTeam <= 512, "tensor memory has 512 columns");
   static constexpr uint32_t kHead = 1024;  // barriers, the place of the tensor memory; TMA's places start on 1024 bytes
   static constexpr uint32_t kTops = NC * 4;
-  __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t groups, uint32_t depth) {
-    return 1024 + kHead + (uint64_t)kTeams * depth * kWideStage + WideLaid<NC>::bytes(units, groups) + kTops;
+  __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t depth) {
+    return 1024 + kHead + (uint64_t)kTeams * depth * kWideStage + WideLaid<NC>::bytes(units, 0) + kTops;
   }
 };
 
-template <int N>
-__device__ inline void tmem_st(uint32_t at, const uint32_t* v);
-template <>
-__device__ inline void tmem_st<2>(uint32_t at, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};\n" ::"r"(at), "r"(v[0]), "r"(v[1]) : "memory");
+// What is added to a row's codes of a group: z * 2^-24 twice, z * 2^-20 twice. z + 128 at the bottom of the f16 1024
+// is 1152 + z; subnormal products are exact.
+struct Offsets {
+  __half2 low, high;
+  __device__ Offsets() {}
+  __device__ explicit Offsets(uint32_t word) {
+    const uint32_t b = __byte_perm(word, 0x64u, 0x4040) ^ 0x00800080u;
+    const __half2 z = __hsub2(*(const __half2*)&b, __float2half2_rn(1152.f));
+    low = __hmul2(z, __float2half2_rn(0x1p-24f));
+    high = __hmul2(z, __float2half2_rn(0x1p-20f));
+  }
+};
+// Eight codes as four operands of two.
+__device__ inline void operands(uint32_t w, const Offsets& z, uint32_t& a0, uint32_t& a1, uint32_t& a2, uint32_t& a3) {
+  auto plus = [](uint32_t code, __half2 z) {
+    const __half2 r = __hadd2(*(const __half2*)&code, z);
+    return *(const uint32_t*)&r;
+  };
+  a0 = plus(w & 0x000f000fu, z.low);
+  a1 = plus(w & 0x00f000f0u, z.high);
+  a2 = plus((w >> 8) & 0x000f000fu, z.low);
+  a3 = plus((w >> 8) & 0x00f000f0u, z.high);
 }
-template <>
-__device__ inline void tmem_st<4>(uint32_t at, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-               "r"(v[3])
-               : "memory");
-}
-template <>
-__device__ inline void tmem_st<8>(uint32_t at, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(at), "r"(v[0]),
-               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-template <>
-__device__ inline void tmem_st<16>(uint32_t at, const uint32_t* v) {
+
+__device__ inline void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
       "%16};\n" ::"r"(at),
@@ -156,7 +142,7 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
   const uint32_t slice = share % p.slices;
   const uint64_t chunk = share / p.slices;
   const uint32_t b0 = slice * p.slice, blocks = min(p.slice, p.blocks - b0);
-  const uint32_t units = min(4 * p.slice, p.units - 4 * b0), groups = min(p.slice * W, p.groups - b0 * W);
+  const uint32_t units = min(4 * p.slice, p.units - 4 * b0);
   if (row_of == 0) {
     for (uint32_t i = 0; i < kWideDepth + 1; ++i) mbar_init(bars + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -170,8 +156,8 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
   raven_tc::tc_fence_before();
   __syncthreads();
   raven_tc::tc_fence_after();
-  const uint32_t tmem = *slot_of_tmem + team * S::kTeam, tmem_z = *slot_of_tmem + S::kZ + 8 * team;
-  const uint32_t lanes = (warp & 3) << 21, mine = tmem + lanes;  // this warp's 32 lanes
+  const uint32_t tmem = *slot_of_tmem + team * S::kTeam;
+  const uint32_t mine = tmem + ((warp & 3) << 21);  // this warp's 32 lanes
   after_previous();
 
   // copies: by the team's first thread
@@ -192,29 +178,22 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
   if (row_of == 0)
     for (uint32_t i = 0; i < p.depth; ++i) copy_next();
 
-  uint8_t* sums = held + Q::frags(units);
-  float* back = (float*)(sums + Q::sums(groups));
+  float* back = (float*)(held + Q::frags(units));
   if (p.q) {
-    lay_out_any<Q, G, F32>(p, chunk * kQueries, kQueries, 0, 4 * b0, units, groups, held, (uint32_t*)(back + 4 * NC));
+    lay_out_any<Q, G, F32>(p, chunk * kQueries, kQueries, 0, 4 * b0, units, 0, held, (uint32_t*)(back + 4 * NC));
   } else {
-    const uint8_t* from = p.laid + chunk * Q::bytes(p.units, p.groups);
+    const uint8_t* from = p.laid + chunk * Q::bytes(p.units, 0);
     auto bring = [&](void* to, const uint8_t* what, uint32_t bytes) {
       for (uint32_t i = tid * 16; i < bytes; i += S::kThreads * 16) *(uint4*)((uint8_t*)to + i) = *(const uint4*)(what + i);
     };
     bring(held, from + Q::frags(4 * b0), (uint32_t)Q::frags(units));
-    from += Q::frags(p.units);
-    bring(sums, from + Q::sums(b0 * W), (uint32_t)Q::sums(groups));
-    bring(back, from + Q::sums(p.groups), NC * 16);
-  }
-  {  // of the operands beside the z that are written, those of groups that are not there stay 0
-    const uint32_t zero[8] = {};
-    tmem_st<8>(tmem_z + lanes, zero);
+    bring(back, from + Q::frags(p.units), NC * 16);
   }
   asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // the queries, to the instructions
   __syncthreads();
   bool plain = true;  // every column has one factor
   for (uint32_t q = 0; q < kQueries; ++q) plain &= back[3 * NC + q] == 0.f;
-  const uint64_t b_desc = raven_tc::sw128_desc(smem_u32(held)), z_desc = raven_tc::sw128_desc(smem_u32(sums));
+  const uint64_t b_desc = raven_tc::sw128_desc(smem_u32(held));
   constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(NC >> 3) << 17) | (8u << 24);  // f32 sums, f16 operands
 
   bool ok = true;
@@ -255,15 +234,11 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
         // word u * quarter + unit of a block of u units
         auto put_unit = [&](uint32_t unit, uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3) {
           const uint32_t w[4] = {c0, c1, c2, c3};
+          const Offsets z(word[unit / U]);
           uint32_t a[16];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            a[4 * i] = w[i] & 0x000f000fu;
-            a[4 * i + 1] = w[i] & 0x00f000f0u;
-            a[4 * i + 2] = (w[i] >> 8) & 0x000f000fu;
-            a[4 * i + 3] = (w[i] >> 8) & 0x00f000f0u;
-          }
-          tmem_st<16>(mine + 16 * unit, a);
+          for (int i = 0; i < 4; ++i) operands(w[i], z, a[4 * i], a[4 * i + 1], a[4 * i + 2], a[4 * i + 3]);
+          tmem_st16(mine + 16 * unit, a);
         };
         if (u == 4) {
           put_unit(0, c[0], c[4], c[8], c[12]);
@@ -280,14 +255,6 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
         } else {
           put_unit(0, c[0], c[1], c[2], c[3]);
         }
-        uint32_t zs[2 * W];
-#pragma unroll
-        for (uint32_t g = 0; g < W; ++g) {
-          const __half2 z = __float2half2_rn(raven_int4::zero_of(word[g]) * 0x1p-10f);
-          zs[2 * g] = *(const uint32_t*)&z;
-          zs[2 * g + 1] = zs[2 * g] & 0xffffu;
-        }
-        tmem_st<2 * W>(tmem_z + lanes, zs);
         asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
       }
       const uint32_t taken = now;
@@ -314,8 +281,6 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
             mma_ts(tmem + S::kAcc, tmem + 16 * unit + 8, at + 2, idesc, 1);
             add = 1;
           }
-          const uint32_t group = b * W + g;
-          mma_ts(tmem + S::kAcc, tmem_z, z_desc + (group / 4 * Q::kBlockBytes >> 4) + (group & 3) * 2, idesc, 1);
           raven_tc::mma_commit(done);
         }
         if (ok && !warp_waits(done, done_phase)) ok = false;

@@ -64,14 +64,15 @@ def values(codes, words, dim, group):
 
 
 def score_bound(q, codes, words, dim, group, alpha, bias, out_eps, exact, f32_queries):
-    """How far a score may be off. Against a group, sum c q and z * sum q are
-    summed in f32 from products that are exact: at most 2 * group additions (two
-    parts of each f32 value), each off by 2^-23 of the magnitudes so far
-    (truncation counted), and the groups of a row by as many additions more as
-    there are groups, with three roundings each. f32 queries keep 22 bits (off by
-    2^-23), and every query loses what is below 2^-34 of its largest value. alpha
-    and bias add an f32 rounding each, the type of the scores half a step; 1e-37
-    covers scores near f32's underflow."""
+    """How far a score may be off. Against a group either sum c q and z * sum q or
+    sum (c + z) q are summed in f32 from products that are exact: at most 2 * group
+    additions (two parts of each f32 value), each off by 2^-23 of the magnitudes so
+    far (truncation counted; those of the first form are no less than the
+    other's), and the groups of a row by as many additions more as there are
+    groups, with three roundings each. f32 queries keep 22 bits (off by 2^-23), and
+    every query loses what is below 2^-34 of its largest value. alpha and bias add
+    an f32 rounding each, the type of the scores half a step; 1e-37 covers scores
+    near f32's underflow."""
     w = np.asarray(words).astype(np.int64) & 0xFFFFFFFF
     z = ((w & 255) ^ 128) - 128
     step = (w & 0xFFFFFF00).astype(np.uint32).view(np.float32).astype(np.float64)
