@@ -1,22 +1,23 @@
 // Scores of queries against 4-bit rows (int4.cuh has their layout):
 //
-//   S[i, j] = alpha * sum_g step_jg (z_jg sum_k q_ik + sum_k code_jk q_ik) + bias[j]
+//   S[i, j] = alpha * sum_g step_jg ((z_jg + 8) sum_k q_ik + sum_k (code_jk - 8) q_ik) + bias[j]
 //
-// The inner sums run on the tensor cores (mma m16n8k16, f16 operands, f32 sums)
-// with rows as the M side and queries as the N side. A code is not converted: 4
-// bits at the bottom of a 16-bit lane are the f16 subnormal code * 2^-24, at bits
-// 4-7 code * 2^-20, so one AND makes two operands (five instructions per eight
-// codes). What a fragment's lane holds of K is free as long as both sides agree:
-// lane t of a row's four takes the eight values 8t.. of each unit of 32 (one
-// word), as pairs (0, 4), (1, 5), (2, 6), (3, 7).
+// The inner sums run on the tensor cores (here mma m16n8k16, f16 operands, f32 sums)
+// with rows as the M side and queries as the N side. 4 bits at the bottom of the f16
+// 1024 are 1024 + code, at bits 4-7 1024 + 16 code: one LOP3 and one f16 addition (or
+// multiply-add) make code - 8 of two codes, nine instructions per eight. Without the
+// additions the 4 bits alone are an f16 too, a subnormal, but the tensor cores line
+// products up by their exponent fields and drop what is below the sum's bits, and
+// subnormals lose as many of them as they have leading zeros: scores were off by 1e-6
+// to 2.3e-6 of their size. What a fragment's lane holds of K is free as long as both
+// sides agree: lane t of a row's four takes the eight values 8t.. of each unit of 32
+// (one word), as pairs (0, 4), (1, 5), (2, 6), (3, 7).
 //
 // Queries are brought to a largest magnitude in [2^14, 2^15) by a power of two
 // each, so that f16 holds what f32, f16 and bf16 values may be: 11 bits of a value
-// in one part, 22 in two (f32), nothing below 2^-35 of the largest (values paired
-// with codes at bits 4-7 are kept as sixteenths). The sum of a group starts at
-// z * sum(q), and its step is applied in f32 when the group ends: the scale is
-// never rounded into an operand.
-//
+// in one part, 22 in two (f32), nothing below 2^-39 of the largest. The sum of a
+// group starts at (z + 8) * sum(q), and its step is applied in f32 when the group
+// ends: the scale is never rounded into an operand.
 // Two parts of an f32 query are two columns of the N side, added up at the end.
 //
 // What bounds it: reading the codes. Each warp has its own ring of tiles of 32 or 64
@@ -51,6 +52,7 @@ using raven_tc::mbar_init;
 using raven_tc::smem_u32;
 using raven_tc::tma_load_2d;
 
+constexpr int kStepShift = 16;     // steps are taken times 2^-16: sums are up to 2^29 times a query's largest value
 constexpr uint32_t kMaxDepth = 6;  // tiles under way per warp, at most
 
 struct Params {
@@ -90,7 +92,7 @@ struct Laid {
   __host__ __device__ static uint64_t bytes(uint32_t units, uint32_t groups) {
     return frags(units) + sums(groups) + NT * 8 * 16;
   }
-  // Where a quarter of a unit of a column is; a group's sum (times 2^-24), where `to` are the sums.
+  // Where a quarter of a unit of a column is; a group's sum, where `to` are the sums.
   __device__ static uint32_t frag_at(uint32_t unit, uint32_t quarter, uint32_t col) {
     return (unit * NT + col / 8) * 512 + ((col & 7) * 4 + quarter) * 16;
   }
@@ -175,14 +177,14 @@ __device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, 
     for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const uint32_t c = col + (F32 ? 2 * q : q);
     if (i % L == 0 && i / L < groups) {
-      Q::put_sum(sums, i / L, c, sum * 0x1p-24f);
+      Q::put_sum(sums, i / L, c, sum);
       if (F32) Q::put_sum(sums, i / L, c + 1, 0.f);
     }
     if (i < units * 4) {
       __align__(16) __half part[F32 ? 2 : 1][8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float w = k & 1 ? v[k] * 0.0625f : v[k];
+        const float w = v[k];
         const int s = (k & 3) * 2 + (k >> 2);
         part[0][s] = __float2half_rn(w);
         if constexpr (F32) part[1][s] = __float2half_rn(w - __half2float(part[0][s]));
@@ -192,7 +194,7 @@ __device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, 
         *(uint4*)(to + Q::frag_at(i >> 2, i & 3, c + h)) = *(const uint4*)part[h];
     }
     if (i == 0) {
-      const int b = 24 - e;  // -139 .. 137
+      const int b = kStepShift - e;  // -147 .. 129
       // exact where alpha's exponent leaves it among the normal numbers
       const int a = p.alpha == 0.f ? 0 : ilogbf(p.alpha) + b;
       const bool plain = a >= -120 && a <= 120 && (p.alpha == 0.f || fabsf(p.alpha) < INFINITY) && b >= -126 && b <= 127;
@@ -250,6 +252,23 @@ __device__ inline bool wait(uint32_t bar, uint32_t parity) {
 }
 __device__ inline void meet(uint32_t id, uint32_t threads) {
   asm volatile("bar.sync %0, %1;\n" ::"r"(id), "r"(threads) : "memory");
+}
+
+// Eight codes less 8 as four operands of two.
+__device__ inline void operands(uint32_t w, uint32_t& a0, uint32_t& a1, uint32_t& a2, uint32_t& a3) {
+  auto low = [](uint32_t code) {
+    const __half2 r = __hadd2(*(const __half2*)&code, __float2half2_rn(-1032.f));
+    return *(const uint32_t*)&r;
+  };
+  auto high = [](uint32_t code) {
+    const __half2 r = __hfma2(*(const __half2*)&code, __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
+    return *(const uint32_t*)&r;
+  };
+  const uint32_t v = w >> 8;
+  a0 = low((w & 0x000f000fu) | 0x64006400u);
+  a1 = high((w & 0x00f000f0u) | 0x64006400u);
+  a2 = low((v & 0x000f000fu) | 0x64006400u);
+  a3 = high((v & 0x00f000f0u) | 0x64006400u);
 }
 
 __device__ inline void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -425,8 +444,8 @@ __global__ void __launch_bounds__(Layout<NT, MT, G>::kThreads, 1) score4_kernel(
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const uint32_t w = word[(4 * (m0 + m) + 2 * h) * S::kWords + gi];
-              sc[m][h] = raven_int4::step_of(w);
-              z[h] = raven_int4::zero_of(w);
+              sc[m][h] = raven_int4::step_of(w) * (1.f / (1 << kStepShift));
+              z[h] = raven_int4::zero_of(w) + 8.f;
             }
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -449,10 +468,7 @@ __global__ void __launch_bounds__(Layout<NT, MT, G>::kThreads, 1) score4_kernel(
               for (int h = 0; h < 2; ++h) {
                 const uint4 c = code[m][h];
                 const uint32_t w = unit == 0 ? c.x : unit == 1 ? c.y : unit == 2 ? c.z : c.w;
-                a[h][0] = w & 0x000f000fu;
-                a[h][1] = w & 0x00f000f0u;
-                a[h][2] = (w >> 8) & 0x000f000fu;
-                a[h][3] = (w >> 8) & 0x00f000f0u;
+                operands(w, a[h][0], a[h][1], a[h][2], a[h][3]);
               }
 #pragma unroll
               for (int j = 0; j < NT; ++j) mma(acc[m][j], a[0][0], a[1][0], a[0][1], a[1][1], x[unit][j].x, x[unit][j].y);

@@ -5,9 +5,8 @@
 // themselves from 16 columns on.
 //
 // A group of four warps takes a tile of 128 rows, a row a thread. Codes come by TMA;
-// a thread turns its row's 128 codes of a block into f16 operands code + z (nine
-// instructions per eight codes: those of score4.cuh, and an f16 addition of z * 2^-24 or
-// z * 2^-20 to every two, which is exact) and writes them to tensor memory,
+// a thread turns its row's 128 codes of a block into f16 operands code + z (as many
+// instructions as code - 8 in score4.cuh; z is its own row's) and writes them to tensor memory,
 // which the instruction reads its M side from: shared memory holds queries only,
 // and its bandwidth goes to them. A scale group is a chain of instructions of its
 // own; the thread then reads its row's sums of the group and adds them,
@@ -64,28 +63,32 @@ struct Wide {
   }
 };
 
-// What is added to a row's codes of a group: z * 2^-24 twice, z * 2^-20 twice. z + 128 at the bottom of the f16 1024
-// is 1152 + z; subnormal products are exact.
+// What is added to a row's codes of a group: z - 1024 to 1024 + code, z - 64 to a sixteenth of 1024 + 16 code. All
+// are whole numbers below 2048, which f16 holds. z + 128 at the bottom of the f16 1024 is 1152 + z.
 struct Offsets {
   __half2 low, high;
-  __device__ Offsets() {}
   __device__ explicit Offsets(uint32_t word) {
     const uint32_t b = __byte_perm(word, 0x64u, 0x4040) ^ 0x00800080u;
     const __half2 z = __hsub2(*(const __half2*)&b, __float2half2_rn(1152.f));
-    low = __hmul2(z, __float2half2_rn(0x1p-24f));
-    high = __hmul2(z, __float2half2_rn(0x1p-20f));
+    low = __hadd2(z, __float2half2_rn(-1024.f));
+    high = __hadd2(z, __float2half2_rn(-64.f));
   }
 };
-// Eight codes as four operands of two.
+// Eight codes, with z, as four operands of two.
 __device__ inline void operands(uint32_t w, const Offsets& z, uint32_t& a0, uint32_t& a1, uint32_t& a2, uint32_t& a3) {
-  auto plus = [](uint32_t code, __half2 z) {
-    const __half2 r = __hadd2(*(const __half2*)&code, z);
+  auto low = [&](uint32_t code) {
+    const __half2 r = __hadd2(*(const __half2*)&code, z.low);
     return *(const uint32_t*)&r;
   };
-  a0 = plus(w & 0x000f000fu, z.low);
-  a1 = plus(w & 0x00f000f0u, z.high);
-  a2 = plus((w >> 8) & 0x000f000fu, z.low);
-  a3 = plus((w >> 8) & 0x00f000f0u, z.high);
+  auto high = [&](uint32_t code) {
+    const __half2 r = __hfma2(*(const __half2*)&code, __float2half2_rn(0.0625f), z.high);
+    return *(const uint32_t*)&r;
+  };
+  const uint32_t v = w >> 8;
+  a0 = low((w & 0x000f000fu) | 0x64006400u);
+  a1 = high((w & 0x00f000f0u) | 0x64006400u);
+  a2 = low((v & 0x000f000fu) | 0x64006400u);
+  a3 = high((v & 0x00f000f0u) | 0x64006400u);
 }
 
 __device__ inline void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
@@ -286,7 +289,7 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
         if (ok && !warp_waits(done, done_phase)) ok = false;
         done_phase ^= 1u;
         raven_tc::tc_fence_after();
-        const float sc = raven_int4::step_of(word[g]);
+        const float sc = raven_int4::step_of(word[g]) * (1.f / (1 << kStepShift));
         constexpr int P = 2;  // pieces of 16 columns at once
 #pragma unroll
         for (int j = 0; j < NC / (16 * P); ++j) {

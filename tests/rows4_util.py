@@ -64,20 +64,20 @@ def values(codes, words, dim, group):
 
 
 def score_bound(q, codes, words, dim, group, alpha, bias, out_eps, exact, f32_queries):
-    """How far a score may be off. Against a group either sum c q and z * sum q or
-    sum (c + z) q are summed in f32 from products that are exact: at most 2 * group
+    """How far a score may be off. Against a group either sum (c - 8) q and
+    (z + 8) * sum q or sum (c + z) q are summed in f32 from products that are exact
+    (|c + z| <= |c - 8| + |z + 8|, so the first form bounds both): at most 2 * group
     additions (two parts of each f32 value), each off by 2^-23 of the magnitudes so
-    far (truncation counted; those of the first form are no less than the
-    other's), and the groups of a row by as many additions more as there are
-    groups, with three roundings each. f32 queries keep 22 bits (off by 2^-23), and
-    every query loses what is below 2^-34 of its largest value. alpha and bias add
-    an f32 rounding each, the type of the scores half a step; 1e-37 covers scores
-    near f32's underflow."""
+    far (truncation counted), and the groups of a row by as many additions more as
+    there are groups, with three roundings each. f32 queries keep 22 bits (off by
+    2^-23), and every query loses what is below 2^-34 of its largest value. alpha
+    and bias add an f32 rounding each, the type of the scores half a step; 1e-37
+    covers scores near f32's underflow."""
     w = np.asarray(words).astype(np.int64) & 0xFFFFFFFF
     z = ((w & 255) ^ 128) - 128
     step = (w & 0xFFFFFF00).astype(np.uint32).view(np.float32).astype(np.float64)
     g = np.arange(dim) // group
-    mag = (unpack(codes, dim) + np.abs(z[:, g])) * np.abs(step[:, g])  # of a product's parts, before they cancel
+    mag = (np.abs(unpack(codes, dim) - 8) + np.abs(z[:, g] + 8)) * np.abs(step[:, g])  # of a product's parts, before they cancel
     mags = np.abs(q) @ mag.T
     adds = 2 * min(group, dim) + 3 * (-(-dim // group)) + 4
     off = adds * 2.0 ** -23 * mags + (2.0 ** -23 * mags if f32_queries else 0.0)
