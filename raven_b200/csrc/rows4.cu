@@ -238,8 +238,9 @@ cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, 
   constexpr uint32_t kQueries = F32 ? NC / 2 : NC;
   p.chunks = (uint32_t)((p.nq + kQueries - 1) / kQueries);
   p.tiles = (uint32_t)((p.n + kWideRows - 1) / kWideRows);
-  // Slices of a row: those that take least time, in blocks of a team (half a microsecond), with a block and a half a
-  // tile for its end and what the sums' join costs.
+  // Slices of a row: those that take least time, in microseconds. A block of a team takes 0.6 and 0.55 for each scale
+  // group's chain, a tile's end 0.7, a block of queries NC / 128, the join 3 and its bytes (40 x 5000 x 1000, groups of
+  // 32: 30 us in one slice, 13.6 in those that this gives).
   auto bytes = [&](uint32_t slice, uint32_t depth) {
     return L::bytes(std::min(4 * slice, p.units), depth);
   };
@@ -250,7 +251,8 @@ cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, 
     if (slices != n || bytes(slice, 2) > kMostShared) continue;
     const uint64_t shares = (uint64_t)p.chunks * slices, c = std::max<uint64_t>(1, (uint64_t)sms / shares);
     const uint64_t rounds = (p.tiles + L::kTeams * c - 1) / (L::kTeams * c) * ((shares + sms - 1) / sms);
-    const double time = rounds * (slice + 1.5) + (slices > 1 ? 6 + 4e-6 * p.nq * p.n * slices : 0);
+    const double block = 0.6 + 0.55 * (kBlock / G);
+    const double time = rounds * (slice * block + 0.7) + slice * NC / 128.0 + (slices > 1 ? 3 + 1.6e-6 * p.nq * p.n * slices : 0);
     if (best == 0 || time < best) {
       best = time;
       columns = c;
