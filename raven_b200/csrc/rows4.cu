@@ -149,6 +149,25 @@ cudaError_t launch_score4(const CUtensorMap& map, const raven_score4::Params& p,
   return launch(score4_kernel<NT, MT, G, F32, O>, ctas, Layout<NT, MT, G>::kThreads, (uint32_t)smem, allowed, st, map, p);
 }
 
+// Sums of slices take scratch, slices times what the scores take: above this the rows are taken in two halves.
+constexpr uint64_t kMostSums = 1ull << 30;
+
+template <typename F>
+cudaError_t in_halves(const raven_rows* v, const raven_score4::Params& p, int out_type, F&& run) {
+  const uint64_t half = (p.n / 2 + 127) / 128 * 128;
+  raven_rows a = *v, b = *v;
+  raven_score4::Params pa = p, pb = p;
+  a.rows = pa.n = half;
+  b.rows = pb.n = p.n - half;
+  b.data = (const uint8_t*)v->data + half * v->ld;
+  b.exps = (const uint8_t*)((const uint32_t*)v->exps + half * v->ld_exps);
+  pb.words = (const uint32_t*)b.exps;
+  pb.out = (uint8_t*)p.out + half * (out_type == 0 ? 4 : 2);
+  if (p.bias) pb.bias = p.bias + half;
+  const cudaError_t e = run(&a, pa);
+  return e == cudaSuccess ? run(&b, pb) : e;
+}
+
 cudaError_t launch_join(const raven_score4::Join& j, int out_type, int sms, cudaStream_t st) {
   using namespace raven_score4;
   static Allowed none;
@@ -163,6 +182,7 @@ cudaError_t run_score4(const raven_rows* v, raven_score4::Params p, int out_type
   using L = Layout<NT, MT, G>;
   using Q = Laid<NT>;
   constexpr uint32_t kQueries = F32 ? NT * 4 : NT * 8;
+  const Params whole = p;
   p.chunks = (uint32_t)((p.nq + kQueries - 1) / kQueries);
   // slices of a row: as few as let a CTA hold its queries beside its rings
   p.slices = 1;
@@ -196,6 +216,10 @@ cudaError_t run_score4(const raven_rows* v, raven_score4::Params p, int out_type
   const bool lay = std::min<uint64_t>(p.nq, kQueries) * p.dim > kOwnLayout;
   const uint64_t laid = lay ? (p.chunks * Q::bytes(p.units, p.groups) + 255) / 256 * 256 : 0;
   const uint64_t wide = (p.n + 3) / 4 * 4, sums = p.slices > 1 ? p.slices * p.nq * wide * 4 : 0;
+  if (sums > kMostSums && p.n >= 512)
+    return in_halves(v, whole, out_type, [&](const raven_rows* r, const Params& q) {
+      return run_score4<NT, MT, G, F32>(r, q, out_type, sms, st);
+    });
   if (laid + sums && (e = cudaMallocAsync((void**)&tmp, laid + sums, st)) != cudaSuccess) return e;
   Join j{(const float*)(tmp + laid), wide, p.nq * wide, p.slices, p.nq, p.n, p.alpha, p.bias, p.out, p.ld};
   if (p.slices > 1) {
@@ -236,6 +260,7 @@ cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, 
   using L = Wide<NC>;
   using Q = WideLaid<NC>;
   constexpr uint32_t kQueries = F32 ? NC / 2 : NC;
+  const Params whole = p;
   p.chunks = (uint32_t)((p.nq + kQueries - 1) / kQueries);
   p.tiles = (uint32_t)((p.n + kWideRows - 1) / kWideRows);
   // Slices of a row: those that take least time, in microseconds. A block of a team takes 0.6 and 0.55 for each scale
@@ -269,6 +294,9 @@ cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, 
   const bool lay = std::min<uint64_t>(p.nq, kQueries) * p.dim > kOwnLayout;
   const uint64_t laid = lay ? (p.chunks * Q::bytes(p.units, 0) + 255) / 256 * 256 : 0;
   const uint64_t wide = (p.n + 3) / 4 * 4, sums = p.slices > 1 ? p.slices * p.nq * wide * 4 : 0;
+  if (sums > kMostSums && p.n >= 512)
+    return in_halves(v, whole, out_type,
+                     [&](const raven_rows* r, const Params& q) { return run_wide<NC, G, F32>(r, q, out_type, sms, st); });
   if (laid + sums && (e = cudaMallocAsync((void**)&tmp, laid + sums, st)) != cudaSuccess) return e;
   Join j{(const float*)(tmp + laid), wide, p.nq * wide, p.slices, p.nq, p.n, p.alpha, p.bias, p.out, p.ld};
   if (p.slices > 1) {
@@ -327,7 +355,7 @@ cudaError_t dispatch_score4(const raven_rows* v, const raven_score4::Params& p, 
 template <typename T>
 cudaError_t launch_adjust(const raven_adjust::Params& p, bool largest, cudaStream_t st) {
   static Allowed none;
-  const uint32_t smem = raven_adjust::shared_bytes(p.tile, p.seen != nullptr);
+  const uint32_t smem = raven_adjust::shared_bytes(p.tile, p.starts != nullptr);
   return launch(largest ? raven_adjust::adjust_kernel<T, true> : raven_adjust::adjust_kernel<T, false>, p.nq * p.tiles,
                 raven_adjust::kThreads, smem, none, st, p);
 }

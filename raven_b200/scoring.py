@@ -303,18 +303,20 @@ class Int4Rows:
                         torch.empty(n, -(-dim // BLOCK) * (BLOCK // group), dtype=torch.int32, device=device), dim, group)
 
     @staticmethod
-    def encode(x: torch.Tensor, group: int = 64, out: Optional["Int4Rows"] = None) -> "Int4Rows":
+    def encode(x: torch.Tensor, group: Optional[int] = None, out: Optional["Int4Rows"] = None) -> "Int4Rows":
         """The rows of a float32, float16 or bfloat16 matrix. A group's step is
         the least, of 16 significant bits, whose 15 multiples cover the group's
         range (and 127 its largest magnitude); values are rounded to the nearest
         multiple, halves to even. A group with an infinity or a NaN is NaN as a
-        whole. `out`: rows to write instead of new ones (len(x) of them)."""
+        whole. `group`: 64, or what `out` has. `out`: rows to write instead of new
+        ones (len(x) of them)."""
         pitch = _matrix(x, "x")
         n, dim = x.shape
         if out is None:
-            out = Int4Rows.empty(n, dim, x.device, group)
-        elif len(out) != n or out.dim != dim:
-            raise ValueError(f"out holds {len(out)} rows of {out.dim}, expected {n} of {dim}")
+            out = Int4Rows.empty(n, dim, x.device, 64 if group is None else group)
+        elif len(out) != n or out.dim != dim or group not in (None, out.group):
+            raise ValueError(f"out holds {len(out)} rows of {out.dim} in groups of {out.group}, expected {n} of {dim}"
+                             + ("" if group is None else f" in groups of {group}"))
         out._write(x, pitch, None, None)
         return out
 

@@ -413,6 +413,46 @@ def test_scores_exactly(S):
             assert torch.equal(S.scores(q, rows), want)
 
 
+@pytest.mark.parametrize("dim", [8200, 20_000, 65_535, 65_536])
+@pytest.mark.parametrize("group", GROUPS)
+def test_scores_of_long_rows_exactly(S, dim, group):
+    """Rows too long to hold all queries for: slices, whose sums a second kernel adds up. Small whole numbers."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    x = torch.randint(-7, 8, (300, dim), generator=g, device="cuda").float()
+    x[:, ::32], x[:, 1::32] = -7, 8
+    rows = S.Int4Rows.encode(x, group)
+    assert torch.equal(rows.decode(), x)
+    bias = torch.arange(300, device="cuda").float()
+    for nq in (1, 7, 12, 20, 40, 70):
+        for t, out in (("f32", "f32"), ("f16", "f32"), ("bf16", "bf16")):
+            q = torch.randint(-2, 3, (nq, dim), generator=g, device="cuda").to(_dt(t))
+            want = (q.double() @ x.double().T).float()
+            assert torch.equal(S.scores(q, rows, dtype=_dt(out)), want.to(_dt(out)))
+        assert torch.equal(S.scores(q, rows, alpha=-2.0, bias=bias), -2.0 * want + bias)
+
+
+def test_scores_of_slices_in_pieces(S):
+    """Sums of slices that would take more than 1 GB of scratch: the rows are taken in halves."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n, dim = 30_011, 16_384
+    x = torch.randint(-7, 8, (n, 32), generator=g, device="cuda").float()
+    x[:, 0], x[:, 1] = -7, 8
+    short = S.Int4Rows.encode(x, 32)
+    codes = short.codes.repeat(1, 1).new_empty((n, dim // 2))
+    # the same 32 values 512 times: a block holds its four units' words side by side by quarter
+    w = short.codes.view(torch.int32)  # [n, 4]: a word for each quarter
+    codes.view(torch.int32).copy_(w.repeat_interleave(4, 1).repeat(1, dim // 128))
+    rows = S.Int4Rows(codes, short.scales[:, :1].repeat(1, dim // 32).contiguous(), dim, 32)
+    assert torch.equal(rows.decode(torch.tensor([0, n - 1], dtype=torch.int32, device="cuda")), x[[0, n - 1]].repeat(1, dim // 32))
+    q = torch.randint(-2, 3, (1500, dim), generator=g, device="cuda").half()
+    bias = torch.arange(n, device="cuda") % 100 + 0.0
+    got = S.scores(q, rows, bias=bias)
+    want = q.float().view(1500, dim // 32, 32).sum(1) @ x.T + bias
+    assert torch.equal(got, want)
+
+
 def test_scores_past_2_31(S):
     torch = _torch()
     nq, n = 70_000, 33_000
@@ -563,8 +603,11 @@ def test_adjust_bad_histories_and_filters(S):
     got = S.adjust(x, allow=allow, allow_rows=i32(0, 2, -7, 2 ** 31 - 1, 1), status=status)
     assert int(status) == 8 and S.take_status() == 0
     assert torch.equal(got[[0, 2, 4]], x[[0, 2, 4]]) and bool((got[[1, 3]] == -float("inf")).all())
-    # no history at all
+    # no history at all; starts that leave it
     assert torch.equal(S.adjust(x, seen=i32()[:0], seen_starts=i64(0, 0, 0, 0, 0, 0), presence=1.0), x)
+    assert S.take_status() == 0
+    assert torch.equal(S.adjust(x, seen=i32()[:0], seen_starts=i64(0, 0, 1, 1, 1, 1), presence=1.0), x)
+    assert S.take_status() == 1
 
 
 def test_adjust_past_2_31(S):
@@ -778,6 +821,7 @@ def test_refusals(S):
         lambda: S.Int4Rows.encode(x.double()),
         lambda: S.Int4Rows.encode(x.cpu()),
         lambda: S.Int4Rows.encode(x, out=rows),
+        lambda: S.Int4Rows.encode(x, 32, out=rows.rows(0, 4)),
         lambda: S.Int4Rows.encode(torch.randn(4, 0, device="cuda")),
         lambda: S.Int4Rows.empty(-1, 64, "cuda"),
         lambda: S.Int4Rows(u8(4, 16), w(4, 2), 64, 64),
