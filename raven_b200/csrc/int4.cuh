@@ -160,7 +160,9 @@ __device__ inline uint32_t codes_of(float (&x)[8], float step, int z) {
 // A lane takes eight values (two 16-byte loads of f32, one of 16-bit types), the
 // L = group / 8 lanes of a group share its range by shuffles, and of two such
 // pieces at once every group's word is worked out by a lane of its own (64-bit
-// arithmetic that 16 lanes did alike took as long as the reading).
+// arithmetic that 16 lanes did alike took as long as the reading). What bounds it:
+// issue slots and memory about even (1000000 x 128 f32 into slots in random order 200 us,
+// 680 MB at 3.4 TB/s: words and codes fill sectors in part, which are read first).
 // VEC: pitch and address let 16 bytes be read at once. LANE: lane-major rows
 // (element e of the first 16C at (e % 16) * C + e / 16).
 template <typename T, uint32_t L, bool VEC, bool LANE>
@@ -188,7 +190,7 @@ __global__ void __launch_bounds__(256, 5) write_kernel(const Write p) {
       }
     }
     to[threadIdx.x] = s < 0 ? -1 : (int32_t)s;
-    later[threadIdx.x] = 0;
+    if (!p.table) later[threadIdx.x] = 0;
   };
   const uint64_t stride = (uint64_t)gridDim.x * p.run;
   uint32_t cur = 0;
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(256, 5) write_kernel(const Write p) {
         const uint32_t i = at[n], d = 8 * i;
         int32_t to = -1;
         if (u0 + n * 256 + threadIdx.x < items)
-          to = !p.slots ? (int32_t)(r0 + from[n]) : later[from[n]] ? -1 : dest[cur][from[n]];
+          to = !p.slots ? (int32_t)(r0 + from[n]) : !p.table && later[from[n]] ? -1 : dest[cur][from[n]];
         if (to < 0) continue;
         uint32_t word = 0;
         if (odd[n]) {
@@ -310,7 +312,8 @@ __global__ void __launch_bounds__(256, 5) write_kernel(const Write p) {
 
 // ---------------------------------------------------------------------------
 // Reading: a lane writes 16 bytes of the output, half a word of f32 or a whole one
-// of 16-bit values, four such pieces at once. Rows of no id are 0.
+// of 16-bit values, four such pieces at once. Rows of no id are 0. 1000000 random rows x
+// 128 as bf16 71 us, 360 MB at 5.1 TB/s: memory and issue slots about even.
 // ---------------------------------------------------------------------------
 struct Read {
   const uint8_t* codes;

@@ -1,23 +1,24 @@
 // Scores of more than a few queries against 4-bit rows: as score4.cuh, with the sums
-// by tcgen05.mma. 32 or 64 columns (queries; two for one of f32) are the N side, 128
+// by tcgen05.mma. 32, 64 or 96 columns (queries; two for one of f32) are the N side, 128
 // rows the M side. What a warp of mma.sync instructions does per query (fragments
 // from shared memory, sums in registers) took more instructions than the codes
 // themselves from 16 columns on.
 //
 // A group of four warps takes a tile of 128 rows, a row a thread. Codes come by TMA;
 // a thread turns its row's 128 codes of a block into f16 operands code + z (as many
-// instructions as code - 8 in score4.cuh; z is its own row's) and writes them to tensor memory,
-// which the instruction reads its M side from: shared memory holds queries only,
-// and its bandwidth goes to them. A scale group is a chain of instructions of its
-// own; the thread then reads its row's sums of the group and adds them,
-// times the group's step, to its own in registers. Three or four such groups of warps
-// per SM (teams) work on tiles of their own, so that one's instructions and waits are
-// hidden by the others'. A thread has all scores of its row, and a warp writes 32
+// instructions as code - 8 in score4.cuh; z is its own row's) and writes them to
+// tensor memory, which the instruction reads its M side from: shared memory holds
+// queries only, and its bandwidth goes to them. A scale group is a chain of
+// instructions of its own; the thread then reads its row's sums of the group and adds
+// them, times the group's step, to its own in registers. Three or four such groups of
+// warps per SM (teams) work on tiles of their own, so that one's instructions and waits
+// are hidden by the others'. A thread has all scores of its row, and a warp writes 32
 // scores of a query side by side, wherever the query's scores start.
 //
-// An instruction of 16 values takes about 64 cycles up to 96 columns, since that is
-// how long its M side takes to come from tensor memory: 512 for a block, of which
-// teams that wait for one another's make 1000.
+// What bounds it: a team's chain on a block (operands, instructions, sums). Chains of 32
+// and of 64 columns took the same time, as if an instruction of 16 values took about 64
+// cycles, three teams' waiting for one another. 64 x 1000000 x 128 70 us, 4.7 TB/s;
+// 32 x 65536 x 1024 23 us, 1.9 TB/s.
 #pragma once
 
 #include "score4.cuh"
