@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "../../include/raven_gpu.h"
 #include "internal.h"
@@ -176,6 +177,13 @@ cudaError_t launch_join(const raven_score4::Join& j, int out_type, int sms, cuda
                 0, none, st, j);
 }
 
+// The slices take alpha's power of two and the join what it leaves, 1 to 2: a slice's sum is of the score's size, so
+// what it loses among the subnormal numbers is lost of the score, not of what alpha has yet to make large.
+void share_alpha(raven_score4::Params* p, raven_score4::Join* j) {
+  j->alpha = p->alpha;
+  p->alpha = 1.f;
+}
+
 template <int NT, int MT, int G, bool F32>
 cudaError_t run_score4(const raven_rows* v, raven_score4::Params p, int out_type, int sms, cudaStream_t st) {
   using namespace raven_score4;
@@ -226,7 +234,7 @@ cudaError_t run_score4(const raven_rows* v, raven_score4::Params p, int out_type
     p.out = tmp + laid;
     p.ld = wide;
     p.ld_slice = p.nq * wide;
-    p.alpha = 1.f;
+    share_alpha(&p, &j);
     p.bias = nullptr;
   }
   if (lay) {
@@ -303,7 +311,7 @@ cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, 
     p.out = tmp + laid;
     p.ld = wide;
     p.ld_slice = p.nq * wide;
-    p.alpha = 1.f;
+    share_alpha(&p, &j);
     p.bias = nullptr;
   }
   if (lay) {
@@ -411,7 +419,8 @@ int int4_scores(const raven_rows* q, const raven_rows* v, uint32_t dim, float al
   p.blocks = (dim + raven_int4::kBlock - 1) / raven_int4::kBlock;
   const uint32_t group = int4_group(v->type);
   p.groups = (dim + group - 1) / group;
-  p.alpha = alpha;
+  p.alpha_exp = alpha != 0.f && std::isfinite(alpha) ? std::ilogb(alpha) : 0;
+  p.alpha = std::scalbn(alpha, -p.alpha_exp);
   p.bias = bias;
   p.out = out;
   p.ld = ld;

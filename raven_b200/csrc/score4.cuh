@@ -54,7 +54,8 @@ using raven_tc::mbar_init;
 using raven_tc::smem_u32;
 using raven_tc::tma_load_2d;
 
-constexpr int kStepShift = 16;     // steps are taken times 2^-16: sums are up to 2^29 times a query's largest value
+// Steps are taken times 2^-16: sums are up to 2^29 times a query's largest value. Steps below 2^-110 lose low bits by it.
+constexpr int kStepShift = 16;
 constexpr uint32_t kMaxDepth = 6;  // tiles under way per warp, at most
 
 struct Params {
@@ -72,7 +73,8 @@ struct Params {
   uint32_t depth;     // of the rings
   uint32_t chunks;    // of the queries
   uint32_t tiles;     // of a CTA's rows
-  float alpha;
+  float alpha;        // times 2^alpha_exp; 1 to 2 in size, or 0 or not finite
+  int alpha_exp;
   const float* bias;
   void* out;          // of slice s at out + s * ld_slice
   uint64_t ld, ld_slice;
@@ -82,8 +84,8 @@ struct Params {
 
 // A chunk of queries as the kernel takes it, NT * 8 columns: fragments (for each
 // unit and N tile 16 bytes a lane), then per group the columns' sums, then per
-// query what brings its sums back: alpha times a power of two, or where that is no
-// f32 a NaN, and the power as two factors. f32 queries have two columns side by
+// query what brings its sums back, alpha times a power of two: as one factor, or
+// where that is near the ends of f32's range as three. f32 queries have two columns side by
 // side, the second for what the first leaves and without sums.
 template <int NT>
 struct Laid {
@@ -101,7 +103,7 @@ struct Laid {
   __device__ static void put_sum(uint8_t* to, uint32_t group, uint32_t col, float sum) {
     ((float*)to)[group * (NT * 8) + col] = sum;
   }
-  // What brings query q's sums back: a factor, two, a flag.
+  // What brings query q's sums back: three factors, whether the last two are not 1.
   __device__ static void put_back(float* back, uint32_t q, float f, float k0, float k1, float flag) {
     *(float4*)(back + 4 * q) = make_float4(f, k0, k1, flag);
   }
@@ -197,11 +199,13 @@ __device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, 
     }
     if (i == 0) {
       const int b = kStepShift - e;  // -147 .. 129
-      // exact where alpha's exponent leaves it among the normal numbers
-      const int a = p.alpha == 0.f ? 0 : ilogbf(p.alpha) + b;
-      const bool plain = a >= -120 && a <= 120 && (p.alpha == 0.f || fabsf(p.alpha) < INFINITY) && b >= -126 && b <= 127;
-      const float none = __uint_as_float(0x7fc00000u), k0 = bad ? none : pow2(b / 2), k1 = pow2(b - b / 2);
-      Q::put_back(back, F32 ? c / 2 : c, plain && !bad ? p.alpha * k0 * k1 : none, k0, k1, plain || bad ? 0.f : 1.f);
+      // Three factors of one third of the exponent each, so all on one side of 1: a product in between is
+      // subnormal only where the score is nearer to 0 still. With alpha last a sum of 1e-43 would have lost its bits.
+      const int by = p.alpha_exp + b;  // -296 .. 256
+      const bool plain = bad || (by >= -120 && by <= 120);
+      const int third = plain ? 0 : by / 3;
+      const float k = pow2(third), f = bad ? __uint_as_float(0x7fc00000u) : p.alpha * pow2(by - 2 * third);
+      Q::put_back(back, F32 ? c / 2 : c, f, k, k, plain ? 0.f : 1.f);
     }
   }
 }
@@ -563,9 +567,9 @@ __global__ void __launch_bounds__(Layout<NT, MT, G>::kThreads, 1) score4_kernel(
 #pragma unroll
             for (int r = 0; r < R; ++r) o[r] = rounded<O>(fmaf(f, y[r], bias[r]));
           } else {
-            const float k0 = back[4 * (F32 ? col / 2 : col) + 1], k1 = back[4 * (F32 ? col / 2 : col) + 2];
+            const float4 f = *(const float4*)(back + 4 * (F32 ? col / 2 : col));
 #pragma unroll
-            for (int r = 0; r < R; ++r) o[r] = rounded<O>(fmaf(p.alpha, y[r] * k0 * k1, bias[r]));
+            for (int r = 0; r < R; ++r) o[r] = rounded<O>(fmaf(y[r] * f.x * f.y, f.z, bias[r]));
           }
           O* to = (O*)p.out + slice * p.ld_slice + query * p.ld + row;
           if (p.whole && row + R <= p.n) {

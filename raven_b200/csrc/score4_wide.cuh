@@ -38,7 +38,7 @@ struct WideLaid {
     return unit / 2 * kBlockBytes + col * 128 + ((((unit & 1) * 4 + quarter) ^ (col & 7)) * 16);
   }
   __device__ static void put_sum(uint8_t*, uint32_t, uint32_t, float) {}
-  // What brings query q's sums back: a factor, or two and a flag.
+  // What brings query q's sums back: three factors, whether the last two are not 1.
   __device__ static void put_back(float* back, uint32_t q, float f, float k0, float k1, float flag) {
     back[q] = f;
     back[NC + 2 * q] = k0;
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
           if (q < here) {
             const float y = F32 ? total[2 * q] + total[2 * q + 1] : total[q];
             *to = rounded<O>(plain ? fmaf(back[q], y, bias)
-                                   : fmaf(p.alpha, y * back[NC + 2 * q] * back[NC + 2 * q + 1], bias));
+                                   : fmaf(y * back[q] * back[NC + 2 * q], back[NC + 2 * q + 1], bias));
             to += p.ld;
           }
         }

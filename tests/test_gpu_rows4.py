@@ -279,7 +279,7 @@ def _check(got, q, rows, t, alpha=1.0, bias=None, f32_queries=True):
 
 SCORES = [(1, 1, 1), (1, 7, 32), (2, 33, 96), (3, 65, 100), (5, 130, 128), (7, 100, 129), (8, 257, 200), (9, 300, 256),
           (16, 100, 384), (17, 500, 515), (31, 130, 1000), (33, 1000, 64), (64, 333, 130), (65, 200, 96), (130, 90, 300),
-          (1, 5000, 128), (4, 3, 4096), (2, 40, 5000)]
+          (1, 5000, 128), (4, 3, 4096), (2, 40, 5000), (20, 70, 1), (40, 300, 20), (70, 129, 33), (96, 128, 128), (25, 1, 500)]
 
 
 @pytest.mark.parametrize("group", GROUPS)
@@ -309,6 +309,20 @@ def test_scores_alpha_bias_pitch(S):
     _check(S.scores(wide, rows), _np(wide), rows, "f32", f32_queries=False)
     one = _gpu(_data(300, 3, 3, 1.0))[:, 1]
     _check(S.scores(one.reshape(300, 1).T.contiguous(), rows), _np(one)[None], rows, "f32")
+
+
+@pytest.mark.parametrize("nq", [3, 12, 40])
+def test_scores_any_alpha(S, nq):
+    """alpha and a query's scale, apart and together at the ends of f32's range."""
+    torch = _torch()
+    rows = S.Int4Rows.encode(_gpu(_data(50, 100, 1, 1.0)), 32)
+    q = _data(nq, 100, 2, 1.0)
+    for alpha, scale in ((0.0, 1.0), (-3.0, 1.0), (1e30, 1e-25), (1e-30, 1e25), (1e38, 1e-38), (1e-38, 1e30), (1e-42, 1e20), (3e38, 1e-44)):
+        x = _gpu(q * scale)
+        got, a = S.scores(x, rows, alpha=alpha), float(np.float32(alpha))
+        _check(got, _np(x), rows, "f32", alpha=a)
+    for alpha in (float("inf"), float("nan")):
+        assert not bool(torch.isfinite(S.scores(_gpu(q), rows, alpha=alpha)).any())
 
 
 def test_scores_of_wide_ranges(S):
@@ -385,7 +399,10 @@ def test_scores_every_code_and_offset(S):
     rows = S.Int4Rows(codes, torch.from_numpy(word.reshape(-1, 1)).cuda(), 1, 128)
     want = (c + z) * step.astype(np.float64)
     np.testing.assert_array_equal(_np(rows.decode())[:, 0], want)
-    np.testing.assert_array_equal(_np(S.scores(torch.full((1, 1), 2.0, device="cuda"), rows))[0], 2 * want)
+    for nq in (1, 6, 12, 20, 40):
+        for t in TYPES:
+            got = _np(S.scores(torch.full((nq, 1), 2.0, device="cuda", dtype=_dt(t)), rows))
+            np.testing.assert_array_equal(got, np.broadcast_to(2 * want, got.shape))
 
 
 def test_scores_empty(S):
