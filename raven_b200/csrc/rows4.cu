@@ -273,7 +273,7 @@ cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, 
   p.tiles = (uint32_t)((p.n + kWideRows - 1) / kWideRows);
   // Slices of a row: those that take least time, in microseconds. A block of a team takes 0.6 and 0.55 for each scale
   // group's chain, a tile's end 0.7, a block of queries NC / 128, the join 3 and its bytes (40 x 5000 x 1000, groups of
-  // 32: 30 us in one slice, 13.6 in those that this gives).
+  // 32: 30 us in one slice, 13.9 in those that this gives).
   auto bytes = [&](uint32_t slice, uint32_t depth) {
     return L::bytes(std::min(4 * slice, p.units), depth);
   };

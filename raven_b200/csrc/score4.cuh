@@ -85,8 +85,8 @@ struct Params {
 // A chunk of queries as the kernel takes it, NT * 8 columns: fragments (for each
 // unit and N tile 16 bytes a lane), then per group the columns' sums, then per
 // query what brings its sums back, alpha times a power of two: as one factor, or
-// where that is near the ends of f32's range as three. f32 queries have two columns side by
-// side, the second for what the first leaves and without sums.
+// where that is near the ends of f32's range as three. f32 queries have two
+// columns side by side, the second for what the first leaves and without sums.
 template <int NT>
 struct Laid {
   static constexpr uint32_t kColumns = NT * 8;

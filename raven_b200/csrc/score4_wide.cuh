@@ -18,7 +18,7 @@
 // What bounds it: a team's chain on a block (operands, instructions, sums). Chains of 32
 // and of 64 columns took the same time, as if an instruction of 16 values took about 64
 // cycles, three teams' waiting for one another. 64 x 1000000 x 128 70 us, 4.7 TB/s;
-// 32 x 65536 x 1024 23 us, 1.9 TB/s.
+// 32 x 65536 x 1024 23.5 us, 1.9 TB/s.
 #pragma once
 
 #include "score4.cuh"
