@@ -177,13 +177,6 @@ cudaError_t launch_join(const raven_score4::Join& j, int out_type, int sms, cuda
                 0, none, st, j);
 }
 
-// The slices take alpha's power of two and the join what it leaves, 1 to 2: a slice's sum is of the score's size, so
-// what it loses among the subnormal numbers is lost of the score, not of what alpha has yet to make large.
-void share_alpha(raven_score4::Params* p, raven_score4::Join* j) {
-  j->alpha = p->alpha;
-  p->alpha = 1.f;
-}
-
 template <int NT, int MT, int G, bool F32>
 cudaError_t run_score4(const raven_rows* v, raven_score4::Params p, int out_type, int sms, cudaStream_t st) {
   using namespace raven_score4;
@@ -224,17 +217,18 @@ cudaError_t run_score4(const raven_rows* v, raven_score4::Params p, int out_type
   const bool lay = std::min<uint64_t>(p.nq, kQueries) * p.dim > kOwnLayout;
   const uint64_t laid = lay ? (p.chunks * Q::bytes(p.units, p.groups) + 255) / 256 * 256 : 0;
   const uint64_t wide = (p.n + 3) / 4 * 4, sums = p.slices > 1 ? p.slices * p.nq * wide * 4 : 0;
+  const uint64_t backs = p.slices > 1 ? (uint64_t)p.chunks * kQueries * 16 : 0;
   if (sums > kMostSums && p.n >= 512)
     return in_halves(v, whole, out_type, [&](const raven_rows* r, const Params& q) {
       return run_score4<NT, MT, G, F32>(r, q, out_type, sms, st);
     });
-  if (laid + sums && (e = cudaMallocAsync((void**)&tmp, laid + sums, st)) != cudaSuccess) return e;
-  Join j{(const float*)(tmp + laid), wide, p.nq * wide, p.slices, p.nq, p.n, p.alpha, p.bias, p.out, p.ld};
+  if (laid + sums + backs && (e = cudaMallocAsync((void**)&tmp, laid + sums + backs, st)) != cudaSuccess) return e;
+  if (backs) p.backs = (float4*)(tmp + laid + sums);
+  const Join j{(const float*)(tmp + laid), wide, p.nq * wide, p.slices, p.nq, p.n, p.backs, p.bias, p.out, p.ld};
   if (p.slices > 1) {
     p.out = tmp + laid;
     p.ld = wide;
     p.ld_slice = p.nq * wide;
-    share_alpha(&p, &j);
     p.bias = nullptr;
   }
   if (lay) {
@@ -302,16 +296,17 @@ cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, 
   const bool lay = std::min<uint64_t>(p.nq, kQueries) * p.dim > kOwnLayout;
   const uint64_t laid = lay ? (p.chunks * Q::bytes(p.units, 0) + 255) / 256 * 256 : 0;
   const uint64_t wide = (p.n + 3) / 4 * 4, sums = p.slices > 1 ? p.slices * p.nq * wide * 4 : 0;
+  const uint64_t backs = p.slices > 1 ? (uint64_t)p.chunks * kQueries * 16 : 0;
   if (sums > kMostSums && p.n >= 512)
     return in_halves(v, whole, out_type,
                      [&](const raven_rows* r, const Params& q) { return run_wide<NC, G, F32>(r, q, out_type, sms, st); });
-  if (laid + sums && (e = cudaMallocAsync((void**)&tmp, laid + sums, st)) != cudaSuccess) return e;
-  Join j{(const float*)(tmp + laid), wide, p.nq * wide, p.slices, p.nq, p.n, p.alpha, p.bias, p.out, p.ld};
+  if (laid + sums + backs && (e = cudaMallocAsync((void**)&tmp, laid + sums + backs, st)) != cudaSuccess) return e;
+  if (backs) p.backs = (float4*)(tmp + laid + sums);
+  const Join j{(const float*)(tmp + laid), wide, p.nq * wide, p.slices, p.nq, p.n, p.backs, p.bias, p.out, p.ld};
   if (p.slices > 1) {
     p.out = tmp + laid;
     p.ld = wide;
     p.ld_slice = p.nq * wide;
-    share_alpha(&p, &j);
     p.bias = nullptr;
   }
   if (lay) {
@@ -421,6 +416,8 @@ int int4_scores(const raven_rows* q, const raven_rows* v, uint32_t dim, float al
   p.groups = (dim + group - 1) / group;
   p.alpha_exp = alpha != 0.f && std::isfinite(alpha) ? std::ilogb(alpha) : 0;
   p.alpha = std::scalbn(alpha, -p.alpha_exp);
+  p.top = 14;
+  while (p.top > 10 && dim > 4096u << (14 - p.top)) --p.top;
   p.bias = bias;
   p.out = out;
   p.ld = ld;

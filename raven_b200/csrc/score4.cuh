@@ -4,8 +4,8 @@
 //
 // The inner sums run on the tensor cores (here mma m16n8k16, f16 operands, f32 sums)
 // with rows as the M side and queries as the N side. 4 bits at the bottom of the f16
-// 1024 are 1024 + code, at bits 4-7 1024 + 16 code: one LOP3 and one f16 addition (or
-// multiply-add) make code - 8 of two codes, nine instructions per eight. Without the
+// 1024 (times 2^-12, see below) are 1024 + code, at bits 4-7 1024 + 16 code: one LOP3 and one
+// f16 addition (or multiply-add) make code - 8 of two codes, nine instructions per eight. Without the
 // additions the 4 bits alone are an f16 too, a subnormal, but the tensor cores line
 // products up by their exponent fields and drop what is below the sum's bits, and
 // subnormals lose as many of them as they have leading zeros: scores were off by 1e-6
@@ -13,9 +13,10 @@
 // sides agree: lane t of a row's four takes the eight values 8t.. of each unit of 32
 // (one word), as pairs (0, 4), (1, 5), (2, 6), (3, 7).
 //
-// Queries are brought to a largest magnitude in [2^14, 2^15) by a power of two
-// each, so that f16 holds what f32, f16 and bf16 values may be: 11 bits of a value
-// in one part, 22 in two (f32), nothing below 2^-39 of the largest. The sum of a
+// Queries are brought to a largest magnitude in [2^14, 2^15) (less for rows of more
+// than 4096 values) by a power of two each, so that f16 holds what f32, f16 and bf16
+// values may be: 11 bits of a value in one part, 22 in two (f32), nothing below 2^-39
+// of the largest (2^-35 in the longest rows). The sum of a
 // group starts at (z + 8) * sum(q), and its step is applied in f32 when the group
 // ends: the scale is never rounded into an operand. Two parts of an f32 query are two
 // columns of the N side, added up at the end.
@@ -54,8 +55,16 @@ using raven_tc::mbar_init;
 using raven_tc::smem_u32;
 using raven_tc::tma_load_2d;
 
-// Steps are taken times 2^-16: sums are up to 2^29 times a query's largest value. Steps below 2^-110 lose low bits by it.
-constexpr int kStepShift = 16;
+// A row's sum is kept times 2^-28, and a query is brought to a largest magnitude in [2^14, 2^15), in rows of more than
+// 4096 values to one lower by what they have more (2^10 for 65536): of dim products with values below 2^128 (a little
+// above where a group goes from f32's lowest to its largest) it is at most 2^127 then, whatever the values are and
+// however they cancel. It is brought to the score's size at the very end. Of the 2^-28 the operands take 2^-12 (code - 8
+// and code + z are whole numbers of 8 bits: f16 holds them as well times that), which costs nothing, and the steps
+// 2^-16, so that a step, of 16 significant bits, is exact down to 2^-118. A group's addition to a sum loses what is
+// below 2^-136 of a query's largest value (2^-132 in the longest rows).
+constexpr int kCodeShift = 12, kStepShift = 16;
+constexpr float kCodeScale = 1.f / (1 << kCodeShift);
+constexpr uint32_t kCodeBase = 0x34003400u;  // the f16 1024 * 2^-12, twice: 4 bits at its bottom are a code * 2^-12 more
 constexpr uint32_t kMaxDepth = 6;  // tiles under way per warp, at most
 
 struct Params {
@@ -75,9 +84,11 @@ struct Params {
   uint32_t tiles;     // of a CTA's rows
   float alpha;        // times 2^alpha_exp; 1 to 2 in size, or 0 or not finite
   int alpha_exp;
+  int top;            // queries are brought to a largest magnitude in [2^top, 2^(top + 1))
   const float* bias;
-  void* out;          // of slice s at out + s * ld_slice
+  void* out;          // of slice s at out + s * ld_slice: sums as they are kept
   uint64_t ld, ld_slice;
+  float4* backs;      // of slices: what brings each query's sums back, or null
   bool whole;         // four scores of a query can be written at once
   int* status;
 };
@@ -168,7 +179,7 @@ __device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, 
   for (uint32_t u0 = 0; u0 < count * n8; u0 += blockDim.x) {
     const uint32_t u = u0 + threadIdx.x, q = min(u / n8, count - 1), i = u - q * n8;  // past the last item: past the last unit
     const bool bad = top[q] >= 0x7f800000u;
-    const int e = top[q] == 0 || bad ? 14 : 14 - ilogbf(__uint_as_float(top[q]));  // -113 .. 163
+    const int e = top[q] == 0 || bad ? p.top : p.top - ilogbf(__uint_as_float(top[q]));  // -117 .. 163
     const float m0 = pow2(e / 2), m1 = pow2(e - e / 2);
     float v[8], sum = 0.f;
     load(q, 4 * unit0 + i, v);
@@ -181,7 +192,7 @@ __device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, 
     for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const uint32_t c = col + (F32 ? 2 * q : q);
     if (i % L == 0 && i / L < groups) {
-      Q::put_sum(sums, i / L, c, sum);
+      Q::put_sum(sums, i / L, c, sum * kCodeScale);
       if (F32) Q::put_sum(sums, i / L, c + 1, 0.f);
     }
     if (i < units * 4) {
@@ -198,14 +209,19 @@ __device__ inline void lay_out(const Params& p, uint64_t first, uint32_t count, 
         *(uint4*)(to + Q::frag_at(i >> 2, i & 3, c + h)) = *(const uint4*)part[h];
     }
     if (i == 0) {
-      const int b = kStepShift - e;  // -147 .. 129
       // Three factors of one third of the exponent each, so all on one side of 1: a product in between is
-      // subnormal only where the score is nearer to 0 still. With alpha last a sum of 1e-43 would have lost its bits.
-      const int by = p.alpha_exp + b;  // -296 .. 256
+      // subnormal only where the score is nearer to 0 still, and infinite only where the score is. With alpha last a
+      // sum of 1e-43 would have lost its bits.
+      const int by = p.alpha_exp + kCodeShift + kStepShift - e;  // -284 .. 272
       const bool plain = bad || (by >= -120 && by <= 120);
       const int third = plain ? 0 : by / 3;
       const float k = pow2(third), f = bad ? __uint_as_float(0x7fc00000u) : p.alpha * pow2(by - 2 * third);
-      Q::put_back(back, F32 ? c / 2 : c, f, k, k, plain ? 0.f : 1.f);
+      if (p.backs) {  // the join brings sums back; CTAs that have this query write the same
+        p.backs[first + q] = make_float4(f, k, k, plain ? 0.f : 1.f);
+        Q::put_back(back, F32 ? c / 2 : c, 1.f, 1.f, 1.f, 0.f);
+      } else {
+        Q::put_back(back, F32 ? c / 2 : c, f, k, k, plain ? 0.f : 1.f);
+      }
     }
   }
 }
@@ -260,21 +276,21 @@ __device__ inline void meet(uint32_t id, uint32_t threads) {
   asm volatile("bar.sync %0, %1;\n" ::"r"(id), "r"(threads) : "memory");
 }
 
-// Eight codes less 8 as four operands of two.
+// Eight codes less 8, times 2^-12, as four operands of two.
 __device__ inline void operands(uint32_t w, uint32_t& a0, uint32_t& a1, uint32_t& a2, uint32_t& a3) {
   auto low = [](uint32_t code) {
-    const __half2 r = __hadd2(*(const __half2*)&code, __float2half2_rn(-1032.f));
+    const __half2 r = __hadd2(*(const __half2*)&code, __float2half2_rn(-1032.f * kCodeScale));
     return *(const uint32_t*)&r;
   };
   auto high = [](uint32_t code) {
-    const __half2 r = __hfma2(*(const __half2*)&code, __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
+    const __half2 r = __hfma2(*(const __half2*)&code, __float2half2_rn(0.0625f), __float2half2_rn(-72.f * kCodeScale));
     return *(const uint32_t*)&r;
   };
   const uint32_t v = w >> 8;
-  a0 = low((w & 0x000f000fu) | 0x64006400u);
-  a1 = high((w & 0x00f000f0u) | 0x64006400u);
-  a2 = low((v & 0x000f000fu) | 0x64006400u);
-  a3 = high((v & 0x00f000f0u) | 0x64006400u);
+  a0 = low((w & 0x000f000fu) | kCodeBase);
+  a1 = high((w & 0x00f000f0u) | kCodeBase);
+  a2 = low((v & 0x000f000fu) | kCodeBase);
+  a3 = high((v & 0x00f000f0u) | kCodeBase);
 }
 
 __device__ inline void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -604,7 +620,7 @@ struct Join {
   uint64_t ld, ld_slice;  // of the sums
   uint32_t slices;
   uint64_t nq, n;
-  float alpha;
+  const float4* backs;
   const float* bias;
   void* out;
   uint64_t ld_out;
@@ -625,9 +641,13 @@ __global__ void __launch_bounds__(256) join_kernel(const Join p) {
       v.w += x.w;
     }
     const float y[4] = {v.x, v.y, v.z, v.w};
+    const float4 f = p.backs[q];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (j + r < p.n) ((O*)p.out)[q * p.ld_out + j + r] = rounded<O>(fmaf(p.alpha, y[r], p.bias ? p.bias[j + r] : 0.f));
+    for (int r = 0; r < 4; ++r) {
+      if (j + r >= p.n) continue;
+      const float bias = p.bias ? p.bias[j + r] : 0.f;
+      ((O*)p.out)[q * p.ld_out + j + r] = rounded<O>(f.w == 0.f ? fmaf(f.x, y[r], bias) : fmaf(y[r] * f.x * f.y, f.z, bias));
+    }
   }
 }
 

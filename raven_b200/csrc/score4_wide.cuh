@@ -64,15 +64,16 @@ struct Wide {
   }
 };
 
-// What is added to a row's codes of a group: z - 1024 to 1024 + code, z - 64 to a sixteenth of 1024 + 16 code. All
-// are whole numbers below 2048, which f16 holds. z + 128 at the bottom of the f16 1024 is 1152 + z.
+// What is added to a row's codes of a group, in units of 2^-12 (kCodeShift): z - 1024 to 1024 + code, z - 64 to a
+// sixteenth of 1024 + 16 code. All are whole numbers below 2048, which f16 holds. z + 128 at the bottom of 1024
+// is 1152 + z.
 struct Offsets {
   __half2 low, high;
   __device__ explicit Offsets(uint32_t word) {
-    const uint32_t b = __byte_perm(word, 0x64u, 0x4040) ^ 0x00800080u;
-    const __half2 z = __hsub2(*(const __half2*)&b, __float2half2_rn(1152.f));
-    low = __hadd2(z, __float2half2_rn(-1024.f));
-    high = __hadd2(z, __float2half2_rn(-64.f));
+    const uint32_t b = __byte_perm(word, kCodeBase >> 24, 0x4040) ^ 0x00800080u;
+    const __half2 z = __hsub2(*(const __half2*)&b, __float2half2_rn(1152.f * kCodeScale));
+    low = __hadd2(z, __float2half2_rn(-1024.f * kCodeScale));
+    high = __hadd2(z, __float2half2_rn(-64.f * kCodeScale));
   }
 };
 // Eight codes, with z, as four operands of two.
@@ -86,10 +87,10 @@ __device__ inline void operands(uint32_t w, const Offsets& z, uint32_t& a0, uint
     return *(const uint32_t*)&r;
   };
   const uint32_t v = w >> 8;
-  a0 = low((w & 0x000f000fu) | 0x64006400u);
-  a1 = high((w & 0x00f000f0u) | 0x64006400u);
-  a2 = low((v & 0x000f000fu) | 0x64006400u);
-  a3 = high((v & 0x00f000f0u) | 0x64006400u);
+  a0 = low((w & 0x000f000fu) | kCodeBase);
+  a1 = high((w & 0x00f000f0u) | kCodeBase);
+  a2 = low((v & 0x000f000fu) | kCodeBase);
+  a3 = high((v & 0x00f000f0u) | kCodeBase);
 }
 
 __device__ inline void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {

@@ -1,0 +1,92 @@
+"""4-bit rows, scores against them and adjusted scores at the ends: of f32's range, of sizes, of what a call allows."""
+import numpy as np
+import pytest
+
+import rows4_util as U
+
+pytestmark = pytest.mark.gpu
+
+GROUPS = (32, 64, 128)
+
+
+def _torch():
+    import torch
+
+    return torch
+
+
+@pytest.fixture(scope="module")
+def S(raven_lib):
+    from raven_b200 import scoring
+
+    return scoring
+
+
+def _gpu(x, t="float32"):
+    torch = _torch()
+    return torch.from_numpy(np.ascontiguousarray(x)).cuda().to(getattr(torch, t))
+
+
+def _np(t):
+    return t.double().cpu().numpy()
+
+
+def _words(rows):
+    return rows.scales.cpu().numpy().view(np.uint32)
+
+
+def _check(got, q, rows, alpha=1.0, bias=None):
+    """f32 scores against the definition in 64 bits; rows4_util.score_bound says how far off they may be. Scores whose
+    exact value f32 holds with that bound to spare have to be finite."""
+    codes, words = rows.codes.cpu().numpy(), _words(rows)
+    v = U.values(codes, words, rows.dim, rows.group)
+    exact = alpha * (q @ v.T) + (0.0 if bias is None else bias[None, :])
+    lim = U.score_bound(q, codes, words, rows.dim, rows.group, alpha, bias, 2.0 ** -23, exact, True)
+    got = _np(got)
+    held = np.abs(exact) + lim < np.finfo(np.float32).max
+    assert np.isfinite(got[held]).all()
+    off = np.abs(got[held] - exact[held])
+    assert np.all(off <= lim[held]), (off / lim[held]).max()
+    return held
+
+
+# Few queries, wide ones of 32, 64 and 96 columns; rows that are one slice of all of them, and rows of several.
+@pytest.mark.parametrize("dim", [1, 64, 200, 1000, 8200, 20_000])
+@pytest.mark.parametrize("nq", [1, 6, 12, 30, 45])
+def test_scores_of_the_largest_values(S, nq, dim):
+    """Rows of up to f32's largest values against small queries, or with a small alpha: the scores are ordinary ones."""
+    r = np.random.default_rng(nq * dim)
+    x = 3.4e38 * np.where(np.arange(40)[:, None] % 2 == 0, 1.0, r.uniform(-1, 1, (40, dim)))
+    x[::5] *= r.choice([-1.0, 1.0], (8, dim))
+    x[1::5] *= 1e-3
+    u = r.uniform(0.5, 1.0, (nq, dim)) * r.choice([-1.0, 1.0], (nq, 1))
+    for group in GROUPS if dim < 8000 else (GROUPS[nq % 3],):
+        rows = S.Int4Rows.encode(_gpu(x), group)
+        for size, alpha in ((1e-38, 1.0), (1e-3 / dim, 1.0), (1.0, 1e-30), (1e10, -1e-42), (1e-30, 1e-10), (1e-36, 1e30)):
+            q = _gpu(u * size)
+            bias = _gpu(r.normal(size=40)) if alpha == 1.0 else None
+            got = S.scores(q, rows, alpha=alpha, bias=bias)
+            assert _check(got, _np(q), rows, float(np.float32(alpha)), None if bias is None else _np(bias)).all()
+
+
+@pytest.mark.parametrize("dim", [64, 512, 20_032])
+@pytest.mark.parametrize("nq", [1, 12, 45])
+def test_scores_of_the_largest_values_that_cancel(S, nq, dim):
+    """The first half of a row against the second: sums pass f32's largest value on the way, most scores do not. (Of the
+    longest rows against a query of 1 the bound alone passes it: 1900 roundings of 2^-23 of magnitudes of 6e42.)"""
+    half = dim // 2
+    x = np.full((9, dim), 3e38)
+    x[:, half:] *= -np.linspace(0.0, 1.0, 9)[:, None]
+    rows = S.Int4Rows.encode(_gpu(x), 32)
+    q = _gpu(np.repeat(2.0 ** -np.arange(float(nq))[:, None], dim, 1))
+    _check(S.scores(q, rows), _np(q), rows)
+
+
+def test_scores_tell_what_is_too_large(S):
+    """Past f32's largest value a score is infinite, with its sign."""
+    torch = _torch()
+    rows = S.Int4Rows.encode(torch.full((3, 96), 3e38, device="cuda"))
+    for nq in (1, 12, 45):
+        q = torch.ones(nq, 96, device="cuda")
+        assert bool((S.scores(q, rows) == float("inf")).all())
+        assert bool((S.scores(q, rows, alpha=-1.0) == -float("inf")).all())
