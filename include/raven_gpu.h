@@ -339,8 +339,9 @@ RAVEN_API int raven_index_int4_device(raven_index* ix, const raven_rows* out, vo
  * With 4-bit vectors they are f32, f16 or bf16 rows at any ld >= dim; nothing is
  * rounded before the sums but f32 queries, to 22 bits of each value, and what is
  * below 2^-34 of a query's largest. No sum overflows where its score does not,
- * whatever the sizes of rows, queries and alpha are; steps below 2^-110 lose low
- * bits. A query with an infinity or a NaN has scores of NaN. */
+ * whatever the sizes of rows, queries and alpha are; steps below 2^-118 lose low
+ * bits, and a group's share of a sum what is below 2^-132 of the query's largest
+ * value. A query with an infinity or a NaN has scores of NaN. */
 RAVEN_API int raven_scores_device(const raven_rows* q, const raven_rows* v, uint32_t dim, float alpha,
                                   const float* d_bias, void* d_out, int32_t out_type, uint64_t ld_out,
                                   int32_t* d_status, void* stream);

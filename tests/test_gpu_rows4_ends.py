@@ -90,3 +90,35 @@ def test_scores_tell_what_is_too_large(S):
         q = torch.ones(nq, 96, device="cuda")
         assert bool((S.scores(q, rows) == float("inf")).all())
         assert bool((S.scores(q, rows, alpha=-1.0) == -float("inf")).all())
+
+
+@pytest.mark.parametrize("dim", [1, 128, 5000, 65_536])
+def test_scores_of_the_smallest_steps(S, dim):
+    """Steps of 16 significant bits are exact down to 2^-118, and lose what is below 2^-134 from there on. One value of
+    a query is not 0, so a score is one product: off by that loss, and by half of what the last bit of a sum stands
+    for, 2^-149 * 2^28 / 2^10 / 2 = 2^-132 of the query's largest value (2^28 the sum's scale, 2^10 the query's in the
+    longest rows, 2^14 in short ones)."""
+    torch = _torch()
+    r = np.random.default_rng(dim)
+    n = 4096
+    exp = np.repeat(np.arange(-127, -95), n // 32)
+    step = (2 ** 15 + r.integers(0, 2 ** 15, n)) * 2.0 ** (exp - 15)
+    c, z = r.integers(0, 16, n), r.integers(-127, 113, n)
+    for group in GROUPS:
+        rows = S.Int4Rows.empty(n, dim, "cuda", group)
+        rows.codes.zero_(), rows.scales.zero_()
+        at, shift = U.held_codes(dim)
+        last = dim - 1  # a value of the last group
+        rows.codes[:, int(at[last])] = _gpu((c << shift[last]).astype(np.uint8), "uint8")
+        word = step.astype(np.float32).view(np.uint32) & np.uint32(0xFFFFFF00) | (z & 255).astype(np.uint32)
+        rows.scales[:, last // group] = _gpu(word.view(np.int32), "int32")
+        held = (word & np.uint32(0xFFFFFF00)).view(np.float32).astype(np.float64)  # below 2^-126 fewer bits are left
+        want = (c + z) * held
+        assert np.array_equal(_np(rows.decode()[:, last]), want)
+        lost = np.abs(c + z) * np.where(held >= 2.0 ** -118, 0.0, 2.0 ** -134)
+        for nq in (1, 12, 45):
+            for size in (1.0, 2.0 ** 40):
+                q = torch.zeros(nq, dim, device="cuda")
+                q[:, last] = size
+                got = _np(S.scores(q, rows)) / size
+                assert np.all(np.abs(got - want) <= lost + 2.0 ** (-132 if dim > 4096 else -136) + 2.0 ** -149)
