@@ -19,7 +19,7 @@ LIB = os.path.join(LIBDIR, "libraven_gpu.so")
 
 SOURCES = ["raven_gpu.cu", "scoring.cu", "rows4.cu", "host_index.cpp"]
 DEPS = SOURCES + ["search_kernel.cuh", "search_cta.cuh", "knn_tc.cuh", "score_tc.cuh", "topk.cuh", "fp8.cuh",
-                  "int4.cuh", "score4.cuh", "score4_wide.cuh", "adjust.cuh", "status.cuh", "launch.h", "internal.h", "host_index.h"]
+                  "int4.cuh", "score4.cuh", "score4_wide.cuh", "adjust.cuh", "status.cuh", "waits.h", "launch.h", "internal.h", "host_index.h"]
 
 
 def nvcc_path() -> str:

@@ -22,6 +22,7 @@
 #pragma once
 
 #include "score4.cuh"
+#include "waits.h"
 
 namespace raven_score4 {
 
@@ -166,14 +167,15 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
   after_previous();
 
   // copies: by the team's first thread
-  uint32_t ahead = first, ahead_b = 0, slot = 0, pending = 0;
+  Ring stages;
+  uint32_t ahead = first, ahead_b = 0;
   auto copy_next = [&]() {
     if (ahead < p.tiles) {
-      mbar_expect_tx(bars + 8 * slot, kWideStage);
-      tma_load_2d(smem_u32(ring) + slot * kWideStage, &map, (int)(64 * (b0 + ahead_b)),
-                  (int)min((uint64_t)ahead * kWideRows, p.n), bars + 8 * slot);
-      pending |= 1u << slot;
-      slot = slot + 1 == p.depth ? 0 : slot + 1;
+      const uint32_t bar = bars + 8 * stages.slot;
+      mbar_expect_tx(bar, kWideStage);
+      tma_load_2d(smem_u32(ring) + stages.slot * kWideStage, &map, (int)(64 * (b0 + ahead_b)),
+                  (int)min((uint64_t)ahead * kWideRows, p.n), bar);
+      stages.begun(p.depth);
       if (++ahead_b == blocks) {
         ahead_b = 0;
         ahead += step;
@@ -202,7 +204,7 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
   constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(NC >> 3) << 17) | (8u << 24);  // f32 sums, f16 operands
 
   bool ok = true;
-  uint32_t now = 0, phases = 0, done_phase = 0;
+  Chain chain;
   // the words of the thread's row, one block ahead
   uint32_t next[W];
   auto fetch = [&](uint32_t tile, uint32_t b) {
@@ -229,10 +231,10 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
         fetch(tile, b + 1);
       else if (tile + step < p.tiles)
         fetch(tile + step, 0);
-      if (ok && !warp_waits(bars + 8 * now, phases >> now & 1u)) ok = false;
+      if (ok && !warp_waits(bars + 8 * stages.now, stages.parity())) ok = false;
       if (ok) {
         // 64 bytes of the row, 16 at a time in the 64-byte swizzle
-        const uint8_t* stage = ring + now * kWideStage + row_of * 64;
+        const uint8_t* stage = ring + stages.now * kWideStage + row_of * 64;
         uint32_t c[16];
 #pragma unroll
         for (int i = 0; i < 4; ++i) *(uint4*)&c[4 * i] = *(const uint4*)(stage + ((i ^ ((row_of >> 1) & 3)) * 16));
@@ -261,20 +263,15 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
           put_unit(0, c[0], c[1], c[2], c[3]);
         }
         asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+        stages.taken(p.depth);
       }
-      const uint32_t taken = now;
-      phases ^= 1u << now;
-      now = now + 1 == p.depth ? 0 : now + 1;
 #pragma unroll
       for (uint32_t g = 0; g < W; ++g) {
         if (g * U >= u) break;
         raven_tc::tc_fence_before();
         meet(1 + team, 128);  // operands are written, the sums before them read
         if (row_of == 0 && ok) {
-          if (g == 0) {
-            pending &= ~(1u << taken);
-            copy_next();  // into the stage that every thread has read
-          }
+          if (g == 0) copy_next();  // into the stage that every thread has read
           raven_tc::tc_fence_after();
           uint32_t add = 0;
 #pragma unroll
@@ -288,8 +285,8 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
           }
           raven_tc::mma_commit(done);
         }
-        if (ok && !warp_waits(done, done_phase)) ok = false;
-        done_phase ^= 1u;
+        if (ok && !warp_waits(done, chain.phase)) ok = false;
+        if (ok) chain.over();
         raven_tc::tc_fence_after();
         const float sc = raven_int4::step_of(word[g]) * (1.f / (1 << kStepShift));
         constexpr int P = 2;  // pieces of 16 columns at once
@@ -338,10 +335,8 @@ __global__ void __launch_bounds__(Wide<NC>::kThreads, 1) wide_kernel(const __gri
   if (!ok && lane == 0) raven_score::tell(p.status, raven_score::kStatusWait);
   // a wait ran out: neither a copy nor an instruction of this team is under way any more
   if (!ok && row_of == 0) {
-    for (uint32_t i = 0; i < p.depth; ++i)
-      if (pending >> i & 1u) wait(bars + 8 * i, phases >> i & 1u);
-    raven_tc::mma_commit(done);
-    wait(done, done_phase);
+    stages.rest(p.depth, [&](uint32_t stage, uint32_t parity) { wait(bars + 8 * stage, parity); });
+    chain.rest([&](uint32_t parity) { wait(done, parity); });
   }
   raven_tc::tc_fence_before();
   __syncthreads();
