@@ -355,6 +355,24 @@ cudaError_t dispatch_score4(const raven_rows* v, const raven_score4::Params& p, 
 // ---------------------------------------------------------------------------
 // Adjusted scores.
 // ---------------------------------------------------------------------------
+// Rows of memory, in bytes; wide enough for any pitch.
+struct Rows {
+  using U = unsigned __int128;
+  U at, rows, pitch, width;
+  Rows(const void* p, U n, U apart, U wide) : at((uintptr_t)p), rows(p && wide ? n : 0), pitch(n > 1 ? apart : wide), width(wide) {}
+  U end() const { return at + (rows - 1) * pitch + width; }
+};
+// Whether rows of a and of b share memory; of different pitches, whether they may.
+bool overlap(Rows a, Rows b) {
+  if (a.rows == 0 || b.rows == 0 || a.at >= b.end() || b.at >= a.end()) return false;
+  if (a.rows == 1) a.pitch = b.pitch;
+  if (b.rows == 1) b.pitch = a.pitch;
+  if (a.pitch != b.pitch || a.width > a.pitch || b.width > a.pitch) return true;
+  // how far behind a row of a the next one of b starts: within it, or so far that the one before reaches into it
+  const Rows::U p = a.pitch, d = (b.at + p * (a.at / p + 1) - a.at) % p;
+  return d < a.width || p - d < b.width;
+}
+
 template <typename T>
 cudaError_t launch_adjust(const raven_adjust::Params& p, bool largest, cudaStream_t st) {
   static Allowed none;
@@ -521,6 +539,18 @@ int raven_adjust_scores_device(const void* d_scores, int32_t type, uint64_t nq, 
   }
   if (by->seen_starts && !by->seen && by->seen_total) return fail(RAVEN_EINVAL, "seen: null");
   if (by->seen && !by->seen_starts) return fail(RAVEN_EINVAL, "seen: needs its starts");
+  const Rows out(d_out, nq, ld_out * Rows::U(size), n * size);
+  const Rows others[] = {Rows(by->bias, by->ld_bias ? nq : 1, by->ld_bias * Rows::U(4), n * 4),
+                         Rows(by->allow, by->allow_count, by->ld_allow * Rows::U(4), (n + 31) / 32 * 4),
+                         Rows(by->allow_rows, 1, 0, nq * 4),
+                         Rows(by->seen, 1, 0, by->seen_total * Rows::U(4)),
+                         Rows(by->seen_starts, 1, 0, (nq + 1) * 8),
+                         Rows(by->repetition, 1, 0, nq * 4),
+                         Rows(by->presence, 1, 0, nq * 4),
+                         Rows(by->frequency, 1, 0, nq * 4),
+                         Rows(d_status, 1, 0, 4)};
+  for (const Rows& r : others)
+    if (overlap(out, r)) return fail(RAVEN_EINVAL, "scores: the output overlaps what they are adjusted by");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   raven_adjust::Params p{};

@@ -580,7 +580,8 @@ def adjust(scores: torch.Tensor, *, bias: Optional[torch.Tensor] = None, allow: 
        `allow_rows` (int32 [nq]) is each query's filter, -1 for none. Without it
        there is one filter, or one for each query.
 
-    `out`: a matrix to write, `scores` itself among them. Ids below 0 count for
+    `out`: a matrix to write, `scores` itself among them, but none that shares memory
+    with another argument. Ids below 0 count for
     nothing; nor do ids of n and more, and a query with a filter that is not there
     may see nothing: `status` (or `take_status`) gets RAVEN_S_IDS. Histories whose
     starts fall or leave `seen` count as empty: RAVEN_S_OFFSETS."""

@@ -122,3 +122,19 @@ def test_scores_of_the_smallest_steps(S, dim):
                 q[:, last] = size
                 got = _np(S.scores(q, rows)) / size
                 assert np.all(np.abs(got - want) <= lost + 2.0 ** (-132 if dim > 4096 else -136) + 2.0 ** -149)
+
+
+def test_adjust_output_over_its_arguments(S):
+    from raven_b200._lib import RavenError
+
+    torch = _torch()
+    x, b = torch.randn(4, 100, device="cuda"), torch.randn(4, 100, device="cuda")
+    words = torch.zeros(4, 100, dtype=torch.int32, device="cuda")
+    for call in (lambda: S.adjust(x, bias=b, out=b), lambda: S.adjust(x, bias=b[1], out=b),
+                 lambda: S.adjust(x, allow=words, out=words.view(torch.float32)),
+                 lambda: S.adjust(x, presence=b.view(-1)[8:12], out=b), lambda: S.adjust(x, bias=x[0], out=x)):
+        with pytest.raises(RavenError, match="overlaps"):
+            call()
+    wide = torch.randn(4, 200, device="cuda")
+    want = x + wide[:, 100:]
+    assert S.adjust(x, bias=wide[:, 100:], out=wide[:, :100]).equal(want)  # beside one another: no memory is shared

@@ -1,0 +1,64 @@
+"""What an output of adjusted scores may share memory with, decided before any device work (no GPU needed)."""
+import numpy as np
+import pytest
+
+
+@pytest.fixture(scope="module")
+def adjust(raven_lib):
+    from raven_b200 import _lib as L
+
+    def call(x=1 << 30, type=0, nq=4, n=100, ld=100, out=1 << 20, ld_out=100, status=None, **k):
+        """Whether the call is refused for what overlaps (without a GPU the others fail later, for that)."""
+        by = L.Adjustments(**k)
+        by.repetition_all = 1.0
+        rc = raven_lib.raven_adjust_scores_device(x, type, nq, n, ld, by, 1, out, ld_out, status, None)
+        refused = rc == L.RAVEN_EINVAL and b"overlaps" in raven_lib.raven_last_error()
+        assert refused or rc == L.RAVEN_ECUDA, (rc, raven_lib.raven_last_error())
+        return refused
+
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses: calls that are not refused must not run")
+    return call
+
+
+def test_output_over_what_scores_are_adjusted_by(adjust):
+    out, end = 1 << 20, (1 << 20) + 1600  # 4 x 100 f32
+    bias = dict(ld_bias=100)
+    assert adjust(bias=out, **bias) and adjust(bias=out + 1596, **bias) and adjust(bias=out - 1596, **bias)
+    assert not adjust(bias=end, **bias) and not adjust(bias=out - 1600, **bias)
+    assert adjust(bias=out + 16) and adjust(bias=out - 396) and not adjust(bias=out - 400)  # one row for all
+    assert adjust(bias=out, type=1, **bias)  # bytes, not values
+    assert adjust(allow=out + 4, allow_count=1, ld_allow=4)
+    assert adjust(allow=out - 48 - 12, allow_count=4, ld_allow=4) and not adjust(allow=out - 64, allow_count=4, ld_allow=4)
+    filters = dict(allow=1 << 25, allow_count=4, ld_allow=4)
+    assert adjust(allow_rows=out + 8, **filters) and not adjust(allow_rows=end, **filters)
+    seen = dict(seen=1 << 25, seen_starts=1 << 26, seen_total=50)
+    assert adjust(**dict(seen, seen=out - 196)) and not adjust(**dict(seen, seen=out - 200))
+    assert adjust(**dict(seen, seen_starts=out - 32)) and not adjust(**dict(seen, seen_starts=out - 40))
+    for name in ("repetition", "presence", "frequency"):
+        assert adjust(**{name: out - 12}) and not adjust(**{name: out - 16}) and not adjust(**{name: end})
+    assert adjust(status=out) and not adjust(status=end)
+
+
+def _shares(a, rows_a, b, rows_b, pitch, wide_a, wide_b):
+    """By every byte."""
+    at = lambda p, rows, wide: (p + pitch * np.arange(rows)[:, None] + np.arange(wide)).ravel()  # noqa: E731
+    return np.intersect1d(at(a, rows_a, wide_a), at(b, rows_b, wide_b)).size > 0
+
+
+def test_rows_beside_one_another_by_every_byte(adjust):
+    """Biases of the output's pitch, and single rows, wherever they start."""
+    r = np.random.default_rng(0)
+    out = 1 << 20
+    seen = [0, 0]
+    for _ in range(3000):
+        nq, n = int(r.integers(1, 5)), int(r.integers(1, 7))
+        ld = n if nq == 1 else n + int(r.integers(0, 9))
+        shift = 4 * int(r.integers(-5 * ld - 2, 5 * ld + 2))
+        one = nq > 1 and bool(r.integers(0, 2))
+        want = _shares(out, nq, out + shift, 1 if one else nq, 4 * ld, 4 * n, 4 * n)
+        assert adjust(nq=nq, n=n, ld=ld, ld_out=ld, bias=out + shift, ld_bias=0 if one or nq == 1 else ld) == want
+        seen[want] += 1
+    assert min(seen) > 500
