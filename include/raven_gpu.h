@@ -404,7 +404,9 @@ typedef struct {
 /* Scores (nq x n at pitch ld, f32, f16 or bf16) put right before the best are
  * taken, into d_out (the same type, nq x n at ld_out; it may be d_scores at ld,
  * and must not overlap it otherwise, nor any array of `by`: those are read while
- * scores are written). In f32, each operation rounded:
+ * scores are written; rows of one pitch may lie beside one another, where pitches
+ * differ the memory from first to last must be apart). In f32, each operation
+ * rounded:
  *   s of a vector that the query has seen c > 0 times:
  *     largest: s = (s > 0 ? s / repetition : s * repetition) - (presence + frequency * c)
  *     else:    s = (s > 0 ? s * repetition : s / repetition) + (presence + frequency * c)

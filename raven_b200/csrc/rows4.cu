@@ -522,9 +522,8 @@ int raven_adjust_scores_device(const void* d_scores, int32_t type, uint64_t nq, 
   if (nq == 1) ld = ld_out = n;
   if (ld < n || ld_out < n) return fail(RAVEN_EINVAL, "scores: pitch below the row length");
   if (ld > 1ull << 40 || ld_out > 1ull << 40) return fail(RAVEN_ELIMIT, "scores: pitch above 2^40");
-  const uintptr_t a = (uintptr_t)d_scores, b = (uintptr_t)d_out;
-  const uint64_t wide = ((nq - 1) * ld + n) * size, wide_out = ((nq - 1) * ld_out + n) * size;
-  if (a < b + wide_out && b < a + wide && !(a == b && ld == ld_out))
+  const Rows out(d_out, nq, ld_out * Rows::U(size), n * size);
+  if (!(d_scores == d_out && ld == ld_out) && overlap(out, Rows(d_scores, nq, ld * Rows::U(size), n * size)))
     return fail(RAVEN_EINVAL, "scores: the output overlaps them, but is not the same");
   if (!aligned(by->bias, 4) || !aligned(by->allow, 4) || !aligned(by->allow_rows, 4) || !aligned(by->seen, 4) ||
       !aligned(by->seen_starts, 8) || !aligned(by->repetition, 4) || !aligned(by->presence, 4) ||
@@ -539,7 +538,6 @@ int raven_adjust_scores_device(const void* d_scores, int32_t type, uint64_t nq, 
   }
   if (by->seen_starts && !by->seen && by->seen_total) return fail(RAVEN_EINVAL, "seen: null");
   if (by->seen && !by->seen_starts) return fail(RAVEN_EINVAL, "seen: needs its starts");
-  const Rows out(d_out, nq, ld_out * Rows::U(size), n * size);
   const Rows others[] = {Rows(by->bias, by->ld_bias ? nq : 1, by->ld_bias * Rows::U(4), n * 4),
                          Rows(by->allow, by->allow_count, by->ld_allow * Rows::U(4), (n + 31) / 32 * 4),
                          Rows(by->allow_rows, 1, 0, nq * 4),

@@ -138,3 +138,19 @@ def test_adjust_output_over_its_arguments(S):
     wide = torch.randn(4, 200, device="cuda")
     want = x + wide[:, 100:]
     assert S.adjust(x, bias=wide[:, 100:], out=wide[:, :100]).equal(want)  # beside one another: no memory is shared
+
+
+@pytest.mark.parametrize("t", ["float32", "float16", "bfloat16"])
+def test_adjust_columns_of_one_matrix(S, t):
+    """Scores and output side by side, in either order, starting anywhere."""
+    torch = _torch()
+    for nq, n, first, gap in ((5, 100, 0, 0), (3, 9001, 3, 1), (7, 63, 5, 0)):
+        room = torch.randn(nq, 2 * n + first + gap + 2, device="cuda").to(getattr(torch, t))
+        a, b = slice(first, first + n), slice(first + n + gap, first + 2 * n + gap)
+        bias = torch.randn(n, device="cuda")
+        for src, dst in ((a, b), (b, a)):
+            buf = room.clone()
+            want = room.clone()
+            want[:, dst] = S.adjust(room[:, src].contiguous(), bias=bias)
+            S.adjust(buf[:, src], bias=bias, out=buf[:, dst])
+            assert torch.equal(buf, want)

@@ -62,3 +62,19 @@ def test_rows_beside_one_another_by_every_byte(adjust):
         assert adjust(nq=nq, n=n, ld=ld, ld_out=ld, bias=out + shift, ld_bias=0 if one or nq == 1 else ld) == want
         seen[want] += 1
     assert min(seen) > 500
+
+
+def test_output_beside_its_scores_by_every_byte(adjust):
+    """Columns of one matrix may be scores and output; where pitches differ the whole of both is apart."""
+    r = np.random.default_rng(1)
+    out, seen = 1 << 20, [0, 0]
+    for _ in range(4000):
+        nq, n, size = int(r.integers(1, 5)), int(r.integers(1, 7)), (4, 2)[int(r.integers(0, 2))]
+        ld = n if nq == 1 else n + int(r.integers(0, 9))
+        shift = size * int(r.integers(-5 * ld - 2, 5 * ld + 2))
+        want = shift != 0 and _shares(out, nq, out + shift, nq, size * ld, size * n, size * n)
+        assert adjust(x=out + shift, type=int(size == 2), nq=nq, n=n, ld=ld, ld_out=ld) == want
+        seen[want] += 1
+    assert min(seen) > 500
+    assert adjust(x=out + 400, ld=201, ld_out=200) and not adjust(x=out + 400, ld=200, ld_out=200)
+    assert adjust(ld=1 << 40, nq=(1 << 31) - 1, x=4096, out=1 << 60, ld_out=100)  # sizes past 64 bits
