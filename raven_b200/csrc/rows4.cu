@@ -150,21 +150,36 @@ cudaError_t launch_score4(const CUtensorMap& map, const raven_score4::Params& p,
   return launch(score4_kernel<NT, MT, G, F32, O>, ctas, Layout<NT, MT, G>::kThreads, (uint32_t)smem, allowed, st, map, p);
 }
 
-// Sums of slices take scratch, slices times what the scores take: above this the rows are taken in two halves.
-constexpr uint64_t kMostSums = 1ull << 30;
+// Scratch of a call: queries laid out (as large as they are) and sums of slices (slices times what the scores take).
+// Above this the queries are taken in halves of whole chunks, of which a kernel's CTAs read every code anyway, so that
+// nothing is laid out twice; the sums of a single chunk in halves of the rows.
+constexpr uint64_t kMostScratch = 1ull << 30;
+
+bool too_much(uint64_t scratch, const raven_score4::Params& p, uint32_t chunk) {
+  return scratch > kMostScratch && (p.nq > chunk || p.n >= 512);
+}
 
 template <typename F>
-cudaError_t in_halves(const raven_rows* v, const raven_score4::Params& p, int out_type, F&& run) {
-  const uint64_t half = (p.n / 2 + 127) / 128 * 128;
+cudaError_t in_halves(const raven_rows* v, const raven_score4::Params& p, int out_type, uint32_t chunk, F&& run) {
   raven_rows a = *v, b = *v;
   raven_score4::Params pa = p, pb = p;
-  a.rows = pa.n = half;
-  b.rows = pb.n = p.n - half;
-  b.data = (const uint8_t*)v->data + half * v->ld;
-  b.exps = (const uint8_t*)((const uint32_t*)v->exps + half * v->ld_exps);
-  pb.words = (const uint32_t*)b.exps;
-  pb.out = (uint8_t*)p.out + half * (out_type == 0 ? 4 : 2);
-  if (p.bias) pb.bias = p.bias + half;
+  const uint64_t size = out_type == 0 ? 4 : 2;
+  if (p.nq > chunk) {
+    const uint64_t half = (p.nq / 2 + chunk - 1) / chunk * chunk;
+    pa.nq = half;
+    pb.nq = p.nq - half;
+    pb.q = (const uint8_t*)p.q + half * p.ld_q * (p.q_type == 0 ? 4 : 2);
+    pb.out = (uint8_t*)p.out + half * p.ld * size;
+  } else {
+    const uint64_t half = (p.n / 2 + 127) / 128 * 128;
+    a.rows = pa.n = half;
+    b.rows = pb.n = p.n - half;
+    b.data = (const uint8_t*)v->data + half * v->ld;
+    b.exps = (const uint8_t*)((const uint32_t*)v->exps + half * v->ld_exps);
+    pb.words = (const uint32_t*)b.exps;
+    pb.out = (uint8_t*)p.out + half * size;
+    if (p.bias) pb.bias = p.bias + half;
+  }
   const cudaError_t e = run(&a, pa);
   return e == cudaSuccess ? run(&b, pb) : e;
 }
@@ -218,8 +233,8 @@ cudaError_t run_score4(const raven_rows* v, raven_score4::Params p, int out_type
   const uint64_t laid = lay ? (p.chunks * Q::bytes(p.units, p.groups) + 255) / 256 * 256 : 0;
   const uint64_t wide = (p.n + 3) / 4 * 4, sums = p.slices > 1 ? p.slices * p.nq * wide * 4 : 0;
   const uint64_t backs = p.slices > 1 ? (uint64_t)p.chunks * kQueries * 16 : 0;
-  if (sums > kMostSums && p.n >= 512)
-    return in_halves(v, whole, out_type, [&](const raven_rows* r, const Params& q) {
+  if (too_much(laid + sums + backs, p, kQueries))
+    return in_halves(v, whole, out_type, kQueries, [&](const raven_rows* r, const Params& q) {
       return run_score4<NT, MT, G, F32>(r, q, out_type, sms, st);
     });
   if (laid + sums + backs && (e = cudaMallocAsync((void**)&tmp, laid + sums + backs, st)) != cudaSuccess) return e;
@@ -297,8 +312,8 @@ cudaError_t run_wide(const raven_rows* v, raven_score4::Params p, int out_type, 
   const uint64_t laid = lay ? (p.chunks * Q::bytes(p.units, 0) + 255) / 256 * 256 : 0;
   const uint64_t wide = (p.n + 3) / 4 * 4, sums = p.slices > 1 ? p.slices * p.nq * wide * 4 : 0;
   const uint64_t backs = p.slices > 1 ? (uint64_t)p.chunks * kQueries * 16 : 0;
-  if (sums > kMostSums && p.n >= 512)
-    return in_halves(v, whole, out_type,
+  if (too_much(laid + sums + backs, p, kQueries))
+    return in_halves(v, whole, out_type, kQueries,
                      [&](const raven_rows* r, const Params& q) { return run_wide<NC, G, F32>(r, q, out_type, sms, st); });
   if (laid + sums + backs && (e = cudaMallocAsync((void**)&tmp, laid + sums + backs, st)) != cudaSuccess) return e;
   if (backs) p.backs = (float4*)(tmp + laid + sums);

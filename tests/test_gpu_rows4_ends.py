@@ -1,4 +1,6 @@
 """4-bit rows, scores against them and adjusted scores at the ends: of f32's range, of sizes, of what a call allows."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -154,3 +156,49 @@ def test_adjust_columns_of_one_matrix(S, t):
             want[:, dst] = S.adjust(room[:, src].contiguous(), bias=bias)
             S.adjust(buf[:, src], bias=bias, out=buf[:, dst])
             assert torch.equal(buf, want)
+
+
+class _Scratch:
+    """The most that the device's default pool, which scratch comes from, has given out at once."""
+
+    HIGH = 8  # CU_MEMPOOL_ATTR_USED_MEM_HIGH
+
+    def __init__(self):
+        self.cuda, self.pool = C.CDLL("libcuda.so.1"), C.c_void_p()
+        assert self.cuda.cuDeviceGetDefaultMemPool(C.byref(self.pool), _torch().cuda.current_device()) == 0
+        _torch().cuda.synchronize()
+        assert self.cuda.cuMemPoolSetAttribute(self.pool, self.HIGH, C.byref(C.c_uint64(0))) == 0
+
+    def high(self):
+        _torch().cuda.synchronize()
+        most = C.c_uint64(0)
+        assert self.cuda.cuMemPoolGetAttribute(self.pool, self.HIGH, C.byref(most)) == 0
+        return most.value
+
+
+def _repeated(S, n, dim, g):
+    """(x, rows): n rows of dim values, the 32 of x again and again, whole numbers of -7..8 exactly."""
+    torch = _torch()
+    x = torch.randint(-7, 8, (n, 32), generator=g, device="cuda").float()
+    x[:, 0], x[:, 1] = -7, 8
+    short = S.Int4Rows.encode(x, 32)
+    codes = torch.empty(n, dim // 2, dtype=torch.uint8, device="cuda")
+    # a block holds the words of its four units side by side by quarter
+    codes.view(torch.int32).copy_(short.codes.view(torch.int32).repeat_interleave(4, 1).repeat(1, dim // 128))
+    return x, S.Int4Rows(codes, short.scales[:, :1].repeat(1, dim // 32).contiguous(), dim, 32)
+
+
+@pytest.mark.parametrize("nq,n,dim,t", [(40_003, 300, 16_384, "float16"),     # many long queries, few rows, in slices
+                                        (300_001, 20, 1024, "float32"),       # queries laid out, no slices
+                                        (64, 340_007, 16_384, "float16")])    # one chunk of queries: halves of the rows
+def test_scores_in_little_scratch(S, nq, n, dim, t):
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, rows = _repeated(S, n, dim, g)
+    q = torch.randint(-2, 3, (nq, dim), generator=g, device="cuda", dtype=torch.int8).to(getattr(torch, t))
+    bias = torch.arange(n, device="cuda") % 100 + 0.0
+    want = torch.cat([p.view(len(p), dim // 32, 32).sum(1, dtype=torch.float32) for p in q.split(5000)]) @ x.T + bias
+    scratch = _Scratch()
+    got = S.scores(q, rows, bias=bias)
+    assert scratch.high() <= (1 << 30) + (1 << 20)  # the pool rounds up
+    assert torch.equal(got, want)
