@@ -413,9 +413,9 @@ typedef struct {
  *   s = s + bias
  *   s = -infinity (largest; else infinity) where the query's filter has no bit
  * rounded once to the type. Ids below 0 count for nothing, nor do those of n and
- * more (RAVEN_S_IDS); a history whose starts fall or leave `seen` counts as empty
- * (RAVEN_S_OFFSETS); a query with a filter of allow_count and more may see nothing
- * (RAVEN_S_IDS). */
+ * more (RAVEN_S_IDS); a history whose starts fall or leave `seen`, or of 2^32 ids
+ * and more, counts as empty (RAVEN_S_OFFSETS); a query with a filter of
+ * allow_count and more may see nothing (RAVEN_S_IDS). */
 RAVEN_API int raven_adjust_scores_device(const void* d_scores, int32_t type, uint64_t nq, uint64_t n, uint64_t ld,
                                          const raven_adjustments* by, int32_t largest, void* d_out, uint64_t ld_out,
                                          int32_t* d_status, void* stream);

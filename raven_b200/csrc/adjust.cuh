@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_kernel(const Params p) {
   if (threadIdx.x == 0) found = 0;
   __syncthreads();
   if (p.starts) {
-    if (a < 0 || b < a || (uint64_t)b > p.seen_total) {
+    if (a < 0 || b < a || (uint64_t)b > p.seen_total || (uint64_t)(b - a) >> 32) {  // ids are counted in 32 bits
       if (threadIdx.x == 0) raven_score::tell(p.status, kStatusOffsets);
       a = b = 0;
     }

@@ -584,7 +584,8 @@ def adjust(scores: torch.Tensor, *, bias: Optional[torch.Tensor] = None, allow: 
     with another argument. Ids below 0 count for
     nothing; nor do ids of n and more, and a query with a filter that is not there
     may see nothing: `status` (or `take_status`) gets RAVEN_S_IDS. Histories whose
-    starts fall or leave `seen` count as empty: RAVEN_S_OFFSETS."""
+    starts fall or leave `seen`, and those of 2^32 ids and more, count as empty:
+    RAVEN_S_OFFSETS."""
     ld = _scores_matrix(scores, "scores")
     (nq, n), device = scores.shape, scores.get_device()
     bias_at, ld_bias = None, 0

@@ -202,3 +202,21 @@ def test_scores_in_little_scratch(S, nq, n, dim, t):
     got = S.scores(q, rows, bias=bias)
     assert scratch.high() <= (1 << 30) + (1 << 20)  # the pool rounds up
     assert torch.equal(got, want)
+
+
+def test_adjust_histories_past_32_bits(S):
+    """2^32 ids of one query are more than are counted; many histories may have as many together."""
+    from raven_b200 import _lib as L
+
+    torch = _torch()
+    torch.cuda.empty_cache()
+    many = (1 << 32) + 3
+    seen = torch.full((many + 40,), 5, dtype=torch.int32, device="cuda")
+    seen[many:] = torch.arange(40, dtype=torch.int32, device="cuda") // 2
+    x = torch.zeros(3, 100, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, many, many + 10, many + 40], device="cuda")
+    got = S.adjust(x, seen=seen, seen_starts=starts, presence=1.0, frequency=0.5, status=status)
+    want = torch.zeros(3, 100, device="cuda")
+    want[1, :5], want[2, 5:20] = -2.0, -2.0
+    assert torch.equal(got, want) and int(status) == L.RAVEN_S_OFFSETS
