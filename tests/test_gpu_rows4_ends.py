@@ -220,3 +220,56 @@ def test_adjust_histories_past_32_bits(S):
     want = torch.zeros(3, 100, device="cuda")
     want[1, :5], want[2, 5:20] = -2.0, -2.0
     assert torch.equal(got, want) and int(status) == L.RAVEN_S_OFFSETS
+
+
+@pytest.mark.parametrize("t", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("largest", [True, False])
+def test_adjust_infinities_are_not_the_largest_values(S, t, largest):
+    """Infinities, the type's largest and lowest values and NaN, seen or not, hidden or not, with biases of each kind: each
+    stays what it is, and what passes the largest value (or, in 16 bits, half a step above it) becomes an infinity."""
+    torch = _torch()
+    dt = getattr(torch, t)
+    top, f32 = torch.finfo(dt).max, float(torch.finfo(torch.float32).max)
+    half = top * (1 + torch.finfo(dt).eps / 4)  # in f32: half a step above the largest value, which rounds to infinity
+    vals = [np.inf, -np.inf, np.nan, top, -top, 0.0, -0.0, 1.0, -1.0, top / 2, -top / 2, 1e-45, -1e-45]
+    biases = [0.0, np.inf, -np.inf, np.nan, 1.0, half - top, top - half, top, -top, f32, -f32]
+    x, bias = np.meshgrid(np.float64(vals), np.float64(biases))
+    x, bias = np.tile(x.reshape(-1), 30), np.tile(bias.reshape(-1), 30).astype(np.float32)
+    nq, n = 3, len(x)
+    scores = torch.from_numpy(np.tile(x, (nq, 1))).to(dt).cuda()
+    r = np.random.default_rng(0)
+    starts = np.array([0, 0, n, n + 2 * n])
+    seen = np.concatenate([np.arange(n), r.integers(0, n, 2 * n)]).astype(np.int32)
+    allow = r.integers(-2 ** 31, 2 ** 31, (2, -(-n // 32))).astype(np.int32)
+    rows = np.array([0, -1, 1], np.int32)
+    with np.errstate(all="ignore"):
+        for b in (None, bias):
+            for rep, pre, freq in ((1.5, 0.5, 0.25), (0.5, top, 0.0), (1.0, -top, 0.0)):
+                got = S.adjust(scores, bias=None if b is None else _gpu(b), allow=_gpu(allow, "int32"),
+                               allow_rows=_gpu(rows, "int32"), seen=_gpu(seen, "int32"), seen_starts=_gpu(starts, "int64"),
+                               repetition=rep, presence=pre, frequency=freq, largest=largest).cpu()
+                want = torch.from_numpy(U.adjust(scores.float().cpu().numpy(), largest, b, allow, rows, seen, starts, rep, pre,
+                                                 freq)).to(dt)
+                assert torch.equal(got.isnan(), want.isnan())
+                assert torch.equal(got[~got.isnan()], want[~want.isnan()])
+                assert got.isinf().any() and (got.abs() == top).any()
+
+
+@pytest.mark.parametrize("t", ["float32", "float16", "bfloat16"])
+def test_adjust_hides_with_infinities(S, t):
+    """A hidden score is infinite whatever it was, not the type's lowest value, at any start and end of a row."""
+    torch = _torch()
+    dt = getattr(torch, t)
+    for n, first in ((1, 0), (37, 3), (1000, 1), (9000, 5)):
+        room = torch.full((3, n + 8), torch.finfo(dt).min, dtype=dt, device="cuda")
+        x = room[:, first:first + n]
+        x[1] = torch.finfo(dt).max
+        x[2] = float("nan")
+        bits = torch.randint(-2 ** 31, 2 ** 31, (1, -(-n // 32)), device="cuda").int()
+        keep = (bits[0, torch.arange(n, device="cuda") // 32] >> (torch.arange(n, device="cuda") % 32).int() & 1).bool()
+        for largest in (True, False):
+            got = S.adjust(x, allow=bits, largest=largest)
+            worst = torch.tensor(float("-inf" if largest else "inf"), dtype=dt, device="cuda")
+            want = torch.where(keep, x, worst)
+            assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[:2], want[:2])
+            assert bool((got[2][~keep] == worst).all())
