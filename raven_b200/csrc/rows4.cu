@@ -20,6 +20,24 @@ using namespace raven_launch;
 
 namespace {
 
+// Rows of memory, in bytes; wide enough for any pitch.
+struct Rows {
+  using U = unsigned __int128;
+  U at, rows, pitch, width;
+  Rows(const void* p, U n, U apart, U wide) : at((uintptr_t)p), rows(p && wide ? n : 0), pitch(n > 1 ? apart : wide), width(wide) {}
+  U end() const { return at + (rows - 1) * pitch + width; }
+};
+// Whether rows of a and of b share memory; of different pitches, whether they may.
+bool overlap(Rows a, Rows b) {
+  if (a.rows == 0 || b.rows == 0 || a.at >= b.end() || b.at >= a.end()) return false;
+  if (a.rows == 1) a.pitch = b.pitch;
+  if (b.rows == 1) b.pitch = a.pitch;
+  if (a.pitch != b.pitch || a.width > a.pitch || b.width > a.pitch) return true;
+  // how far behind a row of a the next one of b starts: within it, or so far that the one before reaches into it
+  const Rows::U p = a.pitch, d = (b.at + p * (a.at / p + 1) - a.at) % p;
+  return d < a.width || p - d < b.width;
+}
+
 // ---------------------------------------------------------------------------
 // 4-bit rows.
 // ---------------------------------------------------------------------------
@@ -370,24 +388,6 @@ cudaError_t dispatch_score4(const raven_rows* v, const raven_score4::Params& p, 
 // ---------------------------------------------------------------------------
 // Adjusted scores.
 // ---------------------------------------------------------------------------
-// Rows of memory, in bytes; wide enough for any pitch.
-struct Rows {
-  using U = unsigned __int128;
-  U at, rows, pitch, width;
-  Rows(const void* p, U n, U apart, U wide) : at((uintptr_t)p), rows(p && wide ? n : 0), pitch(n > 1 ? apart : wide), width(wide) {}
-  U end() const { return at + (rows - 1) * pitch + width; }
-};
-// Whether rows of a and of b share memory; of different pitches, whether they may.
-bool overlap(Rows a, Rows b) {
-  if (a.rows == 0 || b.rows == 0 || a.at >= b.end() || b.at >= a.end()) return false;
-  if (a.rows == 1) a.pitch = b.pitch;
-  if (b.rows == 1) b.pitch = a.pitch;
-  if (a.pitch != b.pitch || a.width > a.pitch || b.width > a.pitch) return true;
-  // how far behind a row of a the next one of b starts: within it, or so far that the one before reaches into it
-  const Rows::U p = a.pitch, d = (b.at + p * (a.at / p + 1) - a.at) % p;
-  return d < a.width || p - d < b.width;
-}
-
 template <typename T>
 cudaError_t launch_adjust(const raven_adjust::Params& p, bool largest, cudaStream_t st) {
   static Allowed none;
@@ -430,6 +430,14 @@ int int4_scores(const raven_rows* q, const raven_rows* v, uint32_t dim, float al
   if (!out) return fail(RAVEN_EINVAL, "scores: null output");
   if (!aligned(out, type_size(out_type))) return fail(RAVEN_EINVAL, "scores: output is not aligned to its type");
   if (ld < v->rows) return fail(RAVEN_EINVAL, "scores: output pitch below the number of vectors");
+  const uint64_t wide = raven_int4::kBlock, per = wide / int4_group(v->type), in = type_size(q->type), size = type_size(out_type);
+  const Rows scores(out, q->rows, ld * Rows::U(size), v->rows * size);
+  const Rows others[] = {Rows(q->data, q->rows, q->ld * Rows::U(in), dim * in),
+                         Rows(v->data, v->rows, v->ld, (dim + 31ull) / 32 * 16),
+                         Rows(v->exps, v->rows, v->ld_exps * 4, (dim + wide - 1) / wide * per * 4),
+                         Rows(bias, 1, 0, v->rows * 4)};
+  for (const Rows& r : others)
+    if (overlap(scores, r)) return fail(RAVEN_EINVAL, "scores: the output overlaps queries, vectors or bias");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   cudaStream_t st = (cudaStream_t)stream;

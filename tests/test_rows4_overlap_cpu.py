@@ -1,4 +1,5 @@
-"""What an output of adjusted scores may share memory with, decided before any device work (no GPU needed)."""
+"""What an output of scores, or of adjusted ones, may share memory with, decided before any device work (no GPU
+needed)."""
 import numpy as np
 import pytest
 
@@ -78,3 +79,25 @@ def test_output_beside_its_scores_by_every_byte(adjust):
     assert min(seen) > 500
     assert adjust(x=out + 400, ld=201, ld_out=200) and not adjust(x=out + 400, ld=200, ld_out=200)
     assert adjust(ld=1 << 40, nq=(1 << 31) - 1, x=4096, out=1 << 60, ld_out=100)  # sizes past 64 bits
+
+
+def test_scores_over_what_they_are_made_of(adjust, raven_lib):
+    from raven_b200 import _lib as L
+
+    def refused(out, q=1 << 30, bias=None, codes=1 << 28, words=1 << 29, nq=4, n=8, dim=128, ld_q=128, ld=8, type=0, out_type=0):
+        rc = raven_lib.raven_scores_device(L.Rows(q, None, nq, ld_q, 0, type), L.Rows(codes, words, n, 64, 2, 5), dim, 1.0, bias,
+                                           out, out_type, ld, None, None)
+        no = rc == L.RAVEN_EINVAL and b"overlaps" in raven_lib.raven_last_error()
+        assert no or rc == L.RAVEN_ECUDA, (rc, raven_lib.raven_last_error())
+        return no
+
+    at = 1 << 20
+    assert refused(at, q=at) and refused(at, q=at + 124) and not refused(at, q=at + 128)
+    assert not refused(at, q=at - 2048) and refused(at, q=at - 2044)
+    assert refused(at, q=at, n=128, ld=128) and refused(at, q=at + 128, n=32, ld=128)
+    assert not refused(at + 512, q=at, n=8, ld=136, ld_q=136) and refused(at + 508, q=at, n=8, ld=136, ld_q=136)  # columns
+    assert refused(at, bias=at + 4) and not refused(at, bias=at - 32)
+    assert refused(at, codes=at + 64) and not refused(at, codes=at + 128) and refused(at, codes=at - 448 - 48)
+    assert refused(at, words=at + 120) and not refused(at, words=at + 128) and not refused(at, words=at - 64)
+    assert refused(at + 62, out_type=1, bias=at + 124) and not refused(at + 62, out_type=1, bias=at + 128)
+    assert not refused(at, nq=1, q=at + 32, ld=1 << 40)  # one row, at any pitch
