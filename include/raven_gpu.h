@@ -318,13 +318,15 @@ RAVEN_API int raven_index_fp8_device(raven_index* ix, uint8_t* d_codes, uint64_t
  * to 16 significant bits, z = lo / step and code = x / step - z, both quotients
  * rounded to nearest even, the code at most 15. A group with an infinity or a NaN
  * is NaN as a whole. Codes past dim, up to a multiple of 32 values, and words past
- * the last group, up to a multiple of W, are 0; what is behind them is left. */
+ * the last group, up to a multiple of W, are 0; what is behind them is left. The
+ * rows that are written must not overlap those that are read, nor the slots. */
 RAVEN_API int raven_int4_write_device(const void* d_rows, int32_t type, uint64_t m, uint32_t dim, uint64_t ld,
                                       const int32_t* d_slots, const raven_rows* out, int32_t* d_status, void* stream);
 /* The values that m of the rows stand for, rounded once to out_type (f32, in
  * which they are exact unless they overflow, f16, bf16): those of d_ids, or the
  * first m with NULL d_ids. Rows of an id that is not one of the rows' are 0 (one
- * that is not below them, but not one below 0, sets RAVEN_S_IDS). */
+ * that is not below them, but not one below 0, sets RAVEN_S_IDS). The output must
+ * overlap neither the rows nor the ids. */
 RAVEN_API int raven_int4_read_device(const raven_rows* rows, uint32_t dim, const int32_t* d_ids, uint64_t m, void* d_out,
                                      int32_t out_type, uint64_t ld, int32_t* d_status, void* stream);
 /* 4-bit rows of an index's uploaded vectors (n x dim, in the caller's order of

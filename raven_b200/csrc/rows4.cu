@@ -65,6 +65,12 @@ int check_int4(const raven_rows* r, uint32_t dim, const char* what) {
   return RAVEN_OK;
 }
 
+// The memory of 4-bit rows that are as they should be: their codes, their words.
+Rows codes_of(const raven_rows* r, uint32_t dim) { return Rows(r->data, r->rows, r->ld, (dim + 31ull) / 32 * 16); }
+Rows words_of(const raven_rows* r, uint32_t dim) {
+  return Rows(r->exps, r->rows, r->ld_exps * 4, (dim + kBlock - 1ull) / kBlock * (kBlock / int4_group(r->type)) * 4);
+}
+
 // Rows of a CTA at once: `items` pieces a thread, as long as every SM gets rows. Sets what divides by `per`.
 uint32_t rows_at_once(uint64_t m, uint32_t per, uint32_t items, int sms, uint32_t most, uint32_t* magic) {
   *magic = per > 1 ? (uint32_t)((0x100000000ull + per - 1) / per) : 0;
@@ -430,14 +436,11 @@ int int4_scores(const raven_rows* q, const raven_rows* v, uint32_t dim, float al
   if (!out) return fail(RAVEN_EINVAL, "scores: null output");
   if (!aligned(out, type_size(out_type))) return fail(RAVEN_EINVAL, "scores: output is not aligned to its type");
   if (ld < v->rows) return fail(RAVEN_EINVAL, "scores: output pitch below the number of vectors");
-  const uint64_t wide = raven_int4::kBlock, per = wide / int4_group(v->type), in = type_size(q->type), size = type_size(out_type);
+  const uint64_t in = type_size(q->type), size = type_size(out_type);
   const Rows scores(out, q->rows, ld * Rows::U(size), v->rows * size);
-  const Rows others[] = {Rows(q->data, q->rows, q->ld * Rows::U(in), dim * in),
-                         Rows(v->data, v->rows, v->ld, (dim + 31ull) / 32 * 16),
-                         Rows(v->exps, v->rows, v->ld_exps * 4, (dim + wide - 1) / wide * per * 4),
-                         Rows(bias, 1, 0, v->rows * 4)};
-  for (const Rows& r : others)
-    if (overlap(scores, r)) return fail(RAVEN_EINVAL, "scores: the output overlaps queries, vectors or bias");
+  if (overlap(scores, Rows(q->data, q->rows, q->ld * Rows::U(in), dim * in)) || overlap(scores, codes_of(v, dim)) ||
+      overlap(scores, words_of(v, dim)) || overlap(scores, Rows(bias, 1, 0, v->rows * 4)))
+    return fail(RAVEN_EINVAL, "scores: the output overlaps queries, vectors or bias");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
@@ -492,6 +495,10 @@ int raven_int4_write_device(const void* d_rows, int32_t type, uint64_t m, uint32
   if (ld > kMaxPitch) return fail(RAVEN_ELIMIT, "rows: pitch of 2^32 and more");
   if (!aligned(d_rows, type_size(type))) return fail(RAVEN_EINVAL, "rows: not aligned to their type");
   if (!d_slots && m > out->rows) return fail(RAVEN_EINVAL, "out: fewer rows than are written");
+  const Rows codes = codes_of(out, dim), words = words_of(out, dim), slots(d_slots, 1, 0, m * 4);
+  const Rows in(d_rows, m, ld * type_size(type), dim * type_size(type));
+  if (overlap(codes, in) || overlap(words, in) || overlap(codes, slots) || overlap(words, slots))
+    return fail(RAVEN_EINVAL, "out: overlaps the rows that are written, or their slots");
   return write_rows(d_rows, type, m, dim, ld, false, d_slots, out, d_status, (cudaStream_t)stream);
 }
 
@@ -508,6 +515,9 @@ int raven_int4_read_device(const raven_rows* rows, uint32_t dim, const int32_t* 
   if (ld < dim) return fail(RAVEN_EINVAL, "output: pitch below dim");
   if (ld > kMaxPitch) return fail(RAVEN_ELIMIT, "output: pitch of 2^32 and more");
   if (!d_ids && m > rows->rows) return fail(RAVEN_EINVAL, "rows: fewer than are read");
+  const Rows out(d_out, m, ld * type_size(out_type), dim * type_size(out_type));
+  if (overlap(out, codes_of(rows, dim)) || overlap(out, words_of(rows, dim)) || overlap(out, Rows(d_ids, 1, 0, m * 4)))
+    return fail(RAVEN_EINVAL, "output: overlaps the rows that are read, or their ids");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   raven_int4::Read p{};

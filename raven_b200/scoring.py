@@ -352,7 +352,8 @@ class Int4Rows:
         """The values, [n, dim], or those of the rows `ids` (int32, on the GPU):
         float32 (exact), float16 or bfloat16 (rounded once). Rows of ids below 0
         are 0; so are those of ids of len(self) and more, and `status` (or
-        `take_status`) gets RAVEN_S_IDS. `out`: a matrix to write."""
+        `take_status`) gets RAVEN_S_IDS. `out`: a matrix to write that shares no
+        memory with the rows or `ids`."""
         rows, device = self._rows, self.device_index
         m = rows.rows if ids is None else _ids("ids", ids, device)
         if out is not None:

@@ -101,3 +101,30 @@ def test_scores_over_what_they_are_made_of(adjust, raven_lib):
     assert refused(at, words=at + 120) and not refused(at, words=at + 128) and not refused(at, words=at - 64)
     assert refused(at + 62, out_type=1, bias=at + 124) and not refused(at + 62, out_type=1, bias=at + 128)
     assert not refused(at, nq=1, q=at + 32, ld=1 << 40)  # one row, at any pitch
+
+
+def test_rows_over_what_they_are_made_of(adjust, raven_lib):
+    from raven_b200 import _lib as L
+
+    def said(rc):
+        no = rc == L.RAVEN_EINVAL and b"overlaps" in raven_lib.raven_last_error()
+        assert no or rc == L.RAVEN_ECUDA, (rc, raven_lib.raven_last_error())
+        return no
+
+    at, far = 1 << 20, 1 << 30
+
+    def write(x=far, slots=None, codes=at, words=1 << 25, m=4, dim=128, ld=128, rows=8, pitch=64, type=0):
+        return said(raven_lib.raven_int4_write_device(x, type, m, dim, ld, slots, L.Rows(codes, words, rows, pitch, 2, 5), None,
+                                                      None))
+
+    assert write(x=at) and write(x=at + 508) and not write(x=at + 512) and not write(x=at - 2048) and write(x=at - 2044)
+    assert write(x=at, pitch=512) and not write(x=at + 64, pitch=576, ld=144) and write(x=at + 60, pitch=576, ld=144)
+    assert write(words=far + 8) and write(words=far + 2040) and not write(words=far + 2048) and not write(words=far - 64)
+    assert write(slots=at + 8) and not write(slots=at - 16) and write(slots=(1 << 25) + 60) and not write(slots=(1 << 25) + 64)
+    assert write(x=at - 1020, type=1) and not write(x=at - 1024, type=1)
+
+    def read(out=far, ids=None, codes=at, words=1 << 25, m=4, dim=128, ld=128, rows=8, type=0):
+        return said(raven_lib.raven_int4_read_device(L.Rows(codes, words, rows, 64, 2, 5), dim, ids, m, out, type, ld, None, None))
+
+    assert read(out=at) and read(out=at + 508) and not read(out=at + 512) and not read(out=at - 2048) and read(out=at - 2044)
+    assert read(out=(1 << 25) + 60) and not read(out=(1 << 25) + 64) and read(ids=far + 16) and not read(ids=far + 2048)
