@@ -161,8 +161,9 @@ __device__ inline uint32_t codes_of(float (&x)[8], float step, int z) {
 // L = group / 8 lanes of a group share its range by shuffles, and of two such
 // pieces at once every group's word is worked out by a lane of its own (64-bit
 // arithmetic that 16 lanes did alike took as long as the reading). What bounds it:
-// issue slots and memory about even (1000000 x 128 f32 into slots in random order 200 us,
-// 680 MB at 3.4 TB/s: words and codes fill sectors in part, which are read first).
+// the barrier before a run's slots are known (the largest stall) and issue slots (67 %);
+// memory is at 3.4 TB/s (1000000 x 128 f32 into slots in random order 200 us, 680 MB:
+// words and codes fill sectors in part, which are read first).
 // VEC: pitch and address let 16 bytes be read at once. LANE: lane-major rows
 // (element e of the first 16C at (e % 16) * C + e / 16).
 template <typename T, uint32_t L, bool VEC, bool LANE>
@@ -171,6 +172,7 @@ __global__ void __launch_bounds__(256, 5) write_kernel(const Write p) {
   __shared__ uint32_t later[kRun];
   after_previous();
   // With a table the next run's rows are settled while this one's are worked on: two reads far apart, one after the other.
+  // A CTA has a next run where there are more than 64 an SM (1000000 x 128: 3.3 runs a CTA; 30000 x 768 has none).
   auto settle = [&](uint64_t r0, int32_t* to) {
     if (r0 + threadIdx.x >= p.m || threadIdx.x >= p.run) return;
     int64_t s = (int64_t)p.slots[r0 + threadIdx.x];

@@ -96,7 +96,8 @@ cudaError_t group_write(const raven_int4::Write& p, int sms, cudaStream_t st) {
                          : launch_write<T, 16, LANE>(p, sms, st);
 }
 
-// Up to here every CTA looks for its slots among the later ones.
+// Up to here every CTA looks for its slots among the later ones, without the table's two launches: 1024 rows x 128 f16
+// take 4.5 us (12.0 with a table), 4096 x 768 15.0 (20.4); 4096 x 128 are just past it (18.6, 15.3), 8192 x 768 well (32.2, 26.5).
 constexpr uint64_t kFewSlots = 4096;
 constexpr uint64_t kMaxSlots = 1ull << 30;
 
@@ -153,7 +154,10 @@ cudaError_t launch_read(raven_int4::Read p, int sms, cudaStream_t st) {
 // Scores.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kMostShared = 227 * 1024;
-constexpr uint64_t kOwnLayout = 16384;  // values of queries that each CTA lays out for itself
+// Values of a chunk's queries that each CTA lays out for itself; more are laid out once, by a launch before. On either
+// side of it: 8 x 65536 x 1024 16.7 us (laid out before 17.2), 1 x 100000 x 1024 21.9 (23.2); 4 x 32768 x 4096 33.8 (32.2),
+// 8 x 32768 x 4096 37.1 (32.1), 64 x 65536 x 512 36.4 (27.1).
+constexpr uint64_t kOwnLayout = 16384;
 
 // Codes as boxes of `wide` bytes (64: a block) x `rows` rows; what is past a row's end or the last row reads 0.
 bool codes_map(CUtensorMap* m, const raven_rows* v, uint32_t units, uint32_t wide, uint32_t rows, CUtensorMapSwizzle swizzle) {
@@ -607,7 +611,8 @@ int raven_adjust_scores_device(const void* d_scores, int32_t type, uint64_t nq, 
   p.presence_all = by->presence_all;
   p.frequency_all = by->frequency_all;
   p.status = d_status;
-  // the largest tiles, since each scans its row's history, that leave every SM four
+  // the largest tiles, since each scans its row's history, that leave every SM four; 1024 places at least (1 x 100000 4.4 us,
+  // 4.7 with 256 as with 2048; 4 x 100000 bf16 5.9, 8.3 with 256)
   const uint64_t most = 16 / size - 1;  // columns before a row's first
   p.tile = raven_adjust::kMostPlaces;
   while (p.tile > 1024 && nq * ((n + most + p.tile - 1) / p.tile) < 4ull * sms) p.tile /= 2;

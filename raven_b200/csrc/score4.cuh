@@ -21,9 +21,10 @@
 // ends: the scale is never rounded into an operand. Two parts of an f32 query are two
 // columns of the N side, added up at the end.
 //
-// What bounds it: issue slots, half of them for turning codes into operands (1 x
-// 1000000 x 128 24 us, 3.0 TB/s; 8 x 65536 x 1024 15 us, 2.5 TB/s), so what is around
-// them is kept small. Each warp has its own ring of tiles of 32 or 64
+// What bounds it: no unit by itself. The 16 warps that an SM's registers hold issue in
+// 54 to 59 % of the slots, half of that to turn codes into operands, and wait for one
+// another's results in the others (1 x 1000000 x 128 24 us, 3.0 TB/s; 8 x 65536 x 1024
+// 15 us, 2.5 TB/s), so what is around the operands is kept small. Each warp has its own ring of tiles of 32 or 64
 // rows x 128 values in shared memory: one TMA copy of 2 or 4 KB, and a copy of 4 to
 // 16 bytes a row for the scale words. Where a CTA's tiles are few or large, warps
 // share a tile's rows and take its blocks of 128 values in turn; their sums meet in
