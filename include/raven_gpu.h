@@ -341,10 +341,11 @@ RAVEN_API int raven_index_int4_device(raven_index* ix, const raven_rows* out, vo
  * With 4-bit vectors they are f32, f16 or bf16 rows at any ld >= dim; nothing is
  * rounded before the sums but f32 queries, to 22 bits of each value, and what is
  * below 2^-34 of a query's largest. Of values that f32 holds no sum overflows
- * where its score does not, whatever the sizes of queries and alpha are; steps below 2^-118 lose low
- * bits, and a group's share of a sum what is below 2^-132 of the query's largest
- * value. A query with an infinity or a NaN has scores of NaN. The scores must not
- * overlap what they are made of (rows of one pitch may lie beside one another). */
+ * where its score does not, whatever the sizes of queries and alpha are; steps
+ * below 2^-118 lose low bits, and a group's share of a sum what is below 2^-132
+ * of the query's largest value. A query with an infinity or a NaN has scores of
+ * NaN. The scores must not overlap what they are made of (rows of one pitch may
+ * lie beside one another). */
 RAVEN_API int raven_scores_device(const raven_rows* q, const raven_rows* v, uint32_t dim, float alpha,
                                   const float* d_bias, void* d_out, int32_t out_type, uint64_t ld_out,
                                   int32_t* d_status, void* stream);

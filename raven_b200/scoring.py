@@ -445,10 +445,11 @@ def scores(queries: Rows, vectors: Rows, *, alpha: float = 1.0, bias: Optional[t
            status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """alpha * <query, vector> + bias[vector] for every pair, [nq, n] of `dtype`:
     summed in float32 on the tensor cores, rounded once. Float queries against
-    FP8 rows are encoded first; against 4-bit rows they are taken as they are. alpha = -2 with the vectors' squared norms as
-    bias ranks like squared distances. `out`: a matrix of `dtype` to write (any
-    row pitch) that shares no memory with the other arguments. `status`: an int32 that gets RAVEN_S_* bits; without it
-    `take_status` tells whether the scores are valid."""
+    FP8 rows are encoded first; against 4-bit rows they are taken as they are.
+    alpha = -2 with the vectors' squared norms as bias ranks like squared
+    distances. `out`: a matrix of `dtype` to write (any row pitch) that shares no
+    memory with the other arguments. `status`: an int32 that gets RAVEN_S_* bits;
+    without it `take_status` tells whether the scores are valid."""
     device, dim, nq, n, q, v, keep = _operands(queries, vectors, dtype, bias)
     pitch = n
     if out is None:
