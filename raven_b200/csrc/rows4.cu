@@ -65,10 +65,10 @@ int check_int4(const raven_rows* r, uint32_t dim, const char* what) {
   return RAVEN_OK;
 }
 
-// The memory of 4-bit rows that are as they should be: their codes, their words.
-Rows codes_of(const raven_rows* r, uint32_t dim) { return Rows(r->data, r->rows, r->ld, (dim + 31ull) / 32 * 16); }
-Rows words_of(const raven_rows* r, uint32_t dim) {
-  return Rows(r->exps, r->rows, r->ld_exps * 4, (dim + kBlock - 1ull) / kBlock * (kBlock / int4_group(r->type)) * 4);
+// The memory of the first n of 4-bit rows that are as they should be: their codes, their words.
+Rows codes_of(const raven_rows* r, uint64_t n, uint32_t dim) { return Rows(r->data, n, r->ld, (dim + 31ull) / 32 * 16); }
+Rows words_of(const raven_rows* r, uint64_t n, uint32_t dim) {
+  return Rows(r->exps, n, r->ld_exps * 4, (dim + kBlock - 1ull) / kBlock * (kBlock / int4_group(r->type)) * 4);
 }
 
 // Rows of a CTA at once: `items` pieces a thread, as long as every SM gets rows. Sets what divides by `per`.
@@ -442,8 +442,8 @@ int int4_scores(const raven_rows* q, const raven_rows* v, uint32_t dim, float al
   if (ld < v->rows) return fail(RAVEN_EINVAL, "scores: output pitch below the number of vectors");
   const uint64_t in = type_size(q->type), size = type_size(out_type);
   const Rows scores(out, q->rows, ld * Rows::U(size), v->rows * size);
-  if (overlap(scores, Rows(q->data, q->rows, q->ld * Rows::U(in), dim * in)) || overlap(scores, codes_of(v, dim)) ||
-      overlap(scores, words_of(v, dim)) || overlap(scores, Rows(bias, 1, 0, v->rows * 4)))
+  if (overlap(scores, Rows(q->data, q->rows, q->ld * Rows::U(in), dim * in)) || overlap(scores, codes_of(v, v->rows, dim)) ||
+      overlap(scores, words_of(v, v->rows, dim)) || overlap(scores, Rows(bias, 1, 0, v->rows * 4)))
     return fail(RAVEN_EINVAL, "scores: the output overlaps queries, vectors or bias");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
@@ -499,7 +499,8 @@ int raven_int4_write_device(const void* d_rows, int32_t type, uint64_t m, uint32
   if (ld > kMaxPitch) return fail(RAVEN_ELIMIT, "rows: pitch of 2^32 and more");
   if (!aligned(d_rows, type_size(type))) return fail(RAVEN_EINVAL, "rows: not aligned to their type");
   if (!d_slots && m > out->rows) return fail(RAVEN_EINVAL, "out: fewer rows than are written");
-  const Rows codes = codes_of(out, dim), words = words_of(out, dim), slots(d_slots, 1, 0, m * 4);
+  const uint64_t n = d_slots ? out->rows : m;
+  const Rows codes = codes_of(out, n, dim), words = words_of(out, n, dim), slots(d_slots, 1, 0, m * 4);
   const Rows in(d_rows, m, ld * type_size(type), dim * type_size(type));
   if (overlap(codes, in) || overlap(words, in) || overlap(codes, slots) || overlap(words, slots))
     return fail(RAVEN_EINVAL, "out: overlaps the rows that are written, or their slots");
@@ -520,7 +521,8 @@ int raven_int4_read_device(const raven_rows* rows, uint32_t dim, const int32_t* 
   if (ld > kMaxPitch) return fail(RAVEN_ELIMIT, "output: pitch of 2^32 and more");
   if (!d_ids && m > rows->rows) return fail(RAVEN_EINVAL, "rows: fewer than are read");
   const Rows out(d_out, m, ld * type_size(out_type), dim * type_size(out_type));
-  if (overlap(out, codes_of(rows, dim)) || overlap(out, words_of(rows, dim)) || overlap(out, Rows(d_ids, 1, 0, m * 4)))
+  const uint64_t n = d_ids ? rows->rows : m;
+  if (overlap(out, codes_of(rows, n, dim)) || overlap(out, words_of(rows, n, dim)) || overlap(out, Rows(d_ids, 1, 0, m * 4)))
     return fail(RAVEN_EINVAL, "output: overlaps the rows that are read, or their ids");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;

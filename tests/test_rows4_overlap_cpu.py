@@ -117,7 +117,10 @@ def test_rows_over_what_they_are_made_of(adjust, raven_lib):
         return said(raven_lib.raven_int4_write_device(x, type, m, dim, ld, slots, L.Rows(codes, words, rows, pitch, 2, 5), None,
                                                       None))
 
-    assert write(x=at) and write(x=at + 508) and not write(x=at + 512) and not write(x=at - 2048) and write(x=at - 2044)
+    slots = dict(slots=1 << 28)
+    assert write(x=at) and write(x=at + 252) and not write(x=at + 256)  # the rows that are written: the first 4
+    assert write(x=at + 508, **slots) and not write(x=at + 512, **slots)
+    assert not write(x=at - 2048) and write(x=at - 2044)
     assert write(x=at, pitch=512) and not write(x=at + 64, pitch=576, ld=144) and write(x=at + 60, pitch=576, ld=144)
     assert write(words=far + 8) and write(words=far + 2040) and not write(words=far + 2048) and not write(words=far - 64)
     assert write(slots=at + 8) and not write(slots=at - 16) and write(slots=(1 << 25) + 60) and not write(slots=(1 << 25) + 64)
@@ -126,5 +129,6 @@ def test_rows_over_what_they_are_made_of(adjust, raven_lib):
     def read(out=far, ids=None, codes=at, words=1 << 25, m=4, dim=128, ld=128, rows=8, type=0):
         return said(raven_lib.raven_int4_read_device(L.Rows(codes, words, rows, 64, 2, 5), dim, ids, m, out, type, ld, None, None))
 
-    assert read(out=at) and read(out=at + 508) and not read(out=at + 512) and not read(out=at - 2048) and read(out=at - 2044)
-    assert read(out=(1 << 25) + 60) and not read(out=(1 << 25) + 64) and read(ids=far + 16) and not read(ids=far + 2048)
+    assert read(out=at) and read(out=at + 252) and not read(out=at + 256) and not read(out=at - 2048) and read(out=at - 2044)
+    assert read(out=at + 508, ids=1 << 28) and not read(out=at + 512, ids=1 << 28)
+    assert read(out=(1 << 25) + 60, ids=1 << 28) and not read(out=(1 << 25) + 64, ids=1 << 28) and not read(out=(1 << 25) + 32) and read(ids=far + 16) and not read(ids=far + 2048)
